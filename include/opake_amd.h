@@ -513,6 +513,46 @@ int dpc_per_example_grads_grouped(int n, const void* const* A, const void* const
  * squared norms into per-example totals in a fixed order. */
 int dpc_row_sum_f64(const double* x, int B, int n, int accumulate, double* out, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Losses of a vocabulary head without its logits (no reference counterpart:
+ * the reference's per-example losses take materialised logits).
+ *
+ * hidden [N, D] and weight [V, D] in `dtype` (bf16 or fp32), 16-byte aligned;
+ * z = hidden weight^T / temperature, p = softmax(z) over the vocabulary.
+ *   teacher NULL (cross entropy, K = 1): index [N] is each row's target;
+ *     loss = temperature^2 * -log p[target], 0 for a row whose index is
+ *     ignore_index.
+ *   teacher [N, K] (distillation): the teacher's logits at the columns
+ *     index [N, K]; q = softmax(teacher / temperature) over the row's present
+ *     entries (index >= 0), loss = temperature^2 * sum_k q_k (log q_k - log
+ *     p[index_k]).  An entry may be repeated (its q's add up) or -inf (q = 0);
+ *     a row with no entry above -inf has loss 0.
+ * An index outside the vocabulary that is not ignored makes its row's loss
+ * (and gradients) NaN.  Sums are float32; float32 operands are multiplied
+ * exactly, as three bf16 parts each.
+ *
+ * Rows without a target take no part in any product, whatever they hold.
+ *
+ * dpc_head_loss writes loss and, for the gradient, rows [2 N + 1], lse [N], cols
+ * [N, K] and corr [N, K] (not written where fewer than N rows have a target).
+ * dpc_head_loss_grad takes those four (rows is only read) and grad_loss [N] (the
+ * gradient of the losses; not used where there is no target) and writes, where not NULL, hidden_grad [N, D] and
+ * weight_grad [V, D] in `dtype`, rounded once from float32 sums; dz is
+ * computed again, in pieces of the vocabulary, and held as bf16 (fp32: as
+ * three bf16 parts) for the two products.  All results are deterministic.
+ * -------------------------------------------------------------------------*/
+size_t dpc_head_loss_workspace_bytes(int64_t N, int D, int V, int K, int dtype);
+int dpc_head_loss(const void* hidden, const void* weight, int64_t N, int D, int V, int dtype,
+                  const int64_t* index, const float* teacher, int K, int64_t ignore_index,
+                  double temperature, float* loss, int32_t* rows, float* lse, int32_t* cols,
+                  float* corr, void* ws, size_t ws_bytes, void* stream);
+size_t dpc_head_loss_grad_workspace_bytes(int64_t N, int D, int V, int K, int dtype,
+                                          int want_hidden, int want_weight);
+int dpc_head_loss_grad(const void* hidden, const void* weight, int64_t N, int D, int V, int dtype,
+                       int32_t* rows, const int32_t* cols, const float* corr, int K,
+                       const float* lse, const float* grad_loss, double temperature, void* hidden_grad,
+                       void* weight_grad, void* ws, size_t ws_bytes, void* stream);
+
 /* Measurement helper with no counterpart in the reference (used by bench.py
  * to put the roofline in context): `grid` workgroups of 8 waves run `iters`
  * rounds of 8 independent 32x32x16 bf16 MFMAs on operands taken from

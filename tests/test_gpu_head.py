@@ -1,0 +1,376 @@
+"""Head losses without logits: values and gradients against 64 bits (GPU).
+
+Error model the tolerances come from (u = 2^-23, one extra addend of slack per
+16 products, as for the Gram kernels): a product sum of n terms is off by at
+most 1.125 n u times the sum of the terms' magnitudes.  So a logit is off by
+``zerr = 1.125 n u |h| |w|``; a loss by twice that and a few ulp of the log sum
+exp; dz by its bf16 rounding (float32: three exact parts) and by what the logits'
+error does to p; and a gradient by dz's error and the sum's own, rounded once.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from opake_amd import head
+from opake_amd.exceptions import ConfigurationError, InputTypeError
+
+U = 2.0**-23
+
+
+def _inputs(dev, lead, D, V, dtype, seed, spread=2.0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    h = torch.randn(*lead, D, generator=g, device=dev).to(dtype)
+    W = (torch.randn(V, D, generator=g, device=dev) * (spread / math.sqrt(D))).to(dtype)
+    up = torch.rand(*lead, generator=g, device=dev) + 0.5
+    return g, h, W, up
+
+
+def _reference(h, W, q, ent, tau, up):
+    """Losses and gradients in 64 bits from the dense target distribution q [N, V]
+    (rows of zeros: no target) and its negative entropy, with error bounds."""
+    D = h.shape[-1]
+    hd, Wd, u = h.detach().double().reshape(-1, D), W.detach().double(), up.double().reshape(-1, 1)
+    f32 = h.dtype == torch.float32
+    used = q.sum(1, keepdim=True)
+    z = hd @ Wd.t() / tau
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    logp = z - lse
+    loss = tau * tau * (ent - (q * logp).sum(1))
+    n = (6 if f32 else 1) * (D + 64)
+    zerr = 1.125 * n * U * hd.norm(dim=1, keepdim=True) * Wd.norm(dim=1).max() / tau
+    sharp = 2 * zerr + 2.0**-19 * (1 + logp.abs().amin(1, keepdim=True) + lse.abs())
+    loss_tol = tau * tau * (2 * sharp.squeeze(1) + 2.0**-20 * (1 + loss.abs() + ent.abs()))
+    p = logp.exp() * used
+    dz = (p - q) * (tau * u)
+    rnd = 2.0**-22 if f32 else 2.0**-8
+    # p's relative error: the logits' and the exponential's (its argument's rounding).
+    perr = (p * (sharp + 2.0**-22 * logp.abs()) + 2.0**-21 * q) * (tau * u)
+    dzerr = dz.abs() * rnd + perr
+    out = 2.0**-23 if f32 else 2.0**-8
+
+    def product(x, xerr, y, terms):
+        val = x @ y
+        terms *= 6 if f32 else 1
+        tol = (xerr + 1.125 * (terms + 64) * U * x.abs()) @ y.abs() + out * val.abs()
+        return val, tol + 1e-30
+
+    N, V = q.shape
+    dh = product(dz, dzerr, Wd, V)
+    dW = product(dz.t().contiguous(), dzerr.t().contiguous(), hd, N)
+    return (loss, loss_tol), dh, dW
+
+
+def _close(got, want, what):
+    val, tol = want
+    err = (got.detach().double().reshape(val.shape) - val).abs()
+    worst = (err / tol).max().item() if err.numel() else 0.0
+    assert torch.isfinite(got).all(), what
+    assert worst <= 1.0, f"{what}: {worst:.3f} of its tolerance"
+
+
+def _onehot(t, V, ignore):
+    t = t.reshape(-1)
+    q = torch.zeros(t.numel(), V, dtype=torch.float64, device=t.device)
+    r = torch.nonzero(t != ignore).flatten()
+    q[r, t[r].long()] = 1.0
+    return q
+
+
+SHAPES = [
+    # lead, D, V: one of everything, odd ones, tile edges and past them, long K
+    ((1,), 1, 1), ((1,), 8, 2), ((3,), 7, 5), ((2, 5), 64, 256), ((255,), 65, 257),
+    ((256,), 128, 512), ((257,), 72, 511), ((1, 1), 264, 1000), ((4, 100), 200, 3001),
+    ((700,), 24, 777), ((33,), 1000, 5003),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lead,D,V", SHAPES)
+def test_cross_entropy(dev, lead, D, V, dtype):
+    g, h, W, up = _inputs(dev, lead, D, V, dtype, seed=D + V)
+    t = torch.randint(0, V, lead, generator=g, device=dev)
+    if t.numel() > 2:
+        t.view(-1)[::5] = -100
+    h.requires_grad_(True)
+    W.requires_grad_(True)
+    loss = head.linear_cross_entropy(h, W, t)
+    assert loss.shape == lead and loss.dtype == torch.float32
+    dh, dW = torch.autograd.grad(loss, [h, W], up)
+    assert dh.shape == h.shape and dh.dtype == dtype and dW.dtype == dtype
+    q = _onehot(t, V, -100)
+    L, DH, DW = _reference(h, W, q, torch.zeros(q.shape[0], dtype=torch.float64, device=dev), 1.0,
+                           up)
+    _close(loss, L, "loss")
+    _close(dh, DH, "hidden_grad")
+    _close(dW, DW, "weight_grad")
+    ignored = (t == -100)
+    assert (loss[ignored] == 0).all() and (dh[ignored] == 0).all()
+
+
+def _teacher(g, dev, lead, V, K, duplicates=False):
+    if duplicates:
+        idx = torch.randint(0, max(1, V // 3), (*lead, K), generator=g, device=dev)
+    else:
+        idx = torch.rand(*lead, V, generator=g, device=dev).topk(K, -1).indices
+    return torch.randn(*lead, K, generator=g, device=dev) * 2 + 3, idx
+
+
+def _soft(tl, ti, V, tau):
+    """Dense q and its negative entropy per entry (repeated entries add up in q)."""
+    K = ti.shape[-1]
+    tl, ti = tl.double().reshape(-1, K) / tau, ti.reshape(-1, K)
+    there = (ti >= 0) & (tl > -math.inf)
+    some = there.any(1, keepdim=True)
+    e = torch.softmax(torch.where(there, tl, -math.inf), 1)
+    e = torch.where(some, e, 0.0)
+    ent = torch.special.xlogy(e, e).sum(1)
+    q = torch.zeros(ti.shape[0], V, dtype=torch.float64, device=tl.device)
+    q.scatter_add_(1, ti.clamp(min=0), e)
+    return q, ent
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lead,D,V,K,tau,dup", [
+    ((1,), 8, 1, 1, 1.0, False), ((5,), 16, 9, 9, 0.5, False), ((2, 130), 64, 300, 8, 2.0, False),
+    ((129,), 40, 513, 64, 1.5, False), ((70,), 100, 700, 65, 4.0, False),
+    ((31,), 64, 1025, 200, 1.0, True), ((300,), 33, 257, 6, 2.0, True),
+])
+def test_distillation(dev, lead, D, V, K, tau, dup, dtype):
+    g, h, W, up = _inputs(dev, lead, D, V, dtype, seed=K + V)
+    tl, ti = _teacher(g, dev, lead, V, K, dup)
+    flat_i, flat_l = ti.view(-1, K), tl.view(-1, K)
+    n = flat_i.shape[0]
+    if n > 4:  # rows cut short, rows with none, entries the teacher rules out
+        keep = torch.randint(0, K + 1, (n, 1), generator=g, device=dev)
+        flat_i[torch.arange(K, device=dev) >= keep] = -1
+        flat_i[0] = -1
+        flat_l[1, :] = -math.inf
+        flat_l[2, 0] = -math.inf
+    h.requires_grad_(True)
+    W.requires_grad_(True)
+    loss = head.topk_distillation(h, W, tl, ti, temperature=tau)
+    dh, dW = torch.autograd.grad(loss, [h, W], up)
+    q, ent = _soft(tl, ti, V, tau)
+    L, DH, DW = _reference(h, W, q, ent, tau, up)
+    _close(loss, L, "loss")
+    _close(dh, DH, "hidden_grad")
+    _close(dW, DW, "weight_grad")
+    empty = q.sum(1).view(lead) == 0
+    assert (loss[empty] == 0).all() and (dh[empty] == 0).all()
+
+
+@pytest.mark.gpu
+def test_distillation_from_one_entry_is_cross_entropy(dev):
+    g, h, W, _ = _inputs(dev, (90,), 64, 700, torch.bfloat16, 5)
+    t = torch.randint(0, 700, (90,), generator=g, device=dev)
+    a = head.linear_cross_entropy(h, W, t)
+    b = head.topk_distillation(h, W, torch.full((90, 1), 7.0, device=dev), t[:, None])
+    assert (a - b).abs().max() <= 2.0**-20 * (1 + a.abs().max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_many_pieces(dev, dtype):
+    """Enough tokens that the backward takes the vocabulary in several pieces."""
+    N, D, V = 300_001, 8, 600
+    g, h, W, up = _inputs(dev, (N,), D, V, dtype, 11)
+    t = torch.randint(0, V, (N,), generator=g, device=dev)
+    h.requires_grad_(True)
+    W.requires_grad_(True)
+    loss = head.linear_cross_entropy(h, W, t)
+    dh, dW = torch.autograd.grad(loss, [h, W], up)
+    L, DH, DW = _reference(h, W, _onehot(t, V, -100), torch.zeros(N, dtype=torch.float64,
+                                                                   device=dev), 1.0, up)
+    _close(loss, L, "loss")
+    _close(dh, DH, "hidden_grad")
+    _close(dW, DW, "weight_grad")
+
+
+@pytest.mark.gpu
+def test_strided_and_unaligned_operands(dev):
+    """Views: a transposed batch, a slice of a wider tensor, an odd element offset."""
+    g, h, W, up = _inputs(dev, (6, 40), 64, 300, torch.bfloat16, 3)
+    t = torch.randint(0, 300, (6, 40), generator=g, device=dev)
+    want = head.linear_cross_entropy(h, W, t)
+    hv = h.transpose(0, 1).contiguous().transpose(0, 1)
+    Wv = torch.cat([W, W], 1)[:, :64]
+    buf = torch.empty(h.numel() + 1, dtype=h.dtype, device=dev)
+    ho = buf[1:].view(h.shape)
+    ho.copy_(h)
+    tv = t.to(torch.int32).t().contiguous().t()
+    assert torch.equal(head.linear_cross_entropy(hv, Wv, tv), want)
+    assert torch.equal(head.linear_cross_entropy(ho, W, t), want)
+    grads = []
+    for x, y in ((h, W), (hv, Wv), (ho, W)):
+        x, y = x.detach().requires_grad_(True), y.detach().requires_grad_(True)
+        # A broadcast upstream gradient (stride 0).
+        grads.append(torch.autograd.grad(head.linear_cross_entropy(x, y, t).sum(), [x, y]))
+    for got in grads[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got, grads[0]))
+
+
+@pytest.mark.gpu
+def test_only_what_is_asked_for(dev):
+    g, h, W, up = _inputs(dev, (50,), 64, 300, torch.bfloat16, 9)
+    t = torch.randint(0, 300, (50,), generator=g, device=dev)
+    h1, W1 = h.clone().requires_grad_(True), W.clone().requires_grad_(True)
+    both = torch.autograd.grad(head.linear_cross_entropy(h1, W1, t), [h1, W1], up)
+    (dh,) = torch.autograd.grad(head.linear_cross_entropy(h1, W, t), [h1], up)
+    (dW,) = torch.autograd.grad(head.linear_cross_entropy(h, W1, t), [W1], up)
+    assert torch.equal(dh, both[0]) and torch.equal(dW, both[1])
+    assert not head.linear_cross_entropy(h, W, t).requires_grad
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_large_logits_and_nonfinite_rows(dev, dtype):
+    """Logits of hundreds (one column takes all the mass); a NaN or infinite hidden row
+    spoils its own loss and hidden gradient only; so does a target outside the vocabulary."""
+    g, h, W, up = _inputs(dev, (40,), 64, 600, dtype, 21, spread=60.0)
+    t = torch.randint(0, 600, (40,), generator=g, device=dev)
+    h.requires_grad_(True)
+    loss = head.linear_cross_entropy(h, W, t)
+    (dh,) = torch.autograd.grad(loss, [h], up)
+    q = _onehot(t, 600, -100)
+    L, DH, _ = _reference(h, W, q, torch.zeros(40, dtype=torch.float64, device=dev), 1.0, up)
+    _close(loss, L, "loss")
+    _close(dh, DH, "hidden_grad")
+    h2, t2 = h.detach().clone(), t.clone()
+    h2[3, 5], h2[7, 0] = math.nan, math.inf
+    t2[11], t2[12] = 600, -7
+    h2.requires_grad_(True)
+    loss2 = head.linear_cross_entropy(h2, W, t2)
+    (dh2,) = torch.autograd.grad(loss2, [h2], up)
+    bad = torch.zeros(40, dtype=torch.bool, device=dev)
+    bad[[3, 7, 11, 12]] = True
+    assert (~torch.isfinite(loss2[bad])).all() and torch.isnan(dh2[bad]).any(1).all()
+    assert torch.equal(loss2[~bad], loss[~bad]) and torch.equal(dh2[~bad], dh[~bad])
+
+
+@pytest.mark.gpu
+def test_nan_in_rows_without_a_target_reaches_nothing(dev):
+    """Padding rows may hold anything: ignored, they change no loss and no gradient."""
+    g, h, W, up = _inputs(dev, (300,), 64, 600, torch.bfloat16, 2)
+    t = torch.randint(0, 600, (300,), generator=g, device=dev)
+    t[10:90] = -100
+    h1, W1 = h.clone().requires_grad_(True), W.clone().requires_grad_(True)
+    l1 = head.linear_cross_entropy(h1, W1, t)
+    g1 = torch.autograd.grad(l1, [h1, W1], up)
+    h2 = h.clone()
+    h2[10:50], h2[50:90] = math.nan, math.inf
+    h2.requires_grad_(True)
+    up2 = up.clone()
+    up2[10:90] = math.nan
+    l2 = head.linear_cross_entropy(h2, W1, t)
+    g2 = torch.autograd.grad(l2, [h2, W1], up2)
+    assert torch.equal(l1, l2) and torch.equal(g1[0], g2[0]) and torch.equal(g1[1], g2[1])
+
+
+@pytest.mark.gpu
+def test_no_tokens(dev):
+    h = torch.zeros(0, 16, device=dev, requires_grad=True)
+    W = torch.randn(30, 16, device=dev, requires_grad=True)
+    loss = head.linear_cross_entropy(h, W, torch.zeros(0, dtype=torch.int64, device=dev))
+    dh, dW = torch.autograd.grad(loss.sum(), [h, W])
+    assert loss.shape == (0,) and dh.shape == (0, 16) and (dW == 0).all()
+
+
+@pytest.mark.gpu
+def test_differences(dev):
+    """<gradient, d> against central differences of the kernel's own losses along d.
+    The third derivative of a log sum exp along d is a third central moment of w.d,
+    at most range^3 / (6 sqrt 3)."""
+    N, D, V, eps = 40, 48, 350, 2.0**-5
+    g, h, W, up = _inputs(dev, (N,), D, V, torch.float32, 31)
+    tl, ti = _teacher(g, dev, (N,), V, 12)
+    h.requires_grad_(True)
+    loss = head.topk_distillation(h, W, tl, ti, temperature=1.0)
+    (dh,) = torch.autograd.grad(loss, [h], up)
+    d = torch.randn(N, D, generator=g, device=dev)
+    with torch.no_grad():
+        hi = head.topk_distillation(h + eps * d, W, tl, ti, temperature=1.0).double()
+        lo = head.topk_distillation(h - eps * d, W, tl, ti, temperature=1.0).double()
+    slope = (hi - lo) / (2 * eps)
+    want = (dh.double() * d.double()).sum(1) / up.double()
+    s = d.double() @ W.double().t()
+    span = s.amax(1) - s.amin(1)
+    q, ent = _soft(tl, ti, V, 1.0)
+    (_, ltol), (_, gtol), _ = _reference(h, W, q, ent, 1.0, up)
+    # The step itself rounds each coordinate of h by half an ulp.
+    step = (h.detach().abs().double() + eps * d.abs().double()) * 2.0**-24
+    tol = (2 * ltol / (2 * eps) + eps**2 / 6 * span**3 / (6 * 3**0.5)
+           + (gtol * d.double().abs()).sum(1) / up.double()
+           + (step * (2 * W.double().abs().amax(0))).sum(1) / eps)
+    assert ((slope - want).abs() <= tol).all(), ((slope - want).abs() / tol).max().item()
+
+
+@pytest.mark.gpu
+def test_repeats_streams_and_graph(dev):
+    """The same bits call after call, on another stream and from a replayed graph."""
+    g, h, W, up = _inputs(dev, (3, 130), 64, 700, torch.bfloat16, 17)
+    t = torch.randint(0, 700, (3, 130), generator=g, device=dev)
+    h.requires_grad_(True)
+    W.requires_grad_(True)
+
+    def step():
+        loss = head.linear_cross_entropy(h, W, t)
+        return (loss.detach(), *torch.autograd.grad(loss, [h, W], up))
+
+    want = step()
+    assert all(torch.equal(a, b) for a, b in zip(step(), want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(other, want))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(3):
+        for x in out:
+            x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        torch.randn(1000, device=dev).sum().item()
+
+
+@pytest.mark.gpu
+def test_refusals(dev):
+    h, W = torch.zeros(4, 16, device=dev), torch.zeros(9, 16, device=dev)
+    t = torch.zeros(4, dtype=torch.int64, device=dev)
+    tl, ti = torch.zeros(4, 3, device=dev), torch.zeros(4, 3, dtype=torch.int64, device=dev)
+    bad = [
+        (ConfigurationError, lambda: head.linear_cross_entropy(h, W[:, :8], t)),
+        (ConfigurationError, lambda: head.linear_cross_entropy(h, W.bfloat16(), t)),
+        (ConfigurationError, lambda: head.linear_cross_entropy(h.half(), W.half(), t)),
+        (ConfigurationError, lambda: head.linear_cross_entropy(h, W, t[:3])),
+        (ConfigurationError, lambda: head.linear_cross_entropy(h, W[:0], t)),
+        (InputTypeError, lambda: head.linear_cross_entropy(h, W, t.float())),
+        (ConfigurationError, lambda: head.topk_distillation(h, W, tl, ti[:, :2])),
+        (ConfigurationError, lambda: head.topk_distillation(h, W, tl[:, :0], ti[:, :0])),
+        (InputTypeError, lambda: head.topk_distillation(h, W, tl.long(), ti)),
+        (InputTypeError, lambda: head.topk_distillation(h, W, tl, tl)),
+        (ConfigurationError, lambda: head.topk_distillation(h, W, tl, ti, temperature=0.0)),
+        (ConfigurationError, lambda: head.topk_distillation(h, W, tl, ti, temperature=math.nan)),
+        (InputTypeError, lambda: head.topk_distillation(h, W, tl, ti, temperature="2")),
+    ]
+    for kind, call in bad:
+        with pytest.raises(kind):
+            call()
+
+
+def test_cpu_tensors_are_refused():
+    h, W = torch.zeros(4, 16), torch.zeros(9, 16)
+    with pytest.raises(ConfigurationError, match="ROCm device"):
+        head.linear_cross_entropy(h, W, torch.zeros(4, dtype=torch.int64))
+    with pytest.raises(ConfigurationError, match="ROCm device"):
+        head.topk_distillation(h, W, torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int64))
