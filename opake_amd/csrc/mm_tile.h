@@ -94,48 +94,89 @@ struct MmStage {
       }
     }
   }
-  // Step at k0 of plane `pl` of the tile from index i0, into LDS address `lds`.
-  // Rows past the operand's and k past kl are out of the buffer's range (zeros).
-  DPC_DEVICE void issue(const MmOperand& o, int pl, int i0, int k0, int kl, uint32_t lds,
-                        int w) const {
+  // The step at k0 of plane `pl` of the tile from index i0: the buffer it reads, and
+  // `bad`, out of the buffer's range for lanes whose k is past kl.  Rows past the
+  // operand's are out of range too: all such reads give zeros.
+  DPC_DEVICE u32x4_t buffer(const MmOperand& o, int pl, int i0, int k0, int kl, int* bad) const {
     const uint16_t* base = o.p + (int64_t)pl * o.plane;
     uint32_t bytes;
-    int bad = 0;
+    *bad = 0;
     if (kKc) {
       base += (int64_t)i0 * o.ld + k0;
       bytes = (uint32_t)((min(o.rows - i0, kMmTile) * o.ld - k0) * 2);
-      bad = k0 + kchunk >= kl ? kMmOutOfRange : 0;
+      *bad = k0 + kchunk >= kl ? kMmOutOfRange : 0;
     } else {
       base += (int64_t)k0 * o.ld + i0;
       bytes = (uint32_t)((min(kl - k0, kMmStep) * o.ld - i0) * 2);
     }
-    const u32x4_t rs = rsrc_words(base, bytes);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) dma16(rs, lds + (w + 8 * j) * 1024, voff[j] | bad, 0);
+    return rsrc_words(base, bytes);
+  }
+  DPC_DEVICE void issue(u32x4_t buf, int bad, uint32_t lds, int w, int j) const {
+    dma16(buf, lds + (w + 8 * j) * 1024, voff[j] | bad, 0);
   }
 };
 
-// Fragment of 16 indices from c0, 32-deep sub-step kk.  kMixed: the other
-// operand is K-slow, whose transposing reads fix the order of the k-slots
-// (frag16_off: slot 8 q + 4 h + e is k = 16 h + 4 q + e).
-template <bool kKc, bool kMixed>
-DPC_DEVICE bf16x8_t mm_frag(const uint8_t* tile, int c0, int kk, int lane) {
-  if (!kKc) {
-    const int o = frag16_off(c0, 0, lane) + kk * 32 * kTileRowBytes;
-    return join_frag(read_tr(tile, o), read_tr(tile, o + 16 * kTileRowBytes));
+// Reads the 16 x 32 fragments of a wave's blocks from an operand's tile.  kMixed:
+// the other operand is K-slow, whose transposing reads fix the order of the
+// k-slots (frag16_off: slot 8 q + 4 h + e is k = 16 h + 4 q + e).  A lane keeps a
+// few byte offsets; blocks, sub-steps and stages are added as immediates.
+template <bool kKc, bool kMixed, int kBlocks>
+struct MmFrags {
+  static constexpr int kOffsets = kKc ? (kMixed ? 4 : 2) : kBlocks / 2;
+  int o[kOffsets];
+  // Tile at byte `at` of the workgroup's LDS, first block at index c0.
+  DPC_DEVICE void init(int at, int c0, int lane) {
+    const int row = c0 + (lane & 15), q = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < kOffsets; ++i) {
+      if (!kKc)
+        o[i] = at + frag16_off(c0 + 32 * i, 0, lane);
+      else if (kMixed)  // i: 2 kk + h
+        o[i] = at + mm_kc_off(row, 2 * i + (q >> 1)) + 8 * (q & 1);
+      else
+        o[i] = at + mm_kc_off(row, 4 * i + q);
+    }
   }
-  const int row = c0 + (lane & 15), q = lane >> 4;
-  if (!kMixed)
-    return *reinterpret_cast<const bf16x8_t*>(tile + mm_kc_off(row, 4 * kk + q));
-  const i16x4_t lo = *reinterpret_cast<const i16x4_t*>(
-      tile + mm_kc_off(row, 4 * kk + (q >> 1)) + 8 * (q & 1));
-  const i16x4_t hi = *reinterpret_cast<const i16x4_t*>(
-      tile + mm_kc_off(row, 4 * kk + 2 + (q >> 1)) + 8 * (q & 1));
-  return join_frag(lo, hi);
-}
+  // Block i, sub-step kk, `off` bytes on (the stage).
+  DPC_DEVICE bf16x8_t read(const uint8_t* lds, int i, int kk, int off) const {
+    if (!kKc) {  // odd blocks are the other half of a 64-byte LDS block
+      const int p = (o[i >> 1] ^ (32 * (i & 1))) + off + kk * 32 * kTileRowBytes;
+      return join_frag(read_tr(lds, p), read_tr(lds, p + 16 * kTileRowBytes));
+    }
+    if (!kMixed) return *reinterpret_cast<const bf16x8_t*>(lds + o[kk] + off + i * 2048);
+    const i16x4_t lo = *reinterpret_cast<const i16x4_t*>(lds + o[2 * kk] + off + i * 2048);
+    const i16x4_t hi = *reinterpret_cast<const i16x4_t*>(lds + o[2 * kk + 1] + off + i * 2048);
+    return join_frag(lo, hi);
+  }
+};
 
-// The K loop of one tile: steps [s0, s1) into acc.  One LDS stage (64 KiB of
-// `lds`).  Ends with a barrier, after which `lds` is free.
+// A place in the K loop: plane pair and first k.  `next` stays at the last step
+// past the end, so a pipeline may go on fetching (in range) into a stage that
+// nothing reads.
+struct MmPlace {
+  int left, pair, k0;
+  DPC_DEVICE void next(int kl) {
+    if (left <= 1) return;
+    --left;
+    k0 += kMmStep;
+    if (k0 >= kl) {
+      k0 = 0;
+      ++pair;
+    }
+  }
+};
+
+// The K loop of one tile: steps of slice `split` into acc.  Two LDS stages of each
+// operand (A, A, B, B: every read is a lane's offset plus a 16-bit immediate), all
+// transfers straight from memory into LDS.
+//
+// A step is two 32-deep sub-steps of two phases of 16 MFMAs: the wave's upper and
+// lower four A blocks against its four B blocks.  Fragments are read one phase
+// ahead.  Before phase 3 a barrier: the other stage has arrived, and this one has
+// been read for the last time.  A's transfers of step s + 2 go out right after it,
+// B's of step s + 1 at the start of step s, so each has most of a step or more to
+// land and the barrier is the only place where a wave waits.
+// Ends with a barrier, after which `lds` is free.
 template <bool kAKc, bool kBKc>
 DPC_DEVICE void mm_loop(const MmArgs& g, int ta, int tb, int split, uint8_t* lds, MmAcc& acc) {
   const int tid = threadIdx.x, lane = tid & 63,
@@ -148,39 +189,105 @@ DPC_DEVICE void mm_loop(const MmArgs& g, int ta, int tb, int split, uint8_t* lds
   const int ks = max(1, (g.kl + kMmStep - 1) / kMmStep);
   const long long n = mm_steps(g);
   const int s0 = (int)(n * split / g.splits), s1 = (int)(n * (split + 1) / g.splits);
-  int pair = s0 / ks, k0 = (s0 - pair * ks) * kMmStep;
-  pair = __builtin_amdgcn_readfirstlane(g.planes == 1 ? 5 : pair);
-  k0 = __builtin_amdgcn_readfirstlane(k0);
-  uint8_t* la = lds;
-  uint8_t* lb = lds + kMmOperandBytes;
+  const int steps = __builtin_amdgcn_readfirstlane(s1 - s0);
+  if (steps <= 0) return;
+  const int pair0 = __builtin_amdgcn_readfirstlane(s0 / ks);
+  MmPlace pa = {steps, g.planes == 1 ? 5 : pair0, (s0 - pair0 * ks) * kMmStep}, pb = pa;
   MmStage<kAKc> sa;
   MmStage<kBKc> sb;
   sa.init(g.a, w, lane);
   sb.init(g.b, w, lane);
   constexpr bool kMixed = kAKc != kBKc;
-  for (int s = s0; s < s1; ++s) {
-    sa.issue(g.a, (kMmPairsA >> (4 * pair)) & 15, ta * kMmTile, k0, g.kl, lds_addr(la), w);
-    sb.issue(g.b, (kMmPairsB >> (4 * pair)) & 15, tb * kMmTile, k0, g.kl, lds_addr(lb), w);
-    k0 += kMmStep;
-    if (k0 >= g.kl) {
-      k0 = 0;
-      ++pair;
+  u32x4_t buf;
+  int bad;
+  auto next_a = [&]() __attribute__((always_inline)) {
+    buf = sa.buffer(g.a, (kMmPairsA >> (4 * pa.pair)) & 15, ta * kMmTile, pa.k0, g.kl, &bad);
+    pa.next(g.kl);
+  };
+  auto next_b = [&]() __attribute__((always_inline)) {
+    buf = sb.buffer(g.b, (kMmPairsB >> (4 * pb.pair)) & 15, tb * kMmTile, pb.k0, g.kl, &bad);
+    pb.next(g.kl);
+  };
+  auto fetch_a = [&](int stage, int j) __attribute__((always_inline)) {
+    sa.issue(buf, bad, lds_addr(lds) + stage * kMmOperandBytes, w, j);
+  };
+  auto fetch_b = [&](int stage, int j) __attribute__((always_inline)) {
+    sb.issue(buf, bad, lds_addr(lds) + (2 + stage) * kMmOperandBytes, w, j);
+  };
+  bf16x8_t fa0[4], fa1[4], fb0[4], fb1[4];
+  MmFrags<kAKc, kMixed, 8> ra;
+  MmFrags<kBKc, kMixed, 4> rb;
+  ra.init(0, wm * 128, lane);
+  rb.init(2 * kMmOperandBytes, wn * 64, lane);
+  // One phase: 16 MFMAs in the order of `a`, `b`, and after MFMA m what slot(m) issues
+  // (a fragment of the next phase, a transfer); the order is the one written.
+  auto phase = [&](const bf16x8_t* a, const bf16x8_t* b, int ih, auto slot)
+      __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < 16; ++m) {
+      const int i = m >> 2, j = m & 3;
+      acc.v[4 * ih + i][j] =
+          __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc.v[4 * ih + i][j], 0, 0, 0);
+      slot(m);
+      __builtin_amdgcn_sched_barrier(0);
     }
+  };
+  auto read_a = [&](int stage, int kk, int ih, bf16x8_t* f, int i) __attribute__((always_inline)) {
+    f[i] = ra.read(lds, 4 * ih + i, kk, stage * kMmOperandBytes);
+  };
+  auto read_b = [&](int stage, int kk, bf16x8_t* f, int j) __attribute__((always_inline)) {
+    f[j] = rb.read(lds, j, kk, stage * kMmOperandBytes);
+  };
+  auto step = [&](int cur, int nxt) __attribute__((always_inline)) {
+    next_b();
+    __builtin_amdgcn_sched_barrier(0);
+    phase(fa0, fb0, 0, [&](int m) __attribute__((always_inline)) {
+      if (m % 2 == 0 && m < 8) read_a(cur, 0, 1, fa1, m / 2);
+      if (m % 4 == 3) fetch_b(nxt, m / 4);
+    });
+    phase(fa1, fb0, 1, [&](int m) __attribute__((always_inline)) {
+      if (m < 8) {
+        if (m & 1) read_a(cur, 1, 0, fa0, m / 2);
+        else read_b(cur, 1, fb1, m / 2);
+      }
+    });
+    phase(fa0, fb1, 0, [&](int m) __attribute__((always_inline)) {
+      if (m % 2 == 0 && m < 8) read_a(cur, 1, 1, fa1, m / 2);
+    });
+    next_a();
     DPC_WAIT_VMCNT(0);
     __syncthreads();
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      bf16x8_t fb[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) fb[j] = mm_frag<kBKc, kMixed>(lb, wn * 64 + j * 16, kk, lane);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bf16x8_t fa = mm_frag<kAKc, kMixed>(la, wm * 128 + i * 16, kk, lane);
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc.v[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa, fb[j], acc.v[i][j], 0, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    phase(fa1, fb1, 1, [&](int m) __attribute__((always_inline)) {
+      if (m < 8) {
+        if (m & 1) read_a(nxt, 0, 0, fa0, m / 2);
+        else read_b(nxt, 0, fb0, m / 2);
       }
-    }
-    __syncthreads();
+      if (m % 4 == 3) fetch_a(cur, m / 4);
+    });
+  };
+  next_a();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) fetch_a(0, j);
+  next_b();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) fetch_b(0, j);
+  next_a();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) fetch_a(1, j);
+  DPC_WAIT_VMCNT(4);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    read_b(0, 0, fb0, j);
+    read_a(0, 0, 0, fa0, j);
   }
+  int s = 0;
+  for (; s + 1 < steps; s += 2) {
+    step(0, 1);
+    step(1, 0);
+  }
+  if (s < steps) step(0, 1);
+  DPC_WAIT_VMCNT(0);
+  __syncthreads();
 }
