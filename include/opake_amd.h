@@ -38,6 +38,7 @@ extern "C" {
  * take DPC_F16 and DPC_F64. */
 enum dpc_dtype { DPC_F32 = 0, DPC_BF16 = 1, DPC_F16 = 2, DPC_F64 = 3 };
 enum dpc_scale_kind { DPC_SCALE_FIXED = 0, DPC_SCALE_AUTO_S = 1 };
+enum dpc_route_score { DPC_ROUTE_SOFTMAX = 0, DPC_ROUTE_SIGMOID = 1 };
 enum dpc_noise_mode { DPC_NOISE_NONE = 0, DPC_NOISE_INJECTED = 1, DPC_NOISE_PHILOX = 2 };
 
 /* Library ABI version (major * 100 + minor). */
@@ -552,6 +553,32 @@ int dpc_head_loss_grad(const void* hidden, const void* weight, int64_t N, int D,
                        int32_t* rows, const int32_t* cols, const float* corr, int K,
                        const float* lse, const float* grad_loss, double temperature, void* hidden_grad,
                        void* weight_grad, void* ws, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Routing of tokens to experts (the reference's MoE layers take router logits
+ * through torch's softmax and topk, packages/opake-patches/src/opake/api/patches/
+ * kernels/moe.py:570-627; this adds the scores, bias and groups of other routers).
+ *
+ * logits [N, E] (fp32, bf16 or fp16), E <= 1024; `score` is an enum
+ * dpc_route_score; bias [E] or NULL is added to the scores for the choice only.
+ * The experts form `groups` equal groups of consecutive ones, of which the
+ * top_groups with the largest key take part; of theirs, the k (<= 64) largest
+ * keys are chosen, in descending order, ties to the lower index.  The keys are
+ * the float32 scores plus bias, or without a bias the logits (the same order).
+ * weights [N, k]: the scores, divided by their sum over the chosen if
+ * `renormalize` (0 if that is 0), times scale.  A logit or key of -inf or NaN is
+ * never chosen; slots with nothing left get expert -1 and weight 0; a NaN logit
+ * makes its row's weights NaN.  scores [N, k] is written for the gradient.
+ *
+ * dpc_route_topk_grad writes grad_logits [N, E] from grad_weights [N, k] in the
+ * logits' dtype; the choice itself has no gradient. */
+int dpc_route_topk(const void* logits, int64_t N, int E, int dtype, const float* bias, int k,
+                   int score, int groups, int top_groups, int renormalize, double scale,
+                   float* weights, int64_t* experts, float* scores, void* stream);
+int dpc_route_topk_grad(const void* logits, int64_t N, int E, int dtype, int k, int score,
+                        int renormalize, double scale, const int64_t* experts,
+                        const float* weights, const float* scores, const float* grad_weights,
+                        void* grad_logits, void* stream);
 
 /* Measurement helper with no counterpart in the reference (used by bench.py
  * to put the roofline in context): `grid` workgroups of 8 waves run `iters`

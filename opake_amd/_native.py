@@ -31,6 +31,8 @@ DPC_F16 = 2
 DPC_F64 = 3
 SCALE_FIXED = 0
 SCALE_AUTO_S = 1
+ROUTE_SOFTMAX = 0
+ROUTE_SIGMOID = 1
 NOISE_NONE = 0
 NOISE_INJECTED = 1
 NOISE_PHILOX = 2
@@ -185,6 +187,16 @@ SIGNATURES = {
         _c_int,
         [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_void_p,
          _c_void_p, _c_void_p],
+    ),
+    "dpc_route_topk": (
+        _c_int,
+        [_c_void_p, _c_i64, _c_int, _c_int, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_int,
+         _c_double, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
+    ),
+    "dpc_route_topk_grad": (
+        _c_int,
+        [_c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_double, _c_void_p,
+         _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
     ),
     "dpc_head_loss_workspace_bytes": (_c_size_t, [_c_i64, _c_int, _c_int, _c_int, _c_int]),
     "dpc_head_loss": (

@@ -1,0 +1,320 @@
+// Routing of tokens to experts: scores of router logits z [N, E], the k experts
+// with the largest keys, their weights, and the gradient of z.
+//
+//   s_e = softmax(z)_e or 1 / (1 + exp(-z_e));  key_e = s_e + bias_e, or z_e without a
+//   bias (the same order, no rounding)
+//   groups: E / groups consecutive experts each; only the top_groups groups whose
+//   largest keys are largest take part
+//   w_j = scale s_j, or scale s_j / sum over the chosen s
+//
+// Ties go to the lower index.  An expert whose logit or key is -inf or NaN is never
+// chosen; a slot for which none is left gets expert -1 and weight 0.  A NaN logit
+// makes its row's weights NaN.
+//
+// A row lives in kLanes lanes of a wave (64 / kLanes rows a wave), kVals experts a
+// lane, as order-preserving 32-bit keys; a round finds the largest key and then the
+// lowest index that has it, by lane moves within the row's lanes.  Rounds: one a
+// group kept, one an expert chosen.
+#include <math.h>
+
+#include "common.h"
+
+namespace {
+
+struct RouteArgs {
+  const void* logits;
+  int64_t N;
+  int E, dtype;
+  const float* bias;  // [E] or null
+  int k, sigmoid, groups, top_groups, renormalize;
+  float scale;
+  float* weights;   // [N, k]
+  int64_t* experts;  // [N, k]
+  float* scores;    // [N, k]
+};
+
+DPC_DEVICE float load_logit(const void* p, int64_t i, int dtype) {
+  return (float)load_as_f64(p, i, dtype);
+}
+
+// Unsigned order of the float order; 0 for -inf and NaN.  -0 counts as +0.
+DPC_DEVICE uint32_t order_key(float x) {
+  if (!(x > -INFINITY)) return 0;
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+template <int kCtrl>
+DPC_DEVICE uint32_t lane_move(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, kCtrl, 0xf, 0xf, false);
+}
+
+// op over the row's lanes, in every one of them.
+template <int kLanes, typename Op>
+DPC_DEVICE uint32_t row_all(uint32_t x, Op op) {
+  if (kLanes >= 2) x = op(x, lane_move<0xB1>(x));   // quad_perm [1, 0, 3, 2]
+  if (kLanes >= 4) x = op(x, lane_move<0x4E>(x));   // quad_perm [2, 3, 0, 1]
+  if (kLanes >= 8) x = op(x, lane_move<0x141>(x));  // row_half_mirror
+  if (kLanes >= 16) x = op(x, lane_move<0x140>(x));  // row_mirror
+  if (kLanes >= 64) {
+    const uint32_t a = __builtin_amdgcn_readlane(x, 0), b = __builtin_amdgcn_readlane(x, 16),
+                   c = __builtin_amdgcn_readlane(x, 32), d = __builtin_amdgcn_readlane(x, 48);
+    x = op(op(a, b), op(c, d));
+  }
+  return x;
+}
+
+struct MaxU {
+  DPC_DEVICE uint32_t operator()(uint32_t a, uint32_t b) const { return a > b ? a : b; }
+};
+struct MinU {
+  DPC_DEVICE uint32_t operator()(uint32_t a, uint32_t b) const { return a < b ? a : b; }
+};
+struct OrU {
+  DPC_DEVICE uint32_t operator()(uint32_t a, uint32_t b) const { return a | b; }
+};
+struct MaxF {
+  DPC_DEVICE uint32_t operator()(uint32_t a, uint32_t b) const {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
+};
+struct AddF {
+  DPC_DEVICE uint32_t operator()(uint32_t a, uint32_t b) const {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }
+};
+template <int kLanes>
+DPC_DEVICE float row_max(float x) {
+  return __uint_as_float(row_all<kLanes>(__float_as_uint(x), MaxF()));
+}
+template <int kLanes>
+DPC_DEVICE float row_sum(float x) {
+  return __uint_as_float(row_all<kLanes>(__float_as_uint(x), AddF()));
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+DPC_DEVICE float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+DPC_DEVICE float sigmoid(float z) { return 1.0f / (1.0f + fast_exp(-z)); }
+
+// The largest key among key[] and its lowest index (none: 0).
+template <int kLanes, int kVals>
+DPC_DEVICE uint32_t row_first(const uint32_t (&key)[kVals], int lane, int* index) {
+  uint32_t m = key[0];
+#pragma unroll
+  for (int v = 1; v < kVals; ++v) m = MaxU()(m, key[v]);
+  m = row_all<kLanes>(m, MaxU());
+  uint32_t at = 0xffffffffu;
+#pragma unroll
+  for (int v = kVals - 1; v >= 0; --v)
+    if (key[v] == m) at = lane + v * kLanes;
+  *index = (int)row_all<kLanes>(at, MinU());
+  return m;
+}
+
+template <int kLanes, int kVals>
+__global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
+  constexpr int kRows = 64 / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const int64_t row =
+      ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)) * kRows + (threadIdx.x & 63) / kLanes;
+  const bool in = row < a.N;
+  const int64_t base = in ? row * a.E : 0;
+  float z[kVals];
+  uint32_t key[kVals];
+  bool nan = false;
+#pragma unroll
+  for (int v = 0; v < kVals; ++v) {
+    const int e = lane + v * kLanes;
+    z[v] = in && e < a.E ? load_logit(a.logits, base + e, a.dtype) : -INFINITY;
+    nan |= isnan(z[v]);
+  }
+  nan = row_all<kLanes>(nan ? 1u : 0u, OrU()) != 0;
+  float top = -INFINITY, inv = 0.0f;
+  if (!a.sigmoid && (a.bias || !a.renormalize)) {
+#pragma unroll
+    for (int v = 0; v < kVals; ++v) top = fmaxf(top, z[v]);
+    top = row_max<kLanes>(top);
+    const float b = top > -INFINITY ? top : 0.0f;
+    float sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kVals; ++v) sum += fast_exp(z[v] - b);
+    sum = row_sum<kLanes>(sum);
+    inv = 1.0f / sum;
+    top = b;
+  }
+#pragma unroll
+  for (int v = 0; v < kVals; ++v) {
+    const int e = lane + v * kLanes;
+    float x = z[v];
+    if (a.bias && x > -INFINITY) {
+      const float s = a.sigmoid ? sigmoid(x) : fast_exp(x - top) * inv;
+      x = s + (e < a.E ? a.bias[e] : 0.0f);
+    }
+    key[v] = order_key(x);
+  }
+  if (a.top_groups < a.groups) {
+    // Each round keeps the group of the largest key outside the kept groups.
+    const int size = a.E / a.groups;
+    const uint32_t magic = (1u << 20) / size + 1;  // e / size for e, size <= 1024
+    uint32_t open[kVals];
+    uint32_t kept = 0;  // bit v: key[v]'s group is kept
+#pragma unroll
+    for (int v = 0; v < kVals; ++v) open[v] = key[v];
+    for (int r = 0; r < a.top_groups; ++r) {
+      int at;
+      const uint32_t m = row_first<kLanes, kVals>(open, lane, &at);
+      const int g = m ? (int)(((uint32_t)at * magic) >> 20) : -1;
+#pragma unroll
+      for (int v = 0; v < kVals; ++v)
+        if ((int)(((uint32_t)(lane + v * kLanes) * magic) >> 20) == g) {
+          open[v] = 0;
+          kept |= 1u << v;
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < kVals; ++v)
+      if (!((kept >> v) & 1)) key[v] = 0;
+  }
+  int mine = -1;  // lane j: slot j's expert
+  for (int j = 0; j < a.k; ++j) {
+    int at;
+    const uint32_t m = row_first<kLanes, kVals>(key, lane, &at);
+    if (lane == j && m) mine = at;
+#pragma unroll
+    for (int v = 0; v < kVals; ++v)
+      if (lane + v * kLanes == at) key[v] = 0;
+  }
+  float s = 0.0f, w = 0.0f;
+  const float zj = mine >= 0 ? load_logit(a.logits, base + mine, a.dtype) : -INFINITY;
+  if (!a.sigmoid && a.renormalize) {
+    // Softmax over the chosen: the same quotients, nothing to underflow.
+    const float m = row_max<kLanes>(zj);
+    s = mine >= 0 ? fast_exp(zj - m) : 0.0f;
+  } else if (mine >= 0) {
+    s = a.sigmoid ? sigmoid(zj) : fast_exp(zj - top) * inv;
+  }
+  w = s;
+  if (a.renormalize) {
+    const float sum = row_sum<kLanes>(s);
+    w = sum != 0.0f ? s / sum : 0.0f;
+  }
+  w = nan ? NAN : w * a.scale;
+  if (in && lane < a.k) {
+    a.weights[row * a.k + lane] = mine >= 0 ? w : (nan ? NAN : 0.0f);
+    a.experts[row * a.k + lane] = mine;
+    a.scores[row * a.k + lane] = s;
+  }
+}
+
+struct RouteGradArgs {
+  const void* logits;  // read for the softmax's own weights only
+  int64_t N;
+  int E, dtype, k, sigmoid, renormalize;
+  float scale;
+  const int64_t* experts;
+  const float* weights;
+  const float* scores;
+  const float* g;  // [N, k]: gradient of the weights
+  void* dz;
+};
+
+// One wave a row.  The chosen experts' gradients meet the row's other values in
+// LDS.
+__global__ void __launch_bounds__(256) route_grad_kernel(RouteGradArgs a) {
+  __shared__ float rows[4][1024];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t row = (int64_t)blockIdx.x * 4 + w;
+  const bool in = row < a.N;
+  float* mine = rows[w];
+  for (int e = lane; e < a.E; e += 64) mine[e] = 0.0f;
+  __syncthreads();
+  const bool on = in && lane < a.k && a.experts[row * a.k + lane] >= 0;
+  const int64_t at = row * a.k + lane;
+  const int e = on ? (int)a.experts[at] : 0;
+  const float g = on ? a.g[at] * a.scale : 0.0f, s = on ? a.scores[at] : 0.0f;
+  const float share = on && a.scale != 0.0f ? a.weights[at] / a.scale : 0.0f;
+  float x = g;
+  const float dot = row_sum<64>(g * (a.renormalize ? share : s));
+  if (a.renormalize) {
+    x = g - dot;
+    if (a.sigmoid) {
+      const float sum = row_sum<64>(s);
+      x = sum != 0.0f ? x / sum : 0.0f;
+    } else {
+      x *= share;
+    }
+  }
+  if (a.sigmoid) x *= s * (1.0f - s);
+  if (on) mine[e] = x;
+  __syncthreads();
+  if (!in) return;
+  float top = -INFINITY, inv = 0.0f;
+  const bool dense = !a.sigmoid && !a.renormalize;
+  if (dense) {
+    for (int i = lane; i < a.E; i += 64) top = fmaxf(top, load_logit(a.logits, row * a.E + i, a.dtype));
+    top = row_max<64>(top);
+    top = top > -INFINITY ? top : 0.0f;
+    float sum = 0.0f;
+    for (int i = lane; i < a.E; i += 64)
+      sum += fast_exp(load_logit(a.logits, row * a.E + i, a.dtype) - top);
+    sum = row_sum<64>(sum);
+    inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+  }
+  for (int i = lane; i < a.E; i += 64) {
+    float y = mine[i];
+    if (dense) y = fast_exp(load_logit(a.logits, row * a.E + i, a.dtype) - top) * inv * (y - dot);
+    store_from_f64(a.dz, row * a.E + i, (double)y, a.dtype);
+  }
+}
+
+bool valid_route(int64_t N, int E, int k, int dtype, int score) {
+  return N >= 0 && N <= 0x7fffff00ll && E >= 1 && E <= 1024 && k >= 1 && k <= E && k <= 64 &&
+         (dtype == DPC_F32 || dtype == DPC_BF16 || dtype == DPC_F16) &&
+         (score == DPC_ROUTE_SOFTMAX || score == DPC_ROUTE_SIGMOID);
+}
+
+template <int kLanes, int kVals>
+int launch_route(const RouteArgs& a, hipStream_t s) {
+  constexpr int kRows = 4 * (64 / kLanes);
+  hipLaunchKernelGGL((route_kernel<kLanes, kVals>), dim3((unsigned)((a.N + kRows - 1) / kRows)),
+                     dim3(256), 0, s, a);
+  DPC_HIP_CHECK(hipGetLastError());
+  return DPC_OK;
+}
+
+}  // namespace
+
+extern "C" int dpc_route_topk(const void* logits, int64_t N, int E, int dtype, const float* bias,
+                              int k, int score, int groups, int top_groups, int renormalize,
+                              double scale, float* weights, int64_t* experts, float* scores,
+                              void* stream) {
+  if (!valid_route(N, E, k, dtype, score) || groups < 1 || E % groups || top_groups < 1 ||
+      top_groups > groups || k > top_groups * (E / groups))
+    return DPC_EINVAL;
+  if (N == 0) return DPC_OK;
+  if (!logits || !weights || !experts || !scores) return DPC_EINVAL;
+  const RouteArgs a = {logits, N, E, dtype, bias, k, score == DPC_ROUTE_SIGMOID, groups, top_groups,
+                       renormalize != 0, (float)scale, weights, experts, scores};
+  hipStream_t s = (hipStream_t)stream;
+  if (k <= 4 && E <= 8) return launch_route<4, 2>(a, s);
+  if (k <= 16 && E <= 64) return launch_route<16, 4>(a, s);
+  if (k <= 16 && E <= 256 && N >= 4096) return launch_route<16, 16>(a, s);
+  if (E <= 256) return launch_route<64, 4>(a, s);
+  return launch_route<64, 16>(a, s);
+}
+
+extern "C" int dpc_route_topk_grad(const void* logits, int64_t N, int E, int dtype, int k, int score,
+                                   int renormalize, double scale, const int64_t* experts,
+                                   const float* weights, const float* scores,
+                                   const float* grad_weights, void* grad_logits, void* stream) {
+  if (!valid_route(N, E, k, dtype, score)) return DPC_EINVAL;
+  if (N == 0) return DPC_OK;
+  if (!logits || !experts || !weights || !scores || !grad_weights || !grad_logits)
+    return DPC_EINVAL;
+  const RouteGradArgs a = {logits, N, E, dtype, k, score == DPC_ROUTE_SIGMOID, renormalize != 0,
+                           (float)scale, experts, weights, scores, grad_weights, grad_logits};
+  hipLaunchKernelGGL(route_grad_kernel, dim3((unsigned)((N + 3) / 4)), dim3(256), 0,
+                     (hipStream_t)stream, a);
+  DPC_HIP_CHECK(hipGetLastError());
+  return DPC_OK;
+}

@@ -1,0 +1,115 @@
+"""Routing of tokens to experts.
+
+``route_topk`` turns router logits into each token's ``k`` experts and their
+weights in one launch, and its backward is one launch too (``csrc/route.hip``).
+The reference routes by softmax and top-k (packages/opake-patches/src/opake/api/
+patches/kernels/moe.py:570-627); the sigmoid scores, the balancing bias and the
+groups are those of routers trained without a balancing loss.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from opake_amd import _native as nat
+from opake_amd.exceptions import ConfigurationError, InputTypeError
+
+MAX_EXPERTS = 1024
+MAX_TOP_K = 64
+_SCORES = {"softmax": nat.ROUTE_SOFTMAX, "sigmoid": nat.ROUTE_SIGMOID}
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, k, score, groups, top_groups, renormalize, scale):
+        dev = nat.require_device(logits, bias)
+        code = nat.dtype_code(logits.dtype, wide=True)
+        lead, E = logits.shape[:-1], logits.shape[-1]
+        z = logits.detach().contiguous()
+        N = z.numel() // E
+        weights = torch.empty((*lead, k), dtype=torch.float32, device=dev)
+        experts = torch.empty((*lead, k), dtype=torch.int64, device=dev)
+        scores = torch.empty((N, k), dtype=torch.float32, device=dev)
+        with torch.cuda.device(dev):
+            nat.call("dpc_route_topk", nat.ptr(z), N, E, code, nat.ptr(bias), k, score, groups,
+                     top_groups, int(renormalize), scale, nat.ptr(weights), nat.ptr(experts),
+                     nat.ptr(scores), nat.stream_handle(dev))
+        ctx.save_for_backward(logits, weights, experts, scores)
+        ctx.mark_non_differentiable(experts)
+        ctx.set_materialize_grads(False)
+        ctx.options = (k, score, int(renormalize), scale)
+        return weights, experts
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _):
+        if grad is None:
+            return (None,) * 8
+        logits, weights, experts, scores = ctx.saved_tensors
+        k, score, renormalize, scale = ctx.options
+        dev, E = logits.device, logits.shape[-1]
+        z = logits.detach().contiguous()
+        g = grad.to(torch.float32).contiguous()
+        dz = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
+        with torch.cuda.device(dev):
+            nat.call("dpc_route_topk_grad", nat.ptr(z), z.numel() // E, E,
+                     nat.dtype_code(logits.dtype, wide=True), k, score, renormalize, scale,
+                     nat.ptr(experts), nat.ptr(weights), nat.ptr(scores), nat.ptr(g), nat.ptr(dz),
+                     nat.stream_handle(dev))
+        return dz, None, None, None, None, None, None, None
+
+
+def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax",
+               bias: torch.Tensor | None = None, groups: int = 1, top_groups: int | None = None,
+               renormalize: bool = True, scale: float = 1.0):
+    """Experts and weights of every token: ``(weights float32 [..., k], experts int64 [..., k])``.
+
+    ``logits`` [..., E] (float32, bfloat16 or float16, E <= 1024).  ``score``:
+    ``"softmax"`` over the experts or ``"sigmoid"`` of each.  ``bias`` [E] (float32)
+    is added to the scores for the choice only, as a balancing rule adjusts it; it
+    has no gradient.  ``groups``: the experts form that many equal groups of
+    consecutive ones, and only the ``top_groups`` whose best expert is best take part
+    (all by default).  The ``k`` best come in descending order, ties to the lower
+    index.  Their weights are the scores, divided by their sum if ``renormalize``,
+    times ``scale``; gradients reach ``logits`` through them.
+
+    An expert whose logit is -inf (masked) is never chosen: a token with fewer than
+    ``k`` left gets expert -1 with weight 0 in its last places.  A NaN logit makes
+    its token's weights NaN."""
+    nat.require_device(logits, bias)
+    for name, v in (("k", k), ("groups", groups), ("top_groups", top_groups)):
+        if v is not None and (isinstance(v, bool) or not isinstance(v, int)):
+            raise InputTypeError(f"{name} must be an int, got {type(v)}")
+    if isinstance(scale, bool) or not isinstance(scale, (int, float)):
+        raise InputTypeError(f"scale must be a number, got {type(scale)}")
+    if score not in _SCORES:
+        raise ConfigurationError(f"score must be one of {sorted(_SCORES)}, got {score!r}")
+    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ConfigurationError(
+            f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+    if logits.dim() < 1 or not 1 <= logits.shape[-1] <= MAX_EXPERTS:
+        raise ConfigurationError(
+            f"expected logits [..., E] with 1 <= E <= {MAX_EXPERTS}, got {tuple(logits.shape)}")
+    E = logits.shape[-1]
+    top_groups = groups if top_groups is None else top_groups
+    if groups < 1 or E % groups or not 1 <= top_groups <= groups:
+        raise ConfigurationError(
+            f"{E} experts need groups that divide them and 1 <= top_groups <= groups, got "
+            f"{groups} and {top_groups}")
+    if not 1 <= k <= min(MAX_TOP_K, top_groups * (E // groups)):
+        raise ConfigurationError(
+            f"k must be between 1 and {min(MAX_TOP_K, top_groups * (E // groups))}, got {k}")
+    if not math.isfinite(scale):
+        raise ConfigurationError(f"scale must be finite, got {scale}")
+    if bias is not None:
+        if bias.dtype != torch.float32 or tuple(bias.shape) != (E,):
+            raise ConfigurationError(f"bias must be float32 [{E}], got {bias.dtype} "
+                                     f"{tuple(bias.shape)}")
+        bias = bias.detach().contiguous()
+    return _Route.apply(logits, bias, k, _SCORES[score], groups, top_groups, bool(renormalize),
+                        float(scale))
+
+
+__all__ = ["MAX_EXPERTS", "MAX_TOP_K", "route_topk"]
