@@ -534,25 +534,31 @@ int dpc_row_sum_f64(const double* x, int B, int n, int accumulate, double* out, 
  *
  * Rows without a target take no part in any product, whatever they hold.
  *
- * dpc_head_loss writes loss and, for the gradient, rows [2 N + 1], lse [N], cols
- * [N, K] and corr [N, K] (not written where fewer than N rows have a target).
- * dpc_head_loss_grad takes those four (rows is only read) and grad_loss [N] (the
- * gradient of the losses; not used where there is no target) and writes, where not NULL, hidden_grad [N, D] and
- * weight_grad [V, D] in `dtype`, rounded once from float32 sums; dz is
- * computed again, in pieces of the vocabulary, and held as bf16 (fp32: as
- * three bf16 parts) for the two products.  All results are deterministic.
+ * want_hidden / want_weight say which gradients will be asked for; `state` then
+ * keeps what they need (dpc_head_loss_state_bytes; NULL if neither).  With
+ * want_hidden alone and bf16 operands it keeps the hidden gradient itself, for
+ * grad_loss 1, in float32.  Otherwise dpc_head_loss_grad computes dz again, in
+ * pieces of the vocabulary, held as bf16 (fp32: as three bf16 parts) for the two
+ * products.  It takes the same arguments, grad_loss [N] (the gradient of the losses;
+ * not used where there is no target) and writes, where not NULL, hidden_grad [N, D]
+ * and weight_grad [V, D] in `dtype`, 16-byte aligned, rounded once from float32 sums.
+ * `state` is not changed.  All results are deterministic.  K <= 65536, V <= 2^21.
  * -------------------------------------------------------------------------*/
-size_t dpc_head_loss_workspace_bytes(int64_t N, int D, int V, int K, int dtype);
+size_t dpc_head_loss_state_bytes(int64_t N, int D, int V, int K, int dtype, int want_hidden,
+                                 int want_weight);
+size_t dpc_head_loss_workspace_bytes(int64_t N, int D, int V, int K, int dtype, int want_hidden,
+                                     int want_weight);
 int dpc_head_loss(const void* hidden, const void* weight, int64_t N, int D, int V, int dtype,
                   const int64_t* index, const float* teacher, int K, int64_t ignore_index,
-                  double temperature, float* loss, int32_t* rows, float* lse, int32_t* cols,
-                  float* corr, void* ws, size_t ws_bytes, void* stream);
+                  double temperature, int want_hidden, int want_weight, float* loss, void* state,
+                  size_t state_bytes, void* ws, size_t ws_bytes, void* stream);
 size_t dpc_head_loss_grad_workspace_bytes(int64_t N, int D, int V, int K, int dtype,
                                           int want_hidden, int want_weight);
 int dpc_head_loss_grad(const void* hidden, const void* weight, int64_t N, int D, int V, int dtype,
-                       int32_t* rows, const int32_t* cols, const float* corr, int K,
-                       const float* lse, const float* grad_loss, double temperature, void* hidden_grad,
-                       void* weight_grad, void* ws, size_t ws_bytes, void* stream);
+                       int K, double temperature, int want_hidden, int want_weight,
+                       const void* state, size_t state_bytes, const float* grad_loss,
+                       void* hidden_grad, void* weight_grad, void* ws, size_t ws_bytes,
+                       void* stream);
 
 /* ------------------------------------------------------------------------
  * Routing of tokens to experts (the reference's MoE layers take router logits

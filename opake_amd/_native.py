@@ -198,20 +198,19 @@ SIGNATURES = {
         [_c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_double, _c_void_p,
          _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
     ),
-    "dpc_head_loss_workspace_bytes": (_c_size_t, [_c_i64, _c_int, _c_int, _c_int, _c_int]),
+    "dpc_head_loss_state_bytes": (_c_size_t, [_c_i64] + [_c_int] * 6),
+    "dpc_head_loss_workspace_bytes": (_c_size_t, [_c_i64] + [_c_int] * 6),
     "dpc_head_loss": (
         _c_int,
         [_c_void_p, _c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_int,
-         _c_i64, _c_double, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
-         _c_size_t, _c_void_p],
+         _c_i64, _c_double, _c_int, _c_int, _c_void_p, _c_void_p, _c_size_t, _c_void_p, _c_size_t,
+         _c_void_p],
     ),
-    "dpc_head_loss_grad_workspace_bytes": (
-        _c_size_t, [_c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int]),
+    "dpc_head_loss_grad_workspace_bytes": (_c_size_t, [_c_i64] + [_c_int] * 6),
     "dpc_head_loss_grad": (
         _c_int,
-        [_c_void_p, _c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_void_p, _c_void_p, _c_void_p,
-         _c_int, _c_void_p, _c_void_p, _c_double, _c_void_p, _c_void_p, _c_void_p, _c_size_t,
-         _c_void_p],
+        [_c_void_p, _c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_double, _c_int, _c_int,
+         _c_void_p, _c_size_t, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_size_t, _c_void_p],
     ),
     "dpc_grouped_clipped_sum": (
         _c_int,

@@ -16,14 +16,22 @@
 // kernels run over that many.  So such rows cost nothing and whatever they hold
 // (padding, NaN) reaches nothing.
 //
-// Forward: one product whose 256 x 256 tiles never leave the chip; each leaves
-// its maximum and sum of exponentials per token and the logits at the entries'
-// columns; a join turns them into lse and the loss.  Backward, in pieces of the
-// vocabulary: the logits' tiles again, turned into dz in the accumulators and
-// written as bf16 (float32 inputs: as three bf16 planes, exact), then the two
-// products dz W (added up over the pieces in float32) and dz^T H.  dz at an
-// entry's column, where p and q may cancel, is formed in float32 by the join and
-// put in place of the tile's value.
+// Loss: one product whose 256 x 256 tiles never leave the chip; each leaves its
+// maximum and sum of exponentials per row and the logits at the entries' columns; a
+// join turns them into lse and the loss.
+//
+// Gradients, in one of two ways:
+//   * the hidden states' alone, bf16 (a frozen head): the rows go in chunks, whose
+//     tiles also leave exp(z - tile's maximum) as fp16.  The join turns a chunk's
+//     rows into p - q (bf16) in place, and one product with W gives dH for g = 1,
+//     kept in float32 until the backward multiplies each row by its g.  Two
+//     products in all instead of three.
+//   * otherwise in the backward, in pieces of the vocabulary: the logits' tiles
+//     again, turned into dz in the accumulators and written as bf16 (float32 inputs:
+//     as three bf16 parts, exact), then the products dz W (added up over the pieces
+//     in float32) and dz^T H.
+// dz at an entry's column, where p and q may cancel, is formed in float32 by the
+// join and put in place of the tile's value.
 #include <math.h>
 
 #include "common.h"
@@ -39,7 +47,7 @@ constexpr int kLdsBytes = 131072;
 __shared__ __attribute__((aligned(16))) uint8_t lds_all[kLdsBytes];
 
 // ---------------------------------------------------------------------------
-// Operands as the tiles read them.
+// Rows, entries and operands as the tiles read them.
 // ---------------------------------------------------------------------------
 
 // Plane p (0..2) of x: x0 = bf16(x), x1 = bf16(x - x0), x2 = x - x0 - x1, which
@@ -65,8 +73,6 @@ struct Rows {
   int32_t* place;
 };
 
-Rows rows_of(int32_t* rows, int64_t N) { return Rows{rows, rows + 1, rows + 1 + N}; }
-
 // Distillation: whether a row has an entry that counts (or one that is wrong: an
 // index outside the vocabulary, a NaN).  One wave a row.
 __global__ void __launch_bounds__(256) entries_kernel(const int64_t* __restrict__ index,
@@ -81,64 +87,78 @@ __global__ void __launch_bounds__(256) entries_kernel(const int64_t* __restrict_
     const float t = teacher[n * K + k];
     has |= c >= V || (c >= 0 && !(t == -INFINITY));
   }
-  if (__any(has) && lane == 0) flag[n] = 1;
-  else if (!__any(has) && lane == 0) flag[n] = 0;
+  has = __any(has);
+  if (lane == 0) flag[n] = has;
 }
 
 // Numbers the rows with a target, and writes the others' losses (0).  One
-// workgroup; a thread takes 32 consecutive rows a round, whose flags are the bits
-// of a word.  `flag` (distillation) is rows.place before it is overwritten.
+// workgroup, 8192 rows a round (8 loads in flight a thread): ballots count a wave's
+// 64 rows, and one wave adds up the round's 128 counts.  `flags` (distillation):
+// rows.place holds entries_kernel's flags.
 __global__ void __launch_bounds__(1024) rows_kernel(const int64_t* __restrict__ index,
                                                     int64_t ignore, int flags, int64_t N,
                                                     Rows rows, float* __restrict__ loss) {
-  __shared__ int wave_total[16];
+  __shared__ int total[128], before[129];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   int64_t base = 0;
-  for (int64_t r0 = 0; r0 < N; r0 += 32 * 1024) {
-    const int64_t left = N - r0;
-    const int per = (int)(left >= 32 * 1024 ? 32 : (left + 1023) / 1024);
-    const int64_t first = r0 + (int64_t)tid * per;
-    uint32_t bits = 0;
-    for (int i = 0; i < per; ++i)
-      if (first + i < N && (flags ? rows.place[first + i] != 0 : index[first + i] != ignore))
-        bits |= 1u << i;
-    const int mine = __popc(bits);
-    int upto = mine;  // inclusive sum over the wave
+  for (int64_t r0 = 0; r0 < N; r0 += 8192) {
+    bool on[8];
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(upto, d);
-      if (lane >= d) upto += o;
+    for (int t = 0; t < 8; ++t) {
+      const int64_t n = r0 + t * 1024 + tid;
+      on[t] = n < N && (flags ? rows.place[n] != 0 : index[n] != ignore);
     }
-    if (lane == 63) wave_total[w] = upto;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const unsigned long long m = __ballot(on[t]);
+      if (lane == 0) total[t * 16 + w] = __popcll(m);
+    }
     __syncthreads();
-    int before = 0, all = 0;
-    for (int i = 0; i < 16; ++i) {
-      before += i < w ? wave_total[i] : 0;
-      all += wave_total[i];
+    if (w == 0) {
+      const int a = total[2 * lane], b = total[2 * lane + 1];
+      int upto = a + b;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(upto, d);
+        if (lane >= d) upto += o;
+      }
+      before[2 * lane] = upto - a - b;
+      before[2 * lane + 1] = upto - b;
+      if (lane == 63) before[128] = upto;
     }
-    int64_t at = base + before + upto - mine;
-    for (int i = 0; i < per; ++i) {
-      const int64_t n = first + i;
-      if (n >= N) break;
-      const bool on = (bits >> i) & 1;
-      rows.place[n] = on ? (int32_t)at : -1;
-      if (on)
-        rows.active[at++] = (int32_t)n;
-      else
-        loss[n] = 0.f;
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      const int64_t n = r0 + t * 1024 + tid;
+      const unsigned long long m = __ballot(on[t]);
+      const int64_t at = base + before[t * 16 + w] + __popcll(m & ((1ull << lane) - 1));
+      if (n < N) {
+        rows.place[n] = on[t] ? (int32_t)at : -1;
+        if (on[t])
+          rows.active[at] = (int32_t)n;
+        else
+          loss[n] = 0.f;
+      }
     }
-    base += all;
+    base += before[128];
     __syncthreads();
   }
   if (tid == 0) *rows.count = (int32_t)base;
 }
 
-// Operands as the tiles read them, in planes of bf16 rows padded with zeros:
-// the rows with a target of `hidden` (bf16 rows of whole 16-byte chunks: only if
-// some are left out, else the tiles read the caller's own) and, where the weight
-// needs planes or padding, the weight.  With `index` also the entries' columns in
-// 32 bits (-1: absent, -2: outside the vocabulary); with `zero` also the zero
-// rows of the hidden gradient.
+// The entries of 256 consecutive numbered rows (one B tile) sorted by the 256-wide
+// piece of the vocabulary that they fall into, so that a tile finds its own at
+// start[tile] .. start[tile + 1] - 1 of the block's list.
+struct Entries {
+  int32_t* cols;    // [rows, K]: the column; -1: absent, -2: outside the vocabulary
+  uint2* list;      // [blocks][256 K]: {row in block * K + k, row in block << 8 | column in tile}
+  int32_t* start;   // [blocks][tiles + 1]
+};
+
+// Operands as the tiles read them, in planes of bf16 rows padded with zeros: the
+// rows with a target of `hidden` (bf16 rows of whole 16-byte chunks: only if some
+// are left out, else the tiles read the caller's own) and, where it needs planes or
+// padding, the weight.  The first `blocks` workgroups make the entries' lists.
 struct PrepArgs {
   const void* hidden;
   const void* weight;  // null: read as it is
@@ -150,8 +170,11 @@ struct PrepArgs {
   bool pack;
   const int64_t* index;
   bool teacher;
-  int32_t* cols;
-  void* zero;
+  int blocks, tiles;
+  Entries entries;
+  void* zero;          // the hidden gradient, whose rows without a target are zeroed
+  const float* g;      // backward: the losses' gradient,
+  float* gmax;         // and its largest magnitude that is finite (1 if all are 0)
 };
 
 DPC_DEVICE void pack_chunk(const void* src, int dtype, int64_t row, int D, int c, int64_t ld,
@@ -182,16 +205,81 @@ DPC_DEVICE void pack_chunk(const void* src, int dtype, int64_t row, int D, int c
   }
 }
 
-__global__ void __launch_bounds__(256) prep_kernel(PrepArgs a) {
-  const int64_t count = *a.rows.count;
-  const int64_t t0 = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
-  if (a.index) {
-    for (int64_t i = t0; i < count * a.K; i += step) {
-      const int64_t c = i / a.K;
-      const int64_t t = a.index[(int64_t)a.rows.active[c] * a.K + (i - c * a.K)];
-      a.cols[i] = a.teacher && t < 0 ? -1 : (t >= 0 && t < a.V ? (int32_t)t : -2);
+constexpr int kPrepThreads = 512;
+constexpr int kMaxTiles = 1 << 13;  // of the vocabulary (lists' counters in LDS)
+
+DPC_DEVICE void list_entries(const PrepArgs& a, int block, int64_t count, int* counter) {
+  const int tid = threadIdx.x;
+  const int64_t first = (int64_t)block * kMmTile;
+  if (first >= count) return;
+  const int rows = (int)(count - first < kMmTile ? count - first : kMmTile);
+  const int n = rows * a.K;
+  for (int t = tid; t <= a.tiles; t += kPrepThreads) counter[t] = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += kPrepThreads) {
+    const int r = i / a.K;
+    const int64_t t = a.index[(int64_t)a.rows.active[first + r] * a.K + (i - r * a.K)];
+    const int c = a.teacher && t < 0 ? -1 : (t >= 0 && t < a.V ? (int)t : -2);
+    a.entries.cols[first * a.K + i] = c;
+    if (c >= 0) atomicAdd(&counter[(c >> 8) + 1], 1);
+  }
+  __syncthreads();
+  if (tid < 64) {  // counts -> starts, 64 tiles at a time
+    int base = 0;
+    for (int t0 = 0; t0 <= a.tiles; t0 += 64) {
+      const int t = t0 + tid;
+      const int mine = t <= a.tiles ? counter[t] : 0;
+      int upto = mine;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(upto, d);
+        if (tid >= d) upto += o;
+      }
+      if (t <= a.tiles) {
+        counter[t] = base + upto;
+        a.entries.start[(int64_t)block * (a.tiles + 1) + t] = base + upto;
+      }
+      base += __shfl(upto, 63);
     }
   }
+  __syncthreads();
+  // The order within a tile's entries is that of the atomics: each entry has a place
+  // of its own in every output, so no result depends on it.
+  uint2* list = a.entries.list + first * a.K;
+  for (int i = tid; i < n; i += kPrepThreads) {
+    const int c = a.entries.cols[first * a.K + i];
+    if (c < 0) continue;
+    const int at = atomicAdd(&counter[c >> 8], 1);
+    list[at] = make_uint2((uint32_t)i, (uint32_t)((i / a.K) << 8 | (c & 255)));
+  }
+}
+
+__global__ void __launch_bounds__(kPrepThreads) prep_kernel(PrepArgs a) {
+  extern __shared__ int counter[];
+  const int64_t count = *a.rows.count;
+  if ((int)blockIdx.x < a.blocks) {
+    list_entries(a, blockIdx.x, count, counter);
+    return;
+  }
+  if (a.g && blockIdx.x == 0) {
+    __shared__ float wave_top[kPrepThreads / 64];
+    float top = 0.f;
+#pragma unroll 8
+    for (int64_t i = threadIdx.x; i < count; i += kPrepThreads) {
+      const float x = fabsf(a.g[a.rows.active[i]]);
+      if (x < INFINITY) top = fmaxf(top, x);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if ((threadIdx.x & 63) == 0) wave_top[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < kPrepThreads / 64; ++i) top = fmaxf(top, wave_top[i]);
+      *a.gmax = top > 0.f ? top : 1.f;
+    }
+  }
+  const int64_t t0 = (int64_t)(blockIdx.x - a.blocks) * kPrepThreads + threadIdx.x,
+                step = (int64_t)(gridDim.x - a.blocks) * kPrepThreads;
   const int64_t chunks = a.ld / 8;
   if (a.h && (a.pack || count < a.N))
     for (int64_t i = t0; i < count * chunks; i += step) {
@@ -216,24 +304,25 @@ __global__ void __launch_bounds__(256) prep_kernel(PrepArgs a) {
 }
 
 // The hidden rows that a launch reads: the caller's where every row has a target
-// and needs no padding, else the packed ones; and how many.
+// and needs no padding, else the packed ones; `first`, `most`: the launch's chunk.
 struct Hidden {
   const uint16_t* own;  // null: always the packed rows
   const uint16_t* packed;
   const int32_t* count;
-  int64_t N;
+  int64_t N, ld;
+  int first, most;
 };
 
 DPC_DEVICE int hidden_rows(const Hidden& h, const uint16_t** p) {
   const int count = __builtin_amdgcn_readfirstlane(*h.count);
-  *p = h.own && count == h.N ? h.own : h.packed;
-  return count;
+  *p = (h.own && count == h.N ? h.own : h.packed) + h.first * h.ld;
+  return max(0, min(count - h.first, h.most));
 }
 
 DPC_DEVICE int tiles_of(int rows) { return (rows + kMmTile - 1) / kMmTile; }
 
 // ---------------------------------------------------------------------------
-// Forward: the tile's statistics and the entries' logits.
+// Loss: the tile's statistics and the entries' logits.
 // ---------------------------------------------------------------------------
 
 struct StatsArgs {
@@ -241,11 +330,29 @@ struct StatsArgs {
   Hidden h;
   int V, K;
   float inv_tau;
-  const int32_t* cols;  // [rows, K]
-  float* picked;        // [rows, K]: z at the entries' columns
-  f32x2_t* part;        // [rows, tiles_a]: maximum and sum of exponentials of each tile
+  Entries entries;
+  float* picked;   // [rows, K]: z at the entries' columns
+  f32x2_t* part;   // [rows, tiles_a]: maximum and sum of exponentials of each tile
+  _Float16* e;     // [chunk's rows, lde]: exp(z - the tile's maximum)
+  int64_t lde;
 };
 
+// Byte of (row of the tile, column) in a 256 x 256 tile of 2-byte values in LDS:
+// 512-byte rows whose 16-byte chunks are XOR-swizzled by the row.
+DPC_DEVICE int tile16_off(int row, int col) {
+  return row * 512 + (((col >> 3) ^ (row & 15)) << 4) + (col & 7) * 2;
+}
+
+// The staged tile to dst [rows, ld] (16 bytes a lane).
+DPC_DEVICE void store_tile16(uint16_t* dst, int64_t ld, int rows) {
+  for (int i = threadIdx.x; i < rows * 32; i += kMmThreads) {
+    const int t = i >> 5, c = i & 31;
+    *reinterpret_cast<u32x4_t*>(dst + t * ld + 8 * c) =
+        *reinterpret_cast<const u32x4_t*>(lds_all + tile16_off(t, 8 * c));
+  }
+}
+
+template <bool kEmit>
 __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) {
   int split, ta, tb;
   const int N = hidden_rows(s.h, &s.mm.b.p);
@@ -254,12 +361,60 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
   if (!mm_tile_of(s.mm, &split, &ta, &tb)) return;
   MmAcc acc;
   mm_loop<true, true>(s.mm, ta, tb, 0, lds_all, acc);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w & 1, wn = w >> 1;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6),
+            wm = w & 1, wn = w >> 1;
   const int v0 = ta * kMmTile, n0 = tb * kMmTile;
+  const int64_t g0 = s.h.first + n0;  // the row's number
   const int vl = wm * 128 + 4 * (lane >> 4);  // + 16 i + r
   const int tl = wn * 64 + (lane & 15);       // + 16 j
   const int vleft = s.V - v0 - vl;
-  f32x2_t* st = reinterpret_cast<f32x2_t*>(lds_all);  // [2][256]
+  if (s.inv_tau != 1.0f) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc.v[i][j] *= s.inv_tau;
+  }
+  // Entries: the blocks of 16 rows that have one, in float32 through LDS (rows of 1
+  // KiB, 16-byte chunks XOR-swizzled by the row), eight at a time.
+  const int64_t blk = g0 / kMmTile;
+  const int32_t* start = s.entries.start + blk * (s.mm.tiles_a + 1) + ta;
+  const uint2* list = s.entries.list + g0 * s.K;
+  const int e0 = start[0], e1 = start[1];
+  if (e1 > e0) {
+    uint32_t hit = 0;
+    for (int e = e0 + lane; e < e1; e += 64) hit |= 1u << (list[e].y >> 12);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) hit |= __shfl_xor(hit, d);
+    hit = __builtin_amdgcn_readfirstlane(hit);
+    const int slots = __popc(hit);
+    for (int p = 0; p < slots; p += 8) {
+      if (p) __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int b = wn * 4 + j, slot = __popc(hit & ((1u << b) - 1)) - p;
+        if (((hit >> b) & 1) && slot >= 0 && slot < 8) {
+          const int t = lane & 15;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<f32x4_t*>(lds_all + slot * 16384 + t * 1024 +
+                                        ((((vl + 16 * i) >> 2) ^ t) << 4)) = acc.v[i][j];
+        }
+      }
+      __syncthreads();
+      for (int e = e0 + tid; e < e1; e += kMmThreads) {
+        const uint2 x = list[e];
+        const int t = (x.y >> 8) & 15, c = x.y & 255, b = x.y >> 12;
+        const int slot = __popc(hit & ((1u << b) - 1)) - p;
+        if (slot >= 0 && slot < 8)
+          s.picked[g0 * s.K + x.x] = *reinterpret_cast<const float*>(
+              lds_all + slot * 16384 + t * 1024 + (((c >> 2) ^ t) << 4) + (c & 3) * 4);
+      }
+    }
+    __syncthreads();
+  }
+  // Maxima, then exponentials against the tile's (both halves of the vocabulary).
+  float* tops = reinterpret_cast<float*>(lds_all);  // [2][256]
+  float* sums = tops + 512;                         // [2][256]
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float m = -INFINITY;
@@ -267,60 +422,50 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float z = acc.v[i][j][r] * s.inv_tau;
-        acc.v[i][j][r] = z;
-        if (16 * i + r < vleft) m = fmaxf(m, z);
+        if (16 * i + r >= vleft) acc.v[i][j][r] = -INFINITY;
+        m = fmaxf(m, acc.v[i][j][r]);
       }
     m = fmaxf(m, __shfl_xor(m, 16));
     m = fmaxf(m, __shfl_xor(m, 32));
+    if (lane < 16) tops[wm * 256 + tl + 16 * j] = m;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float m = fmaxf(tops[tl + 16 * j], tops[256 + tl + 16 * j]);
+    const float base = (m == -INFINITY ? 0.f : m) * kLog2e;
     float sum = 0.f;
-    const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (16 * i + r < vleft) sum += fast_exp(acc.v[i][j][r] - base);
+      for (int r = 0; r < 4; ++r) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(acc.v[i][j][r], kLog2e, -base));
+        acc.v[i][j][r] = e;
+        sum += e;
+      }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    if (lane < 16) st[wm * 256 + tl + 16 * j] = f32x2_t{m, sum};
+    if (lane < 16) sums[wm * 256 + tl + 16 * j] = sum;
   }
   __syncthreads();
-  if (tid < kMmTile && n0 + tid < N) {
-    const f32x2_t a = st[tid], b = st[256 + tid];
-    const float m = fmaxf(a.x, b.x), base = m == -INFINITY ? 0.f : m;
-    s.part[(int64_t)(n0 + tid) * s.mm.tiles_a + ta] =
-        f32x2_t{m, a.y * fast_exp(a.x - base) + b.y * fast_exp(b.x - base)};
-  }
-  // Entries: the tile in float32, 128 tokens at a time, rows of 1 KiB whose
-  // 16-byte chunks are XOR-swizzled by the token.
-#pragma unroll
-  for (int p = 0; p < 2; ++p) {
+  if (tid < kMmTile && n0 + tid < N)
+    s.part[(g0 + tid) * s.mm.tiles_a + ta] =
+        f32x2_t{fmaxf(tops[tid], tops[256 + tid]), sums[tid] + sums[256 + tid]};
+  if constexpr (kEmit) {
     __syncthreads();
-    if ((wn >> 1) == p) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int t = (tl + 16 * j) & 127, v = vl + 16 * i;
-          *reinterpret_cast<f32x4_t*>(lds_all + t * 1024 + (((v >> 2) ^ (t & 15)) << 4)) =
-              acc.v[i][j];
-        }
-    }
-    __syncthreads();
-    const int64_t first = n0 + 128 * p;
-    const int64_t left = N - first;
-    if (left > 0) {
-      const int64_t base = first * s.K;
-      const int count = (int)(left < 128 ? left : 128) * s.K;
-      for (int e = tid; e < count; e += kMmThreads) {
-        const int c = s.cols[base + e] - v0;
-        if ((unsigned)c < (unsigned)kMmTile) {
-          const int t = e / s.K;
-          s.picked[base + e] = *reinterpret_cast<const float*>(
-              lds_all + t * 1024 + (((c >> 2) ^ (t & 15)) << 4) + (c & 3) * 4);
-        }
+      for (int i = 0; i < 8; ++i) {
+        typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+        half4_t h;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) h[r] = (_Float16)acc.v[i][j][r];
+        *reinterpret_cast<half4_t*>(lds_all + tile16_off(tl + 16 * j, vl + 16 * i)) = h;
       }
-    }
+    __syncthreads();
+    store_tile16(reinterpret_cast<uint16_t*>(s.e) + (int64_t)n0 * s.lde + v0, s.lde,
+                 min(N - n0, kMmTile));
   }
 }
 
@@ -346,13 +491,14 @@ struct JoinArgs {
   float* loss;  // at the row's own place; the others by the row's number
   float* lse;   // NaN: an entry outside the vocabulary or NaN
   float* corr;  // [rows, K]: p - sum of the q of all entries of the column
+  // A chunk's rows, to be turned into p - q in place.
+  int first, most;
+  uint16_t* e;
+  int64_t lde;
 };
 
-// One wave a row.
-__global__ void __launch_bounds__(256) head_join_kernel(JoinArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (n >= *a.rows.count) return;
+// Row n by one wave; its lse.
+DPC_DEVICE float join_row(const JoinArgs& a, int64_t n, int lane) {
   const int64_t own = a.rows.active[n];
   const f32x2_t* part = a.part + n * a.parts;
   float m = -INFINITY, sum = 0.f;
@@ -369,28 +515,28 @@ __global__ void __launch_bounds__(256) head_join_kernel(JoinArgs a) {
   const float* picked = a.picked + n * a.K;
   float* corr = a.corr + n * a.K;
   if (!a.teacher) {
+    const int c = cols[0];
+    if (c < 0) lse = NAN;
+    const float z = c >= 0 ? picked[0] : 0.f;
     if (lane == 0) {
-      const int c = cols[0];
-      if (c < 0) lse = NAN;
-      const float z = c >= 0 ? picked[0] : 0.f;
       a.loss[own] = (lse - z) * a.loss_scale;
       a.lse[n] = lse;
       corr[0] = fast_exp(z - lse) - 1.0f;
     }
-    return;
+    return lse;
   }
   const float* teacher = a.teacher + own * a.K;
   float tm = -INFINITY;
-  bool bad = false, nan = false;
+  bool bad = false;
   for (int k = lane; k < a.K; k += 64) {
     const int c = cols[k];
     bad |= c == -2;
     if (c >= 0) {
-      nan |= isnan(teacher[k]);
+      bad |= isnan(teacher[k]);
       tm = fmaxf(tm, teacher[k] * a.inv_tau);
     }
   }
-  bad = __any(bad || nan);
+  bad = __any(bad);
   tm = wave_max(tm);
   float es = 0.f;
   for (int k = lane; k < a.K; k += 64)
@@ -398,24 +544,106 @@ __global__ void __launch_bounds__(256) head_join_kernel(JoinArgs a) {
   es = wave_sum(es);
   const float logs = logf(es);
   float loss = 0.f;
-  for (int k = lane; k < a.K; k += 64) {
-    const int c = cols[k];
-    float out = 0.f;
-    if (c >= 0) {
-      const float lq = teacher[k] * a.inv_tau - tm - logs, q = fast_exp(lq);
-      const float z = picked[k];
-      if (q != 0.f) loss += q * (lq - (z - lse));
-      float qs = 0.f;
-      for (int i = 0; i < a.K; ++i)
-        if (cols[i] == c) qs += fast_exp(teacher[i] * a.inv_tau - tm - logs);
-      out = fast_exp(z - lse) - qs;
+  for (int k0 = 0; k0 < a.K; k0 += 64) {
+    const int k = k0 + lane;
+    const int c = k < a.K ? cols[k] : -1;
+    const float lq = c >= 0 ? teacher[k] * a.inv_tau - tm - logs : -INFINITY;
+    const float q = fast_exp(lq), z = c >= 0 ? picked[k] : 0.f;
+    if (c >= 0 && q != 0.f) loss += q * (lq - (z - lse));
+    // q of every entry of this column: the other entries, 64 at a time.
+    float qs = 0.f;
+    for (int i0 = 0; i0 < a.K; i0 += 64) {
+      const int i = i0 + lane;
+      const int ci = i < a.K ? cols[i] : -1;
+      const float qi = ci >= 0 ? fast_exp(teacher[i] * a.inv_tau - tm - logs) : 0.f;
+      const int left = min(64, a.K - i0);
+      for (int o = 0; o < left; ++o) {
+        const int co = __builtin_amdgcn_readlane(ci, o);
+        const float qo = __builtin_bit_cast(
+            float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, qi), o));
+        if (co == c) qs += qo;
+      }
     }
-    corr[k] = out;
+    if (k < a.K) corr[k] = c >= 0 ? fast_exp(z - lse) - qs : 0.f;
   }
   loss = wave_sum(loss);
+  if (bad) lse = NAN;
   if (lane == 0) {
     a.loss[own] = bad ? NAN : loss * a.loss_scale;
-    a.lse[n] = bad ? NAN : lse;
+    a.lse[n] = lse;
+  }
+  return lse;
+}
+
+// One wave a row.
+__global__ void __launch_bounds__(256) head_join_kernel(JoinArgs a) {
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (n < *a.rows.count) join_row(a, n, threadIdx.x & 63);
+}
+
+// One workgroup a row of a chunk: the join, then the row's exp(z - tile's maximum)
+// times exp(tile's maximum - lse), and at the entries' columns p - q.
+__global__ void __launch_bounds__(256) head_join_chunk_kernel(JoinArgs a) {
+  __shared__ float shared_lse;
+  const int tid = threadIdx.x;
+  const int64_t n = a.first + (int64_t)blockIdx.x;
+  if ((int)blockIdx.x >= a.most || n >= *a.rows.count) return;
+  if (tid < 64) {
+    const float lse = join_row(a, n, tid);
+    if (tid == 0) shared_lse = lse;
+  }
+  __syncthreads();
+  const float lse = shared_lse;
+  typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+  uint16_t* row = a.e + (int64_t)blockIdx.x * a.lde;
+  const f32x2_t* part = a.part + n * a.parts;
+  const int chunks = (int)(a.lde / 8);
+#pragma unroll 4
+  for (int i = tid; i < chunks; i += 256) {
+    const half8_t h = *reinterpret_cast<const half8_t*>(row + 8 * i);
+    const float f = fast_exp(part[i >> 5].x - lse);
+    u32x4_t o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      o[e] = f32x2_to_bf16x2_bits((float)h[2 * e] * f, (float)h[2 * e + 1] * f);
+    *reinterpret_cast<u32x4_t*>(row + 8 * i) = o;
+  }
+  __syncthreads();
+  for (int k = tid; k < a.K; k += 256) {
+    const int c = a.cols[n * a.K + k];
+    if (c >= 0) row[c] = f32_to_bf16_bits(a.corr[n * a.K + k]);
+  }
+}
+
+// out row n = unit's row place[n] times g[n] coef; 0 without a target.
+__global__ void __launch_bounds__(256) head_scale_kernel(const float* __restrict__ unit, Rows rows,
+                                                         const float* __restrict__ g, float coef,
+                                                         int64_t N, int D,
+                                                         uint16_t* __restrict__ out) {
+  if (D % 8 == 0) {
+    const int chunks = D / 8;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < N * chunks;
+         i += (int64_t)gridDim.x * 256) {
+      const int64_t n = i / chunks;
+      const int c = (int)(i - n * chunks) * 8;
+      const int at = rows.place[n];
+      u32x4_t o = {0u, 0u, 0u, 0u};
+      if (at >= 0) {
+        const float f = g[n] * coef;
+        const f32x4_t* u = reinterpret_cast<const f32x4_t*>(unit + (int64_t)at * D + c);
+        const f32x4_t x = u[0] * f, y = u[1] * f;
+        o = u32x4_t{f32x2_to_bf16x2_bits(x[0], x[1]), f32x2_to_bf16x2_bits(x[2], x[3]),
+                    f32x2_to_bf16x2_bits(y[0], y[1]), f32x2_to_bf16x2_bits(y[2], y[3])};
+      }
+      *reinterpret_cast<u32x4_t*>(out + n * D + c) = o;
+    }
+  } else {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < N * D;
+         i += (int64_t)gridDim.x * 256) {
+      const int64_t n = i / D;
+      const int at = rows.place[n];
+      out[i] = at < 0 ? 0 : f32_to_bf16_bits(unit[at * (int64_t)D + (i - n * D)] * (g[n] * coef));
+    }
   }
 }
 
@@ -427,13 +655,15 @@ struct GradArgs {
   MmArgs mm;  // A = W from the piece's first row, B = H
   Hidden h;
   const int32_t* active;
-  int V, K, first;  // the piece's first column
-  float inv_tau, coef;
-  const int32_t* cols;
+  int V, K, tile0, tiles;  // the piece's first tile; tiles of the vocabulary
+  float inv_tau;
+  Entries entries;
   const float* corr;
   const float* lse;
-  const float* g;  // [N]: the losses' gradient, at the rows' own places
-  uint16_t* dz;    // [planes][rows][ld]
+  const float* g;     // [N]: the losses' gradient, at the rows' own places
+  const float* gmax;  // dz is held over gmax, so a gradient that is the same for all
+                      // rows (one over the tokens) is not rounded with every value
+  uint16_t* dz;       // [planes][rows][ld]
   int64_t ld, plane;
 };
 
@@ -447,30 +677,29 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
   MmAcc acc;
   mm_loop<true, true>(s.mm, ta, tb, 0, lds_all, acc);
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w & 1, wn = w >> 1;
-  const int p0 = ta * kMmTile, v0 = s.first + p0;
-  const int64_t n0 = (int64_t)tb * kMmTile;
+  const int vt = s.tile0 + ta, n0 = tb * kMmTile;
   const int vl = wm * 128 + 4 * (lane >> 4);
   const int tl = wn * 64 + (lane & 15);
-  const int vleft = s.V - v0 - vl;
+  const int vleft = s.V - vt * kMmTile - vl;
+  const float gmax = *s.gmax;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int64_t n = n0 + tl + 16 * j;
-    const float lse = n < N ? s.lse[n] : 0.f;
-    const float g = n < N ? s.g[s.active[n]] * s.coef : 0.f;
+    const int n = n0 + tl + 16 * j;
+    const float base = n < N ? s.lse[n] * kLog2e : 0.f;
+    const float g = n < N ? s.g[s.active[n]] / gmax : 0.f;
+    const float c = s.inv_tau * kLog2e;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float z = acc.v[i][j][r] * s.inv_tau;
-        acc.v[i][j][r] = 16 * i + r < vleft ? fast_exp(z - lse) * g : 0.f;
+        const float e = __builtin_amdgcn_exp2f(fmaf(acc.v[i][j][r], c, -base)) * g;
+        acc.v[i][j][r] = 16 * i + r < vleft ? e : 0.f;
       }
   }
-  const int64_t left = N - n0;
-  const int rows = (int)(left < kMmTile ? left : kMmTile);
-  const int64_t base = n0 * s.K;
-  const int count = rows * s.K;
-  // One plane at a time through LDS: 256 tokens of 512 bytes, 16-byte chunks
-  // XOR-swizzled by the token.
+  const int rows = min(N - n0, kMmTile);
+  const int32_t* start = s.entries.start + (int64_t)tb * (s.tiles + 1) + vt;
+  const uint2* list = s.entries.list + (int64_t)n0 * s.K;
+  const int e0 = start[0], e1 = start[1];
 #pragma unroll 1
   for (int pl = 0; pl < kPlanes; ++pl) {
     if (pl) __syncthreads();
@@ -478,7 +707,6 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int t = tl + 16 * j, v = vl + 16 * i;
         const f32x4_t x = acc.v[i][j];
         uint32_t lo, hi;
         if (kPlanes == 1) {
@@ -488,26 +716,19 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
           lo = split_plane(x[0], pl) | ((uint32_t)split_plane(x[1], pl) << 16);
           hi = split_plane(x[2], pl) | ((uint32_t)split_plane(x[3], pl) << 16);
         }
-        *reinterpret_cast<uint2*>(lds_all + t * 512 + (((v >> 3) ^ (t & 15)) << 4) + (v & 4) * 2) =
+        *reinterpret_cast<uint2*>(lds_all + tile16_off(tl + 16 * j, vl + 16 * i)) =
             make_uint2(lo, hi);
       }
     __syncthreads();
-    for (int e = tid; e < count; e += kMmThreads) {
-      const int c = s.cols[base + e] - v0;
-      if ((unsigned)c < (unsigned)kMmTile) {
-        const int t = e / s.K;
-        const float x = s.corr[base + e] * (s.g[s.active[n0 + t]] * s.coef);
-        *reinterpret_cast<uint16_t*>(lds_all + t * 512 + (((c >> 3) ^ (t & 15)) << 4) +
-                                     (c & 7) * 2) =
-            kPlanes == 1 ? f32_to_bf16_bits(x) : split_plane(x, pl);
-      }
+    for (int e = e0 + tid; e < e1; e += kMmThreads) {
+      const uint2 y = list[e];
+      const int t = y.y >> 8;
+      const float x = s.corr[(int64_t)n0 * s.K + y.x] * (s.g[s.active[n0 + t]] / gmax);
+      *reinterpret_cast<uint16_t*>(lds_all + tile16_off(t, y.y & 255)) =
+          kPlanes == 1 ? f32_to_bf16_bits(x) : split_plane(x, pl);
     }
     __syncthreads();
-    for (int i = tid; i < rows * 32; i += kMmThreads) {
-      const int t = i >> 5, c = i & 31;
-      *reinterpret_cast<u32x4_t*>(s.dz + pl * s.plane + (n0 + t) * s.ld + p0 + 8 * c) =
-          *reinterpret_cast<const u32x4_t*>(lds_all + t * 512 + ((c ^ (t & 15)) << 4));
-    }
+    store_tile16(s.dz + pl * s.plane + (int64_t)n0 * s.ld + ta * kMmTile, s.ld, rows);
   }
 }
 
@@ -518,18 +739,28 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
 struct ProductArgs {
   MmArgs mm;
   Hidden h;         // dH: the rows of B and of the output; dW: A and its K
-  const int32_t* active;  // dH, straight to out: the rows' own places
+  const int32_t* active;  // dH straight to out: the rows' own places, or null
   int rows_b;       // dW: the output's rows
   int rows_a;       // the output's row length
   float* partial;   // [splits][plane] float32 rows of lda, or null: straight to out
   int64_t plane;
   int64_t lda;      // rows_a rounded up to 4
   int accumulate;   // add to what partial holds
+  const float* scale;  // straight to out: multiplied by *scale times coef (null: as it is)
+  float coef;
   void* out;
   int out_bf16;
 };
 
-DPC_DEVICE void store_row4(void* out, int64_t at, int left, int bf16, f32x4_t x) {
+DPC_DEVICE void store_row4(void* out, int64_t at, int left, bool whole, int bf16, f32x4_t x) {
+  if (whole) {  // rows of whole quads
+    if (bf16)
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) =
+          make_uint2(f32x2_to_bf16x2_bits(x[0], x[1]), f32x2_to_bf16x2_bits(x[2], x[3]));
+    else
+      *reinterpret_cast<f32x4_t*>(static_cast<float*>(out) + at) = x;
+    return;
+  }
 #pragma unroll
   for (int r = 0; r < 4; ++r)
     if (r < left) {
@@ -540,8 +771,8 @@ DPC_DEVICE void store_row4(void* out, int64_t at, int left, int bf16, f32x4_t x)
     }
 }
 
-// kHidden: dH (A = W, K the piece's columns, B = dz by rows); else dW (A = H, K the
-// rows, B = dz by columns).
+// kHidden: dH (A = W, K the vocabulary, B = dz by rows); else dW (A = H, K the rows,
+// B = dz by columns).
 template <bool kHidden>
 __global__ void __launch_bounds__(kMmThreads, 1) head_product_kernel(ProductArgs s) {
   int split, ta, tb;
@@ -561,11 +792,13 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_product_kernel(ProductArgs
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w & 1, wn = w >> 1;
   const int a0 = ta * kMmTile + wm * 128 + 4 * (lane >> 4);
   const int b0 = tb * kMmTile + wn * 64 + (lane & 15);
+  const bool whole = s.rows_a % 4 == 0;
+  const float f = s.scale ? *s.scale * s.coef : 1.f;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int b = b0 + 16 * j;
     if (b >= rows_b) continue;
-    const int64_t row = kHidden && !s.partial ? s.active[b] : b;
+    const int64_t row = kHidden && s.active && !s.partial ? s.active[b] : b;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int a = a0 + 16 * i;
@@ -576,28 +809,46 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_product_kernel(ProductArgs
         if (s.accumulate) x += *p;
         *p = x;
       } else {
-        store_row4(s.out, row * s.rows_a + a, s.rows_a - a, s.out_bf16, x);
+        store_row4(s.out, row * s.rows_a + a, s.rows_a - a, whole, s.out_bf16, x * f);
       }
     }
   }
 }
 
-// The slices of partial added up in order: row r to out's row active[r] (or r).
-__global__ void __launch_bounds__(256) head_reduce_kernel(const float* __restrict__ partial,
-                                                          int splits, int64_t plane, int64_t rows,
-                                                          const int32_t* __restrict__ count,
-                                                          const int32_t* __restrict__ active,
-                                                          int D, int64_t lda,
-                                                          void* __restrict__ out, int out_bf16) {
-  const int64_t quads = lda / 4, total = (count ? *count : rows) * quads;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total;
+// The slices of partial added up in order, times *scale coef: row r to out's row
+// active[r] (or r).
+struct ReduceArgs {
+  const float* partial;
+  int splits;
+  int64_t plane, rows, lda;
+  const int32_t* count;  // rows from here on the device: clamp(*count - first, 0, rows)
+  int first;
+  const int32_t* active;
+  const float* scale;
+  float coef;
+  int D;
+  void* out;
+  int out_bf16;
+};
+
+__global__ void __launch_bounds__(256) head_reduce_kernel(ReduceArgs a) {
+  const int64_t quads = a.lda / 4;
+  int64_t rows = a.rows;
+  if (a.count) {
+    const int64_t left = (int64_t)*a.count - a.first;
+    rows = left < 0 ? 0 : (left < rows ? left : rows);
+  }
+  const float f = a.scale ? *a.scale * a.coef : 1.f;
+  const bool whole = a.D % 4 == 0;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * quads;
        i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / quads;
     const int c = (int)(i - row * quads) * 4;
-    f32x4_t x = *reinterpret_cast<const f32x4_t*>(partial + row * lda + c);
-    for (int s = 1; s < splits; ++s)
-      x += *reinterpret_cast<const f32x4_t*>(partial + s * plane + row * lda + c);
-    store_row4(out, (active ? active[row] : row) * (int64_t)D + c, D - c, out_bf16, x);
+    f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.partial + row * a.lda + c);
+    for (int s = 1; s < a.splits; ++s)
+      x += *reinterpret_cast<const f32x4_t*>(a.partial + s * a.plane + row * a.lda + c);
+    store_row4(a.out, (a.active ? a.active[row] : row) * (int64_t)a.D + c, a.D - c, whole,
+               a.out_bf16, x * f);
   }
 }
 
@@ -605,23 +856,10 @@ __global__ void __launch_bounds__(256) head_reduce_kernel(const float* __restric
 // Host side.
 // ---------------------------------------------------------------------------
 
-constexpr int64_t kDzBytes = 256ll << 20;  // dz of one piece
+// Held at once: dz of a piece of the vocabulary, or a chunk's exponentials.
+constexpr int64_t kPieceBytes = 256ll << 20;
 
 int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
-int64_t up_bytes(int64_t x) { return up(x, 256); }
-
-struct Plan {
-  int64_t N;
-  int D, V, K, planes;
-  int64_t ld;  // of the operands as the tiles read them
-  bool pack;
-  int tiles_v, tiles_n, tiles_d;
-  int piece_tiles, pieces;
-  int splits_h, splits_w;
-  int64_t lda;
-  // Byte offsets in the workspace.
-  int64_t h, w, picked, part, dz, ph, pw, bytes;
-};
 
 // Slices of `steps` K steps for `tiles` tiles: about one workgroup a compute
 // unit, no slice under 8 steps.
@@ -633,201 +871,351 @@ int slices(int64_t tiles, int64_t steps) {
 }
 
 bool valid_head(int64_t N, int D, int V, int K, int dtype) {
-  return N >= 0 && N <= 0x7fffff00ll && D >= 1 && D <= (1 << 20) && V >= 1 && V <= (1 << 30) &&
-         K >= 1 && K <= (1 << 16) && (dtype == DPC_F32 || dtype == DPC_BF16);
+  return N >= 0 && N <= 0x7fffff00ll && D >= 1 && D <= (1 << 20) && V >= 1 &&
+         V <= kMaxTiles * kMmTile && K >= 1 && K <= (1 << 16) &&
+         (dtype == DPC_F32 || dtype == DPC_BF16);
 }
 
-Plan head_plan(int64_t N, int D, int V, int K, int dtype, bool backward, bool dh, bool dw) {
+// What a call needs and where it lies.
+struct Plan {
+  int64_t N;
+  int D, V, K, dtype, planes;
+  bool want_h, want_w, emit;
+  int64_t ld;  // of the operands as the tiles read them
+  bool pack;
+  int tiles_v, tiles_n, tiles_d;
+  int64_t lda;
+  int chunk, splits_c;           // emit: rows of a chunk, slices of its product
+  int piece_tiles, pieces;       // backward
+  int splits_h, splits_w;
+  // Byte offsets: state (kept for the backward), workspaces.
+  int64_t s_rows, s_lse, s_corr, s_list, s_start, s_unit, state_bytes;
+  int64_t f_rows, f_lse, f_corr, f_list, f_start, f_cols, f_h, f_w, f_picked, f_part, f_e, f_pc,
+      fwd_bytes;
+  int64_t b_h, b_w, b_g, b_dz, b_ph, b_pw, bwd_bytes;
+};
+
+Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w) {
   Plan p = {};
   p.N = N;
   p.D = D;
   p.V = V;
   p.K = K;
+  p.dtype = dtype;
   p.planes = dtype == DPC_F32 ? 3 : 1;
+  p.want_h = want_h != 0;
+  p.want_w = want_w != 0;
+  p.emit = p.want_h && !p.want_w && p.planes == 1;
   p.ld = up(D, 8);
   p.pack = dtype == DPC_F32 || D % 8 != 0;
   p.tiles_v = (V + kMmTile - 1) / kMmTile;
   p.tiles_n = (int)((N + kMmTile - 1) / kMmTile);
   p.tiles_d = (D + kMmTile - 1) / kMmTile;
   p.lda = up(D, 4);
+  const int pairs = p.planes == 1 ? 1 : 6;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
-    at += up_bytes(bytes);
+    at += up(bytes, 256);
     return o;
   };
-  p.h = take(p.planes * N * p.ld * 2);
-  if (p.pack) p.w = take(p.planes * (int64_t)V * p.ld * 2);
-  if (!backward) {
-    p.picked = take(N * K * 4);
-    p.part = take(N * p.tiles_v * 8);
-  } else {
-    int64_t t = kDzBytes / (p.planes * N * kMmTile * 2);
+  const int64_t rows_b = (2 * N + 1) * 4, lse_b = N * 4, corr_b = N * K * 4, list_b = N * K * 8,
+                start_b = (int64_t)p.tiles_n * (p.tiles_v + 1) * 4;
+  const bool keep = (p.want_h || p.want_w) && !p.emit;
+  if (p.want_h || p.want_w) p.s_rows = take(rows_b);
+  if (keep) {
+    p.s_lse = take(lse_b);
+    p.s_corr = take(corr_b);
+    p.s_list = take(list_b);
+    p.s_start = take(start_b);
+  }
+  if (p.emit) p.s_unit = take(N * D * 4);
+  p.state_bytes = at;
+  at = 0;
+  if (!p.want_h && !p.want_w) p.f_rows = take(rows_b);
+  if (!keep) {
+    p.f_lse = take(lse_b);
+    p.f_corr = take(corr_b);
+    p.f_list = take(list_b);
+    p.f_start = take(start_b);
+  }
+  p.f_cols = take(N * K * 4);
+  p.f_h = take(p.planes * N * p.ld * 2);
+  if (p.pack) p.f_w = take(p.planes * (int64_t)V * p.ld * 2);
+  p.f_picked = take(N * K * 4);
+  p.f_part = take(N * p.tiles_v * 8);
+  if (p.emit) {
+    int64_t c = kPieceBytes / ((int64_t)p.tiles_v * kMmTile * 2) / kMmTile * kMmTile;
+    if (c < kMmTile) c = kMmTile;
+    // Chunks of equal size.
+    const int64_t rows = up(N, kMmTile);
+    if (c > rows) c = rows;
+    const int64_t n = (rows + c - 1) / c;
+    p.chunk = (int)up((rows + n - 1) / n, kMmTile);
+    p.splits_c = slices((int64_t)p.tiles_d * (p.chunk / kMmTile), p.tiles_v * 4);
+    p.f_e = take(p.chunk * (int64_t)p.tiles_v * kMmTile * 2);
+    if (p.splits_c > 1) p.f_pc = take(p.splits_c * p.chunk * p.lda * 4);
+  }
+  p.fwd_bytes = at;
+  at = 0;
+  if (keep) {
+    p.b_h = take(p.planes * N * p.ld * 2);
+    if (p.pack) p.b_w = take(p.planes * (int64_t)V * p.ld * 2);
+    p.b_g = take(4);
+    int64_t t = kPieceBytes / (p.planes * N * kMmTile * 2);
     if (t < 1) t = 1;
     if (t > p.tiles_v) t = p.tiles_v;
     p.pieces = (int)((p.tiles_v + t - 1) / t);
     p.piece_tiles = (p.tiles_v + p.pieces - 1) / p.pieces;
-    const int pairs = p.planes == 1 ? 1 : 6;
-    p.dz = take(p.planes * N * p.piece_tiles * kMmTile * 2);
-    if (dh) {
+    p.pieces = (p.tiles_v + p.piece_tiles - 1) / p.piece_tiles;
+    p.b_dz = take(p.planes * N * p.piece_tiles * kMmTile * 2);
+    if (p.want_h) {
       p.splits_h = slices((int64_t)p.tiles_d * p.tiles_n, (int64_t)pairs * p.piece_tiles * 4);
-      if (p.pieces > 1 || p.splits_h > 1) p.ph = take(p.splits_h * N * p.lda * 4);
+      if (p.pieces > 1 || p.splits_h > 1) p.b_ph = take(p.splits_h * N * p.lda * 4);
     }
-    if (dw) {
+    if (p.want_w) {
       p.splits_w = slices((int64_t)p.tiles_d * p.piece_tiles, pairs * ((N + 63) / 64));
       if (p.splits_w > 1)
-        p.pw = take(p.splits_w * (int64_t)p.piece_tiles * kMmTile * p.lda * 4);
+        p.b_pw = take(p.splits_w * (int64_t)p.piece_tiles * kMmTile * p.lda * 4);
     }
   }
-  p.bytes = at;
+  p.bwd_bytes = at;
   return p;
 }
 
-unsigned grid_for(int64_t items) {
-  int64_t g = (items + 255) / 256;
-  return (unsigned)(g > 16384 ? 16384 : (g < 1 ? 1 : g));
+Rows rows_at(uint8_t* base, int64_t N) {
+  int32_t* r = reinterpret_cast<int32_t*>(base);
+  return Rows{r, r + 1, r + 1 + N};
 }
 
-// Numbers of rows and operands: the prep launch, and W and H as the tiles read them.
-int operands(const Plan& p, PrepArgs& a, uint8_t* ws, hipStream_t s, Hidden* h, MmOperand* w) {
+// The prep launch, and W and H as the tiles read them.
+int operands(const Plan& p, PrepArgs& a, const void* hidden, const void* weight, uint8_t* h,
+             uint8_t* w, hipStream_t s, Hidden* ho, MmOperand* wo) {
+  a.hidden = hidden;
+  a.weight = p.pack ? weight : nullptr;
+  a.dtype = p.dtype;
+  a.D = p.D;
+  a.V = p.V;
+  a.K = p.K;
+  a.N = p.N;
   a.ld = p.ld;
   a.pack = p.pack;
-  a.h = reinterpret_cast<uint16_t*>(ws + p.h);
-  a.w = reinterpret_cast<uint16_t*>(ws + p.w);
-  const void* weight = a.weight;
-  if (!p.pack) a.weight = nullptr;
+  a.h = reinterpret_cast<uint16_t*>(h);
+  a.w = reinterpret_cast<uint16_t*>(w);
   int64_t items = p.N * p.ld / 8;
   if (p.pack && p.V * p.ld / 8 > items) items = p.V * p.ld / 8;
-  hipLaunchKernelGGL(prep_kernel, dim3(grid_for(items)), dim3(256), 0, s, a);
+  int64_t grid = (items + kPrepThreads - 1) / kPrepThreads;
+  if (grid > 4096) grid = 4096;
+  const size_t lds = a.blocks ? (size_t)(a.tiles + 1) * 4 : 0;
+  hipLaunchKernelGGL(prep_kernel, dim3((unsigned)(a.blocks + grid)), dim3(kPrepThreads), lds, s, a);
   DPC_HIP_CHECK(hipGetLastError());
-  *h = Hidden{p.pack ? nullptr : static_cast<const uint16_t*>(a.hidden), a.h, a.rows.count, p.N};
-  *w = MmOperand{p.pack ? a.w : static_cast<const uint16_t*>(weight), p.ld, (int64_t)p.V * p.ld,
-                 p.V};
+  *ho = Hidden{p.pack ? nullptr : static_cast<const uint16_t*>(hidden), a.h, a.rows.count, p.N,
+               p.ld, 0, (int)p.N};
+  *wo = MmOperand{p.pack ? a.w : static_cast<const uint16_t*>(weight), p.ld, (int64_t)p.V * p.ld,
+                  p.V};
+  return DPC_OK;
+}
+
+int reduce(const ReduceArgs& a, hipStream_t s) {
+  int64_t grid = (a.rows * (a.lda / 4) + 255) / 256;
+  if (grid > 8192) grid = 8192;
+  hipLaunchKernelGGL(head_reduce_kernel, dim3((unsigned)grid), dim3(256), 0, s, a);
+  DPC_HIP_CHECK(hipGetLastError());
   return DPC_OK;
 }
 
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
+bool valid_temperature(double t) { return t > 0.0 && t < 1e15; }
+
 }  // namespace
 
-extern "C" size_t dpc_head_loss_workspace_bytes(int64_t N, int D, int V, int K, int dtype) {
+extern "C" size_t dpc_head_loss_state_bytes(int64_t N, int D, int V, int K, int dtype,
+                                            int want_hidden, int want_weight) {
   if (!valid_head(N, D, V, K, dtype) || N == 0) return 0;
-  return (size_t)head_plan(N, D, V, K, dtype, false, false, false).bytes;
+  return (size_t)head_plan(N, D, V, K, dtype, want_hidden, want_weight).state_bytes;
+}
+
+extern "C" size_t dpc_head_loss_workspace_bytes(int64_t N, int D, int V, int K, int dtype,
+                                                int want_hidden, int want_weight) {
+  if (!valid_head(N, D, V, K, dtype) || N == 0) return 0;
+  return (size_t)head_plan(N, D, V, K, dtype, want_hidden, want_weight).fwd_bytes;
 }
 
 extern "C" size_t dpc_head_loss_grad_workspace_bytes(int64_t N, int D, int V, int K, int dtype,
                                                      int want_hidden, int want_weight) {
   if (!valid_head(N, D, V, K, dtype) || N == 0) return 0;
-  return (size_t)head_plan(N, D, V, K, dtype, true, want_hidden != 0, want_weight != 0).bytes;
+  return (size_t)head_plan(N, D, V, K, dtype, want_hidden, want_weight).bwd_bytes;
 }
 
 extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, int D, int V,
                              int dtype, const int64_t* index, const float* teacher, int K,
-                             int64_t ignore_index, double temperature, float* loss, int32_t* rows,
-                             float* lse, int32_t* cols, float* corr, void* ws, size_t ws_bytes,
-                             void* stream) {
-  if (!valid_head(N, D, V, K, dtype) || !(temperature > 0.0) || !(temperature < 1e30))
-    return DPC_EINVAL;
+                             int64_t ignore_index, double temperature, int want_hidden,
+                             int want_weight, float* loss, void* state, size_t state_bytes,
+                             void* ws, size_t ws_bytes, void* stream) {
+  if (!valid_head(N, D, V, K, dtype) || !valid_temperature(temperature)) return DPC_EINVAL;
   if (!teacher && K != 1) return DPC_EINVAL;
   if (N == 0) return DPC_OK;
-  if (!hidden || !weight || !index || !loss || !rows || !lse || !cols || !corr || !ws) return DPC_EINVAL;
-  const Plan p = head_plan(N, D, V, K, dtype, false, false, false);
+  if (!hidden || !weight || !index || !loss || !ws) return DPC_EINVAL;
+  const Plan p = head_plan(N, D, V, K, dtype, want_hidden, want_weight);
   if (!p.pack && (misaligned(hidden) || misaligned(weight))) return DPC_EINVAL;
+  if (p.state_bytes && (!state || misaligned(state))) return DPC_EINVAL;
   if (misaligned(ws)) return DPC_EINVAL;
-  if (ws_bytes < (size_t)p.bytes) return DPC_ENOSPC;
+  if (ws_bytes < (size_t)p.fwd_bytes || state_bytes < (size_t)p.state_bytes) return DPC_ENOSPC;
   if ((int64_t)p.tiles_v * p.tiles_n > 0x7fffffffll) return DPC_EINVAL;
   hipStream_t s = (hipStream_t)stream;
   uint8_t* base = static_cast<uint8_t*>(ws);
-  const Rows r = rows_of(rows, N);
+  uint8_t* kept = static_cast<uint8_t*>(state);
+  const bool any = p.want_h || p.want_w, keep = any && !p.emit;
+  auto place = [&](bool in_state, int64_t so, int64_t fo) { return in_state ? kept + so : base + fo; };
+  const Rows rows = rows_at(place(any, p.s_rows, p.f_rows), N);
+  const Entries entries = {reinterpret_cast<int32_t*>(base + p.f_cols),
+                           reinterpret_cast<uint2*>(place(keep, p.s_list, p.f_list)),
+                           reinterpret_cast<int32_t*>(place(keep, p.s_start, p.f_start))};
+  float* lse = reinterpret_cast<float*>(place(keep, p.s_lse, p.f_lse));
+  float* corr = reinterpret_cast<float*>(place(keep, p.s_corr, p.f_corr));
   if (teacher) {
     hipLaunchKernelGGL(entries_kernel, dim3((unsigned)((N + 3) / 4)), dim3(256), 0, s, index,
-                       teacher, N, K, V, r.place);
+                       teacher, N, K, V, rows.place);
     DPC_HIP_CHECK(hipGetLastError());
   }
   hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, s, index, ignore_index,
-                     teacher != nullptr, N, r, loss);
+                     teacher != nullptr, N, rows, loss);
   DPC_HIP_CHECK(hipGetLastError());
   PrepArgs q = {};
-  q.hidden = hidden;
-  q.weight = weight;
-  q.dtype = dtype;
-  q.D = D;
-  q.V = V;
-  q.K = K;
-  q.N = N;
-  q.rows = r;
+  q.rows = rows;
   q.index = index;
   q.teacher = teacher != nullptr;
-  q.cols = cols;
+  q.blocks = p.tiles_n;
+  q.tiles = p.tiles_v;
+  q.entries = entries;
   StatsArgs a = {};
-  const int rc = operands(p, q, base, s, &a.h, &a.mm.a);
+  const int rc = operands(p, q, hidden, weight, base + p.f_h, base + p.f_w, s, &a.h, &a.mm.a);
   if (rc != DPC_OK) return rc;
+  const MmOperand w = a.mm.a;
   a.mm.b = MmOperand{nullptr, p.ld, N * p.ld, 0};
   a.mm.kl = (int)p.ld;
   a.mm.planes = p.planes;
   a.mm.tiles_a = p.tiles_v;
-  a.mm.tiles_b = p.tiles_n;
   a.mm.splits = 1;
   a.V = V;
   a.K = K;
   a.inv_tau = (float)(1.0 / temperature);
-  a.cols = cols;
-  a.picked = reinterpret_cast<float*>(base + p.picked);
-  a.part = reinterpret_cast<f32x2_t*>(base + p.part);
-  hipLaunchKernelGGL(head_stats_kernel, dim3((unsigned)p.tiles_v * (unsigned)p.tiles_n),
-                     dim3(kMmThreads), 0, s, a);
-  DPC_HIP_CHECK(hipGetLastError());
-  JoinArgs j = {r,         K,       p.tiles_v, a.inv_tau, (float)(temperature * temperature),
-                cols,      a.picked, teacher,   a.part,    loss,
-                lse,       corr};
-  hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)((N + 3) / 4)), dim3(256), 0, s, j);
-  DPC_HIP_CHECK(hipGetLastError());
+  a.entries = entries;
+  a.picked = reinterpret_cast<float*>(base + p.f_picked);
+  a.part = reinterpret_cast<f32x2_t*>(base + p.f_part);
+  JoinArgs j = {};
+  j.rows = rows;
+  j.K = K;
+  j.parts = p.tiles_v;
+  j.inv_tau = a.inv_tau;
+  j.loss_scale = (float)(temperature * temperature);
+  j.cols = entries.cols;
+  j.picked = a.picked;
+  j.teacher = teacher;
+  j.part = a.part;
+  j.loss = loss;
+  j.lse = lse;
+  j.corr = corr;
+  if (!p.emit) {
+    hipLaunchKernelGGL((head_stats_kernel<false>), dim3((unsigned)p.tiles_v * (unsigned)p.tiles_n),
+                       dim3(kMmThreads), 0, s, a);
+    DPC_HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)((N + 3) / 4)), dim3(256), 0, s, j);
+    DPC_HIP_CHECK(hipGetLastError());
+    return DPC_OK;
+  }
+  a.lde = (int64_t)p.tiles_v * kMmTile;
+  a.e = reinterpret_cast<_Float16*>(base + p.f_e);
+  j.e = reinterpret_cast<uint16_t*>(a.e);
+  j.lde = a.lde;
+  const int tiles_c = p.chunk / kMmTile;
+  float* unit = reinterpret_cast<float*>(kept + p.s_unit);
+  for (int64_t first = 0; first < N; first += p.chunk) {
+    a.h.first = j.first = (int)first;
+    a.h.most = j.most = p.chunk;
+    hipLaunchKernelGGL((head_stats_kernel<true>), dim3((unsigned)p.tiles_v * (unsigned)tiles_c),
+                       dim3(kMmThreads), 0, s, a);
+    DPC_HIP_CHECK(hipGetLastError());
+    hipLaunchKernelGGL(head_join_chunk_kernel, dim3((unsigned)p.chunk), dim3(256), 0, s, j);
+    DPC_HIP_CHECK(hipGetLastError());
+    ProductArgs m = {};
+    m.mm = MmArgs{w, MmOperand{j.e, a.lde, 0, 0}, V, 1, p.tiles_d, tiles_c, p.splits_c};
+    m.h = a.h;
+    m.rows_a = D;
+    m.lda = p.lda;
+    m.plane = p.chunk * p.lda;
+    m.partial = p.splits_c > 1 ? reinterpret_cast<float*>(base + p.f_pc) : nullptr;
+    m.out = unit + first * D;
+    hipLaunchKernelGGL((head_product_kernel<true>),
+                       dim3((unsigned)(p.tiles_d * tiles_c * p.splits_c)), dim3(kMmThreads), 0, s,
+                       m);
+    DPC_HIP_CHECK(hipGetLastError());
+    if (m.partial) {
+      ReduceArgs r = {};
+      r.partial = m.partial;
+      r.splits = p.splits_c;
+      r.plane = m.plane;
+      r.rows = p.chunk;
+      r.lda = p.lda;
+      r.count = rows.count;
+      r.first = (int)first;
+      r.D = D;
+      r.out = m.out;
+      const int rr = reduce(r, s);
+      if (rr != DPC_OK) return rr;
+    }
+  }
   return DPC_OK;
 }
 
 extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_t N, int D, int V,
-                                  int dtype, int32_t* rows, const int32_t* cols,
-                                  const float* corr, int K, const float* lse, const float* grad_loss, double temperature,
-                                  void* hidden_grad, void* weight_grad, void* ws, size_t ws_bytes,
-                                  void* stream) {
-  if (!valid_head(N, D, V, K, dtype) || !(temperature > 0.0) || !(temperature < 1e30))
-    return DPC_EINVAL;
+                                  int dtype, int K, double temperature, int want_hidden,
+                                  int want_weight, const void* state, size_t state_bytes,
+                                  const float* grad_loss, void* hidden_grad, void* weight_grad,
+                                  void* ws, size_t ws_bytes, void* stream) {
+  if (!valid_head(N, D, V, K, dtype) || !valid_temperature(temperature)) return DPC_EINVAL;
   if (N == 0) return DPC_OK;
   if (!hidden_grad && !weight_grad) return DPC_EINVAL;
-  if (!hidden || !weight || !rows || !cols || !corr || !lse || !grad_loss || !ws) return DPC_EINVAL;
-  const Plan p = head_plan(N, D, V, K, dtype, true, hidden_grad != nullptr, weight_grad != nullptr);
+  if ((hidden_grad && !want_hidden) || (weight_grad && !want_weight)) return DPC_EINVAL;
+  if (!hidden || !weight || !state || !grad_loss) return DPC_EINVAL;
+  const Plan p = head_plan(N, D, V, K, dtype, want_hidden, want_weight);
   if (!p.pack && (misaligned(hidden) || misaligned(weight))) return DPC_EINVAL;
-  if (misaligned(ws)) return DPC_EINVAL;
-  if (ws_bytes < (size_t)p.bytes) return DPC_ENOSPC;
-  if ((int64_t)p.piece_tiles * p.tiles_n > 0x7fffffffll) return DPC_EINVAL;
+  if (misaligned(hidden_grad) || misaligned(weight_grad) || misaligned(state)) return DPC_EINVAL;
+  if (p.bwd_bytes && (!ws || misaligned(ws))) return DPC_EINVAL;
+  if (ws_bytes < (size_t)p.bwd_bytes || state_bytes < (size_t)p.state_bytes) return DPC_ENOSPC;
   hipStream_t s = (hipStream_t)stream;
   uint8_t* base = static_cast<uint8_t*>(ws);
-  const Rows r = rows_of(rows, N);
+  uint8_t* kept = static_cast<uint8_t*>(const_cast<void*>(state));
+  const Rows rows = rows_at(kept + p.s_rows, N);
+  if (p.emit) {
+    const int64_t items = D % 8 == 0 ? N * D / 8 : N * D;
+    int64_t grid = (items + 255) / 256;
+    if (grid > 8192) grid = 8192;
+    hipLaunchKernelGGL(head_scale_kernel, dim3((unsigned)grid), dim3(256), 0, s,
+                       reinterpret_cast<const float*>(kept + p.s_unit), rows, grad_loss,
+                       (float)temperature, N, D, static_cast<uint16_t*>(hidden_grad));
+    DPC_HIP_CHECK(hipGetLastError());
+    return DPC_OK;
+  }
+  if ((int64_t)p.piece_tiles * p.tiles_n > 0x7fffffffll) return DPC_EINVAL;
   PrepArgs pa = {};
-  pa.hidden = hidden;
-  pa.weight = weight;
-  pa.dtype = dtype;
-  pa.D = D;
-  pa.V = V;
-  pa.K = K;
-  pa.N = N;
-  pa.rows = r;
+  pa.rows = rows;
   pa.zero = hidden_grad;
+  pa.g = grad_loss;
+  pa.gmax = reinterpret_cast<float*>(base + p.b_g);
   Hidden h;
   MmOperand w;
-  const int rc = operands(p, pa, base, s, &h, &w);
+  const int rc = operands(p, pa, hidden, weight, base + p.b_h, base + p.b_w, s, &h, &w);
   if (rc != DPC_OK) return rc;
   const MmOperand hop = {nullptr, p.ld, N * p.ld, 0};
   const int out_bf16 = dtype == DPC_BF16;
   const int64_t esz = out_bf16 ? 2 : 4;
   const int64_t ldz = (int64_t)p.piece_tiles * kMmTile;
-  uint16_t* dz = reinterpret_cast<uint16_t*>(base + p.dz);
+  uint16_t* dz = reinterpret_cast<uint16_t*>(base + p.b_dz);
   for (int i = 0; i < p.pieces; ++i) {
-    const int first = i * p.piece_tiles * kMmTile;
-    const int tiles = p.tiles_v - i * p.piece_tiles < p.piece_tiles
-                          ? p.tiles_v - i * p.piece_tiles
-                          : p.piece_tiles;
-    if (tiles <= 0) break;
+    const int tile0 = i * p.piece_tiles, first = tile0 * kMmTile;
+    const int tiles = p.tiles_v - tile0 < p.piece_tiles ? p.tiles_v - tile0 : p.piece_tiles;
     const int cols_here = V - first < tiles * kMmTile ? V - first : tiles * kMmTile;
     MmOperand wpiece = w;
     wpiece.p = w.p + (int64_t)first * w.ld;
@@ -835,16 +1223,18 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
     GradArgs a = {};
     a.mm = MmArgs{wpiece, hop, (int)p.ld, p.planes, tiles, p.tiles_n, 1};
     a.h = h;
-    a.active = r.active;
+    a.active = rows.active;
     a.V = V;
     a.K = K;
-    a.first = first;
+    a.tile0 = tile0;
+    a.tiles = p.tiles_v;
     a.inv_tau = (float)(1.0 / temperature);
-    a.coef = (float)temperature;
-    a.cols = cols;
-    a.corr = corr;
-    a.lse = lse;
+    a.entries = Entries{nullptr, reinterpret_cast<uint2*>(kept + p.s_list),
+                        reinterpret_cast<int32_t*>(kept + p.s_start)};
+    a.corr = reinterpret_cast<const float*>(kept + p.s_corr);
+    a.lse = reinterpret_cast<const float*>(kept + p.s_lse);
     a.g = grad_loss;
+    a.gmax = pa.gmax;
     a.dz = dz;
     a.ld = ldz;
     a.plane = N * ldz;
@@ -855,53 +1245,68 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
       hipLaunchKernelGGL((head_grad_kernel<3>), grid, dim3(kMmThreads), 0, s, a);
     DPC_HIP_CHECK(hipGetLastError());
     const MmOperand zop = {dz, ldz, N * ldz, 0};
+    ProductArgs q = {};
+    q.h = h;
+    q.rows_a = D;
+    q.lda = p.lda;
+    q.scale = pa.gmax;
+    q.coef = (float)temperature;
+    q.out_bf16 = out_bf16;
+    ReduceArgs r = {};
+    r.lda = p.lda;
+    r.scale = pa.gmax;
+    r.coef = q.coef;
+    r.D = D;
+    r.out_bf16 = out_bf16;
     if (hidden_grad) {
-      // A = W (D, K-slow: a row holds one vocabulary entry), B = dz (tokens).
-      // dz is zero past the vocabulary; W's rows there read as zeros.
-      ProductArgs q = {};
-      q.mm = MmArgs{wpiece, zop, cols_here, p.planes, p.tiles_d, p.tiles_n, p.splits_h};
-      q.h = h;
-      q.active = r.active;
-      q.rows_a = D;
-      q.lda = p.lda;
-      q.plane = N * p.lda;
+      // A = W (D, K-slow: a row holds one vocabulary entry), B = dz by rows.  dz is zero
+      // past the vocabulary, and W's rows there read as zeros.
+      ProductArgs m = q;
+      m.mm = MmArgs{wpiece, zop, cols_here, p.planes, p.tiles_d, p.tiles_n, p.splits_h};
+      m.active = rows.active;
+      m.plane = N * p.lda;
       const bool direct = p.pieces == 1 && p.splits_h == 1;
-      q.partial = direct ? nullptr : reinterpret_cast<float*>(base + p.ph);
-      q.accumulate = i > 0;
-      q.out = hidden_grad;
-      q.out_bf16 = out_bf16;
+      m.partial = direct ? nullptr : reinterpret_cast<float*>(base + p.b_ph);
+      m.accumulate = i > 0;
+      m.out = hidden_grad;
       hipLaunchKernelGGL((head_product_kernel<true>),
                          dim3((unsigned)(p.tiles_d * p.tiles_n * p.splits_h)), dim3(kMmThreads), 0,
-                         s, q);
+                         s, m);
       DPC_HIP_CHECK(hipGetLastError());
       if (!direct && i + 1 == p.pieces) {
-        hipLaunchKernelGGL(head_reduce_kernel, dim3(grid_for(N * p.lda / 4)), dim3(256), 0, s,
-                           q.partial, p.splits_h, q.plane, N, r.count, r.active, D, p.lda,
-                           hidden_grad, out_bf16);
-        DPC_HIP_CHECK(hipGetLastError());
+        r.partial = m.partial;
+        r.splits = p.splits_h;
+        r.plane = m.plane;
+        r.rows = N;
+        r.count = rows.count;
+        r.active = rows.active;
+        r.out = hidden_grad;
+        const int rr = reduce(r, s);
+        if (rr != DPC_OK) return rr;
       }
     }
     if (weight_grad) {
-      ProductArgs q = {};
-      q.mm = MmArgs{hop, zop, 0, p.planes, p.tiles_d, tiles, p.splits_w};
-      q.h = h;
-      q.rows_b = cols_here;
-      q.rows_a = D;
-      q.lda = p.lda;
-      q.plane = (int64_t)cols_here * p.lda;
-      q.partial = p.splits_w == 1 ? nullptr : reinterpret_cast<float*>(base + p.pw);
-      q.out = static_cast<uint8_t*>(weight_grad) + (int64_t)first * D * esz;
-      q.out_bf16 = out_bf16;
+      ProductArgs m = q;
+      m.mm = MmArgs{hop, zop, 0, p.planes, p.tiles_d, tiles, p.splits_w};
+      m.rows_b = cols_here;
+      m.plane = (int64_t)cols_here * p.lda;
+      m.partial = p.splits_w == 1 ? nullptr : reinterpret_cast<float*>(base + p.b_pw);
+      m.out = static_cast<uint8_t*>(weight_grad) + (int64_t)first * D * esz;
       hipLaunchKernelGGL((head_product_kernel<false>),
                          dim3((unsigned)(p.tiles_d * tiles * p.splits_w)), dim3(kMmThreads), 0, s,
-                         q);
+                         m);
       DPC_HIP_CHECK(hipGetLastError());
-      if (q.partial) {
-        hipLaunchKernelGGL(head_reduce_kernel, dim3(grid_for((int64_t)cols_here * p.lda / 4)),
-                           dim3(256), 0, s, q.partial, p.splits_w, q.plane, (int64_t)cols_here,
-                           (const int32_t*)nullptr, (const int32_t*)nullptr, D, p.lda, q.out,
-                           out_bf16);
-        DPC_HIP_CHECK(hipGetLastError());
+      if (m.partial) {
+        r.partial = m.partial;
+        r.splits = p.splits_w;
+        r.plane = m.plane;
+        r.rows = cols_here;
+        r.count = nullptr;
+        r.first = 0;
+        r.active = nullptr;
+        r.out = m.out;
+        const int rr = reduce(r, s);
+        if (rr != DPC_OK) return rr;
       }
     }
   }

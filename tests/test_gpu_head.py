@@ -5,7 +5,9 @@ Error model the tolerances come from (u = 2^-23, one extra addend of slack per
 most 1.125 n u times the sum of the terms' magnitudes.  So a logit is off by
 ``zerr = 1.125 n u |h| |w|``; a loss by twice that and a few ulp of the log sum
 exp; dz by its bf16 rounding (float32: three exact parts) and by what the logits'
-error does to p; and a gradient by dz's error and the sum's own, rounded once.
+error does to p; and a gradient by dz's error and the sum's own, rounded once.  With a
+frozen head (bf16) dz goes through fp16 exponentials relative to a tile's maximum:
+another 2^-12 of it, or 2^-25 where they are subnormal.
 """
 
 from __future__ import annotations
@@ -29,7 +31,7 @@ def _inputs(dev, lead, D, V, dtype, seed, spread=2.0):
     return g, h, W, up
 
 
-def _reference(h, W, q, ent, tau, up):
+def _reference(h, W, q, ent, tau, up, frozen=False):
     """Losses and gradients in 64 bits from the dense target distribution q [N, V]
     (rows of zeros: no target) and its negative entropy, with error bounds."""
     D = h.shape[-1]
@@ -50,6 +52,8 @@ def _reference(h, W, q, ent, tau, up):
     # p's relative error: the logits' and the exponential's (its argument's rounding).
     perr = (p * (sharp + 2.0**-22 * logp.abs()) + 2.0**-21 * q) * (tau * u)
     dzerr = dz.abs() * rnd + perr
+    if frozen and not f32:
+        dzerr = dzerr + (p * 2.0**-11 + 2.0**-25 * used) * (tau * u)
     out = 2.0**-23 if f32 else 2.0**-8
 
     def product(x, xerr, y, terms):
@@ -110,6 +114,21 @@ def test_cross_entropy(dev, lead, D, V, dtype):
     _close(dW, DW, "weight_grad")
     ignored = (t == -100)
     assert (loss[ignored] == 0).all() and (dh[ignored] == 0).all()
+    _frozen(lambda x, y: head.linear_cross_entropy(x, y, t), h, W, up, loss, q,
+            torch.zeros(q.shape[0], dtype=torch.float64, device=dev), 1.0, ignored)
+
+
+def _frozen(call, h, W, up, loss, q, ent, tau, empty):
+    """The same with a frozen head, whose gradient is made in the forward."""
+    frozen = call(h, W.detach())
+    (dh,) = torch.autograd.grad(frozen, [h], up, retain_graph=True)
+    assert torch.equal(frozen, loss)
+    _, DH, _ = _reference(h, W, q, ent, tau, up, frozen=True)
+    _close(dh, DH, "hidden_grad of a frozen head")
+    assert (dh[empty] == 0).all()
+    # A second backward of the same graph, with another gradient.
+    (again,) = torch.autograd.grad(frozen, [h], 2 * up)
+    assert torch.equal(again, 2 * dh)
 
 
 def _teacher(g, dev, lead, V, K, duplicates=False):
@@ -163,6 +182,8 @@ def test_distillation(dev, lead, D, V, K, tau, dup, dtype):
     _close(dW, DW, "weight_grad")
     empty = q.sum(1).view(lead) == 0
     assert (loss[empty] == 0).all() and (dh[empty] == 0).all()
+    _frozen(lambda x, y: head.topk_distillation(x, y, tl, ti, temperature=tau), h, W, up, loss, q,
+            ent, tau, empty)
 
 
 @pytest.mark.gpu
@@ -177,7 +198,8 @@ def test_distillation_from_one_entry_is_cross_entropy(dev):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 def test_many_pieces(dev, dtype):
-    """Enough tokens that the backward takes the vocabulary in several pieces."""
+    """Enough tokens that the backward takes the vocabulary in several pieces, and a frozen
+    head's forward the tokens in several chunks."""
     N, D, V = 300_001, 8, 600
     g, h, W, up = _inputs(dev, (N,), D, V, dtype, 11)
     t = torch.randint(0, V, (N,), generator=g, device=dev)
@@ -185,11 +207,13 @@ def test_many_pieces(dev, dtype):
     W.requires_grad_(True)
     loss = head.linear_cross_entropy(h, W, t)
     dh, dW = torch.autograd.grad(loss, [h, W], up)
-    L, DH, DW = _reference(h, W, _onehot(t, V, -100), torch.zeros(N, dtype=torch.float64,
-                                                                   device=dev), 1.0, up)
+    q, zero = _onehot(t, V, -100), torch.zeros(N, dtype=torch.float64, device=dev)
+    L, DH, DW = _reference(h, W, q, zero, 1.0, up)
     _close(loss, L, "loss")
     _close(dh, DH, "hidden_grad")
     _close(dW, DW, "weight_grad")
+    del DH, DW
+    _frozen(lambda x, y: head.linear_cross_entropy(x, y, t), h, W, up, loss, q, zero, 1.0, t == -100)
 
 
 @pytest.mark.gpu
@@ -221,8 +245,8 @@ def test_only_what_is_asked_for(dev):
     t = torch.randint(0, 300, (50,), generator=g, device=dev)
     h1, W1 = h.clone().requires_grad_(True), W.clone().requires_grad_(True)
     both = torch.autograd.grad(head.linear_cross_entropy(h1, W1, t), [h1, W1], up)
-    (dh,) = torch.autograd.grad(head.linear_cross_entropy(h1, W, t), [h1], up)
     (dW,) = torch.autograd.grad(head.linear_cross_entropy(h, W1, t), [W1], up)
+    (dh,) = torch.autograd.grad(head.linear_cross_entropy(h1, W1, t), [h1], up)
     assert torch.equal(dh, both[0]) and torch.equal(dW, both[1])
     assert not head.linear_cross_entropy(h, W, t).requires_grad
 
@@ -270,6 +294,9 @@ def test_nan_in_rows_without_a_target_reaches_nothing(dev):
     l2 = head.linear_cross_entropy(h2, W1, t)
     g2 = torch.autograd.grad(l2, [h2, W1], up2)
     assert torch.equal(l1, l2) and torch.equal(g1[0], g2[0]) and torch.equal(g1[1], g2[1])
+    f1 = torch.autograd.grad(head.linear_cross_entropy(h1, W, t), [h1], up)
+    f2 = torch.autograd.grad(head.linear_cross_entropy(h2, W, t), [h2], up2)
+    assert torch.equal(f1[0], f2[0])
 
 
 @pytest.mark.gpu
@@ -320,7 +347,9 @@ def test_repeats_streams_and_graph(dev):
 
     def step():
         loss = head.linear_cross_entropy(h, W, t)
-        return (loss.detach(), *torch.autograd.grad(loss, [h, W], up))
+        frozen = head.linear_cross_entropy(h, W.detach(), t)
+        return (loss.detach(), *torch.autograd.grad(loss, [h, W], up),
+                *torch.autograd.grad(frozen, [h], up))
 
     want = step()
     assert all(torch.equal(a, b) for a, b in zip(step(), want))
