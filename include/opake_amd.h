@@ -574,17 +574,17 @@ int dpc_head_loss_grad(const void* hidden, const void* weight, int64_t N, int D,
  * weights [N, k]: the scores, divided by their sum over the chosen if
  * `renormalize` (0 if that is 0), times scale.  A logit or key of -inf or NaN is
  * never chosen; slots with nothing left get expert -1 and weight 0; a NaN logit
- * makes its row's weights NaN.  scores [N, k] is written for the gradient.
+ * makes its row's weights NaN.
  *
- * dpc_route_topk_grad writes grad_logits [N, E] from grad_weights [N, k] in the
- * logits' dtype; the choice itself has no gradient. */
+ * dpc_route_topk_grad takes the two outputs and writes grad_logits [N, E] from
+ * grad_weights [N, k] in the logits' dtype; the choice itself has no gradient. */
 int dpc_route_topk(const void* logits, int64_t N, int E, int dtype, const float* bias, int k,
                    int score, int groups, int top_groups, int renormalize, double scale,
-                   float* weights, int64_t* experts, float* scores, void* stream);
+                   float* weights, int64_t* experts, void* stream);
 int dpc_route_topk_grad(const void* logits, int64_t N, int E, int dtype, int k, int score,
                         int renormalize, double scale, const int64_t* experts,
-                        const float* weights, const float* scores, const float* grad_weights,
-                        void* grad_logits, void* stream);
+                        const float* weights, const float* grad_weights, void* grad_logits,
+                        void* stream);
 
 /* Measurement helper with no counterpart in the reference (used by bench.py
  * to put the roofline in context): `grid` workgroups of 8 waves run `iters`

@@ -30,7 +30,6 @@ struct RouteArgs {
   float scale;
   float* weights;   // [N, k]
   int64_t* experts;  // [N, k]
-  float* scores;    // [N, k]
 };
 
 DPC_DEVICE float load_logit(const void* p, int64_t i, int dtype) {
@@ -202,18 +201,16 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
   if (in && lane < a.k) {
     a.weights[row * a.k + lane] = mine >= 0 ? w : (nan ? NAN : 0.0f);
     a.experts[row * a.k + lane] = mine;
-    a.scores[row * a.k + lane] = s;
   }
 }
 
 struct RouteGradArgs {
-  const void* logits;  // read for the softmax's own weights only
+  const void* logits;
   int64_t N;
   int E, dtype, k, sigmoid, renormalize;
   float scale;
   const int64_t* experts;
   const float* weights;
-  const float* scores;
   const float* g;  // [N, k]: gradient of the weights
   void* dz;
 };
@@ -231,8 +228,11 @@ __global__ void __launch_bounds__(256) route_grad_kernel(RouteGradArgs a) {
   const bool on = in && lane < a.k && a.experts[row * a.k + lane] >= 0;
   const int64_t at = row * a.k + lane;
   const int e = on ? (int)a.experts[at] : 0;
-  const float g = on ? a.g[at] * a.scale : 0.0f, s = on ? a.scores[at] : 0.0f;
+  const float g = on ? a.g[at] * a.scale : 0.0f;
+  // The weight without its scale; a sigmoid again from its logit.
   const float share = on && a.scale != 0.0f ? a.weights[at] / a.scale : 0.0f;
+  const float s =
+      !a.sigmoid ? share : (on ? sigmoid(load_logit(a.logits, row * a.E + e, a.dtype)) : 0.0f);
   float x = g;
   const float dot = row_sum<64>(g * (a.renormalize ? share : s));
   if (a.renormalize) {
@@ -286,15 +286,14 @@ int launch_route(const RouteArgs& a, hipStream_t s) {
 
 extern "C" int dpc_route_topk(const void* logits, int64_t N, int E, int dtype, const float* bias,
                               int k, int score, int groups, int top_groups, int renormalize,
-                              double scale, float* weights, int64_t* experts, float* scores,
-                              void* stream) {
+                              double scale, float* weights, int64_t* experts, void* stream) {
   if (!valid_route(N, E, k, dtype, score) || groups < 1 || E % groups || top_groups < 1 ||
       top_groups > groups || k > top_groups * (E / groups))
     return DPC_EINVAL;
   if (N == 0) return DPC_OK;
-  if (!logits || !weights || !experts || !scores) return DPC_EINVAL;
+  if (!logits || !weights || !experts) return DPC_EINVAL;
   const RouteArgs a = {logits, N, E, dtype, bias, k, score == DPC_ROUTE_SIGMOID, groups, top_groups,
-                       renormalize != 0, (float)scale, weights, experts, scores};
+                       renormalize != 0, (float)scale, weights, experts};
   hipStream_t s = (hipStream_t)stream;
   if (k <= 4 && E <= 8) return launch_route<4, 2>(a, s);
   if (k <= 16 && E <= 64) return launch_route<16, 4>(a, s);
@@ -305,14 +304,14 @@ extern "C" int dpc_route_topk(const void* logits, int64_t N, int E, int dtype, c
 
 extern "C" int dpc_route_topk_grad(const void* logits, int64_t N, int E, int dtype, int k, int score,
                                    int renormalize, double scale, const int64_t* experts,
-                                   const float* weights, const float* scores,
-                                   const float* grad_weights, void* grad_logits, void* stream) {
+                                   const float* weights, const float* grad_weights,
+                                   void* grad_logits, void* stream) {
   if (!valid_route(N, E, k, dtype, score)) return DPC_EINVAL;
   if (N == 0) return DPC_OK;
-  if (!logits || !experts || !weights || !scores || !grad_weights || !grad_logits)
+  if (!logits || !experts || !weights || !grad_weights || !grad_logits)
     return DPC_EINVAL;
   const RouteGradArgs a = {logits, N, E, dtype, k, score == DPC_ROUTE_SIGMOID, renormalize != 0,
-                           (float)scale, experts, weights, scores, grad_weights, grad_logits};
+                           (float)scale, experts, weights, grad_weights, grad_logits};
   hipLaunchKernelGGL(route_grad_kernel, dim3((unsigned)((N + 3) / 4)), dim3(256), 0,
                      (hipStream_t)stream, a);
   DPC_HIP_CHECK(hipGetLastError());

@@ -58,11 +58,11 @@ class _HeadLoss(torch.autograd.Function):
         dev = hidden.device
         lead, D = hidden.shape[:-1], hidden.shape[-1]
         V = weight.shape[0]
-        h, w = _aligned(hidden.detach()), _aligned(weight.detach())
+        h, w = _aligned(hidden), _aligned(weight)
         N, K = h.numel() // D, 1 if teacher is None else index.shape[-1]
         index = index.to(torch.int64).contiguous()
         if teacher is not None:
-            teacher = teacher.detach().to(torch.float32).contiguous()
+            teacher = teacher.to(torch.float32).contiguous()
         want_h, want_w = ctx.needs_input_grad[:2]
         lib, sizes = nat.load(), (N, D, V, K, code, int(want_h), int(want_w))
         loss = torch.empty(lead, dtype=torch.float32, device=dev)
@@ -70,11 +70,10 @@ class _HeadLoss(torch.autograd.Function):
         state = torch.empty(state_bytes, dtype=torch.uint8, device=dev)
         ws_bytes = lib.dpc_head_loss_workspace_bytes(*sizes)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            nat.call("dpc_head_loss", h.data_ptr(), w.data_ptr(), N, D, V, code, index.data_ptr(),
-                     nat.ptr(teacher), K, ignore_index, temperature, int(want_h), int(want_w),
-                     loss.data_ptr(), state.data_ptr(), state_bytes, ws.data_ptr(), ws_bytes,
-                     nat.stream_handle(dev))
+        nat.call_on(dev, "dpc_head_loss", h.data_ptr(), w.data_ptr(), N, D, V, code,
+                    index.data_ptr(), 0 if teacher is None else teacher.data_ptr(), K,
+                    ignore_index, temperature, int(want_h), int(want_w), loss.data_ptr(),
+                    state.data_ptr(), state_bytes, ws.data_ptr(), ws_bytes)
         if want_h or want_w:
             ctx.save_for_backward(hidden, weight, state)
             ctx.sizes, ctx.temperature = sizes, temperature
@@ -90,7 +89,7 @@ class _HeadLoss(torch.autograd.Function):
         if not want_h and not want_w:
             return (None,) * 7
         dev = hidden.device
-        h, w = _aligned(hidden.detach()), _aligned(weight.detach())
+        h, w = _aligned(hidden), _aligned(weight)
         g = grad.to(torch.float32).contiguous()
         dh = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if want_h else None
         dw = None
@@ -98,11 +97,10 @@ class _HeadLoss(torch.autograd.Function):
             dw = (torch.empty if N else torch.zeros)((V, D), dtype=weight.dtype, device=dev)
         ws_bytes = nat.load().dpc_head_loss_grad_workspace_bytes(*sizes)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            nat.call("dpc_head_loss_grad", h.data_ptr(), w.data_ptr(), N, D, V, code, K,
-                     ctx.temperature, forward_h, forward_w, state.data_ptr(), state.numel(),
-                     g.data_ptr(), nat.ptr(dh), nat.ptr(dw), ws.data_ptr(), ws_bytes,
-                     nat.stream_handle(dev))
+        nat.call_on(dev, "dpc_head_loss_grad", h.data_ptr(), w.data_ptr(), N, D, V, code, K,
+                    ctx.temperature, forward_h, forward_w, state.data_ptr(), state.numel(),
+                    g.data_ptr(), 0 if dh is None else dh.data_ptr(),
+                    0 if dw is None else dw.data_ptr(), ws.data_ptr(), ws_bytes)
         return dh, dw, None, None, None, None, None
 
 

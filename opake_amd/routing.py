@@ -23,42 +23,37 @@ _SCORES = {"softmax": nat.ROUTE_SOFTMAX, "sigmoid": nat.ROUTE_SIGMOID}
 
 class _Route(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, bias, k, score, groups, top_groups, renormalize, scale):
-        dev = nat.require_device(logits, bias)
-        code = nat.dtype_code(logits.dtype, wide=True)
-        lead, E = logits.shape[:-1], logits.shape[-1]
-        z = logits.detach().contiguous()
-        N = z.numel() // E
+    def forward(ctx, logits, bias, code, k, score, groups, top_groups, renormalize, scale):
+        dev = logits.device
+        z = logits.contiguous()
+        lead, E = z.shape[:-1], z.shape[-1]
         weights = torch.empty((*lead, k), dtype=torch.float32, device=dev)
         experts = torch.empty((*lead, k), dtype=torch.int64, device=dev)
-        scores = torch.empty((N, k), dtype=torch.float32, device=dev)
-        with torch.cuda.device(dev):
-            nat.call("dpc_route_topk", nat.ptr(z), N, E, code, nat.ptr(bias), k, score, groups,
-                     top_groups, int(renormalize), scale, nat.ptr(weights), nat.ptr(experts),
-                     nat.ptr(scores), nat.stream_handle(dev))
-        ctx.save_for_backward(logits, weights, experts, scores)
+        nat.call_on(dev, "dpc_route_topk", z.data_ptr(), z.numel() // E, E, code,
+                    0 if bias is None else bias.data_ptr(), k, score, groups, top_groups,
+                    renormalize, scale, weights.data_ptr(), experts.data_ptr())
         ctx.mark_non_differentiable(experts)
-        ctx.set_materialize_grads(False)
-        ctx.options = (k, score, int(renormalize), scale)
+        if ctx.needs_input_grad[0]:
+            ctx.set_materialize_grads(False)
+            ctx.save_for_backward(logits, weights, experts)
+            ctx.options = (code, k, score, renormalize, scale)
         return weights, experts
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _):
         if grad is None:
-            return (None,) * 8
-        logits, weights, experts, scores = ctx.saved_tensors
-        k, score, renormalize, scale = ctx.options
-        dev, E = logits.device, logits.shape[-1]
-        z = logits.detach().contiguous()
+            return (None,) * 9
+        logits, weights, experts = ctx.saved_tensors
+        z = logits.contiguous()
+        E = z.shape[-1]
         g = grad.to(torch.float32).contiguous()
-        dz = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        with torch.cuda.device(dev):
-            nat.call("dpc_route_topk_grad", nat.ptr(z), z.numel() // E, E,
-                     nat.dtype_code(logits.dtype, wide=True), k, score, renormalize, scale,
-                     nat.ptr(experts), nat.ptr(weights), nat.ptr(scores), nat.ptr(g), nat.ptr(dz),
-                     nat.stream_handle(dev))
-        return dz, None, None, None, None, None, None, None
+        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        code, k, score, renormalize, scale = ctx.options
+        nat.call_on(z.device, "dpc_route_topk_grad", z.data_ptr(), z.numel() // E, E, code, k,
+                    score, renormalize, scale, experts.data_ptr(), weights.data_ptr(),
+                    g.data_ptr(), dz.data_ptr())
+        return dz, None, None, None, None, None, None, None, None
 
 
 def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax",
@@ -108,8 +103,8 @@ def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax",
             raise ConfigurationError(f"bias must be float32 [{E}], got {bias.dtype} "
                                      f"{tuple(bias.shape)}")
         bias = bias.detach().contiguous()
-    return _Route.apply(logits, bias, k, _SCORES[score], groups, top_groups, bool(renormalize),
-                        float(scale))
+    return _Route.apply(logits, bias, nat.dtype_code(logits.dtype, wide=True), k, _SCORES[score],
+                        groups, top_groups, int(bool(renormalize)), float(scale))
 
 
 __all__ = ["MAX_EXPERTS", "MAX_TOP_K", "route_topk"]
