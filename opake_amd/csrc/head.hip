@@ -208,20 +208,44 @@ DPC_DEVICE void pack_chunk(const void* src, int dtype, int64_t row, int D, int c
 constexpr int kPrepThreads = 512;
 constexpr int kMaxTiles = 1 << 13;  // of the vocabulary (lists' counters in LDS)
 
+// i / K for i < 2^24 (exact in float; the quotient is off by one at most).
+DPC_DEVICE int row_of(int i, int K, float inv) {
+  int r = (int)((float)i * inv);
+  r -= r * K > i;
+  r += (r + 1) * K <= i;
+  return r;
+}
+
 DPC_DEVICE void list_entries(const PrepArgs& a, int block, int64_t count, int* counter) {
+  constexpr int kBatch = 8;  // loads in flight a thread
   const int tid = threadIdx.x;
   const int64_t first = (int64_t)block * kMmTile;
   if (first >= count) return;
   const int rows = (int)(count - first < kMmTile ? count - first : kMmTile);
   const int n = rows * a.K;
+  const float inv = 1.0f / (float)a.K;
+  const int32_t* active = a.rows.active + first;
+  int32_t* cols = a.entries.cols + first * a.K;
   for (int t = tid; t <= a.tiles; t += kPrepThreads) counter[t] = 0;
   __syncthreads();
-  for (int i = tid; i < n; i += kPrepThreads) {
-    const int r = i / a.K;
-    const int64_t t = a.index[(int64_t)a.rows.active[first + r] * a.K + (i - r * a.K)];
-    const int c = a.teacher && t < 0 ? -1 : (t >= 0 && t < a.V ? (int)t : -2);
-    a.entries.cols[first * a.K + i] = c;
-    if (c >= 0) atomicAdd(&counter[(c >> 8) + 1], 1);
+  for (int i0 = tid; i0 < n; i0 += kBatch * kPrepThreads) {
+    int64_t from[kBatch], x[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int i = i0 + b * kPrepThreads;
+      const int r = i < n ? row_of(i, a.K, inv) : 0;
+      from[b] = i < n ? (int64_t)active[r] * a.K + (i - r * a.K) : 0;
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) x[b] = a.index[from[b]];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int i = i0 + b * kPrepThreads;
+      if (i >= n) break;
+      const int c = a.teacher && x[b] < 0 ? -1 : (x[b] >= 0 && x[b] < a.V ? (int)x[b] : -2);
+      cols[i] = c;
+      if (c >= 0) atomicAdd(&counter[(c >> 8) + 1], 1);
+    }
   }
   __syncthreads();
   if (tid < 64) {  // counts -> starts, 64 tiles at a time
@@ -246,11 +270,20 @@ DPC_DEVICE void list_entries(const PrepArgs& a, int block, int64_t count, int* c
   // The order within a tile's entries is that of the atomics: each entry has a place
   // of its own in every output, so no result depends on it.
   uint2* list = a.entries.list + first * a.K;
-  for (int i = tid; i < n; i += kPrepThreads) {
-    const int c = a.entries.cols[first * a.K + i];
-    if (c < 0) continue;
-    const int at = atomicAdd(&counter[c >> 8], 1);
-    list[at] = make_uint2((uint32_t)i, (uint32_t)((i / a.K) << 8 | (c & 255)));
+  for (int i0 = tid; i0 < n; i0 += kBatch * kPrepThreads) {
+    int c[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int i = i0 + b * kPrepThreads;
+      c[b] = i < n ? cols[i] : -1;
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int i = i0 + b * kPrepThreads;
+      if (c[b] < 0) continue;
+      const int at = atomicAdd(&counter[c[b] >> 8], 1);
+      list[at] = make_uint2((uint32_t)i, (uint32_t)(row_of(i, a.K, inv) << 8 | (c[b] & 255)));
+    }
   }
 }
 
@@ -359,7 +392,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
   s.mm.b.rows = N;
   s.mm.tiles_b = tiles_of(N);
   if (!mm_tile_of(s.mm, &split, &ta, &tb)) return;
-  MmAcc acc;
+  MmAcc<false> acc;
   mm_loop<true, true>(s.mm, ta, tb, 0, lds_all, acc);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6),
             wm = w & 1, wn = w >> 1;
@@ -412,6 +445,15 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
     }
     __syncthreads();
   }
+  if (v0 + kMmTile > s.V) {  // past the vocabulary
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * i + r >= vleft) acc.v[i][j][r] = -INFINITY;
+  }
   // Maxima, then exponentials against the tile's (both halves of the vocabulary).
   float* tops = reinterpret_cast<float*>(lds_all);  // [2][256]
   float* sums = tops + 512;                         // [2][256]
@@ -421,10 +463,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (16 * i + r >= vleft) acc.v[i][j][r] = -INFINITY;
-        m = fmaxf(m, acc.v[i][j][r]);
-      }
+      for (int r = 0; r < 4; ++r) m = fmaxf(m, acc.v[i][j][r]);
     m = fmaxf(m, __shfl_xor(m, 16));
     m = fmaxf(m, __shfl_xor(m, 32));
     if (lane < 16) tops[wm * 256 + tl + 16 * j] = m;
@@ -674,7 +713,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
   s.mm.b.rows = N;
   s.mm.tiles_b = tiles_of(N);
   if (!mm_tile_of(s.mm, &split, &ta, &tb)) return;
-  MmAcc acc;
+  MmAcc<false> acc;
   mm_loop<true, true>(s.mm, ta, tb, 0, lds_all, acc);
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w & 1, wn = w >> 1;
   const int vt = s.tile0 + ta, n0 = tb * kMmTile;
@@ -787,20 +826,20 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_product_kernel(ProductArgs
     s.mm.kl = count;
   }
   if (!mm_tile_of(s.mm, &split, &ta, &tb)) return;
-  MmAcc acc;
+  MmAcc<kHidden> acc;
   mm_loop<false, kHidden>(s.mm, ta, tb, split, lds_all, acc);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w & 1, wn = w >> 1;
-  const int a0 = ta * kMmTile + wm * 128 + 4 * (lane >> 4);
-  const int b0 = tb * kMmTile + wn * 64 + (lane & 15);
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int a0 = ta * kMmTile + acc.row0(w) + 4 * (lane >> 4);
+  const int b0 = tb * kMmTile + acc.col0(w) + (lane & 15);
   const bool whole = s.rows_a % 4 == 0;
   const float f = s.scale ? *s.scale * s.coef : 1.f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < MmAcc<kHidden>::kB; ++j) {
     const int b = b0 + 16 * j;
     if (b >= rows_b) continue;
     const int64_t row = kHidden && s.active && !s.partial ? s.active[b] : b;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < MmAcc<kHidden>::kA; ++i) {
       const int a = a0 + 16 * i;
       if (a >= s.rows_a) continue;
       f32x4_t x = acc.v[i][j];

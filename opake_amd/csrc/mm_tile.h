@@ -71,10 +71,16 @@ DPC_DEVICE bool mm_tile_of(const MmArgs& g, int* split, int* ta, int* tb) {
   return true;
 }
 
-// The wave's 128 x 64 accumulators: rows (wave & 1) * 128 of A, columns
-// (wave >> 1) * 64 of B.
+// A wave's accumulators: 128 x 64 of the tile (rows (wave & 1) * 128 of A, columns
+// (wave >> 1) * 64 of B), or with kWideB 64 x 128 ((wave & 3) * 64, (wave >> 2) * 128).
+// The narrow side's fragments are read half as often: it suits the operand whose
+// reads cost more (K-slow ones: 109 against 250 bytes a clock).
+template <bool kWideB>
 struct MmAcc {
-  f32x4_t v[8][4];
+  static constexpr int kA = kWideB ? 4 : 8, kB = kWideB ? 8 : 4;
+  f32x4_t v[kA][kB];
+  static DPC_DEVICE int row0(int w) { return kWideB ? (w & 3) * 64 : (w & 1) * 128; }
+  static DPC_DEVICE int col0(int w) { return kWideB ? (w >> 2) * 128 : (w >> 1) * 64; }
 };
 
 template <bool kKc>
@@ -170,22 +176,22 @@ struct MmPlace {
 // operand (A, A, B, B: every read is a lane's offset plus a 16-bit immediate), all
 // transfers straight from memory into LDS.
 //
-// A step is two 32-deep sub-steps of two phases of 16 MFMAs: the wave's upper and
-// lower four A blocks against its four B blocks.  Fragments are read one phase
+// A step is two 32-deep sub-steps of two phases of 16 MFMAs: the first and the last
+// four blocks of the wide operand against the other's four.  Fragments are read one phase
 // ahead.  Before phase 3 a barrier: the other stage has arrived, and this one has
 // been read for the last time.  A's transfers of step s + 2 go out right after it,
 // B's of step s + 1 at the start of step s, so each has most of a step or more to
 // land and the barrier is the only place where a wave waits.
 // Ends with a barrier, after which `lds` is free.
-template <bool kAKc, bool kBKc>
-DPC_DEVICE void mm_loop(const MmArgs& g, int ta, int tb, int split, uint8_t* lds, MmAcc& acc) {
+template <bool kAKc, bool kBKc, bool kWideB>
+DPC_DEVICE void mm_loop(const MmArgs& g, int ta, int tb, int split, uint8_t* lds,
+                        MmAcc<kWideB>& acc) {
   const int tid = threadIdx.x, lane = tid & 63,
             w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = w & 1, wn = w >> 1;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < MmAcc<kWideB>::kA; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc.v[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < MmAcc<kWideB>::kB; ++j) acc.v[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const int ks = max(1, (g.kl + kMmStep - 1) / kMmStep);
   const long long n = mm_steps(g);
   const int s0 = (int)(n * split / g.splits), s1 = (int)(n * (split + 1) / g.splits);
@@ -214,54 +220,65 @@ DPC_DEVICE void mm_loop(const MmArgs& g, int ta, int tb, int split, uint8_t* lds
   auto fetch_b = [&](int stage, int j) __attribute__((always_inline)) {
     sb.issue(buf, bad, lds_addr(lds) + (2 + stage) * kMmOperandBytes, w, j);
   };
-  bf16x8_t fa0[4], fa1[4], fb0[4], fb1[4];
-  MmFrags<kAKc, kMixed, 8> ra;
-  MmFrags<kBKc, kMixed, 4> rb;
-  ra.init(0, wm * 128, lane);
-  rb.init(2 * kMmOperandBytes, wn * 64, lane);
-  // One phase: 16 MFMAs in the order of `a`, `b`, and after MFMA m what slot(m) issues
-  // (a fragment of the next phase, a transfer); the order is the one written.
-  auto phase = [&](const bf16x8_t* a, const bf16x8_t* b, int ih, auto slot)
+  // x: the wide operand's fragments (half of its blocks), y: the narrow one's.
+  bf16x8_t x0[4], x1[4], y0[4], y1[4];
+  MmFrags<kAKc, kMixed, MmAcc<kWideB>::kA> ra;
+  MmFrags<kBKc, kMixed, MmAcc<kWideB>::kB> rb;
+  ra.init(0, acc.row0(w), lane);
+  rb.init(2 * kMmOperandBytes, acc.col0(w), lane);
+  auto read_x = [&](int stage, int kk, int half, bf16x8_t* f, int i) __attribute__((always_inline)) {
+    if constexpr (kWideB)
+      f[i] = rb.read(lds, 4 * half + i, kk, stage * kMmOperandBytes);
+    else
+      f[i] = ra.read(lds, 4 * half + i, kk, stage * kMmOperandBytes);
+  };
+  auto read_y = [&](int stage, int kk, bf16x8_t* f, int i) __attribute__((always_inline)) {
+    if constexpr (kWideB)
+      f[i] = ra.read(lds, i, kk, stage * kMmOperandBytes);
+    else
+      f[i] = rb.read(lds, i, kk, stage * kMmOperandBytes);
+  };
+  // One phase: 16 MFMAs, and after MFMA m what slot(m) issues (a fragment of the next
+  // phase, a transfer); the order is the one written.
+  auto phase = [&](const bf16x8_t* x, const bf16x8_t* y, int half, auto slot)
       __attribute__((always_inline)) {
 #pragma unroll
     for (int m = 0; m < 16; ++m) {
       const int i = m >> 2, j = m & 3;
-      acc.v[4 * ih + i][j] =
-          __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[j], acc.v[4 * ih + i][j], 0, 0, 0);
+      if constexpr (kWideB)
+        acc.v[j][4 * half + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            y[j], x[i], acc.v[j][4 * half + i], 0, 0, 0);
+      else
+        acc.v[4 * half + i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            x[i], y[j], acc.v[4 * half + i][j], 0, 0, 0);
       slot(m);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto read_a = [&](int stage, int kk, int ih, bf16x8_t* f, int i) __attribute__((always_inline)) {
-    f[i] = ra.read(lds, 4 * ih + i, kk, stage * kMmOperandBytes);
-  };
-  auto read_b = [&](int stage, int kk, bf16x8_t* f, int j) __attribute__((always_inline)) {
-    f[j] = rb.read(lds, j, kk, stage * kMmOperandBytes);
-  };
   auto step = [&](int cur, int nxt) __attribute__((always_inline)) {
     next_b();
     __builtin_amdgcn_sched_barrier(0);
-    phase(fa0, fb0, 0, [&](int m) __attribute__((always_inline)) {
-      if (m % 2 == 0 && m < 8) read_a(cur, 0, 1, fa1, m / 2);
+    phase(x0, y0, 0, [&](int m) __attribute__((always_inline)) {
+      if (m % 2 == 0 && m < 8) read_x(cur, 0, 1, x1, m / 2);
       if (m % 4 == 3) fetch_b(nxt, m / 4);
     });
-    phase(fa1, fb0, 1, [&](int m) __attribute__((always_inline)) {
+    phase(x1, y0, 1, [&](int m) __attribute__((always_inline)) {
       if (m < 8) {
-        if (m & 1) read_a(cur, 1, 0, fa0, m / 2);
-        else read_b(cur, 1, fb1, m / 2);
+        if (m & 1) read_x(cur, 1, 0, x0, m / 2);
+        else read_y(cur, 1, y1, m / 2);
       }
     });
-    phase(fa0, fb1, 0, [&](int m) __attribute__((always_inline)) {
-      if (m % 2 == 0 && m < 8) read_a(cur, 1, 1, fa1, m / 2);
+    phase(x0, y1, 0, [&](int m) __attribute__((always_inline)) {
+      if (m % 2 == 0 && m < 8) read_x(cur, 1, 1, x1, m / 2);
     });
     next_a();
     DPC_WAIT_VMCNT(0);
     __syncthreads();
     __builtin_amdgcn_sched_barrier(0);
-    phase(fa1, fb1, 1, [&](int m) __attribute__((always_inline)) {
+    phase(x1, y1, 1, [&](int m) __attribute__((always_inline)) {
       if (m < 8) {
-        if (m & 1) read_a(nxt, 0, 0, fa0, m / 2);
-        else read_b(nxt, 0, fb0, m / 2);
+        if (m & 1) read_x(nxt, 0, 0, x0, m / 2);
+        else read_y(nxt, 0, y0, m / 2);
       }
       if (m % 4 == 3) fetch_a(cur, m / 4);
     });
@@ -279,8 +296,8 @@ DPC_DEVICE void mm_loop(const MmArgs& g, int ta, int tb, int split, uint8_t* lds
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    read_b(0, 0, fb0, j);
-    read_a(0, 0, 0, fa0, j);
+    read_y(0, 0, y0, j);
+    read_x(0, 0, 0, x0, j);
   }
   int s = 0;
   for (; s + 1 < steps; s += 2) {
