@@ -366,8 +366,8 @@ struct StatsArgs {
   Entries entries;
   float* picked;   // [rows, K]: z at the entries' columns
   f32x2_t* part;   // [rows, tiles_a]: maximum and sum of exponentials of each tile
-  _Float16* e;     // [chunk's rows, lde]: exp(z - the tile's maximum)
-  int64_t lde;
+  uint16_t* e;     // the chunk's exp(z - the tile's maximum) as fp16, in blocks
+  int64_t lde;     // blocks of a row of them
 };
 
 // Byte of (row of the tile, column) in a 256 x 256 tile of 2-byte values in LDS:
@@ -376,12 +376,13 @@ DPC_DEVICE int tile16_off(int row, int col) {
   return row * 512 + (((col >> 3) ^ (row & 15)) << 4) + (col & 7) * 2;
 }
 
-// The staged tile to dst [rows, ld] (16 bytes a lane).
-DPC_DEVICE void store_tile16(uint16_t* dst, int64_t ld, int rows) {
-  for (int i = threadIdx.x; i < rows * 32; i += kMmThreads) {
-    const int t = i >> 5, c = i & 31;
-    *reinterpret_cast<u32x4_t*>(dst + t * ld + 8 * c) =
-        *reinterpret_cast<const u32x4_t*>(lds_all + tile16_off(t, 8 * c));
+// The staged tile to its four blocks (128 KiB in a row).
+DPC_DEVICE void store_tile16(uint16_t* dst) {
+#pragma unroll 4
+  for (int i = threadIdx.x; i < 4 * kMmTile * 8; i += kMmThreads) {
+    const int row = (i >> 3) & 255, col = (i >> 11) * kMmStep + (i & 7) * 8;
+    *reinterpret_cast<u32x4_t*>(dst + 8 * i) =
+        *reinterpret_cast<const u32x4_t*>(lds_all + tile16_off(row, col));
   }
 }
 
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
   s.mm.tiles_b = tiles_of(N);
   if (!mm_tile_of(s.mm, &split, &ta, &tb)) return;
   MmAcc<false> acc;
-  mm_loop<true, true>(s.mm, ta, tb, 0, lds_all, acc);
+  mm_loop<true, true, false>(s.mm, ta, tb, 0, lds_all, acc);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6),
             wm = w & 1, wn = w >> 1;
   const int v0 = ta * kMmTile, n0 = tb * kMmTile;
@@ -503,8 +504,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
         *reinterpret_cast<half4_t*>(lds_all + tile16_off(tl + 16 * j, vl + 16 * i)) = h;
       }
     __syncthreads();
-    store_tile16(reinterpret_cast<uint16_t*>(s.e) + (int64_t)n0 * s.lde + v0, s.lde,
-                 min(N - n0, kMmTile));
+    store_tile16(s.e + (tb * s.lde + 4 * ta) * kMmBlock);
   }
 }
 
@@ -620,37 +620,45 @@ __global__ void __launch_bounds__(256) head_join_kernel(JoinArgs a) {
   if (n < *a.rows.count) join_row(a, n, threadIdx.x & 63);
 }
 
-// One workgroup a row of a chunk: the join, then the row's exp(z - tile's maximum)
-// times exp(tile's maximum - lse), and at the entries' columns p - q.
+// Eight rows of a chunk a workgroup: the joins, then the rows' exp(z - tile's
+// maximum) times exp(tile's maximum - lse), and at the entries' columns p - q.  The
+// eight rows are 1 KiB of every block; a wave takes one block of each tile.
+constexpr int kJoinRows = 8;
+
 __global__ void __launch_bounds__(256) head_join_chunk_kernel(JoinArgs a) {
-  __shared__ float shared_lse;
-  const int tid = threadIdx.x;
-  const int64_t n = a.first + (int64_t)blockIdx.x;
-  if ((int)blockIdx.x >= a.most || n >= *a.rows.count) return;
-  if (tid < 64) {
-    const float lse = join_row(a, n, tid);
-    if (tid == 0) shared_lse = lse;
+  __shared__ float lses[kJoinRows];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int local = blockIdx.x * kJoinRows;  // first row in the chunk
+  const int64_t n0 = a.first + local, count = *a.rows.count;
+  if (local >= a.most || n0 >= count) return;
+  const int rows = (int)(count - n0 < kJoinRows ? count - n0 : kJoinRows);
+  for (int r = w; r < kJoinRows; r += 4) {
+    const float lse = r < rows ? join_row(a, n0 + r, lane) : 0.f;
+    if (lane == 0) lses[r] = lse;
   }
   __syncthreads();
-  const float lse = shared_lse;
   typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-  uint16_t* row = a.e + (int64_t)blockIdx.x * a.lde;
-  const f32x2_t* part = a.part + n * a.parts;
-  const int chunks = (int)(a.lde / 8);
+  uint16_t* tile = a.e + (local >> 8) * a.lde * kMmBlock + (local & 255) * kMmStep;
+  const int r = lane >> 3;
+  const float lse = lses[r];
+  const f32x2_t* part = a.part + (n0 + min(r, rows - 1)) * a.parts;
 #pragma unroll 4
-  for (int i = tid; i < chunks; i += 256) {
-    const half8_t h = *reinterpret_cast<const half8_t*>(row + 8 * i);
-    const float f = fast_exp(part[i >> 5].x - lse);
+  for (int t = 0; t < a.parts; ++t) {
+    uint16_t* at = tile + (4 * t + w) * kMmBlock + lane * 8;
+    const half8_t h = *reinterpret_cast<const half8_t*>(at);
+    const float f = fast_exp(part[t].x - lse);
     u32x4_t o;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
       o[e] = f32x2_to_bf16x2_bits((float)h[2 * e] * f, (float)h[2 * e + 1] * f);
-    *reinterpret_cast<u32x4_t*>(row + 8 * i) = o;
+    *reinterpret_cast<u32x4_t*>(at) = o;
   }
   __syncthreads();
-  for (int k = tid; k < a.K; k += 256) {
-    const int c = a.cols[n * a.K + k];
-    if (c >= 0) row[c] = f32_to_bf16_bits(a.corr[n * a.K + k]);
+  for (int i = tid; i < rows * a.K; i += 256) {
+    const int c = a.cols[n0 * a.K + i];
+    if (c >= 0)
+      tile[(c >> 6) * kMmBlock + (i / a.K) * kMmStep + (c & 63)] =
+          f32_to_bf16_bits(a.corr[n0 * a.K + i]);
   }
 }
 
@@ -702,8 +710,8 @@ struct GradArgs {
   const float* g;     // [N]: the losses' gradient, at the rows' own places
   const float* gmax;  // dz is held over gmax, so a gradient that is the same for all
                       // rows (one over the tokens) is not rounded with every value
-  uint16_t* dz;       // [planes][rows][ld]
-  int64_t ld, plane;
+  uint16_t* dz;       // [planes], in blocks
+  int64_t ld, plane;  // blocks of a row of them, elements
 };
 
 template <int kPlanes>
@@ -714,7 +722,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
   s.mm.tiles_b = tiles_of(N);
   if (!mm_tile_of(s.mm, &split, &ta, &tb)) return;
   MmAcc<false> acc;
-  mm_loop<true, true>(s.mm, ta, tb, 0, lds_all, acc);
+  mm_loop<true, true, false>(s.mm, ta, tb, 0, lds_all, acc);
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w & 1, wn = w >> 1;
   const int vt = s.tile0 + ta, n0 = tb * kMmTile;
   const int vl = wm * 128 + 4 * (lane >> 4);
@@ -735,7 +743,6 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
         acc.v[i][j][r] = 16 * i + r < vleft ? e : 0.f;
       }
   }
-  const int rows = min(N - n0, kMmTile);
   const int32_t* start = s.entries.start + (int64_t)tb * (s.tiles + 1) + vt;
   const uint2* list = s.entries.list + (int64_t)n0 * s.K;
   const int e0 = start[0], e1 = start[1];
@@ -767,7 +774,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
           kPlanes == 1 ? f32_to_bf16_bits(x) : split_plane(x, pl);
     }
     __syncthreads();
-    store_tile16(s.dz + pl * s.plane + (int64_t)n0 * s.ld + ta * kMmTile, s.ld, rows);
+    store_tile16(s.dz + pl * s.plane + (tb * s.ld + 4 * ta) * kMmBlock);
   }
 }
 
@@ -827,7 +834,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_product_kernel(ProductArgs
   }
   if (!mm_tile_of(s.mm, &split, &ta, &tb)) return;
   MmAcc<kHidden> acc;
-  mm_loop<false, kHidden>(s.mm, ta, tb, split, lds_all, acc);
+  mm_loop<false, kHidden, true>(s.mm, ta, tb, split, lds_all, acc);
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int a0 = ta * kMmTile + acc.row0(w) + 4 * (lane >> 4);
   const int b0 = tb * kMmTile + acc.col0(w) + (lane & 15);
@@ -896,7 +903,7 @@ __global__ void __launch_bounds__(256) head_reduce_kernel(ReduceArgs a) {
 // ---------------------------------------------------------------------------
 
 // Held at once: dz of a piece of the vocabulary, or a chunk's exponentials.
-constexpr int64_t kPieceBytes = 256ll << 20;
+constexpr int64_t kPieceBytes = 512ll << 20;
 
 int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
@@ -1001,13 +1008,14 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
     p.b_h = take(p.planes * N * p.ld * 2);
     if (p.pack) p.b_w = take(p.planes * (int64_t)V * p.ld * 2);
     p.b_g = take(4);
-    int64_t t = kPieceBytes / (p.planes * N * kMmTile * 2);
+    const int64_t rows = (int64_t)p.tiles_n * kMmTile;
+    int64_t t = kPieceBytes / (p.planes * rows * kMmTile * 2);
     if (t < 1) t = 1;
     if (t > p.tiles_v) t = p.tiles_v;
     p.pieces = (int)((p.tiles_v + t - 1) / t);
     p.piece_tiles = (p.tiles_v + p.pieces - 1) / p.pieces;
     p.pieces = (p.tiles_v + p.piece_tiles - 1) / p.piece_tiles;
-    p.b_dz = take(p.planes * N * p.piece_tiles * kMmTile * 2);
+    p.b_dz = take(p.planes * rows * p.piece_tiles * kMmTile * 2);
     if (p.want_h) {
       p.splits_h = slices((int64_t)p.tiles_d * p.tiles_n, (int64_t)pairs * p.piece_tiles * 4);
       if (p.pieces > 1 || p.splits_h > 1) p.b_ph = take(p.splits_h * N * p.lda * 4);
@@ -1164,9 +1172,9 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
     DPC_HIP_CHECK(hipGetLastError());
     return DPC_OK;
   }
-  a.lde = (int64_t)p.tiles_v * kMmTile;
-  a.e = reinterpret_cast<_Float16*>(base + p.f_e);
-  j.e = reinterpret_cast<uint16_t*>(a.e);
+  a.lde = (int64_t)p.tiles_v * 4;
+  a.e = reinterpret_cast<uint16_t*>(base + p.f_e);
+  j.e = a.e;
   j.lde = a.lde;
   const int tiles_c = p.chunk / kMmTile;
   float* unit = reinterpret_cast<float*>(kept + p.s_unit);
@@ -1176,7 +1184,8 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
     hipLaunchKernelGGL((head_stats_kernel<true>), dim3((unsigned)p.tiles_v * (unsigned)tiles_c),
                        dim3(kMmThreads), 0, s, a);
     DPC_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL(head_join_chunk_kernel, dim3((unsigned)p.chunk), dim3(256), 0, s, j);
+    hipLaunchKernelGGL(head_join_chunk_kernel, dim3((unsigned)(p.chunk / kJoinRows)), dim3(256), 0,
+                       s, j);
     DPC_HIP_CHECK(hipGetLastError());
     ProductArgs m = {};
     m.mm = MmArgs{w, MmOperand{j.e, a.lde, 0, 0}, V, 1, p.tiles_d, tiles_c, p.splits_c};
@@ -1250,7 +1259,8 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
   const MmOperand hop = {nullptr, p.ld, N * p.ld, 0};
   const int out_bf16 = dtype == DPC_BF16;
   const int64_t esz = out_bf16 ? 2 : 4;
-  const int64_t ldz = (int64_t)p.piece_tiles * kMmTile;
+  const int64_t ldz = (int64_t)p.piece_tiles * 4;
+  const int64_t plane = p.tiles_n * ldz * kMmBlock;
   uint16_t* dz = reinterpret_cast<uint16_t*>(base + p.b_dz);
   for (int i = 0; i < p.pieces; ++i) {
     const int tile0 = i * p.piece_tiles, first = tile0 * kMmTile;
@@ -1276,14 +1286,14 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
     a.gmax = pa.gmax;
     a.dz = dz;
     a.ld = ldz;
-    a.plane = N * ldz;
+    a.plane = plane;
     const dim3 grid((unsigned)tiles * (unsigned)p.tiles_n);
     if (p.planes == 1)
       hipLaunchKernelGGL((head_grad_kernel<1>), grid, dim3(kMmThreads), 0, s, a);
     else
       hipLaunchKernelGGL((head_grad_kernel<3>), grid, dim3(kMmThreads), 0, s, a);
     DPC_HIP_CHECK(hipGetLastError());
-    const MmOperand zop = {dz, ldz, N * ldz, 0};
+    const MmOperand zop = {dz, ldz, plane, 0};
     ProductArgs q = {};
     q.h = h;
     q.rows_a = D;

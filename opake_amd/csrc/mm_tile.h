@@ -2,6 +2,11 @@
 // (gfx950), for operands of either orientation:
 //   K-contiguous: element (i, k) at p[i * ld + k]  (a row holds one index's K values)
 //   K-slow:       element (i, k) at p[k * ld + i]  (a row holds one k of every index)
+// or blocked: a [rows, columns] matrix in blocks of 256 rows x 64 columns (32 KiB,
+// row by row, the blocks of 256 rows side by side, ld of them), whose rows are the
+// index and columns K (K-contiguous) or the other way round (K-slow).  A step of a
+// tile is then one block, or four pieces of 8 KiB: whole pages of memory, where
+// 128-byte pieces of 256 long rows cost a quarter of the product's rate.
 //
 // acc[i][j] of a wave holds 16 x 16 blocks: lane l has rows 4 (l / 16) + r
 // (r < 4) of operand A's index and column l % 16 of operand B's, so four
@@ -20,7 +25,7 @@
 
 struct MmOperand {
   const uint16_t* p;  // 16-byte aligned
-  int64_t ld;         // elements, a multiple of 8
+  int64_t ld;         // elements, a multiple of 8; blocked: blocks
   int64_t plane;      // elements between planes
   int rows;           // valid indices
 };
@@ -83,7 +88,9 @@ struct MmAcc {
   static DPC_DEVICE int col0(int w) { return kWideB ? (w >> 2) * 128 : (w >> 1) * 64; }
 };
 
-template <bool kKc>
+constexpr int64_t kMmBlock = kMmTile * kMmStep;  // elements
+
+template <bool kKc, bool kBlocked>
 struct MmStage {
   int voff[4];  // byte offsets of this lane's four 16-byte chunks of a step
   int kchunk;   // K-contiguous: first k of the lane's chunk
@@ -93,21 +100,30 @@ struct MmStage {
       if (kKc) {
         const int row = 8 * (w + 8 * j) + (lane >> 3);
         kchunk = ((lane & 7) ^ ((row >> 1) & 7)) * 8;
-        voff[j] = (int)((row * o.ld + kchunk) * 2);
+        voff[j] = (int)((row * (kBlocked ? kMmStep : o.ld) + kchunk) * 2);
       } else {
-        const int row = 2 * (w + 8 * j) + (lane >> 5);
-        voff[j] = (int)((row * o.ld + tile_slot_col(row, lane & 31)) * 2);
+        const int row = 2 * (w + 8 * j) + (lane >> 5), col = tile_slot_col(row, lane & 31);
+        voff[j] = kBlocked ? (int)(((col >> 6) * kMmBlock + row * kMmStep + (col & 63)) * 2)
+                           : (int)((row * o.ld + col) * 2);
       }
     }
   }
-  // The step at k0 of plane `pl` of the tile from index i0: the buffer it reads, and
-  // `bad`, out of the buffer's range for lanes whose k is past kl.  Rows past the
-  // operand's are out of range too: all such reads give zeros.
-  DPC_DEVICE u32x4_t buffer(const MmOperand& o, int pl, int i0, int k0, int kl, int* bad) const {
+  // The step at k0 of plane `pl` of tile t: the buffer it reads, and `bad`, out of the
+  // buffer's range for lanes whose k is past kl.  Rows past the operand's are out of
+  // range too: all such reads give zeros.  (Blocks are whole; past their matrix they
+  // hold zeros.)
+  DPC_DEVICE u32x4_t buffer(const MmOperand& o, int pl, int t, int k0, int kl, int* bad) const {
     const uint16_t* base = o.p + (int64_t)pl * o.plane;
     uint32_t bytes;
     *bad = 0;
-    if (kKc) {
+    const int i0 = t * kMmTile;
+    if (kBlocked && kKc) {
+      base += (t * o.ld + (k0 >> 6)) * kMmBlock;
+      bytes = kMmBlock * 2;
+    } else if (kBlocked) {
+      base += ((k0 >> 8) * o.ld + 4 * t) * kMmBlock + (k0 & 255) * kMmStep;
+      bytes = (uint32_t)((4 * kMmBlock - (k0 & 255) * kMmStep) * 2);
+    } else if (kKc) {
       base += (int64_t)i0 * o.ld + k0;
       bytes = (uint32_t)((min(o.rows - i0, kMmTile) * o.ld - k0) * 2);
       *bad = k0 + kchunk >= kl ? kMmOutOfRange : 0;
@@ -183,7 +199,7 @@ struct MmPlace {
 // B's of step s + 1 at the start of step s, so each has most of a step or more to
 // land and the barrier is the only place where a wave waits.
 // Ends with a barrier, after which `lds` is free.
-template <bool kAKc, bool kBKc, bool kWideB>
+template <bool kAKc, bool kBKc, bool kBBlocked, bool kWideB>
 DPC_DEVICE void mm_loop(const MmArgs& g, int ta, int tb, int split, uint8_t* lds,
                         MmAcc<kWideB>& acc) {
   const int tid = threadIdx.x, lane = tid & 63,
@@ -199,19 +215,19 @@ DPC_DEVICE void mm_loop(const MmArgs& g, int ta, int tb, int split, uint8_t* lds
   if (steps <= 0) return;
   const int pair0 = __builtin_amdgcn_readfirstlane(s0 / ks);
   MmPlace pa = {steps, g.planes == 1 ? 5 : pair0, (s0 - pair0 * ks) * kMmStep}, pb = pa;
-  MmStage<kAKc> sa;
-  MmStage<kBKc> sb;
+  MmStage<kAKc, false> sa;
+  MmStage<kBKc, kBBlocked> sb;
   sa.init(g.a, w, lane);
   sb.init(g.b, w, lane);
   constexpr bool kMixed = kAKc != kBKc;
   u32x4_t buf;
   int bad;
   auto next_a = [&]() __attribute__((always_inline)) {
-    buf = sa.buffer(g.a, (kMmPairsA >> (4 * pa.pair)) & 15, ta * kMmTile, pa.k0, g.kl, &bad);
+    buf = sa.buffer(g.a, (kMmPairsA >> (4 * pa.pair)) & 15, ta, pa.k0, g.kl, &bad);
     pa.next(g.kl);
   };
   auto next_b = [&]() __attribute__((always_inline)) {
-    buf = sb.buffer(g.b, (kMmPairsB >> (4 * pb.pair)) & 15, tb * kMmTile, pb.k0, g.kl, &bad);
+    buf = sb.buffer(g.b, (kMmPairsB >> (4 * pb.pair)) & 15, tb, pb.k0, g.kl, &bad);
     pb.next(g.kl);
   };
   auto fetch_a = [&](int stage, int j) __attribute__((always_inline)) {

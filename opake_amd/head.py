@@ -9,7 +9,7 @@ per-example clipping needs, and both are differentiable with respect to ``hidden
 
 Forward, one matrix-core product leaves the maximum and the sum of
 exponentials of every 256-wide piece of the vocabulary per token
-(``csrc/head.hip``).  No ``[tokens, vocabulary]`` tensor is kept: at most 256 MiB
+(``csrc/head.hip``).  No ``[tokens, vocabulary]`` tensor is kept: at most 512 MiB
 of it exist at a time (one 256-wide column or row block, where that is more).
 Where only ``hidden`` (bfloat16) requires a gradient -- a frozen head, the usual
 case under per-example clipping -- its gradient is made in the forward, chunk
