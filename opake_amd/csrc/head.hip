@@ -358,6 +358,9 @@ DPC_DEVICE int tiles_of(int rows) { return (rows + kMmTile - 1) / kMmTile; }
 // Loss: the tile's statistics and the entries' logits.
 // ---------------------------------------------------------------------------
 
+// A tile is two halves of 128 columns (one a wave): statistics are per half, so the
+// waves finish their halves without waiting for each other or using LDS, while the
+// workgroup's next tile is on its way into it.
 struct StatsArgs {
   MmArgs mm;  // A = W (vocabulary), B = H (rows with a target)
   Hidden h;
@@ -365,40 +368,42 @@ struct StatsArgs {
   float inv_tau;
   Entries entries;
   float* picked;   // [rows, K]: z at the entries' columns
-  f32x2_t* part;   // [rows, tiles_a]: maximum and sum of exponentials of each tile
-  uint16_t* e;     // the chunk's exp(z - the tile's maximum) as fp16, in blocks
+  f32x2_t* part;   // [2 tiles_a][N]: maximum and sum of exponentials of each half
+  int64_t N;
+  uint16_t* e;     // the chunk's exp(z - the half's maximum) as fp16, native order
   int64_t lde;     // blocks of a row of them
 };
 
-// Byte of (row of the tile, column) in a 256 x 256 tile of 2-byte values in LDS:
-// 512-byte rows whose 16-byte chunks are XOR-swizzled by the row.
-DPC_DEVICE int tile16_off(int row, int col) {
-  return row * 512 + (((col >> 3) ^ (row & 15)) << 4) + (col & 7) * 2;
+// The lane, of unknown value to the compiler: what an epilogue computes from it would
+// otherwise be kept in registers through the product's loop, which has none to spare.
+DPC_DEVICE int epilogue_lane() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
 }
 
-// The staged tile to its four blocks (128 KiB in a row).
-DPC_DEVICE void store_tile16(uint16_t* dst) {
-#pragma unroll 4
-  for (int i = threadIdx.x; i < 4 * kMmTile * 8; i += kMmThreads) {
-    const int row = (i >> 3) & 255, col = (i >> 11) * kMmStep + (i & 7) * 8;
-    *reinterpret_cast<u32x4_t*>(dst + 8 * i) =
-        *reinterpret_cast<const u32x4_t*>(lds_all + tile16_off(row, col));
+// The block ij / 4, ij % 4 of a wave's accumulators (ij uniform).  The empty asm keeps
+// the cases apart: merged into one load at a computed address they would move the
+// accumulators to memory.
+DPC_DEVICE f32x4_t acc_block(const MmAcc<false>& acc, int ij) {
+  f32x4_t x = acc.v[0][0];
+#define HEAD_CASE(n) case n: x = acc.v[(n) >> 2][(n) & 3]; asm volatile("" : "+v"(x)); break;
+#define HEAD_CASE4(n) HEAD_CASE(n) HEAD_CASE(n + 1) HEAD_CASE(n + 2) HEAD_CASE(n + 3)
+  switch (ij) {
+    HEAD_CASE4(0) HEAD_CASE4(4) HEAD_CASE4(8) HEAD_CASE4(12)
+    HEAD_CASE4(16) HEAD_CASE4(20) HEAD_CASE4(24) HEAD_CASE4(28)
   }
+#undef HEAD_CASE4
+#undef HEAD_CASE
+  return x;
 }
 
 template <bool kEmit>
-__global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) {
-  int split, ta, tb;
-  const int N = hidden_rows(s.h, &s.mm.b.p);
-  s.mm.b.rows = N;
-  s.mm.tiles_b = tiles_of(N);
-  if (!mm_tile_of(s.mm, &split, &ta, &tb)) return;
-  MmAcc<false> acc;
-  mm_loop<true, true, false>(s.mm, ta, tb, 0, lds_all, acc);
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6),
+DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, int N, int ta, int tb,
+                               int64_t g0, const uint2* list, int e0, int e1, uint2 first) {
+  const int lane = epilogue_lane(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
             wm = w & 1, wn = w >> 1;
   const int v0 = ta * kMmTile, n0 = tb * kMmTile;
-  const int64_t g0 = s.h.first + n0;  // the row's number
   const int vl = wm * 128 + 4 * (lane >> 4);  // + 16 i + r
   const int tl = wn * 64 + (lane & 15);       // + 16 j
   const int vleft = s.V - v0 - vl;
@@ -408,43 +413,22 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc.v[i][j] *= s.inv_tau;
   }
-  // Entries: the blocks of 16 rows that have one, in float32 through LDS (rows of 1
-  // KiB, 16-byte chunks XOR-swizzled by the row), eight at a time.
-  const int64_t blk = g0 / kMmTile;
-  const int32_t* start = s.entries.start + blk * (s.mm.tiles_a + 1) + ta;
-  const uint2* list = s.entries.list + g0 * s.K;
-  const int e0 = start[0], e1 = start[1];
-  if (e1 > e0) {
-    uint32_t hit = 0;
-    for (int e = e0 + lane; e < e1; e += 64) hit |= 1u << (list[e].y >> 12);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) hit |= __shfl_xor(hit, d);
-    hit = __builtin_amdgcn_readfirstlane(hit);
-    const int slots = __popc(hit);
-    for (int p = 0; p < slots; p += 8) {
-      if (p) __syncthreads();
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int b = wn * 4 + j, slot = __popc(hit & ((1u << b) - 1)) - p;
-        if (((hit >> b) & 1) && slot >= 0 && slot < 8) {
-          const int t = lane & 15;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            *reinterpret_cast<f32x4_t*>(lds_all + slot * 16384 + t * 1024 +
-                                        ((((vl + 16 * i) >> 2) ^ t) << 4)) = acc.v[i][j];
-        }
-      }
-      __syncthreads();
-      for (int e = e0 + tid; e < e1; e += kMmThreads) {
-        const uint2 x = list[e];
-        const int t = (x.y >> 8) & 15, c = x.y & 255, b = x.y >> 12;
-        const int slot = __popc(hit & ((1u << b) - 1)) - p;
-        if (slot >= 0 && slot < 8)
-          s.picked[g0 * s.K + x.x] = *reinterpret_cast<const float*>(
-              lds_all + slot * 16384 + t * 1024 + (((c >> 2) ^ t) << 4) + (c & 3) * 4);
-      }
+  // Entries: a wave goes through the tile's, 64 at a time, and takes those of its own
+  // rows and columns out of its accumulators one by one.
+  for (int e = e0; e < e1; e += 64) {
+    const uint2 x = e == e0 ? first
+                            : (e + lane < e1 ? list[e + lane] : make_uint2(0u, 0xffffffffu));
+    const bool mine = ((x.y >> 7) & 1) == (uint32_t)wm && (x.y >> 14) == (uint32_t)wn;
+    unsigned long long todo = __ballot(mine);
+    while (todo) {
+      const int from = __builtin_ctzll(todo);
+      todo &= todo - 1;
+      const uint32_t y = __builtin_amdgcn_readlane(x.y, from);
+      const uint32_t to = __builtin_amdgcn_readlane(x.x, from);
+      const f32x4_t b = acc_block(acc, (int)(((y >> 4) & 7) << 2 | ((y >> 12) & 3)));
+      const float v = y & 2 ? (y & 1 ? b[3] : b[2]) : (y & 1 ? b[1] : b[0]);
+      if (lane == (int)(((y >> 8) & 15) | ((y >> 2) & 3) << 4)) s.picked[g0 * s.K + to] = v;
     }
-    __syncthreads();
   }
   if (v0 + kMmTile > s.V) {  // past the vocabulary
 #pragma unroll
@@ -455,9 +439,8 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
         for (int r = 0; r < 4; ++r)
           if (16 * i + r >= vleft) acc.v[i][j][r] = -INFINITY;
   }
-  // Maxima, then exponentials against the tile's (both halves of the vocabulary).
-  float* tops = reinterpret_cast<float*>(lds_all);  // [2][256]
-  float* sums = tops + 512;                         // [2][256]
+  f32x2_t* part = s.part + (int64_t)(2 * ta + wm) * s.N + g0 + tl;
+  uint16_t* out = s.e + (tb * s.lde + 4 * ta + 2 * wm) * kMmBlock + wn * 2048 + lane * 8;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float m = -INFINITY;
@@ -467,12 +450,6 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
       for (int r = 0; r < 4; ++r) m = fmaxf(m, acc.v[i][j][r]);
     m = fmaxf(m, __shfl_xor(m, 16));
     m = fmaxf(m, __shfl_xor(m, 32));
-    if (lane < 16) tops[wm * 256 + tl + 16 * j] = m;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float m = fmaxf(tops[tl + 16 * j], tops[256 + tl + 16 * j]);
     const float base = (m == -INFINITY ? 0.f : m) * kLog2e;
     float sum = 0.f;
 #pragma unroll
@@ -483,28 +460,47 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
         acc.v[i][j][r] = e;
         sum += e;
       }
+    if constexpr (kEmit) {
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {  // 32 columns: half p % 2 of block p / 2
+        typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+        half8_t h;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) h[r] = (_Float16)acc.v[2 * p + (r >> 2)][j][r & 3];
+        *reinterpret_cast<half8_t*>(out + (p >> 1) * kMmBlock + (p & 1) * 8192 + j * 512) = h;
+      }
+    }
     sum += __shfl_xor(sum, 16);
     sum += __shfl_xor(sum, 32);
-    if (lane < 16) sums[wm * 256 + tl + 16 * j] = sum;
+    if (lane < 16 && n0 + tl + 16 * j < N) part[16 * j] = f32x2_t{m, sum};
   }
-  __syncthreads();
-  if (tid < kMmTile && n0 + tid < N)
-    s.part[(g0 + tid) * s.mm.tiles_a + ta] =
-        f32x2_t{fmaxf(tops[tid], tops[256 + tid]), sums[tid] + sums[256 + tid]};
-  if constexpr (kEmit) {
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
-        half4_t h;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) h[r] = (_Float16)acc.v[i][j][r];
-        *reinterpret_cast<half4_t*>(lds_all + tile16_off(tl + 16 * j, vl + 16 * i)) = h;
-      }
-    __syncthreads();
-    store_tile16(s.e + (tb * s.lde + 4 * ta) * kMmBlock);
+}
+
+template <bool kEmit>
+__global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) {
+  const int lane = threadIdx.x & 63;
+  const int N = hidden_rows(s.h, &s.mm.b.p);
+  s.mm.b.rows = N;
+  s.mm.tiles_b = tiles_of(N);
+  MmTile<true, true, false, false> tile(s.mm, lds_all);
+  MmAcc<false> acc;
+  int split, ta, tb, ta2, tb2, id = blockIdx.x;
+  bool more = mm_tile_of(s.mm, id, &split, &ta2, &tb2);
+  if (more) tile.begin(ta2, tb2, 0);
+  while (more) {
+    ta = ta2;
+    tb = tb2;
+    // The tile's entries, its first 64 loaded beside the product.
+    const int64_t g0 = s.h.first + (int64_t)tb * kMmTile;  // the first row's number
+    const int32_t* start = s.entries.start + (g0 / kMmTile) * (s.mm.tiles_a + 1) + ta;
+    const uint2* list = s.entries.list + g0 * s.K;
+    const int e0 = start[0], e1 = start[1];
+    const uint2 first = e0 + lane < e1 ? list[e0 + lane] : make_uint2(0u, 0xffffffffu);
+    tile.run(acc);
+    id += gridDim.x;
+    more = mm_tile_of(s.mm, id, &split, &ta2, &tb2);
+    if (more) tile.begin(ta2, tb2, 0);
+    stats_epilogue<kEmit>(s, acc, N, ta, tb, g0, list, e0, e1, first);
   }
 }
 
@@ -521,6 +517,7 @@ DPC_DEVICE float wave_sum(float v) {
 
 struct JoinArgs {
   Rows rows;
+  int64_t N;
   int K, parts;
   float inv_tau, loss_scale;
   const int32_t* cols;
@@ -530,26 +527,12 @@ struct JoinArgs {
   float* loss;  // at the row's own place; the others by the row's number
   float* lse;   // NaN: an entry outside the vocabulary or NaN
   float* corr;  // [rows, K]: p - sum of the q of all entries of the column
-  // A chunk's rows, to be turned into p - q in place.
-  int first, most;
-  uint16_t* e;
-  int64_t lde;
+  int first;
 };
 
-// Row n by one wave; its lse.
-DPC_DEVICE float join_row(const JoinArgs& a, int64_t n, int lane) {
+// Row n by one wave, from its lse.
+DPC_DEVICE void join_row(const JoinArgs& a, int64_t n, float lse, int lane) {
   const int64_t own = a.rows.active[n];
-  const f32x2_t* part = a.part + n * a.parts;
-  float m = -INFINITY, sum = 0.f;
-  for (int i = lane; i < a.parts; i += 64) {
-    const f32x2_t x = part[i];
-    const float nm = fmaxf(m, x.x), base = nm == -INFINITY ? 0.f : nm;
-    sum = sum * fast_exp(m - base) + x.y * fast_exp(x.x - base);
-    m = nm;
-  }
-  const float top = wave_max(m), tb = top == -INFINITY ? 0.f : top;
-  sum = wave_sum(sum * fast_exp(m - tb));
-  float lse = top + logf(sum);
   const int32_t* cols = a.cols + n * a.K;
   const float* picked = a.picked + n * a.K;
   float* corr = a.corr + n * a.K;
@@ -562,7 +545,7 @@ DPC_DEVICE float join_row(const JoinArgs& a, int64_t n, int lane) {
       a.lse[n] = lse;
       corr[0] = fast_exp(z - lse) - 1.0f;
     }
-    return lse;
+    return;
   }
   const float* teacher = a.teacher + own * a.K;
   float tm = -INFINITY;
@@ -611,54 +594,90 @@ DPC_DEVICE float join_row(const JoinArgs& a, int64_t n, int lane) {
     a.loss[own] = bad ? NAN : loss * a.loss_scale;
     a.lse[n] = lse;
   }
-  return lse;
 }
 
-// One wave a row.
-__global__ void __launch_bounds__(256) head_join_kernel(JoinArgs a) {
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (n < *a.rows.count) join_row(a, n, threadIdx.x & 63);
+// 16 rows a workgroup of 8 waves: their lse from the halves' statistics (16 lanes side
+// by side read 16 rows), then their losses (a wave two rows).
+constexpr int kJoinRows = 16, kJoinThreads = 512;
+
+__global__ void __launch_bounds__(kJoinThreads) head_join_kernel(JoinArgs a) {
+  __shared__ f32x2_t stats[kJoinThreads];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int64_t n0 = a.first + (int64_t)blockIdx.x * kJoinRows, count = *a.rows.count;
+  if (n0 >= count) return;
+  const int rows = (int)(count - n0 < kJoinRows ? count - n0 : kJoinRows);
+  const f32x2_t* part = a.part + n0 + min(tid & 15, rows - 1);
+  float m = -INFINITY, sum = 0.f;
+#pragma unroll 4
+  for (int i = tid >> 4; i < a.parts; i += kJoinThreads / 16) {
+    const f32x2_t x = part[i * a.N];
+    const float nm = fmaxf(m, x.x), base = nm == -INFINITY ? 0.f : nm;
+    sum = sum * fast_exp(m - base) + x.y * fast_exp(x.x - base);
+    m = nm;
+  }
+  stats[tid] = f32x2_t{m, sum};
+  __syncthreads();
+  for (int k = w; k < rows; k += kJoinThreads / 64) {
+    const f32x2_t x = lane < 32 ? stats[lane * 16 + k] : f32x2_t{-INFINITY, 0.f};
+    const float top = wave_max(x.x), base = top == -INFINITY ? 0.f : top;
+    join_row(a, n0 + k, top + logf(wave_sum(x.y * fast_exp(x.x - base))), lane);
+  }
 }
 
-// Eight rows of a chunk a workgroup: the joins, then the rows' exp(z - tile's
-// maximum) times exp(tile's maximum - lse), and at the entries' columns p - q.  The
-// eight rows are 1 KiB of every block; a wave takes one block of each tile.
-constexpr int kJoinRows = 8;
+// A chunk's exp(z - half's maximum) times exp(half's maximum - lse), in place, and p - q
+// at the entries' columns: 16 rows x 8 tiles a workgroup.  The 16 rows are 1 KiB of every
+// 32 columns; a wave takes one of each tile's eight, all its loads in flight at once.
+constexpr int kFixTiles = 8;
 
-__global__ void __launch_bounds__(256) head_join_chunk_kernel(JoinArgs a) {
-  __shared__ float lses[kJoinRows];
+struct FixArgs {
+  const int32_t* count;
+  int64_t N;
+  int K, tiles, first;
+  const int32_t* cols;
+  const f32x2_t* part;
+  const float* lse;
+  const float* corr;
+  uint16_t* e;
+  int64_t lde;
+};
+
+__global__ void __launch_bounds__(kJoinThreads) head_fix_kernel(FixArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int local = blockIdx.x * kJoinRows;  // first row in the chunk
-  const int64_t n0 = a.first + local, count = *a.rows.count;
-  if (local >= a.most || n0 >= count) return;
+  const int64_t n0 = a.first + local, count = *a.count;
+  if (n0 >= count) return;
   const int rows = (int)(count - n0 < kJoinRows ? count - n0 : kJoinRows);
-  for (int r = w; r < kJoinRows; r += 4) {
-    const float lse = r < rows ? join_row(a, n0 + r, lane) : 0.f;
-    if (lane == 0) lses[r] = lse;
-  }
-  __syncthreads();
+  const int t0 = blockIdx.y * kFixTiles, tiles = min(kFixTiles, a.tiles - t0);
   typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-  uint16_t* tile = a.e + (local >> 8) * a.lde * kMmBlock + (local & 255) * kMmStep;
-  const int r = lane >> 3;
-  const float lse = lses[r];
-  const f32x2_t* part = a.part + (n0 + min(r, rows - 1)) * a.parts;
-#pragma unroll 4
-  for (int t = 0; t < a.parts; ++t) {
-    uint16_t* at = tile + (4 * t + w) * kMmBlock + lane * 8;
-    const half8_t h = *reinterpret_cast<const half8_t*>(at);
-    const float f = fast_exp(part[t].x - lse);
-    u32x4_t o;
+  uint16_t* block = a.e + (local >> 8) * a.lde * kMmBlock + ((local & 255) >> 4) * 512;
+  uint16_t* at = block + (4 * t0 + (w >> 1)) * kMmBlock + (w & 1) * 8192 + lane * 8;
+  const int64_t n = n0 + min(lane & 15, rows - 1);
+  const f32x2_t* top = a.part + (2 * t0 + (w >> 2)) * a.N + n;
+  const float lse = a.lse[n];
+  half8_t h[kFixTiles];
+  float f[kFixTiles];
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      o[e] = f32x2_to_bf16x2_bits((float)h[2 * e] * f, (float)h[2 * e + 1] * f);
-    *reinterpret_cast<u32x4_t*>(at) = o;
-  }
+  for (int t = 0; t < kFixTiles; ++t)
+    if (t < tiles) {
+      h[t] = *reinterpret_cast<const half8_t*>(at + 4 * t * kMmBlock);
+      f[t] = top[2 * t * a.N].x;
+    }
+#pragma unroll
+  for (int t = 0; t < kFixTiles; ++t)
+    if (t < tiles) {
+      const float x = fast_exp(f[t] - lse);
+      u32x4_t o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        o[e] = f32x2_to_bf16x2_bits((float)h[t][2 * e] * x, (float)h[t][2 * e + 1] * x);
+      *reinterpret_cast<u32x4_t*>(at + 4 * t * kMmBlock) = o;
+    }
   __syncthreads();
-  for (int i = tid; i < rows * a.K; i += 256) {
+  for (int i = tid; i < rows * a.K; i += kJoinThreads) {
     const int c = a.cols[n0 * a.K + i];
-    if (c >= 0)
-      tile[(c >> 6) * kMmBlock + (i / a.K) * kMmStep + (c & 63)] =
-          f32_to_bf16_bits(a.corr[n0 * a.K + i]);
+    if (c >= 0 && (c >> 8) >= t0 && (c >> 8) < t0 + tiles)
+      block[(c >> 6) * kMmBlock + ((c >> 5) & 1) * 8192 + ((c >> 2) & 3) * 128 + (i / a.K) * 8 +
+            ((c >> 4) & 1) * 4 + (c & 3)] = f32_to_bf16_bits(a.corr[n0 * a.K + i]);
   }
 }
 
@@ -710,20 +729,15 @@ struct GradArgs {
   const float* g;     // [N]: the losses' gradient, at the rows' own places
   const float* gmax;  // dz is held over gmax, so a gradient that is the same for all
                       // rows (one over the tokens) is not rounded with every value
-  uint16_t* dz;       // [planes], in blocks
+  uint16_t* dz;       // [planes], native order
   int64_t ld, plane;  // blocks of a row of them, elements
 };
 
 template <int kPlanes>
-__global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
-  int split, ta, tb;
-  const int N = hidden_rows(s.h, &s.mm.b.p);
-  s.mm.b.rows = N;
-  s.mm.tiles_b = tiles_of(N);
-  if (!mm_tile_of(s.mm, &split, &ta, &tb)) return;
-  MmAcc<false> acc;
-  mm_loop<true, true, false>(s.mm, ta, tb, 0, lds_all, acc);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, wm = w & 1, wn = w >> 1;
+DPC_DEVICE void grad_epilogue(const GradArgs& s, MmAcc<false>& acc, int N, int ta, int tb,
+                              const uint2* list, int e0, int e1, uint2 first) {
+  const int lane = epilogue_lane(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
+            wm = w & 1, wn = w >> 1;
   const int vt = s.tile0 + ta, n0 = tb * kMmTile;
   const int vl = wm * 128 + 4 * (lane >> 4);
   const int tl = wn * 64 + (lane & 15);
@@ -738,43 +752,92 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(acc.v[i][j][r], c, -base)) * g;
-        acc.v[i][j][r] = 16 * i + r < vleft ? e : 0.f;
-      }
+      for (int r = 0; r < 4; ++r)
+        acc.v[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc.v[i][j][r], c, -base)) * g;
   }
-  const int32_t* start = s.entries.start + (int64_t)tb * (s.tiles + 1) + vt;
-  const uint2* list = s.entries.list + (int64_t)n0 * s.K;
-  const int e0 = start[0], e1 = start[1];
-#pragma unroll 1
-  for (int pl = 0; pl < kPlanes; ++pl) {
-    if (pl) __syncthreads();
+  if ((vt + 1) * kMmTile > s.V) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const f32x4_t x = acc.v[i][j];
-        uint32_t lo, hi;
-        if (kPlanes == 1) {
-          lo = f32x2_to_bf16x2_bits(x[0], x[1]);
-          hi = f32x2_to_bf16x2_bits(x[2], x[3]);
-        } else {
-          lo = split_plane(x[0], pl) | ((uint32_t)split_plane(x[1], pl) << 16);
-          hi = split_plane(x[2], pl) | ((uint32_t)split_plane(x[3], pl) << 16);
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * i + r >= vleft) acc.v[i][j][r] = 0.f;
+  }
+  uint16_t* out = s.dz + (tb * s.ld + 4 * ta + 2 * wm) * kMmBlock + wn * 2048 + lane * 8;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      uint16_t* at = out + (p >> 1) * kMmBlock + (p & 1) * 8192 + j * 512;
+      const f32x4_t x = acc.v[2 * p][j], y = acc.v[2 * p + 1][j];
+      if (kPlanes == 1) {
+        *reinterpret_cast<u32x4_t*>(at) =
+            u32x4_t{f32x2_to_bf16x2_bits(x[0], x[1]), f32x2_to_bf16x2_bits(x[2], x[3]),
+                    f32x2_to_bf16x2_bits(y[0], y[1]), f32x2_to_bf16x2_bits(y[2], y[3])};
+      } else {
+#pragma unroll
+        for (int pl = 0; pl < kPlanes; ++pl) {
+          u32x4_t o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const f32x4_t& z = e < 2 ? x : y;
+            o[e] = split_plane(z[2 * (e & 1)], pl) |
+                   ((uint32_t)split_plane(z[2 * (e & 1) + 1], pl) << 16);
+          }
+          *reinterpret_cast<u32x4_t*>(at + pl * s.plane) = o;
         }
-        *reinterpret_cast<uint2*>(lds_all + tile16_off(tl + 16 * j, vl + 16 * i)) =
-            make_uint2(lo, hi);
       }
-    __syncthreads();
-    for (int e = e0 + tid; e < e1; e += kMmThreads) {
-      const uint2 y = list[e];
-      const int t = y.y >> 8;
-      const float x = s.corr[(int64_t)n0 * s.K + y.x] * (s.g[s.active[n0 + t]] / gmax);
-      *reinterpret_cast<uint16_t*>(lds_all + tile16_off(t, y.y & 255)) =
-          kPlanes == 1 ? f32_to_bf16_bits(x) : split_plane(x, pl);
     }
-    __syncthreads();
-    store_tile16(s.dz + pl * s.plane + (tb * s.ld + 4 * ta) * kMmBlock);
+  // Entries: put in place by the lane that stored the value.
+  for (int e = e0; e < e1; e += 64) {
+    const uint2 x = e == e0 ? first
+                            : (e + lane < e1 ? list[e + lane] : make_uint2(0u, 0xffffffffu));
+    const bool mine = ((x.y >> 7) & 1) == (uint32_t)wm && (x.y >> 14) == (uint32_t)wn;
+    unsigned long long todo = __ballot(mine);
+    const float d = mine ? s.corr[(int64_t)n0 * s.K + x.x] * (s.g[s.active[n0 + (x.y >> 8)]] / gmax)
+                         : 0.f;
+    while (todo) {
+      const int from = __builtin_ctzll(todo);
+      todo &= todo - 1;
+      const uint32_t y = __builtin_amdgcn_readlane(x.y, from);
+      const float v = __builtin_bit_cast(
+          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, d), from));
+      const int c = y & 127, j = (y >> 12) & 3;
+      uint16_t* at = out + (c >> 6) * kMmBlock + ((c >> 5) & 1) * 8192 + j * 512 +
+                     ((c >> 4) & 1) * 4 + (c & 3);
+      if (lane == (int)(((y >> 8) & 15) | ((y >> 2) & 3) << 4)) {
+#pragma unroll
+        for (int pl = 0; pl < kPlanes; ++pl)
+          at[pl * s.plane] = kPlanes == 1 ? f32_to_bf16_bits(v) : split_plane(v, pl);
+      }
+    }
+  }
+}
+
+template <int kPlanes>
+__global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
+  const int lane = threadIdx.x & 63;
+  const int N = hidden_rows(s.h, &s.mm.b.p);
+  s.mm.b.rows = N;
+  s.mm.tiles_b = tiles_of(N);
+  MmTile<true, true, false, false> tile(s.mm, lds_all);
+  MmAcc<false> acc;
+  int split, ta, tb, ta2, tb2, id = blockIdx.x;
+  bool more = mm_tile_of(s.mm, id, &split, &ta2, &tb2);
+  if (more) tile.begin(ta2, tb2, 0);
+  while (more) {
+    ta = ta2;
+    tb = tb2;
+    const int32_t* start = s.entries.start + (int64_t)tb * (s.tiles + 1) + s.tile0 + ta;
+    const uint2* list = s.entries.list + (int64_t)tb * kMmTile * s.K;
+    const int e0 = start[0], e1 = start[1];
+    const uint2 first = e0 + lane < e1 ? list[e0 + lane] : make_uint2(0u, 0xffffffffu);
+    tile.run(acc);
+    id += gridDim.x;
+    more = mm_tile_of(s.mm, id, &split, &ta2, &tb2);
+    if (more) tile.begin(ta2, tb2, 0);
+    grad_epilogue<kPlanes>(s, acc, N, ta, tb, list, e0, e1, first);
   }
 }
 
@@ -832,9 +895,11 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_product_kernel(ProductArgs
     s.mm.a.p = hp;
     s.mm.kl = count;
   }
-  if (!mm_tile_of(s.mm, &split, &ta, &tb)) return;
+  if (!mm_tile_of(s.mm, blockIdx.x, &split, &ta, &tb)) return;
+  MmTile<false, kHidden, true, kHidden> tile(s.mm, lds_all);
   MmAcc<kHidden> acc;
-  mm_loop<false, kHidden, true>(s.mm, ta, tb, split, lds_all, acc);
+  tile.begin(ta, tb, split);
+  tile.run(acc);
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int a0 = ta * kMmTile + acc.row0(w) + 4 * (lane >> 4);
   const int b0 = tb * kMmTile + acc.col0(w) + (lane & 15);
@@ -905,12 +970,14 @@ __global__ void __launch_bounds__(256) head_reduce_kernel(ReduceArgs a) {
 // Held at once: dz of a piece of the vocabulary, or a chunk's exponentials.
 constexpr int64_t kPieceBytes = 512ll << 20;
 
+constexpr int kUnits = 256;  // compute units of an MI355X
+
 int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
 // Slices of `steps` K steps for `tiles` tiles: about one workgroup a compute
 // unit, no slice under 8 steps.
 int slices(int64_t tiles, int64_t steps) {
-  int64_t s = 256 / tiles;
+  int64_t s = kUnits / tiles;
   if (s > steps / 8) s = steps / 8;
   if (s > 32) s = 32;
   return s < 1 ? 1 : (int)s;
@@ -989,7 +1056,7 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
   p.f_h = take(p.planes * N * p.ld * 2);
   if (p.pack) p.f_w = take(p.planes * (int64_t)V * p.ld * 2);
   p.f_picked = take(N * K * 4);
-  p.f_part = take(N * p.tiles_v * 8);
+  p.f_part = take(N * p.tiles_v * 16);
   if (p.emit) {
     int64_t c = kPieceBytes / ((int64_t)p.tiles_v * kMmTile * 2) / kMmTile * kMmTile;
     if (c < kMmTile) c = kMmTile;
@@ -1071,6 +1138,9 @@ int reduce(const ReduceArgs& a, hipStream_t s) {
   return DPC_OK;
 }
 
+// Workgroups that go through `tiles` tiles, one a compute unit (LDS holds one).
+dim3 tile_grid(int64_t tiles) { return dim3((unsigned)(tiles < kUnits ? tiles : kUnits)); }
+
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
 bool valid_temperature(double t) { return t > 0.0 && t < 1e15; }
@@ -1151,10 +1221,12 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
   a.entries = entries;
   a.picked = reinterpret_cast<float*>(base + p.f_picked);
   a.part = reinterpret_cast<f32x2_t*>(base + p.f_part);
+  a.N = N;
   JoinArgs j = {};
   j.rows = rows;
+  j.N = N;
   j.K = K;
-  j.parts = p.tiles_v;
+  j.parts = 2 * p.tiles_v;
   j.inv_tau = a.inv_tau;
   j.loss_scale = (float)(temperature * temperature);
   j.cols = entries.cols;
@@ -1165,30 +1237,36 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
   j.lse = lse;
   j.corr = corr;
   if (!p.emit) {
-    hipLaunchKernelGGL((head_stats_kernel<false>), dim3((unsigned)p.tiles_v * (unsigned)p.tiles_n),
+    hipLaunchKernelGGL((head_stats_kernel<false>), tile_grid((int64_t)p.tiles_v * p.tiles_n),
                        dim3(kMmThreads), 0, s, a);
     DPC_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)((N + 3) / 4)), dim3(256), 0, s, j);
+    hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)((N + kJoinRows - 1) / kJoinRows)),
+                       dim3(kJoinThreads), 0, s, j);
     DPC_HIP_CHECK(hipGetLastError());
     return DPC_OK;
   }
   a.lde = (int64_t)p.tiles_v * 4;
   a.e = reinterpret_cast<uint16_t*>(base + p.f_e);
-  j.e = a.e;
-  j.lde = a.lde;
   const int tiles_c = p.chunk / kMmTile;
   float* unit = reinterpret_cast<float*>(kept + p.s_unit);
   for (int64_t first = 0; first < N; first += p.chunk) {
     a.h.first = j.first = (int)first;
-    a.h.most = j.most = p.chunk;
-    hipLaunchKernelGGL((head_stats_kernel<true>), dim3((unsigned)p.tiles_v * (unsigned)tiles_c),
+    a.h.most = p.chunk;
+    hipLaunchKernelGGL((head_stats_kernel<true>), tile_grid((int64_t)p.tiles_v * tiles_c),
                        dim3(kMmThreads), 0, s, a);
     DPC_HIP_CHECK(hipGetLastError());
-    hipLaunchKernelGGL(head_join_chunk_kernel, dim3((unsigned)(p.chunk / kJoinRows)), dim3(256), 0,
-                       s, j);
+    hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)(p.chunk / kJoinRows)),
+                       dim3(kJoinThreads), 0, s, j);
+    DPC_HIP_CHECK(hipGetLastError());
+    const FixArgs x = {rows.count, N, K, p.tiles_v, (int)first, entries.cols, a.part, lse, corr,
+                       a.e, a.lde};
+    hipLaunchKernelGGL(head_fix_kernel,
+                       dim3((unsigned)(p.chunk / kJoinRows),
+                            (unsigned)((p.tiles_v + kFixTiles - 1) / kFixTiles)),
+                       dim3(kJoinThreads), 0, s, x);
     DPC_HIP_CHECK(hipGetLastError());
     ProductArgs m = {};
-    m.mm = MmArgs{w, MmOperand{j.e, a.lde, 0, 0}, V, 1, p.tiles_d, tiles_c, p.splits_c};
+    m.mm = MmArgs{w, MmOperand{a.e, a.lde, 0, 0}, V, 1, p.tiles_d, tiles_c, p.splits_c};
     m.h = a.h;
     m.rows_a = D;
     m.lda = p.lda;
@@ -1287,7 +1365,7 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
     a.dz = dz;
     a.ld = ldz;
     a.plane = plane;
-    const dim3 grid((unsigned)tiles * (unsigned)p.tiles_n);
+    const dim3 grid = tile_grid((int64_t)tiles * p.tiles_n);
     if (p.planes == 1)
       hipLaunchKernelGGL((head_grad_kernel<1>), grid, dim3(kMmThreads), 0, s, a);
     else

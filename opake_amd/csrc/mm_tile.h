@@ -2,11 +2,13 @@
 // (gfx950), for operands of either orientation:
 //   K-contiguous: element (i, k) at p[i * ld + k]  (a row holds one index's K values)
 //   K-slow:       element (i, k) at p[k * ld + i]  (a row holds one k of every index)
-// or blocked: a [rows, columns] matrix in blocks of 256 rows x 64 columns (32 KiB,
-// row by row, the blocks of 256 rows side by side, ld of them), whose rows are the
-// index and columns K (K-contiguous) or the other way round (K-slow).  A step of a
-// tile is then one block, or four pieces of 8 KiB: whole pages of memory, where
-// 128-byte pieces of 256 long rows cost a quarter of the product's rate.
+// or native: a [rows, columns] matrix as the matrix cores hold it, in blocks of 256
+// rows x 64 columns (32 KiB each, `ld` of them side by side for every 256 rows), each
+// of 1 KiB pieces of 16 rows x 32 columns: lane l's 16 bytes are row l % 16 at columns
+// 4 (l / 16) + r and 16 + 4 (l / 16) + r (r < 4).  That is what a lane has in the
+// accumulators of a tile whose A index is the column, so a product's result is stored
+// as it is, and read back as the K-contiguous operand (index: row) of the next product
+// as it is, or through the transposing reads as a K-slow one (index: column).
 //
 // acc[i][j] of a wave holds 16 x 16 blocks: lane l has rows 4 (l / 16) + r
 // (r < 4) of operand A's index and column l % 16 of operand B's, so four
@@ -25,7 +27,7 @@
 
 struct MmOperand {
   const uint16_t* p;  // 16-byte aligned
-  int64_t ld;         // elements, a multiple of 8; blocked: blocks
+  int64_t ld;         // elements, a multiple of 8; native: blocks
   int64_t plane;      // elements between planes
   int rows;           // valid indices
 };
@@ -57,15 +59,15 @@ DPC_DEVICE int mm_steps(const MmArgs& g) {
   return (g.planes == 1 ? 1 : 6) * ((g.kl + kMmStep - 1) / kMmStep);
 }
 
-// Linear workgroup id -> (split, tile of A, tile of B); false past the last.
-// Dispatch is round-robin over the 8 XCDs: each XCD takes a contiguous range of
-// ids, walked in groups of four B tiles, so it re-reads operand tiles from its own
-// L2.
-DPC_DEVICE bool mm_tile_of(const MmArgs& g, int* split, int* ta, int* tb) {
-  const int tiles = g.tiles_a * g.tiles_b, n = tiles * g.splits, blk = blockIdx.x;
-  if (blk >= n) return false;
-  const int xcd = blk & 7;
-  int lin = xcd * (n >> 3) + min(xcd, n & 7) + (blk >> 3);
+// Linear id -> (split, tile of A, tile of B); false past the last.  Dispatch is
+// round-robin over the 8 XCDs: each XCD takes a contiguous range of ids, walked in
+// groups of four B tiles, so it re-reads operand tiles from its own L2.  (A workgroup
+// that takes several tiles steps its id by the grid's size, a multiple of 8.)
+DPC_DEVICE bool mm_tile_of(const MmArgs& g, int id, int* split, int* ta, int* tb) {
+  const int tiles = g.tiles_a * g.tiles_b, n = tiles * g.splits;
+  if (id >= n) return false;
+  const int xcd = id & 7;
+  int lin = xcd * (n >> 3) + min(xcd, n & 7) + (id >> 3);
   const int sp = lin / tiles;
   lin -= sp * tiles;
   const int per = 4 * g.tiles_a, grp = lin / per, first = grp * 4;
@@ -90,39 +92,49 @@ struct MmAcc {
 
 constexpr int64_t kMmBlock = kMmTile * kMmStep;  // elements
 
-template <bool kKc, bool kBlocked>
+// A native piece in LDS: slot l ^ 4 (l / 16) holds lane l's 16 bytes, so that the
+// transposing reads, which take 4 rows x 16 columns, land on distinct banks too.
+DPC_DEVICE int mm_native_slot(int row, int q) { return (row ^ (4 * q)) + 16 * q; }
+
+template <bool kKc, bool kNative>
 struct MmStage {
   int voff[4];  // byte offsets of this lane's four 16-byte chunks of a step
   int kchunk;   // K-contiguous: first k of the lane's chunk
   DPC_DEVICE void init(const MmOperand& o, int w, int lane) {
+    kchunk = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (kKc) {
+      if (kNative) {
+        const int from = mm_native_slot(lane & 15, lane >> 4) * 16;
+        // K-contiguous: the block as it is.  K-slow: eight pieces of 32 columns (four
+        // blocks) x four of 16 rows.
+        voff[j] = kKc ? (w + 8 * j) * 1024 + from
+                      : (int)(j * kMmBlock * 2) + (w >> 2) * 16384 + (w & 3) * 1024 + from;
+      } else if (kKc) {
         const int row = 8 * (w + 8 * j) + (lane >> 3);
         kchunk = ((lane & 7) ^ ((row >> 1) & 7)) * 8;
-        voff[j] = (int)((row * (kBlocked ? kMmStep : o.ld) + kchunk) * 2);
+        voff[j] = (int)((row * o.ld + kchunk) * 2);
       } else {
-        const int row = 2 * (w + 8 * j) + (lane >> 5), col = tile_slot_col(row, lane & 31);
-        voff[j] = kBlocked ? (int)(((col >> 6) * kMmBlock + row * kMmStep + (col & 63)) * 2)
-                           : (int)((row * o.ld + col) * 2);
+        const int row = 2 * (w + 8 * j) + (lane >> 5);
+        voff[j] = (int)((row * o.ld + tile_slot_col(row, lane & 31)) * 2);
       }
     }
   }
   // The step at k0 of plane `pl` of tile t: the buffer it reads, and `bad`, out of the
   // buffer's range for lanes whose k is past kl.  Rows past the operand's are out of
-  // range too: all such reads give zeros.  (Blocks are whole; past their matrix they
-  // hold zeros.)
+  // range too: all such reads give zeros.  (Native blocks are whole; past their matrix
+  // they hold zeros.)
   DPC_DEVICE u32x4_t buffer(const MmOperand& o, int pl, int t, int k0, int kl, int* bad) const {
     const uint16_t* base = o.p + (int64_t)pl * o.plane;
     uint32_t bytes;
     *bad = 0;
     const int i0 = t * kMmTile;
-    if (kBlocked && kKc) {
+    if (kNative && kKc) {
       base += (t * o.ld + (k0 >> 6)) * kMmBlock;
       bytes = kMmBlock * 2;
-    } else if (kBlocked) {
-      base += ((k0 >> 8) * o.ld + 4 * t) * kMmBlock + (k0 & 255) * kMmStep;
-      bytes = (uint32_t)((4 * kMmBlock - (k0 & 255) * kMmStep) * 2);
+    } else if (kNative) {
+      base += ((k0 >> 8) * o.ld + 4 * t) * kMmBlock + ((k0 & 255) >> 4) * 512;
+      bytes = (uint32_t)(4 * kMmBlock * 2 - ((k0 & 255) >> 4) * 1024);
     } else if (kKc) {
       base += (int64_t)i0 * o.ld + k0;
       bytes = (uint32_t)((min(o.rows - i0, kMmTile) * o.ld - k0) * 2);
@@ -140,18 +152,23 @@ struct MmStage {
 
 // Reads the 16 x 32 fragments of a wave's blocks from an operand's tile.  kMixed:
 // the other operand is K-slow, whose transposing reads fix the order of the
-// k-slots (frag16_off: slot 8 q + 4 h + e is k = 16 h + 4 q + e).  A lane keeps a
-// few byte offsets; blocks, sub-steps and stages are added as immediates.
-template <bool kKc, bool kMixed, int kBlocks>
+// k-slots (frag16_off: slot 8 q + 4 h + e is k = 16 h + 4 q + e; a native piece has
+// that order too).  A lane keeps a few byte offsets; blocks, sub-steps and stages are
+// added as immediates.
+template <bool kKc, bool kNative, bool kMixed, int kBlocks>
 struct MmFrags {
-  static constexpr int kOffsets = kKc ? (kMixed ? 4 : 2) : kBlocks / 2;
+  static constexpr int kOffsets = kNative ? 1 : kKc ? (kMixed ? 4 : 2) : kBlocks / 2;
   int o[kOffsets];
   // Tile at byte `at` of the workgroup's LDS, first block at index c0.
   DPC_DEVICE void init(int at, int c0, int lane) {
     const int row = c0 + (lane & 15), q = lane >> 4;
 #pragma unroll
     for (int i = 0; i < kOffsets; ++i) {
-      if (!kKc)
+      if (kNative && kKc)
+        o[i] = at + (c0 >> 4) * 1024 + mm_native_slot(lane & 15, q) * 16;
+      else if (kNative)  // lane L of 16: row 4 q + L / 4, columns 4 (L % 4) ..
+        o[i] = at + (c0 >> 5) * 4096 + mm_native_slot(4 * q + ((lane & 15) >> 2), lane & 3) * 16;
+      else if (!kKc)
         o[i] = at + frag16_off(c0 + 32 * i, 0, lane);
       else if (kMixed)  // i: 2 kk + h
         o[i] = at + mm_kc_off(row, 2 * i + (q >> 1)) + 8 * (q & 1);
@@ -161,6 +178,12 @@ struct MmFrags {
   }
   // Block i, sub-step kk, `off` bytes on (the stage).
   DPC_DEVICE bf16x8_t read(const uint8_t* lds, int i, int kk, int off) const {
+    if (kNative && kKc)
+      return *reinterpret_cast<const bf16x8_t*>(lds + o[0] + off + kk * 16384 + i * 1024);
+    if (kNative) {  // 32 columns: four pieces of 16 rows, two of them this sub-step's
+      const int p = o[0] + off + (i >> 1) * 4096 + (i & 1) * 8 + kk * 2048;
+      return join_frag(read_tr(lds, p), read_tr(lds, p + 1024));
+    }
     if (!kKc) {  // odd blocks are the other half of a 64-byte LDS block
       const int p = (o[i >> 1] ^ (32 * (i & 1))) + off + kk * 32 * kTileRowBytes;
       return join_frag(read_tr(lds, p), read_tr(lds, p + 16 * kTileRowBytes));
@@ -177,18 +200,13 @@ struct MmFrags {
 // nothing reads.
 struct MmPlace {
   int left, pair, k0;
-  DPC_DEVICE void next(int kl) {
-    if (left <= 1) return;
-    --left;
-    k0 += kMmStep;
-    if (k0 >= kl) {
-      k0 = 0;
-      ++pair;
-    }
+  DPC_DEVICE MmPlace next(int kl) const {  // (selects: no branch in the loop)
+    const int go = left > 1 ? 1 : 0, k = k0 + kMmStep, wrap = k >= kl ? 1 : 0;
+    return MmPlace{left - go, pair + (go & wrap), go ? (wrap ? 0 : k) : k0};
   }
 };
 
-// The K loop of one tile: steps of slice `split` into acc.  Two LDS stages of each
+// The K loop of a tile: steps of slice `split` into acc.  Two LDS stages of each
 // operand (A, A, B, B: every read is a lane's offset plus a 16-bit immediate), all
 // transfers straight from memory into LDS.
 //
@@ -198,129 +216,148 @@ struct MmPlace {
 // been read for the last time.  A's transfers of step s + 2 go out right after it,
 // B's of step s + 1 at the start of step s, so each has most of a step or more to
 // land and the barrier is the only place where a wave waits.
-// Ends with a barrier, after which `lds` is free.
-template <bool kAKc, bool kBKc, bool kBBlocked, bool kWideB>
-DPC_DEVICE void mm_loop(const MmArgs& g, int ta, int tb, int split, uint8_t* lds,
-                        MmAcc<kWideB>& acc) {
-  const int tid = threadIdx.x, lane = tid & 63,
-            w = __builtin_amdgcn_readfirstlane(tid >> 6);
-#pragma unroll
-  for (int i = 0; i < MmAcc<kWideB>::kA; ++i)
-#pragma unroll
-    for (int j = 0; j < MmAcc<kWideB>::kB; ++j) acc.v[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const int ks = max(1, (g.kl + kMmStep - 1) / kMmStep);
-  const long long n = mm_steps(g);
-  const int s0 = (int)(n * split / g.splits), s1 = (int)(n * (split + 1) / g.splits);
-  const int steps = __builtin_amdgcn_readfirstlane(s1 - s0);
-  if (steps <= 0) return;
-  const int pair0 = __builtin_amdgcn_readfirstlane(s0 / ks);
-  MmPlace pa = {steps, g.planes == 1 ? 5 : pair0, (s0 - pair0 * ks) * kMmStep}, pb = pa;
+//
+// begin() sends the first transfers, run() does the rest and ends with a barrier,
+// after which `lds` is free: the next tile's begin() goes before this one's epilogue,
+// so that its first step has arrived when the epilogue ends.
+template <bool kAKc, bool kBKc, bool kBNative, bool kWideB>
+struct MmTile {
+  const MmArgs& g;
+  uint8_t* lds;
+  int lane, w, ta, tb, steps;
+  MmPlace pa, pb;
   MmStage<kAKc, false> sa;
-  MmStage<kBKc, kBBlocked> sb;
-  sa.init(g.a, w, lane);
-  sb.init(g.b, w, lane);
-  constexpr bool kMixed = kAKc != kBKc;
+  MmStage<kBKc, kBNative> sb;
   u32x4_t buf;
   int bad;
-  auto next_a = [&]() __attribute__((always_inline)) {
+
+  DPC_DEVICE MmTile(const MmArgs& args, uint8_t* l) : g(args), lds(l) {
+    lane = threadIdx.x & 63;
+    w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    sa.init(g.a, w, lane);
+    sb.init(g.b, w, lane);
+  }
+  DPC_DEVICE void next_a() {
     buf = sa.buffer(g.a, (kMmPairsA >> (4 * pa.pair)) & 15, ta, pa.k0, g.kl, &bad);
-    pa.next(g.kl);
-  };
-  auto next_b = [&]() __attribute__((always_inline)) {
+    pa = pa.next(g.kl);
+  }
+  DPC_DEVICE void next_b() {
     buf = sb.buffer(g.b, (kMmPairsB >> (4 * pb.pair)) & 15, tb, pb.k0, g.kl, &bad);
-    pb.next(g.kl);
-  };
-  auto fetch_a = [&](int stage, int j) __attribute__((always_inline)) {
+    pb = pb.next(g.kl);
+  }
+  DPC_DEVICE void fetch_a(int stage, int j) {
     sa.issue(buf, bad, lds_addr(lds) + stage * kMmOperandBytes, w, j);
-  };
-  auto fetch_b = [&](int stage, int j) __attribute__((always_inline)) {
+  }
+  DPC_DEVICE void fetch_b(int stage, int j) {
     sb.issue(buf, bad, lds_addr(lds) + (2 + stage) * kMmOperandBytes, w, j);
-  };
-  // x: the wide operand's fragments (half of its blocks), y: the narrow one's.
-  bf16x8_t x0[4], x1[4], y0[4], y1[4];
-  MmFrags<kAKc, kMixed, MmAcc<kWideB>::kA> ra;
-  MmFrags<kBKc, kMixed, MmAcc<kWideB>::kB> rb;
-  ra.init(0, acc.row0(w), lane);
-  rb.init(2 * kMmOperandBytes, acc.col0(w), lane);
-  auto read_x = [&](int stage, int kk, int half, bf16x8_t* f, int i) __attribute__((always_inline)) {
-    if constexpr (kWideB)
-      f[i] = rb.read(lds, 4 * half + i, kk, stage * kMmOperandBytes);
-    else
-      f[i] = ra.read(lds, 4 * half + i, kk, stage * kMmOperandBytes);
-  };
-  auto read_y = [&](int stage, int kk, bf16x8_t* f, int i) __attribute__((always_inline)) {
-    if constexpr (kWideB)
-      f[i] = ra.read(lds, i, kk, stage * kMmOperandBytes);
-    else
-      f[i] = rb.read(lds, i, kk, stage * kMmOperandBytes);
-  };
-  // One phase: 16 MFMAs, and after MFMA m what slot(m) issues (a fragment of the next
-  // phase, a transfer); the order is the one written.
-  auto phase = [&](const bf16x8_t* x, const bf16x8_t* y, int half, auto slot)
-      __attribute__((always_inline)) {
-#pragma unroll
-    for (int m = 0; m < 16; ++m) {
-      const int i = m >> 2, j = m & 3;
-      if constexpr (kWideB)
-        acc.v[j][4 * half + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            y[j], x[i], acc.v[j][4 * half + i], 0, 0, 0);
-      else
-        acc.v[4 * half + i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            x[i], y[j], acc.v[4 * half + i][j], 0, 0, 0);
-      slot(m);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-  auto step = [&](int cur, int nxt) __attribute__((always_inline)) {
-    next_b();
-    __builtin_amdgcn_sched_barrier(0);
-    phase(x0, y0, 0, [&](int m) __attribute__((always_inline)) {
-      if (m % 2 == 0 && m < 8) read_x(cur, 0, 1, x1, m / 2);
-      if (m % 4 == 3) fetch_b(nxt, m / 4);
-    });
-    phase(x1, y0, 1, [&](int m) __attribute__((always_inline)) {
-      if (m < 8) {
-        if (m & 1) read_x(cur, 1, 0, x0, m / 2);
-        else read_y(cur, 1, y1, m / 2);
-      }
-    });
-    phase(x0, y1, 0, [&](int m) __attribute__((always_inline)) {
-      if (m % 2 == 0 && m < 8) read_x(cur, 1, 1, x1, m / 2);
-    });
+  }
+
+  DPC_DEVICE void begin(int tile_a, int tile_b, int split) {
+    ta = tile_a;
+    tb = tile_b;
+    const int ks = max(1, (g.kl + kMmStep - 1) / kMmStep);
+    const long long n = mm_steps(g);
+    const int s0 = (int)(n * split / g.splits), s1 = (int)(n * (split + 1) / g.splits);
+    steps = __builtin_amdgcn_readfirstlane(s1 - s0);
+    if (steps <= 0) return;
+    const int pair0 = __builtin_amdgcn_readfirstlane(s0 / ks);
+    pa = MmPlace{steps, g.planes == 1 ? 5 : pair0, (s0 - pair0 * ks) * kMmStep};
+    pb = pa;
     next_a();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fetch_a(0, j);
+    next_b();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fetch_b(0, j);
+    next_a();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) fetch_a(1, j);
+  }
+
+  DPC_DEVICE void run(MmAcc<kWideB>& acc) {
+#pragma unroll
+    for (int i = 0; i < MmAcc<kWideB>::kA; ++i)
+#pragma unroll
+      for (int j = 0; j < MmAcc<kWideB>::kB; ++j) acc.v[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if (steps <= 0) return;
+    constexpr bool kMixed = kAKc != kBKc;
+    // x: the wide operand's fragments (half of its blocks), y: the narrow one's.
+    bf16x8_t x0[4], x1[4], y0[4], y1[4];
+    MmFrags<kAKc, false, kMixed, MmAcc<kWideB>::kA> ra;
+    MmFrags<kBKc, kBNative, kMixed, MmAcc<kWideB>::kB> rb;
+    ra.init(0, acc.row0(w), lane);
+    rb.init(2 * kMmOperandBytes, acc.col0(w), lane);
+    auto read_x = [&](int stage, int kk, int half, bf16x8_t* f, int i) __attribute__((always_inline)) {
+      if constexpr (kWideB)
+        f[i] = rb.read(lds, 4 * half + i, kk, stage * kMmOperandBytes);
+      else
+        f[i] = ra.read(lds, 4 * half + i, kk, stage * kMmOperandBytes);
+    };
+    auto read_y = [&](int stage, int kk, bf16x8_t* f, int i) __attribute__((always_inline)) {
+      if constexpr (kWideB)
+        f[i] = ra.read(lds, i, kk, stage * kMmOperandBytes);
+      else
+        f[i] = rb.read(lds, i, kk, stage * kMmOperandBytes);
+    };
+    // One phase: 16 MFMAs, and after MFMA m what slot(m) issues (a fragment of the next
+    // phase, a transfer); the order is the one written.
+    auto phase = [&](const bf16x8_t* x, const bf16x8_t* y, int half, auto slot)
+        __attribute__((always_inline)) {
+#pragma unroll
+      for (int m = 0; m < 16; ++m) {
+        const int i = m >> 2, j = m & 3;
+        if constexpr (kWideB)
+          acc.v[j][4 * half + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              y[j], x[i], acc.v[j][4 * half + i], 0, 0, 0);
+        else
+          acc.v[4 * half + i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              x[i], y[j], acc.v[4 * half + i][j], 0, 0, 0);
+        slot(m);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    auto step = [&](int cur, int nxt) __attribute__((always_inline)) {
+      next_b();
+      __builtin_amdgcn_sched_barrier(0);
+      phase(x0, y0, 0, [&](int m) __attribute__((always_inline)) {
+        if (m % 2 == 0 && m < 8) read_x(cur, 0, 1, x1, m / 2);
+        if (m % 4 == 3) fetch_b(nxt, m / 4);
+      });
+      phase(x1, y0, 1, [&](int m) __attribute__((always_inline)) {
+        if (m < 8) {
+          if (m & 1) read_x(cur, 1, 0, x0, m / 2);
+          else read_y(cur, 1, y1, m / 2);
+        }
+      });
+      phase(x0, y1, 0, [&](int m) __attribute__((always_inline)) {
+        if (m % 2 == 0 && m < 8) read_x(cur, 1, 1, x1, m / 2);
+      });
+      next_a();
+      DPC_WAIT_VMCNT(0);
+      __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
+      phase(x1, y1, 1, [&](int m) __attribute__((always_inline)) {
+        if (m < 8) {
+          if (m & 1) read_x(nxt, 0, 0, x0, m / 2);
+          else read_y(nxt, 0, y0, m / 2);
+        }
+        if (m % 4 == 3) fetch_a(cur, m / 4);
+      });
+    };
+    DPC_WAIT_VMCNT(4);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      read_y(0, 0, y0, j);
+      read_x(0, 0, 0, x0, j);
+    }
+    int s = 0;
+    for (; s + 1 < steps; s += 2) {
+      step(0, 1);
+      step(1, 0);
+    }
+    if (s < steps) step(0, 1);
     DPC_WAIT_VMCNT(0);
     __syncthreads();
-    __builtin_amdgcn_sched_barrier(0);
-    phase(x1, y1, 1, [&](int m) __attribute__((always_inline)) {
-      if (m < 8) {
-        if (m & 1) read_x(nxt, 0, 0, x0, m / 2);
-        else read_y(nxt, 0, y0, m / 2);
-      }
-      if (m % 4 == 3) fetch_a(cur, m / 4);
-    });
-  };
-  next_a();
-#pragma unroll
-  for (int j = 0; j < 4; ++j) fetch_a(0, j);
-  next_b();
-#pragma unroll
-  for (int j = 0; j < 4; ++j) fetch_b(0, j);
-  next_a();
-#pragma unroll
-  for (int j = 0; j < 4; ++j) fetch_a(1, j);
-  DPC_WAIT_VMCNT(4);
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    read_y(0, 0, y0, j);
-    read_x(0, 0, 0, x0, j);
   }
-  int s = 0;
-  for (; s + 1 < steps; s += 2) {
-    step(0, 1);
-    step(1, 0);
-  }
-  if (s < steps) step(0, 1);
-  DPC_WAIT_VMCNT(0);
-  __syncthreads();
-}
+};
