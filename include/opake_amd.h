@@ -542,7 +542,7 @@ int dpc_row_sum_f64(const double* x, int B, int n, int accumulate, double* out, 
  * products.  It takes the same arguments, grad_loss [N] (the gradient of the losses;
  * not used where there is no target) and writes, where not NULL, hidden_grad [N, D]
  * and weight_grad [V, D] in `dtype`, 16-byte aligned, rounded once from float32 sums.
- * `state` is not changed.  All results are deterministic.  K <= 65536, V <= 2^21.
+ * `state` is not changed.  All results are deterministic.  K <= 65536, V <= 2^19.
  * -------------------------------------------------------------------------*/
 size_t dpc_head_loss_state_bytes(int64_t N, int D, int V, int K, int dtype, int want_hidden,
                                  int want_weight);

@@ -146,14 +146,19 @@ __global__ void __launch_bounds__(1024) rows_kernel(const int64_t* __restrict__ 
   if (tid == 0) *rows.count = (int32_t)base;
 }
 
-// The entries of 256 consecutive numbered rows (one B tile) sorted by the 256-wide
-// piece of the vocabulary that they fall into, so that a tile finds its own at
-// start[tile] .. start[tile + 1] - 1 of the block's list.
+// The entries of 256 consecutive numbered rows (one B tile) sorted by the part of a
+// tile that they fall into: 256 columns, and of those the wave whose accumulators hold
+// the entry (wave w: columns (w & 1) * 128, rows (w >> 1) * 64).  Wave w of tile t finds
+// its own at start[8 t + w] .. start[8 t + w + 1] - 1 of the block's list.
 struct Entries {
   int32_t* cols;    // [rows, K]: the column; -1: absent, -2: outside the vocabulary
   uint2* list;      // [blocks][256 K]: {row in block * K + k, row in block << 8 | column in tile}
-  int32_t* start;   // [blocks][tiles + 1]
+  int32_t* start;   // [blocks][8 tiles + 1]
 };
+
+DPC_DEVICE int entry_part(int row, int col) {
+  return (col >> 8) * 8 + ((row >> 6) << 1 | ((col >> 7) & 1));
+}
 
 // Operands as the tiles read them, in planes of bf16 rows padded with zeros: the
 // rows with a target of `hidden` (bf16 rows of whole 16-byte chunks: only if some
@@ -170,11 +175,12 @@ struct PrepArgs {
   bool pack;
   const int64_t* index;
   bool teacher;
-  int blocks, tiles;
+  int blocks, parts;
   Entries entries;
   void* zero;          // the hidden gradient, whose rows without a target are zeroed
   const float* g;      // backward: the losses' gradient,
-  float* gmax;         // and its largest magnitude that is finite (1 if all are 0)
+  float* gmax;         // its largest magnitude that is finite (1 if all are 0), and
+  float* g_over;       // [rows]: the gradient over that, by the rows' numbers
 };
 
 DPC_DEVICE void pack_chunk(const void* src, int dtype, int64_t row, int D, int c, int64_t ld,
@@ -206,7 +212,7 @@ DPC_DEVICE void pack_chunk(const void* src, int dtype, int64_t row, int D, int c
 }
 
 constexpr int kPrepThreads = 512;
-constexpr int kMaxTiles = 1 << 13;  // of the vocabulary (lists' counters in LDS)
+constexpr int kMaxTiles = 1 << 11;  // of the vocabulary (8 counters each in LDS)
 
 // i / K for i < 2^24 (exact in float; the quotient is off by one at most).
 DPC_DEVICE int row_of(int i, int K, float inv) {
@@ -226,7 +232,7 @@ DPC_DEVICE void list_entries(const PrepArgs& a, int block, int64_t count, int* c
   const float inv = 1.0f / (float)a.K;
   const int32_t* active = a.rows.active + first;
   int32_t* cols = a.entries.cols + first * a.K;
-  for (int t = tid; t <= a.tiles; t += kPrepThreads) counter[t] = 0;
+  for (int t = tid; t <= a.parts; t += kPrepThreads) counter[t] = 0;
   __syncthreads();
   for (int i0 = tid; i0 < n; i0 += kBatch * kPrepThreads) {
     int64_t from[kBatch], x[kBatch];
@@ -244,30 +250,30 @@ DPC_DEVICE void list_entries(const PrepArgs& a, int block, int64_t count, int* c
       if (i >= n) break;
       const int c = a.teacher && x[b] < 0 ? -1 : (x[b] >= 0 && x[b] < a.V ? (int)x[b] : -2);
       cols[i] = c;
-      if (c >= 0) atomicAdd(&counter[(c >> 8) + 1], 1);
+      if (c >= 0) atomicAdd(&counter[entry_part(row_of(i, a.K, inv), c) + 1], 1);
     }
   }
   __syncthreads();
-  if (tid < 64) {  // counts -> starts, 64 tiles at a time
+  if (tid < 64) {  // counts -> starts, 64 at a time
     int base = 0;
-    for (int t0 = 0; t0 <= a.tiles; t0 += 64) {
+    for (int t0 = 0; t0 <= a.parts; t0 += 64) {
       const int t = t0 + tid;
-      const int mine = t <= a.tiles ? counter[t] : 0;
+      const int mine = t <= a.parts ? counter[t] : 0;
       int upto = mine;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
         const int o = __shfl_up(upto, d);
         if (tid >= d) upto += o;
       }
-      if (t <= a.tiles) {
+      if (t <= a.parts) {
         counter[t] = base + upto;
-        a.entries.start[(int64_t)block * (a.tiles + 1) + t] = base + upto;
+        a.entries.start[(int64_t)block * (a.parts + 1) + t] = base + upto;
       }
       base += __shfl(upto, 63);
     }
   }
   __syncthreads();
-  // The order within a tile's entries is that of the atomics: each entry has a place
+  // The order within a part is that of the atomics: each entry has a place
   // of its own in every output, so no result depends on it.
   uint2* list = a.entries.list + first * a.K;
   for (int i0 = tid; i0 < n; i0 += kBatch * kPrepThreads) {
@@ -281,8 +287,9 @@ DPC_DEVICE void list_entries(const PrepArgs& a, int block, int64_t count, int* c
     for (int b = 0; b < kBatch; ++b) {
       const int i = i0 + b * kPrepThreads;
       if (c[b] < 0) continue;
-      const int at = atomicAdd(&counter[c[b] >> 8], 1);
-      list[at] = make_uint2((uint32_t)i, (uint32_t)(row_of(i, a.K, inv) << 8 | (c[b] & 255)));
+      const int r = row_of(i, a.K, inv);
+      const int at = atomicAdd(&counter[entry_part(r, c[b])], 1);
+      list[at] = make_uint2((uint32_t)i, (uint32_t)(r << 8 | (c[b] & 255)));
     }
   }
 }
@@ -306,10 +313,13 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(PrepArgs a) {
     for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
     if ((threadIdx.x & 63) == 0) wave_top[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) {
-      for (int i = 1; i < kPrepThreads / 64; ++i) top = fmaxf(top, wave_top[i]);
-      *a.gmax = top > 0.f ? top : 1.f;
-    }
+    top = wave_top[0];
+    for (int i = 1; i < kPrepThreads / 64; ++i) top = fmaxf(top, wave_top[i]);
+    if (!(top > 0.f)) top = 1.f;
+    if (threadIdx.x == 0) *a.gmax = top;
+#pragma unroll 8
+    for (int64_t i = threadIdx.x; i < count; i += kPrepThreads)
+      a.g_over[i] = a.g[a.rows.active[i]] / top;
   }
   const int64_t t0 = (int64_t)(blockIdx.x - a.blocks) * kPrepThreads + threadIdx.x,
                 step = (int64_t)(gridDim.x - a.blocks) * kPrepThreads;
@@ -382,6 +392,13 @@ DPC_DEVICE int epilogue_lane() {
   return lane;
 }
 
+// Loaded values that have to be there: a later wait for them would also wait for the
+// next tile's transfers, which the compiler does not count.
+template <typename T>
+DPC_DEVICE void arrived(T& x) {
+  asm volatile("" : "+v"(x));
+}
+
 // The block ij / 4, ij % 4 of a wave's accumulators (ij uniform).  The empty asm keeps
 // the cases apart: merged into one load at a computed address they would move the
 // accumulators to memory.
@@ -413,18 +430,13 @@ DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, int N, int
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc.v[i][j] *= s.inv_tau;
   }
-  // Entries: a wave goes through the tile's, 64 at a time, and takes those of its own
-  // rows and columns out of its accumulators one by one.
+  // Entries: taken out of the wave's accumulators one by one.
   for (int e = e0; e < e1; e += 64) {
-    const uint2 x = e == e0 ? first
-                            : (e + lane < e1 ? list[e + lane] : make_uint2(0u, 0xffffffffu));
-    const bool mine = ((x.y >> 7) & 1) == (uint32_t)wm && (x.y >> 14) == (uint32_t)wn;
-    unsigned long long todo = __ballot(mine);
-    while (todo) {
-      const int from = __builtin_ctzll(todo);
-      todo &= todo - 1;
-      const uint32_t y = __builtin_amdgcn_readlane(x.y, from);
-      const uint32_t to = __builtin_amdgcn_readlane(x.x, from);
+    const uint2 x = e == e0 ? first : list[min(e + lane, e1 - 1)];
+    const int here = min(e1 - e, 64);
+    for (int i = 0; i < here; ++i) {
+      const uint32_t y = __builtin_amdgcn_readlane(x.y, i);
+      const uint32_t to = __builtin_amdgcn_readlane(x.x, i);
       const f32x4_t b = acc_block(acc, (int)(((y >> 4) & 7) << 2 | ((y >> 12) & 3)));
       const float v = y & 2 ? (y & 1 ? b[3] : b[2]) : (y & 1 ? b[1] : b[0]);
       if (lane == (int)(((y >> 8) & 15) | ((y >> 2) & 3) << 4)) s.picked[g0 * s.K + to] = v;
@@ -478,7 +490,7 @@ DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, int N, int
 
 template <bool kEmit>
 __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int N = hidden_rows(s.h, &s.mm.b.p);
   s.mm.b.rows = N;
   s.mm.tiles_b = tiles_of(N);
@@ -490,13 +502,15 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
   while (more) {
     ta = ta2;
     tb = tb2;
-    // The tile's entries, its first 64 loaded beside the product.
+    // The wave's entries, the first 64 loaded beside the product.
     const int64_t g0 = s.h.first + (int64_t)tb * kMmTile;  // the first row's number
-    const int32_t* start = s.entries.start + (g0 / kMmTile) * (s.mm.tiles_a + 1) + ta;
+    const int32_t* start = s.entries.start + (g0 / kMmTile) * (8 * s.mm.tiles_a + 1) + 8 * ta + w;
     const uint2* list = s.entries.list + g0 * s.K;
     const int e0 = start[0], e1 = start[1];
-    const uint2 first = e0 + lane < e1 ? list[e0 + lane] : make_uint2(0u, 0xffffffffu);
+    uint2 first = e0 < e1 ? list[min(e0 + lane, e1 - 1)] : make_uint2(0u, 0u);
     tile.run(acc);
+    arrived(first.x);
+    arrived(first.y);
     id += gridDim.x;
     more = mm_tile_of(s.mm, id, &split, &ta2, &tb2);
     if (more) tile.begin(ta2, tb2, 0);
@@ -720,40 +734,40 @@ __global__ void __launch_bounds__(256) head_scale_kernel(const float* __restrict
 struct GradArgs {
   MmArgs mm;  // A = W from the piece's first row, B = H
   Hidden h;
-  const int32_t* active;
   int V, K, tile0, tiles;  // the piece's first tile; tiles of the vocabulary
   float inv_tau;
   Entries entries;
   const float* corr;
   const float* lse;
-  const float* g;     // [N]: the losses' gradient, at the rows' own places
-  const float* gmax;  // dz is held over gmax, so a gradient that is the same for all
-                      // rows (one over the tokens) is not rounded with every value
+  const float* g;     // [rows]: the losses' gradient over the largest: dz is held over that,
+                      // so a gradient that is the same for all rows (one over the tokens)
+                      // is not rounded with every value
   uint16_t* dz;       // [planes], native order
   int64_t ld, plane;  // blocks of a row of them, elements
 };
 
+// dz at an entry's column.
+DPC_DEVICE float entry_change(const GradArgs& s, int tb, uint2 x) {
+  return s.corr[(int64_t)tb * kMmTile * s.K + x.x] * s.g[tb * kMmTile + (x.y >> 8)];
+}
+
 template <int kPlanes>
-DPC_DEVICE void grad_epilogue(const GradArgs& s, MmAcc<false>& acc, int N, int ta, int tb,
-                              const uint2* list, int e0, int e1, uint2 first) {
+DPC_DEVICE void grad_epilogue(const GradArgs& s, MmAcc<false>& acc, int ta, int tb,
+                              const f32x4_t& lse, const f32x4_t& g, const uint2* list, int e0,
+                              int e1, uint2 first, float change) {
   const int lane = epilogue_lane(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
             wm = w & 1, wn = w >> 1;
-  const int vt = s.tile0 + ta, n0 = tb * kMmTile;
-  const int vl = wm * 128 + 4 * (lane >> 4);
-  const int tl = wn * 64 + (lane & 15);
-  const int vleft = s.V - vt * kMmTile - vl;
-  const float gmax = *s.gmax;
+  const int vt = s.tile0 + ta;
+  const int vleft = s.V - vt * kMmTile - wm * 128 - 4 * (lane >> 4);
+  const float c = s.inv_tau * kLog2e;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int n = n0 + tl + 16 * j;
-    const float base = n < N ? s.lse[n] * kLog2e : 0.f;
-    const float g = n < N ? s.g[s.active[n]] / gmax : 0.f;
-    const float c = s.inv_tau * kLog2e;
+    const float base = lse[j] * kLog2e;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        acc.v[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc.v[i][j][r], c, -base)) * g;
+        acc.v[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc.v[i][j][r], c, -base)) * g[j];
   }
   if ((vt + 1) * kMmTile > s.V) {
 #pragma unroll
@@ -791,18 +805,17 @@ DPC_DEVICE void grad_epilogue(const GradArgs& s, MmAcc<false>& acc, int N, int t
     }
   // Entries: put in place by the lane that stored the value.
   for (int e = e0; e < e1; e += 64) {
-    const uint2 x = e == e0 ? first
-                            : (e + lane < e1 ? list[e + lane] : make_uint2(0u, 0xffffffffu));
-    const bool mine = ((x.y >> 7) & 1) == (uint32_t)wm && (x.y >> 14) == (uint32_t)wn;
-    unsigned long long todo = __ballot(mine);
-    const float d = mine ? s.corr[(int64_t)n0 * s.K + x.x] * (s.g[s.active[n0 + (x.y >> 8)]] / gmax)
-                         : 0.f;
-    while (todo) {
-      const int from = __builtin_ctzll(todo);
-      todo &= todo - 1;
-      const uint32_t y = __builtin_amdgcn_readlane(x.y, from);
-      const float v = __builtin_bit_cast(
-          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, d), from));
+    uint2 x = first;
+    float d = change;
+    if (e > e0) {
+      x = list[min(e + lane, e1 - 1)];
+      d = entry_change(s, tb, x);
+    }
+    const int here = min(e1 - e, 64);
+    for (int i = 0; i < here; ++i) {
+      const uint32_t y = __builtin_amdgcn_readlane(x.y, i);
+      const float v =
+          __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, d), i));
       const int c = y & 127, j = (y >> 12) & 3;
       uint16_t* at = out + (c >> 6) * kMmBlock + ((c >> 5) & 1) * 8192 + j * 512 +
                      ((c >> 4) & 1) * 4 + (c & 3);
@@ -817,7 +830,7 @@ DPC_DEVICE void grad_epilogue(const GradArgs& s, MmAcc<false>& acc, int N, int t
 
 template <int kPlanes>
 __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int N = hidden_rows(s.h, &s.mm.b.p);
   s.mm.b.rows = N;
   s.mm.tiles_b = tiles_of(N);
@@ -829,15 +842,29 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
   while (more) {
     ta = ta2;
     tb = tb2;
-    const int32_t* start = s.entries.start + (int64_t)tb * (s.tiles + 1) + s.tile0 + ta;
+    const int32_t* start =
+        s.entries.start + (int64_t)tb * (8 * s.tiles + 1) + 8 * (s.tile0 + ta) + w;
     const uint2* list = s.entries.list + (int64_t)tb * kMmTile * s.K;
     const int e0 = start[0], e1 = start[1];
-    const uint2 first = e0 + lane < e1 ? list[e0 + lane] : make_uint2(0u, 0xffffffffu);
+    uint2 first = e0 < e1 ? list[min(e0 + lane, e1 - 1)] : make_uint2(0u, 0u);
     tile.run(acc);
+    f32x4_t lse, g;
+    float change = e0 < e1 ? entry_change(s, tb, first) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = tb * kMmTile + (w >> 1) * 64 + 16 * j + (lane & 15);
+      lse[j] = n < N ? s.lse[n] : 0.f;
+      g[j] = n < N ? s.g[n] : 0.f;
+    }
+    arrived(first.x);
+    arrived(first.y);
+    arrived(lse);
+    arrived(g);
+    arrived(change);
     id += gridDim.x;
     more = mm_tile_of(s.mm, id, &split, &ta2, &tb2);
     if (more) tile.begin(ta2, tb2, 0);
-    grad_epilogue<kPlanes>(s, acc, N, ta, tb, list, e0, e1, first);
+    grad_epilogue<kPlanes>(s, acc, ta, tb, lse, g, list, e0, e1, first, change);
   }
 }
 
@@ -1033,7 +1060,7 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
     return o;
   };
   const int64_t rows_b = (2 * N + 1) * 4, lse_b = N * 4, corr_b = N * K * 4, list_b = N * K * 8,
-                start_b = (int64_t)p.tiles_n * (p.tiles_v + 1) * 4;
+                start_b = (int64_t)p.tiles_n * (8 * p.tiles_v + 1) * 4;
   const bool keep = (p.want_h || p.want_w) && !p.emit;
   if (p.want_h || p.want_w) p.s_rows = take(rows_b);
   if (keep) {
@@ -1074,7 +1101,7 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
   if (keep) {
     p.b_h = take(p.planes * N * p.ld * 2);
     if (p.pack) p.b_w = take(p.planes * (int64_t)V * p.ld * 2);
-    p.b_g = take(4);
+    p.b_g = take(4 + N * 4);
     const int64_t rows = (int64_t)p.tiles_n * kMmTile;
     int64_t t = kPieceBytes / (p.planes * rows * kMmTile * 2);
     if (t < 1) t = 1;
@@ -1120,7 +1147,7 @@ int operands(const Plan& p, PrepArgs& a, const void* hidden, const void* weight,
   if (p.pack && p.V * p.ld / 8 > items) items = p.V * p.ld / 8;
   int64_t grid = (items + kPrepThreads - 1) / kPrepThreads;
   if (grid > 4096) grid = 4096;
-  const size_t lds = a.blocks ? (size_t)(a.tiles + 1) * 4 : 0;
+  const size_t lds = a.blocks ? (size_t)(a.parts + 1) * 4 : 0;
   hipLaunchKernelGGL(prep_kernel, dim3((unsigned)(a.blocks + grid)), dim3(kPrepThreads), lds, s, a);
   DPC_HIP_CHECK(hipGetLastError());
   *ho = Hidden{p.pack ? nullptr : static_cast<const uint16_t*>(hidden), a.h, a.rows.count, p.N,
@@ -1204,7 +1231,7 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
   q.index = index;
   q.teacher = teacher != nullptr;
   q.blocks = p.tiles_n;
-  q.tiles = p.tiles_v;
+  q.parts = 8 * p.tiles_v;
   q.entries = entries;
   StatsArgs a = {};
   const int rc = operands(p, q, hidden, weight, base + p.f_h, base + p.f_w, s, &a.h, &a.mm.a);
@@ -1330,6 +1357,7 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
   pa.zero = hidden_grad;
   pa.g = grad_loss;
   pa.gmax = reinterpret_cast<float*>(base + p.b_g);
+  pa.g_over = pa.gmax + 1;
   Hidden h;
   MmOperand w;
   const int rc = operands(p, pa, hidden, weight, base + p.b_h, base + p.b_w, s, &h, &w);
@@ -1350,7 +1378,6 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
     GradArgs a = {};
     a.mm = MmArgs{wpiece, hop, (int)p.ld, p.planes, tiles, p.tiles_n, 1};
     a.h = h;
-    a.active = rows.active;
     a.V = V;
     a.K = K;
     a.tile0 = tile0;
@@ -1360,8 +1387,7 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
                         reinterpret_cast<int32_t*>(kept + p.s_start)};
     a.corr = reinterpret_cast<const float*>(kept + p.s_corr);
     a.lse = reinterpret_cast<const float*>(kept + p.s_lse);
-    a.g = grad_loss;
-    a.gmax = pa.gmax;
+    a.g = pa.g_over;
     a.dz = dz;
     a.ld = ldz;
     a.plane = plane;

@@ -28,7 +28,7 @@ from opake_amd import _native as nat
 from opake_amd.exceptions import ConfigurationError, InputTypeError
 from opake_amd.ops import _aligned
 
-MAX_VOCABULARY = 1 << 21
+MAX_VOCABULARY = 1 << 19
 MAX_WIDTH = 1 << 20
 MAX_ENTRIES = 1 << 16  # of the teacher, a token
 
