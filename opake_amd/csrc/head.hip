@@ -34,6 +34,8 @@
 // join and put in place of the tile's value.
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.h"
 #include "mm_tile.h"
 
@@ -399,20 +401,52 @@ DPC_DEVICE void arrived(T& x) {
   asm volatile("" : "+v"(x));
 }
 
-// The block ij / 4, ij % 4 of a wave's accumulators (ij uniform).  The empty asm keeps
-// the cases apart: merged into one load at a computed address they would move the
-// accumulators to memory.
-DPC_DEVICE f32x4_t acc_block(const MmAcc<false>& acc, int ij) {
-  f32x4_t x = acc.v[0][0];
-#define HEAD_CASE(n) case n: x = acc.v[(n) >> 2][(n) & 3]; asm volatile("" : "+v"(x)); break;
-#define HEAD_CASE4(n) HEAD_CASE(n) HEAD_CASE(n + 1) HEAD_CASE(n + 2) HEAD_CASE(n + 3)
-  switch (ij) {
-    HEAD_CASE4(0) HEAD_CASE4(4) HEAD_CASE4(8) HEAD_CASE4(12)
-    HEAD_CASE4(16) HEAD_CASE4(20) HEAD_CASE4(24) HEAD_CASE4(28)
-  }
-#undef HEAD_CASE4
-#undef HEAD_CASE
-  return x;
+// x over lanes l, l ^ 16, l ^ 32, l ^ 48 (the lanes that share a column of the
+// accumulators), in each of them.
+template <typename Op>
+DPC_DEVICE float column_all(float x, Op op) {
+  const uint32_t u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  x = op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const uint32_t v = __float_as_uint(x);
+  const auto t = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return op(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+
+// OR of x over the wave, uniform.
+DPC_DEVICE uint32_t wave_or(uint32_t x) {
+  auto step = [&](auto ctrl) __attribute__((always_inline)) {
+    x |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, false);
+  };
+  step(std::integral_constant<int, 0xB1>());   // quad_perm [1, 0, 3, 2]
+  step(std::integral_constant<int, 0x4E>());   // quad_perm [2, 3, 0, 1]
+  step(std::integral_constant<int, 0x141>());  // row_half_mirror
+  step(std::integral_constant<int, 0x140>());  // row_mirror
+  return __builtin_amdgcn_readlane(x, 0) | __builtin_amdgcn_readlane(x, 16) |
+         __builtin_amdgcn_readlane(x, 32) | __builtin_amdgcn_readlane(x, 48);
+}
+
+// Entry y (row in block << 8 | column in tile) is value r of block i, j of the wave's
+// accumulators in lane from: the values of up to 64 entries, one a lane, by a lane
+// move of each block that holds one.
+DPC_DEVICE float entry_values(const MmAcc<false>& acc, uint32_t y, bool on) {
+  const int block = (int)(((y >> 4) & 7) << 2 | ((y >> 12) & 3));
+  const int from = (int)(((y >> 8) & 15) | ((y >> 2) & 3) << 4) * 4;
+  const uint32_t hit = wave_or(on ? 1u << block : 0u);
+  float v = 0.f;
+#pragma unroll
+  for (int n = 0; n < 32; ++n)
+    if ((hit >> n) & 1) {
+      float b[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float a = acc.v[n >> 2][n & 3][r];
+        b[r] = __int_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_int(a)));
+      }
+      const float x = y & 2 ? (y & 1 ? b[3] : b[2]) : (y & 1 ? b[1] : b[0]);
+      v = block == n ? x : v;
+    }
+  return v;
 }
 
 template <bool kEmit>
@@ -430,17 +464,11 @@ DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, int N, int
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc.v[i][j] *= s.inv_tau;
   }
-  // Entries: taken out of the wave's accumulators one by one.
   for (int e = e0; e < e1; e += 64) {
     const uint2 x = e == e0 ? first : list[min(e + lane, e1 - 1)];
-    const int here = min(e1 - e, 64);
-    for (int i = 0; i < here; ++i) {
-      const uint32_t y = __builtin_amdgcn_readlane(x.y, i);
-      const uint32_t to = __builtin_amdgcn_readlane(x.x, i);
-      const f32x4_t b = acc_block(acc, (int)(((y >> 4) & 7) << 2 | ((y >> 12) & 3)));
-      const float v = y & 2 ? (y & 1 ? b[3] : b[2]) : (y & 1 ? b[1] : b[0]);
-      if (lane == (int)(((y >> 8) & 15) | ((y >> 2) & 3) << 4)) s.picked[g0 * s.K + to] = v;
-    }
+    const bool on = e + lane < e1;
+    const float v = entry_values(acc, x.y, on);
+    if (on) s.picked[g0 * s.K + x.x] = v;
   }
   if (v0 + kMmTile > s.V) {  // past the vocabulary
 #pragma unroll
@@ -453,6 +481,7 @@ DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, int N, int
   }
   f32x2_t* part = s.part + (int64_t)(2 * ta + wm) * s.N + g0 + tl;
   uint16_t* out = s.e + (tb * s.lde + 4 * ta + 2 * wm) * kMmBlock + wn * 2048 + lane * 8;
+  float tops[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float m = -INFINITY;
@@ -460,17 +489,19 @@ DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, int N, int
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) m = fmaxf(m, acc.v[i][j][r]);
-    m = fmaxf(m, __shfl_xor(m, 16));
-    m = fmaxf(m, __shfl_xor(m, 32));
-    const float base = (m == -INFINITY ? 0.f : m) * kLog2e;
-    float sum = 0.f;
+    tops[j] = column_all(m, [](float a, float b) { return fmaxf(a, b); });
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float m = tops[j], base = (m == -INFINITY ? 0.f : m) * kLog2e;
+    float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float e = __builtin_amdgcn_exp2f(fmaf(acc.v[i][j][r], kLog2e, -base));
         acc.v[i][j][r] = e;
-        sum += e;
+        sums[r] += e;
       }
     if constexpr (kEmit) {
 #pragma unroll
@@ -482,8 +513,8 @@ DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, int N, int
         *reinterpret_cast<half8_t*>(out + (p >> 1) * kMmBlock + (p & 1) * 8192 + j * 512) = h;
       }
     }
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
+    const float sum = column_all((sums[0] + sums[1]) + (sums[2] + sums[3]),
+                                 [](float a, float b) { return a + b; });
     if (lane < 16 && n0 + tl + 16 * j < N) part[16 * j] = f32x2_t{m, sum};
   }
 }
