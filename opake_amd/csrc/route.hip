@@ -33,7 +33,9 @@ struct RouteArgs {
 };
 
 DPC_DEVICE float load_logit(const void* p, int64_t i, int dtype) {
-  return (float)load_as_f64(p, i, dtype);
+  if (dtype == DPC_BF16) return bf16_bits_to_f32(global_ptr<const uint16_t>(p)[i]);
+  if (dtype == DPC_F16) return (float)global_ptr<const _Float16>(p)[i];
+  return global_ptr<const float>(p)[i];
 }
 
 // Unsigned order of the float order; 0 for -inf and NaN.  -0 counts as +0.
@@ -72,6 +74,9 @@ struct MinU {
 struct OrU {
   DPC_DEVICE uint32_t operator()(uint32_t a, uint32_t b) const { return a | b; }
 };
+struct AddU {
+  DPC_DEVICE uint32_t operator()(uint32_t a, uint32_t b) const { return a + b; }
+};
 struct MaxF {
   DPC_DEVICE uint32_t operator()(uint32_t a, uint32_t b) const {
     return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
@@ -93,7 +98,8 @@ DPC_DEVICE float row_sum(float x) {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 DPC_DEVICE float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
-DPC_DEVICE float sigmoid(float z) { return 1.0f / (1.0f + fast_exp(-z)); }
+// (The hardware's reciprocal, 1 ulp; of infinity 0.)
+DPC_DEVICE float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-z)); }
 
 // The largest key among key[] and its lowest index (none: 0).
 template <int kLanes, int kVals>
@@ -108,6 +114,107 @@ DPC_DEVICE uint32_t row_first(const uint32_t (&key)[kVals], int lane, int* index
     if (key[v] == m) at = lane + v * kLanes;
   *index = (int)row_all<kLanes>(at, MinU());
   return m;
+}
+
+// The k largest keys in order: lane j's `mine` is the j-th's expert.  Three operations
+// a key and round: whatever equals the round's largest is taken out at once, and its
+// index is the lowest of them.  False where a row has equal keys among its largest
+// (more were taken out than rounds found one): then every round has to take one alone.
+template <int kLanes, int kVals>
+DPC_DEVICE bool choose_distinct(uint32_t (&key)[kVals], int lane, int k, int* mine) {
+  int taken = 0, rounds = 0;
+#pragma unroll
+  for (int v = 0; v < kVals; ++v) taken += key[v] != 0;
+  for (int j = 0; j < k; ++j) {
+    uint32_t m = key[0];
+#pragma unroll
+    for (int v = 1; v < kVals; ++v) m = MaxU()(m, key[v]);
+    m = row_all<kLanes>(m, MaxU());
+    uint32_t at = 0xffffffffu;
+    const uint32_t some = m ? m : 1u;
+#pragma unroll
+    for (int v = kVals - 1; v >= 0; --v) {
+      const bool hit = key[v] == some;
+      at = hit ? (uint32_t)(lane + v * kLanes) : at;
+      key[v] = hit ? 0u : key[v];
+    }
+    rounds += m != 0;
+    at = row_all<kLanes>(at, MinU());
+    if (lane == j && m) *mine = (int)at;
+  }
+#pragma unroll
+  for (int v = 0; v < kVals; ++v) taken -= key[v] != 0;
+  return (int)row_all<kLanes>((uint32_t)taken, AddU()) == rounds;
+}
+
+template <int kLanes, int kVals>
+DPC_DEVICE void choose_any(uint32_t (&key)[kVals], int lane, int k, int* mine) {
+  for (int j = 0; j < k; ++j) {
+    int at;
+    const uint32_t m = row_first<kLanes, kVals>(key, lane, &at);
+    if (lane == j && m) *mine = at;
+#pragma unroll
+    for (int v = 0; v < kVals; ++v)
+      if (lane + v * kLanes == at) key[v] = 0;
+  }
+}
+
+// Groups of kSlots * kLanes experts: group g is key[kSlots g ..] of all the row's
+// lanes, so their best are row maxima that every lane holds.  Keys outside the
+// top_groups best groups become 0.
+template <int kLanes, int kVals, int kSlots>
+DPC_DEVICE void keep_groups(uint32_t (&key)[kVals], int top_groups) {
+  constexpr int kGroups = kVals / kSlots;
+  uint32_t best[kGroups];
+#pragma unroll
+  for (int g = 0; g < kGroups; ++g) {
+    uint32_t m = key[g * kSlots];
+#pragma unroll
+    for (int v = 1; v < kSlots; ++v) m = MaxU()(m, key[g * kSlots + v]);
+    best[g] = row_all<kLanes>(m, MaxU());
+  }
+  uint32_t kept = 0;
+  for (int r = 0; r < top_groups; ++r) {
+    uint32_t m = best[0];
+#pragma unroll
+    for (int g = 1; g < kGroups; ++g) m = MaxU()(m, best[g]);
+    int at = -1;
+#pragma unroll
+    for (int g = kGroups - 1; g >= 0; --g)
+      if (best[g] == m) at = g;
+#pragma unroll
+    for (int g = 0; g < kGroups; ++g)
+      if (g == at) best[g] = 0;
+    kept |= m ? 1u << at : 0u;
+  }
+#pragma unroll
+  for (int v = 0; v < kVals; ++v)
+    if (!((kept >> (v / kSlots)) & 1)) key[v] = 0;
+}
+
+// Groups of any size: each round keeps the group of the largest key outside the kept
+// ones.
+template <int kLanes, int kVals>
+DPC_DEVICE void keep_any_groups(uint32_t (&key)[kVals], int lane, int size, int top_groups) {
+  const uint32_t magic = (1u << 20) / size + 1;  // e / size for e, size <= 1024
+  uint32_t open[kVals];
+  uint32_t kept = 0;  // bit v: key[v]'s group is kept
+#pragma unroll
+  for (int v = 0; v < kVals; ++v) open[v] = key[v];
+  for (int r = 0; r < top_groups; ++r) {
+    int at;
+    const uint32_t m = row_first<kLanes, kVals>(open, lane, &at);
+    const int g = m ? (int)(((uint32_t)at * magic) >> 20) : -1;
+#pragma unroll
+    for (int v = 0; v < kVals; ++v)
+      if ((int)(((uint32_t)(lane + v * kLanes) * magic) >> 20) == g) {
+        open[v] = 0;
+        kept |= 1u << v;
+      }
+  }
+#pragma unroll
+  for (int v = 0; v < kVals; ++v)
+    if (!((kept >> v) & 1)) key[v] = 0;
 }
 
 template <int kLanes, int kVals>
@@ -152,36 +259,24 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
     key[v] = order_key(x);
   }
   if (a.top_groups < a.groups) {
-    // Each round keeps the group of the largest key outside the kept groups.
-    const int size = a.E / a.groups;
-    const uint32_t magic = (1u << 20) / size + 1;  // e / size for e, size <= 1024
-    uint32_t open[kVals];
-    uint32_t kept = 0;  // bit v: key[v]'s group is kept
-#pragma unroll
-    for (int v = 0; v < kVals; ++v) open[v] = key[v];
-    for (int r = 0; r < a.top_groups; ++r) {
-      int at;
-      const uint32_t m = row_first<kLanes, kVals>(open, lane, &at);
-      const int g = m ? (int)(((uint32_t)at * magic) >> 20) : -1;
-#pragma unroll
-      for (int v = 0; v < kVals; ++v)
-        if ((int)(((uint32_t)(lane + v * kLanes) * magic) >> 20) == g) {
-          open[v] = 0;
-          kept |= 1u << v;
-        }
-    }
-#pragma unroll
-    for (int v = 0; v < kVals; ++v)
-      if (!((kept >> v) & 1)) key[v] = 0;
+    const int size = a.E / a.groups, slots = size / kLanes;
+    if (size % kLanes == 0 && kVals >= 2 && slots == 1)
+      keep_groups<kLanes, kVals, 1>(key, a.top_groups);
+    else if (size % kLanes == 0 && kVals >= 4 && slots == 2)
+      keep_groups<kLanes, kVals, kVals >= 4 ? 2 : 1>(key, a.top_groups);
+    else if (size % kLanes == 0 && kVals >= 8 && slots == 4)
+      keep_groups<kLanes, kVals, kVals >= 8 ? 4 : 1>(key, a.top_groups);
+    else
+      keep_any_groups<kLanes, kVals>(key, lane, size, a.top_groups);
   }
   int mine = -1;  // lane j: slot j's expert
-  for (int j = 0; j < a.k; ++j) {
-    int at;
-    const uint32_t m = row_first<kLanes, kVals>(key, lane, &at);
-    if (lane == j && m) mine = at;
+  uint32_t left[kVals];
 #pragma unroll
-    for (int v = 0; v < kVals; ++v)
-      if (lane + v * kLanes == at) key[v] = 0;
+  for (int v = 0; v < kVals; ++v) left[v] = key[v];
+  const bool distinct = choose_distinct<kLanes, kVals>(left, lane, a.k, &mine);
+  if (__any(!distinct)) {
+    mine = -1;
+    choose_any<kLanes, kVals>(key, lane, a.k, &mine);
   }
   float s = 0.0f, w = 0.0f;
   const float zj = mine >= 0 ? load_logit(a.logits, base + mine, a.dtype) : -INFINITY;
@@ -215,55 +310,107 @@ struct RouteGradArgs {
   void* dz;
 };
 
-// One wave a row.  The chosen experts' gradients meet the row's other values in
-// LDS.
-__global__ void __launch_bounds__(256) route_grad_kernel(RouteGradArgs a) {
-  __shared__ float rows[4][1024];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t row = (int64_t)blockIdx.x * 4 + w;
-  const bool in = row < a.N;
-  float* mine = rows[w];
-  for (int e = lane; e < a.E; e += 64) mine[e] = 0.0f;
-  __syncthreads();
-  const bool on = in && lane < a.k && a.experts[row * a.k + lane] >= 0;
-  const int64_t at = row * a.k + lane;
-  const int e = on ? (int)a.experts[at] : 0;
+// The gradient of a chosen expert's logit from its lane's weight gradient; a row's
+// slots lie in kLanes lanes.  `dot`: the sum over them that the dense form takes off.
+template <int kLanes>
+DPC_DEVICE float chosen_grad(const RouteGradArgs& a, int64_t row, int slot, bool in, int* expert,
+                             float* dot) {
+  const int64_t at = row * a.k + slot;
+  *expert = in && slot < a.k ? (int)a.experts[at] : -1;
+  const bool on = *expert >= 0;
   const float g = on ? a.g[at] * a.scale : 0.0f;
   // The weight without its scale; a sigmoid again from its logit.
   const float share = on && a.scale != 0.0f ? a.weights[at] / a.scale : 0.0f;
-  const float s =
-      !a.sigmoid ? share : (on ? sigmoid(load_logit(a.logits, row * a.E + e, a.dtype)) : 0.0f);
+  const float s = !a.sigmoid ? share
+                             : (on ? sigmoid(load_logit(a.logits, row * a.E + *expert, a.dtype))
+                                   : 0.0f);
   float x = g;
-  const float dot = row_sum<64>(g * (a.renormalize ? share : s));
+  *dot = row_sum<kLanes>(g * (a.renormalize ? share : s));
   if (a.renormalize) {
-    x = g - dot;
+    x = g - *dot;
     if (a.sigmoid) {
-      const float sum = row_sum<64>(s);
+      const float sum = row_sum<kLanes>(s);
       x = sum != 0.0f ? x / sum : 0.0f;
     } else {
       x *= share;
     }
   }
-  if (a.sigmoid) x *= s * (1.0f - s);
-  if (on) mine[e] = x;
+  return a.sigmoid ? x * (s * (1.0f - s)) : x;
+}
+
+// All but the softmax's own weights: only the chosen logits have a gradient.  A
+// workgroup writes whole rows, zeros and all, from LDS in 16-byte stores: `rows` of
+// them (a multiple of 8, so that they are whole 16-byte chunks).
+template <int kLanes>
+__global__ void __launch_bounds__(256) route_sparse_grad_kernel(RouteGradArgs a, int rows) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t tile[];
+  const int lane = threadIdx.x % kLanes;
+  const int64_t row0 = (int64_t)blockIdx.x * rows;
+  const int here = (int)(a.N - row0 < rows ? a.N - row0 : rows);
+  const int esz = a.dtype == DPC_F32 ? 4 : 2, bytes = rows * a.E * esz;
+  for (int i = threadIdx.x * 16; i < bytes; i += 256 * 16)
+    *reinterpret_cast<u32x4_t*>(tile + i) = u32x4_t{0u, 0u, 0u, 0u};
   __syncthreads();
-  if (!in) return;
-  float top = -INFINITY, inv = 0.0f;
-  const bool dense = !a.sigmoid && !a.renormalize;
-  if (dense) {
-    for (int i = lane; i < a.E; i += 64) top = fmaxf(top, load_logit(a.logits, row * a.E + i, a.dtype));
-    top = row_max<64>(top);
-    top = top > -INFINITY ? top : 0.0f;
-    float sum = 0.0f;
-    for (int i = lane; i < a.E; i += 64)
-      sum += fast_exp(load_logit(a.logits, row * a.E + i, a.dtype) - top);
-    sum = row_sum<64>(sum);
-    inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+  for (int r = threadIdx.x / kLanes; r < rows; r += 256 / kLanes) {
+    int e;
+    float dot;
+    const float x = chosen_grad<kLanes>(a, row0 + r, lane, r < here, &e, &dot);
+    if (e >= 0) {
+      if (a.dtype == DPC_F32)
+        reinterpret_cast<float*>(tile)[r * a.E + e] = x;
+      else if (a.dtype == DPC_BF16)
+        reinterpret_cast<uint16_t*>(tile)[r * a.E + e] = f32_to_bf16_bits(x);
+      else
+        reinterpret_cast<_Float16*>(tile)[r * a.E + e] = (_Float16)x;
+    }
   }
-  for (int i = lane; i < a.E; i += 64) {
-    float y = mine[i];
-    if (dense) y = fast_exp(load_logit(a.logits, row * a.E + i, a.dtype) - top) * inv * (y - dot);
-    store_from_f64(a.dz, row * a.E + i, (double)y, a.dtype);
+  __syncthreads();
+  uint8_t* out = static_cast<uint8_t*>(a.dz) + row0 * a.E * esz;
+  const int whole = here * a.E * esz;
+  for (int i = threadIdx.x * 16; i < whole; i += 256 * 16) {
+    if (i + 16 <= whole)
+      *reinterpret_cast<u32x4_t*>(out + i) = *reinterpret_cast<const u32x4_t*>(tile + i);
+    else
+      for (int b = i; b < whole; b += 2)
+        *reinterpret_cast<uint16_t*>(out + b) = *reinterpret_cast<const uint16_t*>(tile + b);
+  }
+}
+
+// The softmax's own weights: every logit of the row has one, p_e (y_e - dot), y the
+// chosen experts' gradients.  kLanes lanes a row.
+template <int kLanes>
+__global__ void __launch_bounds__(256) route_dense_grad_kernel(RouteGradArgs a) {
+  extern __shared__ float chosen[];  // [256 / kLanes][E]
+  const int lane = threadIdx.x % kLanes, r = threadIdx.x / kLanes;
+  const int64_t row = (int64_t)blockIdx.x * (256 / kLanes) + r;
+  const bool in = row < a.N;
+  float* y = chosen + r * a.E;
+  for (int e = lane; e < a.E; e += kLanes) y[e] = 0.0f;
+  __syncthreads();
+  int e;
+  float dot;
+  const float x = chosen_grad<kLanes>(a, row, lane, in, &e, &dot);
+  if (e >= 0) y[e] = x;
+  __syncthreads();
+  const int E = in ? a.E : 0;
+  float top = -INFINITY, sum = 0.0f;
+  for (int i = lane; i < E; i += kLanes)
+    top = fmaxf(top, load_logit(a.logits, row * a.E + i, a.dtype));
+  top = row_max<kLanes>(top);
+  top = top > -INFINITY ? top : 0.0f;
+  for (int i = lane; i < E; i += kLanes)
+    sum += fast_exp(load_logit(a.logits, row * a.E + i, a.dtype) - top);
+  sum = row_sum<kLanes>(sum);
+  const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+  for (int i = lane; i < E; i += kLanes) {
+    const float p = fast_exp(load_logit(a.logits, row * a.E + i, a.dtype) - top) * inv;
+    const float d = p * (y[i] - dot);
+    if (a.dtype == DPC_F32)
+      global_ptr<float>(a.dz)[row * a.E + i] = d;
+    else if (a.dtype == DPC_BF16)
+      global_ptr<uint16_t>(a.dz)[row * a.E + i] = f32_to_bf16_bits(d);
+    else
+      global_ptr<_Float16>(a.dz)[row * a.E + i] = (_Float16)d;
   }
 }
 
@@ -312,8 +459,30 @@ extern "C" int dpc_route_topk_grad(const void* logits, int64_t N, int E, int dty
     return DPC_EINVAL;
   const RouteGradArgs a = {logits, N, E, dtype, k, score == DPC_ROUTE_SIGMOID, renormalize != 0,
                            (float)scale, experts, weights, grad_weights, grad_logits};
-  hipLaunchKernelGGL(route_grad_kernel, dim3((unsigned)((N + 3) / 4)), dim3(256), 0,
-                     (hipStream_t)stream, a);
+  if ((reinterpret_cast<uintptr_t>(grad_logits) & 15) != 0) return DPC_EINVAL;
+  hipStream_t s = (hipStream_t)stream;
+  if (!a.sigmoid && !a.renormalize) {
+    if (k <= 16)
+      hipLaunchKernelGGL((route_dense_grad_kernel<16>), dim3((unsigned)((N + 15) / 16)), dim3(256),
+                         16 * E * 4, s, a);
+    else
+      hipLaunchKernelGGL((route_dense_grad_kernel<64>), dim3((unsigned)((N + 3) / 4)), dim3(256),
+                         4 * E * 4, s, a);
+  } else {
+    // Rows of about 16 KiB a workgroup, 8 at least.
+    const int esz = dtype == DPC_F32 ? 4 : 2;
+    int rows = 16384 / (E * esz) / 8 * 8;
+    rows = rows < 8 ? 8 : (rows > 256 ? 256 : rows);
+    const dim3 grid((unsigned)((N + rows - 1) / rows));
+    if (k <= 4)
+      hipLaunchKernelGGL((route_sparse_grad_kernel<4>), grid, dim3(256), rows * E * esz, s, a, rows);
+    else if (k <= 16)
+      hipLaunchKernelGGL((route_sparse_grad_kernel<16>), grid, dim3(256), rows * E * esz, s, a,
+                         rows);
+    else
+      hipLaunchKernelGGL((route_sparse_grad_kernel<64>), grid, dim3(256), rows * E * esz, s, a,
+                         rows);
+  }
   DPC_HIP_CHECK(hipGetLastError());
   return DPC_OK;
 }
