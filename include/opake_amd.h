@@ -530,15 +530,16 @@ int dpc_row_sum_f64(const double* x, int B, int n, int accumulate, double* out, 
  *     a row with no entry above -inf has loss 0.
  * An index outside the vocabulary that is not ignored makes its row's loss
  * (and gradients) NaN.  Sums are float32; float32 operands are multiplied
- * exactly, as three bf16 parts each.
+ * as two fp16 planes each, 2^-24 of a value (and 2^-39 of its row of H's or of W's
+ * largest) away from it.
  *
  * Rows without a target take no part in any product, whatever they hold.
  *
  * want_hidden / want_weight say which gradients will be asked for; `state` then
  * keeps what they need (dpc_head_loss_state_bytes; NULL if neither).  With
- * want_hidden alone and bf16 operands it keeps the hidden gradient itself, for
- * grad_loss 1, in float32.  Otherwise dpc_head_loss_grad computes dz again, in
- * pieces of the vocabulary, held as bf16 (fp32: as three bf16 parts) for the two
+ * want_hidden alone it keeps the hidden gradient itself, for grad_loss 1, in
+ * float32.  Otherwise dpc_head_loss_grad computes dz again, in
+ * pieces of the vocabulary, held as bf16 (fp32: as two fp16 planes) for the two
  * products.  It takes the same arguments, grad_loss [N] (the gradient of the losses;
  * not used where there is no target) and writes, where not NULL, hidden_grad [N, D]
  * and weight_grad [V, D] in `dtype`, 16-byte aligned, rounded once from float32 sums.

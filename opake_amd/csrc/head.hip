@@ -9,6 +9,10 @@
 //   gradient        dz_nv = g_n coef (p_nv - sum_k q_nk [col_nk = v])
 //                   dH = dz W,  dW = dz^T H
 //
+// Logits, lse and their differences are held in units of log 2 (as exp2 takes them), and
+// exponentials are taken of differences that are formed first: exact where a logit is
+// its row's largest, however large it is.
+//
 // Cross entropy is the K = 1, q = 1 case, so both share every kernel.
 //
 // Rows without a target (the ignored index; no teacher entry above -inf) are left
@@ -21,14 +25,14 @@
 // join turns them into lse and the loss.
 //
 // Gradients, in one of two ways:
-//   * the hidden states' alone, bf16 (a frozen head): the rows go in chunks, whose
-//     tiles also leave exp(z - tile's maximum) as fp16.  The join turns a chunk's
-//     rows into p - q (bf16) in place, and one product with W gives dH for g = 1,
-//     kept in float32 until the backward multiplies each row by its g.  Two
-//     products in all instead of three.
+//   * the hidden states' alone (a frozen head): the rows go in chunks, whose tiles also
+//     leave exp(z - half a tile's maximum) as fp16 (float32 inputs: two planes).  A pass
+//     turns the chunk into p - q (bf16, or planes) in place, and one product with W
+//     gives dH for g = 1, kept in float32 until the backward multiplies each row by its
+//     g.  Two products in all instead of three.
 //   * otherwise in the backward, in pieces of the vocabulary: the logits' tiles
 //     again, turned into dz in the accumulators and written as bf16 (float32 inputs:
-//     as three bf16 parts, exact), then the products dz W (added up over the pieces
+//     as two fp16 planes), then the products dz W (added up over the pieces
 //     in float32) and dz^T H.
 // dz at an entry's column, where p and q may cancel, is formed in float32 by the
 // join and put in place of the tile's value.
@@ -41,9 +45,11 @@
 
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
+constexpr double kLog2e64 = 1.44269504088896340736;
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.693147180559945309417f;
 
-DPC_DEVICE float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+DPC_DEVICE float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+DPC_DEVICE float fast_exp(float x) { return exp2_fast(x * kLog2e); }
 
 constexpr int kLdsBytes = 131072;
 __shared__ __attribute__((aligned(16))) uint8_t lds_all[kLdsBytes];
@@ -52,19 +58,24 @@ __shared__ __attribute__((aligned(16))) uint8_t lds_all[kLdsBytes];
 // Rows, entries and operands as the tiles read them.
 // ---------------------------------------------------------------------------
 
-// Plane p (0..2) of x: x0 = bf16(x), x1 = bf16(x - x0), x2 = x - x0 - x1, which
-// sum to x exactly (8 + 8 + 8 bits; parts below the normal range are flushed by
-// the matrix cores).  A value that rounds past the largest bf16 is truncated
-// instead.  Not finite: plane 0 alone carries it.
-DPC_DEVICE uint16_t split_plane(float x, int p) {
-  if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u) return p ? 0 : f32_to_bf16_bits(x);
-  uint16_t b = 0;
-  for (int i = 0; i <= p; ++i) {
-    b = f32_to_bf16_bits(x);
-    if ((b & 0x7f80u) == 0x7f80u) b = (uint16_t)(__float_as_uint(x) >> 16);
-    x -= bf16_bits_to_f32(b);
-  }
-  return b;
+// float32 as two fp16 planes (mm_tile.h): the shift that brings magnitude `top` (the
+// float's bits) to [2^14, 2^15), and plane p of an x that is already shifted.  Values
+// that fp16 holds as subnormals go to the next plane, which starts 2^-11 lower, so
+// nothing depends on whether the matrix cores keep those.
+constexpr int kDzShift = 14;  // of dz, which is at most 1 (its gradient is applied later)
+
+DPC_DEVICE int half_shift(uint32_t top) {
+  const int e = (int)(top >> 23) & 255;
+  return top == 0 ? 0 : 14 + 127 - (e ? e : 1);
+}
+
+DPC_DEVICE float half_part(float x) { return fabsf(x) < 0x1.0p-14f ? 0.f : (float)(_Float16)x; }
+
+DPC_DEVICE uint16_t half_plane(float x, int p) {
+  if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u)  // not finite: plane 0 carries it
+    return p ? 0 : __builtin_bit_cast(uint16_t, (_Float16)x);
+  const float x0 = half_part(x);
+  return __builtin_bit_cast(uint16_t, (_Float16)(p ? half_part((x - x0) * 2048.f) : x0));
 }
 
 // The rows that have a target, in order: count, active[count], and each row's
@@ -73,6 +84,15 @@ struct Rows {
   int32_t* count;
   int32_t* active;
   int32_t* place;
+};
+
+// The largest finite magnitudes that the planes' shifts come from, as bits.  Each row
+// of H has its own for the logits, so that one row's outlier costs the others nothing;
+// dW's sums over rows and W's over the vocabulary take one for the tensor.
+struct Tops {
+  uint32_t* h;
+  uint32_t* w;
+  uint32_t* row;  // [rows with a target]
 };
 
 // Distillation: whether a row has an entry that counts (or one that is wrong: an
@@ -99,7 +119,8 @@ __global__ void __launch_bounds__(256) entries_kernel(const int64_t* __restrict_
 // rows.place holds entries_kernel's flags.
 __global__ void __launch_bounds__(1024) rows_kernel(const int64_t* __restrict__ index,
                                                     int64_t ignore, int flags, int64_t N,
-                                                    Rows rows, float* __restrict__ loss) {
+                                                    Rows rows, float* __restrict__ loss,
+                                                    Tops tops) {
   __shared__ int total[128], before[129];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   int64_t base = 0;
@@ -146,6 +167,7 @@ __global__ void __launch_bounds__(1024) rows_kernel(const int64_t* __restrict__ 
     __syncthreads();
   }
   if (tid == 0) *rows.count = (int32_t)base;
+  if (tid == 0) *tops.h = *tops.w = 0u;
 }
 
 // The entries of 256 consecutive numbered rows (one B tile) sorted by the part of a
@@ -162,7 +184,7 @@ DPC_DEVICE int entry_part(int row, int col) {
   return (col >> 8) * 8 + ((row >> 6) << 1 | ((col >> 7) & 1));
 }
 
-// Operands as the tiles read them, in planes of bf16 rows padded with zeros: the
+// Operands as the tiles read them, in planes of 16-bit rows padded with zeros: the
 // rows with a target of `hidden` (bf16 rows of whole 16-byte chunks: only if some
 // are left out, else the tiles read the caller's own) and, where it needs planes or
 // padding, the weight.  The first `blocks` workgroups make the entries' lists.
@@ -175,6 +197,8 @@ struct PrepArgs {
   uint16_t* h;
   uint16_t* w;
   bool pack;
+  Tops tops;     // float32
+  uint16_t* hg;          // float32, for dW: planes of H times the losses' gradient over gmax
   const int64_t* index;
   bool teacher;
   int blocks, parts;
@@ -186,30 +210,92 @@ struct PrepArgs {
 };
 
 DPC_DEVICE void pack_chunk(const void* src, int dtype, int64_t row, int D, int c, int64_t ld,
-                           int64_t plane, uint16_t* dst, int64_t to) {
-  const int planes = dtype == DPC_F32 ? 3 : 1;
+                           int64_t plane, uint16_t* dst, int64_t to, int shift, float times) {
   float x[8];
-  uint16_t h[8];
+  u32x4_t o;
+  if (dtype == DPC_BF16) {
+    uint16_t h[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    x[e] = 0.f;
-    h[e] = 0;
-    if (c + e < D) {
-      if (dtype == DPC_F32)
-        x[e] = static_cast<const float*>(src)[row * D + c + e];
-      else
-        h[e] = static_cast<const uint16_t*>(src)[row * D + c + e];
+    for (int e = 0; e < 8; ++e)
+      h[e] = c + e < D ? static_cast<const uint16_t*>(src)[row * D + c + e] : (uint16_t)0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = (uint32_t)h[2 * e] | ((uint32_t)h[2 * e + 1] << 16);
+    *reinterpret_cast<u32x4_t*>(dst + to * ld + c) = o;
+    return;
+  }
+  const float* from = static_cast<const float*>(src) + row * D + c;
+  if (D % 8 == 0 && ((uintptr_t)src & 15) == 0) {
+    const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(from),
+                  hi = *reinterpret_cast<const f32x4_t*>(from + 4);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = e < 4 ? lo[e] : hi[e - 4];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = c + e < D ? from[e] : 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = ldexpf(x[e] * times, shift);
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      o[e] = (uint32_t)half_plane(x[2 * e], p) | ((uint32_t)half_plane(x[2 * e + 1], p) << 16);
+    *reinterpret_cast<u32x4_t*>(dst + p * plane + to * ld + c) = o;
+  }
+}
+
+DPC_DEVICE uint32_t finite_bits(float x) {
+  const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
+  return u < 0x7f800000u ? u : 0u;
+}
+
+DPC_DEVICE uint32_t wave_max_bits(uint32_t x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x = max(x, (uint32_t)__shfl_xor((int)x, d));
+  return x;
+}
+
+// blockIdx.y 0: H's rows with a target, one wave a row; 1: W.  (Maxima: any order gives
+// the same.)
+__global__ void __launch_bounds__(256) tops_kernel(const float* __restrict__ hidden,
+                                                   const float* __restrict__ weight, int D, int V,
+                                                   Rows rows, Tops tops) {
+  __shared__ uint32_t waves[4];
+  const int lane = threadIdx.x & 63;
+  const bool of_w = blockIdx.y == 1;
+  uint32_t top = 0;
+  if (of_w) {
+    const int64_t n = V * (int64_t)D, t0 = (int64_t)blockIdx.x * 256 + threadIdx.x,
+                  step = (int64_t)gridDim.x * 256;
+    const int64_t whole = ((uintptr_t)weight & 15) == 0 ? n / 4 : 0;
+#pragma unroll 4
+    for (int64_t i = t0; i < whole; i += step) {
+      const f32x4_t x = reinterpret_cast<const f32x4_t*>(weight)[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = max(top, finite_bits(x[e]));
+    }
+#pragma unroll 4
+    for (int64_t i = 4 * whole + t0; i < n; i += step) top = max(top, finite_bits(weight[i]));
+    top = wave_max_bits(top);
+  } else {
+    const int64_t count = *rows.count;
+    for (int64_t c = blockIdx.x * 4ll + (threadIdx.x >> 6); c < count; c += gridDim.x * 4ll) {
+      const float* x = hidden + (int64_t)rows.active[c] * D;
+      uint32_t mine = 0;
+#pragma unroll 4
+      for (int d = lane; d < D; d += 64) mine = max(mine, finite_bits(x[d]));
+      mine = wave_max_bits(mine);
+      if (lane == 0) tops.row[c] = mine;
+      top = max(top, mine);
     }
   }
-  for (int p = 0; p < planes; ++p) {
-    u32x4_t o;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint16_t a = planes == 1 ? h[2 * e] : split_plane(x[2 * e], p);
-      const uint16_t b = planes == 1 ? h[2 * e + 1] : split_plane(x[2 * e + 1], p);
-      o[e] = (uint32_t)a | ((uint32_t)b << 16);
-    }
-    *reinterpret_cast<u32x4_t*>(dst + p * plane + to * ld + c) = o;
+  // One atomic a workgroup: those of a word go one after the other (2048 of them took
+  // 40 us).
+  if (lane == 0) waves[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    top = max(max(waves[0], waves[1]), max(waves[2], waves[3]));
+    if (top) atomicMax(of_w ? tops.w : tops.h, top);
   }
 }
 
@@ -296,6 +382,32 @@ DPC_DEVICE void list_entries(const PrepArgs& a, int block, int64_t count, int* c
   }
 }
 
+// The losses' gradient over its largest finite magnitude, by one workgroup.
+DPC_DEVICE void over_gmax(const PrepArgs& a, int64_t count) {
+  __shared__ float wave_top[kPrepThreads / 64];
+  float top = 0.f;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < count; i += kPrepThreads) {
+    const float x = fabsf(a.g[a.rows.active[i]]);
+    if (x < INFINITY) top = fmaxf(top, x);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  if ((threadIdx.x & 63) == 0) wave_top[threadIdx.x >> 6] = top;
+  __syncthreads();
+  top = wave_top[0];
+  for (int i = 1; i < kPrepThreads / 64; ++i) top = fmaxf(top, wave_top[i]);
+  if (!(top > 0.f)) top = 1.f;
+  if (threadIdx.x == 0) *a.gmax = top;
+#pragma unroll 8
+  for (int64_t i = threadIdx.x; i < count; i += kPrepThreads)
+    a.g_over[i] = a.g[a.rows.active[i]] / top;
+}
+
+__global__ void __launch_bounds__(kPrepThreads) gmax_kernel(PrepArgs a) {
+  over_gmax(a, *a.rows.count);
+}
+
 __global__ void __launch_bounds__(kPrepThreads) prep_kernel(PrepArgs a) {
   extern __shared__ int counter[];
   const int64_t count = *a.rows.count;
@@ -303,40 +415,27 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(PrepArgs a) {
     list_entries(a, blockIdx.x, count, counter);
     return;
   }
-  if (a.g && blockIdx.x == 0) {
-    __shared__ float wave_top[kPrepThreads / 64];
-    float top = 0.f;
-#pragma unroll 8
-    for (int64_t i = threadIdx.x; i < count; i += kPrepThreads) {
-      const float x = fabsf(a.g[a.rows.active[i]]);
-      if (x < INFINITY) top = fmaxf(top, x);
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if ((threadIdx.x & 63) == 0) wave_top[threadIdx.x >> 6] = top;
-    __syncthreads();
-    top = wave_top[0];
-    for (int i = 1; i < kPrepThreads / 64; ++i) top = fmaxf(top, wave_top[i]);
-    if (!(top > 0.f)) top = 1.f;
-    if (threadIdx.x == 0) *a.gmax = top;
-#pragma unroll 8
-    for (int64_t i = threadIdx.x; i < count; i += kPrepThreads)
-      a.g_over[i] = a.g[a.rows.active[i]] / top;
-  }
+  if (a.g && !a.hg && blockIdx.x == 0) over_gmax(a, count);
   const int64_t t0 = (int64_t)(blockIdx.x - a.blocks) * kPrepThreads + threadIdx.x,
                 step = (int64_t)(gridDim.x - a.blocks) * kPrepThreads;
   const int64_t chunks = a.ld / 8;
+  const bool f32 = a.dtype == DPC_F32;
+  const int shift_h = f32 ? half_shift(*a.tops.h) : 0, shift_w = f32 ? half_shift(*a.tops.w) : 0;
   if (a.h && (a.pack || count < a.N))
     for (int64_t i = t0; i < count * chunks; i += step) {
       const int64_t c = i / chunks;
-      pack_chunk(a.hidden, a.dtype, a.rows.active[c], a.D, (int)(i - c * chunks) * 8, a.ld,
-                 a.N * a.ld, a.h, c);
+      const int at = (int)(i - c * chunks) * 8;
+      pack_chunk(a.hidden, a.dtype, a.rows.active[c], a.D, at, a.ld, a.N * a.ld, a.h, c,
+                 f32 ? half_shift(a.tops.row[c]) : 0, 1.f);
+      if (a.hg)
+        pack_chunk(a.hidden, a.dtype, a.rows.active[c], a.D, at, a.ld, a.N * a.ld, a.hg, c,
+                   shift_h, a.g_over[c]);
     }
   if (a.weight)
     for (int64_t i = t0; i < a.V * chunks; i += step) {
       const int64_t v = i / chunks;
       pack_chunk(a.weight, a.dtype, v, a.D, (int)(i - v * chunks) * 8, a.ld, (int64_t)a.V * a.ld,
-                 a.w, v);
+                 a.w, v, shift_w, 1.f);
     }
   if (a.zero && count < a.N)
     for (int64_t i = t0; i < a.N * a.D; i += step)
@@ -377,14 +476,22 @@ struct StatsArgs {
   MmArgs mm;  // A = W (vocabulary), B = H (rows with a target)
   Hidden h;
   int V, K;
-  float inv_tau;
+  float inv_tau;  // times log2 e
+  Tops tops;
   Entries entries;
   float* picked;   // [rows, K]: z at the entries' columns
   f32x2_t* part;   // [2 tiles_a][N]: maximum and sum of exponentials of each half
   int64_t N;
   uint16_t* e;     // the chunk's exp(z - the half's maximum) as fp16, native order
-  int64_t lde;     // blocks of a row of them
+                   // (float32 inputs: times 2^kDzShift, in two planes)
+  int64_t lde, plane;  // blocks of a row of them, elements
 };
+
+// What a row's products are to be multiplied by (the planes' shifts undone).
+DPC_DEVICE float logit_factor(float inv_tau, uint32_t top_h, uint32_t top_w) {
+  const int n = -(half_shift(top_h) + half_shift(top_w));
+  return ldexpf(inv_tau, max(-126, min(126, n)));
+}
 
 // The lane, of unknown value to the compiler: what an epilogue computes from it would
 // otherwise be kept in registers through the product's loop, which has none to spare.
@@ -449,21 +556,21 @@ DPC_DEVICE float entry_values(const MmAcc<false>& acc, uint32_t y, bool on) {
   return v;
 }
 
-template <bool kEmit>
-DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, int N, int ta, int tb,
-                               int64_t g0, const uint2* list, int e0, int e1, uint2 first) {
+template <bool kEmit, bool kHalf>
+DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, const f32x4_t& factor,
+                               int N, int ta, int tb, int64_t g0, const uint2* list, int e0,
+                               int e1, uint2 first) {
+#pragma clang fp contract(off)  // the difference is of the rounded logit and its maximum
   const int lane = epilogue_lane(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
             wm = w & 1, wn = w >> 1;
   const int v0 = ta * kMmTile, n0 = tb * kMmTile;
   const int vl = wm * 128 + 4 * (lane >> 4);  // + 16 i + r
   const int tl = wn * 64 + (lane & 15);       // + 16 j
   const int vleft = s.V - v0 - vl;
-  if (s.inv_tau != 1.0f) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) acc.v[i][j] *= s.inv_tau;
-  }
+    for (int i = 0; i < 8; ++i) acc.v[i][j] *= kHalf ? factor[j] : s.inv_tau;
   for (int e = e0; e < e1; e += 64) {
     const uint2 x = e == e0 ? first : list[min(e + lane, e1 - 1)];
     const bool on = e + lane < e1;
@@ -493,13 +600,13 @@ DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, int N, int
   }
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float m = tops[j], base = (m == -INFINITY ? 0.f : m) * kLog2e;
+    const float m = tops[j], base = m == -INFINITY ? 0.f : m;
     float sums[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float e = __builtin_amdgcn_exp2f(fmaf(acc.v[i][j][r], kLog2e, -base));
+        const float e = exp2_fast(acc.v[i][j][r] - base);
         acc.v[i][j][r] = e;
         sums[r] += e;
       }
@@ -507,10 +614,22 @@ DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, int N, int
 #pragma unroll
       for (int p = 0; p < 4; ++p) {  // 32 columns: half p % 2 of block p / 2
         typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+        uint16_t* at = out + (p >> 1) * kMmBlock + (p & 1) * 8192 + j * 512;
         half8_t h;
+        if constexpr (kHalf) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) h[r] = (_Float16)acc.v[2 * p + (r >> 2)][j][r & 3];
-        *reinterpret_cast<half8_t*>(out + (p >> 1) * kMmBlock + (p & 1) * 8192 + j * 512) = h;
+          for (int pl = 0; pl < 2; ++pl) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+              h[r] = __builtin_bit_cast(
+                  _Float16, half_plane(ldexpf(acc.v[2 * p + (r >> 2)][j][r & 3], kDzShift), pl));
+            *reinterpret_cast<half8_t*>(at + pl * s.plane) = h;
+          }
+        } else {
+#pragma unroll
+          for (int r = 0; r < 8; ++r) h[r] = (_Float16)acc.v[2 * p + (r >> 2)][j][r & 3];
+          *reinterpret_cast<half8_t*>(at) = h;
+        }
       }
     }
     const float sum = column_all((sums[0] + sums[1]) + (sums[2] + sums[3]),
@@ -519,14 +638,15 @@ DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, int N, int
   }
 }
 
-template <bool kEmit>
+template <bool kEmit, bool kHalf>
 __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int N = hidden_rows(s.h, &s.mm.b.p);
   s.mm.b.rows = N;
   s.mm.tiles_b = tiles_of(N);
-  MmTile<true, true, false, false> tile(s.mm, lds_all);
+  MmTile<true, true, false, false, kHalf> tile(s.mm, lds_all);
   MmAcc<false> acc;
+  const uint32_t top_w = kHalf ? *s.tops.w : 0u;
   int split, ta, tb, ta2, tb2, id = blockIdx.x;
   bool more = mm_tile_of(s.mm, id, &split, &ta2, &tb2);
   if (more) tile.begin(ta2, tb2, 0);
@@ -540,12 +660,23 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
     const int e0 = start[0], e1 = start[1];
     uint2 first = e0 < e1 ? list[min(e0 + lane, e1 - 1)] : make_uint2(0u, 0u);
     tile.run(acc);
+    f32x4_t factor = {};
+    if constexpr (kHalf) {
+      const int late = epilogue_lane();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int n = tb * kMmTile + (w >> 1) * 64 + 16 * j + (late & 15);
+        const uint32_t top = n < N ? s.tops.row[s.h.first + n] : 0u;
+        factor[j] = logit_factor(s.inv_tau, top, top_w);
+      }
+      arrived(factor);
+    }
     arrived(first.x);
     arrived(first.y);
     id += gridDim.x;
     more = mm_tile_of(s.mm, id, &split, &ta2, &tb2);
     if (more) tile.begin(ta2, tb2, 0);
-    stats_epilogue<kEmit>(s, acc, N, ta, tb, g0, list, e0, e1, first);
+    stats_epilogue<kEmit, kHalf>(s, acc, factor, N, ta, tb, g0, list, e0, e1, first);
   }
 }
 
@@ -586,9 +717,9 @@ DPC_DEVICE void join_row(const JoinArgs& a, int64_t n, float lse, int lane) {
     if (c < 0) lse = NAN;
     const float z = c >= 0 ? picked[0] : 0.f;
     if (lane == 0) {
-      a.loss[own] = (lse - z) * a.loss_scale;
+      a.loss[own] = (lse - z) * kLn2 * a.loss_scale;
       a.lse[n] = lse;
-      corr[0] = fast_exp(z - lse) - 1.0f;
+      corr[0] = exp2_fast(z - lse) - 1.0f;
     }
     return;
   }
@@ -616,7 +747,7 @@ DPC_DEVICE void join_row(const JoinArgs& a, int64_t n, float lse, int lane) {
     const int c = k < a.K ? cols[k] : -1;
     const float lq = c >= 0 ? teacher[k] * a.inv_tau - tm - logs : -INFINITY;
     const float q = fast_exp(lq), z = c >= 0 ? picked[k] : 0.f;
-    if (c >= 0 && q != 0.f) loss += q * (lq - (z - lse));
+    if (c >= 0 && q != 0.f) loss += q * (lq - (z - lse) * kLn2);
     // q of every entry of this column: the other entries, 64 at a time.
     float qs = 0.f;
     for (int i0 = 0; i0 < a.K; i0 += 64) {
@@ -631,7 +762,7 @@ DPC_DEVICE void join_row(const JoinArgs& a, int64_t n, float lse, int lane) {
         if (co == c) qs += qo;
       }
     }
-    if (k < a.K) corr[k] = c >= 0 ? fast_exp(z - lse) - qs : 0.f;
+    if (k < a.K) corr[k] = c >= 0 ? exp2_fast(z - lse) - qs : 0.f;
   }
   loss = wave_sum(loss);
   if (bad) lse = NAN;
@@ -657,7 +788,7 @@ __global__ void __launch_bounds__(kJoinThreads) head_join_kernel(JoinArgs a) {
   for (int i = tid >> 4; i < a.parts; i += kJoinThreads / 16) {
     const f32x2_t x = part[i * a.N];
     const float nm = fmaxf(m, x.x), base = nm == -INFINITY ? 0.f : nm;
-    sum = sum * fast_exp(m - base) + x.y * fast_exp(x.x - base);
+    sum = sum * exp2_fast(m - base) + x.y * exp2_fast(x.x - base);
     m = nm;
   }
   stats[tid] = f32x2_t{m, sum};
@@ -665,7 +796,7 @@ __global__ void __launch_bounds__(kJoinThreads) head_join_kernel(JoinArgs a) {
   for (int k = w; k < rows; k += kJoinThreads / 64) {
     const f32x2_t x = lane < 32 ? stats[lane * 16 + k] : f32x2_t{-INFINITY, 0.f};
     const float top = wave_max(x.x), base = top == -INFINITY ? 0.f : top;
-    join_row(a, n0 + k, top + logf(wave_sum(x.y * fast_exp(x.x - base))), lane);
+    join_row(a, n0 + k, top + log2f(wave_sum(x.y * exp2_fast(x.x - base))), lane);
   }
 }
 
@@ -683,9 +814,10 @@ struct FixArgs {
   const float* lse;
   const float* corr;
   uint16_t* e;
-  int64_t lde;
+  int64_t lde, plane;
 };
 
+template <bool kHalf>
 __global__ void __launch_bounds__(kJoinThreads) head_fix_kernel(FixArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int local = blockIdx.x * kJoinRows;  // first row in the chunk
@@ -699,61 +831,92 @@ __global__ void __launch_bounds__(kJoinThreads) head_fix_kernel(FixArgs a) {
   const int64_t n = n0 + min(lane & 15, rows - 1);
   const f32x2_t* top = a.part + (2 * t0 + (w >> 2)) * a.N + n;
   const float lse = a.lse[n];
-  half8_t h[kFixTiles];
+  constexpr int kPlanes = kHalf ? 2 : 1;
+  half8_t h[kFixTiles][kPlanes];
   float f[kFixTiles];
 #pragma unroll
   for (int t = 0; t < kFixTiles; ++t)
     if (t < tiles) {
-      h[t] = *reinterpret_cast<const half8_t*>(at + 4 * t * kMmBlock);
+#pragma unroll
+      for (int pl = 0; pl < kPlanes; ++pl)
+        h[t][pl] = *reinterpret_cast<const half8_t*>(at + pl * a.plane + 4 * t * kMmBlock);
       f[t] = top[2 * t * a.N].x;
     }
 #pragma unroll
   for (int t = 0; t < kFixTiles; ++t)
     if (t < tiles) {
-      const float x = fast_exp(f[t] - lse);
-      u32x4_t o;
+      const float x = exp2_fast(f[t] - lse);
+      uint16_t* to = at + 4 * t * kMmBlock;
+      if constexpr (kHalf) {
+        half8_t o[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        o[e] = f32x2_to_bf16x2_bits((float)h[t][2 * e] * x, (float)h[t][2 * e + 1] * x);
-      *reinterpret_cast<u32x4_t*>(at + 4 * t * kMmBlock) = o;
+        for (int e = 0; e < 8; ++e) {
+          const float y = fmaf((float)h[t][1][e], 0x1.0p-11f, (float)h[t][0][e]) * x;
+#pragma unroll
+          for (int pl = 0; pl < 2; ++pl) o[pl][e] = __builtin_bit_cast(_Float16, half_plane(y, pl));
+        }
+        *reinterpret_cast<half8_t*>(to) = o[0];
+        *reinterpret_cast<half8_t*>(to + a.plane) = o[1];
+      } else {
+        u32x4_t o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[e] = f32x2_to_bf16x2_bits((float)h[t][0][2 * e] * x, (float)h[t][0][2 * e + 1] * x);
+        *reinterpret_cast<u32x4_t*>(to) = o;
+      }
     }
   __syncthreads();
   for (int i = tid; i < rows * a.K; i += kJoinThreads) {
     const int c = a.cols[n0 * a.K + i];
-    if (c >= 0 && (c >> 8) >= t0 && (c >> 8) < t0 + tiles)
-      block[(c >> 6) * kMmBlock + ((c >> 5) & 1) * 8192 + ((c >> 2) & 3) * 128 + (i / a.K) * 8 +
-            ((c >> 4) & 1) * 4 + (c & 3)] = f32_to_bf16_bits(a.corr[n0 * a.K + i]);
+    if (c >= 0 && (c >> 8) >= t0 && (c >> 8) < t0 + tiles) {
+      uint16_t* to = block + (c >> 6) * kMmBlock + ((c >> 5) & 1) * 8192 + ((c >> 2) & 3) * 128 +
+                     (i / a.K) * 8 + ((c >> 4) & 1) * 4 + (c & 3);
+      const float x = a.corr[n0 * a.K + i];
+#pragma unroll
+      for (int pl = 0; pl < kPlanes; ++pl)
+        to[pl * a.plane] = kHalf ? half_plane(ldexpf(x, kDzShift), pl) : f32_to_bf16_bits(x);
+    }
   }
 }
 
 // out row n = unit's row place[n] times g[n] coef; 0 without a target.
 __global__ void __launch_bounds__(256) head_scale_kernel(const float* __restrict__ unit, Rows rows,
                                                          const float* __restrict__ g, float coef,
-                                                         int64_t N, int D,
-                                                         uint16_t* __restrict__ out) {
+                                                         int64_t N, int D, int out_bf16,
+                                                         void* __restrict__ out) {
+  const int64_t t0 = (int64_t)blockIdx.x * 256 + threadIdx.x, step = (int64_t)gridDim.x * 256;
   if (D % 8 == 0) {
     const int chunks = D / 8;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < N * chunks;
-         i += (int64_t)gridDim.x * 256) {
+    for (int64_t i = t0; i < N * chunks; i += step) {
       const int64_t n = i / chunks;
       const int c = (int)(i - n * chunks) * 8;
       const int at = rows.place[n];
-      u32x4_t o = {0u, 0u, 0u, 0u};
+      f32x4_t x = {0.f, 0.f, 0.f, 0.f}, y = x;
       if (at >= 0) {
         const float f = g[n] * coef;
         const f32x4_t* u = reinterpret_cast<const f32x4_t*>(unit + (int64_t)at * D + c);
-        const f32x4_t x = u[0] * f, y = u[1] * f;
-        o = u32x4_t{f32x2_to_bf16x2_bits(x[0], x[1]), f32x2_to_bf16x2_bits(x[2], x[3]),
-                    f32x2_to_bf16x2_bits(y[0], y[1]), f32x2_to_bf16x2_bits(y[2], y[3])};
+        x = u[0] * f;
+        y = u[1] * f;
       }
-      *reinterpret_cast<u32x4_t*>(out + n * D + c) = o;
+      if (out_bf16) {
+        *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(out) + n * D + c) =
+            u32x4_t{f32x2_to_bf16x2_bits(x[0], x[1]), f32x2_to_bf16x2_bits(x[2], x[3]),
+                    f32x2_to_bf16x2_bits(y[0], y[1]), f32x2_to_bf16x2_bits(y[2], y[3])};
+      } else {
+        f32x4_t* o = reinterpret_cast<f32x4_t*>(static_cast<float*>(out) + n * D + c);
+        o[0] = x;
+        o[1] = y;
+      }
     }
   } else {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < N * D;
-         i += (int64_t)gridDim.x * 256) {
+    for (int64_t i = t0; i < N * D; i += step) {
       const int64_t n = i / D;
       const int at = rows.place[n];
-      out[i] = at < 0 ? 0 : f32_to_bf16_bits(unit[at * (int64_t)D + (i - n * D)] * (g[n] * coef));
+      const float x = at < 0 ? 0.f : unit[at * (int64_t)D + (i - n * D)] * (g[n] * coef);
+      if (out_bf16)
+        static_cast<uint16_t*>(out)[i] = f32_to_bf16_bits(x);
+      else
+        static_cast<float*>(out)[i] = x;
     }
   }
 }
@@ -770,35 +933,41 @@ struct GradArgs {
   Entries entries;
   const float* corr;
   const float* lse;
-  const float* g;     // [rows]: the losses' gradient over the largest: dz is held over that,
-                      // so a gradient that is the same for all rows (one over the tokens)
-                      // is not rounded with every value
+  const float* g;     // [rows]: the losses' gradient over the largest: bf16's dz is held over
+                      // that, so a gradient that is the same for all rows (one over the
+                      // tokens) is not rounded with every value.  (float32: dz is held
+                      // without a gradient, which dH's rows and dW's H carry.)
+  Tops tops;
   uint16_t* dz;       // [planes], native order
   int64_t ld, plane;  // blocks of a row of them, elements
 };
 
 // dz at an entry's column.
+template <bool kHalf>
 DPC_DEVICE float entry_change(const GradArgs& s, int tb, uint2 x) {
-  return s.corr[(int64_t)tb * kMmTile * s.K + x.x] * s.g[tb * kMmTile + (x.y >> 8)];
+  const float c = s.corr[(int64_t)tb * kMmTile * s.K + x.x];
+  return kHalf ? ldexpf(c, kDzShift) : c * s.g[tb * kMmTile + (x.y >> 8)];
 }
 
-template <int kPlanes>
+template <bool kHalf>
 DPC_DEVICE void grad_epilogue(const GradArgs& s, MmAcc<false>& acc, int ta, int tb,
                               const f32x4_t& lse, const f32x4_t& g, const uint2* list, int e0,
                               int e1, uint2 first, float change) {
+#pragma clang fp contract(off)  // the forward's rounded logit
   const int lane = epilogue_lane(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
             wm = w & 1, wn = w >> 1;
   const int vt = s.tile0 + ta;
   const int vleft = s.V - vt * kMmTile - wm * 128 - 4 * (lane >> 4);
-  const float c = s.inv_tau * kLog2e;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float base = lse[j] * kLog2e;
+    // g, float32: what the products are to be multiplied by.
+    const float c = kHalf ? g[j] : s.inv_tau;
+    const float by = kHalf ? ldexpf(1.f, kDzShift) : g[j];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        acc.v[i][j][r] = __builtin_amdgcn_exp2f(fmaf(acc.v[i][j][r], c, -base)) * g[j];
+        acc.v[i][j][r] = exp2_fast(acc.v[i][j][r] * c - lse[j]) * by;
   }
   if ((vt + 1) * kMmTile > s.V) {
 #pragma unroll
@@ -816,19 +985,19 @@ DPC_DEVICE void grad_epilogue(const GradArgs& s, MmAcc<false>& acc, int ta, int 
     for (int p = 0; p < 4; ++p) {
       uint16_t* at = out + (p >> 1) * kMmBlock + (p & 1) * 8192 + j * 512;
       const f32x4_t x = acc.v[2 * p][j], y = acc.v[2 * p + 1][j];
-      if (kPlanes == 1) {
+      if (!kHalf) {
         *reinterpret_cast<u32x4_t*>(at) =
             u32x4_t{f32x2_to_bf16x2_bits(x[0], x[1]), f32x2_to_bf16x2_bits(x[2], x[3]),
                     f32x2_to_bf16x2_bits(y[0], y[1]), f32x2_to_bf16x2_bits(y[2], y[3])};
       } else {
 #pragma unroll
-        for (int pl = 0; pl < kPlanes; ++pl) {
+        for (int pl = 0; pl < 2; ++pl) {
           u32x4_t o;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const f32x4_t& z = e < 2 ? x : y;
-            o[e] = split_plane(z[2 * (e & 1)], pl) |
-                   ((uint32_t)split_plane(z[2 * (e & 1) + 1], pl) << 16);
+            const float lo = z[2 * (e & 1)], hi = z[2 * (e & 1) + 1];
+            o[e] = half_plane(lo, pl) | ((uint32_t)half_plane(hi, pl) << 16);
           }
           *reinterpret_cast<u32x4_t*>(at + pl * s.plane) = o;
         }
@@ -840,7 +1009,7 @@ DPC_DEVICE void grad_epilogue(const GradArgs& s, MmAcc<false>& acc, int ta, int 
     float d = change;
     if (e > e0) {
       x = list[min(e + lane, e1 - 1)];
-      d = entry_change(s, tb, x);
+      d = entry_change<kHalf>(s, tb, x);
     }
     const int here = min(e1 - e, 64);
     for (int i = 0; i < here; ++i) {
@@ -852,21 +1021,22 @@ DPC_DEVICE void grad_epilogue(const GradArgs& s, MmAcc<false>& acc, int ta, int 
                      ((c >> 4) & 1) * 4 + (c & 3);
       if (lane == (int)(((y >> 8) & 15) | ((y >> 2) & 3) << 4)) {
 #pragma unroll
-        for (int pl = 0; pl < kPlanes; ++pl)
-          at[pl * s.plane] = kPlanes == 1 ? f32_to_bf16_bits(v) : split_plane(v, pl);
+        for (int pl = 0; pl < (kHalf ? 2 : 1); ++pl)
+          at[pl * s.plane] = kHalf ? half_plane(v, pl) : f32_to_bf16_bits(v);
       }
     }
   }
 }
 
-template <int kPlanes>
+template <bool kHalf>
 __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int N = hidden_rows(s.h, &s.mm.b.p);
   s.mm.b.rows = N;
   s.mm.tiles_b = tiles_of(N);
-  MmTile<true, true, false, false> tile(s.mm, lds_all);
+  MmTile<true, true, false, false, kHalf> tile(s.mm, lds_all);
   MmAcc<false> acc;
+  const uint32_t top_w = kHalf ? *s.tops.w : 0u;
   int split, ta, tb, ta2, tb2, id = blockIdx.x;
   bool more = mm_tile_of(s.mm, id, &split, &ta2, &tb2);
   if (more) tile.begin(ta2, tb2, 0);
@@ -880,12 +1050,15 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
     uint2 first = e0 < e1 ? list[min(e0 + lane, e1 - 1)] : make_uint2(0u, 0u);
     tile.run(acc);
     f32x4_t lse, g;
-    float change = e0 < e1 ? entry_change(s, tb, first) : 0.f;
+    float change = e0 < e1 ? entry_change<kHalf>(s, tb, first) : 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int n = tb * kMmTile + (w >> 1) * 64 + 16 * j + (lane & 15);
       lse[j] = n < N ? s.lse[n] : 0.f;
-      g[j] = n < N ? s.g[n] : 0.f;
+      if constexpr (kHalf)
+        g[j] = logit_factor(s.inv_tau, n < N ? s.tops.row[n] : 0u, top_w);
+      else
+        g[j] = n < N ? s.g[n] : 0.f;
     }
     arrived(first.x);
     arrived(first.y);
@@ -895,7 +1068,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
     id += gridDim.x;
     more = mm_tile_of(s.mm, id, &split, &ta2, &tb2);
     if (more) tile.begin(ta2, tb2, 0);
-    grad_epilogue<kPlanes>(s, acc, ta, tb, lse, g, list, e0, e1, first, change);
+    grad_epilogue<kHalf>(s, acc, ta, tb, lse, g, list, e0, e1, first, change);
   }
 }
 
@@ -913,11 +1086,21 @@ struct ProductArgs {
   int64_t plane;
   int64_t lda;      // rows_a rounded up to 4
   int accumulate;   // add to what partial holds
-  const float* scale;  // straight to out: multiplied by *scale times coef (null: as it is)
+  // Straight to out: multiplied by *scale (null: 1), by the row's by_row (null: 1; by the
+  // rows' numbers) and by coef.
+  const float* scale;
+  const float* by_row;
   float coef;
+  const uint32_t* shift;  // float32: the magnitude that A's planes were shifted by
   void* out;
   int out_bf16;
 };
+
+// What undoes the shifts of dz and of a product's other operand.
+DPC_DEVICE int product_shift(const uint32_t* top) { return top ? -(kDzShift + half_shift(*top)) : 0; }
+DPC_DEVICE f32x4_t shifted(f32x4_t x, int n) {
+  return n ? f32x4_t{ldexpf(x[0], n), ldexpf(x[1], n), ldexpf(x[2], n), ldexpf(x[3], n)} : x;
+}
 
 DPC_DEVICE void store_row4(void* out, int64_t at, int left, bool whole, int bf16, f32x4_t x) {
   if (whole) {  // rows of whole quads
@@ -940,7 +1123,7 @@ DPC_DEVICE void store_row4(void* out, int64_t at, int left, bool whole, int bf16
 
 // kHidden: dH (A = W, K the vocabulary, B = dz by rows); else dW (A = H, K the rows,
 // B = dz by columns).
-template <bool kHidden>
+template <bool kHidden, bool kHalf>
 __global__ void __launch_bounds__(kMmThreads, 1) head_product_kernel(ProductArgs s) {
   int split, ta, tb;
   const uint16_t* hp;
@@ -954,7 +1137,7 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_product_kernel(ProductArgs
     s.mm.kl = count;
   }
   if (!mm_tile_of(s.mm, blockIdx.x, &split, &ta, &tb)) return;
-  MmTile<false, kHidden, true, kHidden> tile(s.mm, lds_all);
+  MmTile<false, kHidden, true, kHidden, kHalf> tile(s.mm, lds_all);
   MmAcc<kHidden> acc;
   tile.begin(ta, tb, split);
   tile.run(acc);
@@ -962,11 +1145,13 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_product_kernel(ProductArgs
   const int a0 = ta * kMmTile + acc.row0(w) + 4 * (lane >> 4);
   const int b0 = tb * kMmTile + acc.col0(w) + (lane & 15);
   const bool whole = s.rows_a % 4 == 0;
-  const float f = s.scale ? *s.scale * s.coef : 1.f;
+  const float all = (s.scale ? *s.scale : 1.f) * s.coef;
+  const int shift = kHalf ? product_shift(s.shift) : 0;
 #pragma unroll
   for (int j = 0; j < MmAcc<kHidden>::kB; ++j) {
     const int b = b0 + 16 * j;
     if (b >= rows_b) continue;
+    const float f = s.by_row ? all * s.by_row[b] : all;
     const int64_t row = kHidden && s.active && !s.partial ? s.active[b] : b;
 #pragma unroll
     for (int i = 0; i < MmAcc<kHidden>::kA; ++i) {
@@ -978,14 +1163,15 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_product_kernel(ProductArgs
         if (s.accumulate) x += *p;
         *p = x;
       } else {
-        store_row4(s.out, row * s.rows_a + a, s.rows_a - a, whole, s.out_bf16, x * f);
+        store_row4(s.out, row * s.rows_a + a, s.rows_a - a, whole, s.out_bf16,
+                   shifted(x * f, shift));
       }
     }
   }
 }
 
-// The slices of partial added up in order, times *scale coef: row r to out's row
-// active[r] (or r).
+// The slices of partial added up in order, multiplied as a product's own output: row r
+// to out's row active[r] (or r).
 struct ReduceArgs {
   const float* partial;
   int splits;
@@ -994,7 +1180,9 @@ struct ReduceArgs {
   int first;
   const int32_t* active;
   const float* scale;
+  const float* by_row;
   float coef;
+  const uint32_t* shift;
   int D;
   void* out;
   int out_bf16;
@@ -1007,7 +1195,8 @@ __global__ void __launch_bounds__(256) head_reduce_kernel(ReduceArgs a) {
     const int64_t left = (int64_t)*a.count - a.first;
     rows = left < 0 ? 0 : (left < rows ? left : rows);
   }
-  const float f = a.scale ? *a.scale * a.coef : 1.f;
+  const float all = (a.scale ? *a.scale : 1.f) * a.coef;
+  const int shift = product_shift(a.shift);
   const bool whole = a.D % 4 == 0;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * quads;
        i += (int64_t)gridDim.x * 256) {
@@ -1017,7 +1206,7 @@ __global__ void __launch_bounds__(256) head_reduce_kernel(ReduceArgs a) {
     for (int s = 1; s < a.splits; ++s)
       x += *reinterpret_cast<const f32x4_t*>(a.partial + s * a.plane + row * a.lda + c);
     store_row4(a.out, (a.active ? a.active[row] : row) * (int64_t)a.D + c, a.D - c, whole,
-               a.out_bf16, x * f);
+               a.out_bf16, shifted(x * (a.by_row ? all * a.by_row[row] : all), shift));
   }
 }
 
@@ -1060,10 +1249,10 @@ struct Plan {
   int piece_tiles, pieces;       // backward
   int splits_h, splits_w;
   // Byte offsets: state (kept for the backward), workspaces.
-  int64_t s_rows, s_lse, s_corr, s_list, s_start, s_unit, state_bytes;
-  int64_t f_rows, f_lse, f_corr, f_list, f_start, f_cols, f_h, f_w, f_picked, f_part, f_e, f_pc,
+  int64_t s_rows, s_tops, s_lse, s_corr, s_list, s_start, s_unit, state_bytes;
+  int64_t f_rows, f_tops, f_lse, f_corr, f_list, f_start, f_cols, f_h, f_w, f_picked, f_part, f_e, f_pc,
       fwd_bytes;
-  int64_t b_h, b_w, b_g, b_dz, b_ph, b_pw, bwd_bytes;
+  int64_t b_h, b_w, b_hg, b_g, b_dz, b_ph, b_pw, bwd_bytes;
 };
 
 Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w) {
@@ -1073,17 +1262,17 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
   p.V = V;
   p.K = K;
   p.dtype = dtype;
-  p.planes = dtype == DPC_F32 ? 3 : 1;
+  p.planes = dtype == DPC_F32 ? 2 : 1;
   p.want_h = want_h != 0;
   p.want_w = want_w != 0;
-  p.emit = p.want_h && !p.want_w && p.planes == 1;
+  p.emit = p.want_h && !p.want_w;
   p.ld = up(D, 8);
   p.pack = dtype == DPC_F32 || D % 8 != 0;
   p.tiles_v = (V + kMmTile - 1) / kMmTile;
   p.tiles_n = (int)((N + kMmTile - 1) / kMmTile);
   p.tiles_d = (D + kMmTile - 1) / kMmTile;
   p.lda = up(D, 4);
-  const int pairs = p.planes == 1 ? 1 : 6;
+  const int pairs = p.planes == 1 ? 1 : 3;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -1093,7 +1282,10 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
   const int64_t rows_b = (2 * N + 1) * 4, lse_b = N * 4, corr_b = N * K * 4, list_b = N * K * 8,
                 start_b = (int64_t)p.tiles_n * (8 * p.tiles_v + 1) * 4;
   const bool keep = (p.want_h || p.want_w) && !p.emit;
-  if (p.want_h || p.want_w) p.s_rows = take(rows_b);
+  if (p.want_h || p.want_w) {
+    p.s_rows = take(rows_b);
+    p.s_tops = take(8 + N * 4);
+  }
   if (keep) {
     p.s_lse = take(lse_b);
     p.s_corr = take(corr_b);
@@ -1103,7 +1295,10 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
   if (p.emit) p.s_unit = take(N * D * 4);
   p.state_bytes = at;
   at = 0;
-  if (!p.want_h && !p.want_w) p.f_rows = take(rows_b);
+  if (!p.want_h && !p.want_w) {
+    p.f_rows = take(rows_b);
+    p.f_tops = take(8 + N * 4);
+  }
   if (!keep) {
     p.f_lse = take(lse_b);
     p.f_corr = take(corr_b);
@@ -1116,15 +1311,16 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
   p.f_picked = take(N * K * 4);
   p.f_part = take(N * p.tiles_v * 16);
   if (p.emit) {
-    int64_t c = kPieceBytes / ((int64_t)p.tiles_v * kMmTile * 2) / kMmTile * kMmTile;
+    const int64_t row_bytes = p.planes * (int64_t)p.tiles_v * kMmTile * 2;
+    int64_t c = kPieceBytes / row_bytes / kMmTile * kMmTile;
     if (c < kMmTile) c = kMmTile;
     // Chunks of equal size.
     const int64_t rows = up(N, kMmTile);
     if (c > rows) c = rows;
     const int64_t n = (rows + c - 1) / c;
     p.chunk = (int)up((rows + n - 1) / n, kMmTile);
-    p.splits_c = slices((int64_t)p.tiles_d * (p.chunk / kMmTile), p.tiles_v * 4);
-    p.f_e = take(p.chunk * (int64_t)p.tiles_v * kMmTile * 2);
+    p.splits_c = slices((int64_t)p.tiles_d * (p.chunk / kMmTile), pairs * (int64_t)p.tiles_v * 4);
+    p.f_e = take(p.chunk * row_bytes);
     if (p.splits_c > 1) p.f_pc = take(p.splits_c * p.chunk * p.lda * 4);
   }
   p.fwd_bytes = at;
@@ -1132,6 +1328,7 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
   if (keep) {
     p.b_h = take(p.planes * N * p.ld * 2);
     if (p.pack) p.b_w = take(p.planes * (int64_t)V * p.ld * 2);
+    if (p.planes == 2 && p.want_w) p.b_hg = take(p.planes * N * p.ld * 2);
     p.b_g = take(4 + N * 4);
     const int64_t rows = (int64_t)p.tiles_n * kMmTile;
     int64_t t = kPieceBytes / (p.planes * rows * kMmTile * 2);
@@ -1158,6 +1355,11 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
 Rows rows_at(uint8_t* base, int64_t N) {
   int32_t* r = reinterpret_cast<int32_t*>(base);
   return Rows{r, r + 1, r + 1 + N};
+}
+
+Tops tops_at(uint8_t* base) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(base);
+  return Tops{r, r + 1, r + 2};
 }
 
 // The prep launch, and W and H as the tiles read them.
@@ -1244,6 +1446,7 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
   const bool any = p.want_h || p.want_w, keep = any && !p.emit;
   auto place = [&](bool in_state, int64_t so, int64_t fo) { return in_state ? kept + so : base + fo; };
   const Rows rows = rows_at(place(any, p.s_rows, p.f_rows), N);
+  const Tops tops = tops_at(place(any, p.s_tops, p.f_tops));
   const Entries entries = {reinterpret_cast<int32_t*>(base + p.f_cols),
                            reinterpret_cast<uint2*>(place(keep, p.s_list, p.f_list)),
                            reinterpret_cast<int32_t*>(place(keep, p.s_start, p.f_start))};
@@ -1255,10 +1458,17 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
     DPC_HIP_CHECK(hipGetLastError());
   }
   hipLaunchKernelGGL(rows_kernel, dim3(1), dim3(1024), 0, s, index, ignore_index,
-                     teacher != nullptr, N, rows, loss);
+                     teacher != nullptr, N, rows, loss, tops);
   DPC_HIP_CHECK(hipGetLastError());
+  if (dtype == DPC_F32) {
+    hipLaunchKernelGGL(tops_kernel, dim3(256, 2), dim3(256), 0, s,
+                       static_cast<const float*>(hidden), static_cast<const float*>(weight), D, V,
+                       rows, tops);
+    DPC_HIP_CHECK(hipGetLastError());
+  }
   PrepArgs q = {};
   q.rows = rows;
+  q.tops = tops;
   q.index = index;
   q.teacher = teacher != nullptr;
   q.blocks = p.tiles_n;
@@ -1275,7 +1485,8 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
   a.mm.splits = 1;
   a.V = V;
   a.K = K;
-  a.inv_tau = (float)(1.0 / temperature);
+  a.inv_tau = (float)(kLog2e64 / temperature);
+  a.tops = tops;
   a.entries = entries;
   a.picked = reinterpret_cast<float*>(base + p.f_picked);
   a.part = reinterpret_cast<f32x2_t*>(base + p.f_part);
@@ -1285,7 +1496,7 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
   j.N = N;
   j.K = K;
   j.parts = 2 * p.tiles_v;
-  j.inv_tau = a.inv_tau;
+  j.inv_tau = (float)(1.0 / temperature);
   j.loss_scale = (float)(temperature * temperature);
   j.cols = entries.cols;
   j.picked = a.picked;
@@ -1295,8 +1506,11 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
   j.lse = lse;
   j.corr = corr;
   if (!p.emit) {
-    hipLaunchKernelGGL((head_stats_kernel<false>), tile_grid((int64_t)p.tiles_v * p.tiles_n),
-                       dim3(kMmThreads), 0, s, a);
+    const dim3 grid = tile_grid((int64_t)p.tiles_v * p.tiles_n);
+    if (p.planes == 1)
+      hipLaunchKernelGGL((head_stats_kernel<false, false>), grid, dim3(kMmThreads), 0, s, a);
+    else
+      hipLaunchKernelGGL((head_stats_kernel<false, true>), grid, dim3(kMmThreads), 0, s, a);
     DPC_HIP_CHECK(hipGetLastError());
     hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)((N + kJoinRows - 1) / kJoinRows)),
                        dim3(kJoinThreads), 0, s, j);
@@ -1304,36 +1518,49 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
     return DPC_OK;
   }
   a.lde = (int64_t)p.tiles_v * 4;
+  a.plane = p.chunk / kMmTile * a.lde * kMmBlock;
   a.e = reinterpret_cast<uint16_t*>(base + p.f_e);
   const int tiles_c = p.chunk / kMmTile;
   float* unit = reinterpret_cast<float*>(kept + p.s_unit);
   for (int64_t first = 0; first < N; first += p.chunk) {
     a.h.first = j.first = (int)first;
     a.h.most = p.chunk;
-    hipLaunchKernelGGL((head_stats_kernel<true>), tile_grid((int64_t)p.tiles_v * tiles_c),
-                       dim3(kMmThreads), 0, s, a);
+    const dim3 grid = tile_grid((int64_t)p.tiles_v * tiles_c);
+    if (p.planes == 1)
+      hipLaunchKernelGGL((head_stats_kernel<true, false>), grid, dim3(kMmThreads), 0, s, a);
+    else
+      hipLaunchKernelGGL((head_stats_kernel<true, true>), grid, dim3(kMmThreads), 0, s, a);
     DPC_HIP_CHECK(hipGetLastError());
     hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)(p.chunk / kJoinRows)),
                        dim3(kJoinThreads), 0, s, j);
     DPC_HIP_CHECK(hipGetLastError());
     const FixArgs x = {rows.count, N, K, p.tiles_v, (int)first, entries.cols, a.part, lse, corr,
-                       a.e, a.lde};
-    hipLaunchKernelGGL(head_fix_kernel,
-                       dim3((unsigned)(p.chunk / kJoinRows),
-                            (unsigned)((p.tiles_v + kFixTiles - 1) / kFixTiles)),
-                       dim3(kJoinThreads), 0, s, x);
+                       a.e, a.lde, a.plane};
+    const dim3 fix_grid((unsigned)(p.chunk / kJoinRows),
+                        (unsigned)((p.tiles_v + kFixTiles - 1) / kFixTiles));
+    if (p.planes == 1)
+      hipLaunchKernelGGL((head_fix_kernel<false>), fix_grid, dim3(kJoinThreads), 0, s, x);
+    else
+      hipLaunchKernelGGL((head_fix_kernel<true>), fix_grid, dim3(kJoinThreads), 0, s, x);
     DPC_HIP_CHECK(hipGetLastError());
     ProductArgs m = {};
-    m.mm = MmArgs{w, MmOperand{a.e, a.lde, 0, 0}, V, 1, p.tiles_d, tiles_c, p.splits_c};
+    m.mm = MmArgs{w, MmOperand{a.e, a.lde, a.plane, 0}, V, p.planes, p.tiles_d, tiles_c,
+                  p.splits_c};
+    m.coef = 1.f;
+    m.shift = p.planes == 2 ? tops.w : nullptr;
     m.h = a.h;
     m.rows_a = D;
     m.lda = p.lda;
     m.plane = p.chunk * p.lda;
     m.partial = p.splits_c > 1 ? reinterpret_cast<float*>(base + p.f_pc) : nullptr;
     m.out = unit + first * D;
-    hipLaunchKernelGGL((head_product_kernel<true>),
-                       dim3((unsigned)(p.tiles_d * tiles_c * p.splits_c)), dim3(kMmThreads), 0, s,
-                       m);
+    const dim3 product_grid((unsigned)(p.tiles_d * tiles_c * p.splits_c));
+    if (p.planes == 1)
+      hipLaunchKernelGGL((head_product_kernel<true, false>), product_grid, dim3(kMmThreads), 0, s,
+                         m);
+    else
+      hipLaunchKernelGGL((head_product_kernel<true, true>), product_grid, dim3(kMmThreads), 0, s,
+                         m);
     DPC_HIP_CHECK(hipGetLastError());
     if (m.partial) {
       ReduceArgs r = {};
@@ -1344,6 +1571,8 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
       r.lda = p.lda;
       r.count = rows.count;
       r.first = (int)first;
+      r.coef = 1.f;
+      r.shift = m.shift;
       r.D = D;
       r.out = m.out;
       const int rr = reduce(r, s);
@@ -1378,7 +1607,7 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
     if (grid > 8192) grid = 8192;
     hipLaunchKernelGGL(head_scale_kernel, dim3((unsigned)grid), dim3(256), 0, s,
                        reinterpret_cast<const float*>(kept + p.s_unit), rows, grad_loss,
-                       (float)temperature, N, D, static_cast<uint16_t*>(hidden_grad));
+                       (float)temperature, N, D, dtype == DPC_BF16, hidden_grad);
     DPC_HIP_CHECK(hipGetLastError());
     return DPC_OK;
   }
@@ -1389,6 +1618,17 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
   pa.g = grad_loss;
   pa.gmax = reinterpret_cast<float*>(base + p.b_g);
   pa.g_over = pa.gmax + 1;
+  const Tops tops = tops_at(kept + p.s_tops);
+  pa.tops = tops;
+  const bool half = p.planes == 2;
+  if (half) {
+    hipLaunchKernelGGL(gmax_kernel, dim3(1), dim3(kPrepThreads), 0, s, pa);
+    DPC_HIP_CHECK(hipGetLastError());
+    if (weight_grad)
+      pa.hg = reinterpret_cast<uint16_t*>(base + p.b_hg);
+    else
+      pa.g = nullptr;
+  }
   Hidden h;
   MmOperand w;
   const int rc = operands(p, pa, hidden, weight, base + p.b_h, base + p.b_w, s, &h, &w);
@@ -1413,20 +1653,21 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
     a.K = K;
     a.tile0 = tile0;
     a.tiles = p.tiles_v;
-    a.inv_tau = (float)(1.0 / temperature);
+    a.inv_tau = (float)(kLog2e64 / temperature);
     a.entries = Entries{nullptr, reinterpret_cast<uint2*>(kept + p.s_list),
                         reinterpret_cast<int32_t*>(kept + p.s_start)};
     a.corr = reinterpret_cast<const float*>(kept + p.s_corr);
     a.lse = reinterpret_cast<const float*>(kept + p.s_lse);
     a.g = pa.g_over;
+    a.tops = tops;
     a.dz = dz;
     a.ld = ldz;
     a.plane = plane;
     const dim3 grid = tile_grid((int64_t)tiles * p.tiles_n);
-    if (p.planes == 1)
-      hipLaunchKernelGGL((head_grad_kernel<1>), grid, dim3(kMmThreads), 0, s, a);
+    if (half)
+      hipLaunchKernelGGL((head_grad_kernel<true>), grid, dim3(kMmThreads), 0, s, a);
     else
-      hipLaunchKernelGGL((head_grad_kernel<3>), grid, dim3(kMmThreads), 0, s, a);
+      hipLaunchKernelGGL((head_grad_kernel<false>), grid, dim3(kMmThreads), 0, s, a);
     DPC_HIP_CHECK(hipGetLastError());
     const MmOperand zop = {dz, ldz, plane, 0};
     ProductArgs q = {};
@@ -1453,9 +1694,15 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
       m.partial = direct ? nullptr : reinterpret_cast<float*>(base + p.b_ph);
       m.accumulate = i > 0;
       m.out = hidden_grad;
-      hipLaunchKernelGGL((head_product_kernel<true>),
-                         dim3((unsigned)(p.tiles_d * p.tiles_n * p.splits_h)), dim3(kMmThreads), 0,
-                         s, m);
+      m.by_row = half ? pa.g_over : nullptr;
+      m.shift = half ? tops.w : nullptr;
+      const dim3 product_grid((unsigned)(p.tiles_d * p.tiles_n * p.splits_h));
+      if (half)
+        hipLaunchKernelGGL((head_product_kernel<true, true>), product_grid, dim3(kMmThreads), 0, s,
+                           m);
+      else
+        hipLaunchKernelGGL((head_product_kernel<true, false>), product_grid, dim3(kMmThreads), 0,
+                           s, m);
       DPC_HIP_CHECK(hipGetLastError());
       if (!direct && i + 1 == p.pieces) {
         r.partial = m.partial;
@@ -1464,6 +1711,8 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
         r.rows = N;
         r.count = rows.count;
         r.active = rows.active;
+        r.by_row = m.by_row;
+        r.shift = m.shift;
         r.out = hidden_grad;
         const int rr = reduce(r, s);
         if (rr != DPC_OK) return rr;
@@ -1476,9 +1725,15 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
       m.plane = (int64_t)cols_here * p.lda;
       m.partial = p.splits_w == 1 ? nullptr : reinterpret_cast<float*>(base + p.b_pw);
       m.out = static_cast<uint8_t*>(weight_grad) + (int64_t)first * D * esz;
-      hipLaunchKernelGGL((head_product_kernel<false>),
-                         dim3((unsigned)(p.tiles_d * tiles * p.splits_w)), dim3(kMmThreads), 0, s,
-                         m);
+      m.shift = half ? tops.h : nullptr;
+      if (half) m.h.packed = pa.hg;
+      const dim3 product_grid((unsigned)(p.tiles_d * tiles * p.splits_w));
+      if (half)
+        hipLaunchKernelGGL((head_product_kernel<false, true>), product_grid, dim3(kMmThreads), 0,
+                           s, m);
+      else
+        hipLaunchKernelGGL((head_product_kernel<false, false>), product_grid, dim3(kMmThreads), 0,
+                           s, m);
       DPC_HIP_CHECK(hipGetLastError());
       if (m.partial) {
         r.partial = m.partial;
@@ -1488,6 +1743,8 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
         r.count = nullptr;
         r.first = 0;
         r.active = nullptr;
+        r.by_row = nullptr;
+        r.shift = m.shift;
         r.out = m.out;
         const int rr = reduce(r, s);
         if (rr != DPC_OK) return rr;

@@ -1,4 +1,4 @@
-// One 256 x 256 tile of a product of two bf16 matrices on the matrix cores
+// One 256 x 256 tile of a product of two 16-bit matrices on the matrix cores
 // (gfx950), for operands of either orientation:
 //   K-contiguous: element (i, k) at p[i * ld + k]  (a row holds one index's K values)
 //   K-slow:       element (i, k) at p[k * ld + i]  (a row holds one k of every index)
@@ -15,12 +15,13 @@
 // consecutive A indices sit in a lane's four registers.  A is therefore always
 // the operand whose index is contiguous in the output.
 //
-// float32 operands come as three bf16 planes, x = x0 + x1 + x2 exactly, each the
-// rounding of what the ones before leave (|x1| <= 2^-9 |x|, |x2| <= 2^-18 |x|).
-// The K loop runs over six plane pairs, smallest first: (0,2) (1,1) (2,0) (0,1)
-// (1,0) (0,0); the three left out are below 2^-26 of the product.  The products
-// are exact and the sums are the MFMA's float32 ones.  At 6 of the bf16 rate's
-// 2500 TFLOP/s this is 2.6 times the float32 matrix instructions' 157.
+// float32 operands (kHalf) come as two fp16 planes, x = (x0 + 2^-11 x1) 2^-shift with
+// the shift that brings the tensor's largest magnitude to [2^14, 2^15): x0 is x's
+// rounding to 11 bits, x1 that of what it leaves, so 2^-24 |x| is lost at most.  The K
+// loop takes the plane pairs (0, 1) and (1, 0), scales the accumulators by 2^-11, and
+// goes on with (0, 0); the pair left out is below 2^-24 of the product.  The products are
+// exact and the sums are the MFMA's float32 ones: float32 accuracy at three bf16-rate
+// products, 2500 / 3 TFLOP/s against the float32 matrix instructions' 157.
 #pragma once
 
 #include "lds_stage.h"
@@ -35,7 +36,7 @@ struct MmOperand {
 struct MmArgs {
   MmOperand a, b;
   int kl;      // valid K, K-contiguous operands: a multiple of 8 (zero-padded)
-  int planes;  // 1 (bf16) or 3 (float32)
+  int planes;  // 1 (bf16) or 2 (float32)
   int tiles_a, tiles_b;
   int splits;  // the K steps go out in this many slices
 };
@@ -44,8 +45,9 @@ constexpr int kMmTile = 256, kMmStep = 64, kMmThreads = 512, kMmWaves = 8;
 constexpr int kMmOperandBytes = kMmTile * kMmStep * 2;  // 32 KiB
 constexpr int kMmOutOfRange = 0x7ff00000;
 
-// Plane pairs, nibble i of each word: pair i's plane of A and of B.
-constexpr uint32_t kMmPairsA = 0x010210u, kMmPairsB = 0x001012u;
+// Plane pairs, nibble i of each word: pair i's plane of A and of B (planes 1: pair 2).
+constexpr uint32_t kMmPairsA = 0x010u, kMmPairsB = 0x001u;
+constexpr float kMmCross = 0x1.0p-11f;  // of the pairs before the last
 
 // K-contiguous tile: rows of 64 k = 128 bytes, eight 16-byte chunks
 // XOR-swizzled by bits 1-3 of the row.  The 64 banks span two rows, so 16
@@ -55,8 +57,11 @@ DPC_DEVICE int mm_kc_off(int row, int chunk) {
   return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4);
 }
 
-DPC_DEVICE int mm_steps(const MmArgs& g) {
-  return (g.planes == 1 ? 1 : 6) * ((g.kl + kMmStep - 1) / kMmStep);
+// Steps of a plane pair: an even number for float32, so that the accumulators are
+// scaled between two rounds of the two LDS stages.
+DPC_HOST_DEVICE int mm_pair_steps(int kl, int planes) {
+  const int n = (kl + kMmStep - 1) / kMmStep;
+  return planes == 1 ? n : n + (n & 1);
 }
 
 // Linear id -> (split, tile of A, tile of B); false past the last.  Dispatch is
@@ -120,6 +125,8 @@ struct MmStage {
       }
     }
   }
+  // (A step past kl, or none: nothing is in range.)
+  static DPC_DEVICE uint32_t in_range(int64_t bytes) { return bytes > 0 ? (uint32_t)bytes : 0u; }
   // The step at k0 of plane `pl` of tile t: the buffer it reads, and `bad`, out of the
   // buffer's range for lanes whose k is past kl.  Rows past the operand's are out of
   // range too: all such reads give zeros.  (Native blocks are whole; past their matrix
@@ -137,11 +144,11 @@ struct MmStage {
       bytes = (uint32_t)(4 * kMmBlock * 2 - ((k0 & 255) >> 4) * 1024);
     } else if (kKc) {
       base += (int64_t)i0 * o.ld + k0;
-      bytes = (uint32_t)((min(o.rows - i0, kMmTile) * o.ld - k0) * 2);
+      bytes = in_range((min(o.rows - i0, kMmTile) * o.ld - k0) * 2);
       *bad = k0 + kchunk >= kl ? kMmOutOfRange : 0;
     } else {
       base += (int64_t)k0 * o.ld + i0;
-      bytes = (uint32_t)((min(kl - k0, kMmStep) * o.ld - i0) * 2);
+      bytes = in_range((min(kl - k0, kMmStep) * o.ld - i0) * 2);
     }
     return rsrc_words(base, bytes);
   }
@@ -200,8 +207,8 @@ struct MmFrags {
 // nothing reads.
 struct MmPlace {
   int left, pair, k0;
-  DPC_DEVICE MmPlace next(int kl) const {  // (selects: no branch in the loop)
-    const int go = left > 1 ? 1 : 0, k = k0 + kMmStep, wrap = k >= kl ? 1 : 0;
+  DPC_DEVICE MmPlace next(int end) const {  // (selects: no branch in the loop)
+    const int go = left > 1 ? 1 : 0, k = k0 + kMmStep, wrap = k >= end ? 1 : 0;
     return MmPlace{left - go, pair + (go & wrap), go ? (wrap ? 0 : k) : k0};
   }
 };
@@ -220,11 +227,13 @@ struct MmPlace {
 // begin() sends the first transfers, run() does the rest and ends with a barrier,
 // after which `lds` is free: the next tile's begin() goes before this one's epilogue,
 // so that its first step has arrived when the epilogue ends.
-template <bool kAKc, bool kBKc, bool kBNative, bool kWideB>
+template <bool kAKc, bool kBKc, bool kBNative, bool kWideB, bool kHalf>
 struct MmTile {
   const MmArgs& g;
   uint8_t* lds;
   int lane, w, ta, tb, steps;
+  int end;    // k at which a plane pair ends
+  int cross;  // steps before the pair (0, 0)
   MmPlace pa, pb;
   MmStage<kAKc, false> sa;
   MmStage<kBKc, kBNative> sb;
@@ -239,11 +248,11 @@ struct MmTile {
   }
   DPC_DEVICE void next_a() {
     buf = sa.buffer(g.a, (kMmPairsA >> (4 * pa.pair)) & 15, ta, pa.k0, g.kl, &bad);
-    pa = pa.next(g.kl);
+    pa = pa.next(end);
   }
   DPC_DEVICE void next_b() {
     buf = sb.buffer(g.b, (kMmPairsB >> (4 * pb.pair)) & 15, tb, pb.k0, g.kl, &bad);
-    pb = pb.next(g.kl);
+    pb = pb.next(end);
   }
   DPC_DEVICE void fetch_a(int stage, int j) {
     sa.issue(buf, bad, lds_addr(lds) + stage * kMmOperandBytes, w, j);
@@ -252,16 +261,30 @@ struct MmTile {
     sb.issue(buf, bad, lds_addr(lds) + (2 + stage) * kMmOperandBytes, w, j);
   }
 
+  static DPC_DEVICE f32x4_t mma(bf16x8_t a, bf16x8_t b, f32x4_t c) {
+    typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+    if constexpr (kHalf)
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a),
+                                                    __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+
   DPC_DEVICE void begin(int tile_a, int tile_b, int split) {
     ta = tile_a;
     tb = tile_b;
-    const int ks = max(1, (g.kl + kMmStep - 1) / kMmStep);
-    const long long n = mm_steps(g);
-    const int s0 = (int)(n * split / g.splits), s1 = (int)(n * (split + 1) / g.splits);
-    steps = __builtin_amdgcn_readfirstlane(s1 - s0);
+    const int ks = mm_pair_steps(g.kl, g.planes);
+    end = ks * kMmStep;
+    // Slices of whole rounds of two steps (float32; bf16: of steps).
+    const long long rounds = kHalf ? 3ll * ks / 2 : ks;
+    const int each = kHalf ? 2 : 1;
+    const int s0 = __builtin_amdgcn_readfirstlane((int)(rounds * split / g.splits) * each),
+              s1 = __builtin_amdgcn_readfirstlane((int)(rounds * (split + 1) / g.splits) * each);
+    steps = s1 - s0;
     if (steps <= 0) return;
-    const int pair0 = __builtin_amdgcn_readfirstlane(s0 / ks);
-    pa = MmPlace{steps, g.planes == 1 ? 5 : pair0, (s0 - pair0 * ks) * kMmStep};
+    const int pair0 = kHalf ? __builtin_amdgcn_readfirstlane(s0 / ks) : 2;
+    cross = kHalf ? max(0, min(steps, 2 * ks - s0)) : 0;
+    pa = MmPlace{steps, pair0, kHalf ? (s0 - pair0 * ks) * kMmStep : s0 * kMmStep};
     pb = pa;
     next_a();
 #pragma unroll
@@ -307,11 +330,9 @@ struct MmTile {
       for (int m = 0; m < 16; ++m) {
         const int i = m >> 2, j = m & 3;
         if constexpr (kWideB)
-          acc.v[j][4 * half + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              y[j], x[i], acc.v[j][4 * half + i], 0, 0, 0);
+          acc.v[j][4 * half + i] = mma(y[j], x[i], acc.v[j][4 * half + i]);
         else
-          acc.v[4 * half + i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              x[i], y[j], acc.v[4 * half + i][j], 0, 0, 0);
+          acc.v[4 * half + i][j] = mma(x[i], y[j], acc.v[4 * half + i][j]);
         slot(m);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -355,6 +376,12 @@ struct MmTile {
     for (; s + 1 < steps; s += 2) {
       step(0, 1);
       step(1, 0);
+      if (kHalf && s + 2 == cross) {
+#pragma unroll
+        for (int i = 0; i < MmAcc<kWideB>::kA; ++i)
+#pragma unroll
+          for (int j = 0; j < MmAcc<kWideB>::kB; ++j) acc.v[i][j] *= kMmCross;
+      }
     }
     if (s < steps) step(0, 1);
     DPC_WAIT_VMCNT(0);

@@ -4,7 +4,7 @@ Error model the tolerances come from (u = 2^-23, one extra addend of slack per
 16 products, as for the Gram kernels): a product sum of n terms is off by at
 most 1.125 n u times the sum of the terms' magnitudes.  So a logit is off by
 ``zerr = 1.125 n u |h| |w|``; a loss by twice that and a few ulp of the log sum
-exp; dz by its bf16 rounding (float32: three exact parts) and by what the logits'
+exp; dz by its bf16 rounding (float32: two fp16 planes, 2^-24) and by what the logits'
 error does to p; and a gradient by dz's error and the sum's own, rounded once.  With a
 frozen head (bf16) dz goes through fp16 exponentials relative to a tile's maximum:
 another 2^-12 of it, or 2^-25 where they are subnormal.
@@ -297,6 +297,48 @@ def test_nan_in_rows_without_a_target_reaches_nothing(dev):
     f1 = torch.autograd.grad(head.linear_cross_entropy(h1, W, t), [h1], up)
     f2 = torch.autograd.grad(head.linear_cross_entropy(h2, W, t), [h2], up2)
     assert torch.equal(f1[0], f2[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("power", [-60, 40, 90])
+def test_float32_of_any_magnitude(dev, power):
+    """float32 operands are held relative to their largest: powers of two that cancel
+    in the logits change nothing, and come out of the gradients as they went in."""
+    g, h, W, up = _inputs(dev, (130,), 72, 300, torch.float32, 11)
+    t = torch.randint(0, 300, (130,), generator=g, device=dev)
+
+    def run(h, W, both):
+        h, W = h.clone().requires_grad_(), W.clone().requires_grad_(both)
+        loss = head.linear_cross_entropy(h, W, t)
+        loss.backward(up)
+        return loss.detach(), h.grad, W.grad
+
+    f = 2.0**power
+    for both in (False, True):
+        a, b = run(h, W, both), run(h * f, W / f, both)
+        assert torch.equal(a[0], b[0])
+        assert torch.equal(a[1], b[1] * f)
+        if both:
+            assert torch.equal(a[2], b[2] / f)
+
+
+@pytest.mark.gpu
+def test_float32_rows_keep_their_own_scale(dev):
+    """A row far larger than the others does not change their losses or gradients."""
+    g, h, W, up = _inputs(dev, (130,), 72, 300, torch.float32, 12)
+    t = torch.randint(0, 300, (130,), generator=g, device=dev)
+    big = h.clone()
+    big[77] *= 2.0**60
+    keep = torch.arange(130, device=dev) != 77
+    for both in (False, True):
+        res = []
+        for x in (h, big):
+            x, w = x.clone().requires_grad_(), W.clone().requires_grad_(both)
+            loss = head.linear_cross_entropy(x, w, t)
+            loss.backward(up)
+            assert torch.isfinite(loss).all() and torch.isfinite(x.grad).all()
+            res.append((loss.detach()[keep], x.grad[keep]))
+        assert torch.equal(res[0][0], res[1][0]) and torch.equal(res[0][1], res[1][1])
 
 
 @pytest.mark.gpu
