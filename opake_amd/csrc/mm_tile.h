@@ -157,14 +157,14 @@ struct MmStage {
   }
 };
 
-// Reads the 16 x 32 fragments of a wave's blocks from an operand's tile.  kMixed:
-// the other operand is K-slow, whose transposing reads fix the order of the
-// k-slots (frag16_off: slot 8 q + 4 h + e is k = 16 h + 4 q + e; a native piece has
-// that order too).  A lane keeps a few byte offsets; blocks, sub-steps and stages are
+// Reads the 16 x 32 fragments of a wave's blocks from an operand's tile.  Both of a
+// product's operands give the k-slots one order: by rows (K-contiguous), or that of the
+// transposing reads (frag16_off: slot 8 q + 4 h + e is k = 16 h + 4 q + e), which a native
+// piece has too.  A lane keeps a few byte offsets; blocks, sub-steps and stages are
 // added as immediates.
-template <bool kKc, bool kNative, bool kMixed, int kBlocks>
+template <bool kKc, bool kNative, int kBlocks>
 struct MmFrags {
-  static constexpr int kOffsets = kNative ? 1 : kKc ? (kMixed ? 4 : 2) : kBlocks / 2;
+  static constexpr int kOffsets = kNative ? 1 : kKc ? 2 : kBlocks / 2;
   int o[kOffsets];
   // Tile at byte `at` of the workgroup's LDS, first block at index c0.
   DPC_DEVICE void init(int at, int c0, int lane) {
@@ -177,8 +177,6 @@ struct MmFrags {
         o[i] = at + (c0 >> 5) * 4096 + mm_native_slot(4 * q + ((lane & 15) >> 2), lane & 3) * 16;
       else if (!kKc)
         o[i] = at + frag16_off(c0 + 32 * i, 0, lane);
-      else if (kMixed)  // i: 2 kk + h
-        o[i] = at + mm_kc_off(row, 2 * i + (q >> 1)) + 8 * (q & 1);
       else
         o[i] = at + mm_kc_off(row, 4 * i + q);
     }
@@ -195,10 +193,7 @@ struct MmFrags {
       const int p = (o[i >> 1] ^ (32 * (i & 1))) + off + kk * 32 * kTileRowBytes;
       return join_frag(read_tr(lds, p), read_tr(lds, p + 16 * kTileRowBytes));
     }
-    if (!kMixed) return *reinterpret_cast<const bf16x8_t*>(lds + o[kk] + off + i * 2048);
-    const i16x4_t lo = *reinterpret_cast<const i16x4_t*>(lds + o[2 * kk] + off + i * 2048);
-    const i16x4_t hi = *reinterpret_cast<const i16x4_t*>(lds + o[2 * kk + 1] + off + i * 2048);
-    return join_frag(lo, hi);
+    return *reinterpret_cast<const bf16x8_t*>(lds + o[kk] + off + i * 2048);
   }
 };
 
@@ -303,11 +298,11 @@ struct MmTile {
 #pragma unroll
       for (int j = 0; j < MmAcc<kWideB>::kB; ++j) acc.v[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     if (steps <= 0) return;
-    constexpr bool kMixed = kAKc != kBKc;
+    static_assert(kAKc == (kBKc && !kBNative), "one order of the k-slots");
     // x: the wide operand's fragments (half of its blocks), y: the narrow one's.
     bf16x8_t x0[4], x1[4], y0[4], y1[4];
-    MmFrags<kAKc, false, kMixed, MmAcc<kWideB>::kA> ra;
-    MmFrags<kBKc, kBNative, kMixed, MmAcc<kWideB>::kB> rb;
+    MmFrags<kAKc, false, MmAcc<kWideB>::kA> ra;
+    MmFrags<kBKc, kBNative, MmAcc<kWideB>::kB> rb;
     ra.init(0, acc.row0(w), lane);
     rb.init(2 * kMmOperandBytes, acc.col0(w), lane);
     auto read_x = [&](int stage, int kk, int half, bf16x8_t* f, int i) __attribute__((always_inline)) {

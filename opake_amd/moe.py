@@ -12,7 +12,14 @@ Layout: each expert is its own module with two bias-free linear layers
 (``experts.<e>.gate_up`` [2I, d] and ``experts.<e>.down`` [d, I]), so the
 parameter pytree has one leaf per expert and projection and a ``PerGroup``
 can put each expert in its own clipping group.  The router is a frozen
-linear layer; ``forward`` also accepts router logits directly.
+linear layer; ``forward`` also accepts router logits directly.  With ``routing``
+the choice is ``routing.route_topk``'s instead: softmax or sigmoid scores, a
+balancing bias (the buffer ``route_bias``), groups of experts, and masked experts
+(a token left with fewer than ``k`` goes to those alone).
+
+``RoutedLM`` puts such an FFN behind a transformer block, between a frozen
+embedding and a frozen head, and takes its losses from the hidden states with
+``head.linear_cross_entropy`` and ``head.topk_distillation``: no logits are kept.
 
 Dispatch sorts the (token, slot) assignments by expert and, within an
 expert, by token, so expert ``e``'s input rows are its examples' tokens in
@@ -30,6 +37,10 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from opake_amd.head import linear_cross_entropy, topk_distillation
+from opake_amd.routing import route_topk
+from opake_amd.transformer import LlamaBlock
+
 
 class SwiGLUExpert(nn.Module):
     def __init__(self, d: int, inter: int, *, dtype=None, device=None):
@@ -45,10 +56,13 @@ class SwiGLUExpert(nn.Module):
 
 
 class TopKMoE(nn.Module):
-    """``d``-wide top-``k`` MoE FFN with ``n_experts`` SwiGLU experts of width ``inter``."""
+    """``d``-wide top-``k`` MoE FFN with ``n_experts`` SwiGLU experts of width ``inter``.
 
-    def __init__(self, d: int, inter: int, n_experts: int, top_k: int = 2, *, dtype=None,
-                 device=None):
+    ``routing``: keyword arguments of ``route_topk`` (``score``, ``groups``,
+    ``top_groups``, ``renormalize``, ``scale``), which then routes."""
+
+    def __init__(self, d: int, inter: int, n_experts: int, top_k: int = 2, *,
+                 routing: dict | None = None, dtype=None, device=None):
         super().__init__()
         if not 1 <= top_k <= n_experts:
             raise ValueError("top_k must be between 1 and n_experts")
@@ -57,11 +71,18 @@ class TopKMoE(nn.Module):
         self.router.weight.requires_grad_(False)
         self.experts = nn.ModuleList(
             SwiGLUExpert(d, inter, dtype=dtype, device=device) for _ in range(n_experts))
+        self.routing = None if routing is None else dict(routing)
+        if routing is not None:
+            self.register_buffer("route_bias",
+                                 torch.zeros(n_experts, dtype=torch.float32, device=device))
         self.last_counts: torch.Tensor | None = None  # [E, B] host copy of the last routing
 
     def route(self, x: torch.Tensor, router_logits: torch.Tensor | None = None):
-        """Top-k expert indices and weights ([B, T, k] each)."""
+        """Top-k expert indices and weights ([B, T, k] each); -1: none (``routing`` only)."""
         logits = self.router(x) if router_logits is None else router_logits
+        if self.routing is not None:
+            top_w, top_i = route_topk(logits, self.top_k, bias=self.route_bias, **self.routing)
+            return top_i, top_w.to(x.dtype)
         top_v, top_i = torch.topk(logits.float(), self.top_k, dim=-1)
         return top_i, torch.softmax(top_v, dim=-1).to(x.dtype)
 
@@ -71,6 +92,10 @@ class TopKMoE(nn.Module):
         top_i, top_w = self.route(x, router_logits)
         expert = top_i.reshape(-1)
         token = torch.arange(B * T, device=x.device).repeat_interleave(k)
+        weight = top_w.reshape(-1)
+        if self.routing is not None:
+            chosen = expert >= 0
+            expert, token, weight = expert[chosen], token[chosen], weight[chosen]
         order = torch.argsort(expert * (B * T) + token, stable=True)
         counts = torch.bincount(expert * B + token // T, minlength=E * B).view(E, B).cpu()
         self.last_counts = counts
@@ -87,10 +112,56 @@ class TopKMoE(nn.Module):
             mod.down.dpc_row_segments = seg
             outs.append(mod(xs[start:start + n]))
             start += n
-        y = torch.cat(outs) * top_w.reshape(-1)[order].unsqueeze(1)
+        y = torch.cat(outs) * weight[order].unsqueeze(1)
         out = torch.zeros((B * T, d), dtype=torch.float32, device=x.device)
         out.index_add_(0, tok_sorted, y.float())
         return out.to(x.dtype).view(B, T, d)
+
+
+class RoutedLM(nn.Module):
+    """Frozen embedding -> ``LlamaBlock`` -> RMSNorm and ``TopKMoE`` (residual) ->
+    frozen head.  ``forward`` returns hidden states [B, T, d]; ``loss`` takes them.
+
+    For distillation the teacher's top logits and their columns ([B, T, K] each) go
+    in with the tokens, and ``loss`` mixes ``distill`` of KL into the cross entropy:
+
+        fn, state = ghost_clipped_grad(model, model.loss, clipping_norm=1.0)
+        fn((ids, teacher_logits, teacher_indices), targets, state=state)
+    """
+
+    def __init__(self, vocab: int, d: int, n_heads: int, ffn: int, inter: int, n_experts: int,
+                 top_k: int = 2, *, routing: dict | None = None, distill: float = 0.5,
+                 temperature: float = 1.0, ignore_index: int = -100, dtype=None, device=None):
+        super().__init__()
+        kw = dict(dtype=dtype, device=device)
+        self.distill, self.temperature = distill, temperature
+        self.ignore_index = ignore_index
+        self.embed = nn.Embedding(vocab, d, **kw)
+        self.block = LlamaBlock(d, n_heads, ffn, **kw)
+        self.moe_norm = nn.RMSNorm(d, eps=1e-5, **kw)
+        self.moe = TopKMoE(d, inter, n_experts, top_k, routing=routing or {}, **kw)
+        self.head = nn.Linear(d, vocab, bias=False, **kw)
+        self.embed.weight.requires_grad_(False)
+        self.head.weight.requires_grad_(False)
+
+    def forward(self, ids: torch.Tensor, teacher_logits: torch.Tensor | None = None,
+                teacher_indices: torch.Tensor | None = None):
+        x = self.block(self.embed(ids))
+        x = x + self.moe(self.moe_norm(x))
+        return x if teacher_logits is None else (x, teacher_logits, teacher_indices)
+
+    def loss(self, outputs, targets: torch.Tensor) -> torch.Tensor:
+        """Each example's loss [B] (float32): the mean over its tokens.  Tokens whose
+        target is ``ignore_index`` count as zeros."""
+        hidden, teacher = (outputs, None) if torch.is_tensor(outputs) else (outputs[0],
+                                                                             outputs[1:])
+        loss = linear_cross_entropy(hidden, self.head.weight, targets,
+                                    ignore_index=self.ignore_index)
+        if teacher is not None:
+            kl = topk_distillation(hidden, self.head.weight, *teacher,
+                                   temperature=self.temperature)
+            loss = (1.0 - self.distill) * loss + self.distill * kl
+        return loss.mean(dim=1)
 
 
 def expert_groups(model: TopKMoE, prefix: str = "", clipping_norm: float = 1.0):
@@ -110,4 +181,4 @@ def expert_groups(model: TopKMoE, prefix: str = "", clipping_norm: float = 1.0):
     return PerGroup(groups, values)
 
 
-__all__ = ["SwiGLUExpert", "TopKMoE", "expert_groups"]
+__all__ = ["RoutedLM", "SwiGLUExpert", "TopKMoE", "expert_groups"]
