@@ -59,9 +59,7 @@ __shared__ __attribute__((aligned(16))) uint8_t lds_all[kLdsBytes];
 // ---------------------------------------------------------------------------
 
 // float32 as two fp16 planes (mm_tile.h): the shift that brings magnitude `top` (the
-// float's bits) to [2^14, 2^15), and plane p of an x that is already shifted.  Values
-// that fp16 holds as subnormals go to the next plane, which starts 2^-11 lower, so
-// nothing depends on whether the matrix cores keep those.
+// float's bits) to [2^14, 2^15), and plane p of an x that is already shifted.
 constexpr int kDzShift = 14;  // of dz, which is at most 1 (its gradient is applied later)
 
 DPC_DEVICE int half_shift(uint32_t top) {
@@ -69,13 +67,11 @@ DPC_DEVICE int half_shift(uint32_t top) {
   return top == 0 ? 0 : 14 + 127 - (e ? e : 1);
 }
 
-DPC_DEVICE float half_part(float x) { return fabsf(x) < 0x1.0p-14f ? 0.f : (float)(_Float16)x; }
-
 DPC_DEVICE uint16_t half_plane(float x, int p) {
-  if ((__float_as_uint(x) & 0x7f800000u) == 0x7f800000u)  // not finite: plane 0 carries it
-    return p ? 0 : __builtin_bit_cast(uint16_t, (_Float16)x);
-  const float x0 = half_part(x);
-  return __builtin_bit_cast(uint16_t, (_Float16)(p ? half_part((x - x0) * 2048.f) : x0));
+  const _Float16 x0 = (_Float16)x;
+  if (p == 0) return __builtin_bit_cast(uint16_t, x0);
+  const float rest = x - (float)x0;  // not finite: plane 0 carries it
+  return __builtin_bit_cast(uint16_t, (_Float16)(fabsf(x) < INFINITY ? rest : 0.f));
 }
 
 // The rows that have a target, in order: count, active[count], and each row's
@@ -851,7 +847,7 @@ __global__ void __launch_bounds__(kJoinThreads) head_fix_kernel(FixArgs a) {
         half8_t o[2];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float y = fmaf((float)h[t][1][e], 0x1.0p-11f, (float)h[t][0][e]) * x;
+          const float y = ((float)h[t][1][e] + (float)h[t][0][e]) * x;
 #pragma unroll
           for (int pl = 0; pl < 2; ++pl) o[pl][e] = __builtin_bit_cast(_Float16, half_plane(y, pl));
         }
@@ -1480,7 +1476,6 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
   const MmOperand w = a.mm.a;
   a.mm.b = MmOperand{nullptr, p.ld, N * p.ld, 0};
   a.mm.kl = (int)p.ld;
-  a.mm.planes = p.planes;
   a.mm.tiles_a = p.tiles_v;
   a.mm.splits = 1;
   a.V = V;
@@ -1544,8 +1539,7 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
       hipLaunchKernelGGL((head_fix_kernel<true>), fix_grid, dim3(kJoinThreads), 0, s, x);
     DPC_HIP_CHECK(hipGetLastError());
     ProductArgs m = {};
-    m.mm = MmArgs{w, MmOperand{a.e, a.lde, a.plane, 0}, V, p.planes, p.tiles_d, tiles_c,
-                  p.splits_c};
+    m.mm = MmArgs{w, MmOperand{a.e, a.lde, a.plane, 0}, V, p.tiles_d, tiles_c, p.splits_c};
     m.coef = 1.f;
     m.shift = p.planes == 2 ? tops.w : nullptr;
     m.h = a.h;
@@ -1647,7 +1641,7 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
     wpiece.p = w.p + (int64_t)first * w.ld;
     wpiece.rows = cols_here;
     GradArgs a = {};
-    a.mm = MmArgs{wpiece, hop, (int)p.ld, p.planes, tiles, p.tiles_n, 1};
+    a.mm = MmArgs{wpiece, hop, (int)p.ld, tiles, p.tiles_n, 1};
     a.h = h;
     a.V = V;
     a.K = K;
@@ -1687,7 +1681,7 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
       // A = W (D, K-slow: a row holds one vocabulary entry), B = dz by rows.  dz is zero
       // past the vocabulary, and W's rows there read as zeros.
       ProductArgs m = q;
-      m.mm = MmArgs{wpiece, zop, cols_here, p.planes, p.tiles_d, p.tiles_n, p.splits_h};
+      m.mm = MmArgs{wpiece, zop, cols_here, p.tiles_d, p.tiles_n, p.splits_h};
       m.active = rows.active;
       m.plane = N * p.lda;
       const bool direct = p.pieces == 1 && p.splits_h == 1;
@@ -1720,7 +1714,7 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
     }
     if (weight_grad) {
       ProductArgs m = q;
-      m.mm = MmArgs{hop, zop, 0, p.planes, p.tiles_d, tiles, p.splits_w};
+      m.mm = MmArgs{hop, zop, 0, p.tiles_d, tiles, p.splits_w};
       m.rows_b = cols_here;
       m.plane = (int64_t)cols_here * p.lda;
       m.partial = p.splits_w == 1 ? nullptr : reinterpret_cast<float*>(base + p.b_pw);

@@ -15,13 +15,14 @@
 // consecutive A indices sit in a lane's four registers.  A is therefore always
 // the operand whose index is contiguous in the output.
 //
-// float32 operands (kHalf) come as two fp16 planes, x = (x0 + 2^-11 x1) 2^-shift with
-// the shift that brings the tensor's largest magnitude to [2^14, 2^15): x0 is x's
-// rounding to 11 bits, x1 that of what it leaves, so 2^-24 |x| is lost at most.  The K
-// loop takes the plane pairs (0, 1) and (1, 0), scales the accumulators by 2^-11, and
-// goes on with (0, 0); the pair left out is below 2^-24 of the product.  The products are
-// exact and the sums are the MFMA's float32 ones: float32 accuracy at three bf16-rate
-// products, 2500 / 3 TFLOP/s against the float32 matrix instructions' 157.
+// float32 operands (kHalf) come as two fp16 planes, x = (x0 + x1) 2^-shift with the
+// shift that brings the tensor's largest magnitude to [2^14, 2^15): x0 is x's rounding to
+// 11 bits, x1 that of what it leaves.  So 2^-24 |x| is lost, or 2^-39 of the largest where
+// x1 is subnormal (the matrix cores keep fp16's subnormals).  A step of 64 k goes over the
+// plane pairs (0, 1), (1, 0), (0, 0), one after the other while the caches hold them; the
+// pair left out is below 2^-24 of the product.  The products are exact and the sums are
+// the MFMA's float32 ones: float32 accuracy at three bf16-rate products, 2500 / 3
+// TFLOP/s against the float32 matrix instructions' 157.
 #pragma once
 
 #include "lds_stage.h"
@@ -36,7 +37,6 @@ struct MmOperand {
 struct MmArgs {
   MmOperand a, b;
   int kl;      // valid K, K-contiguous operands: a multiple of 8 (zero-padded)
-  int planes;  // 1 (bf16) or 2 (float32)
   int tiles_a, tiles_b;
   int splits;  // the K steps go out in this many slices
 };
@@ -45,9 +45,9 @@ constexpr int kMmTile = 256, kMmStep = 64, kMmThreads = 512, kMmWaves = 8;
 constexpr int kMmOperandBytes = kMmTile * kMmStep * 2;  // 32 KiB
 constexpr int kMmOutOfRange = 0x7ff00000;
 
-// Plane pairs, nibble i of each word: pair i's plane of A and of B (planes 1: pair 2).
+// A step's plane pairs, nibble i of each word: pair i's plane of A and of B.
 constexpr uint32_t kMmPairsA = 0x010u, kMmPairsB = 0x001u;
-constexpr float kMmCross = 0x1.0p-11f;  // of the pairs before the last
+constexpr int kMmPairs = 3;
 
 // K-contiguous tile: rows of 64 k = 128 bytes, eight 16-byte chunks
 // XOR-swizzled by bits 1-3 of the row.  The 64 banks span two rows, so 16
@@ -55,13 +55,6 @@ constexpr float kMmCross = 0x1.0p-11f;  // of the pairs before the last
 // bank groups.
 DPC_DEVICE int mm_kc_off(int row, int chunk) {
   return row * 128 + ((chunk ^ ((row >> 1) & 7)) << 4);
-}
-
-// Steps of a plane pair: an even number for float32, so that the accumulators are
-// scaled between two rounds of the two LDS stages.
-DPC_HOST_DEVICE int mm_pair_steps(int kl, int planes) {
-  const int n = (kl + kMmStep - 1) / kMmStep;
-  return planes == 1 ? n : n + (n & 1);
 }
 
 // Linear id -> (split, tile of A, tile of B); false past the last.  Dispatch is
@@ -125,8 +118,6 @@ struct MmStage {
       }
     }
   }
-  // (A step past kl, or none: nothing is in range.)
-  static DPC_DEVICE uint32_t in_range(int64_t bytes) { return bytes > 0 ? (uint32_t)bytes : 0u; }
   // The step at k0 of plane `pl` of tile t: the buffer it reads, and `bad`, out of the
   // buffer's range for lanes whose k is past kl.  Rows past the operand's are out of
   // range too: all such reads give zeros.  (Native blocks are whole; past their matrix
@@ -144,11 +135,11 @@ struct MmStage {
       bytes = (uint32_t)(4 * kMmBlock * 2 - ((k0 & 255) >> 4) * 1024);
     } else if (kKc) {
       base += (int64_t)i0 * o.ld + k0;
-      bytes = in_range((min(o.rows - i0, kMmTile) * o.ld - k0) * 2);
+      bytes = (uint32_t)((min(o.rows - i0, kMmTile) * o.ld - k0) * 2);
       *bad = k0 + kchunk >= kl ? kMmOutOfRange : 0;
     } else {
       base += (int64_t)k0 * o.ld + i0;
-      bytes = in_range((min(kl - k0, kMmStep) * o.ld - i0) * 2);
+      bytes = (uint32_t)((min(kl - k0, kMmStep) * o.ld - i0) * 2);
     }
     return rsrc_words(base, bytes);
   }
@@ -200,11 +191,15 @@ struct MmFrags {
 // A place in the K loop: plane pair and first k.  `next` stays at the last step
 // past the end, so a pipeline may go on fetching (in range) into a stage that
 // nothing reads.
+template <bool kHalf>
 struct MmPlace {
   int left, pair, k0;
-  DPC_DEVICE MmPlace next(int end) const {  // (selects: no branch in the loop)
-    const int go = left > 1 ? 1 : 0, k = k0 + kMmStep, wrap = k >= end ? 1 : 0;
-    return MmPlace{left - go, pair + (go & wrap), go ? (wrap ? 0 : k) : k0};
+  DPC_DEVICE MmPlace next() const {  // (selects: no branch in the loop)
+    const int go = left > 1 ? 1 : 0;
+    if (!kHalf) return MmPlace{left - go, 0, k0 + (go ? kMmStep : 0)};
+    const int wrap = pair + 1 == kMmPairs ? 1 : 0;
+    return MmPlace{left - go, go ? (wrap ? 0 : pair + 1) : pair,
+                   k0 + (go & wrap ? kMmStep : 0)};
   }
 };
 
@@ -227,9 +222,7 @@ struct MmTile {
   const MmArgs& g;
   uint8_t* lds;
   int lane, w, ta, tb, steps;
-  int end;    // k at which a plane pair ends
-  int cross;  // steps before the pair (0, 0)
-  MmPlace pa, pb;
+  MmPlace<kHalf> pa, pb;
   MmStage<kAKc, false> sa;
   MmStage<kBKc, kBNative> sb;
   u32x4_t buf;
@@ -242,12 +235,12 @@ struct MmTile {
     sb.init(g.b, w, lane);
   }
   DPC_DEVICE void next_a() {
-    buf = sa.buffer(g.a, (kMmPairsA >> (4 * pa.pair)) & 15, ta, pa.k0, g.kl, &bad);
-    pa = pa.next(end);
+    buf = sa.buffer(g.a, kHalf ? (kMmPairsA >> (4 * pa.pair)) & 15 : 0, ta, pa.k0, g.kl, &bad);
+    pa = pa.next();
   }
   DPC_DEVICE void next_b() {
-    buf = sb.buffer(g.b, (kMmPairsB >> (4 * pb.pair)) & 15, tb, pb.k0, g.kl, &bad);
-    pb = pb.next(end);
+    buf = sb.buffer(g.b, kHalf ? (kMmPairsB >> (4 * pb.pair)) & 15 : 0, tb, pb.k0, g.kl, &bad);
+    pb = pb.next();
   }
   DPC_DEVICE void fetch_a(int stage, int j) {
     sa.issue(buf, bad, lds_addr(lds) + stage * kMmOperandBytes, w, j);
@@ -268,18 +261,14 @@ struct MmTile {
   DPC_DEVICE void begin(int tile_a, int tile_b, int split) {
     ta = tile_a;
     tb = tile_b;
-    const int ks = mm_pair_steps(g.kl, g.planes);
-    end = ks * kMmStep;
-    // Slices of whole rounds of two steps (float32; bf16: of steps).
-    const long long rounds = kHalf ? 3ll * ks / 2 : ks;
-    const int each = kHalf ? 2 : 1;
-    const int s0 = __builtin_amdgcn_readfirstlane((int)(rounds * split / g.splits) * each),
-              s1 = __builtin_amdgcn_readfirstlane((int)(rounds * (split + 1) / g.splits) * each);
+    const long long all =
+        (long long)((g.kl + kMmStep - 1) / kMmStep) * (kHalf ? kMmPairs : 1);
+    const int s0 = __builtin_amdgcn_readfirstlane((int)(all * split / g.splits)),
+              s1 = __builtin_amdgcn_readfirstlane((int)(all * (split + 1) / g.splits));
     steps = s1 - s0;
     if (steps <= 0) return;
-    const int pair0 = kHalf ? __builtin_amdgcn_readfirstlane(s0 / ks) : 2;
-    cross = kHalf ? max(0, min(steps, 2 * ks - s0)) : 0;
-    pa = MmPlace{steps, pair0, kHalf ? (s0 - pair0 * ks) * kMmStep : s0 * kMmStep};
+    const int step0 = kHalf ? s0 / kMmPairs : s0;
+    pa = MmPlace<kHalf>{steps, s0 - step0 * (kHalf ? kMmPairs : 1), step0 * kMmStep};
     pb = pa;
     next_a();
 #pragma unroll
@@ -371,12 +360,6 @@ struct MmTile {
     for (; s + 1 < steps; s += 2) {
       step(0, 1);
       step(1, 0);
-      if (kHalf && s + 2 == cross) {
-#pragma unroll
-        for (int i = 0; i < MmAcc<kWideB>::kA; ++i)
-#pragma unroll
-          for (int j = 0; j < MmAcc<kWideB>::kB; ++j) acc.v[i][j] *= kMmCross;
-      }
     }
     if (s < steps) step(0, 1);
     DPC_WAIT_VMCNT(0);
