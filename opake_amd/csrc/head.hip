@@ -194,7 +194,7 @@ struct PrepArgs {
   uint16_t* w;
   bool pack;
   Tops tops;     // float32
-  uint16_t* hg;          // float32, for dW: planes of H times the losses' gradient over gmax
+  uint16_t* hg;        // float32, for dW: planes of H times the losses' gradient over gmax
   const int64_t* index;
   bool teacher;
   int blocks, parts;
@@ -417,12 +417,14 @@ __global__ void __launch_bounds__(kPrepThreads) prep_kernel(PrepArgs a) {
   const int64_t chunks = a.ld / 8;
   const bool f32 = a.dtype == DPC_F32;
   const int shift_h = f32 ? half_shift(*a.tops.h) : 0, shift_w = f32 ? half_shift(*a.tops.w) : 0;
-  if (a.h && (a.pack || count < a.N))
+  const bool pack_h = a.h && (a.pack || count < a.N);
+  if (pack_h || a.hg)
     for (int64_t i = t0; i < count * chunks; i += step) {
       const int64_t c = i / chunks;
       const int at = (int)(i - c * chunks) * 8;
-      pack_chunk(a.hidden, a.dtype, a.rows.active[c], a.D, at, a.ld, a.N * a.ld, a.h, c,
-                 f32 ? half_shift(a.tops.row[c]) : 0, 1.f);
+      if (pack_h)
+        pack_chunk(a.hidden, a.dtype, a.rows.active[c], a.D, at, a.ld, a.N * a.ld, a.h, c,
+                   f32 ? half_shift(a.tops.row[c]) : 0, 1.f);
       if (a.hg)
         pack_chunk(a.hidden, a.dtype, a.rows.active[c], a.D, at, a.ld, a.N * a.ld, a.hg, c,
                    shift_h, a.g_over[c]);
@@ -554,11 +556,10 @@ DPC_DEVICE float entry_values(const MmAcc<false>& acc, uint32_t y, bool on) {
 
 template <bool kEmit, bool kHalf>
 DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, const f32x4_t& factor,
-                               int N, int ta, int tb, int64_t g0, const uint2* list, int e0,
-                               int e1, uint2 first) {
+                               int N, int ta, int tb, int w, int64_t g0, const uint2* list,
+                               int e0, int e1, uint2 first) {
 #pragma clang fp contract(off)  // the difference is of the rounded logit and its maximum
-  const int lane = epilogue_lane(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
-            wm = w & 1, wn = w >> 1;
+  const int lane = epilogue_lane(), wm = w & 1, wn = w >> 1;
   const int v0 = ta * kMmTile, n0 = tb * kMmTile;
   const int vl = wm * 128 + 4 * (lane >> 4);  // + 16 i + r
   const int tl = wn * 64 + (lane & 15);       // + 16 j
@@ -634,6 +635,34 @@ DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, const f32x
   }
 }
 
+// A wave's entries of a tile, in a list by row block, tile and wave: [e0, e1), the first
+// 64 of them.
+struct WaveEntries {
+  const uint2* list;
+  int e0, e1;
+  uint2 first;
+  DPC_DEVICE WaveEntries(const Entries& e, int K, int tiles_v, int vt, int64_t block, int w,
+                         int lane) {
+    const int32_t* start = e.start + block * (8 * tiles_v + 1) + 8 * vt + w;
+    list = e.list + block * kMmTile * K;
+    e0 = start[0];
+    e1 = start[1];
+    first = e0 < e1 ? list[min(e0 + lane, e1 - 1)] : make_uint2(0u, 0u);
+  }
+};
+
+// What the products of the lane's rows are to be multiplied by (float32).
+DPC_DEVICE f32x4_t row_factors(const StatsArgs& s, int N, int tb, int w, uint32_t top_w) {
+  const int lane = epilogue_lane();
+  f32x4_t f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int n = tb * kMmTile + (w >> 1) * 64 + 16 * j + (lane & 15);
+    f[j] = logit_factor(s.inv_tau, n < N ? s.tops.row[s.h.first + n] : 0u, top_w);
+  }
+  return f;
+}
+
 template <bool kEmit, bool kHalf>
 __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -649,31 +678,90 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
   while (more) {
     ta = ta2;
     tb = tb2;
-    // The wave's entries, the first 64 loaded beside the product.
     const int64_t g0 = s.h.first + (int64_t)tb * kMmTile;  // the first row's number
-    const int32_t* start = s.entries.start + (g0 / kMmTile) * (8 * s.mm.tiles_a + 1) + 8 * ta + w;
-    const uint2* list = s.entries.list + g0 * s.K;
-    const int e0 = start[0], e1 = start[1];
-    uint2 first = e0 < e1 ? list[min(e0 + lane, e1 - 1)] : make_uint2(0u, 0u);
+    WaveEntries own(s.entries, s.K, s.mm.tiles_a, ta, g0 / kMmTile, w, lane);
     tile.run(acc);
     f32x4_t factor = {};
     if constexpr (kHalf) {
-      const int late = epilogue_lane();
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = tb * kMmTile + (w >> 1) * 64 + 16 * j + (late & 15);
-        const uint32_t top = n < N ? s.tops.row[s.h.first + n] : 0u;
-        factor[j] = logit_factor(s.inv_tau, top, top_w);
-      }
+      factor = row_factors(s, N, tb, w, top_w);
       arrived(factor);
     }
-    arrived(first.x);
-    arrived(first.y);
+    arrived(own.first.x);
+    arrived(own.first.y);
     id += gridDim.x;
     more = mm_tile_of(s.mm, id, &split, &ta2, &tb2);
     if (more) tile.begin(ta2, tb2, 0);
-    stats_epilogue<kEmit, kHalf>(s, acc, factor, N, ta, tb, g0, list, e0, e1, first);
+    stats_epilogue<kEmit, kHalf>(s, acc, factor, N, ta, tb, w, g0, own.list, own.e0, own.e1,
+                                 own.first);
   }
+}
+
+// Few tiles (few rows, or a small vocabulary): the products' K steps in slices, each
+// slice's accumulators left as they are held ([slice][tile][wave][block][lane]), then
+// the same epilogues by single waves that add them up in order.  Rows past the last
+// are neither written nor read.
+struct LogitsArgs {
+  MmArgs mm;
+  Hidden h;
+  f32x4_t* z;
+  int tiles;  // of a slice
+};
+
+DPC_DEVICE int64_t logits_at(int64_t tile, int w) { return (tile * 8 + w) * 32 * 64; }
+
+template <bool kHalf>
+__global__ void __launch_bounds__(kMmThreads, 1) head_logits_kernel(LogitsArgs s) {
+  const int N = hidden_rows(s.h, &s.mm.b.p);
+  s.mm.b.rows = N;
+  s.mm.tiles_b = tiles_of(N);
+  int split, ta, tb;
+  if (!mm_tile_of(s.mm, blockIdx.x, &split, &ta, &tb)) return;
+  MmTile<true, true, false, false, kHalf> tile(s.mm, lds_all);
+  MmAcc<false> acc;
+  tile.begin(ta, tb, split);
+  tile.run(acc);
+  const int lane = epilogue_lane(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  f32x4_t* z = s.z + logits_at((int64_t)split * s.tiles + tb * s.mm.tiles_a + ta, w) + lane;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (tb * kMmTile + (w >> 1) * 64 + 16 * j < N)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[(j * 8 + i) * 64] = acc.v[i][j];
+}
+
+DPC_DEVICE void add_logits(const f32x4_t* z, int slices, int tiles, int64_t tile, int w, int row0,
+                           int N, MmAcc<false>& acc) {
+  const int lane = epilogue_lane();
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc.v[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < slices; ++s) {
+    const f32x4_t* from = z + logits_at((int64_t)s * tiles + tile, w) + lane;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (row0 + 16 * j < N)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc.v[i][j] += from[(j * 8 + i) * 64];
+  }
+}
+
+template <bool kEmit, bool kHalf>
+__global__ void __launch_bounds__(64) head_split_stats_kernel(StatsArgs s, const f32x4_t* z,
+                                                              int slices, int tiles) {
+  const int id = blockIdx.x >> 3, w = blockIdx.x & 7, tb = id / s.mm.tiles_a,
+            ta = id - tb * s.mm.tiles_a;
+  const uint16_t* unused;
+  const int N = hidden_rows(s.h, &unused);
+  if (tb * kMmTile >= N) return;
+  const int64_t g0 = s.h.first + (int64_t)tb * kMmTile;
+  const WaveEntries own(s.entries, s.K, s.mm.tiles_a, ta, g0 / kMmTile, w, threadIdx.x);
+  MmAcc<false> acc;
+  add_logits(z, slices, tiles, id, w, tb * kMmTile + (w >> 1) * 64, N, acc);
+  f32x4_t factor = {};
+  if constexpr (kHalf) factor = row_factors(s, N, tb, w, *s.tops.w);
+  stats_epilogue<kEmit, kHalf>(s, acc, factor, N, ta, tb, w, g0, own.list, own.e0, own.e1,
+                               own.first);
 }
 
 DPC_DEVICE float wave_max(float v) {
@@ -796,8 +884,8 @@ __global__ void __launch_bounds__(kJoinThreads) head_join_kernel(JoinArgs a) {
   }
 }
 
-// A chunk's exp(z - half's maximum) times exp(half's maximum - lse), in place, and p - q
-// at the entries' columns: 16 rows x 8 tiles a workgroup.  The 16 rows are 1 KiB of every
+// exp(z - half's maximum) times exp(half's maximum - lse), and p - q at the entries'
+// columns: 16 rows x 8 tiles a workgroup.  The 16 rows are 1 KiB of every
 // 32 columns; a wave takes one of each tile's eight, all its loads in flight at once.
 constexpr int kFixTiles = 8;
 
@@ -809,7 +897,9 @@ struct FixArgs {
   const f32x2_t* part;
   const float* lse;
   const float* corr;
-  uint16_t* e;
+  const float* g;  // [rows] to be multiplied by, or null
+  const uint16_t* e;
+  uint16_t* out;   // may be e
   int64_t lde, plane;
 };
 
@@ -818,15 +908,17 @@ __global__ void __launch_bounds__(kJoinThreads) head_fix_kernel(FixArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int local = blockIdx.x * kJoinRows;  // first row in the chunk
   const int64_t n0 = a.first + local, count = *a.count;
-  if (n0 >= count) return;
-  const int rows = (int)(count - n0 < kJoinRows ? count - n0 : kJoinRows);
+  // Rows past the last are zeros as far as a K step of dW reads.
+  if (n0 >= (count + kMmStep - 1) / kMmStep * kMmStep) return;
+  const int rows = max(0, (int)(count - n0 < kJoinRows ? count - n0 : kJoinRows));
   const int t0 = blockIdx.y * kFixTiles, tiles = min(kFixTiles, a.tiles - t0);
   typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-  uint16_t* block = a.e + (local >> 8) * a.lde * kMmBlock + ((local & 255) >> 4) * 512;
-  uint16_t* at = block + (4 * t0 + (w >> 1)) * kMmBlock + (w & 1) * 8192 + lane * 8;
+  const int64_t block = (local >> 8) * a.lde * kMmBlock + ((local & 255) >> 4) * 512;
+  const int64_t at = block + (4 * t0 + (w >> 1)) * kMmBlock + (w & 1) * 8192 + lane * 8;
+  const bool live = (lane & 15) < rows;
   const int64_t n = n0 + min(lane & 15, rows - 1);
   const f32x2_t* top = a.part + (2 * t0 + (w >> 2)) * a.N + n;
-  const float lse = a.lse[n];
+  const float lse = a.lse[n], g = a.g ? a.g[n] : 1.f;
   constexpr int kPlanes = kHalf ? 2 : 1;
   half8_t h[kFixTiles][kPlanes];
   float f[kFixTiles];
@@ -835,19 +927,19 @@ __global__ void __launch_bounds__(kJoinThreads) head_fix_kernel(FixArgs a) {
     if (t < tiles) {
 #pragma unroll
       for (int pl = 0; pl < kPlanes; ++pl)
-        h[t][pl] = *reinterpret_cast<const half8_t*>(at + pl * a.plane + 4 * t * kMmBlock);
+        h[t][pl] = *reinterpret_cast<const half8_t*>(a.e + at + pl * a.plane + 4 * t * kMmBlock);
       f[t] = top[2 * t * a.N].x;
     }
 #pragma unroll
   for (int t = 0; t < kFixTiles; ++t)
     if (t < tiles) {
-      const float x = exp2_fast(f[t] - lse);
-      uint16_t* to = at + 4 * t * kMmBlock;
+      const float x = exp2_fast(f[t] - lse) * g;
+      uint16_t* to = a.out + at + 4 * t * kMmBlock;
       if constexpr (kHalf) {
         half8_t o[2];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float y = ((float)h[t][1][e] + (float)h[t][0][e]) * x;
+          const float y = live ? ((float)h[t][1][e] + (float)h[t][0][e]) * x : 0.f;
 #pragma unroll
           for (int pl = 0; pl < 2; ++pl) o[pl][e] = __builtin_bit_cast(_Float16, half_plane(y, pl));
         }
@@ -857,7 +949,9 @@ __global__ void __launch_bounds__(kJoinThreads) head_fix_kernel(FixArgs a) {
         u32x4_t o;
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          o[e] = f32x2_to_bf16x2_bits((float)h[t][0][2 * e] * x, (float)h[t][0][2 * e + 1] * x);
+          o[e] = live ? f32x2_to_bf16x2_bits((float)h[t][0][2 * e] * x,
+                                             (float)h[t][0][2 * e + 1] * x)
+                      : 0u;
         *reinterpret_cast<u32x4_t*>(to) = o;
       }
     }
@@ -865,9 +959,10 @@ __global__ void __launch_bounds__(kJoinThreads) head_fix_kernel(FixArgs a) {
   for (int i = tid; i < rows * a.K; i += kJoinThreads) {
     const int c = a.cols[n0 * a.K + i];
     if (c >= 0 && (c >> 8) >= t0 && (c >> 8) < t0 + tiles) {
-      uint16_t* to = block + (c >> 6) * kMmBlock + ((c >> 5) & 1) * 8192 + ((c >> 2) & 3) * 128 +
-                     (i / a.K) * 8 + ((c >> 4) & 1) * 4 + (c & 3);
-      const float x = a.corr[n0 * a.K + i];
+      const int r = i / a.K;
+      uint16_t* to = a.out + block + (c >> 6) * kMmBlock + ((c >> 5) & 1) * 8192 +
+                     ((c >> 2) & 3) * 128 + r * 8 + ((c >> 4) & 1) * 4 + (c & 3);
+      const float x = a.corr[n0 * a.K + i] * (a.g ? a.g[n0 + r] : 1.f);
 #pragma unroll
       for (int pl = 0; pl < kPlanes; ++pl)
         to[pl * a.plane] = kHalf ? half_plane(ldexpf(x, kDzShift), pl) : f32_to_bf16_bits(x);
@@ -946,12 +1041,11 @@ DPC_DEVICE float entry_change(const GradArgs& s, int tb, uint2 x) {
 }
 
 template <bool kHalf>
-DPC_DEVICE void grad_epilogue(const GradArgs& s, MmAcc<false>& acc, int ta, int tb,
+DPC_DEVICE void grad_epilogue(const GradArgs& s, MmAcc<false>& acc, int ta, int tb, int w,
                               const f32x4_t& lse, const f32x4_t& g, const uint2* list, int e0,
                               int e1, uint2 first, float change) {
 #pragma clang fp contract(off)  // the forward's rounded logit
-  const int lane = epilogue_lane(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6),
-            wm = w & 1, wn = w >> 1;
+  const int lane = epilogue_lane(), wm = w & 1, wn = w >> 1;
   const int vt = s.tile0 + ta;
   const int vleft = s.V - vt * kMmTile - wm * 128 - 4 * (lane >> 4);
 #pragma unroll
@@ -1024,6 +1118,24 @@ DPC_DEVICE void grad_epilogue(const GradArgs& s, MmAcc<false>& acc, int ta, int 
   }
 }
 
+// What the epilogue needs of the wave's rows.
+struct GradRows {
+  f32x4_t lse, g;
+  template <bool kHalf>
+  DPC_DEVICE void load(const GradArgs& s, int N, int tb, int w, uint32_t top_w) {
+    const int lane = epilogue_lane();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = tb * kMmTile + (w >> 1) * 64 + 16 * j + (lane & 15);
+      lse[j] = n < N ? s.lse[n] : 0.f;
+      if constexpr (kHalf)
+        g[j] = logit_factor(s.inv_tau, n < N ? s.tops.row[n] : 0u, top_w);
+      else
+        g[j] = n < N ? s.g[n] : 0.f;
+    }
+  }
+};
+
 template <bool kHalf>
 __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1039,33 +1151,40 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
   while (more) {
     ta = ta2;
     tb = tb2;
-    const int32_t* start =
-        s.entries.start + (int64_t)tb * (8 * s.tiles + 1) + 8 * (s.tile0 + ta) + w;
-    const uint2* list = s.entries.list + (int64_t)tb * kMmTile * s.K;
-    const int e0 = start[0], e1 = start[1];
-    uint2 first = e0 < e1 ? list[min(e0 + lane, e1 - 1)] : make_uint2(0u, 0u);
+    WaveEntries own(s.entries, s.K, s.tiles, s.tile0 + ta, tb, w, lane);
     tile.run(acc);
-    f32x4_t lse, g;
-    float change = e0 < e1 ? entry_change<kHalf>(s, tb, first) : 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = tb * kMmTile + (w >> 1) * 64 + 16 * j + (lane & 15);
-      lse[j] = n < N ? s.lse[n] : 0.f;
-      if constexpr (kHalf)
-        g[j] = logit_factor(s.inv_tau, n < N ? s.tops.row[n] : 0u, top_w);
-      else
-        g[j] = n < N ? s.g[n] : 0.f;
-    }
-    arrived(first.x);
-    arrived(first.y);
-    arrived(lse);
-    arrived(g);
+    GradRows rows;
+    float change = own.e0 < own.e1 ? entry_change<kHalf>(s, tb, own.first) : 0.f;
+    rows.load<kHalf>(s, N, tb, w, top_w);
+    arrived(own.first.x);
+    arrived(own.first.y);
+    arrived(rows.lse);
+    arrived(rows.g);
     arrived(change);
     id += gridDim.x;
     more = mm_tile_of(s.mm, id, &split, &ta2, &tb2);
     if (more) tile.begin(ta2, tb2, 0);
-    grad_epilogue<kHalf>(s, acc, ta, tb, lse, g, list, e0, e1, first, change);
+    grad_epilogue<kHalf>(s, acc, ta, tb, w, rows.lse, rows.g, own.list, own.e0, own.e1, own.first,
+                         change);
   }
+}
+
+template <bool kHalf>
+__global__ void __launch_bounds__(64) head_split_grad_kernel(GradArgs s, const f32x4_t* z,
+                                                             int slices, int tiles) {
+  const int id = blockIdx.x >> 3, w = blockIdx.x & 7, tb = id / s.mm.tiles_a,
+            ta = id - tb * s.mm.tiles_a;
+  const uint16_t* unused;
+  const int N = hidden_rows(s.h, &unused);
+  if (tb * kMmTile >= N) return;
+  const WaveEntries own(s.entries, s.K, s.tiles, s.tile0 + ta, tb, w, threadIdx.x);
+  const float change = own.e0 < own.e1 ? entry_change<kHalf>(s, tb, own.first) : 0.f;
+  MmAcc<false> acc;
+  add_logits(z, slices, tiles, id, w, tb * kMmTile + (w >> 1) * 64, N, acc);
+  GradRows rows;
+  rows.load<kHalf>(s, N, tb, w, kHalf ? *s.tops.w : 0u);
+  grad_epilogue<kHalf>(s, acc, ta, tb, w, rows.lse, rows.g, own.list, own.e0, own.e1, own.first,
+                       change);
 }
 
 // ---------------------------------------------------------------------------
@@ -1226,6 +1345,17 @@ int slices(int64_t tiles, int64_t steps) {
   return s < 1 ? 1 : (int)s;
 }
 
+// The logits' K steps in slices where their tiles leave compute units idle.  A step
+// takes 1.2 us, adding up a slice 1.3 us for a tile's 256 rows: the number of slices that
+// makes the sum of both least.
+int logit_slices(int64_t tiles, int64_t steps, int64_t N) {
+  const int64_t rows = N < kMmTile ? N : kMmTile;
+  int64_t s = (int64_t)sqrt((double)steps * kMmTile / (double)rows);
+  if (s > kUnits / tiles) s = kUnits / tiles;
+  if (s > steps / 4) s = steps / 4;
+  return s < 2 ? 1 : (int)s;
+}
+
 bool valid_head(int64_t N, int D, int V, int K, int dtype) {
   return N >= 0 && N <= 0x7fffff00ll && D >= 1 && D <= (1 << 20) && V >= 1 &&
          V <= kMaxTiles * kMmTile && K >= 1 && K <= (1 << 16) &&
@@ -1243,12 +1373,14 @@ struct Plan {
   int64_t lda;
   int chunk, splits_c;           // emit: rows of a chunk, slices of its product
   int piece_tiles, pieces;       // backward
-  int splits_h, splits_w;
+  int splits_h, splits_w, splits_z, splits_g;
+  bool held;  // dz for g = 1 is kept in the state
   // Byte offsets: state (kept for the backward), workspaces.
-  int64_t s_rows, s_tops, s_lse, s_corr, s_list, s_start, s_unit, state_bytes;
-  int64_t f_rows, f_tops, f_lse, f_corr, f_list, f_start, f_cols, f_h, f_w, f_picked, f_part, f_e, f_pc,
-      fwd_bytes;
-  int64_t b_h, b_w, b_hg, b_g, b_dz, b_ph, b_pw, bwd_bytes;
+  int64_t s_rows, s_tops, s_lse, s_corr, s_list, s_start, s_cols, s_part, s_unit, s_e,
+      state_bytes;
+  int64_t f_rows, f_tops, f_lse, f_corr, f_list, f_start, f_cols, f_h, f_w, f_picked, f_part, f_e,
+      f_pc, f_z, fwd_bytes;
+  int64_t b_h, b_w, b_hg, b_g, b_dz, b_z, b_ph, b_pw, bwd_bytes;
 };
 
 Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w) {
@@ -1261,13 +1393,15 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
   p.planes = dtype == DPC_F32 ? 2 : 1;
   p.want_h = want_h != 0;
   p.want_w = want_w != 0;
-  p.emit = p.want_h && !p.want_w;
   p.ld = up(D, 8);
   p.pack = dtype == DPC_F32 || D % 8 != 0;
   p.tiles_v = (V + kMmTile - 1) / kMmTile;
   p.tiles_n = (int)((N + kMmTile - 1) / kMmTile);
   p.tiles_d = (D + kMmTile - 1) / kMmTile;
   p.lda = up(D, 4);
+  const int64_t row_bytes = p.planes * (int64_t)p.tiles_v * kMmTile * 2;  // of dz
+  p.held = p.want_w && p.tiles_n * kMmTile * row_bytes <= kPieceBytes;
+  p.emit = (p.held && p.planes == 2) || (p.want_h && !p.want_w);
   const int pairs = p.planes == 1 ? 1 : 3;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -1288,7 +1422,12 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
     p.s_list = take(list_b);
     p.s_start = take(start_b);
   }
-  if (p.emit) p.s_unit = take(N * D * 4);
+  if (keep && p.held) {
+    p.s_cols = take(N * K * 4);
+    p.s_part = take(N * p.tiles_v * 16);
+  }
+  if (p.emit && p.want_h) p.s_unit = take(N * D * 4);
+  if (p.held) p.s_e = take(p.tiles_n * kMmTile * row_bytes);
   p.state_bytes = at;
   at = 0;
   if (!p.want_h && !p.want_w) {
@@ -1301,13 +1440,14 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
     p.f_list = take(list_b);
     p.f_start = take(start_b);
   }
-  p.f_cols = take(N * K * 4);
+  if (!(keep && p.held)) {
+    p.f_cols = take(N * K * 4);
+    p.f_part = take(N * p.tiles_v * 16);
+  }
   p.f_h = take(p.planes * N * p.ld * 2);
   if (p.pack) p.f_w = take(p.planes * (int64_t)V * p.ld * 2);
   p.f_picked = take(N * K * 4);
-  p.f_part = take(N * p.tiles_v * 16);
   if (p.emit) {
-    const int64_t row_bytes = p.planes * (int64_t)p.tiles_v * kMmTile * 2;
     int64_t c = kPieceBytes / row_bytes / kMmTile * kMmTile;
     if (c < kMmTile) c = kMmTile;
     // Chunks of equal size.
@@ -1316,11 +1456,20 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
     const int64_t n = (rows + c - 1) / c;
     p.chunk = (int)up((rows + n - 1) / n, kMmTile);
     p.splits_c = slices((int64_t)p.tiles_d * (p.chunk / kMmTile), pairs * (int64_t)p.tiles_v * 4);
-    p.f_e = take(p.chunk * row_bytes);
-    if (p.splits_c > 1) p.f_pc = take(p.splits_c * p.chunk * p.lda * 4);
+    if (!p.held) p.f_e = take(p.chunk * row_bytes);
+    if (p.want_h && p.splits_c > 1) p.f_pc = take(p.splits_c * p.chunk * p.lda * 4);
   }
+  const int64_t z_tiles = (int64_t)p.tiles_v * (p.emit ? p.chunk / kMmTile : p.tiles_n);
+  p.splits_z = logit_slices(z_tiles, pairs * up(D, kMmStep) / kMmStep, N);
+  if (p.splits_z > 1) p.f_z = take(p.splits_z * z_tiles * kMmTile * kMmTile * 4);
   p.fwd_bytes = at;
   at = 0;
+  if (p.held && p.emit) {
+    p.b_hg = take(p.planes * N * p.ld * 2);
+    p.b_g = take(4 + N * 4);
+    p.splits_w = slices((int64_t)p.tiles_d * p.tiles_v, pairs * ((N + 63) / 64));
+    if (p.splits_w > 1) p.b_pw = take(p.splits_w * (int64_t)V * p.lda * 4);
+  }
   if (keep) {
     p.b_h = take(p.planes * N * p.ld * 2);
     if (p.pack) p.b_w = take(p.planes * (int64_t)V * p.ld * 2);
@@ -1334,6 +1483,9 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
     p.piece_tiles = (p.tiles_v + p.pieces - 1) / p.pieces;
     p.pieces = (p.tiles_v + p.piece_tiles - 1) / p.piece_tiles;
     p.b_dz = take(p.planes * rows * p.piece_tiles * kMmTile * 2);
+    const int64_t piece = (int64_t)p.tiles_n * p.piece_tiles;
+    p.splits_g = p.held ? 1 : logit_slices(piece, pairs * up(D, kMmStep) / kMmStep, N);
+    if (p.splits_g > 1) p.b_z = take(p.splits_g * piece * kMmTile * kMmTile * 4);
     if (p.want_h) {
       p.splits_h = slices((int64_t)p.tiles_d * p.tiles_n, (int64_t)pairs * p.piece_tiles * 4);
       if (p.pieces > 1 || p.splits_h > 1) p.b_ph = take(p.splits_h * N * p.lda * 4);
@@ -1397,6 +1549,116 @@ int reduce(const ReduceArgs& a, hipStream_t s) {
 // Workgroups that go through `tiles` tiles, one a compute unit (LDS holds one).
 dim3 tile_grid(int64_t tiles) { return dim3((unsigned)(tiles < kUnits ? tiles : kUnits)); }
 
+// The statistics of a launch's tiles (`tiles_b` row blocks at most).
+template <bool kEmit>
+int stats(const Plan& p, const StatsArgs& a, int tiles_b, f32x4_t* z, hipStream_t s) {
+  const bool half = p.planes == 2;
+  const int64_t tiles = (int64_t)p.tiles_v * tiles_b;
+  if (p.splits_z > 1) {
+    LogitsArgs l = {a.mm, a.h, z, (int)tiles};
+    l.mm.splits = p.splits_z;
+    const dim3 grid((unsigned)(tiles * p.splits_z)), waves((unsigned)(tiles * 8));
+    if (half) {
+      hipLaunchKernelGGL((head_logits_kernel<true>), grid, dim3(kMmThreads), 0, s, l);
+      DPC_HIP_CHECK(hipGetLastError());
+      hipLaunchKernelGGL((head_split_stats_kernel<kEmit, true>), waves, dim3(64), 0, s, a, z,
+                         p.splits_z, (int)tiles);
+    } else {
+      hipLaunchKernelGGL((head_logits_kernel<false>), grid, dim3(kMmThreads), 0, s, l);
+      DPC_HIP_CHECK(hipGetLastError());
+      hipLaunchKernelGGL((head_split_stats_kernel<kEmit, false>), waves, dim3(64), 0, s, a, z,
+                         p.splits_z, (int)tiles);
+    }
+  } else if (half) {
+    hipLaunchKernelGGL((head_stats_kernel<kEmit, true>), tile_grid(tiles), dim3(kMmThreads), 0, s,
+                       a);
+  } else {
+    hipLaunchKernelGGL((head_stats_kernel<kEmit, false>), tile_grid(tiles), dim3(kMmThreads), 0, s,
+                       a);
+  }
+  DPC_HIP_CHECK(hipGetLastError());
+  return DPC_OK;
+}
+
+int fix(const Plan& p, const FixArgs& a, int64_t rows, hipStream_t s) {
+  const dim3 grid((unsigned)(rows / kJoinRows),
+                  (unsigned)((p.tiles_v + kFixTiles - 1) / kFixTiles));
+  if (p.planes == 1)
+    hipLaunchKernelGGL((head_fix_kernel<false>), grid, dim3(kJoinThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL((head_fix_kernel<true>), grid, dim3(kJoinThreads), 0, s, a);
+  DPC_HIP_CHECK(hipGetLastError());
+  return DPC_OK;
+}
+
+// dz of a piece of the vocabulary.
+int gradients(const Plan& p, const GradArgs& a, f32x4_t* z, hipStream_t s) {
+  const bool half = p.planes == 2;
+  const int64_t tiles = (int64_t)a.mm.tiles_a * p.tiles_n;
+  if (p.splits_g > 1) {
+    LogitsArgs l = {a.mm, a.h, z, (int)tiles};
+    l.mm.splits = p.splits_g;
+    const dim3 grid((unsigned)(tiles * p.splits_g)), waves((unsigned)(tiles * 8));
+    if (half) {
+      hipLaunchKernelGGL((head_logits_kernel<true>), grid, dim3(kMmThreads), 0, s, l);
+      DPC_HIP_CHECK(hipGetLastError());
+      hipLaunchKernelGGL((head_split_grad_kernel<true>), waves, dim3(64), 0, s, a, z, p.splits_g,
+                         (int)tiles);
+    } else {
+      hipLaunchKernelGGL((head_logits_kernel<false>), grid, dim3(kMmThreads), 0, s, l);
+      DPC_HIP_CHECK(hipGetLastError());
+      hipLaunchKernelGGL((head_split_grad_kernel<false>), waves, dim3(64), 0, s, a, z, p.splits_g,
+                         (int)tiles);
+    }
+  } else if (half) {
+    hipLaunchKernelGGL((head_grad_kernel<true>), tile_grid(tiles), dim3(kMmThreads), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((head_grad_kernel<false>), tile_grid(tiles), dim3(kMmThreads), 0, s, a);
+  }
+  DPC_HIP_CHECK(hipGetLastError());
+  return DPC_OK;
+}
+
+// dW's rows of a piece of the vocabulary (`cols` of them, in `tiles`) from its dz, and H.
+int weight_product(const Plan& p, const PrepArgs& g, const Hidden& h, const MmOperand& dz,
+                   const Tops& tops, int cols, int tiles, float coef, float* partial,
+                   void* out, hipStream_t s) {
+  const bool half = p.planes == 2;
+  ProductArgs m = {};
+  m.mm = MmArgs{MmOperand{nullptr, p.ld, p.N * p.ld, 0}, dz, 0, p.tiles_d, tiles, p.splits_w};
+  m.h = h;
+  m.rows_a = p.D;
+  m.rows_b = cols;
+  m.lda = p.lda;
+  m.plane = (int64_t)cols * p.lda;
+  m.scale = g.gmax;
+  m.coef = coef;
+  m.shift = half ? tops.h : nullptr;
+  m.partial = p.splits_w == 1 ? nullptr : partial;
+  m.out = out;
+  m.out_bf16 = p.dtype == DPC_BF16;
+  const dim3 grid((unsigned)(p.tiles_d * tiles * p.splits_w));
+  if (half)
+    hipLaunchKernelGGL((head_product_kernel<false, true>), grid, dim3(kMmThreads), 0, s, m);
+  else
+    hipLaunchKernelGGL((head_product_kernel<false, false>), grid, dim3(kMmThreads), 0, s, m);
+  DPC_HIP_CHECK(hipGetLastError());
+  if (!m.partial) return DPC_OK;
+  ReduceArgs r = {};
+  r.partial = m.partial;
+  r.splits = p.splits_w;
+  r.plane = m.plane;
+  r.rows = cols;
+  r.lda = p.lda;
+  r.scale = m.scale;
+  r.coef = coef;
+  r.shift = m.shift;
+  r.D = p.D;
+  r.out_bf16 = m.out_bf16;
+  r.out = out;
+  return reduce(r, s);
+}
+
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
 bool valid_temperature(double t) { return t > 0.0 && t < 1e15; }
@@ -1443,7 +1705,8 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
   auto place = [&](bool in_state, int64_t so, int64_t fo) { return in_state ? kept + so : base + fo; };
   const Rows rows = rows_at(place(any, p.s_rows, p.f_rows), N);
   const Tops tops = tops_at(place(any, p.s_tops, p.f_tops));
-  const Entries entries = {reinterpret_cast<int32_t*>(base + p.f_cols),
+  const bool held = keep && p.held;  // bf16: the exponentials are kept, not what the rest makes of them
+  const Entries entries = {reinterpret_cast<int32_t*>(place(held, p.s_cols, p.f_cols)),
                            reinterpret_cast<uint2*>(place(keep, p.s_list, p.f_list)),
                            reinterpret_cast<int32_t*>(place(keep, p.s_start, p.f_start))};
   float* lse = reinterpret_cast<float*>(place(keep, p.s_lse, p.f_lse));
@@ -1484,7 +1747,7 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
   a.tops = tops;
   a.entries = entries;
   a.picked = reinterpret_cast<float*>(base + p.f_picked);
-  a.part = reinterpret_cast<f32x2_t*>(base + p.f_part);
+  a.part = reinterpret_cast<f32x2_t*>(place(held, p.s_part, p.f_part));
   a.N = N;
   JoinArgs j = {};
   j.rows = rows;
@@ -1500,44 +1763,33 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
   j.loss = loss;
   j.lse = lse;
   j.corr = corr;
+  f32x4_t* z = reinterpret_cast<f32x4_t*>(base + p.f_z);
+  const int tiles_c = p.emit ? p.chunk / kMmTile : p.tiles_n;
+  a.lde = (int64_t)p.tiles_v * 4;
+  a.plane = tiles_c * a.lde * kMmBlock;
+  a.e = reinterpret_cast<uint16_t*>(place(p.held, p.s_e, p.f_e));
+  a.h.most = tiles_c * kMmTile;
   if (!p.emit) {
-    const dim3 grid = tile_grid((int64_t)p.tiles_v * p.tiles_n);
-    if (p.planes == 1)
-      hipLaunchKernelGGL((head_stats_kernel<false, false>), grid, dim3(kMmThreads), 0, s, a);
-    else
-      hipLaunchKernelGGL((head_stats_kernel<false, true>), grid, dim3(kMmThreads), 0, s, a);
-    DPC_HIP_CHECK(hipGetLastError());
+    const int rz = held ? stats<true>(p, a, tiles_c, z, s) : stats<false>(p, a, tiles_c, z, s);
+    if (rz != DPC_OK) return rz;
     hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)((N + kJoinRows - 1) / kJoinRows)),
                        dim3(kJoinThreads), 0, s, j);
     DPC_HIP_CHECK(hipGetLastError());
     return DPC_OK;
   }
-  a.lde = (int64_t)p.tiles_v * 4;
-  a.plane = p.chunk / kMmTile * a.lde * kMmBlock;
-  a.e = reinterpret_cast<uint16_t*>(base + p.f_e);
-  const int tiles_c = p.chunk / kMmTile;
   float* unit = reinterpret_cast<float*>(kept + p.s_unit);
   for (int64_t first = 0; first < N; first += p.chunk) {
     a.h.first = j.first = (int)first;
-    a.h.most = p.chunk;
-    const dim3 grid = tile_grid((int64_t)p.tiles_v * tiles_c);
-    if (p.planes == 1)
-      hipLaunchKernelGGL((head_stats_kernel<true, false>), grid, dim3(kMmThreads), 0, s, a);
-    else
-      hipLaunchKernelGGL((head_stats_kernel<true, true>), grid, dim3(kMmThreads), 0, s, a);
-    DPC_HIP_CHECK(hipGetLastError());
+    const int rz = stats<true>(p, a, tiles_c, z, s);
+    if (rz != DPC_OK) return rz;
     hipLaunchKernelGGL(head_join_kernel, dim3((unsigned)(p.chunk / kJoinRows)),
                        dim3(kJoinThreads), 0, s, j);
     DPC_HIP_CHECK(hipGetLastError());
     const FixArgs x = {rows.count, N, K, p.tiles_v, (int)first, entries.cols, a.part, lse, corr,
-                       a.e, a.lde, a.plane};
-    const dim3 fix_grid((unsigned)(p.chunk / kJoinRows),
-                        (unsigned)((p.tiles_v + kFixTiles - 1) / kFixTiles));
-    if (p.planes == 1)
-      hipLaunchKernelGGL((head_fix_kernel<false>), fix_grid, dim3(kJoinThreads), 0, s, x);
-    else
-      hipLaunchKernelGGL((head_fix_kernel<true>), fix_grid, dim3(kJoinThreads), 0, s, x);
-    DPC_HIP_CHECK(hipGetLastError());
+                       nullptr, a.e, a.e, a.lde, a.plane};
+    const int rx = fix(p, x, p.chunk, s);
+    if (rx != DPC_OK) return rx;
+    if (!p.want_h) continue;
     ProductArgs m = {};
     m.mm = MmArgs{w, MmOperand{a.e, a.lde, a.plane, 0}, V, p.tiles_d, tiles_c, p.splits_c};
     m.coef = 1.f;
@@ -1595,7 +1847,7 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
   uint8_t* base = static_cast<uint8_t*>(ws);
   uint8_t* kept = static_cast<uint8_t*>(const_cast<void*>(state));
   const Rows rows = rows_at(kept + p.s_rows, N);
-  if (p.emit) {
+  if (p.emit && hidden_grad) {
     const int64_t items = D % 8 == 0 ? N * D / 8 : N * D;
     int64_t grid = (items + 255) / 256;
     if (grid > 8192) grid = 8192;
@@ -1603,12 +1855,11 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
                        reinterpret_cast<const float*>(kept + p.s_unit), rows, grad_loss,
                        (float)temperature, N, D, dtype == DPC_BF16, hidden_grad);
     DPC_HIP_CHECK(hipGetLastError());
-    return DPC_OK;
   }
+  if (p.emit && !weight_grad) return DPC_OK;
   if ((int64_t)p.piece_tiles * p.tiles_n > 0x7fffffffll) return DPC_EINVAL;
   PrepArgs pa = {};
   pa.rows = rows;
-  pa.zero = hidden_grad;
   pa.g = grad_loss;
   pa.gmax = reinterpret_cast<float*>(base + p.b_g);
   pa.g_over = pa.gmax + 1;
@@ -1618,18 +1869,34 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
   if (half) {
     hipLaunchKernelGGL(gmax_kernel, dim3(1), dim3(kPrepThreads), 0, s, pa);
     DPC_HIP_CHECK(hipGetLastError());
-    if (weight_grad)
-      pa.hg = reinterpret_cast<uint16_t*>(base + p.b_hg);
-    else
-      pa.g = nullptr;
+    pa.g = nullptr;
+    if (weight_grad) pa.hg = reinterpret_cast<uint16_t*>(base + p.b_hg);
   }
+  const int64_t esz = dtype == DPC_BF16 ? 2 : 4;
+  if (p.emit) {
+    pa.hidden = hidden;
+    pa.dtype = dtype;
+    pa.D = D;
+    pa.N = N;
+    pa.ld = p.ld;
+    int64_t grid = (N * p.ld / 8 + kPrepThreads - 1) / kPrepThreads;
+    if (grid > 4096) grid = 4096;
+    hipLaunchKernelGGL(prep_kernel, dim3((unsigned)grid), dim3(kPrepThreads), 0, s, pa);
+    DPC_HIP_CHECK(hipGetLastError());
+    const int64_t ldz = (int64_t)p.tiles_v * 4;
+    const MmOperand zop = {reinterpret_cast<const uint16_t*>(kept + p.s_e), ldz,
+                           p.tiles_n * ldz * kMmBlock, 0};
+    const Hidden h = {nullptr, pa.hg, rows.count, N, p.ld, 0, (int)N};
+    return weight_product(p, pa, h, zop, tops, V, p.tiles_v, (float)temperature,
+                          reinterpret_cast<float*>(base + p.b_pw), weight_grad, s);
+  }
+  pa.zero = hidden_grad;
   Hidden h;
   MmOperand w;
   const int rc = operands(p, pa, hidden, weight, base + p.b_h, base + p.b_w, s, &h, &w);
   if (rc != DPC_OK) return rc;
   const MmOperand hop = {nullptr, p.ld, N * p.ld, 0};
   const int out_bf16 = dtype == DPC_BF16;
-  const int64_t esz = out_bf16 ? 2 : 4;
   const int64_t ldz = (int64_t)p.piece_tiles * 4;
   const int64_t plane = p.tiles_n * ldz * kMmBlock;
   uint16_t* dz = reinterpret_cast<uint16_t*>(base + p.b_dz);
@@ -1657,12 +1924,13 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
     a.dz = dz;
     a.ld = ldz;
     a.plane = plane;
-    const dim3 grid = tile_grid((int64_t)tiles * p.tiles_n);
-    if (half)
-      hipLaunchKernelGGL((head_grad_kernel<true>), grid, dim3(kMmThreads), 0, s, a);
-    else
-      hipLaunchKernelGGL((head_grad_kernel<false>), grid, dim3(kMmThreads), 0, s, a);
-    DPC_HIP_CHECK(hipGetLastError());
+    const FixArgs x = {rows.count, N, K, p.tiles_v, 0,
+                       reinterpret_cast<const int32_t*>(kept + p.s_cols),
+                       reinterpret_cast<const f32x2_t*>(kept + p.s_part), a.lse, a.corr, a.g,
+                       reinterpret_cast<const uint16_t*>(kept + p.s_e), dz, ldz, plane};
+    const int rg = p.held ? fix(p, x, (int64_t)p.tiles_n * kMmTile, s)
+                          : gradients(p, a, reinterpret_cast<f32x4_t*>(base + p.b_z), s);
+    if (rg != DPC_OK) return rg;
     const MmOperand zop = {dz, ldz, plane, 0};
     ProductArgs q = {};
     q.h = h;
@@ -1713,36 +1981,13 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
       }
     }
     if (weight_grad) {
-      ProductArgs m = q;
-      m.mm = MmArgs{hop, zop, 0, p.tiles_d, tiles, p.splits_w};
-      m.rows_b = cols_here;
-      m.plane = (int64_t)cols_here * p.lda;
-      m.partial = p.splits_w == 1 ? nullptr : reinterpret_cast<float*>(base + p.b_pw);
-      m.out = static_cast<uint8_t*>(weight_grad) + (int64_t)first * D * esz;
-      m.shift = half ? tops.h : nullptr;
-      if (half) m.h.packed = pa.hg;
-      const dim3 product_grid((unsigned)(p.tiles_d * tiles * p.splits_w));
-      if (half)
-        hipLaunchKernelGGL((head_product_kernel<false, true>), product_grid, dim3(kMmThreads), 0,
-                           s, m);
-      else
-        hipLaunchKernelGGL((head_product_kernel<false, false>), product_grid, dim3(kMmThreads), 0,
-                           s, m);
-      DPC_HIP_CHECK(hipGetLastError());
-      if (m.partial) {
-        r.partial = m.partial;
-        r.splits = p.splits_w;
-        r.plane = m.plane;
-        r.rows = cols_here;
-        r.count = nullptr;
-        r.first = 0;
-        r.active = nullptr;
-        r.by_row = nullptr;
-        r.shift = m.shift;
-        r.out = m.out;
-        const int rr = reduce(r, s);
-        if (rr != DPC_OK) return rr;
-      }
+      Hidden hw = h;
+      if (half) hw.packed = pa.hg;
+      const int rw = weight_product(p, pa, hw, zop, tops, cols_here, tiles,
+                                    (float)temperature, reinterpret_cast<float*>(base + p.b_pw),
+                                    static_cast<uint8_t*>(weight_grad) + (int64_t)first * D * esz,
+                                    s);
+      if (rw != DPC_OK) return rw;
     }
   }
   return DPC_OK;
