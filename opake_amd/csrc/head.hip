@@ -698,8 +698,10 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_stats_kernel(StatsArgs s) 
 
 // Few tiles (few rows, or a small vocabulary): the products' K steps in slices, each
 // slice's accumulators left as they are held ([slice][tile][wave][block][lane]), then
-// the same epilogues by single waves that add them up in order.  Rows past the last
-// are neither written nor read.
+// the same epilogues on their sums.  A workgroup adds up one wave's part of a tile: its
+// four waves every fourth slice each, 16 loads a lane in flight, then the first one theirs,
+// all in a fixed order.  Rows past the last are not written, and zeros; waves that have no
+// others have nothing to do, and `waves` leaves out those that never have any.
 struct LogitsArgs {
   MmArgs mm;
   Hidden h;
@@ -729,35 +731,64 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_logits_kernel(LogitsArgs s
       for (int i = 0; i < 8; ++i) z[(j * 8 + i) * 64] = acc.v[i][j];
 }
 
-DPC_DEVICE void add_logits(const f32x4_t* z, int slices, int tiles, int64_t tile, int w, int row0,
+constexpr int kAddWaves = 4;
+
+// The sums, in the first wave; false in the others.
+DPC_DEVICE bool add_logits(const f32x4_t* z, int slices, int tiles, int64_t tile, int w, int row0,
                            int N, MmAcc<false>& acc) {
-  const int lane = epilogue_lane();
+  const int lane = threadIdx.x & 63, q = threadIdx.x >> 6;
+  f32x4_t* lds = reinterpret_cast<f32x4_t*>(lds_all);  // [kAddWaves - 1][32][64]
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc.v[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < slices; ++s) {
+  for (int s = q; s < slices; s += kAddWaves) {
     const f32x4_t* from = z + logits_at((int64_t)s * tiles + tile, w) + lane;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (row0 + 16 * j < N)
+    for (int j = 0; j < 4; j += 2) {
+      f32x4_t x[2][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc.v[i][j] += from[(j * 8 + i) * 64];
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[k][i] = from[((j + k) * 8 + i) * 64];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc.v[i][j + k] += x[k][i];
+    }
   }
+  if (q > 0)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) lds[((q - 1) * 32 + j * 8 + i) * 64 + lane] = acc.v[i][j];
+  __syncthreads();
+  if (q > 0) return false;
+  for (int k = 0; k < kAddWaves - 1; ++k)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc.v[i][j] += lds[(k * 32 + j * 8 + i) * 64 + lane];
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (row0 + 16 * j >= N)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc.v[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  return true;
 }
 
 template <bool kEmit, bool kHalf>
-__global__ void __launch_bounds__(64) head_split_stats_kernel(StatsArgs s, const f32x4_t* z,
-                                                              int slices, int tiles) {
-  const int id = blockIdx.x >> 3, w = blockIdx.x & 7, tb = id / s.mm.tiles_a,
+__global__ void __launch_bounds__(64 * kAddWaves) head_split_stats_kernel(StatsArgs s, const f32x4_t* z,
+                                                              int slices, int tiles, int waves) {
+  const int id = blockIdx.x / waves, w = blockIdx.x - id * waves, tb = id / s.mm.tiles_a,
             ta = id - tb * s.mm.tiles_a;
   const uint16_t* unused;
   const int N = hidden_rows(s.h, &unused);
-  if (tb * kMmTile >= N) return;
+  if (tb * kMmTile + (w >> 1) * 64 >= N) return;
   const int64_t g0 = s.h.first + (int64_t)tb * kMmTile;
   const WaveEntries own(s.entries, s.K, s.mm.tiles_a, ta, g0 / kMmTile, w, threadIdx.x);
   MmAcc<false> acc;
-  add_logits(z, slices, tiles, id, w, tb * kMmTile + (w >> 1) * 64, N, acc);
+  if (!add_logits(z, slices, tiles, id, w, tb * kMmTile + (w >> 1) * 64, N, acc)) return;
   f32x4_t factor = {};
   if constexpr (kHalf) factor = row_factors(s, N, tb, w, *s.tops.w);
   stats_epilogue<kEmit, kHalf>(s, acc, factor, N, ta, tb, w, g0, own.list, own.e0, own.e1,
@@ -1170,17 +1201,17 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
 }
 
 template <bool kHalf>
-__global__ void __launch_bounds__(64) head_split_grad_kernel(GradArgs s, const f32x4_t* z,
-                                                             int slices, int tiles) {
-  const int id = blockIdx.x >> 3, w = blockIdx.x & 7, tb = id / s.mm.tiles_a,
+__global__ void __launch_bounds__(64 * kAddWaves) head_split_grad_kernel(GradArgs s, const f32x4_t* z,
+                                                             int slices, int tiles, int waves) {
+  const int id = blockIdx.x / waves, w = blockIdx.x - id * waves, tb = id / s.mm.tiles_a,
             ta = id - tb * s.mm.tiles_a;
   const uint16_t* unused;
   const int N = hidden_rows(s.h, &unused);
-  if (tb * kMmTile >= N) return;
+  if (tb * kMmTile + (w >> 1) * 64 >= N) return;
   const WaveEntries own(s.entries, s.K, s.tiles, s.tile0 + ta, tb, w, threadIdx.x);
   const float change = own.e0 < own.e1 ? entry_change<kHalf>(s, tb, own.first) : 0.f;
   MmAcc<false> acc;
-  add_logits(z, slices, tiles, id, w, tb * kMmTile + (w >> 1) * 64, N, acc);
+  if (!add_logits(z, slices, tiles, id, w, tb * kMmTile + (w >> 1) * 64, N, acc)) return;
   GradRows rows;
   rows.load<kHalf>(s, N, tb, w, kHalf ? *s.tops.w : 0u);
   grad_epilogue<kHalf>(s, acc, ta, tb, w, rows.lse, rows.g, own.list, own.e0, own.e1, own.first,
@@ -1346,14 +1377,18 @@ int slices(int64_t tiles, int64_t steps) {
 }
 
 // The logits' K steps in slices where their tiles leave compute units idle.  A step
-// takes 1.2 us, adding up a slice 1.3 us for a tile's 256 rows: the number of slices that
-// makes the sum of both least.
+// takes 1.2 us, the second launch 13 us and 0.6 us a slice of a tile's 256 rows: as many
+// slices as make the sum least, if that beats the steps in a row.  (The loss of 675 rows
+// with a third of them active, 1536 wide, vocabulary 203, float32: 72 steps of one tile
+// take 51 us a call in 12 slices and 114 in one.)
 int logit_slices(int64_t tiles, int64_t steps, int64_t N) {
   const int64_t rows = N < kMmTile ? N : kMmTile;
-  int64_t s = (int64_t)sqrt((double)steps * kMmTile / (double)rows);
+  int64_t s = (int64_t)sqrt(2.0 * (double)steps * kMmTile / (double)rows);
   if (s > kUnits / tiles) s = kUnits / tiles;
   if (s > steps / 4) s = steps / 4;
-  return s < 2 ? 1 : (int)s;
+  return s < 2 || 1.2 * (double)(steps - steps / s) < 13.0 + 0.6 * (double)(s * rows) / kMmTile
+             ? 1
+             : (int)s;
 }
 
 bool valid_head(int64_t N, int D, int V, int K, int dtype) {
@@ -1549,6 +1584,9 @@ int reduce(const ReduceArgs& a, hipStream_t s) {
 // Workgroups that go through `tiles` tiles, one a compute unit (LDS holds one).
 dim3 tile_grid(int64_t tiles) { return dim3((unsigned)(tiles < kUnits ? tiles : kUnits)); }
 
+// Waves of a tile that may have rows.
+int split_waves(const Plan& p) { return 2 * (int)(((p.N < kMmTile ? p.N : kMmTile) + 63) / 64); }
+
 // The statistics of a launch's tiles (`tiles_b` row blocks at most).
 template <bool kEmit>
 int stats(const Plan& p, const StatsArgs& a, int tiles_b, f32x4_t* z, hipStream_t s) {
@@ -1557,17 +1595,17 @@ int stats(const Plan& p, const StatsArgs& a, int tiles_b, f32x4_t* z, hipStream_
   if (p.splits_z > 1) {
     LogitsArgs l = {a.mm, a.h, z, (int)tiles};
     l.mm.splits = p.splits_z;
-    const dim3 grid((unsigned)(tiles * p.splits_z)), waves((unsigned)(tiles * 8));
+    const dim3 grid((unsigned)(tiles * p.splits_z)), waves((unsigned)(tiles * split_waves(p)));
     if (half) {
       hipLaunchKernelGGL((head_logits_kernel<true>), grid, dim3(kMmThreads), 0, s, l);
       DPC_HIP_CHECK(hipGetLastError());
-      hipLaunchKernelGGL((head_split_stats_kernel<kEmit, true>), waves, dim3(64), 0, s, a, z,
-                         p.splits_z, (int)tiles);
+      hipLaunchKernelGGL((head_split_stats_kernel<kEmit, true>), waves, dim3(64 * kAddWaves), 0, s, a, z,
+                         p.splits_z, (int)tiles, split_waves(p));
     } else {
       hipLaunchKernelGGL((head_logits_kernel<false>), grid, dim3(kMmThreads), 0, s, l);
       DPC_HIP_CHECK(hipGetLastError());
-      hipLaunchKernelGGL((head_split_stats_kernel<kEmit, false>), waves, dim3(64), 0, s, a, z,
-                         p.splits_z, (int)tiles);
+      hipLaunchKernelGGL((head_split_stats_kernel<kEmit, false>), waves, dim3(64 * kAddWaves), 0, s, a, z,
+                         p.splits_z, (int)tiles, split_waves(p));
     }
   } else if (half) {
     hipLaunchKernelGGL((head_stats_kernel<kEmit, true>), tile_grid(tiles), dim3(kMmThreads), 0, s,
@@ -1598,17 +1636,17 @@ int gradients(const Plan& p, const GradArgs& a, f32x4_t* z, hipStream_t s) {
   if (p.splits_g > 1) {
     LogitsArgs l = {a.mm, a.h, z, (int)tiles};
     l.mm.splits = p.splits_g;
-    const dim3 grid((unsigned)(tiles * p.splits_g)), waves((unsigned)(tiles * 8));
+    const dim3 grid((unsigned)(tiles * p.splits_g)), waves((unsigned)(tiles * split_waves(p)));
     if (half) {
       hipLaunchKernelGGL((head_logits_kernel<true>), grid, dim3(kMmThreads), 0, s, l);
       DPC_HIP_CHECK(hipGetLastError());
-      hipLaunchKernelGGL((head_split_grad_kernel<true>), waves, dim3(64), 0, s, a, z, p.splits_g,
-                         (int)tiles);
+      hipLaunchKernelGGL((head_split_grad_kernel<true>), waves, dim3(64 * kAddWaves), 0, s, a, z, p.splits_g,
+                         (int)tiles, split_waves(p));
     } else {
       hipLaunchKernelGGL((head_logits_kernel<false>), grid, dim3(kMmThreads), 0, s, l);
       DPC_HIP_CHECK(hipGetLastError());
-      hipLaunchKernelGGL((head_split_grad_kernel<false>), waves, dim3(64), 0, s, a, z, p.splits_g,
-                         (int)tiles);
+      hipLaunchKernelGGL((head_split_grad_kernel<false>), waves, dim3(64 * kAddWaves), 0, s, a, z, p.splits_g,
+                         (int)tiles, split_waves(p));
     }
   } else if (half) {
     hipLaunchKernelGGL((head_grad_kernel<true>), tile_grid(tiles), dim3(kMmThreads), 0, s, a);
