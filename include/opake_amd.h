@@ -537,12 +537,14 @@ int dpc_row_sum_f64(const double* x, int B, int n, int accumulate, double* out, 
  *
  * want_hidden / want_weight say which gradients will be asked for; `state` then
  * keeps what they need (dpc_head_loss_state_bytes; NULL if neither).  With
- * want_hidden alone it keeps the hidden gradient itself, for grad_loss 1, in
- * float32.  Otherwise dpc_head_loss_grad computes dz again, in
- * pieces of the vocabulary, held as bf16 (fp32: as two fp16 planes) for the two
- * products.  It takes the same arguments, grad_loss [N] (the gradient of the losses;
- * not used where there is no target) and writes, where not NULL, hidden_grad [N, D]
- * and weight_grad [V, D] in `dtype`, 16-byte aligned, rounded once from float32 sums.
+ * want_hidden alone that is the hidden gradient itself, for grad_loss 1, in
+ * float32.  With want_weight it is also every row's exponentials (bf16: as fp16;
+ * fp32: two fp16 planes and the hidden gradient) where those take at most 512 MiB;
+ * beyond, dpc_head_loss_grad makes them again, in pieces of the vocabulary.
+ * dpc_head_loss_grad takes the same arguments, grad_loss [N] (the gradient of the
+ * losses; not used where there is no target) and writes, where not NULL,
+ * hidden_grad [N, D] and weight_grad [V, D] in `dtype`, 16-byte aligned, rounded
+ * once from float32 sums of products with dz in bf16 (fp32: two fp16 planes).
  * `state` is not changed.  All results are deterministic.  K <= 65536, V <= 2^19.
  * -------------------------------------------------------------------------*/
 size_t dpc_head_loss_state_bytes(int64_t N, int D, int V, int K, int dtype, int want_hidden,

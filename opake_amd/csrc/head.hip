@@ -24,16 +24,17 @@
 // maximum and sum of exponentials per row and the logits at the entries' columns; a
 // join turns them into lse and the loss.
 //
-// Gradients, in one of two ways:
-//   * the hidden states' alone (a frozen head): the rows go in chunks, whose tiles also
-//     leave exp(z - half a tile's maximum) as fp16 (float32 inputs: two planes).  A pass
-//     turns the chunk into p - q (bf16, or planes) in place, and one product with W
-//     gives dH for g = 1, kept in float32 until the backward multiplies each row by its
-//     g.  Two products in all instead of three.
-//   * otherwise in the backward, in pieces of the vocabulary: the logits' tiles
-//     again, turned into dz in the accumulators and written as bf16 (float32 inputs:
-//     as two fp16 planes), then the products dz W (added up over the pieces
-//     in float32) and dz^T H.
+// Gradients: a product's tiles also leave exp(z - half a tile's maximum) as fp16
+// (float32 inputs: two planes), and a pass turns those into dz (bf16, or planes) once
+// the row's lse is known.  So the logits are made once:
+//   * the hidden states' alone (a frozen head): the rows in chunks of up to 512 MiB of
+//     exponentials, dz for g = 1 in place, and one product with W gives dH for g = 1,
+//     kept in float32 until the backward multiplies each row by its g.  Two products.
+//   * a trained head whose exponentials fit in 512 MiB: they are kept, and the backward
+//     makes dz, dz W and dz^T H of them (float32: dz and dH for g = 1 in the forward;
+//     g goes to dH's rows and to a copy of H).  Three products.
+//   * beyond that the backward makes the logits again, in pieces of the vocabulary, and
+//     turns them into dz in the accumulators.  Four products.
 // dz at an entry's column, where p and q may cancel, is formed in float32 by the
 // join and put in place of the tile's value.
 #include <math.h>
@@ -1200,24 +1201,6 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
   }
 }
 
-template <bool kHalf>
-__global__ void __launch_bounds__(64 * kAddWaves) head_split_grad_kernel(GradArgs s, const f32x4_t* z,
-                                                             int slices, int tiles, int waves) {
-  const int id = blockIdx.x / waves, w = blockIdx.x - id * waves, tb = id / s.mm.tiles_a,
-            ta = id - tb * s.mm.tiles_a;
-  const uint16_t* unused;
-  const int N = hidden_rows(s.h, &unused);
-  if (tb * kMmTile + (w >> 1) * 64 >= N) return;
-  const WaveEntries own(s.entries, s.K, s.tiles, s.tile0 + ta, tb, w, threadIdx.x);
-  const float change = own.e0 < own.e1 ? entry_change<kHalf>(s, tb, own.first) : 0.f;
-  MmAcc<false> acc;
-  if (!add_logits(z, slices, tiles, id, w, tb * kMmTile + (w >> 1) * 64, N, acc)) return;
-  GradRows rows;
-  rows.load<kHalf>(s, N, tb, w, kHalf ? *s.tops.w : 0u);
-  grad_epilogue<kHalf>(s, acc, ta, tb, w, rows.lse, rows.g, own.list, own.e0, own.e1, own.first,
-                       change);
-}
-
 // ---------------------------------------------------------------------------
 // The products with dz: out[b][a] = sum_k A(a, k) B(b, k).
 // ---------------------------------------------------------------------------
@@ -1408,14 +1391,14 @@ struct Plan {
   int64_t lda;
   int chunk, splits_c;           // emit: rows of a chunk, slices of its product
   int piece_tiles, pieces;       // backward
-  int splits_h, splits_w, splits_z, splits_g;
+  int splits_h, splits_w, splits_z;
   bool held;  // dz for g = 1 is kept in the state
   // Byte offsets: state (kept for the backward), workspaces.
   int64_t s_rows, s_tops, s_lse, s_corr, s_list, s_start, s_cols, s_part, s_unit, s_e,
       state_bytes;
   int64_t f_rows, f_tops, f_lse, f_corr, f_list, f_start, f_cols, f_h, f_w, f_picked, f_part, f_e,
       f_pc, f_z, fwd_bytes;
-  int64_t b_h, b_w, b_hg, b_g, b_dz, b_z, b_ph, b_pw, bwd_bytes;
+  int64_t b_h, b_w, b_hg, b_g, b_dz, b_ph, b_pw, bwd_bytes;
 };
 
 Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w) {
@@ -1518,9 +1501,6 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
     p.piece_tiles = (p.tiles_v + p.pieces - 1) / p.pieces;
     p.pieces = (p.tiles_v + p.piece_tiles - 1) / p.piece_tiles;
     p.b_dz = take(p.planes * rows * p.piece_tiles * kMmTile * 2);
-    const int64_t piece = (int64_t)p.tiles_n * p.piece_tiles;
-    p.splits_g = p.held ? 1 : logit_slices(piece, pairs * up(D, kMmStep) / kMmStep, N);
-    if (p.splits_g > 1) p.b_z = take(p.splits_g * piece * kMmTile * kMmTile * 4);
     if (p.want_h) {
       p.splits_h = slices((int64_t)p.tiles_d * p.tiles_n, (int64_t)pairs * p.piece_tiles * 4);
       if (p.pieces > 1 || p.splits_h > 1) p.b_ph = take(p.splits_h * N * p.lda * 4);
@@ -1625,34 +1605,6 @@ int fix(const Plan& p, const FixArgs& a, int64_t rows, hipStream_t s) {
     hipLaunchKernelGGL((head_fix_kernel<false>), grid, dim3(kJoinThreads), 0, s, a);
   else
     hipLaunchKernelGGL((head_fix_kernel<true>), grid, dim3(kJoinThreads), 0, s, a);
-  DPC_HIP_CHECK(hipGetLastError());
-  return DPC_OK;
-}
-
-// dz of a piece of the vocabulary.
-int gradients(const Plan& p, const GradArgs& a, f32x4_t* z, hipStream_t s) {
-  const bool half = p.planes == 2;
-  const int64_t tiles = (int64_t)a.mm.tiles_a * p.tiles_n;
-  if (p.splits_g > 1) {
-    LogitsArgs l = {a.mm, a.h, z, (int)tiles};
-    l.mm.splits = p.splits_g;
-    const dim3 grid((unsigned)(tiles * p.splits_g)), waves((unsigned)(tiles * split_waves(p)));
-    if (half) {
-      hipLaunchKernelGGL((head_logits_kernel<true>), grid, dim3(kMmThreads), 0, s, l);
-      DPC_HIP_CHECK(hipGetLastError());
-      hipLaunchKernelGGL((head_split_grad_kernel<true>), waves, dim3(64 * kAddWaves), 0, s, a, z, p.splits_g,
-                         (int)tiles, split_waves(p));
-    } else {
-      hipLaunchKernelGGL((head_logits_kernel<false>), grid, dim3(kMmThreads), 0, s, l);
-      DPC_HIP_CHECK(hipGetLastError());
-      hipLaunchKernelGGL((head_split_grad_kernel<false>), waves, dim3(64 * kAddWaves), 0, s, a, z, p.splits_g,
-                         (int)tiles, split_waves(p));
-    }
-  } else if (half) {
-    hipLaunchKernelGGL((head_grad_kernel<true>), tile_grid(tiles), dim3(kMmThreads), 0, s, a);
-  } else {
-    hipLaunchKernelGGL((head_grad_kernel<false>), tile_grid(tiles), dim3(kMmThreads), 0, s, a);
-  }
   DPC_HIP_CHECK(hipGetLastError());
   return DPC_OK;
 }
@@ -1962,13 +1914,21 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
     a.dz = dz;
     a.ld = ldz;
     a.plane = plane;
-    const FixArgs x = {rows.count, N, K, p.tiles_v, 0,
-                       reinterpret_cast<const int32_t*>(kept + p.s_cols),
-                       reinterpret_cast<const f32x2_t*>(kept + p.s_part), a.lse, a.corr, a.g,
-                       reinterpret_cast<const uint16_t*>(kept + p.s_e), dz, ldz, plane};
-    const int rg = p.held ? fix(p, x, (int64_t)p.tiles_n * kMmTile, s)
-                          : gradients(p, a, reinterpret_cast<f32x4_t*>(base + p.b_z), s);
-    if (rg != DPC_OK) return rg;
+    if (p.held) {
+      const FixArgs x = {rows.count, N, K, p.tiles_v, 0,
+                         reinterpret_cast<const int32_t*>(kept + p.s_cols),
+                         reinterpret_cast<const f32x2_t*>(kept + p.s_part), a.lse, a.corr, a.g,
+                         reinterpret_cast<const uint16_t*>(kept + p.s_e), dz, ldz, plane};
+      const int rx = fix(p, x, (int64_t)p.tiles_n * kMmTile, s);
+      if (rx != DPC_OK) return rx;
+    } else {
+      const dim3 grid = tile_grid((int64_t)tiles * p.tiles_n);
+      if (half)
+        hipLaunchKernelGGL((head_grad_kernel<true>), grid, dim3(kMmThreads), 0, s, a);
+      else
+        hipLaunchKernelGGL((head_grad_kernel<false>), grid, dim3(kMmThreads), 0, s, a);
+      DPC_HIP_CHECK(hipGetLastError());
+    }
     const MmOperand zop = {dz, ldz, plane, 0};
     ProductArgs q = {};
     q.h = h;

@@ -4,18 +4,19 @@
 against one target a token; ``topk_distillation`` is the Kullback-Leibler
 divergence from a teacher of which only the top logits were kept.  Both return
 one loss a token (float32), so a caller can reduce them per example as
-per-example clipping needs, and both are differentiable with respect to ``hidden`` and, where it requires a gradient,
-``weight``.
+per-example clipping needs, and both are differentiable with respect to
+``hidden`` and, where it requires a gradient, ``weight``.
 
 Forward, one matrix-core product leaves the maximum and the sum of
-exponentials of every 256-wide piece of the vocabulary per token
-(``csrc/head.hip``).  No ``[tokens, vocabulary]`` tensor is kept: at most 512 MiB
-of it exist at a time (one 256-wide column or row block, where that is more).
-Where only ``hidden`` (bfloat16) requires a gradient -- a frozen head, the usual
-case under per-example clipping -- its gradient is made in the forward, chunk
-by chunk of the tokens, and kept in float32 for the backward to scale;
-otherwise the backward computes the logits again, piece by piece of the
-vocabulary.
+exponentials of every 128 columns of the vocabulary per token
+(``csrc/head.hip``).  Where only ``hidden`` requires a gradient -- a frozen head,
+the usual case under per-example clipping -- the exponentials of up to 512 MiB
+of tokens at a time become its gradient in the forward, which is kept in
+float32 for the backward to scale.  A trained head keeps its exponentials (16
+bits each, 32 for float32) where all of them fit in 512 MiB, and makes the
+logits again, piece by piece of the vocabulary, where they do not.  So no more
+than 512 MiB of any ``[tokens, vocabulary]`` kind are kept, and twice that exist
+at a time (one 256-wide row or column block, where that is more).
 """
 
 from __future__ import annotations
@@ -31,6 +32,7 @@ from opake_amd.ops import _aligned
 MAX_VOCABULARY = 1 << 19
 MAX_WIDTH = 1 << 20
 MAX_ENTRIES = 1 << 16  # of the teacher, a token
+
 
 def _check_head(hidden: torch.Tensor, weight: torch.Tensor) -> int:
     if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1]:

@@ -217,6 +217,49 @@ def test_many_pieces(dev, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("grad_h", [True, False], ids=["both", "weight"])
+def test_more_than_is_kept(dev, dtype, grad_h):
+    """A trained head with more exponentials than the forward keeps: the backward makes
+    the logits again, for both gradients or the weight's alone."""
+    N, D, V = 150_001, 8, 1900
+    g, h, W, up = _inputs(dev, (N,), D, V, dtype, 12)
+    t = torch.randint(0, V, (N,), generator=g, device=dev)
+    t[:7] = -100
+    h.requires_grad_(grad_h)
+    W.requires_grad_(True)
+    loss = head.linear_cross_entropy(h, W, t)
+    grads = torch.autograd.grad(loss, [h, W] if grad_h else [W], up)
+    L, DH, DW = _reference(h, W, _onehot(t, V, -100),
+                           torch.zeros(N, dtype=torch.float64, device=dev), 1.0, up)
+    _close(loss, L, "loss")
+    _close(grads[-1], DW, "weight_grad")
+    if grad_h:
+        _close(grads[0], DH, "hidden_grad")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("N,D,V", [(1, 4096, 300), (40, 2500, 1000), (300, 1544, 513)])
+def test_few_tiles_and_a_long_sum(dev, N, D, V, dtype):
+    """The logits' sums in slices: the loss alone, a frozen head, a trained one."""
+    g, h, W, up = _inputs(dev, (N,), D, V, dtype, N)
+    t = torch.randint(0, V, (N,), generator=g, device=dev)
+    q, zero = _onehot(t, V, -100), torch.zeros(N, dtype=torch.float64, device=dev)
+    L, DH, DW = _reference(h, W, q, zero, 1.0, up)
+    alone = head.linear_cross_entropy(h, W, t)
+    _close(alone, L, "loss")
+    h.requires_grad_(True)
+    W.requires_grad_(True)
+    loss = head.linear_cross_entropy(h, W, t)
+    assert torch.equal(loss, alone)
+    dh, dW = torch.autograd.grad(loss, [h, W], up)
+    _close(dh, DH, "hidden_grad")
+    _close(dW, DW, "weight_grad")
+    _frozen(lambda x, y: head.linear_cross_entropy(x, y, t), h, W, up, loss, q, zero, 1.0, t == -100)
+
+
+@pytest.mark.gpu
 def test_strided_and_unaligned_operands(dev):
     """Views: a transposed batch, a slice of a wider tensor, an odd element offset."""
     g, h, W, up = _inputs(dev, (6, 40), 64, 300, torch.bfloat16, 3)
