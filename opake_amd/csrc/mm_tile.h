@@ -90,8 +90,8 @@ struct MmAcc {
 
 constexpr int64_t kMmBlock = kMmTile * kMmStep;  // elements
 
-// A native piece in LDS: slot l ^ 4 (l / 16) holds lane l's 16 bytes, so that the
-// transposing reads, which take 4 rows x 16 columns, land on distinct banks too.
+// A native piece in LDS: as it is where it is read by whole lanes.  For the transposing
+// reads, which take 4 rows x 16 columns, slot l ^ 4 (l / 16) holds lane l's 16 bytes.
 DPC_DEVICE int mm_native_slot(int row, int q) { return (row ^ (4 * q)) + 16 * q; }
 
 template <bool kKc, bool kNative>
@@ -103,7 +103,7 @@ struct MmStage {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (kNative) {
-        const int from = mm_native_slot(lane & 15, lane >> 4) * 16;
+        const int from = (kKc ? lane : mm_native_slot(lane & 15, lane >> 4)) * 16;
         // K-contiguous: the block as it is.  K-slow: eight pieces of 32 columns (four
         // blocks) x four of 16 rows.
         voff[j] = kKc ? (w + 8 * j) * 1024 + from
@@ -163,7 +163,7 @@ struct MmFrags {
 #pragma unroll
     for (int i = 0; i < kOffsets; ++i) {
       if (kNative && kKc)
-        o[i] = at + (c0 >> 4) * 1024 + mm_native_slot(lane & 15, q) * 16;
+        o[i] = at + (c0 >> 4) * 1024 + lane * 16;
       else if (kNative)  // lane L of 16: row 4 q + L / 4, columns 4 (L % 4) ..
         o[i] = at + (c0 >> 5) * 4096 + mm_native_slot(4 * q + ((lane & 15) >> 2), lane & 3) * 16;
       else if (!kKc)
