@@ -1205,14 +1205,29 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
 // The products with dz: out[b][a] = sum_k A(a, k) B(b, k).
 // ---------------------------------------------------------------------------
 
+constexpr int kUnits = 256;  // compute units of an MI355X
+
+// K slices of a product of `tiles` tiles: about one workgroup a compute unit, no slice
+// under 8 steps.  (dH of 2790 rows, 1000 wide, vocabulary 50001, 44 tiles: 288 us in 5
+// slices, 335 in 4.)
+DPC_HOST_DEVICE int slices(int64_t tiles, int64_t steps) {
+  int64_t s = kUnits / tiles;
+  if (s > steps / 8) s = steps / 8;
+  if (s > 32) s = 32;
+  return s < 1 ? 1 : (int)s;
+}
+
 struct ProductArgs {
   MmArgs mm;
   Hidden h;         // dH: the rows of B and of the output; dW: A and its K
   const int32_t* active;  // dH straight to out: the rows' own places, or null
   int rows_b;       // dW: the output's rows
   int rows_a;       // the output's row length
-  float* partial;   // [splits][plane] float32 rows of lda, or null: straight to out
-  int64_t plane;
+  float* partial;   // [splits][rows][lda] float32, or null: straight to out
+  int64_t plane;    // dW: a slice of it, elements
+  int64_t steps;    // dH: the K steps that the number of slices goes by, on the device:
+                    // the rows that have a target are known there
+  bool direct;      // dH: one slice goes straight to out
   int64_t lda;      // rows_a rounded up to 4
   int accumulate;   // add to what partial holds
   // Straight to out: multiplied by *scale (null: 1), by the row's by_row (null: 1; by the
@@ -1261,6 +1276,11 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_product_kernel(ProductArgs
   if (kHidden) {
     rows_b = s.mm.b.rows = count;
     s.mm.tiles_b = tiles_of(count);
+    if (count == 0) return;
+    s.mm.splits =
+        __builtin_amdgcn_readfirstlane(slices((int64_t)s.mm.tiles_a * s.mm.tiles_b, s.steps));
+    s.plane = count * s.lda;
+    if (s.mm.splits == 1 && s.direct) s.partial = nullptr;
   } else {
     s.mm.a.p = hp;
     s.mm.kl = count;
@@ -1305,8 +1325,11 @@ struct ReduceArgs {
   const float* partial;
   int splits;
   int64_t plane, rows, lda;
-  const int32_t* count;  // rows from here on the device: clamp(*count - first, 0, rows)
-  int first;
+  // dH: clamp(*count - first, 0, rows) rows, and the product's slices of them.
+  const int32_t* count;
+  int first, tiles_d;
+  int64_t steps;
+  bool direct;
   const int32_t* active;
   const float* scale;
   const float* by_row;
@@ -1323,6 +1346,10 @@ __global__ void __launch_bounds__(256) head_reduce_kernel(ReduceArgs a) {
   if (a.count) {
     const int64_t left = (int64_t)*a.count - a.first;
     rows = left < 0 ? 0 : (left < rows ? left : rows);
+    if (rows == 0) return;
+    a.splits = slices((int64_t)a.tiles_d * tiles_of((int)rows), a.steps);
+    if (a.splits == 1 && a.direct) return;
+    a.plane = rows * a.lda;
   }
   const float all = (a.scale ? *a.scale : 1.f) * a.coef;
   const int shift = product_shift(a.shift);
@@ -1346,18 +1373,7 @@ __global__ void __launch_bounds__(256) head_reduce_kernel(ReduceArgs a) {
 // Held at once: dz of a piece of the vocabulary, or a chunk's exponentials.
 constexpr int64_t kPieceBytes = 512ll << 20;
 
-constexpr int kUnits = 256;  // compute units of an MI355X
-
 int64_t up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
-
-// Slices of `steps` K steps for `tiles` tiles: about one workgroup a compute
-// unit, no slice under 8 steps.
-int slices(int64_t tiles, int64_t steps) {
-  int64_t s = kUnits / tiles;
-  if (s > steps / 8) s = steps / 8;
-  if (s > 32) s = 32;
-  return s < 1 ? 1 : (int)s;
-}
 
 // The logits' K steps in slices where their tiles leave compute units idle.  A step
 // takes 1.2 us, the second launch 13 us and 0.6 us a slice of a tile's 256 rows: as many
@@ -1389,9 +1405,10 @@ struct Plan {
   bool pack;
   int tiles_v, tiles_n, tiles_d;
   int64_t lda;
-  int chunk, splits_c;           // emit: rows of a chunk, slices of its product
+  int chunk;                     // emit: rows of a chunk
+  int64_t steps_h;               // of dH's products
   int piece_tiles, pieces;       // backward
-  int splits_h, splits_w, splits_z;
+  int splits_w, splits_z;
   bool held;  // dz for g = 1 is kept in the state
   // Byte offsets: state (kept for the backward), workspaces.
   int64_t s_rows, s_tops, s_lse, s_corr, s_list, s_start, s_cols, s_part, s_unit, s_e,
@@ -1400,6 +1417,12 @@ struct Plan {
       f_pc, f_z, fwd_bytes;
   int64_t b_h, b_w, b_hg, b_g, b_dz, b_ph, b_pw, bwd_bytes;
 };
+
+// Rows of all slices together of a dH product, whatever number of rows has a target.
+int64_t slice_rows(const Plan& p, int64_t rows) {
+  const int64_t tiles = (rows + kMmTile - 1) / kMmTile, most = kUnits / p.tiles_d;
+  return (most < 32 * tiles ? most : 32 * tiles) * kMmTile;
+}
 
 Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w) {
   Plan p = {};
@@ -1473,9 +1496,9 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
     if (c > rows) c = rows;
     const int64_t n = (rows + c - 1) / c;
     p.chunk = (int)up((rows + n - 1) / n, kMmTile);
-    p.splits_c = slices((int64_t)p.tiles_d * (p.chunk / kMmTile), pairs * (int64_t)p.tiles_v * 4);
+    p.steps_h = pairs * (int64_t)p.tiles_v * 4;
     if (!p.held) p.f_e = take(p.chunk * row_bytes);
-    if (p.want_h && p.splits_c > 1) p.f_pc = take(p.splits_c * p.chunk * p.lda * 4);
+    if (p.want_h && slices(p.tiles_d, p.steps_h) > 1) p.f_pc = take(slice_rows(p, p.chunk) * p.lda * 4);
   }
   const int64_t z_tiles = (int64_t)p.tiles_v * (p.emit ? p.chunk / kMmTile : p.tiles_n);
   p.splits_z = logit_slices(z_tiles, pairs * up(D, kMmStep) / kMmStep, N);
@@ -1502,8 +1525,10 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
     p.pieces = (p.tiles_v + p.piece_tiles - 1) / p.piece_tiles;
     p.b_dz = take(p.planes * rows * p.piece_tiles * kMmTile * 2);
     if (p.want_h) {
-      p.splits_h = slices((int64_t)p.tiles_d * p.tiles_n, (int64_t)pairs * p.piece_tiles * 4);
-      if (p.pieces > 1 || p.splits_h > 1) p.b_ph = take(p.splits_h * N * p.lda * 4);
+      p.steps_h = pairs * (int64_t)p.piece_tiles * 4;
+      const int64_t most = slices(p.tiles_d, p.steps_h) > 1 ? slice_rows(p, N) : 0;
+      const int64_t need = p.pieces > 1 && N > most ? N : most;
+      if (need) p.b_ph = take(need * p.lda * 4);
     }
     if (p.want_w) {
       p.splits_w = slices((int64_t)p.tiles_d * p.piece_tiles, pairs * ((N + 63) / 64));
@@ -1563,6 +1588,12 @@ int reduce(const ReduceArgs& a, hipStream_t s) {
 
 // Workgroups that go through `tiles` tiles, one a compute unit (LDS holds one).
 dim3 tile_grid(int64_t tiles) { return dim3((unsigned)(tiles < kUnits ? tiles : kUnits)); }
+
+// Workgroups of a dH product over at most tiles_n row blocks, in slices or not.
+dim3 product_tiles(const Plan& p, int tiles_n) {
+  const int64_t tiles = (int64_t)p.tiles_d * tiles_n;
+  return dim3((unsigned)(tiles < kUnits ? kUnits : tiles));
+}
 
 // Waves of a tile that may have rows.
 int split_waves(const Plan& p) { return 2 * (int)(((p.N < kMmTile ? p.N : kMmTile) + 63) / 64); }
@@ -1781,16 +1812,17 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
     if (rx != DPC_OK) return rx;
     if (!p.want_h) continue;
     ProductArgs m = {};
-    m.mm = MmArgs{w, MmOperand{a.e, a.lde, a.plane, 0}, V, p.tiles_d, tiles_c, p.splits_c};
+    m.mm = MmArgs{w, MmOperand{a.e, a.lde, a.plane, 0}, V, p.tiles_d, tiles_c, 1};
+    m.steps = p.steps_h;
+    m.direct = true;
     m.coef = 1.f;
     m.shift = p.planes == 2 ? tops.w : nullptr;
     m.h = a.h;
     m.rows_a = D;
     m.lda = p.lda;
-    m.plane = p.chunk * p.lda;
-    m.partial = p.splits_c > 1 ? reinterpret_cast<float*>(base + p.f_pc) : nullptr;
+    m.partial = p.f_pc ? reinterpret_cast<float*>(base + p.f_pc) : nullptr;
     m.out = unit + first * D;
-    const dim3 product_grid((unsigned)(p.tiles_d * tiles_c * p.splits_c));
+    const dim3 product_grid = product_tiles(p, tiles_c);
     if (p.planes == 1)
       hipLaunchKernelGGL((head_product_kernel<true, false>), product_grid, dim3(kMmThreads), 0, s,
                          m);
@@ -1801,8 +1833,9 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
     if (m.partial) {
       ReduceArgs r = {};
       r.partial = m.partial;
-      r.splits = p.splits_c;
-      r.plane = m.plane;
+      r.tiles_d = p.tiles_d;
+      r.steps = m.steps;
+      r.direct = m.direct;
       r.rows = p.chunk;
       r.lda = p.lda;
       r.count = rows.count;
@@ -1947,16 +1980,16 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
       // A = W (D, K-slow: a row holds one vocabulary entry), B = dz by rows.  dz is zero
       // past the vocabulary, and W's rows there read as zeros.
       ProductArgs m = q;
-      m.mm = MmArgs{wpiece, zop, cols_here, p.tiles_d, p.tiles_n, p.splits_h};
+      m.mm = MmArgs{wpiece, zop, cols_here, p.tiles_d, p.tiles_n, 1};
       m.active = rows.active;
-      m.plane = N * p.lda;
-      const bool direct = p.pieces == 1 && p.splits_h == 1;
-      m.partial = direct ? nullptr : reinterpret_cast<float*>(base + p.b_ph);
+      m.steps = p.steps_h;
+      m.direct = p.pieces == 1;
+      m.partial = p.b_ph ? reinterpret_cast<float*>(base + p.b_ph) : nullptr;
       m.accumulate = i > 0;
       m.out = hidden_grad;
       m.by_row = half ? pa.g_over : nullptr;
       m.shift = half ? tops.w : nullptr;
-      const dim3 product_grid((unsigned)(p.tiles_d * p.tiles_n * p.splits_h));
+      const dim3 product_grid = product_tiles(p, p.tiles_n);
       if (half)
         hipLaunchKernelGGL((head_product_kernel<true, true>), product_grid, dim3(kMmThreads), 0, s,
                            m);
@@ -1964,10 +1997,11 @@ extern "C" int dpc_head_loss_grad(const void* hidden, const void* weight, int64_
         hipLaunchKernelGGL((head_product_kernel<true, false>), product_grid, dim3(kMmThreads), 0,
                            s, m);
       DPC_HIP_CHECK(hipGetLastError());
-      if (!direct && i + 1 == p.pieces) {
+      if (m.partial && i + 1 == p.pieces) {
         r.partial = m.partial;
-        r.splits = p.splits_h;
-        r.plane = m.plane;
+        r.tiles_d = p.tiles_d;
+        r.steps = m.steps;
+        r.direct = m.direct;
         r.rows = N;
         r.count = rows.count;
         r.active = rows.active;
