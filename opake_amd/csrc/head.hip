@@ -35,6 +35,9 @@
 //     g goes to dH's rows and to a copy of H).  Three products.
 //   * beyond that the backward makes the logits again, in pieces of the vocabulary, and
 //     turns them into dz in the accumulators.  Four products.
+// The products bound it: at 8192 rows, 2048 wide, vocabulary 32000 (bf16) the tiles with
+// their exponentials take 850 us, dz 197, dz W 820, a frozen head in all 1.85 ms.  (Two
+// products of that size take 1.50 ms in the library, and one writes 524 MB of logits.)
 // dz at an entry's column, where p and q may cancel, is formed in float32 by the
 // join and put in place of the tile's value.
 #include <math.h>
@@ -110,10 +113,10 @@ __global__ void __launch_bounds__(256) entries_kernel(const int64_t* __restrict_
   if (lane == 0) flag[n] = has;
 }
 
-// Numbers the rows with a target, and writes the others' losses (0).  One
-// workgroup, 8192 rows a round (8 loads in flight a thread): ballots count a wave's
-// 64 rows, and one wave adds up the round's 128 counts.  `flags` (distillation):
-// rows.place holds entries_kernel's flags.
+// Numbers the rows with a target, and writes the others' losses (0).  Latency bounds it
+// (14 us for 16384 rows, two rounds).  One workgroup, 8192 rows a round (8 loads in flight
+// a thread): ballots count a wave's 64 rows, and one wave adds up the round's 128 counts.
+// `flags` (distillation): rows.place holds entries_kernel's flags.
 __global__ void __launch_bounds__(1024) rows_kernel(const int64_t* __restrict__ index,
                                                     int64_t ignore, int flags, int64_t N,
                                                     Rows rows, float* __restrict__ loss,
@@ -184,7 +187,9 @@ DPC_DEVICE int entry_part(int row, int col) {
 // Operands as the tiles read them, in planes of 16-bit rows padded with zeros: the
 // rows with a target of `hidden` (bf16 rows of whole 16-byte chunks: only if some
 // are left out, else the tiles read the caller's own) and, where it needs planes or
-// padding, the weight.  The first `blocks` workgroups make the entries' lists.
+// padding, the weight.  The first `blocks` workgroups make the entries' lists.  Bound by
+// memory (float32, 33 MB of H and 262 MB of W into planes: 105 us, 5.6 TB/s) or by the
+// lists' counters (8192 rows of 64 entries: 37 us).
 struct PrepArgs {
   const void* hidden;
   const void* weight;  // null: read as it is
@@ -252,6 +257,7 @@ DPC_DEVICE uint32_t wave_max_bits(uint32_t x) {
   return x;
 }
 
+// One read of H and W: 262 MB of W in 70 us (3.7 TB/s).
 // blockIdx.y 0: H's rows with a target, one wave a row; 1: W.  (Maxima: any order gives
 // the same.)
 __global__ void __launch_bounds__(256) tops_kernel(const float* __restrict__ hidden,
@@ -468,6 +474,11 @@ DPC_DEVICE int tiles_of(int rows) { return (rows + kMmTile - 1) / kMmTile; }
 // Loss: the tile's statistics and the entries' logits.
 // ---------------------------------------------------------------------------
 
+// A workgroup a compute unit goes through tiles, the next one's first step on its way
+// while a tile's epilogue runs.  2048 rows, 4096 wide, vocabulary 131072: 1.66 ms alone
+// (1.33 PFLOP/s; the K loop's bound, mm_tile.h); 8192 x 2048 x 32000 with exponentials
+// written: 850 us (1.26 PFLOP/s).  Nothing hides the epilogues' exponentials and stores.
+// (A frozen head's call of twice that: 3.83 ms with a workgroup a tile, 3.77 so.)
 // A tile is two halves of 128 columns (one a wave): statistics are per half, so the
 // waves finish their halves without waiting for each other or using LDS, while the
 // workgroup's next tile is on its way into it.
@@ -779,8 +790,8 @@ DPC_DEVICE bool add_logits(const f32x4_t* z, int slices, int tiles, int64_t tile
 }
 
 template <bool kEmit, bool kHalf>
-__global__ void __launch_bounds__(64 * kAddWaves) head_split_stats_kernel(StatsArgs s, const f32x4_t* z,
-                                                              int slices, int tiles, int waves) {
+__global__ void __launch_bounds__(64 * kAddWaves)
+    head_split_stats_kernel(StatsArgs s, const f32x4_t* z, int slices, int tiles, int waves) {
   const int id = blockIdx.x / waves, w = blockIdx.x - id * waves, tb = id / s.mm.tiles_a,
             ta = id - tb * s.mm.tiles_a;
   const uint16_t* unused;
@@ -889,7 +900,9 @@ DPC_DEVICE void join_row(const JoinArgs& a, int64_t n, float lse, int lane) {
 }
 
 // 16 rows a workgroup of 8 waves: their lse from the halves' statistics (16 lanes side
-// by side read 16 rows), then their losses (a wave two rows).
+// by side read 16 rows), then their losses (a wave two rows).  10 us for 8192 rows of 250
+// halves (1.6 TB/s; latency); 25 us with 64 entries a row, whose equal columns are found
+// in K^2 / 64 steps a row.
 constexpr int kJoinRows = 16, kJoinThreads = 512;
 
 __global__ void __launch_bounds__(kJoinThreads) head_join_kernel(JoinArgs a) {
@@ -917,7 +930,8 @@ __global__ void __launch_bounds__(kJoinThreads) head_join_kernel(JoinArgs a) {
 }
 
 // exp(z - half's maximum) times exp(half's maximum - lse), and p - q at the entries'
-// columns: 16 rows x 8 tiles a workgroup.  The 16 rows are 1 KiB of every
+// columns.  Memory bounds it: 8192 x 32000 in place, 1.05 GB, 197 us (5.3 TB/s).  16 rows
+// x 8 tiles a workgroup.  The 16 rows are 1 KiB of every
 // 32 columns; a wave takes one of each tile's eight, all its loads in flight at once.
 constexpr int kFixTiles = 8;
 
@@ -1002,7 +1016,8 @@ __global__ void __launch_bounds__(kJoinThreads) head_fix_kernel(FixArgs a) {
   }
 }
 
-// out row n = unit's row place[n] times g[n] coef; 0 without a target.
+// out row n = unit's row place[n] times g[n] coef; 0 without a target.  16384 x 2048 into
+// bf16: 201 MB, 31 us (6.4 TB/s).
 __global__ void __launch_bounds__(256) head_scale_kernel(const float* __restrict__ unit, Rows rows,
                                                          const float* __restrict__ g, float coef,
                                                          int64_t N, int D, int out_bf16,
@@ -1048,6 +1063,8 @@ __global__ void __launch_bounds__(256) head_scale_kernel(const float* __restrict
 // Backward: dz of one piece of the vocabulary.
 // ---------------------------------------------------------------------------
 
+// The stats kernel's tiles again, with another epilogue: 16384 rows, 2048 wide, 16000 of
+// the vocabulary's columns take 834 us (1.29 PFLOP/s; the K loop's bound).
 struct GradArgs {
   MmArgs mm;  // A = W from the piece's first row, B = H
   Hidden h;
@@ -1241,7 +1258,9 @@ struct ProductArgs {
 };
 
 // What undoes the shifts of dz and of a product's other operand.
-DPC_DEVICE int product_shift(const uint32_t* top) { return top ? -(kDzShift + half_shift(*top)) : 0; }
+DPC_DEVICE int product_shift(const uint32_t* top) {
+  return top ? -(kDzShift + half_shift(*top)) : 0;
+}
 DPC_DEVICE f32x4_t shifted(f32x4_t x, int n) {
   return n ? f32x4_t{ldexpf(x[0], n), ldexpf(x[1], n), ldexpf(x[2], n), ldexpf(x[3], n)} : x;
 }
@@ -1265,7 +1284,8 @@ DPC_DEVICE void store_row4(void* out, int64_t at, int left, bool whole, int bf16
     }
 }
 
-// kHidden: dH (A = W, K the vocabulary, B = dz by rows); else dW (A = H, K the rows,
+// 8192 rows, 2048 wide, vocabulary 32000: dH 820 us, dW 828 (1.30 PFLOP/s; the K loop's
+// bound).  kHidden: dH (A = W, K the vocabulary, B = dz by rows); else dW (A = H, K the rows,
 // B = dz by columns).
 template <bool kHidden, bool kHalf>
 __global__ void __launch_bounds__(kMmThreads, 1) head_product_kernel(ProductArgs s) {
@@ -1498,7 +1518,8 @@ Plan head_plan(int64_t N, int D, int V, int K, int dtype, int want_h, int want_w
     p.chunk = (int)up((rows + n - 1) / n, kMmTile);
     p.steps_h = pairs * (int64_t)p.tiles_v * 4;
     if (!p.held) p.f_e = take(p.chunk * row_bytes);
-    if (p.want_h && slices(p.tiles_d, p.steps_h) > 1) p.f_pc = take(slice_rows(p, p.chunk) * p.lda * 4);
+    if (p.want_h && slices(p.tiles_d, p.steps_h) > 1)
+      p.f_pc = take(slice_rows(p, p.chunk) * p.lda * 4);
   }
   const int64_t z_tiles = (int64_t)p.tiles_v * (p.emit ? p.chunk / kMmTile : p.tiles_n);
   p.splits_z = logit_slices(z_tiles, pairs * up(D, kMmStep) / kMmStep, N);
@@ -1610,13 +1631,13 @@ int stats(const Plan& p, const StatsArgs& a, int tiles_b, f32x4_t* z, hipStream_
     if (half) {
       hipLaunchKernelGGL((head_logits_kernel<true>), grid, dim3(kMmThreads), 0, s, l);
       DPC_HIP_CHECK(hipGetLastError());
-      hipLaunchKernelGGL((head_split_stats_kernel<kEmit, true>), waves, dim3(64 * kAddWaves), 0, s, a, z,
-                         p.splits_z, (int)tiles, split_waves(p));
+      hipLaunchKernelGGL((head_split_stats_kernel<kEmit, true>), waves, dim3(64 * kAddWaves), 0, s,
+                         a, z, p.splits_z, (int)tiles, split_waves(p));
     } else {
       hipLaunchKernelGGL((head_logits_kernel<false>), grid, dim3(kMmThreads), 0, s, l);
       DPC_HIP_CHECK(hipGetLastError());
-      hipLaunchKernelGGL((head_split_stats_kernel<kEmit, false>), waves, dim3(64 * kAddWaves), 0, s, a, z,
-                         p.splits_z, (int)tiles, split_waves(p));
+      hipLaunchKernelGGL((head_split_stats_kernel<kEmit, false>), waves, dim3(64 * kAddWaves), 0, s,
+                         a, z, p.splits_z, (int)tiles, split_waves(p));
     }
   } else if (half) {
     hipLaunchKernelGGL((head_stats_kernel<kEmit, true>), tile_grid(tiles), dim3(kMmThreads), 0, s,
@@ -1723,10 +1744,12 @@ extern "C" int dpc_head_loss(const void* hidden, const void* weight, int64_t N, 
   uint8_t* base = static_cast<uint8_t*>(ws);
   uint8_t* kept = static_cast<uint8_t*>(state);
   const bool any = p.want_h || p.want_w, keep = any && !p.emit;
-  auto place = [&](bool in_state, int64_t so, int64_t fo) { return in_state ? kept + so : base + fo; };
+  auto place = [&](bool in_state, int64_t so, int64_t fo) {
+    return in_state ? kept + so : base + fo;
+  };
   const Rows rows = rows_at(place(any, p.s_rows, p.f_rows), N);
   const Tops tops = tops_at(place(any, p.s_tops, p.f_tops));
-  const bool held = keep && p.held;  // bf16: the exponentials are kept, not what the rest makes of them
+  const bool held = keep && p.held;  // bf16: the backward makes dz of the exponentials
   const Entries entries = {reinterpret_cast<int32_t*>(place(held, p.s_cols, p.f_cols)),
                            reinterpret_cast<uint2*>(place(keep, p.s_list, p.f_list)),
                            reinterpret_cast<int32_t*>(place(keep, p.s_start, p.f_start))};

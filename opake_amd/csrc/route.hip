@@ -15,6 +15,10 @@
 // lane, as order-preserving 32-bit keys; a round finds the largest key and then the
 // lowest index that has it, by lane moves within the row's lanes.  Rounds: one a
 // group kept, one an expert chosen.
+//
+// Few tokens: a launch's latency (16 tokens of 256 experts: 6 us).  Many: the rounds'
+// operations (65536 tokens, 256 experts in 8 groups of which 4, the best 8: 47 us, 67 MB
+// of logits at 1.4 TB/s; 63 us with the index found in every round).
 #include <math.h>
 
 #include "common.h"
@@ -340,7 +344,8 @@ DPC_DEVICE float chosen_grad(const RouteGradArgs& a, int64_t row, int slot, bool
 
 // All but the softmax's own weights: only the chosen logits have a gradient.  A
 // workgroup writes whole rows, zeros and all, from LDS in 16-byte stores: `rows` of
-// them (a multiple of 8, so that they are whole 16-byte chunks).
+// them (a multiple of 8, so that they are whole 16-byte chunks).  Memory bounds it: 65536
+// x 256 float32, 67 MB written in 16 us (4.3 TB/s).
 template <int kLanes>
 __global__ void __launch_bounds__(256) route_sparse_grad_kernel(RouteGradArgs a, int rows) {
   extern __shared__ __attribute__((aligned(16))) uint8_t tile[];
@@ -377,7 +382,8 @@ __global__ void __launch_bounds__(256) route_sparse_grad_kernel(RouteGradArgs a,
 }
 
 // The softmax's own weights: every logit of the row has one, p_e (y_e - dot), y the
-// chosen experts' gradients.  kLanes lanes a row.
+// chosen experts' gradients.  kLanes lanes a row.  9981 tokens of 60 experts: 6 us, a
+// launch's latency.
 template <int kLanes>
 __global__ void __launch_bounds__(256) route_dense_grad_kernel(RouteGradArgs a) {
   extern __shared__ float chosen[];  // [256 / kLanes][E]
