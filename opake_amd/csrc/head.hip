@@ -64,7 +64,9 @@ __shared__ __attribute__((aligned(16))) uint8_t lds_all[kLdsBytes];
 
 // float32 as two fp16 planes (mm_tile.h): the shift that brings magnitude `top` (the
 // float's bits) to [2^14, 2^15), and plane p of an x that is already shifted.
-constexpr int kDzShift = 14;  // of dz, which is at most 1 (its gradient is applied later)
+constexpr int kDzShift = 14;  // of exponentials and dz, which are at most 1 (the gradient
+                              // is applied later)
+constexpr float kDzScale = 1 << kDzShift;
 
 DPC_DEVICE int half_shift(uint32_t top) {
   const int e = (int)(top >> 23) & 255;
@@ -492,8 +494,9 @@ struct StatsArgs {
   float* picked;   // [rows, K]: z at the entries' columns
   f32x2_t* part;   // [2 tiles_a][N]: maximum and sum of exponentials of each half
   int64_t N;
-  uint16_t* e;     // the chunk's exp(z - the half's maximum) as fp16, native order
-                   // (float32 inputs: times 2^kDzShift, in two planes)
+  uint16_t* e;     // the chunk's exp(z - the half's maximum) times 2^kDzShift as fp16
+                   // (float32 inputs: in two planes), native order: 2^-12 of them is
+                   // lost, or 2^-39 of the maximum
   int64_t lde, plane;  // blocks of a row of them, elements
 };
 
@@ -631,12 +634,12 @@ DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, const f32x
 #pragma unroll
             for (int r = 0; r < 8; ++r)
               h[r] = __builtin_bit_cast(
-                  _Float16, half_plane(ldexpf(acc.v[2 * p + (r >> 2)][j][r & 3], kDzShift), pl));
+                  _Float16, half_plane(acc.v[2 * p + (r >> 2)][j][r & 3] * kDzScale, pl));
             *reinterpret_cast<half8_t*>(at + pl * s.plane) = h;
           }
         } else {
 #pragma unroll
-          for (int r = 0; r < 8; ++r) h[r] = (_Float16)acc.v[2 * p + (r >> 2)][j][r & 3];
+          for (int r = 0; r < 8; ++r) h[r] = (_Float16)(acc.v[2 * p + (r >> 2)][j][r & 3] * kDzScale);
           *reinterpret_cast<half8_t*>(at) = h;
         }
       }
@@ -979,7 +982,7 @@ __global__ void __launch_bounds__(kJoinThreads) head_fix_kernel(FixArgs a) {
 #pragma unroll
   for (int t = 0; t < kFixTiles; ++t)
     if (t < tiles) {
-      const float x = exp2_fast(f[t] - lse) * g;
+      const float x = exp2_fast(f[t] - lse) * (kHalf ? g : g / kDzScale);
       uint16_t* to = a.out + at + 4 * t * kMmBlock;
       if constexpr (kHalf) {
         half8_t o[2];
