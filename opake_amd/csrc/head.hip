@@ -1604,7 +1604,7 @@ int operands(const Plan& p, PrepArgs& a, const void* hidden, const void* weight,
 
 int reduce(const ReduceArgs& a, hipStream_t s) {
   int64_t grid = (a.rows * (a.lda / 4) + 255) / 256;
-  if (grid > 8192) grid = 8192;
+  if (grid > 2048) grid = 2048;  // (most of dH's have nothing to add up)
   hipLaunchKernelGGL(head_reduce_kernel, dim3((unsigned)grid), dim3(256), 0, s, a);
   DPC_HIP_CHECK(hipGetLastError());
   return DPC_OK;
