@@ -1287,6 +1287,36 @@ DPC_DEVICE void store_row4(void* out, int64_t at, int left, bool whole, int bf16
     }
 }
 
+template <bool kHidden>
+DPC_DEVICE void product_epilogue(const ProductArgs& s, MmAcc<kHidden>& acc, int ta, int tb, int w,
+                                 int split, int rows_b, float all, int shift) {
+  const int lane = epilogue_lane();
+  const int a0 = ta * kMmTile + acc.row0(w) + 4 * (lane >> 4);
+  const int b0 = tb * kMmTile + acc.col0(w) + (lane & 15);
+  const bool whole = s.rows_a % 4 == 0;
+#pragma unroll
+  for (int j = 0; j < MmAcc<kHidden>::kB; ++j) {
+    const int b = b0 + 16 * j;
+    if (b >= rows_b) continue;
+    const float f = kHidden && s.by_row ? all * s.by_row[b] : all;
+    const int64_t row = kHidden && s.active && !s.partial ? s.active[b] : b;
+#pragma unroll
+    for (int i = 0; i < MmAcc<kHidden>::kA; ++i) {
+      const int a = a0 + 16 * i;
+      if (a >= s.rows_a) continue;
+      f32x4_t x = acc.v[i][j];
+      if (s.partial) {
+        f32x4_t* p = reinterpret_cast<f32x4_t*>(s.partial + split * s.plane + row * s.lda + a);
+        if (s.accumulate) x += *p;
+        *p = x;
+      } else {
+        store_row4(s.out, row * s.rows_a + a, s.rows_a - a, whole, s.out_bf16,
+                   shifted(x * f, shift));
+      }
+    }
+  }
+}
+
 // 8192 rows, 2048 wide, vocabulary 32000: dH 820 us, dW 828 (1.30 PFLOP/s; the K loop's
 // bound).  kHidden: dH (A = W, K the vocabulary, B = dz by rows); else dW (A = H, K the rows,
 // B = dz by columns).
@@ -1308,37 +1338,25 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_product_kernel(ProductArgs
     s.mm.a.p = hp;
     s.mm.kl = count;
   }
-  if (!mm_tile_of(s.mm, blockIdx.x, &split, &ta, &tb)) return;
   MmTile<false, kHidden, true, kHidden, kHalf> tile(s.mm, lds_all);
   MmAcc<kHidden> acc;
-  tile.begin(ta, tb, split);
-  tile.run(acc);
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int a0 = ta * kMmTile + acc.row0(w) + 4 * (lane >> 4);
-  const int b0 = tb * kMmTile + acc.col0(w) + (lane & 15);
-  const bool whole = s.rows_a % 4 == 0;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const float all = (s.scale ? *s.scale : 1.f) * s.coef;
   const int shift = kHalf ? product_shift(s.shift) : 0;
-#pragma unroll
-  for (int j = 0; j < MmAcc<kHidden>::kB; ++j) {
-    const int b = b0 + 16 * j;
-    if (b >= rows_b) continue;
-    const float f = s.by_row ? all * s.by_row[b] : all;
-    const int64_t row = kHidden && s.active && !s.partial ? s.active[b] : b;
-#pragma unroll
-    for (int i = 0; i < MmAcc<kHidden>::kA; ++i) {
-      const int a = a0 + 16 * i;
-      if (a >= s.rows_a) continue;
-      f32x4_t x = acc.v[i][j];
-      if (s.partial) {
-        f32x4_t* p = reinterpret_cast<f32x4_t*>(s.partial + split * s.plane + row * s.lda + a);
-        if (s.accumulate) x += *p;
-        *p = x;
-      } else {
-        store_row4(s.out, row * s.rows_a + a, s.rows_a - a, whole, s.out_bf16,
-                   shifted(x * f, shift));
-      }
-    }
+  int split2, ta2, tb2, id = blockIdx.x;
+  bool more = mm_tile_of(s.mm, id, &split2, &ta2, &tb2);
+  if (more) tile.begin(ta2, tb2, split2);
+  while (more) {
+    split = split2;
+    ta = ta2;
+    tb = tb2;
+    tile.run(acc);
+    // dW: tile after tile, as the logits' (2 to 5% of it).  dH's tiles are a round at most
+    // but for the longest batches, and its epilogue has loads of its own.
+    id += gridDim.x;
+    more = !kHidden && mm_tile_of(s.mm, id, &split2, &ta2, &tb2);
+    if (more) tile.begin(ta2, tb2, split2);
+    product_epilogue<kHidden>(s, acc, ta, tb, w, split, rows_b, all, shift);
   }
 }
 
@@ -1682,7 +1700,7 @@ int weight_product(const Plan& p, const PrepArgs& g, const Hidden& h, const MmOp
   m.partial = p.splits_w == 1 ? nullptr : partial;
   m.out = out;
   m.out_bf16 = p.dtype == DPC_BF16;
-  const dim3 grid((unsigned)(p.tiles_d * tiles * p.splits_w));
+  const dim3 grid = tile_grid((int64_t)p.tiles_d * tiles * p.splits_w);
   if (half)
     hipLaunchKernelGGL((head_product_kernel<false, true>), grid, dim3(kMmThreads), 0, s, m);
   else

@@ -19,7 +19,7 @@
 // shift that brings the tensor's largest magnitude to [2^14, 2^15): x0 is x's rounding to
 // 11 bits, x1 that of what it leaves.  So 2^-24 |x| is lost, or 2^-39 of the largest where
 // x1 is subnormal (the matrix cores keep fp16's subnormals).  A step of 64 k goes over the
-// plane pairs (0, 1), (1, 0), (0, 0), one after the other while the caches hold them; the
+// plane pairs (1, 0), (0, 1), (0, 0), one after the other while the caches hold them; the
 // pair left out is below 2^-24 of the product.  The products are exact and the sums are
 // the MFMA's float32 ones: float32 accuracy at three bf16-rate products, 2500 / 3
 // TFLOP/s against the float32 matrix instructions' 157.
@@ -46,7 +46,7 @@ constexpr int kMmOperandBytes = kMmTile * kMmStep * 2;  // 32 KiB
 constexpr int kMmOutOfRange = 0x7ff00000;
 
 // A step's plane pairs, nibble i of each word: pair i's plane of A and of B.
-constexpr uint32_t kMmPairsA = 0x010u, kMmPairsB = 0x001u;
+constexpr uint32_t kMmPairsA = 0x001u, kMmPairsB = 0x010u;
 constexpr int kMmPairs = 3;
 
 // K-contiguous tile: rows of 64 k = 128 bytes, eight 16-byte chunks
