@@ -1227,14 +1227,29 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_grad_kernel(GradArgs s) {
 
 constexpr int kUnits = 256;  // compute units of an MI355X
 
-// K slices of a product of `tiles` tiles: about one workgroup a compute unit, no slice
-// under 8 steps.  (dH of 2790 rows, 1000 wide, vocabulary 50001, 44 tiles: 288 us in 5
-// slices, 335 in 4.)
+// K slices of a product of `tiles` tiles, none under 8 steps: one, or as many as fill one
+// or two rounds, whichever makes least of the rounds (1.4 us a step, 10 a round) and of
+// the results' way to memory and back (0.11 us each).  In integers: several kernels have
+// to agree on it.  (dH of 2790 rows, 1000 wide, vocabulary 50001, 44 tiles: 288 us in 5
+// slices, 335 in 4.  Of 4900 rows, 2048 wide, vocabulary 32000, 160 tiles: 597 us in 3
+// slices, 756 in one.)
+constexpr int kMostSliced = 512;  // tiles times slices, if more than one
+
 DPC_HOST_DEVICE int slices(int64_t tiles, int64_t steps) {
-  int64_t s = kUnits / tiles;
-  if (s > steps / 8) s = steps / 8;
-  if (s > 32) s = 32;
-  return s < 1 ? 1 : (int)s;
+  if (2 * tiles > kMostSliced || steps < 16) return 1;
+  const int n = (int)tiles, k = steps < 1 << 20 ? (int)steps : 1 << 20;
+  int best = 1, least = 140 * k + 1000;  // (one round: more than 256 tiles do not get here)
+  for (int r = 1; r <= kMostSliced / kUnits; ++r) {
+    int s = r * kUnits / n;
+    if (s > k / 8) s = k / 8;
+    if (s > 32) s = 32;
+    const int t = r * (140 * (k / s) + 1000) + 11 * n * s;
+    if (s > 1 && t < least) {
+      best = s;
+      least = t;
+    }
+  }
+  return best;
 }
 
 struct ProductArgs {
@@ -1330,8 +1345,9 @@ __global__ void __launch_bounds__(kMmThreads, 1) head_product_kernel(ProductArgs
     rows_b = s.mm.b.rows = count;
     s.mm.tiles_b = tiles_of(count);
     if (count == 0) return;
-    s.mm.splits =
-        __builtin_amdgcn_readfirstlane(slices((int64_t)s.mm.tiles_a * s.mm.tiles_b, s.steps));
+    s.mm.splits = s.partial ? __builtin_amdgcn_readfirstlane(
+                                  slices((int64_t)s.mm.tiles_a * s.mm.tiles_b, s.steps))
+                            : 1;
     s.plane = count * s.lda;
     if (s.mm.splits == 1 && s.direct) s.partial = nullptr;
   } else {
@@ -1461,7 +1477,7 @@ struct Plan {
 
 // Rows of all slices together of a dH product, whatever number of rows has a target.
 int64_t slice_rows(const Plan& p, int64_t rows) {
-  const int64_t tiles = (rows + kMmTile - 1) / kMmTile, most = kUnits / p.tiles_d;
+  const int64_t tiles = (rows + kMmTile - 1) / kMmTile, most = kMostSliced / p.tiles_d;
   return (most < 32 * tiles ? most : 32 * tiles) * kMmTile;
 }
 
@@ -1634,7 +1650,7 @@ dim3 tile_grid(int64_t tiles) { return dim3((unsigned)(tiles < kUnits ? tiles : 
 // Workgroups of a dH product over at most tiles_n row blocks, in slices or not.
 dim3 product_tiles(const Plan& p, int tiles_n) {
   const int64_t tiles = (int64_t)p.tiles_d * tiles_n;
-  return dim3((unsigned)(tiles < kUnits ? kUnits : tiles));
+  return dim3((unsigned)(tiles < kMostSliced ? kMostSliced : tiles));
 }
 
 // Waves of a tile that may have rows.

@@ -93,10 +93,10 @@ class _HeadLoss(torch.autograd.Function):
         dev = hidden.device
         h, w = _aligned(hidden), _aligned(weight)
         g = grad.to(torch.float32).contiguous()
-        dh = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if want_h else None
+        dh = torch.empty_like(h) if want_h else None
         dw = None
         if want_w:  # no token, no launch: the sum over none is zero
-            dw = (torch.empty if N else torch.zeros)((V, D), dtype=weight.dtype, device=dev)
+            dw = (torch.empty_like if N else torch.zeros_like)(w)
         ws_bytes = nat.load().dpc_head_loss_grad_workspace_bytes(*sizes)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         nat.call_on(dev, "dpc_head_loss_grad", h.data_ptr(), w.data_ptr(), N, D, V, code, K,

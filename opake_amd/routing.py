@@ -48,7 +48,7 @@ class _Route(torch.autograd.Function):
         z = logits.contiguous()
         E = z.shape[-1]
         g = grad.to(torch.float32).contiguous()
-        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+        dz = torch.empty_like(z)
         code, k, score, renormalize, scale = ctx.options
         nat.call_on(z.device, "dpc_route_topk_grad", z.data_ptr(), z.numel() // E, E, code, k,
                     score, renormalize, scale, experts.data_ptr(), weights.data_ptr(),
