@@ -56,7 +56,8 @@ def _integer(t: torch.Tensor, what: str) -> None:
 
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, hidden, weight, index, teacher, ignore_index, temperature, code):
+    def forward(ctx, hidden, weight, index, teacher, options):
+        ignore_index, temperature, code = options
         dev = hidden.device
         lead, D = hidden.shape[:-1], hidden.shape[-1]
         V = weight.shape[0]
@@ -89,10 +90,10 @@ class _HeadLoss(torch.autograd.Function):
         sizes = ctx.sizes
         N, D, V, K, code, forward_h, forward_w = sizes
         if not want_h and not want_w:
-            return (None,) * 7
+            return (None,) * 5
         dev = hidden.device
         h, w = _aligned(hidden), _aligned(weight)
-        g = grad.to(torch.float32).contiguous()
+        g = (grad if grad.dtype == torch.float32 else grad.float()).contiguous()
         dh = torch.empty_like(h) if want_h else None
         dw = None
         if want_w:  # no token, no launch: the sum over none is zero
@@ -103,7 +104,7 @@ class _HeadLoss(torch.autograd.Function):
                     ctx.temperature, forward_h, forward_w, state.data_ptr(), state.numel(),
                     g.data_ptr(), 0 if dh is None else dh.data_ptr(),
                     0 if dw is None else dw.data_ptr(), ws.data_ptr(), ws_bytes)
-        return dh, dw, None, None, None, None, None
+        return dh, dw, None, None, None
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *,
@@ -120,7 +121,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     if targets.shape != hidden.shape[:-1]:
         raise ConfigurationError(
             f"targets must be {tuple(hidden.shape[:-1])}, got {tuple(targets.shape)}")
-    return _HeadLoss.apply(hidden, weight, targets, None, int(ignore_index), 1.0, code)
+    return _HeadLoss.apply(hidden, weight, targets, None, (int(ignore_index), 1.0, code))
 
 
 def topk_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor,
@@ -149,8 +150,8 @@ def topk_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logits
         raise InputTypeError(f"temperature must be a number, got {type(temperature)}")
     if not (0.0 < temperature < 1e15 and math.isfinite(temperature)):
         raise ConfigurationError(f"temperature must be positive, got {temperature}")
-    return _HeadLoss.apply(hidden, weight, teacher_indices, teacher_logits, 0, float(temperature),
-                           code)
+    return _HeadLoss.apply(hidden, weight, teacher_indices, teacher_logits,
+                           (0, float(temperature), code))
 
 
 __all__ = ["linear_cross_entropy", "topk_distillation"]

@@ -23,7 +23,8 @@ _SCORES = {"softmax": nat.ROUTE_SOFTMAX, "sigmoid": nat.ROUTE_SIGMOID}
 
 class _Route(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, bias, code, k, score, groups, top_groups, renormalize, scale):
+    def forward(ctx, logits, bias, options):
+        code, k, score, groups, top_groups, renormalize, scale = options
         dev = logits.device
         z = logits.contiguous()
         lead, E = z.shape[:-1], z.shape[-1]
@@ -43,17 +44,17 @@ class _Route(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad, _):
         if grad is None:
-            return (None,) * 9
+            return None, None, None
         logits, weights, experts = ctx.saved_tensors
         z = logits.contiguous()
         E = z.shape[-1]
-        g = grad.to(torch.float32).contiguous()
+        g = (grad if grad.dtype == torch.float32 else grad.float()).contiguous()
         dz = torch.empty_like(z)
         code, k, score, renormalize, scale = ctx.options
         nat.call_on(z.device, "dpc_route_topk_grad", z.data_ptr(), z.numel() // E, E, code, k,
                     score, renormalize, scale, experts.data_ptr(), weights.data_ptr(),
                     g.data_ptr(), dz.data_ptr())
-        return dz, None, None, None, None, None, None, None, None
+        return dz, None, None
 
 
 def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax",
@@ -103,8 +104,9 @@ def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax",
             raise ConfigurationError(f"bias must be float32 [{E}], got {bias.dtype} "
                                      f"{tuple(bias.shape)}")
         bias = bias.detach().contiguous()
-    return _Route.apply(logits, bias, nat.dtype_code(logits.dtype, wide=True), k, _SCORES[score],
-                        groups, top_groups, int(bool(renormalize)), float(scale))
+    return _Route.apply(logits, bias,
+                        (nat.dtype_code(logits.dtype, wide=True), k, _SCORES[score], groups,
+                         top_groups, int(bool(renormalize)), float(scale)))
 
 
 __all__ = ["MAX_EXPERTS", "MAX_TOP_K", "route_topk"]
