@@ -477,8 +477,8 @@ DPC_DEVICE int tiles_of(int rows) { return (rows + kMmTile - 1) / kMmTile; }
 // ---------------------------------------------------------------------------
 
 // A workgroup a compute unit goes through tiles, the next one's first step on its way
-// while a tile's epilogue runs.  2048 rows, 4096 wide, vocabulary 131072: 1.66 ms alone
-// (1.33 PFLOP/s; the K loop's bound, mm_tile.h); 8192 x 2048 x 32000 with exponentials
+// while a tile's epilogue runs.  2048 rows, 4096 wide, vocabulary 131072: 1.58 ms a call
+// (1.39 PFLOP/s; the K loop's bound, mm_tile.h); 8192 x 2048 x 32000 with exponentials
 // written: 850 us (1.26 PFLOP/s).  Nothing hides the epilogues' exponentials and stores.
 // (A frozen head's call of twice that: 3.83 ms with a workgroup a tile, 3.77 so.)
 // A tile is two halves of 128 columns (one a wave): statistics are per half, so the
@@ -1326,7 +1326,7 @@ DPC_DEVICE void product_epilogue(const ProductArgs& s, MmAcc<kHidden>& acc, int 
         *p = x;
       } else {
         store_row4(s.out, row * s.rows_a + a, s.rows_a - a, whole, s.out_bf16,
-                   shifted(x * f, shift));
+                   shifted(x, shift) * f);
       }
     }
   }
@@ -1419,7 +1419,7 @@ __global__ void __launch_bounds__(256) head_reduce_kernel(ReduceArgs a) {
     for (int s = 1; s < a.splits; ++s)
       x += *reinterpret_cast<const f32x4_t*>(a.partial + s * a.plane + row * a.lda + c);
     store_row4(a.out, (a.active ? a.active[row] : row) * (int64_t)a.D + c, a.D - c, whole,
-               a.out_bf16, shifted(x * (a.by_row ? all * a.by_row[row] : all), shift));
+               a.out_bf16, shifted(x, shift) * (a.by_row ? all * a.by_row[row] : all));
   }
 }
 
