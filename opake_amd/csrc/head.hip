@@ -639,7 +639,8 @@ DPC_DEVICE void stats_epilogue(const StatsArgs& s, MmAcc<false>& acc, const f32x
           }
         } else {
 #pragma unroll
-          for (int r = 0; r < 8; ++r) h[r] = (_Float16)(acc.v[2 * p + (r >> 2)][j][r & 3] * kDzScale);
+          for (int r = 0; r < 8; ++r)
+            h[r] = (_Float16)(acc.v[2 * p + (r >> 2)][j][r & 3] * kDzScale);
           *reinterpret_cast<half8_t*>(at) = h;
         }
       }
