@@ -240,6 +240,27 @@ def test_more_than_is_kept(dev, dtype, grad_h):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_many_rows_of_broken_lines(dev, dtype):
+    """Widths that are not whole 128-byte lines, with enough tokens to be copied."""
+    N, D, V = 8200, 264, 130
+    g, h, W, up = _inputs(dev, (N,), D, V, dtype, 21)
+    t = torch.randint(0, V, (N,), generator=g, device=dev)
+    t[::5] = -100
+    q, zero = _onehot(t, V, -100), torch.zeros(N, dtype=torch.float64, device=dev)
+    h.requires_grad_(True)
+    W.requires_grad_(True)
+    loss = head.linear_cross_entropy(h, W, t)
+    dh, dW = torch.autograd.grad(loss, [h, W], up)
+    L, DH, DW = _reference(h, W, q, zero, 1.0, up)
+    _close(loss, L, "loss")
+    _close(dh, DH, "hidden_grad")
+    _close(dW, DW, "weight_grad")
+    _frozen(lambda x, y: head.linear_cross_entropy(x, y, t), h, W, up, loss, q, zero, 1.0,
+            t == -100)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("N,D,V", [(1, 4096, 300), (40, 2500, 1000), (300, 1544, 513)])
 def test_few_tiles_and_a_long_sum(dev, N, D, V, dtype):
     """The logits' sums in slices: the loss alone, a frozen head, a trained one."""
