@@ -1661,8 +1661,12 @@ dim3 tile_grid(int64_t tiles) { return dim3((unsigned)(tiles < kUnits ? tiles : 
 
 // Workgroups of a dH product over at most tiles_n row blocks, in slices or not.
 dim3 product_tiles(const Plan& p, int tiles_n) {
-  const int64_t tiles = (int64_t)p.tiles_d * tiles_n;
-  return dim3((unsigned)(tiles < kMostSliced ? kMostSliced : tiles));
+  int64_t most = (int64_t)p.tiles_d * tiles_n;
+  for (int64_t n = p.tiles_d; n <= kUnits && n <= (int64_t)p.tiles_d * tiles_n; n += p.tiles_d) {
+    const int64_t sliced = n * slices(n, p.steps_h);
+    if (sliced > most) most = sliced;
+  }
+  return dim3((unsigned)most);
 }
 
 // Waves of a tile that may have rows.
