@@ -14,7 +14,8 @@ the usual case under per-example clipping -- the exponentials of up to 512 MiB
 of tokens at a time become its gradient in the forward, which is kept in
 float32 for the backward to scale.  A trained head keeps its exponentials (16
 bits each, 32 for float32) where all of them fit in 512 MiB, and makes the
-logits again, piece by piece of the vocabulary, where they do not.  So no more
+logits again, piece by piece of the vocabulary, where they do not.  With gradients
+disabled the loss alone is made, whatever requires one.  So no more
 than 512 MiB of any ``[tokens, vocabulary]`` kind are kept, and twice that exist
 at a time (one 256-wide row or column block, where that is more).
 """
@@ -57,7 +58,7 @@ def _integer(t: torch.Tensor, what: str) -> None:
 class _HeadLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, index, teacher, options):
-        ignore_index, temperature, code = options
+        ignore_index, temperature, code, grad_enabled = options
         dev = hidden.device
         lead, D = hidden.shape[:-1], hidden.shape[-1]
         V = weight.shape[0]
@@ -66,7 +67,8 @@ class _HeadLoss(torch.autograd.Function):
         index = index.to(torch.int64).contiguous()
         if teacher is not None:
             teacher = teacher.to(torch.float32).contiguous()
-        want_h, want_w = ctx.needs_input_grad[:2]
+        # needs_input_grad is true of a parameter under no_grad too.
+        want_h, want_w = (need and grad_enabled for need in ctx.needs_input_grad[:2])
         lib, sizes = nat.load(), (N, D, V, K, code, int(want_h), int(want_w))
         loss = torch.empty(lead, dtype=torch.float32, device=dev)
         state_bytes = lib.dpc_head_loss_state_bytes(*sizes)
@@ -121,7 +123,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     if targets.shape != hidden.shape[:-1]:
         raise ConfigurationError(
             f"targets must be {tuple(hidden.shape[:-1])}, got {tuple(targets.shape)}")
-    return _HeadLoss.apply(hidden, weight, targets, None, (int(ignore_index), 1.0, code))
+    return _HeadLoss.apply(hidden, weight, targets, None,
+                           (int(ignore_index), 1.0, code, torch.is_grad_enabled()))
 
 
 def topk_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logits: torch.Tensor,
@@ -151,7 +154,7 @@ def topk_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logits
     if not (0.0 < temperature < 1e15 and math.isfinite(temperature)):
         raise ConfigurationError(f"temperature must be positive, got {temperature}")
     return _HeadLoss.apply(hidden, weight, teacher_indices, teacher_logits,
-                           (0, float(temperature), code))
+                           (0, float(temperature), code, torch.is_grad_enabled()))
 
 
 __all__ = ["linear_cross_entropy", "topk_distillation"]

@@ -509,3 +509,33 @@ def test_cpu_tensors_are_refused():
         head.linear_cross_entropy(h, W, torch.zeros(4, dtype=torch.int64))
     with pytest.raises(ConfigurationError, match="ROCm device"):
         head.topk_distillation(h, W, torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int64))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_without_grad_mode_only_the_loss_is_made(dev, dtype, mode):
+    """A parameter, or hidden states that require a gradient, evaluated with gradients
+    off: the loss-only plan's memory, and its bits."""
+    N, D, V = 512, 64, 5000
+    g, h, W, _ = _inputs(dev, (N,), D, V, dtype, 41)
+    t = torch.randint(0, V, (N,), generator=g, device=dev)
+
+    def peak(h, W):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        with mode():
+            loss = head.linear_cross_entropy(h, W, t)
+        return loss, torch.cuda.max_memory_allocated() - before
+
+    want, least = peak(h, W)
+    for x, w in ((h, W.requires_grad_()), (h.requires_grad_(), W), (h, W.detach())):
+        loss, most = peak(x, w)
+        assert torch.equal(loss, want) and not loss.requires_grad
+        assert most == least
+    tl, ti = torch.randn(N, 8, device=dev), torch.arange(8, device=dev).expand(N, 8)
+    with mode():
+        a = head.topk_distillation(h, W, tl, ti)
+        b = head.topk_distillation(h.detach(), W.detach(), tl, ti)
+    assert torch.equal(a, b)
