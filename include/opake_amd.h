@@ -38,7 +38,12 @@ extern "C" {
  * take DPC_F16 and DPC_F64. */
 enum dpc_dtype { DPC_F32 = 0, DPC_BF16 = 1, DPC_F16 = 2, DPC_F64 = 3 };
 enum dpc_scale_kind { DPC_SCALE_FIXED = 0, DPC_SCALE_AUTO_S = 1 };
-enum dpc_route_score { DPC_ROUTE_SOFTMAX = 0, DPC_ROUTE_SIGMOID = 1 };
+/* DPC_ROUTE_GROUPS_BY_TWO is added to a score. */
+enum dpc_route_score {
+  DPC_ROUTE_SOFTMAX = 0,
+  DPC_ROUTE_SIGMOID = 1,
+  DPC_ROUTE_GROUPS_BY_TWO = 2
+};
 enum dpc_noise_mode { DPC_NOISE_NONE = 0, DPC_NOISE_INJECTED = 1, DPC_NOISE_PHILOX = 2 };
 
 /* Library ABI version (major * 100 + minor). */
@@ -568,18 +573,21 @@ int dpc_head_loss_grad(const void* hidden, const void* weight, int64_t N, int D,
  * through torch's softmax and topk, packages/opake-patches/src/opake/api/patches/
  * kernels/moe.py:570-627; this adds the scores, bias and groups of other routers).
  *
- * logits [N, E] (fp32, bf16 or fp16), E <= 1024; `score` is an enum
- * dpc_route_score; bias [E] or NULL is added to the scores for the choice only.
+ * logits [N, E] (fp32, bf16 or fp16), E <= 1024; `score` is DPC_ROUTE_SOFTMAX or
+ * DPC_ROUTE_SIGMOID; bias [E] or NULL is added to the scores for the choice only.
  * The experts form `groups` equal groups of consecutive ones, of which the
- * top_groups with the largest key take part; of theirs, the k (<= 64) largest
- * keys are chosen, in descending order, ties to the lower index.  The keys are
- * the float32 scores plus bias, or without a bias the logits (the same order).
+ * top_groups with the largest key take part, or with DPC_ROUTE_GROUPS_BY_TWO (the rule
+ * of the routers that have sigmoid scores and a bias) those whose two largest scores
+ * plus bias have the largest sum; an expert that is alone in its group, or alone is not
+ * masked there, counts for itself.  Of the groups' experts, the k (<= 64) largest
+ * keys are chosen, in descending order, ties to the lower index (of groups too).  The
+ * keys are the float32 scores plus bias, or without a bias the logits (the same order).
  * weights [N, k]: the scores, divided by their sum over the chosen if
  * `renormalize` (0 if that is 0), times scale.  A logit or key of -inf or NaN is
  * never chosen; slots with nothing left get expert -1 and weight 0; a NaN logit
  * makes its row's weights NaN.
  *
- * dpc_route_topk_grad takes the two outputs and writes grad_logits [N, E] from
+ * dpc_route_topk_grad takes the two outputs (and the score alone) and writes grad_logits [N, E] from
  * grad_weights [N, k] in the logits' dtype; the choice itself has no gradient. */
 int dpc_route_topk(const void* logits, int64_t N, int E, int dtype, const float* bias, int k,
                    int score, int groups, int top_groups, int renormalize, double scale,

@@ -33,6 +33,7 @@ SCALE_FIXED = 0
 SCALE_AUTO_S = 1
 ROUTE_SOFTMAX = 0
 ROUTE_SIGMOID = 1
+ROUTE_GROUPS_BY_TWO = 2
 NOISE_NONE = 0
 NOISE_INJECTED = 1
 NOISE_PHILOX = 2

@@ -4,7 +4,8 @@
 //   s_e = softmax(z)_e or 1 / (1 + exp(-z_e));  key_e = s_e + bias_e, or z_e without a
 //   bias (the same order, no rounding)
 //   groups: E / groups consecutive experts each; only the top_groups groups whose
-//   largest keys are largest take part
+//   largest keys are largest take part, or (by_two) those whose two largest s_e + bias_e
+//   have the largest sum (of one expert that is left: that one's)
 //   w_j = scale s_j, or scale s_j / sum over the chosen s
 //
 // Ties go to the lower index.  An expert whose logit or key is -inf or NaN is never
@@ -18,7 +19,8 @@
 //
 // Few tokens: a launch's latency (16 tokens of 256 experts: 6 us).  Many: the rounds'
 // operations (65536 tokens, 256 experts in 8 groups of which 4, the best 8: 47 us, 67 MB
-// of logits at 1.4 TB/s; 63 us with the index found in every round).
+// of logits at 1.4 TB/s; 63 us with the index found in every round; groups by two: 8 us
+// more, 9 where a group is not whole lanes).
 #include <math.h>
 
 #include "common.h"
@@ -32,7 +34,7 @@ struct RouteArgs {
   const float* bias;  // [E] or null
   int k, sigmoid, groups, top_groups, renormalize;
   float scale;
-  float* weights;   // [N, k]
+  float* weights;    // [N, k]
   int64_t* experts;  // [N, k]
 };
 
@@ -47,6 +49,10 @@ DPC_DEVICE uint32_t order_key(float x) {
   if (!(x > -INFINITY)) return 0;
   const uint32_t u = __float_as_uint(x + 0.0f);
   return (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+DPC_DEVICE float key_value(uint32_t key) {
+  return __uint_as_float((key >> 31) ? key & 0x7fffffffu : ~key);
 }
 
 template <int kCtrl>
@@ -104,6 +110,35 @@ constexpr float kLog2e = 1.44269504088896340736f;
 DPC_DEVICE float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 // (The hardware's reciprocal, 1 ulp; of infinity 0.)
 DPC_DEVICE float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.0f + fast_exp(-z)); }
+
+// The two largest keys of each lane (a >= b) to those of the row's lanes, in every one
+// of them.
+template <int kLanes>
+DPC_DEVICE void row_two(uint32_t& a, uint32_t& b) {
+  auto join = [&](uint32_t oa, uint32_t ob) __attribute__((always_inline)) {
+    b = MaxU()(MinU()(a, oa), MaxU()(b, ob));
+    a = MaxU()(a, oa);
+  };
+  if (kLanes >= 2) join(lane_move<0xB1>(a), lane_move<0xB1>(b));
+  if (kLanes >= 4) join(lane_move<0x4E>(a), lane_move<0x4E>(b));
+  if (kLanes >= 8) join(lane_move<0x141>(a), lane_move<0x141>(b));
+  if (kLanes >= 16) join(lane_move<0x140>(a), lane_move<0x140>(b));
+  if (kLanes >= 64) {
+    const uint32_t x = a, y = b;
+    a = __builtin_amdgcn_readlane(x, 0);
+    b = __builtin_amdgcn_readlane(y, 0);
+#pragma unroll
+    for (int l = 16; l < 64; l += 16)
+      join(__builtin_amdgcn_readlane(x, l), __builtin_amdgcn_readlane(y, l));
+  }
+}
+
+// The key of a group's two largest keys' sum; 0 where it has none.  (Sums that overflow
+// downwards still count as there.)
+DPC_DEVICE uint32_t sum_key(uint32_t a, uint32_t b) {
+  if (a == 0) return 0;
+  return MaxU()(order_key(b ? key_value(a) + key_value(b) : key_value(a)), 1u);
+}
 
 // The largest key among key[] and its lowest index (none: 0).
 template <int kLanes, int kVals>
@@ -163,19 +198,28 @@ DPC_DEVICE void choose_any(uint32_t (&key)[kVals], int lane, int k, int* mine) {
   }
 }
 
-// Groups of kSlots * kLanes experts: group g is key[kSlots g ..] of all the row's
-// lanes, so their best are row maxima that every lane holds.  Keys outside the
-// top_groups best groups become 0.
-template <int kLanes, int kVals, int kSlots>
-DPC_DEVICE void keep_groups(uint32_t (&key)[kVals], int top_groups) {
+// Groups of kSlots * kLanes experts: group g is by[kSlots g ..] of all the row's
+// lanes, so their best (kByTwo: the sums of their two best) are row maxima that every
+// lane holds.  Keys outside the top_groups best groups become 0.
+template <int kLanes, int kVals, int kSlots, bool kByTwo>
+DPC_DEVICE void keep_groups(uint32_t (&key)[kVals], const uint32_t (&by)[kVals], int top_groups) {
   constexpr int kGroups = kVals / kSlots;
   uint32_t best[kGroups];
 #pragma unroll
   for (int g = 0; g < kGroups; ++g) {
-    uint32_t m = key[g * kSlots];
+    uint32_t m = by[g * kSlots], second = 0;
 #pragma unroll
-    for (int v = 1; v < kSlots; ++v) m = MaxU()(m, key[g * kSlots + v]);
-    best[g] = row_all<kLanes>(m, MaxU());
+    for (int v = 1; v < kSlots; ++v) {
+      const uint32_t x = by[g * kSlots + v];
+      if (kByTwo) second = MaxU()(second, MinU()(m, x));
+      m = MaxU()(m, x);
+    }
+    if (kByTwo) {
+      row_two<kLanes>(m, second);
+      best[g] = sum_key(m, second);
+    } else {
+      best[g] = row_all<kLanes>(m, MaxU());
+    }
   }
   uint32_t kept = 0;
   for (int r = 0; r < top_groups; ++r) {
@@ -221,7 +265,48 @@ DPC_DEVICE void keep_any_groups(uint32_t (&key)[kVals], int lane, int size, int 
     if (!((kept >> v) & 1)) key[v] = 0;
 }
 
+// The same by the sums of their two largest keys: each group's in a pass over the keys,
+// lane g % kLanes keeps group g's (there are no more groups than experts), then a round
+// for each one kept.
 template <int kLanes, int kVals>
+DPC_DEVICE void keep_any_groups_by_two(uint32_t (&key)[kVals], const uint32_t (&by)[kVals],
+                                       int lane, int size, int groups, int top_groups) {
+  const uint32_t magic = (1u << 20) / size + 1;
+  uint32_t best[kVals];
+  uint32_t kept = 0;
+#pragma unroll
+  for (int v = 0; v < kVals; ++v) best[v] = 0;
+  for (int g = 0; g < groups; ++g) {
+    uint32_t m = 0, second = 0;
+#pragma unroll
+    for (int v = 0; v < kVals; ++v) {
+      const int of = (int)(((uint32_t)(lane + v * kLanes) * magic) >> 20);
+      const uint32_t x = of == g ? by[v] : 0u;
+      second = MaxU()(second, MinU()(m, x));
+      m = MaxU()(m, x);
+    }
+    row_two<kLanes>(m, second);
+    const uint32_t sum = sum_key(m, second);
+#pragma unroll
+    for (int v = 0; v < kVals; ++v)
+      if (lane + v * kLanes == g) best[v] = sum;
+  }
+  for (int r = 0; r < top_groups; ++r) {
+    int at;
+    const uint32_t m = row_first<kLanes, kVals>(best, lane, &at);
+    const int g = m ? at : -1;
+#pragma unroll
+    for (int v = 0; v < kVals; ++v) {
+      if (lane + v * kLanes == g) best[v] = 0;
+      if ((int)(((uint32_t)(lane + v * kLanes) * magic) >> 20) == g) kept |= 1u << v;
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < kVals; ++v)
+    if (!((kept >> v) & 1)) key[v] = 0;
+}
+
+template <int kLanes, int kVals, bool kByTwo>
 __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
   constexpr int kRows = 64 / kLanes;
   const int lane = threadIdx.x % kLanes;
@@ -240,7 +325,7 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
   }
   nan = row_all<kLanes>(nan ? 1u : 0u, OrU()) != 0;
   float top = -INFINITY, inv = 0.0f;
-  if (!a.sigmoid && (a.bias || !a.renormalize)) {
+  if (!a.sigmoid && (a.bias || !a.renormalize || kByTwo)) {
 #pragma unroll
     for (int v = 0; v < kVals; ++v) top = fmaxf(top, z[v]);
     top = row_max<kLanes>(top);
@@ -264,12 +349,21 @@ __global__ void __launch_bounds__(256) route_kernel(RouteArgs a) {
   }
   if (a.top_groups < a.groups) {
     const int size = a.E / a.groups, slots = size / kLanes;
+    uint32_t by[kVals];  // what the groups go by
+#pragma unroll
+    for (int v = 0; v < kVals; ++v) {
+      by[v] = key[v];
+      if (kByTwo && !a.bias && key[v])  // scores: the logits add up in another order
+        by[v] = order_key(a.sigmoid ? sigmoid(z[v]) : fast_exp(z[v] - top) * inv);
+    }
     if (size % kLanes == 0 && kVals >= 2 && slots == 1)
-      keep_groups<kLanes, kVals, 1>(key, a.top_groups);
+      keep_groups<kLanes, kVals, 1, kByTwo>(key, by, a.top_groups);
     else if (size % kLanes == 0 && kVals >= 4 && slots == 2)
-      keep_groups<kLanes, kVals, kVals >= 4 ? 2 : 1>(key, a.top_groups);
+      keep_groups<kLanes, kVals, kVals >= 4 ? 2 : 1, kByTwo>(key, by, a.top_groups);
     else if (size % kLanes == 0 && kVals >= 8 && slots == 4)
-      keep_groups<kLanes, kVals, kVals >= 8 ? 4 : 1>(key, a.top_groups);
+      keep_groups<kLanes, kVals, kVals >= 8 ? 4 : 1, kByTwo>(key, by, a.top_groups);
+    else if (kByTwo)
+      keep_any_groups_by_two<kLanes, kVals>(key, by, lane, size, a.groups, a.top_groups);
     else
       keep_any_groups<kLanes, kVals>(key, lane, size, a.top_groups);
   }
@@ -427,10 +521,13 @@ bool valid_route(int64_t N, int E, int k, int dtype, int score) {
 }
 
 template <int kLanes, int kVals>
-int launch_route(const RouteArgs& a, hipStream_t s) {
+int launch_route(const RouteArgs& a, bool by_two, hipStream_t s) {
   constexpr int kRows = 4 * (64 / kLanes);
-  hipLaunchKernelGGL((route_kernel<kLanes, kVals>), dim3((unsigned)((a.N + kRows - 1) / kRows)),
-                     dim3(256), 0, s, a);
+  const dim3 grid((unsigned)((a.N + kRows - 1) / kRows));
+  if (by_two)
+    hipLaunchKernelGGL((route_kernel<kLanes, kVals, true>), grid, dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((route_kernel<kLanes, kVals, false>), grid, dim3(256), 0, s, a);
   DPC_HIP_CHECK(hipGetLastError());
   return DPC_OK;
 }
@@ -440,6 +537,8 @@ int launch_route(const RouteArgs& a, hipStream_t s) {
 extern "C" int dpc_route_topk(const void* logits, int64_t N, int E, int dtype, const float* bias,
                               int k, int score, int groups, int top_groups, int renormalize,
                               double scale, float* weights, int64_t* experts, void* stream) {
+  const bool by_two = (score & DPC_ROUTE_GROUPS_BY_TWO) != 0 && top_groups < groups;
+  score &= ~DPC_ROUTE_GROUPS_BY_TWO;
   if (!valid_route(N, E, k, dtype, score) || groups < 1 || E % groups || top_groups < 1 ||
       top_groups > groups || k > top_groups * (E / groups))
     return DPC_EINVAL;
@@ -448,11 +547,11 @@ extern "C" int dpc_route_topk(const void* logits, int64_t N, int E, int dtype, c
   const RouteArgs a = {logits, N, E, dtype, bias, k, score == DPC_ROUTE_SIGMOID, groups, top_groups,
                        renormalize != 0, (float)scale, weights, experts};
   hipStream_t s = (hipStream_t)stream;
-  if (k <= 4 && E <= 8) return launch_route<4, 2>(a, s);
-  if (k <= 16 && E <= 64) return launch_route<16, 4>(a, s);
-  if (k <= 16 && E <= 256 && N >= 4096) return launch_route<16, 16>(a, s);
-  if (E <= 256) return launch_route<64, 4>(a, s);
-  return launch_route<64, 16>(a, s);
+  if (k <= 4 && E <= 8) return launch_route<4, 2>(a, by_two, s);
+  if (k <= 16 && E <= 64) return launch_route<16, 4>(a, by_two, s);
+  if (k <= 16 && E <= 256 && N >= 4096) return launch_route<16, 16>(a, by_two, s);
+  if (E <= 256) return launch_route<64, 4>(a, by_two, s);
+  return launch_route<64, 16>(a, by_two, s);
 }
 
 extern "C" int dpc_route_topk_grad(const void* logits, int64_t N, int E, int dtype, int k, int score,

@@ -58,8 +58,8 @@ class SwiGLUExpert(nn.Module):
 class TopKMoE(nn.Module):
     """``d``-wide top-``k`` MoE FFN with ``n_experts`` SwiGLU experts of width ``inter``.
 
-    ``routing``: keyword arguments of ``route_topk`` (``score``, ``groups``,
-    ``top_groups``, ``renormalize``, ``scale``), which then routes."""
+    ``routing``: keyword arguments of ``route_topk`` (``score``, ``groups``, ``top_groups``,
+    ``group_score``, ``renormalize``, ``scale``), which then routes."""
 
     def __init__(self, d: int, inter: int, n_experts: int, top_k: int = 2, *,
                  routing: dict | None = None, dtype=None, device=None):

@@ -293,3 +293,98 @@ def test_refusals(dev):
 def test_cpu_tensors_are_refused():
     with pytest.raises(ConfigurationError, match="ROCm device"):
         routing.route_topk(torch.zeros(4, 12), 2)
+
+
+def _top2_reference(z, k, score, bias, groups, top_groups):
+    """The choice in 64 bits, with the gap of every row's closest decision over the size
+    of its keys."""
+    N, E = z.shape
+    zd = z.double()
+    closed = ~(zd > -math.inf)
+    s = torch.sigmoid(zd) if score == "sigmoid" else torch.softmax(zd, 1).nan_to_num(0.0)
+    key = torch.where(closed, -math.inf, s if bias is None else s + bias.double())
+    two = key.view(N, groups, -1).sort(dim=2, descending=True).values[..., :2]
+    best = torch.where(two > -math.inf, two, 0.0).sum(2)
+    best = torch.where(two[..., 0] > -math.inf, best, -math.inf)
+
+    def ranked(v, n):
+        v, at = v.sort(dim=1, descending=True, stable=True)
+        gap = v[:, :n] - v[:, 1:n + 1] if v.shape[1] > n else v[:, :n - 1] - v[:, 1:n]
+        return v, at, torch.where(gap.isnan(), math.inf, gap)
+
+    v, at, gap = ranked(best, top_groups)
+    near = gap[:, -1] if top_groups < groups else torch.full((N,), math.inf, device=z.device)
+    keep = torch.zeros(N, groups, dtype=torch.bool, device=z.device)
+    keep.scatter_(1, at[:, :top_groups], v[:, :top_groups] > -math.inf)
+    key = torch.where(keep.repeat_interleave(E // groups, 1), key, -math.inf)
+    v, at, gap = ranked(key, k)
+    near = torch.minimum(near, gap.amin(1)) if gap.numel() else near
+    size = torch.where(closed, 0.0, key).nan_to_num(0.0, neginf=0.0).abs().amax(1)
+    return torch.where(v[:, :k] > -math.inf, at[:, :k], -1), near / size
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [True, False])
+@pytest.mark.parametrize("N,E,k,groups,top_groups", [
+    (700, 8, 2, 2, 1), (700, 16, 3, 4, 2), (700, 60, 4, 6, 3), (700, 256, 8, 8, 4),
+    (5000, 256, 8, 8, 4), (5000, 128, 6, 2, 1), (5000, 192, 8, 3, 2), (700, 384, 8, 8, 3),
+    (300, 1024, 32, 64, 8), (700, 12, 2, 12, 5), (700, 36, 5, 18, 7), (900, 64, 17, 4, 3),
+])
+def test_groups_by_the_sum_of_their_two_best(dev, N, E, k, groups, top_groups, score, biased):
+    """Rows in which two of the keys or sums that the choice goes by are nearer than
+    float32 rounding could swap are left out."""
+    g = torch.Generator(device=dev).manual_seed(E + k)
+    z = torch.randn(N, E, generator=g, device=dev) * 1.5
+    z[torch.rand(N, E, generator=g, device=dev) < 0.2] = -math.inf
+    z[0] = -math.inf
+    z[1, 1:] = -math.inf
+    bias = None
+    if biased:
+        bias = torch.randint(-60, 61, (E,), generator=g, device=dev).float() * 1e-3
+    want, near = _top2_reference(z, k, score, bias, groups, top_groups)
+    w, e = routing.route_topk(z, k, score=score, bias=bias, groups=groups,
+                              top_groups=top_groups, group_score="top2")
+    ok = ~(near <= 4e-6)
+    assert ok.sum() >= 0.5 * N
+    assert torch.equal(e[ok], want[ok])
+    # The weights and their gradient are those of the same experts however chosen.
+    up = torch.randn(N, k, generator=g, device=dev)
+    x = z.clone().requires_grad_(True)
+    w, e = routing.route_topk(x, k, score=score, bias=bias, groups=groups, scale=2.5,
+                              top_groups=top_groups, group_score="top2")
+    (dz,) = torch.autograd.grad(w, [x], up)
+    xd = z.double().requires_grad_(True)
+    there = e >= 0
+    zc = xd.gather(1, e.clamp(min=0))
+    s = torch.sigmoid(zc) if score == "sigmoid" else torch.exp(
+        zc - torch.where(there, zc, -math.inf).amax(1, keepdim=True).nan_to_num(0.0, neginf=0.0))
+    s = torch.where(there, s, 0.0)
+    tot = s.sum(1, keepdim=True)
+    wd = 2.5 * s / torch.where(tot > 0, tot, 1.0)
+    (dd,) = torch.autograd.grad(wd, [xd], up.double())
+    dd = torch.where(z > -math.inf, dd.nan_to_num(0.0), 0.0)
+    span = z.nan_to_num(0.0, neginf=0.0).abs().amax(1, keepdim=True).double()
+    rel = 2.0**-20 * (1 + 2 * span) * (k + 2)
+    assert ((w.double() - wd).abs() <= rel * wd.abs() + 1e-30).all()
+    row = 2.5 * up.double().abs().sum(1, keepdim=True)
+    assert ((dz.double() - dd).abs() <= 2 * rel * row).all()
+
+
+@pytest.mark.gpu
+def test_the_group_rules_differ(dev):
+    """A group with the largest key against one with two large ones; ties of sums go to the
+    first group; a group of one open expert counts that alone."""
+    inf = math.inf
+    z = torch.tensor([[3.0, -3.0, 1.0, 1.0], [1.0, 0.0, 0.0, 1.0], [3.0, -inf, 0.0, 0.0],
+                      [3.0, -inf, -9.0, -9.0]], device=dev)
+    for score in ("softmax", "sigmoid"):
+        kw = dict(score=score, groups=2, top_groups=1)
+        assert routing.route_topk(z, 2, **kw)[1].tolist() == [[0, 1], [0, 1], [0, -1], [0, -1]]
+        by_two = routing.route_topk(z, 2, group_score="top2", **kw)[1].tolist()
+        # softmax: 3 against 1 + 1 is e^3 + e^-3 against 2 e
+        first = [0, 1] if score == "softmax" else [2, 3]
+        third = [0, -1] if score == "softmax" else [2, 3]
+        assert by_two == [first, [0, 1], third, [0, -1]]
+    with pytest.raises(ConfigurationError):
+        routing.route_topk(z, 2, group_score="sum", **kw)
