@@ -151,8 +151,10 @@ class RoutedLM(nn.Module):
         return x if teacher_logits is None else (x, teacher_logits, teacher_indices)
 
     def loss(self, outputs, targets: torch.Tensor) -> torch.Tensor:
-        """Each example's loss [B] (float32): the mean over its tokens.  Tokens whose
-        target is ``ignore_index`` count as zeros."""
+        """Each example's loss [B] (float32): the mean over its tokens.  A target of
+        ``ignore_index`` makes its token's cross entropy zero, not its part of the KL,
+        which goes by the teacher's entries: negative ``teacher_indices`` leave a token
+        out of that too."""
         hidden, teacher = (outputs, None) if torch.is_tensor(outputs) else (outputs[0],
                                                                              outputs[1:])
         loss = linear_cross_entropy(hidden, self.head.weight, targets,

@@ -135,3 +135,27 @@ def test_loss_without_a_teacher(dev):
                            ignore_index=-100).view(tgt.shape).mean(dim=1)
     torch.testing.assert_close(model.loss(hidden, tgt.to(dev)).double(), want, rtol=1e-5,
                                atol=1e-5)
+
+
+def test_ignored_targets_and_the_teacher(dev):
+    """An ignored target takes its token out of the cross entropy alone; the teacher's KL
+    there goes by the teacher's entries, and negative indices take it out as well."""
+    ref, ids, tgt, teacher, index = _case(2, 9, seed=11)
+    model = _gpu_model(ref, dev)
+    ids, tgt, teacher, index = (x.to(dev) for x in (ids, tgt, teacher, index))
+    tgt[1, 3] = -100
+    ignored = (tgt == -100).unsqueeze(-1)
+    other = torch.where(ignored, teacher + torch.randn_like(teacher), teacher)
+
+    def run(teacher, index):
+        loss = model.loss(model(ids, teacher, index), tgt)
+        return loss, torch.autograd.grad(loss.sum(), [model.moe.experts[0].down.weight])[0]
+
+    a, b = run(teacher, index), run(other, index)
+    assert (a[0] != b[0]).all() and not torch.equal(a[1], b[1])
+    out = index.masked_fill(ignored, -1)
+    c, d = run(teacher, out), run(other, out)
+    assert torch.equal(c[0], d[0]) and torch.equal(c[1], d[1])
+    hidden = model(ids)
+    want = _plain_loss(ref.double().to(dev))((hidden.double(), teacher, index), tgt)
+    torch.testing.assert_close(a[0].double(), want, rtol=1e-5, atol=1e-5)
