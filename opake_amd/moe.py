@@ -77,6 +77,15 @@ class TopKMoE(nn.Module):
                                  torch.zeros(n_experts, dtype=torch.float32, device=device))
         self.last_counts: torch.Tensor | None = None  # [E, B] host copy of the last routing
 
+    def _apply(self, fn, recurse=True):
+        """Casts leave ``route_bias`` in float32: a balancing rule's steps are below what
+        bfloat16 holds, and ``route_topk`` takes nothing else."""
+        bias = self._buffers.get("route_bias")
+        super()._apply(fn, recurse)
+        if bias is not None and self.route_bias.dtype != torch.float32:
+            self.route_bias = bias.to(self.route_bias.device)
+        return self
+
     def route(self, x: torch.Tensor, router_logits: torch.Tensor | None = None):
         """Top-k expert indices and weights ([B, T, k] each); -1: none (``routing`` only)."""
         logits = self.router(x) if router_logits is None else router_logits

@@ -147,15 +147,23 @@ def test_ignored_targets_and_the_teacher(dev):
     ignored = (tgt == -100).unsqueeze(-1)
     other = torch.where(ignored, teacher + torch.randn_like(teacher), teacher)
 
+    hidden = model(ids).detach().requires_grad_(True)
+
     def run(teacher, index):
-        loss = model.loss(model(ids, teacher, index), tgt)
-        return loss, torch.autograd.grad(loss.sum(), [model.moe.experts[0].down.weight])[0]
+        loss = model.loss((hidden, teacher, index), tgt)
+        return loss, torch.autograd.grad(loss.sum(), [hidden])[0]
 
     a, b = run(teacher, index), run(other, index)
     assert (a[0] != b[0]).all() and not torch.equal(a[1], b[1])
     out = index.masked_fill(ignored, -1)
     c, d = run(teacher, out), run(other, out)
     assert torch.equal(c[0], d[0]) and torch.equal(c[1], d[1])
-    hidden = model(ids)
     want = _plain_loss(ref.double().to(dev))((hidden.double(), teacher, index), tgt)
     torch.testing.assert_close(a[0].double(), want, rtol=1e-5, atol=1e-5)
+
+
+def test_a_cast_model_routes(dev):
+    torch.manual_seed(3)
+    moe = TopKMoE(D, INTER, 4, 2, routing=dict(score="sigmoid")).to(dev, torch.bfloat16)
+    x = torch.randn(2, 3, D, device=dev, dtype=torch.bfloat16)
+    assert moe(x).shape == x.shape and moe(x).dtype == torch.bfloat16
