@@ -103,8 +103,10 @@ class TopKMoE(nn.Module):
         token = torch.arange(B * T, device=x.device).repeat_interleave(k)
         weight = top_w.reshape(-1)
         if self.routing is not None:
-            chosen = expert >= 0
-            expert, token, weight = expert[chosen], token[chosen], weight[chosen]
+            # A token whose logits are all NaN has NaN weights and no expert: any will do to
+            # keep it NaN.
+            chosen = (expert >= 0) | weight.isnan()
+            expert, token, weight = expert[chosen].clamp(min=0), token[chosen], weight[chosen]
         order = torch.argsort(expert * (B * T) + token, stable=True)
         counts = torch.bincount(expert * B + token // T, minlength=E * B).view(E, B).cpu()
         self.last_counts = counts

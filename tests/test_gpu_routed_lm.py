@@ -167,3 +167,22 @@ def test_a_cast_model_routes(dev):
     moe = TopKMoE(D, INTER, 4, 2, routing=dict(score="sigmoid")).to(dev, torch.bfloat16)
     x = torch.randn(2, 3, D, device=dev, dtype=torch.bfloat16)
     assert moe(x).shape == x.shape and moe(x).dtype == torch.bfloat16
+
+
+def test_nan_logits_reach_the_output(dev):
+    """A token of which a logit, or every logit, is NaN has a NaN output, with or without
+    ``routing``; the other tokens keep theirs."""
+    torch.manual_seed(2)
+    plain = TopKMoE(D, INTER, 4, 2, dtype=torch.float32).to(dev)
+    moe = TopKMoE(D, INTER, 4, 2, routing={}, dtype=torch.float32).to(dev)
+    moe.load_state_dict(plain.state_dict(), strict=False)
+    x = torch.randn(2, 3, D, device=dev)
+    logits = torch.randn(2, 3, 4, device=dev)
+    want = moe(x, logits)
+    logits[0, 1] = torch.nan
+    logits[1, 2, 3] = torch.nan
+    bad = torch.isnan(logits).any(-1)
+    for m in (plain, moe):
+        y = m(x, logits)
+        assert torch.isnan(y[bad]).all()
+        torch.testing.assert_close(y[~bad], want[~bad], rtol=1e-5, atol=1e-6)
