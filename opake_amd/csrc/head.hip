@@ -867,21 +867,24 @@ DPC_DEVICE void join_row(const JoinArgs& a, int64_t n, float lse, int lane) {
     bad |= c == -2;
     if (c >= 0) {
       bad |= isnan(teacher[k]);
-      tm = fmaxf(tm, teacher[k] * a.inv_tau);
+      tm = fmaxf(tm, teacher[k]);
     }
   }
   bad = __any(bad);
   tm = wave_max(tm);
+  // Differences first: entries of any size, the type's lowest value among them, neither
+  // overflow nor leave a rounding of their own.
+  auto scaled = [&](int k) __attribute__((always_inline)) { return (teacher[k] - tm) * a.inv_tau; };
   float es = 0.f;
   for (int k = lane; k < a.K; k += 64)
-    if (cols[k] >= 0) es += fast_exp(teacher[k] * a.inv_tau - tm);
+    if (cols[k] >= 0) es += fast_exp(scaled(k));
   es = wave_sum(es);
   const float logs = logf(es);
   float loss = 0.f;
   for (int k0 = 0; k0 < a.K; k0 += 64) {
     const int k = k0 + lane;
     const int c = k < a.K ? cols[k] : -1;
-    const float lq = c >= 0 ? teacher[k] * a.inv_tau - tm - logs : -INFINITY;
+    const float lq = c >= 0 ? scaled(k) - logs : -INFINITY;
     const float q = fast_exp(lq), z = c >= 0 ? picked[k] : 0.f;
     if (c >= 0 && q != 0.f) loss += q * (lq - (z - lse) * kLn2);
     // q of every entry of this column: the other entries, 64 at a time.
@@ -889,7 +892,7 @@ DPC_DEVICE void join_row(const JoinArgs& a, int64_t n, float lse, int lane) {
     for (int i0 = 0; i0 < a.K; i0 += 64) {
       const int i = i0 + lane;
       const int ci = i < a.K ? cols[i] : -1;
-      const float qi = ci >= 0 ? fast_exp(teacher[i] * a.inv_tau - tm - logs) : 0.f;
+      const float qi = ci >= 0 ? fast_exp(scaled(i) - logs) : 0.f;
       const int left = min(64, a.K - i0);
       for (int o = 0; o < left; ++o) {
         const int co = __builtin_amdgcn_readlane(ci, o);

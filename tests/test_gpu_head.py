@@ -539,3 +539,26 @@ def test_without_grad_mode_only_the_loss_is_made(dev, dtype, mode):
         a = head.topk_distillation(h, W, tl, ti)
         b = head.topk_distillation(h.detach(), W.detach(), tl, ti)
     assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tau", [0.5, 1.0, 1.5, 3.0])
+def test_teacher_entries_at_the_lowest_value(dev, tau):
+    """Masks of the type's lowest value: beside other entries they weigh nothing, and a
+    row that holds nothing else is uniform over them.  Logits of any size are weighed by
+    their differences."""
+    V, K = 300, 5
+    low = torch.finfo(torch.float32).min
+    tl = torch.tensor([[1.0, 2.0, 3.0, low, low], [low] * 5, [3e38, 3e38, low, low, 1.0],
+                       [1e30, 1e30, 1e30, -1e30, 0.0], [-1e8, -1e8 - 8, -1e8 + 8, low, -2e8]],
+                      device=dev)
+    n = tl.shape[0]
+    g, h, W, up = _inputs(dev, (n,), 64, V, torch.float32, 43)
+    ti = torch.arange(K, device=dev) * 7 + torch.arange(n, device=dev)[:, None]
+    h.requires_grad_(True)
+    loss = head.topk_distillation(h, W, tl, ti, temperature=tau)
+    (dh,) = torch.autograd.grad(loss, [h], up)
+    q, ent = _soft(tl, ti, V, tau)
+    L, DH, _ = _reference(h, W, q, ent, tau, up, frozen=True)
+    _close(loss, L, "loss")
+    _close(dh, DH, "hidden_grad")
