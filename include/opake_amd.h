@@ -534,7 +534,7 @@ int dpc_row_sum_f64(const double* x, int B, int n, int accumulate, double* out, 
  *     p[index_k]).  An entry may be repeated (its q's add up) or -inf (q = 0);
  *     a row with no entry above -inf has loss 0.
  * An index outside the vocabulary that is not ignored makes its row's loss
- * (and gradients) NaN.  Sums are float32; float32 operands are multiplied
+ * (and gradients) NaN.  1e-15 < temperature < 1e15.  Sums are float32; float32 operands are multiplied
  * as two fp16 planes each, 2^-24 of a value (and 2^-39 of its row of H's or of W's
  * largest) away from it.
  *
@@ -583,7 +583,7 @@ int dpc_head_loss_grad(const void* hidden, const void* weight, int64_t N, int D,
  * keys are chosen, in descending order, ties to the lower index (of groups too).  The
  * keys are the float32 scores plus bias, or without a bias the logits (the same order).
  * weights [N, k]: the scores, divided by their sum over the chosen if
- * `renormalize` (0 if that is 0), times scale.  A logit or key of -inf or NaN is
+ * `renormalize` (0 if that is 0), times scale (a finite float32).  A logit or key of -inf or NaN is
  * never chosen; slots with nothing left get expert -1 and weight 0; a NaN logit
  * makes its row's weights NaN.
  *

@@ -1759,7 +1759,8 @@ int weight_product(const Plan& p, const PrepArgs& g, const Hidden& h, const MmOp
 
 bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; }
 
-bool valid_temperature(double t) { return t > 0.0 && t < 1e15; }
+// (Its square and its reciprocal are taken in float32.)
+bool valid_temperature(double t) { return t > 1e-15 && t < 1e15; }
 
 }  // namespace
 

@@ -21,6 +21,7 @@
 // operations (65536 tokens, 256 experts in 8 groups of which 4, the best 8: 47 us, 67 MB
 // of logits at 1.4 TB/s; 63 us with the index found in every round; groups by two: 8 us
 // more, 9 where a group is not whole lanes).
+#include <float.h>
 #include <math.h>
 
 #include "common.h"
@@ -520,6 +521,8 @@ bool valid_route(int64_t N, int E, int k, int dtype, int score) {
          (score == DPC_ROUTE_SOFTMAX || score == DPC_ROUTE_SIGMOID);
 }
 
+bool valid_scale(double scale) { return fabs(scale) <= FLT_MAX; }
+
 template <int kLanes, int kVals>
 int launch_route(const RouteArgs& a, bool by_two, hipStream_t s) {
   constexpr int kRows = 4 * (64 / kLanes);
@@ -540,7 +543,7 @@ extern "C" int dpc_route_topk(const void* logits, int64_t N, int E, int dtype, c
   const bool by_two = (score & DPC_ROUTE_GROUPS_BY_TWO) != 0 && top_groups < groups;
   score &= ~DPC_ROUTE_GROUPS_BY_TWO;
   if (!valid_route(N, E, k, dtype, score) || groups < 1 || E % groups || top_groups < 1 ||
-      top_groups > groups || k > top_groups * (E / groups))
+      top_groups > groups || k > top_groups * (E / groups) || !valid_scale(scale))
     return DPC_EINVAL;
   if (N == 0) return DPC_OK;
   if (!logits || !weights || !experts) return DPC_EINVAL;
@@ -558,7 +561,7 @@ extern "C" int dpc_route_topk_grad(const void* logits, int64_t N, int E, int dty
                                    int renormalize, double scale, const int64_t* experts,
                                    const float* weights, const float* grad_weights,
                                    void* grad_logits, void* stream) {
-  if (!valid_route(N, E, k, dtype, score)) return DPC_EINVAL;
+  if (!valid_route(N, E, k, dtype, score) || !valid_scale(scale)) return DPC_EINVAL;
   if (N == 0) return DPC_OK;
   if (!logits || !experts || !weights || !grad_weights || !grad_logits)
     return DPC_EINVAL;

@@ -22,8 +22,6 @@ at a time (one 256-wide row or column block, where that is more).
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from opake_amd import _native as nat
@@ -151,8 +149,9 @@ def topk_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logits
             f"{tuple(teacher_logits.shape)} and {tuple(teacher_indices.shape)}")
     if isinstance(temperature, bool) or not isinstance(temperature, (int, float)):
         raise InputTypeError(f"temperature must be a number, got {type(temperature)}")
-    if not (0.0 < temperature < 1e15 and math.isfinite(temperature)):
-        raise ConfigurationError(f"temperature must be positive, got {temperature}")
+    if not 1e-15 < temperature < 1e15:  # its square and reciprocal are float32's
+        raise ConfigurationError(
+            f"temperature must be between 1e-15 and 1e15, got {temperature}")
     return _HeadLoss.apply(hidden, weight, teacher_indices, teacher_logits,
                            (0, float(temperature), code, torch.is_grad_enabled()))
 

@@ -10,8 +10,6 @@ scores, a balancing bias and groups by the sum of their two best experts
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from opake_amd import _native as nat
@@ -19,6 +17,7 @@ from opake_amd.exceptions import ConfigurationError, InputTypeError
 
 MAX_EXPERTS = 1024
 MAX_TOP_K = 64
+_LARGEST = torch.finfo(torch.float32).max
 _SCORES = {"softmax": nat.ROUTE_SOFTMAX, "sigmoid": nat.ROUTE_SIGMOID}
 _GROUP_SCORES = {"max": 0, "top2": nat.ROUTE_GROUPS_BY_TWO}
 
@@ -104,8 +103,8 @@ def route_topk(logits: torch.Tensor, k: int, *, score: str = "softmax",
     if not 1 <= k <= min(MAX_TOP_K, top_groups * (E // groups)):
         raise ConfigurationError(
             f"k must be between 1 and {min(MAX_TOP_K, top_groups * (E // groups))}, got {k}")
-    if not math.isfinite(scale):
-        raise ConfigurationError(f"scale must be finite, got {scale}")
+    if not abs(scale) <= _LARGEST:
+        raise ConfigurationError(f"scale must be a finite float32, got {scale}")
     if bias is not None:
         if bias.dtype != torch.float32 or tuple(bias.shape) != (E,):
             raise ConfigurationError(f"bias must be float32 [{E}], got {bias.dtype} "

@@ -562,3 +562,12 @@ def test_teacher_entries_at_the_lowest_value(dev, tau):
     L, DH, _ = _reference(h, W, q, ent, tau, up, frozen=True)
     _close(loss, L, "loss")
     _close(dh, DH, "hidden_grad")
+
+
+@pytest.mark.gpu
+def test_temperatures_that_float32_cannot_square_are_refused(dev):
+    h, W = torch.zeros(4, 16, device=dev), torch.zeros(9, 16, device=dev)
+    tl, ti = torch.zeros(4, 3, device=dev), torch.zeros(4, 3, dtype=torch.int64, device=dev)
+    for tau in (1e-16, 1e-40, 1e16):
+        with pytest.raises(ConfigurationError):
+            head.topk_distillation(h, W, tl, ti, temperature=tau)

@@ -388,3 +388,11 @@ def test_the_group_rules_differ(dev):
         assert by_two == [first, [0, 1], third, [0, -1]]
     with pytest.raises(ConfigurationError):
         routing.route_topk(z, 2, group_score="sum", **kw)
+
+
+@pytest.mark.gpu
+def test_scales_that_float32_cannot_hold_are_refused(dev):
+    z = torch.zeros(4, 12, device=dev)
+    for scale in (1e39, -1e300):
+        with pytest.raises(ConfigurationError):
+            routing.route_topk(z, 2, scale=scale)
