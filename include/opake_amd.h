@@ -534,9 +534,10 @@ int dpc_row_sum_f64(const double* x, int B, int n, int accumulate, double* out, 
  *     p[index_k]).  An entry may be repeated (its q's add up) or -inf (q = 0);
  *     a row with no entry above -inf has loss 0.
  * An index outside the vocabulary that is not ignored makes its row's loss
- * (and gradients) NaN.  1e-15 < temperature < 1e15.  Sums are float32; float32 operands are multiplied
- * as two fp16 planes each, 2^-24 of a value (and 2^-39 of its row of H's or of W's
- * largest) away from it.
+ * (and gradients) NaN.  1e-15 < temperature < 1e15.  Sums are float32; float32
+ * operands are multiplied as two fp16 planes each, at most 2^-23 of a value (and 2^-39
+ * of its row of H's or of W's largest, of dz 2^-39) away from it, without the product of
+ * the two low ones (at most 2^-22 of the product).
  *
  * Rows without a target take no part in any product, whatever they hold.
  *

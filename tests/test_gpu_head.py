@@ -571,3 +571,94 @@ def test_temperatures_that_float32_cannot_square_are_refused(dev):
     for tau in (1e-16, 1e-40, 1e16):
         with pytest.raises(ConfigurationError):
             head.topk_distillation(h, W, tl, ti, temperature=tau)
+
+
+def _planes(x, top):
+    """x as the two fp16 planes of the kernels over the power of two of `top`: [first,
+    second], in 64 bits."""
+    s = 2.0 ** (14 - math.floor(math.log2(top)))
+    x0 = (x * s).to(torch.float16).double()
+    x1 = (x * s - x0).to(torch.float16).double()
+    return x0 / s, x1 / s
+
+
+def _plane_case(dev):
+    g = torch.Generator(device=dev).manual_seed(51)
+    N, D, V = 24, 8, 24
+    h = torch.randn(N, D, generator=g, device=dev)
+    W = torch.randn(V, D, generator=g, device=dev)
+    t = torch.randint(0, V, (N,), generator=g, device=dev)
+    up = torch.rand(N, generator=g, device=dev) + 0.5
+    return h, W, t, up
+
+
+def _plane_reference(h, W, t, up):
+    """Values in 64 bits and bounds of float32 accuracy.  A value is 2^-23 of itself away
+    from its planes and a product of two low planes is below 2^-22 of the product, so with
+    both operands' planes a term is off by 2^-21; a sum of 3 n products by 1.125 u (3 n)
+    of the terms (u = 2^-23); log sum exp, exponentials and logs add 2^-21 of what they
+    hold."""
+    h, W, up = h.double(), W.double(), up.double()[:, None]
+    N, D, V = h.shape[0], h.shape[1], W.shape[0]
+    q = _onehot(t, V, -100)
+
+    def product(x, xerr, y):  # x @ y, and how far it may be off
+        terms = x.abs() @ y.abs()
+        return x @ y, xerr @ y.abs() + (2.0**-21 + 1.125 * U * 3 * x.shape[1]) * terms
+
+    z, zerr = product(h, torch.zeros_like(h), W.t())
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    logp = z - lse
+    perr = zerr + zerr.amax(1, keepdim=True) + 2.0**-21 * (1 + z.abs() + lse.abs())
+    p = logp.exp()
+    loss, loss_tol = -(q * logp).sum(1), (q * perr).sum(1)
+    dz, dzerr = p - q, p * perr + 2.0**-22 * (p - q).abs()
+    dh, dh_tol = product(dz, dzerr, W)
+    dW, dW_tol = product((dz * up).t(), (dzerr * up).t(), h)
+    rounded = 2.0**-23
+    return ((loss, loss_tol), (dh * up, dh_tol * up + rounded * (dh * up).abs()),
+            (dW, dW_tol + rounded * dW.abs()))
+
+
+@pytest.mark.gpu
+def test_float32_accuracy(dev):
+    """Few terms a sum, so that a plane or a plane product left out would be seen (below)."""
+    h, W, t, up = _plane_case(dev)
+    L, DH, DW = _plane_reference(h, W, t, up)
+    h.requires_grad_(True)
+    frozen = head.linear_cross_entropy(h, W, t)
+    _close(frozen, L, "loss")
+    _close(torch.autograd.grad(frozen, [h], up)[0], DH, "hidden_grad of a frozen head")
+    W.requires_grad_(True)
+    loss = head.linear_cross_entropy(h, W, t)
+    dh, dW = torch.autograd.grad(loss, [h, W], up)
+    _close(loss, L, "loss")
+    _close(dh, DH, "hidden_grad")
+    _close(dW, DW, "weight_grad")
+
+
+def _with_planes(h, W, t, up, pairs):
+    """The loss and gradients with products over the given plane pairs only, in 64 bits."""
+    def product(x, y):
+        xp, yp = _planes(x, x.abs().max().item()), _planes(y, y.abs().max().item())
+        return sum(xp[a] @ yp[b] for a, b in pairs)
+
+    h, W, up = h.double(), W.double(), up.double()[:, None]
+    z = product(h, W.t())
+    logp = z - torch.logsumexp(z, 1, keepdim=True)
+    q = _onehot(t, W.shape[0], -100)
+    dz = logp.exp() - q
+    return -(q * logp).sum(1), product(dz, W) * up, product(dz.t(), h * up)
+
+
+def test_float32_bounds_tell_the_planes_apart():
+    case = _plane_case(torch.device("cpu"))
+    want = _plane_reference(*case)
+
+    def worst(pairs):
+        got = _with_planes(*case, pairs)
+        return [((g - v).abs() / tol).max().item() for g, (v, tol) in zip(got, want)]
+
+    assert max(worst([(1, 0), (0, 1), (0, 0)])) <= 1.0
+    for lost in ([(0, 0)], [(1, 0), (0, 0)], [(0, 1), (0, 0)]):
+        assert min(worst(lost)) > 1.0, lost
