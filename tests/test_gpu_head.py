@@ -662,3 +662,29 @@ def test_float32_bounds_tell_the_planes_apart():
     assert max(worst([(1, 0), (0, 1), (0, 0)])) <= 1.0
     for lost in ([(0, 0)], [(1, 0), (0, 0)], [(0, 1), (0, 0)]):
         assert min(worst(lost)) > 1.0, lost
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("path", ["frozen", "trained"])
+def test_small_exponentials_keep_their_bits(dev, path):
+    """Every half tile's largest column stands 15.6875 above the others (e^-15.6875 = 2.58
+    times 2^-24), whose probabilities alone make up one column of the hidden gradient.  An
+    exponential is off by 2^-11 of itself and 2^-39 of the largest (held without a power of
+    two it would be 3 or 2 times 2^-24), dz in bf16 by 2^-8, the gradient by its own
+    rounding."""
+    dtype = torch.bfloat16
+    N, D, V = 70, 8, 300
+    h = torch.zeros(N, D, device=dev, dtype=dtype)
+    h[:, 1] = 1.0
+    W = torch.zeros(V, D, device=dev, dtype=dtype)
+    W[:, 0], W[:, 1] = 1.0, -15.6875
+    W[::128] = 0.0
+    t = torch.zeros(N, dtype=torch.int64, device=dev)
+    h.requires_grad_(True)
+    W.requires_grad_(path == "trained")
+    (dh,) = torch.autograd.grad(head.linear_cross_entropy(h, W, t).sum(), [h])
+    tops = W[::128].shape[0]
+    low = math.exp(-15.6875)
+    want = (V - tops) * low / (tops + (V - tops) * low)
+    tol = 2.0**-39 / low + 2.0**-11 + 2 * 2.0**-8
+    assert ((dh[:, 0].double() - want).abs() <= tol * want).all()
