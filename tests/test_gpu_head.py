@@ -17,6 +17,7 @@ import math
 import pytest
 import torch
 
+from opake_amd import _native as nat
 from opake_amd import head
 from opake_amd.exceptions import ConfigurationError, InputTypeError
 
@@ -688,3 +689,44 @@ def test_small_exponentials_keep_their_bits(dev, path):
     want = (V - tops) * low / (tops + (V - tops) * low)
     tol = 2.0**-39 / low + 2.0**-11 + 2 * 2.0**-8
     assert ((dh[:, 0].double() - want).abs() <= tol * want).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("kept", [0.01, 0.6, 1.0])
+def test_chunks_and_pieces(dev, dtype, kept):
+    """A frozen head's forward in several chunks of rows and a trained head's backward in
+    several pieces of the vocabulary, with all rows, with so few that the last chunk holds
+    a part or nothing, and (1%) with dH's pieces in slices."""
+    N, D, V = 150_001, 8, 1900
+    lib, code = nat.load(), nat.dtype_code(dtype)
+    planes = 2 if dtype == torch.float32 else 1
+    rows = -(-N // 256) * 256
+    whole = planes * rows * -(-V // 256) * 512  # exponentials, or dz, of all
+    assert whole > 512 << 20
+    sizes = (N, D, V, 1, code)
+    exponentials = (lib.dpc_head_loss_workspace_bytes(*sizes, 1, 0)
+                    - lib.dpc_head_loss_workspace_bytes(*sizes, 1, 1))
+    assert 0 < exponentials < whole
+    assert lib.dpc_head_loss_state_bytes(*sizes, 1, 1) < whole
+    assert lib.dpc_head_loss_grad_workspace_bytes(*sizes, 1, 1) < whole
+    g, h, W, up = _inputs(dev, (N,), D, V, dtype, 61)
+    t = torch.randint(0, V, (N,), generator=g, device=dev)
+    t[torch.rand(N, generator=g, device=dev) >= kept] = -100
+    on = t != -100
+    L, DH, DW = _reference(h[on], W, _onehot(t[on], V, -100),
+                           torch.zeros(int(on.sum()), dtype=torch.float64, device=dev), 1.0,
+                           up[on], frozen=True)
+    h.requires_grad_(True)
+    frozen = head.linear_cross_entropy(h, W, t)
+    (dh,) = torch.autograd.grad(frozen, [h], up)
+    _close(frozen[on], L, "loss")
+    _close(dh[on], DH, "hidden_grad of a frozen head")
+    assert (frozen[~on] == 0).all() and (dh[~on] == 0).all()
+    W.requires_grad_(True)
+    loss = head.linear_cross_entropy(h, W, t)
+    dh, dW = torch.autograd.grad(loss, [h, W], up)
+    assert torch.equal(loss, frozen)
+    _close(dh[on], DH, "hidden_grad")
+    _close(dW, DW, "weight_grad")
+    assert (dh[~on] == 0).all()
