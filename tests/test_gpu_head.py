@@ -730,3 +730,66 @@ def test_chunks_and_pieces(dev, dtype, kept):
     _close(dh[on], DH, "hidden_grad")
     _close(dW, DW, "weight_grad")
     assert (dh[~on] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("N,D,V", [(5, 8, 1 << 19), (3, 1 << 20, 9), (130, 24, (1 << 17) + 3)])
+def test_the_largest_sizes(dev, N, D, V, dtype):
+    """The widest vocabulary and hidden state that are taken; one more of either is not."""
+    g, h, W, up = _inputs(dev, (N,), D, V, dtype, 71)
+    t = torch.randint(0, V, (N,), generator=g, device=dev)
+    t[0] = V - 1
+    q, zero = _onehot(t, V, -100), torch.zeros(N, dtype=torch.float64, device=dev)
+    L, DH, DW = _reference(h, W, q, zero, 1.0, up, frozen=True)
+    h.requires_grad_(True)
+    W.requires_grad_(True)
+    loss = head.linear_cross_entropy(h, W, t)
+    dh, dW = torch.autograd.grad(loss, [h, W], up)
+    _close(loss, L, "loss")
+    _close(dh, DH, "hidden_grad")
+    _close(dW, DW, "weight_grad")
+    frozen = head.linear_cross_entropy(h, W.detach(), t)
+    _close(torch.autograd.grad(frozen, [h], up)[0], DH, "hidden_grad of a frozen head")
+    for more in ((1, 8, (1 << 19) + 1), (1, (1 << 20) + 1, 2)):
+        with pytest.raises(ConfigurationError):
+            head.linear_cross_entropy(torch.zeros(1, more[1], device=dev, dtype=dtype),
+                                      torch.zeros(more[2], more[1], device=dev, dtype=dtype),
+                                      torch.zeros(1, dtype=torch.int64, device=dev))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("N,D,V", [(40, 64, 300), (300, 1544, 513), (700, 100, 3001)])
+def test_no_token_has_a_target(dev, N, D, V, dtype):
+    """Losses and both gradients are zeros, whatever the rows hold."""
+    _, h, W, up = _inputs(dev, (N,), D, V, dtype, 72)
+    h[::2] = math.nan
+    t = torch.full((N,), -100, device=dev)
+    h.requires_grad_(True)
+    for w in (W, W.clone().requires_grad_(True)):
+        for loss in (head.linear_cross_entropy(h, w, t),
+                     head.topk_distillation(h, w, torch.zeros(N, 3, device=dev),
+                                            torch.full((N, 3), -1, device=dev))):
+            assert (loss == 0).all()
+            grads = torch.autograd.grad(loss, [h, w] if w.requires_grad else [h], up)
+            assert all((x == 0).all() for x in grads)
+
+
+@pytest.mark.gpu
+def test_thousands_of_teacher_entries(dev):
+    N, D, V, K, tau = 19, 64, 9000, 3001, 2.0
+    g, h, W, up = _inputs(dev, (N,), D, V, torch.bfloat16, 73)
+    tl = torch.randn(N, K, generator=g, device=dev) * 2
+    ti = torch.randint(0, V, (N, K), generator=g, device=dev)  # some of them repeated
+    ti[:, ::7] = -1
+    ti[3, 1:] = -1
+    h.requires_grad_(True)
+    W.requires_grad_(True)
+    loss = head.topk_distillation(h, W, tl, ti, temperature=tau)
+    dh, dW = torch.autograd.grad(loss, [h, W], up)
+    q, ent = _soft(tl, ti, V, tau)
+    L, DH, DW = _reference(h, W, q, ent, tau, up, frozen=True)
+    _close(loss, L, "loss")
+    _close(dh, DH, "hidden_grad")
+    _close(dW, DW, "weight_grad")

@@ -186,3 +186,37 @@ def test_nan_logits_reach_the_output(dev):
         y = m(x, logits)
         assert torch.isnan(y[bad]).all()
         torch.testing.assert_close(y[~bad], want[~bad], rtol=1e-5, atol=1e-6)
+
+
+def test_bfloat16(dev):
+    """Every expert chosen, so that no rounding can change a choice.  About twenty roundings
+    to 2^-8 (2^-9 on average) forward and back, half of them along one path: 8%."""
+    torch.manual_seed(5)
+    kw = dict(routing=dict(score="sigmoid", scale=1.5), temperature=2.0)
+    ref = RoutedLM(V, D, HEADS, FFN, INTER, 4, 4, dtype=torch.float64, **kw)
+    with torch.no_grad():
+        for p in ref.parameters():
+            p.normal_(0.0, 0.25)
+            p.copy_(p.bfloat16().double())
+    _, ids, tgt, teacher, index = _case(3, 20, seed=8)
+    model = RoutedLM(V, D, HEADS, FFN, INTER, 4, 4, dtype=torch.bfloat16, **kw).to(dev)
+    model.load_state_dict(ref.state_dict())
+
+    def route(x, router_logits=None):
+        score = torch.sigmoid(ref.moe.router(x))
+        every = torch.arange(4).expand(score.shape)
+        return every, 1.5 * score / score.sum(-1, keepdim=True)
+
+    ref.moe.route = route
+    per = ghost_oracle.per_example_grads_loop(ref, _plain_loss(ref), (ids, teacher, index), tgt)
+    names = sorted(n for n, p in model.named_parameters() if p.requires_grad)
+    want = clip_oracle.stream_clip_and_sum([per[n].float() for n in names],
+                                           clip_oracle.conservative_bound(0.45),
+                                           return_aux=True)
+    fn, st = ghost_clipped_grad(model, model.loss, clipping_norm=0.45, return_aux=True)
+    (out, aux), _ = fn(tuple(t.to(dev) for t in (ids, teacher, index)), tgt.to(dev), state=st)
+    torch.testing.assert_close(aux.grad_norms.cpu().double(), want.norms.double(), rtol=0.08,
+                               atol=0)
+    for i, n in enumerate(names):
+        got, exp = out.pytree[n].double().cpu(), want.reduced[i].double()
+        assert ((got - exp).norm() / exp.norm()).item() < 0.08, n
