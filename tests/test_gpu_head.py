@@ -793,3 +793,22 @@ def test_thousands_of_teacher_entries(dev):
     _close(loss, L, "loss")
     _close(dh, DH, "hidden_grad")
     _close(dW, DW, "weight_grad")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [1, 64])
+def test_bfloat16_gradients_in_norm(dev, K):
+    """dz's rounding to bf16 and the gradient's own, independent and at most 2^-8 / sqrt(3)
+    each in the mean square: 0.82 times 2^-8 together, and fp16 exponentials add 2^-11."""
+    N, D, V, tau = 400, 256, 3000, 1.5
+    g, h, W, up = _inputs(dev, (N,), D, V, torch.bfloat16, 81)
+    tl, ti = _teacher(g, dev, (N,), V, K)
+    q, ent = _soft(tl, ti, V, tau)
+    _, (DH, _), (DW, _) = _reference(h, W, q, ent, tau, up)
+    h.requires_grad_(True)
+    for trained in (False, True):
+        W.requires_grad_(trained)
+        loss = head.topk_distillation(h, W, tl, ti, temperature=tau)
+        grads = torch.autograd.grad(loss, [h, W] if trained else [h], up)
+        for got, want in zip(grads, (DH, DW)):
+            assert (got.double() - want).norm() <= 2.0**-8 * want.norm()
