@@ -107,6 +107,8 @@ DPC_DEVICE float row_sum(float x) {
   return __uint_as_float(row_all<kLanes>(__float_as_uint(x), AddF()));
 }
 
+// exp2's argument is rounded once, which makes |x| 2^-24 of the result: a score is held in
+// 32 bits and within 2^-20 (1 + |x|) of itself, as the choice and the weights need it.
 constexpr float kLog2e = 1.44269504088896340736f;
 DPC_DEVICE float fast_exp(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 // (The hardware's reciprocal, 1 ulp; of infinity 0.)
@@ -550,6 +552,11 @@ extern "C" int dpc_route_topk(const void* logits, int64_t N, int E, int dtype, c
   const RouteArgs a = {logits, N, E, dtype, bias, k, score == DPC_ROUTE_SIGMOID, groups, top_groups,
                        renormalize != 0, (float)scale, weights, experts};
   hipStream_t s = (hipStream_t)stream;
+  // As few lanes a row as hold its k slots, and its experts in 2 to 16 registers: 65536
+  // tokens of 8 experts take 3.2 us in 4 lanes and 7.3 in 16, of 64 experts 14 in 16 and 56
+  // in 64.  Up to 256 experts 16 lanes of 16 pay once there are tokens for them all (the
+  // best 8 of 256: 6.4 us against 4.7 in 64 lanes at 2048 tokens, 6.5 against 6.4 at 4096,
+  // 7.2 against 9.8 at 8192; k = 1 turns near 8192, k = 16 near 3500).
   if (k <= 4 && E <= 8) return launch_route<4, 2>(a, by_two, s);
   if (k <= 16 && E <= 64) return launch_route<16, 4>(a, by_two, s);
   if (k <= 16 && E <= 256 && N >= 4096) return launch_route<16, 16>(a, by_two, s);
@@ -569,6 +576,10 @@ extern "C" int dpc_route_topk_grad(const void* logits, int64_t N, int E, int dty
                            (float)scale, experts, weights, grad_weights, grad_logits};
   if ((reinterpret_cast<uintptr_t>(grad_logits) & 15) != 0) return DPC_EINVAL;
   hipStream_t s = (hipStream_t)stream;
+  // Lanes a row by its slots, in both.  Dense, 65536 tokens: of 8 experts 6.7 us in 16 lanes
+  // and 21 in 64, of 256 49 and 53 (16 tokens of 256: 10 and 4).  Sparse: 16384 tokens of 8
+  // experts, k = 2, 4.4 us in 4 lanes and 12 in 16; 65536 of 256, k = 8, 13 in 16 and 18 in
+  // 64.
   if (!a.sigmoid && !a.renormalize) {
     if (k <= 16)
       hipLaunchKernelGGL((route_dense_grad_kernel<16>), dim3((unsigned)((N + 15) / 16)), dim3(256),

@@ -135,7 +135,8 @@ def topk_distillation(hidden: torch.Tensor, weight: torch.Tensor, teacher_logits
     An entry whose index is negative is absent, so rows may hold fewer than K;
     a token with none left has loss 0 and no part in any gradient.  The factor
     ``temperature^2`` keeps the gradient's size when the temperature changes.
-    No gradient reaches the teacher."""
+    No gradient reaches the teacher.  Entries of a row are compared pair by pair: a few
+    thousand of them cost more than the products do."""
     nat.require_device(hidden, weight, teacher_logits, teacher_indices)
     code = _check_head(hidden, weight)
     _integer(teacher_indices, "teacher_indices")
