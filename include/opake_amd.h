@@ -598,6 +598,52 @@ int dpc_route_topk_grad(const void* logits, int64_t N, int E, int dtype, int k, 
                         const float* weights, const float* grad_weights, void* grad_logits,
                         void* stream);
 
+/* ------------------------------------------------------------------------
+ * Rotary positions (no reference counterpart: its models' own code rotates).
+ *
+ * q [B, T, H, h] and k [B, T, KV, h] (KV 0: none) in `dtype` (bf16 or fp32); strides
+ * (host): q's of B, T and heads, then k's, in elements; a head's h elements are side by
+ * side.  Pair i < pairs of a head is elements i and pairs + i, or with `interleaved`
+ * 2 i and 2 i + 1; it turns by position * freqs[i] (float64, radians; `inverse`: by the
+ * negative) and is multiplied by `amplitude`.  Elements from 2 pairs on are copied.
+ * positions[b * pos_stride_b + t * pos_stride_t], or t where NULL.  q_out and k_out are
+ * contiguous and do not overlap the inputs.  h <= 2048, (H + KV) h <= 2^22.
+ * -------------------------------------------------------------------------*/
+int dpc_rotary(const void* q, const void* k, int64_t B, int64_t T, int H, int KV, int h, int dtype,
+               const int64_t* strides, const int64_t* positions, int64_t pos_stride_b,
+               int64_t pos_stride_t, const double* freqs, int pairs, int interleaved,
+               double amplitude, int inverse, void* q_out, void* k_out, void* stream);
+
+/* ------------------------------------------------------------------------
+ * A gated feed-forward layer's projections, activation and product (the reference's
+ * experts form them one after the other, packages/opake-patches/src/opake/api/patches/
+ * kernels/moe.py:74-103).
+ *
+ * x [N, D], w [2 F, D] (F gate rows, then F up rows) in `dtype` (bf16 or fp32), all
+ * operands 16-byte aligned and contiguous, the workspace 256-byte aligned:
+ *   z = x w^T = [g, u] [N, 2 F],  h [N, F] = act(g) u
+ * with act DPC_ACT_SILU (g / (1 + exp(-g))) or DPC_ACT_GELU (g times the normal
+ * distribution function).  h is rounded once from float32; z, if not NULL, is written in
+ * `dtype` for dpc_gated_linear_act_grad, which makes dz [N, 2 F] of it and dh [N, F].
+ * dpc_gated_linear_grad takes dz to dx [N, D] = dz w and dw [2 F, D] =
+ * dz^T x (either may be NULL; x is not read without dw, w not without dx).
+ *
+ * Sums are float32; float32 operands are multiplied as two fp16 planes each: at most
+ * 2^-23 of a value (and 2^-39 of the largest of its row of x or dz, or of w) away from it,
+ * without the product of the two low ones (at most 2^-22 of the product).  All results
+ * are deterministic.  N <= 2^30, D <= 2^20, F <= 2^19.
+ * -------------------------------------------------------------------------*/
+enum { DPC_ACT_SILU = 0, DPC_ACT_GELU = 1 };
+size_t dpc_gated_linear_workspace_bytes(int64_t N, int D, int F, int dtype);
+int dpc_gated_linear(const void* x, const void* w, int64_t N, int D, int F, int dtype,
+                     int activation, void* h, void* z, void* ws, size_t ws_bytes, void* stream);
+int dpc_gated_linear_act_grad(const void* z, const void* dh, int64_t N, int F, int dtype,
+                              int activation, void* dz, void* stream);
+size_t dpc_gated_linear_grad_workspace_bytes(int64_t N, int D, int F, int dtype, int want_x,
+                                             int want_w);
+int dpc_gated_linear_grad(const void* x, const void* w, const void* dz, int64_t N, int D, int F,
+                          int dtype, void* dx, void* dw, void* ws, size_t ws_bytes, void* stream);
+
 /* Measurement helper with no counterpart in the reference (used by bench.py
  * to put the roofline in context): `grid` workgroups of 8 waves run `iters`
  * rounds of 8 independent 32x32x16 bf16 MFMAs on operands taken from

@@ -34,6 +34,8 @@ SCALE_AUTO_S = 1
 ROUTE_SOFTMAX = 0
 ROUTE_SIGMOID = 1
 ROUTE_GROUPS_BY_TWO = 2
+ACT_SILU = 0
+ACT_GELU = 1
 NOISE_NONE = 0
 NOISE_INJECTED = 1
 NOISE_PHILOX = 2
@@ -198,6 +200,27 @@ SIGNATURES = {
         _c_int,
         [_c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_double, _c_void_p,
          _c_void_p, _c_void_p, _c_void_p, _c_void_p],
+    ),
+    "dpc_rotary": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_i64, _c_i64] + [_c_int] * 4 + [_c_void_p, _c_void_p, _c_i64,
+         _c_i64, _c_void_p, _c_int, _c_int, _c_double, _c_int, _c_void_p, _c_void_p, _c_void_p],
+    ),
+    "dpc_gated_linear_workspace_bytes": (_c_size_t, [_c_i64] + [_c_int] * 3),
+    "dpc_gated_linear": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_i64] + [_c_int] * 4 + [_c_void_p, _c_void_p, _c_void_p,
+         _c_size_t, _c_void_p],
+    ),
+    "dpc_gated_linear_act_grad": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
+    ),
+    "dpc_gated_linear_grad_workspace_bytes": (_c_size_t, [_c_i64] + [_c_int] * 5),
+    "dpc_gated_linear_grad": (
+        _c_int,
+        [_c_void_p, _c_void_p, _c_void_p, _c_i64] + [_c_int] * 3 + [_c_void_p, _c_void_p,
+         _c_void_p, _c_size_t, _c_void_p],
     ),
     "dpc_head_loss_state_bytes": (_c_size_t, [_c_i64] + [_c_int] * 6),
     "dpc_head_loss_workspace_bytes": (_c_size_t, [_c_i64] + [_c_int] * 6),

@@ -96,7 +96,10 @@ constexpr int64_t kMmBlock = kMmTile * kMmStep;  // elements
 // reads, which take 4 rows x 16 columns, slot l ^ 4 (l / 16) holds lane l's 16 bytes.
 DPC_DEVICE int mm_native_slot(int row, int q) { return (row ^ (4 * q)) + 16 * q; }
 
-template <bool kKc, bool kNative>
+// kPaired (K-contiguous): a tile is 128 rows of the matrix's first half and the same of
+// its second, `rows` further on, by 64 in turn: a wave's 128 rows hold both of 64 pairs.
+// (The 64 rows of transfer j are of the first half where j is even.)
+template <bool kKc, bool kNative, bool kPaired = false>
 struct MmStage {
   int voff[4];  // byte offsets of this lane's four 16-byte chunks of a step
   int kchunk;   // K-contiguous: first k of the lane's chunk
@@ -113,7 +116,8 @@ struct MmStage {
       } else if (kKc) {
         const int row = 8 * (w + 8 * j) + (lane >> 3);
         kchunk = ((lane & 7) ^ ((row >> 1) & 7)) * 8;
-        voff[j] = (int)((row * o.ld + kchunk) * 2);
+        const int from = kPaired ? (row >> 7) * 64 + (row & 63) : row;
+        voff[j] = (int)((from * o.ld + kchunk) * 2);
       } else {
         const int row = 2 * (w + 8 * j) + (lane >> 5);
         voff[j] = (int)((row * o.ld + tile_slot_col(row, lane & 31)) * 2);
@@ -124,11 +128,14 @@ struct MmStage {
   // buffer's range for lanes whose k is past kl.  Rows past the operand's are out of
   // range too: all such reads give zeros.  (Native blocks are whole; past their matrix
   // they hold zeros.)
-  DPC_DEVICE u32x4_t buffer(const MmOperand& o, int pl, int t, int k0, int kl, int* bad) const {
+  // kPaired: of the matrix's half `half`.
+  DPC_DEVICE u32x4_t buffer(const MmOperand& o, int pl, int t, int k0, int kl, int* bad,
+                            int half = 0) const {
     const uint16_t* base = o.p + (int64_t)pl * o.plane;
     uint32_t bytes;
     *bad = 0;
-    const int i0 = t * kMmTile;
+    constexpr int kRows = kPaired ? kMmTile / 2 : kMmTile;
+    const int i0 = t * kRows;
     if (kNative && kKc) {
       base += (t * o.ld + (k0 >> 6)) * kMmBlock;
       bytes = kMmBlock * 2;
@@ -136,8 +143,8 @@ struct MmStage {
       base += ((k0 >> 8) * o.ld + 4 * t) * kMmBlock + ((k0 & 255) >> 4) * 512;
       bytes = (uint32_t)(4 * kMmBlock * 2 - ((k0 & 255) >> 4) * 1024);
     } else if (kKc) {
-      base += (int64_t)i0 * o.ld + k0;
-      bytes = (uint32_t)((min(o.rows - i0, kMmTile) * o.ld - k0) * 2);
+      base += (int64_t)(kPaired ? half * o.rows + i0 : i0) * o.ld + k0;
+      bytes = (uint32_t)((min(o.rows - i0, kRows) * o.ld - k0) * 2);
       *bad = k0 + kchunk >= kl ? kMmOutOfRange : 0;
     } else {
       base += (int64_t)k0 * o.ld + i0;
@@ -153,11 +160,11 @@ struct MmStage {
 // Reads the 16 x 32 fragments of a wave's blocks from an operand's tile.  Both of a
 // product's operands give the k-slots one order: by rows (K-contiguous), or that of the
 // transposing reads (frag16_off: slot 8 q + 4 h + e is k = 16 h + 4 q + e), which a native
-// piece has too.  A lane keeps a few byte offsets; blocks, sub-steps and stages are
-// added as immediates.
-template <bool kKc, bool kNative, int kBlocks>
+// piece has too, and rows with kSlow (two 8-byte reads).  A lane keeps a few byte offsets;
+// blocks, sub-steps and stages are added as immediates.
+template <bool kKc, bool kNative, int kBlocks, bool kSlow = false>
 struct MmFrags {
-  static constexpr int kOffsets = kNative ? 1 : kKc ? 2 : kBlocks / 2;
+  static constexpr int kOffsets = kNative ? 1 : kKc ? (kSlow ? 4 : 2) : kBlocks / 2;
   int o[kOffsets];
   // Tile at byte `at` of the workgroup's LDS, first block at index c0.
   DPC_DEVICE void init(int at, int c0, int lane) {
@@ -170,6 +177,8 @@ struct MmFrags {
         o[i] = at + (c0 >> 5) * 4096 + mm_native_slot(4 * q + ((lane & 15) >> 2), lane & 3) * 16;
       else if (!kKc)
         o[i] = at + frag16_off(c0 + 32 * i, 0, lane);
+      else if (kSlow)  // sub-step i / 2, half i % 2: k = 16 (i % 2) + 4 q ..
+        o[i] = at + mm_kc_off(row, 2 * i + (q >> 1)) + 8 * (q & 1);
       else
         o[i] = at + mm_kc_off(row, 4 * i + q);
     }
@@ -185,6 +194,11 @@ struct MmFrags {
     if (!kKc) {  // odd blocks are the other half of a 64-byte LDS block
       const int p = (o[i >> 1] ^ (32 * (i & 1))) + off + kk * 32 * kTileRowBytes;
       return join_frag(read_tr(lds, p), read_tr(lds, p + 16 * kTileRowBytes));
+    }
+    if constexpr (kSlow) {
+      const int p = off + i * 2048;
+      return join_frag(*reinterpret_cast<const i16x4_t*>(lds + o[2 * kk] + p),
+                       *reinterpret_cast<const i16x4_t*>(lds + o[2 * kk + 1] + p));
     }
     return *reinterpret_cast<const bf16x8_t*>(lds + o[kk] + off + i * 2048);
   }
@@ -228,15 +242,18 @@ struct MmPlace {
 // begin() sends the first transfers, run() does the rest and ends with a barrier,
 // after which `lds` is free: the next tile's begin() goes before this one's epilogue,
 // so that its first step has arrived when the epilogue ends.
-template <bool kAKc, bool kBKc, bool kBNative, bool kWideB, bool kHalf>
+// kPaired: A in pairs (MmStage).  kBSlow: a K-contiguous B beside a K-slow A, whose `rows`
+// are then the k that it has (B is zero beyond).
+template <bool kAKc, bool kBKc, bool kBNative, bool kWideB, bool kHalf, bool kPaired = false,
+          bool kBSlow = false>
 struct MmTile {
   const MmArgs& g;
   uint8_t* lds;
   int lane, w, ta, tb, steps;
   MmPlace<kHalf> pa, pb;
-  MmStage<kAKc, false> sa;
+  MmStage<kAKc, false, kPaired> sa;
   MmStage<kBKc, kBNative> sb;
-  u32x4_t buf;
+  u32x4_t buf, buf2;
   int bad;
 
   DPC_DEVICE MmTile(const MmArgs& args, uint8_t* l) : g(args), lds(l) {
@@ -246,7 +263,10 @@ struct MmTile {
     sb.init(g.b, w, lane);
   }
   DPC_DEVICE void next_a() {
-    buf = sa.buffer(g.a, kHalf ? (kMmPairsA >> (4 * pa.pair)) & 15 : 0, ta, pa.k0, g.kl, &bad);
+    const int plane = kHalf ? (kMmPairsA >> (4 * pa.pair)) & 15 : 0;
+    const int kl = kBSlow ? g.a.rows : g.kl;
+    buf = sa.buffer(g.a, plane, ta, pa.k0, kl, &bad);
+    if constexpr (kPaired) buf2 = sa.buffer(g.a, plane, ta, pa.k0, kl, &bad, 1);
     pa = pa.next();
   }
   DPC_DEVICE void next_b() {
@@ -254,7 +274,7 @@ struct MmTile {
     pb = pb.next();
   }
   DPC_DEVICE void fetch_a(int stage, int j) {
-    sa.issue(buf, bad, lds_addr(lds) + stage * kMmOperandBytes, w, j);
+    sa.issue(kPaired && (j & 1) ? buf2 : buf, bad, lds_addr(lds) + stage * kMmOperandBytes, w, j);
   }
   DPC_DEVICE void fetch_b(int stage, int j) {
     sb.issue(buf, bad, lds_addr(lds) + (2 + stage) * kMmOperandBytes, w, j);
@@ -298,11 +318,11 @@ struct MmTile {
 #pragma unroll
       for (int j = 0; j < MmAcc<kWideB>::kB; ++j) acc.v[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     if (steps <= 0) return;
-    static_assert(kAKc == (kBKc && !kBNative), "one order of the k-slots");
+    static_assert(kAKc == (kBKc && !kBNative && !kBSlow), "one order of the k-slots");
     // x: the wide operand's fragments (half of its blocks), y: the narrow one's.
     bf16x8_t x0[4], x1[4], y0[4], y1[4];
     MmFrags<kAKc, false, MmAcc<kWideB>::kA> ra;
-    MmFrags<kBKc, kBNative, MmAcc<kWideB>::kB> rb;
+    MmFrags<kBKc, kBNative, MmAcc<kWideB>::kB, kBSlow> rb;
     ra.init(0, acc.row0(w), lane);
     rb.init(2 * kMmOperandBytes, acc.col0(w), lane);
     auto read_x = [&](int stage, int kk, int half, bf16x8_t* f, int i)
