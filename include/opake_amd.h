@@ -644,6 +644,47 @@ size_t dpc_gated_linear_grad_workspace_bytes(int64_t N, int D, int F, int dtype,
 int dpc_gated_linear_grad(const void* x, const void* w, const void* dz, int64_t N, int D, int F,
                           int dtype, void* dx, void* dw, void* ws, size_t ws_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Softmax attention with shared key heads, and its gradients (no reference counterpart:
+ * its models call their framework's).
+ *
+ * q [B, T, H, h]; k and v [B, S, KV, h] in `dtype` (bf16 or fp32), H a multiple of KV:
+ * query head i uses key head i KV / H.  strides (host): of B, tokens and heads, for q, k
+ * and v (dpc_attention_grad: and dout), in elements; a head's h elements are side by
+ * side, and rows, strides and operands are multiples of 16 bytes.  out [B, T, H, h] and
+ * the gradients are contiguous.
+ *   out_i = sum_j softmax_j(scale q_i . k_j) v_j  over the keys j that i sees
+ * Example b has lengths[b] keys (NULL: S; clamped to 0 .. S).  Without `causal` every
+ * query sees them all.  With it, token t is at position starts[b] + t (NULL: S - T + t)
+ * and sees the keys up to it, or with window > 0 the last `window` of those; positions
+ * below 0 or from lengths[b] on are padding.  Queries that see nothing have output 0 and no
+ * part in any gradient; what lies in keys, values and queries that are padding reaches
+ * nothing, whatever it is.  scale > 0.
+ *
+ * lse [B, KV, T, H / KV] (float32, may be NULL in the forward) holds log2 of each row's
+ * sum of exponentials (+inf: sees nothing) for dpc_attention_grad, which takes out, lse
+ * and dout, the output's gradient, and writes dq [B, T, H, h], dk and dv [B, S, KV, h]
+ * (both or neither).
+ * Probabilities are formed again; nothing of size [T, S] is kept.  Sums and statistics are
+ * float32; bf16 products take probabilities and their gradients in bf16.  All results are
+ * deterministic.  h <= 256, a multiple of 16 bytes; T, S <= 2^24.  A tensor whose 65
+ * tokens and H / KV heads span 2 GiB or more is refused (DPC_ENOTSUP).  Workspaces are
+ * 256-byte aligned.
+ * -------------------------------------------------------------------------*/
+size_t dpc_attention_workspace_bytes(int64_t B, int64_t T, int64_t S, int H, int KV, int h,
+                                     int dtype);
+int dpc_attention(const void* q, const void* k, const void* v, const int64_t* strides, int64_t B,
+                  int64_t T, int64_t S, int H, int KV, int h, int dtype, const int64_t* lengths,
+                  const int64_t* starts, int causal, int window, double scale, void* out,
+                  float* lse, void* ws, size_t ws_bytes, void* stream);
+size_t dpc_attention_grad_workspace_bytes(int64_t B, int64_t T, int H);
+int dpc_attention_grad(const void* q, const void* k, const void* v, const void* out,
+                       const void* dout, const int64_t* strides, int64_t B, int64_t T, int64_t S,
+                       int H, int KV, int h, int dtype, const int64_t* lengths,
+                       const int64_t* starts, int causal, int window, double scale,
+                       const float* lse, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes,
+                       void* stream);
+
 /* Measurement helper with no counterpart in the reference (used by bench.py
  * to put the roofline in context): `grid` workgroups of 8 waves run `iters`
  * rounds of 8 independent 32x32x16 bf16 MFMAs on operands taken from

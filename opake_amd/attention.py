@@ -1,0 +1,161 @@
+"""Softmax attention that keeps nothing of size [queries, keys], with its gradients.
+
+``attention`` takes queries, keys and values as the projections leave them ([B, T, heads,
+h], any strides: places of a fused projection go in as they are), shares key heads among
+groups of query heads, and masks by what a query sees: causal, a window, each example's
+length and the position of its first query.  The forward keeps one number a query for the
+backward, which forms the probabilities again (``csrc/attention.hip``).  Results do not depend
+on anything but the inputs: no sums whose order changes.
+"""
+
+from __future__ import annotations
+
+import math
+
+import torch
+import torch.nn.functional as F
+
+from opake_amd import _native as nat
+from opake_amd._autograd import check_leaves, note_leaves
+from opake_amd.exceptions import ConfigurationError, InputTypeError
+
+MAX_HEAD = 256
+MAX_HEADS = 1 << 16
+MAX_TOKENS = 1 << 24
+_MOST_BYTES = 0x7ff00000 - (1 << 20)
+
+
+def _rows(t: torch.Tensor, rep: int = 1) -> torch.Tensor:
+    """Rows of whole 16-byte chunks, and tiles of 65 tokens within a buffer's range."""
+    size = t.element_size()
+    b, n, head, last = t.stride()
+    if (last == 1 and t.data_ptr() % 16 == 0 and b * size % 16 == 0 and n * size % 16 == 0
+            and head * size % 16 == 0 and (65 * n + rep * head) * size <= _MOST_BYTES):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _call(name, dev, tensors, strides, sizes, lengths, starts, options, *rest):
+    causal, window, scale = options
+    nat.call_on(dev, name, *(t.data_ptr() for t in tensors),
+                (nat._c_i64 * len(strides))(*strides), *sizes,
+                0 if lengths is None else lengths.data_ptr(),
+                0 if starts is None else starts.data_ptr(), causal, window, scale, *rest)
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lengths, starts, code, options, grad_enabled):
+        dev = q.device
+        B, T, H, h = q.shape
+        S, KV = k.shape[1:3]
+        qr, kr, vr = _rows(q, H // KV), _rows(k), _rows(v)
+        sizes = (B, T, S, H, KV, h, code)
+        out = torch.empty((B, T, H, h), dtype=q.dtype, device=dev)
+        lse = None
+        # needs_input_grad is true of a parameter under no_grad too.
+        if grad_enabled and any(ctx.needs_input_grad[:3]):
+            note_leaves(ctx)
+            lse = torch.empty((B, KV, T, H // KV), dtype=torch.float32, device=dev)
+            ctx.save_for_backward(q, k, v, out, lse, lengths, starts)
+            ctx.sizes, ctx.options = sizes, options
+        ws_bytes = nat.load().dpc_attention_workspace_bytes(*sizes)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        _call("dpc_attention", dev, (qr, kr, vr),
+              (*qr.stride()[:3], *kr.stride()[:3], *vr.stride()[:3]), sizes, lengths, starts,
+              options, out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws.data_ptr(),
+              ws_bytes)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        check_leaves(ctx)
+        q, k, v, out, lse, lengths, starts = ctx.saved_tensors
+        dev, sizes = q.device, ctx.sizes
+        B, T, S, H, KV, h, _ = sizes
+        rep = H // KV
+        qr, kr, vr, gr = _rows(q, rep), _rows(k), _rows(v), _rows(grad, rep)
+        dq = torch.empty((B, T, H, h), dtype=q.dtype, device=dev)
+        dk = dv = None
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            dk, dv = (torch.empty((B, S, KV, h), dtype=q.dtype, device=dev) for _ in range(2))
+        ws_bytes = nat.load().dpc_attention_grad_workspace_bytes(B, T, H)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        _call("dpc_attention_grad", dev, (qr, kr, vr, out, gr),
+              (*qr.stride()[:3], *kr.stride()[:3], *vr.stride()[:3], *gr.stride()[:3]), sizes,
+              lengths, starts, ctx.options, lse.data_ptr(), dq.data_ptr(),
+              *(0 if t is None else t.data_ptr() for t in (dk, dv)), ws.data_ptr(), ws_bytes)
+        return dq, dk, dv, None, None, None, None, None
+
+
+def _whole(t, name: str, B: int):
+    if t is None:
+        return None
+    if t.dtype not in (torch.int64, torch.int32):
+        raise InputTypeError(f"{name} must be int64 or int32, got {t.dtype}")
+    if tuple(t.shape) != (B,):
+        raise ConfigurationError(f"{name} must be [{B}], got {tuple(t.shape)}")
+    return t.detach().to(torch.int64).contiguous()
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = True,
+              window: int | None = None, lengths: torch.Tensor | None = None,
+              starts: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    """``softmax(scale q k^T) v`` of every head over the keys a query sees: [B, T, H, h].
+
+    ``q`` [B, T, H, h], ``k`` and ``v`` [B, S, KV, h] (bfloat16 or float32, any strides);
+    query heads share key heads in consecutive groups of H / KV.  ``lengths`` (integers
+    [B]): example b has that many keys, those behind are padding (all S by default).  Not
+    ``causal``: a query sees them all.  ``causal``: token t of example b is at position
+    ``starts[b] + t`` (integers; S - T + t by default, so the last query sees the last
+    key) and sees the keys up to its own position, with ``window`` the last ``window`` of
+    them; a token at a position below 0 or not below the length is padding.  ``scale``:
+    positive, 1 / sqrt(h) by default.
+
+    A query that sees no key has output 0 and no part in any gradient.  What padding holds
+    reaches nothing; what a token holds reaches its own example's head group alone, but there a
+    value that is not finite may reach queries that do not see it.  Gradients reach ``q``,
+    ``k`` and ``v``.  For one token of each of several sequences: T = 1, keys and values
+    the caches [B, S, KV, h], ``lengths`` the sequences' and ``starts`` one less."""
+    nat.require_device(q, k, v, lengths, starts)
+    if (q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0]
+            or q.shape[3] != k.shape[3]):
+        raise ConfigurationError(
+            f"expected q [B, T, H, h], k and v [B, S, KV, h], got {tuple(q.shape)}, "
+            f"{tuple(k.shape)} and {tuple(v.shape)}")
+    if q.dtype != k.dtype or q.dtype != v.dtype:
+        raise ConfigurationError(
+            f"q, k and v must share a dtype, got {q.dtype}, {k.dtype} and {v.dtype}")
+    code = nat.dtype_code(q.dtype)
+    B, T, H, h = q.shape
+    S, KV = k.shape[1:3]
+    if not 1 <= h <= MAX_HEAD or KV < 1 or not 1 <= H <= MAX_HEADS or H % KV:
+        raise ConfigurationError(
+            f"heads must be 1 to {MAX_HEAD} wide and query heads (at most {MAX_HEADS}) a "
+            f"multiple of key heads, got {H} and {KV} of {h}")
+    if T > MAX_TOKENS or S > MAX_TOKENS:
+        raise ConfigurationError(f"at most {MAX_TOKENS} tokens, got {T} and {S}")
+    if window is not None:
+        if isinstance(window, bool) or not isinstance(window, int):
+            raise InputTypeError(f"window must be an int, got {type(window)}")
+        if not causal or window < 1:
+            raise ConfigurationError(f"a window is causal and at least 1, got {window}")
+    if starts is not None and not causal:
+        raise ConfigurationError("starts are for causal attention")
+    if scale is None:
+        scale = 1.0 / math.sqrt(h)
+    elif isinstance(scale, bool) or not isinstance(scale, (int, float)):
+        raise InputTypeError(f"scale must be a number, got {type(scale)}")
+    if not 1e-30 < scale < 1e30:
+        raise ConfigurationError(f"scale must be between 1e-30 and 1e30, got {scale}")
+    options = (int(bool(causal)), min(window or 0, MAX_TOKENS), float(scale))
+    odd = -h % (4 if q.dtype == torch.float32 else 8)
+    if odd:  # zeros add nothing to a score, and come out as zeros
+        q, k, v = (F.pad(t, (0, odd)) for t in (q, k, v))
+    out = _Attention.apply(q, k, v, _whole(lengths, "lengths", B), _whole(starts, "starts", B),
+                           code, options, torch.is_grad_enabled())
+    return out[..., :h] if odd else out
+
+
+__all__ = ["attention"]
