@@ -661,29 +661,31 @@ int dpc_gated_linear_grad(const void* x, const void* w, const void* dz, int64_t 
  * part in any gradient; what lies in keys, values and queries that are padding reaches
  * nothing, whatever it is.  scale > 0.
  *
- * lse [B, KV, T, H / KV] (float32, may be NULL in the forward) holds log2 of each row's
- * sum of exponentials (+inf: sees nothing) for dpc_attention_grad, which takes out, lse
- * and dout, the output's gradient, and writes dq [B, T, H, h], dk and dv [B, S, KV, h]
- * (both or neither).
+ * state (dpc_attention_state_bytes, 256-byte aligned; NULL without a gradient) keeps each
+ * row's statistics and, for bf16, what rounding took from out, for dpc_attention_grad,
+ * which takes out, state and dout, the output's gradient, and writes dq [B, T, H, h], dk and
+ * dv [B, S, KV, h] (both or neither).  state is not changed.
  * Probabilities are formed again; nothing of size [T, S] is kept.  Sums and statistics are
  * float32; bf16 products take probabilities and their gradients in bf16.  All results are
- * deterministic.  h <= 256, a multiple of 16 bytes; T, S <= 2^24.  A tensor whose 65
- * tokens and H / KV heads span 2 GiB or more is refused (DPC_ENOTSUP).  Workspaces are
- * 256-byte aligned.
+ * deterministic.  h <= 256, a multiple of 16 bytes; T, S <= 2^24, T H / KV <= 2^30.  A
+ * tensor whose 65 tokens and H / KV heads span 2 GiB or more is refused (DPC_ENOTSUP), and
+ * so are keys or values whose tokens overlap (a stride below h).  Workspaces are 256-byte
+ * aligned.
  * -------------------------------------------------------------------------*/
 size_t dpc_attention_workspace_bytes(int64_t B, int64_t T, int64_t S, int H, int KV, int h,
                                      int dtype);
 int dpc_attention(const void* q, const void* k, const void* v, const int64_t* strides, int64_t B,
                   int64_t T, int64_t S, int H, int KV, int h, int dtype, const int64_t* lengths,
                   const int64_t* starts, int causal, int window, double scale, void* out,
-                  float* lse, void* ws, size_t ws_bytes, void* stream);
+                  void* state, size_t state_bytes, void* ws, size_t ws_bytes, void* stream);
+size_t dpc_attention_state_bytes(int64_t B, int64_t T, int H, int h, int dtype);
 size_t dpc_attention_grad_workspace_bytes(int64_t B, int64_t T, int H);
 int dpc_attention_grad(const void* q, const void* k, const void* v, const void* out,
                        const void* dout, const int64_t* strides, int64_t B, int64_t T, int64_t S,
                        int H, int KV, int h, int dtype, const int64_t* lengths,
                        const int64_t* starts, int causal, int window, double scale,
-                       const float* lse, void* dq, void* dk, void* dv, void* ws, size_t ws_bytes,
-                       void* stream);
+                       const void* state, size_t state_bytes, void* dq, void* dk, void* dv,
+                       void* ws, size_t ws_bytes, void* stream);
 
 /* Measurement helper with no counterpart in the reference (used by bench.py
  * to put the roofline in context): `grid` workgroups of 8 waves run `iters`

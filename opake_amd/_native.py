@@ -226,13 +226,14 @@ SIGNATURES = {
     "dpc_attention": (
         _c_int,
         [_c_void_p] * 4 + [_c_i64] * 3 + [_c_int] * 4 + [_c_void_p, _c_void_p, _c_int, _c_int,
-         _c_double, _c_void_p, _c_void_p, _c_void_p, _c_size_t, _c_void_p],
+         _c_double, _c_void_p, _c_void_p, _c_size_t, _c_void_p, _c_size_t, _c_void_p],
     ),
+    "dpc_attention_state_bytes": (_c_size_t, [_c_i64, _c_i64, _c_int, _c_int, _c_int]),
     "dpc_attention_grad_workspace_bytes": (_c_size_t, [_c_i64, _c_i64, _c_int]),
     "dpc_attention_grad": (
         _c_int,
         [_c_void_p] * 6 + [_c_i64] * 3 + [_c_int] * 4 + [_c_void_p, _c_void_p, _c_int, _c_int,
-         _c_double] + [_c_void_p] * 5 + [_c_size_t, _c_void_p],
+         _c_double, _c_void_p, _c_size_t] + [_c_void_p] * 4 + [_c_size_t, _c_void_p],
     ),
     "dpc_head_loss_state_bytes": (_c_size_t, [_c_i64] + [_c_int] * 6),
     "dpc_head_loss_workspace_bytes": (_c_size_t, [_c_i64] + [_c_int] * 6),

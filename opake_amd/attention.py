@@ -3,7 +3,8 @@
 ``attention`` takes queries, keys and values as the projections leave them ([B, T, heads,
 h], any strides: places of a fused projection go in as they are), shares key heads among
 groups of query heads, and masks by what a query sees: causal, a window, each example's
-length and the position of its first query.  The forward keeps one number a query for the
+length and the position of its first query.  The forward keeps two numbers a query (for
+bfloat16 one, and a byte an element of the output: what rounding took from it) for the
 backward, which forms the probabilities again (``csrc/attention.hip``).  Results do not depend
 on anything but the inputs: no sums whose order changes.
 """
@@ -25,11 +26,12 @@ MAX_TOKENS = 1 << 24
 _MOST_BYTES = 0x7ff00000 - (1 << 20)
 
 
-def _rows(t: torch.Tensor, rep: int = 1) -> torch.Tensor:
-    """Rows of whole 16-byte chunks, and tiles of 65 tokens within a buffer's range."""
+def _rows(t: torch.Tensor, rep: int = 1, apart: int = 0) -> torch.Tensor:
+    """Rows of whole 16-byte chunks, at least ``apart`` elements from each other, and tiles
+    of 65 tokens within a buffer's range."""
     size = t.element_size()
     b, n, head, last = t.stride()
-    if (last == 1 and t.data_ptr() % 16 == 0 and b * size % 16 == 0 and n * size % 16 == 0
+    if (last == 1 and (n >= apart or t.shape[1] < 2) and t.data_ptr() % 16 == 0 and b * size % 16 == 0 and n * size % 16 == 0
             and head * size % 16 == 0 and (65 * n + rep * head) * size <= _MOST_BYTES):
         return t
     return t.clone(memory_format=torch.contiguous_format)
@@ -49,33 +51,34 @@ class _Attention(torch.autograd.Function):
         dev = q.device
         B, T, H, h = q.shape
         S, KV = k.shape[1:3]
-        qr, kr, vr = _rows(q, H // KV), _rows(k), _rows(v)
+        qr, kr, vr = _rows(q, H // KV), _rows(k, 1, h), _rows(v, 1, h)
         sizes = (B, T, S, H, KV, h, code)
         out = torch.empty((B, T, H, h), dtype=q.dtype, device=dev)
-        lse = None
+        lib, state, state_bytes = nat.load(), None, 0
         # needs_input_grad is true of a parameter under no_grad too.
         if grad_enabled and any(ctx.needs_input_grad[:3]):
             note_leaves(ctx)
-            lse = torch.empty((B, KV, T, H // KV), dtype=torch.float32, device=dev)
-            ctx.save_for_backward(q, k, v, out, lse, lengths, starts)
+            state_bytes = lib.dpc_attention_state_bytes(B, T, H, h, code)
+            state = torch.empty(state_bytes, dtype=torch.uint8, device=dev)
+            ctx.save_for_backward(q, k, v, out, state, lengths, starts)
             ctx.sizes, ctx.options = sizes, options
-        ws_bytes = nat.load().dpc_attention_workspace_bytes(*sizes)
+        ws_bytes = lib.dpc_attention_workspace_bytes(*sizes)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         _call("dpc_attention", dev, (qr, kr, vr),
               (*qr.stride()[:3], *kr.stride()[:3], *vr.stride()[:3]), sizes, lengths, starts,
-              options, out.data_ptr(), 0 if lse is None else lse.data_ptr(), ws.data_ptr(),
-              ws_bytes)
+              options, out.data_ptr(), 0 if state is None else state.data_ptr(), state_bytes,
+              ws.data_ptr(), ws_bytes)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         check_leaves(ctx)
-        q, k, v, out, lse, lengths, starts = ctx.saved_tensors
+        q, k, v, out, state, lengths, starts = ctx.saved_tensors
         dev, sizes = q.device, ctx.sizes
         B, T, S, H, KV, h, _ = sizes
         rep = H // KV
-        qr, kr, vr, gr = _rows(q, rep), _rows(k), _rows(v), _rows(grad, rep)
+        qr, kr, vr, gr = _rows(q, rep), _rows(k, 1, h), _rows(v, 1, h), _rows(grad, rep)
         dq = torch.empty((B, T, H, h), dtype=q.dtype, device=dev)
         dk = dv = None
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
@@ -84,7 +87,7 @@ class _Attention(torch.autograd.Function):
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         _call("dpc_attention_grad", dev, (qr, kr, vr, out, gr),
               (*qr.stride()[:3], *kr.stride()[:3], *vr.stride()[:3], *gr.stride()[:3]), sizes,
-              lengths, starts, ctx.options, lse.data_ptr(), dq.data_ptr(),
+              lengths, starts, ctx.options, state.data_ptr(), state.numel(), dq.data_ptr(),
               *(0 if t is None else t.data_ptr() for t in (dk, dv)), ws.data_ptr(), ws_bytes)
         return dq, dk, dv, None, None, None, None, None
 

@@ -32,42 +32,71 @@
 
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kOutOfRange = 0x7ff00000;  // a byte offset past every buffer
 constexpr int kBufferBytes = 0x7ff00000;
 constexpr int kRowsWave = 32;
 
 extern __shared__ __attribute__((aligned(16))) uint8_t lds_dyn[];
 
+DPC_DEVICE int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // A buffer at an address that is the wave's, of which the compiler may not know that.
-DPC_DEVICE u32x4_t wave_buffer(const void* base, uint32_t bytes) {
+DPC_DEVICE u32x4_t wave_buffer(const void* base, int bytes) {
   u32x4_t r = rsrc_words(base, bytes);
-  r[0] = __builtin_amdgcn_readfirstlane(r[0]);
-  r[1] = __builtin_amdgcn_readfirstlane(r[1]);
-  r[2] = __builtin_amdgcn_readfirstlane(r[2]);
+  r[0] = uniform(r[0]);
+  r[1] = uniform(r[1]);
+  r[2] = uniform(r[2]);
   return r;
 }
 
-// The wave's transfers into LDS have arrived and its reads of LDS are done (their place may
-// be written again); no access moves across.
-DPC_DEVICE void transfers_done() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+// All but the wave's last kLeft transfers into LDS have arrived, and its reads of LDS are
+// done (their place may be written again); no access moves across.
+template <int kLeft>
+DPC_DEVICE void transfers_left() {
+  static_assert(kLeft < 64, "six bits");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLeft) : "memory");
+}
+
+// LDS by byte address: with the tile's place a constant, reads take it as their immediate.
+template <typename V>
+DPC_DEVICE V lds_read(int at) {
+  return *(const __attribute__((address_space(3))) V*)(uint32_t)at;
+}
+DPC_DEVICE i16x4_t lds_read_tr(int at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(uint32_t)at);
+}
+
+// n / d for 0 <= n < 2^31 by a multiplication: the factor ceil(2^(31 + s) / d) with 2^(s - 1)
+// < d <= 2^s is e / d too large with e < 2^s, so the quotient is n e / (d 2^(31 + s)) < 1 / d.
+struct Divisor {
+  uint32_t mul;
+  int shift, d;
+  DPC_DEVICE int of(int n) const { return (int)(((uint64_t)(uint32_t)n * mul) >> shift); }
+};
 
 struct Places {  // of one tensor: elements between examples, tokens and heads
-  int64_t b, t;
-  int64_t head;
+  int64_t b, t, head;
 };
 
 struct AttnArgs {
   const void *q, *k, *v, *out, *dout;
-  Places pq, pk, pv, pdo;  // out, lse and the gradients are contiguous
+  Places pq, pk, pv, pdo;  // out, what is kept and the gradients are contiguous
   void *o, *dq, *dk, *dv;
-  float *lse, *delta;      // [B, KV, rows]
+  // Kept for the backward.  bf16: lse = log2 of a row's sum of exponentials (+inf: it sees
+  // nothing) and what rounding took from out (`rest`, by its own places).  float32: the
+  // maximum that exponentials are taken against (+inf) and one over their sum, since
+  // their logarithm rounded to a float is 2^-20 of the probabilities off.
+  float *lse, *inv;        // [B, KV, rows]
+  int8_t* rest;
+  float* delta;            // -D
   int B, T, S, KV, rep, h;
-  int64_t rows;            // of a key head: T * rep
+  int rows;                // of a key head: T * rep
   const int64_t *lengths, *starts;
   int causal, window;
   float scale, c;          // c = scale log2(e)
   int tiles;               // row tiles (dk, dv: key tiles) of a key head
+  int per_xcd, chunk;      // key heads of an XCD (0: not divided among them), of a chunk
+  Divisor by_rep, by_kv, by_splits;
   // Keys in splits (few rows): partial results.
   int splits;
   float* part_o;           // [splits][B * KV * rows][h]
@@ -83,11 +112,11 @@ struct Sight {
   DPC_DEVICE Sight(const AttnArgs& a, int b) : causal(a.causal), window(a.window) {
     int64_t n = a.lengths ? a.lengths[b] : a.S;
     n = n < 0 ? 0 : (n < a.S ? n : a.S);
-    len = __builtin_amdgcn_readfirstlane((int)n);
+    len = uniform((int)n);
     int64_t s = a.starts ? a.starts[b] : (int64_t)a.S - a.T;
     const int64_t most = 1 << 30;
     s = s < -most ? -most : (s < most ? s : most);
-    start = __builtin_amdgcn_readfirstlane((int)s);
+    start = uniform((int)s);
   }
   // The first and last token that see a key at all, of [t0, t1].
   DPC_DEVICE int first(int t0) const { return causal ? max(t0, -start) : t0; }
@@ -101,13 +130,39 @@ struct Sight {
   DPC_DEVICE int hi(int t) const { return causal ? start + t : len - 1; }
 };
 
-// Linear id -> (key head of the batch, tile): each XCD takes a contiguous range, so that
-// the tiles of a key head read its operands from one L2.
-DPC_DEVICE void place_of(int id, int n, int tiles, int* bk, int* tile) {
-  const int xcd = id & 7;
-  const int lin = xcd * (n >> 3) + min(xcd, n & 7) + (id >> 3);
-  *bk = __builtin_amdgcn_readfirstlane(lin / tiles);
-  *tile = __builtin_amdgcn_readfirstlane(lin % tiles);
+// The tokens of rows [r0, r1) that see a key (none: t_first > t_last), the keys that one of
+// them sees, and those that all of them see.
+struct RowRange {
+  int t_first, t_last, lo, hi, lo_all, hi_all;
+  bool none;
+  DPC_DEVICE RowRange(const AttnArgs& a, const Sight& s, int r0, int r1) {
+    t_first = uniform(s.first(a.by_rep.of(r0)));
+    t_last = uniform(r1 > r0 ? s.last(a.by_rep.of(r1 - 1)) : -1);
+    none = t_first > t_last;
+    lo = uniform(s.lo(t_first));
+    hi = uniform(none ? -1 : s.hi(t_last));
+    lo_all = uniform(s.lo(t_last));
+    hi_all = uniform(s.hi(t_first));
+  }
+};
+
+// Linear id -> (key head of the batch, tile).  Each XCD takes its own key heads, so that
+// the tiles of one read its operands from one L2, and of those a few (`chunk`) at a time, the
+// tiles with most work of all of them first: started last, they would end long after the
+// others (8 x 2048 tokens, 32 heads over 8: a quarter of the time with each key head's
+// tiles by themselves).
+DPC_DEVICE void place_of(const AttnArgs& a, int tiles, int* bk, int* tile) {
+  int x = blockIdx.x, first = 0, heads = a.B * a.KV;
+  if (a.per_xcd) {
+    heads = a.per_xcd;
+    first = (x & 7) * heads;
+    x >>= 3;
+  }
+  const uint32_t size = (uint32_t)a.chunk * (uint32_t)tiles;
+  const int c = uniform((uint32_t)x / size), r = x - c * (int)size;
+  const int now = min(a.chunk, heads - c * a.chunk);
+  *tile = uniform((uint32_t)r / (uint32_t)now);
+  *bk = first + c * a.chunk + r - *tile * now;
 }
 
 // ---------------------------------------------------------------------------
@@ -128,124 +183,137 @@ struct Tile {
   static_assert(kChunks >= 8, "rows of 128 bytes at least");
 };
 
-// The two products' operands of a lane: column (or row) lane % 32, the chunks 2 i + lane /
-// 32 of it.
+// An operand of a lane: its column (lane % 32)'s chunks 2 i + lane / 32.
 template <typename T, int kD>
 struct RowFrags {
   u32x4_t v[Tile<T, kD>::kPairs];
 };
 
-DPC_DEVICE f32x16_t mma(u32x4_t a, u32x4_t b, f32x16_t c, uint16_t) {
+DPC_DEVICE f32x16_t mma_bf16(u32x4_t a, u32x4_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
                                                  __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
 }
-DPC_DEVICE f32x16_t mma(u32x4_t a, u32x4_t b, f32x16_t c, float) {
-  const f32x4_t x = __builtin_bit_cast(f32x4_t, a), y = __builtin_bit_cast(f32x4_t, b);
+
+// bf16: a lane's places in a tile.  Fragments are read by rows (row lane % 32 of a block
+// of 32, pair i of its chunks) or by columns (element lane % 32 of block d of 32, 16 rows in
+// the order that row products leave a lane's column in: 4 (lane / 32) + e, then 8 more).
+template <int kD>
+struct Walk {
+  typedef Tile<uint16_t, kD> X;
+  int row_at[X::kPairs], col_at[2 * X::kBlocks];
+  DPC_DEVICE void init(int lane) {
+    const int row = lane & 31, sw = swizzle<X::kChunks>(row) ^ (lane >> 5);
+    const int base = (int)lds_addr(lds_dyn);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], c, 0, 0, 0);
-  return c;
+    for (int i = 0; i < X::kPairs; ++i) row_at[i] = base + row * X::kRow + (((2 * i) ^ sw) << 4);
+    const int L = lane & 15, r = 4 * (lane >> 5) + (L >> 2);
+    const int chunk = ((lane >> 4) & 1) * 2 + ((L & 3) >> 1);
+#pragma unroll
+    for (int d = 0; d < X::kBlocks; ++d)
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+        col_at[2 * d + half] =
+            base + (r + 8 * half) * X::kRow +
+            (((4 * d + chunk) ^ swizzle<X::kChunks>(r + 8 * half)) << 4) + (L & 1) * 8;
+  }
+  // Block e of 32 rows of the tile at `at`.
+  DPC_DEVICE u32x4_t row(int at, int e, int i) const {
+    return lds_read<u32x4_t>(row_at[i] + (at + e * 32 * X::kRow));
+  }
+  // Rows 16 j .. of block e, columns of block d.
+  DPC_DEVICE u32x4_t col(int at, int e, int j, int d) const {
+    const int o = at + (32 * e + 16 * j) * X::kRow;
+    return __builtin_bit_cast(u32x4_t, join_frag(lds_read_tr(col_at[2 * d] + o),
+                                                 lds_read_tr(col_at[2 * d + 1] + o)));
+  }
+};
+
+// Half j of a lane's column as the second product takes it.
+DPC_DEVICE u32x4_t packed_half(const f32x16_t& x, int j) {
+  u32x4_t b;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) b[e] = f32x2_to_bf16x2_bits(x[8 * j + 2 * e], x[8 * j + 2 * e + 1]);
+  return b;
 }
 
-// 32 rows of an LDS tile times a lane's column: c[r] is row 8 (r / 4) + 4 (lane / 32) + r % 4.
-template <typename T, int kD>
-DPC_DEVICE f32x16_t times_rows(const uint8_t* tile, int row0, const RowFrags<T, kD>& b, int lane) {
-  typedef Tile<T, kD> X;
-  const int row = row0 + (lane & 31), hl = lane >> 5;
-  const uint8_t* at = tile + row * X::kRow;
-  const int sw = swizzle<X::kChunks>(row) ^ hl;
+// The same products in float32 (2 matrix instructions of 64 cycles take the place of one of
+// 32, so nothing but they needs an order).
+template <int kD>
+DPC_DEVICE f32x16_t times_rows(int tile, int row0, const RowFrags<float, kD>& b, int lane) {
+  typedef Tile<float, kD> X;
+  const int row = row0 + (lane & 31), sw = swizzle<X::kChunks>(row) ^ (lane >> 5);
+  const uint8_t* at = lds_dyn + tile + row * X::kRow;
   f32x16_t c = {};
 #pragma unroll
-  for (int i = 0; i < X::kPairs; ++i)
-    c = mma(*reinterpret_cast<const u32x4_t*>(at + (((2 * i) ^ sw) << 4)), b.v[i], c, T());
+  for (int i = 0; i < X::kPairs; ++i) {
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(at + (((2 * i) ^ sw) << 4)),
+                  y = __builtin_bit_cast(f32x4_t, b.v[i]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], c, 0, 0, 0);
+  }
   return c;
 }
 
-// acc[d] += sum over the tile's 32 rows from row0 of (element d of the row) x[row]: x in
-// times_rows' order.
-template <typename T, int kD>
-DPC_DEVICE void add_columns(f32x16_t* acc, const uint8_t* tile, int row0, const f32x16_t& x,
-                            int lane) {
-  typedef Tile<T, kD> X;
-  if constexpr (sizeof(T) == 2) {
-    const int L = lane & 15, hl = lane >> 5;
-    const int row = 4 * hl + (L >> 2), chunk = ((lane >> 4) & 1) * 2 + ((L & 3) >> 1);
-    const int s0 = swizzle<X::kChunks>(row), s1 = swizzle<X::kChunks>(row + 8);
-    const int at = (row0 + row) * X::kRow + (L & 1) * 8;
+template <int kD>
+DPC_DEVICE void add_columns(f32x16_t* acc, int tile, int row0, const f32x16_t& x, int lane) {
+  typedef Tile<float, kD> X;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      u32x4_t b;
+  for (int r = 0; r < 16; ++r) {
+    const int row = row0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+    const int sw = swizzle<X::kChunks>(row);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) b[e] = f32x2_to_bf16x2_bits(x[8 * j + 2 * e], x[8 * j + 2 * e + 1]);
-#pragma unroll
-      for (int d = 0; d < X::kBlocks; ++d) {
-        const int o = at + j * 16 * X::kRow;
-        const bf16x8_t a =
-            join_frag(read_tr(tile, o + (((4 * d + chunk) ^ s0) << 4)),
-                      read_tr(tile, o + 8 * X::kRow + (((4 * d + chunk) ^ s1) << 4)));
-        acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8_t, b),
-                                                         acc[d], 0, 0, 0);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int row = row0 + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
-      const int sw = swizzle<X::kChunks>(row);
-#pragma unroll
-      for (int d = 0; d < X::kBlocks; ++d) {
-        const int col = 32 * d + (lane & 31);
-        const float a = *reinterpret_cast<const float*>(
-            tile + row * X::kRow + (((col >> 2) ^ sw) << 4) + (col & 3) * 4);
-        acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, x[r], acc[d], 0, 0, 0);
-      }
+    for (int d = 0; d < X::kBlocks; ++d) {
+      const int col = 32 * d + (lane & 31);
+      const float a = *reinterpret_cast<const float*>(
+          lds_dyn + tile + row * X::kRow + (((col >> 2) ^ sw) << 4) + (col & 3) * 4);
+      acc[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, x[r], acc[d], 0, 0, 0);
     }
   }
 }
 
-// Transfers of a tile of kRows rows by kWaves waves.
+// Transfers of a tile of kRows rows by kWaves waves: transfer j of a wave takes 64 chunks.
 template <typename T, int kD, int kRows, int kWaves>
 struct Loader {
   typedef Tile<T, kD> X;
   static constexpr int kCount = kRows * X::kChunks / (64 * kWaves);
   static_assert(kCount * 64 * kWaves == kRows * X::kChunks, "whole transfers");
-  int chunk[kCount];  // byte offset in the row; out of range past the head's elements
-  int row0;           // of the lane's first
-  static constexpr int kRowStep = 64 * kWaves / X::kChunks;
-  static_assert(64 * kWaves % X::kChunks == 0 || X::kChunks % (64 * kWaves) == 0, "");
+  static_assert(64 * kWaves % X::kChunks == 0, "a lane keeps its place in the row");
+  int voff[kCount];
 
-  DPC_DEVICE void init(int h, int w, int lane) {
-    row0 = (w * 64 + lane) / X::kChunks;
+  static DPC_DEVICE int row(int j, int w, int lane) {
+    return (w * 64 + lane) / X::kChunks + j * (64 * kWaves / X::kChunks);
+  }
+  // Byte offset of the lane's chunk in its row, or out of range.
+  static DPC_DEVICE int chunk(int j, int h, int w, int lane) {
+    const int c = ((w * 64 + lane) & (X::kChunks - 1)) ^ swizzle<X::kChunks>(row(j, w, lane));
+    return c * X::kEach < h ? c * 16 : kOutOfRange;
+  }
+  // Rows `stride` bytes apart.
+  DPC_DEVICE void init(int stride, int h, int w, int lane) {
 #pragma unroll
     for (int j = 0; j < kCount; ++j) {
-      const int c = ((w * 64 + lane) & (X::kChunks - 1)) ^ swizzle<X::kChunks>(row(j));
-      chunk[j] = c * X::kEach < h ? c * 16 : kOutOfRange;
+      const int c = chunk(j, h, w, lane);
+      voff[j] = c == kOutOfRange ? c : row(j, w, lane) * stride + c;
     }
   }
-  DPC_DEVICE int row(int j) const { return row0 + j * kRowStep; }
-  // Rows `stride` bytes apart; rows from `limit` on are zeros.
-  DPC_DEVICE void rows(const void* base, int stride, int limit, uint32_t lds, int w) const {
-    const u32x4_t buf = wave_buffer(base, kBufferBytes);
+  // `limit` rows of them; the others are zeros (their offsets are past the buffer's end:
+  // rows do not overlap).
+  DPC_DEVICE void rows(const void* base, int stride, int limit, int h, uint32_t lds, int w) const {
+    const u32x4_t buf =
+        wave_buffer(base, (min(limit, kRows) - 1) * stride + h * (int)sizeof(T));
 #pragma unroll
-    for (int j = 0; j < kCount; ++j) {
-      const int off = row(j) < limit ? row(j) * stride + chunk[j] : kOutOfRange;
-      dma16(buf, __builtin_amdgcn_readfirstlane(lds + (w + kWaves * j) * 1024), chunk[j] == kOutOfRange ? kOutOfRange : off, 0);
-    }
+    for (int j = 0; j < kCount; ++j)
+      dma16(buf, uniform(lds + (w + kWaves * j) * 1024), voff[j], 0);
   }
-  // Rows of shared key heads: row r is token (g0 + r) / rep of `base`, head (g0 + r) % rep.
-  DPC_DEVICE void shared(const void* base, int g0, int rep, float inv, int token, int head,
-                         int limit, uint32_t lds, int w) const {
-    const u32x4_t buf = wave_buffer(base, kBufferBytes);
-#pragma unroll
-    for (int j = 0; j < kCount; ++j) {
-      const int r = g0 + row(j);
-      int t = (int)((float)r * inv);  // (r < 2^20: off by one at most)
-      t -= t * rep > r;
-      t += (t + 1) * rep <= r;
-      const int off = t * token + (r - t * rep) * head + chunk[j];
-      dma16(buf, __builtin_amdgcn_readfirstlane(lds + (w + kWaves * j) * 1024),
-            row(j) < limit && chunk[j] != kOutOfRange ? off : kOutOfRange, 0);
-    }
-  }
+};
+
+// A tile of rows of shared key heads: whole tokens of all rep heads, or where rep is over
+// kRows, kRows heads of one token at a time.
+struct RowTiles {
+  int tokens, chunks;  // tokens a tile; tiles a token
+  DPC_DEVICE RowTiles(const AttnArgs& a, int rows)
+      : tokens(a.rep <= rows ? uniform((int)((unsigned)rows / (unsigned)a.rep)) : 1),
+        chunks(a.rep <= rows ? 1 : uniform((int)((unsigned)(a.rep + rows - 1) / (unsigned)rows))) {}
 };
 
 // A lane's row of an operand, from memory (zeros where not valid).
@@ -277,28 +345,45 @@ DPC_DEVICE float sum_halves(float x) {
   return a + b;
 }
 
-// Stores a lane's column (kD elements in times_rows' order, over kD / 32 blocks) times f
-// as row `out`, or zeros where !keep.
+// What rounding x to the bf16 `hi` took from it, to 8 more bits: (hi << 16) + (rest << 8)
+// as a float's bits is x within 2^-17.
+DPC_DEVICE int rest_of(float x, uint32_t hi) {
+  const int d = (int)(__float_as_uint(x) - (hi << 16));
+  return max(-128, min(127, (d + 128) >> 8));
+}
+DPC_DEVICE float with_rest(uint32_t hi, int rest) {
+  return __uint_as_float((hi << 16) + ((uint32_t)rest << 8));
+}
+
+// Stores a lane's column (kD elements in the row products' order, kD / 32 blocks) times f
+// as row `out`, or zeros where !keep; bf16: and `rest`, if not null.
 template <typename T, int kD>
-DPC_DEVICE void store_row(T* out, const f32x16_t* acc, float f, bool keep, bool on, int h,
-                          int lane) {
+DPC_DEVICE void store_row(T* out, int8_t* rest, const f32x16_t* acc, float f, bool keep, bool on,
+                          int h, int lane) {
 #pragma unroll
   for (int d = 0; d < kD / 32; ++d) {
     if constexpr (sizeof(T) == 2) {
       // A pair of quads of both halves makes 8 elements a lane.
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        uint32_t p[4];
+        uint32_t p[4], q[2] = {};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float x = acc[d][8 * j + 2 * e] * f, y = acc[d][8 * j + 2 * e + 1] * f;
           p[e] = keep ? f32x2_to_bf16x2_bits(x, y) : 0u;
+          if (rest && keep)
+            q[e >> 1] |= ((uint32_t)(rest_of(x, p[e] & 0xffffu) & 255) |
+                          (uint32_t)(rest_of(y, p[e] >> 16) & 255) << 8) << (16 * (e & 1));
         }
         const auto lo = __builtin_amdgcn_permlane32_swap(p[0], p[2], false, false);
         const auto hi = __builtin_amdgcn_permlane32_swap(p[1], p[3], false, false);
         const int at = 32 * d + 16 * j + 8 * (lane >> 5);
         if (on && at < h)
           *reinterpret_cast<u32x4_t*>(out + at) = u32x4_t{lo[0], hi[0], lo[1], hi[1]};
+        if (rest) {
+          const auto r = __builtin_amdgcn_permlane32_swap(q[0], q[1], false, false);
+          if (on && at < h) *reinterpret_cast<uint2*>(rest + at) = make_uint2(r[0], r[1]);
+        }
       }
     } else {
 #pragma unroll
@@ -313,128 +398,133 @@ DPC_DEVICE void store_row(T* out, const f32x16_t* acc, float f, bool keep, bool 
   }
 }
 
-// A row tile's place: its rows, its tokens' keys, and the wave's own of both.
-struct RowRange {
-  int t_first, t_last;  // tokens that see a key (t_first > t_last: none)
-  int lo, hi;           // keys that one of them sees
-  int lo_all, hi_all;   // keys that all of them see
-  DPC_DEVICE RowRange(const AttnArgs& a, const Sight& s, int64_t r0, int64_t r1) {
-    t_first = s.first((int)(r0 / a.rep));
-    t_last = r1 > r0 ? s.last((int)((r1 - 1) / a.rep)) : -1;
-    if (t_first > t_last) {
-      lo = lo_all = 0;
-      hi = hi_all = -1;
-      return;
-    }
-    lo = s.lo(t_first);
-    hi = s.hi(t_last);
-    lo_all = s.lo(t_last);
-    hi_all = s.hi(t_first);
+// A lane's row (lane % 32 of a wave's): its token and head, whether it is one, whether it
+// sees a key, and which.
+struct LaneRow {
+  int r, t, g, lo, span;  // keys lo .. lo + span
+  bool there, sees;
+  DPC_DEVICE LaneRow(const AttnArgs& a, const Sight& s, const RowRange& mine, int w0, int lane) {
+    r = w0 + (lane & 31);
+    there = r < a.rows;
+    t = a.by_rep.of(there ? r : a.rows - 1);
+    g = r - t * a.rep;
+    sees = there && t >= mine.t_first && t <= mine.t_last;
+    lo = sees ? s.lo(t) : 1 << 30;
+    span = sees ? s.hi(t) - lo : 0;
   }
-  DPC_DEVICE bool none() const { return t_first > t_last; }
 };
+
+// Row x of a lane's column of row products, in a block of 32.
+DPC_DEVICE int column_row(int x, int lane) { return 8 * (x >> 2) + 4 * (lane >> 5) + (x & 3); }
+
+#define DPC_WALL() __builtin_amdgcn_sched_barrier(0)
 
 // ---------------------------------------------------------------------------
 // Forward.
 // ---------------------------------------------------------------------------
 
-template <typename T, int kD>
-struct ForwardShape {
+// Row tiles of kWaves x 32 rows.  Stages of key and value tiles in LDS: as many as 128 KiB
+// hold, at most four, so that a tile is asked for up to three tiles ahead.
+template <typename T, int kD, int kWaves>
+struct RowsShape {
   static constexpr int kRow = Tile<T, kD>::kRow;
   static constexpr int kKeys = kRow <= 512 ? 64 : 32;
-  static constexpr int kWaves = 4;
-  static constexpr int kLds = 4 * kKeys * kRow;  // two stages of keys and values
-  // Keys in splits: a wave takes 32 keys at a time into LDS of its own.
-  static constexpr int kSplitWaves = kRow <= 256 ? 4 : (kRow == 512 ? 2 : 1);
-  static constexpr int kSplitLds = kSplitWaves * 4 * 32 * kRow;
+  static constexpr int kBytes = kKeys * kRow;
+  static constexpr int kFit = 131072 / (2 * kBytes);
+  static constexpr int kStages = kWaves == 1 ? 2 : (kFit < 4 ? kFit : 4);
+  static constexpr int kLds = kStages * 2 * kBytes;
 };
+// Keys in splits: a wave takes 32 keys at a time into LDS of its own.
+template <typename T, int kD>
+struct SplitShape {
+  static constexpr int kRow = Tile<T, kD>::kRow;
+  static constexpr int kWaves = kRow <= 256 ? 4 : (kRow == 512 ? 2 : 1);
+  static constexpr int kLds = kWaves * 4 * 32 * kRow;
+};
+// Rows of whose tiles two waves share a SIMD (256 registers each).
+template <typename T, int kD>
+constexpr int kMostWaves = sizeof(T) == 2 && kD <= 128 ? 8 : 4;
 
-template <typename T, int kD, bool kSplit>
-__global__ void __launch_bounds__((kSplit ? 64 * ForwardShape<T, kD>::kSplitWaves : 256),
-                                  (Tile<T, kD>::kRow <= 256 && !kSplit ? 2 : 1))
+// Fragments in flight between LDS and the matrix cores: a read is issued that many
+// instructions (of 32 cycles) before its product.
+constexpr int kAhead = 8;
+
+template <typename T, int kD, int kWaves, bool kSplit>
+__global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
     attn_forward_kernel(AttnArgs a) {
   typedef Tile<T, kD> X;
-  typedef ForwardShape<T, kD> Sh;
-  constexpr int kKeys = kSplit ? 32 : Sh::kKeys, kWaves = kSplit ? Sh::kSplitWaves : Sh::kWaves;
-  constexpr int kBytes = kKeys * X::kRow;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  typedef RowsShape<T, kD, kWaves> Sh;
+  constexpr int kKeys = kSplit ? 32 : Sh::kKeys, kStages = kSplit ? 2 : Sh::kStages;
+  constexpr int kBytes = kKeys * X::kRow, kParts = kKeys / 32, kNext = kStages - 1;
+  const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
   int bk, tile, split = 0;
-  {
-    const int per = a.tiles * (kSplit ? a.splits : 1);
-    place_of(blockIdx.x, a.B * a.KV * per, per, &bk, &tile);
-    if (kSplit) {
-      split = tile % a.splits * kWaves + w;
-      tile /= a.splits;
-    }
-    tile = a.tiles - 1 - tile;  // the longest first
+  place_of(a, kSplit ? a.tiles * a.splits : a.tiles, &bk, &tile);
+  if (kSplit) {
+    const int t = uniform(a.by_splits.of(tile));
+    split = (tile - t * a.splits) * kWaves + w;
+    tile = t;
   }
-  const int b = bk / a.KV, kv = bk - b * a.KV;
+  tile = a.tiles - 1 - tile;  // the longest first
+  const int b = uniform(a.by_kv.of(bk)), kv = bk - b * a.KV;
   const Sight sight(a, b);
   constexpr int kTileRows = kSplit ? kRowsWave : kRowsWave * kWaves;
-  const int64_t t0 = (int64_t)tile * kTileRows, t1 = min(t0 + kTileRows, a.rows);
-  const int64_t w0 = kSplit ? t0 : t0 + w * kRowsWave, w1 = min(w0 + kRowsWave, t1);
-  const RowRange all(a, sight, t0, t1), mine(a, sight, w0, w1 > w0 ? w1 : w0);
-
-  // The lane's row.
-  const int64_t r = w0 + (lane & 31);
-  const int t = (int)(min(r, a.rows - 1) / a.rep), g = (int)(r - (int64_t)t * a.rep);
-  const bool there = r < a.rows, sees = there && t >= mine.t_first && t <= mine.t_last;
-  const int lo = sees ? sight.lo(t) : 0, hi = sees ? sight.hi(t) : -1;
+  const int t0 = tile * kTileRows, t1 = min(t0 + kTileRows, a.rows);
+  const int w0 = kSplit ? t0 : t0 + w * kRowsWave, w1 = min(w0 + kRowsWave, t1);
+  const RowRange all(a, sight, t0, t1), mine(a, sight, min(w0, a.rows), w1);
+  const LaneRow me(a, sight, mine, w0, lane);
+  const int64_t head = (int64_t)kv * a.rep + me.g;
   RowFrags<T, kD> q;
-  load_row<T, kD>(q, static_cast<const T*>(a.q) + b * a.pq.b + t * a.pq.t +
-                         ((int64_t)kv * a.rep + g) * a.pq.head, sees, a.h, lane);
+  load_row<T, kD>(q, static_cast<const T*>(a.q) + b * a.pq.b + me.t * a.pq.t + head * a.pq.head,
+                  me.sees, a.h, lane);
 
   const T* kbase = static_cast<const T*>(a.k) + b * a.pk.b + kv * a.pk.head;
   const T* vbase = static_cast<const T*>(a.v) + b * a.pv.b + kv * a.pv.head;
   const int kstride = (int)(a.pk.t * sizeof(T)), vstride = (int)(a.pv.t * sizeof(T));
-  constexpr int kLoaders = kSplit ? 1 : kWaves;
-  Loader<T, kD, kKeys, kLoaders> loader;
   const int lw = kSplit ? 0 : w;
-  loader.init(a.h, lw, lane);
-  uint8_t* lds = lds_dyn + (kSplit ? w * 4 * kBytes : 0);
-  const uint32_t lds0 = lds_addr(lds);
+  Loader<T, kD, kKeys, (kSplit ? 1 : kWaves)> kload, vload;
+  kload.init(kstride, a.h, lw, lane);
+  vload.init(vstride, a.h, lw, lane);
+  const int lds0 = kSplit ? w * 4 * kBytes : 0;  // in lds_dyn
+  const uint32_t lds_base = lds_addr(lds_dyn);
+  Walk<(sizeof(T) == 2 ? kD : 64)> walk;
+  if constexpr (sizeof(T) == 2) walk.init(lane);
 
   f32x16_t o[X::kBlocks] = {};
-  float m = -INFINITY, l = 0.f;
-  int n = all.none() ? 0 : all.hi / kKeys - all.lo / kKeys + 1, first = all.lo / kKeys;
+  float m = -INFINITY, l = 0.f, l2 = 0.f;
+  int first = all.lo / kKeys, n = all.none ? 0 : all.hi / kKeys - first + 1;
   if (kSplit && n > 0) {  // this wave's share of the row tile's keys
-    const int parts = a.splits * kWaves, s0 = (int)((int64_t)n * split / parts),
-              s1 = (int)((int64_t)n * (split + 1) / parts);
+    const int parts = a.splits * kWaves;
+    const int s0 = (int)((uint32_t)n * (uint64_t)split / (uint32_t)parts),
+              s1 = (int)((uint32_t)n * (uint64_t)(split + 1) / (uint32_t)parts);
     first += s0;
     n = s1 - s0;
   }
+  first = uniform(first);
+  n = uniform(n);
   const int limit = min(sight.len, all.hi + 1);
-  auto fetch = [&](int i) __attribute__((always_inline)) {
-    const int j0 = (first + i) * kKeys;
-    const uint32_t at = lds0 + (i & 1) * 2 * kBytes;
-    loader.rows(kbase + (int64_t)j0 * a.pk.t, kstride, limit - j0, at, lw);
-    loader.rows(vbase + (int64_t)j0 * a.pv.t, vstride, limit - j0, at + kBytes, lw);
+  // Tile i into a stage (past the last: that again, so that the number of transfers in
+  // flight is always the same).
+  constexpr int kCount = 2 * decltype(kload)::kCount;
+  auto fetch = [&](int i, int stage) __attribute__((always_inline)) {
+    const int j0 = (first + min(i, n - 1)) * kKeys;
+    const uint32_t at = lds_base + lds0 + stage * 2 * kBytes;
+    kload.rows(kbase + j0 * a.pk.t, kstride, limit - j0, a.h, at, lw);
+    vload.rows(vbase + j0 * a.pv.t, vstride, limit - j0, a.h, at + kBytes, lw);
   };
-  if (n > 0) fetch(0);
-  for (int i = 0; i < n; ++i) {
-    transfers_done();
-    if (!kSplit) __syncthreads();
-    if (i + 1 < n) fetch(i + 1);
-    const int j0 = (first + i) * kKeys;
-    if (mine.none() || j0 > mine.hi || j0 + kKeys <= mine.lo) continue;
-    const bool whole = j0 >= mine.lo_all && j0 + kKeys - 1 <= mine.hi_all;
-    const uint8_t* kt = lds + (i & 1) * 2 * kBytes;
-    const uint8_t* vt = kt + kBytes;
-    f32x16_t s[kKeys / 32];
+  // The tile's statistics go into the lane's: what the exponentials are taken against.
+  auto statistics = [&](f32x16_t* s, int j0) __attribute__((always_inline)) {
+    if (j0 < mine.lo_all || j0 + kKeys - 1 > mine.hi_all) {
+      const int from = j0 + 4 * (lane >> 5) - me.lo;
 #pragma unroll
-    for (int e = 0; e < kKeys / 32; ++e) s[e] = times_rows<T, kD>(kt, 32 * e, q, lane);
-    if (!whole) {
+      for (int e = 0; e < kParts; ++e)
 #pragma unroll
-      for (int e = 0; e < kKeys / 32; ++e)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const int j = j0 + 32 * e + 8 * (x >> 2) + 4 * (lane >> 5) + (x & 3);
-          if (j < lo || j > hi) s[e][x] = -INFINITY;
-        }
+        for (int x = 0; x < 16; ++x)
+          if ((uint32_t)(from + 32 * e + 8 * (x >> 2) + (x & 3)) > (uint32_t)me.span)
+            s[e][x] = -INFINITY;
     }
     float top = s[0][0];
 #pragma unroll
-    for (int e = 0; e < kKeys / 32; ++e)
+    for (int e = 0; e < kParts; ++e)
 #pragma unroll
       for (int x = 0; x < 16; ++x) top = fmaxf(top, s[e][x]);
     top = max_halves(top) * a.c;
@@ -445,33 +535,114 @@ __global__ void __launch_bounds__((kSplit ? 64 * ForwardShape<T, kD>::kSplitWave
       const float f = to == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - to);
       m = to;
       l *= f;
+      l2 *= f;
 #pragma unroll
       for (int d = 0; d < X::kBlocks; ++d) o[d] *= f;
     }
-    const float from = m == -INFINITY ? 0.f : m;
+    return m == -INFINITY ? 0.f : m;
+  };
+  auto step = [&](int i, int stage) __attribute__((always_inline)) {
+    transfers_left<(kNext - 1) * kCount>();
+    if (!kSplit) __syncthreads();
+    fetch(i + kNext, (stage + kNext) % kStages);
+    const int j0 = (first + i) * kKeys;
+    if (j0 > mine.hi || j0 + kKeys <= mine.lo) return;
+    const int kt = lds0 + stage * 2 * kBytes, vt = kt + kBytes;
+    f32x16_t s[kParts] = {};
+    if constexpr (sizeof(T) == 2) {
+      constexpr int kScores = kParts * X::kPairs, kValues = kParts * 2 * X::kBlocks;
+      u32x4_t ring[kAhead];
+      // Fragment u of the tile: the keys' rows, then the values' columns.
+      auto read = [&](int u) __attribute__((always_inline)) {
+        if (u < kScores)
+          ring[u % kAhead] = walk.row(kt, u / X::kPairs, u % X::kPairs);
+        else if (u < kScores + kValues)
+          ring[u % kAhead] = walk.col(vt, (u - kScores) / (2 * X::kBlocks),
+                                      (u - kScores) / X::kBlocks % 2, (u - kScores) % X::kBlocks);
+      };
+      DPC_WALL();
 #pragma unroll
-    for (int e = 0; e < kKeys / 32; ++e) {
+      for (int u = 0; u < kAhead; ++u) read(u);
+      DPC_WALL();
+#pragma unroll
+      for (int u = 0; u < kScores; ++u) {
+        s[u / X::kPairs] = mma_bf16(ring[u % kAhead], q.v[u % X::kPairs], s[u / X::kPairs]);
+        read(u + kAhead);
+        DPC_WALL();
+      }
+      const float from = statistics(s, j0);
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
-        s[e][x] = __builtin_amdgcn_exp2f(fmaf(s[e][x], a.c, -from));
-        l += s[e][x];
+        s[0][x] = __builtin_amdgcn_exp2f(fmaf(s[0][x], a.c, -from));
+        (x & 1 ? l2 : l) += s[0][x];
       }
-      add_columns<T, kD>(o, vt, 32 * e, s[e], lane);
+      // The next block's exponentials go between this one's products.
+#pragma unroll
+      for (int e = 0; e < kParts; ++e) {
+        const u32x4_t p[2] = {packed_half(s[e], 0), packed_half(s[e], 1)};
+        DPC_WALL();
+#pragma unroll
+        for (int u = 0; u < 2 * X::kBlocks; ++u) {
+          const int at = kScores + e * 2 * X::kBlocks + u, d = u % X::kBlocks;
+          o[d] = mma_bf16(ring[at % kAhead], p[u / X::kBlocks], o[d]);
+          read(at + kAhead);
+          if (e + 1 < kParts) {
+            constexpr int kEach = 16 / (2 * X::kBlocks);
+#pragma unroll
+            for (int x = u * kEach; x < (u + 1) * kEach; ++x) {
+              s[e + 1][x] = __builtin_amdgcn_exp2f(fmaf(s[e + 1][x], a.c, -from));
+              (x & 1 ? l2 : l) += s[e + 1][x];
+            }
+          }
+          DPC_WALL();
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kParts; ++e) s[e] = times_rows<kD>(kt, 32 * e, q, lane);
+      const float from = statistics(s, j0);
+#pragma unroll
+      for (int e = 0; e < kParts; ++e) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          s[e][x] = __builtin_amdgcn_exp2f(fmaf(s[e][x], a.c, -from));
+          l += s[e][x];
+        }
+        add_columns<kD>(o, vt, 32 * e, s[e], lane);
+      }
     }
+  };
+  if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < kNext; ++i) fetch(i, i);
   }
-  l = sum_halves(l);
-  const int64_t row = (int64_t)bk * a.rows + r;
+  for (int i = 0; i < n; i += kStages) {
+#pragma unroll
+    for (int x = 0; x < kStages; ++x)
+      if (x == 0 || i + x < n) step(i + x, x);
+  }
+  transfers_left<0>();  // none may land in LDS that is another's
+  l = sum_halves(l + l2);
+  const int64_t row = (int64_t)bk * a.rows + me.r;
   if (kSplit) {
     const int64_t at = (int64_t)split * a.B * a.KV * a.rows + row;
-    if (there && lane < 32) a.part_ml[at] = make_float2(sees ? m : -INFINITY, sees ? l : 0.f);
-    store_row<float, kD>(a.part_o + at * a.h, o, 1.f, sees, there, a.h, lane);
+    if (me.there && lane < 32)
+      a.part_ml[at] = make_float2(me.sees ? m : -INFINITY, me.sees ? l : 0.f);
+    store_row<float, kD>(a.part_o + at * a.h, nullptr, o, 1.f, me.sees, me.there, a.h, lane);
     return;
   }
-  const bool some = sees && l != 0.f;  // (NaN too)
-  if (there && lane < 32 && a.lse) a.lse[row] = some ? m + __builtin_amdgcn_logf(l) : INFINITY;
-  T* out = static_cast<T*>(a.o) +
-           ((int64_t)(b * (int64_t)a.T + t) * a.KV * a.rep + (int64_t)kv * a.rep + g) * a.h;
-  store_row<T, kD>(out, o, 1.f / l, some, there, a.h, lane);
+  const bool some = me.sees && l != 0.f;  // (NaN too)
+  if (me.there && lane < 32 && a.lse) {
+    if constexpr (sizeof(T) == 2) {
+      a.lse[row] = some ? m + __builtin_amdgcn_logf(l) : INFINITY;
+    } else {
+      a.lse[row] = some ? m : INFINITY;
+      a.inv[row] = some ? 1.f / l : 0.f;
+    }
+  }
+  const int64_t flat = (((int64_t)b * a.T + me.t) * a.KV * a.rep + head) * a.h;
+  store_row<T, kD>(static_cast<T*>(a.o) + flat, a.rest ? a.rest + flat : nullptr, o, 1.f / l, some,
+                   me.there, a.h, lane);
 }
 
 // The splits of a row joined: one wave a row.
@@ -496,16 +667,27 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int parts) {
   const bool some = l != 0.f;
   const int64_t bk = row / a.rows, r = row - bk * a.rows, b = bk / a.KV, kv = bk - b * a.KV,
                 t = r / a.rep, g = r - t * a.rep;
-  if (a.lse && lane == 0) a.lse[row] = some ? m + __builtin_amdgcn_logf(l) : INFINITY;
-  T* out = static_cast<T*>(a.o) + ((b * a.T + t) * a.KV * a.rep + kv * a.rep + g) * a.h;
+  if (a.lse && lane == 0) {
+    if constexpr (sizeof(T) == 2) {
+      a.lse[row] = some ? m + __builtin_amdgcn_logf(l) : INFINITY;
+    } else {
+      a.lse[row] = some ? m : INFINITY;
+      a.inv[row] = some ? 1.f / l : 0.f;
+    }
+  }
+  const int64_t flat = ((b * a.T + t) * a.KV * a.rep + kv * a.rep + g) * a.h;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (lane + 64 * e < a.h) {
       const float x = some ? o[e] / l : 0.f;
-      if constexpr (sizeof(T) == 2)
-        out[lane + 64 * e] = f32_to_bf16_bits(x);
-      else
-        out[lane + 64 * e] = x;
+      const int64_t at = flat + lane + 64 * e;
+      if constexpr (sizeof(T) == 2) {
+        const uint16_t hi = f32_to_bf16_bits(x);
+        static_cast<uint16_t*>(a.o)[at] = hi;
+        if (a.rest) a.rest[at] = (int8_t)rest_of(x, hi);
+      } else {
+        static_cast<float*>(a.o)[at] = x;
+      }
     }
 }
 
@@ -513,135 +695,203 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int parts) {
 // dq and D: rows fixed, keys walked.
 // ---------------------------------------------------------------------------
 
-template <typename T, int kD>
-__global__ void __launch_bounds__(256, (Tile<T, kD>::kRow <= 256 ? 2 : 1))
+template <typename T, int kD, int kWaves>
+__global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
     attn_dq_kernel(AttnArgs a) {
   typedef Tile<T, kD> X;
-  constexpr int kKeys = ForwardShape<T, kD>::kKeys, kWaves = 4, kBytes = kKeys * X::kRow;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  typedef RowsShape<T, kD, kWaves> Sh;
+  constexpr int kKeys = Sh::kKeys, kBytes = Sh::kBytes, kStages = Sh::kStages;
+  constexpr int kParts = kKeys / 32, kNext = kStages - 1;
+  const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
   int bk, tile;
-  place_of(blockIdx.x, a.B * a.KV * a.tiles, a.tiles, &bk, &tile);
+  place_of(a, a.tiles, &bk, &tile);
   tile = a.tiles - 1 - tile;
-  const int b = bk / a.KV, kv = bk - b * a.KV;
+  const int b = uniform(a.by_kv.of(bk)), kv = bk - b * a.KV;
   const Sight sight(a, b);
-  const int64_t t0 = (int64_t)tile * kRowsWave * kWaves,
-                t1 = min(t0 + kRowsWave * kWaves, a.rows);
-  const int64_t w0 = t0 + w * kRowsWave, w1 = min(w0 + kRowsWave, t1);
-  const RowRange all(a, sight, t0, t1), mine(a, sight, w0, w1 > w0 ? w1 : w0);
-  const int64_t r = w0 + (lane & 31);
-  const int t = (int)(min(r, a.rows - 1) / a.rep), g = (int)(r - (int64_t)t * a.rep);
-  const bool there = r < a.rows, sees = there && t >= mine.t_first && t <= mine.t_last;
-  const int lo = sees ? sight.lo(t) : 0, hi = sees ? sight.hi(t) : -1;
-  const int64_t head = (int64_t)kv * a.rep + g, row = (int64_t)bk * a.rows + r;
-  const int64_t flat = ((int64_t)(b * (int64_t)a.T + t) * a.KV * a.rep + head) * a.h;
-  RowFrags<T, kD> q, dout;
-  load_row<T, kD>(q, static_cast<const T*>(a.q) + b * a.pq.b + t * a.pq.t + head * a.pq.head, sees,
-                  a.h, lane);
-  load_row<T, kD>(dout, static_cast<const T*>(a.dout) + b * a.pdo.b + t * a.pdo.t +
-                            head * a.pdo.head, sees, a.h, lane);
-  float D = 0.f;
-#pragma unroll
-  for (int i = 0; i < X::kPairs; ++i) {
-    const int at = (2 * i + (lane >> 5)) * X::kEach;
-    const u32x4_t x = sees && at < a.h
-        ? *reinterpret_cast<const u32x4_t*>(static_cast<const T*>(a.out) + flat + at) : u32x4_t{};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (sizeof(T) == 2) {
-        D += bf16_bits_to_f32((uint16_t)x[e]) * bf16_bits_to_f32((uint16_t)dout.v[i][e]);
-        D += bf16_bits_to_f32((uint16_t)(x[e] >> 16)) *
-             bf16_bits_to_f32((uint16_t)(dout.v[i][e] >> 16));
-      } else {
-        D += __uint_as_float(x[e]) * __uint_as_float(dout.v[i][e]);
-      }
-    }
-  }
-  D = sum_halves(D);
-  if (there && lane < 32) a.delta[row] = D;
-  const float lse = sees ? a.lse[row] : INFINITY;
+  const int t0 = tile * kRowsWave * kWaves, t1 = min(t0 + kRowsWave * kWaves, a.rows);
+  const int w0 = t0 + w * kRowsWave, w1 = min(w0 + kRowsWave, t1);
+  const RowRange all(a, sight, t0, t1), mine(a, sight, min(w0, a.rows), w1);
+  const LaneRow me(a, sight, mine, w0, lane);
+  const int64_t head = (int64_t)kv * a.rep + me.g, row = (int64_t)bk * a.rows + me.r;
+  const int64_t flat = (((int64_t)b * a.T + me.t) * a.KV * a.rep + head) * a.h;
 
   const T* kbase = static_cast<const T*>(a.k) + b * a.pk.b + kv * a.pk.head;
   const T* vbase = static_cast<const T*>(a.v) + b * a.pv.b + kv * a.pv.head;
   const int kstride = (int)(a.pk.t * sizeof(T)), vstride = (int)(a.pv.t * sizeof(T));
-  Loader<T, kD, kKeys, kWaves> loader;
-  loader.init(a.h, w, lane);
-  const uint32_t lds0 = lds_addr(lds_dyn);
-  f32x16_t dq[X::kBlocks] = {};
-  const int first = all.lo / kKeys, n = all.none() ? 0 : all.hi / kKeys - first + 1;
+  Loader<T, kD, kKeys, kWaves> kload, vload;
+  kload.init(kstride, a.h, w, lane);
+  vload.init(vstride, a.h, w, lane);
+  const uint32_t lds_base = lds_addr(lds_dyn);
+  const int first = uniform(all.lo / kKeys),
+            n = uniform(all.none ? 0 : all.hi / kKeys - first + 1);
   const int limit = min(sight.len, all.hi + 1);
-  auto fetch = [&](int i) __attribute__((always_inline)) {
-    const int j0 = (first + i) * kKeys;
-    const uint32_t at = lds0 + (i & 1) * 2 * kBytes;
-    loader.rows(kbase + (int64_t)j0 * a.pk.t, kstride, limit - j0, at, w);
-    loader.rows(vbase + (int64_t)j0 * a.pv.t, vstride, limit - j0, at + kBytes, w);
+  constexpr int kCount = 2 * decltype(kload)::kCount;
+  auto fetch = [&](int i, int stage) __attribute__((always_inline)) {
+    const int j0 = (first + min(i, n - 1)) * kKeys;
+    const uint32_t at = lds_base + stage * 2 * kBytes;
+    kload.rows(kbase + j0 * a.pk.t, kstride, limit - j0, a.h, at, w);
+    vload.rows(vbase + j0 * a.pv.t, vstride, limit - j0, a.h, at + kBytes, w);
   };
-  if (n > 0) fetch(0);
-  for (int i = 0; i < n; ++i) {
-    transfers_done();
-    __syncthreads();
-    if (i + 1 < n) fetch(i + 1);
-    const int j0 = (first + i) * kKeys;
-    if (mine.none() || j0 > mine.hi || j0 + kKeys <= mine.lo) continue;
-    const bool whole = j0 >= mine.lo_all && j0 + kKeys - 1 <= mine.hi_all;
-    const uint8_t* kt = lds_dyn + (i & 1) * 2 * kBytes;
-    const uint8_t* vt = kt + kBytes;
+  if (n > 0) {
 #pragma unroll
-    for (int e = 0; e < kKeys / 32; ++e) {
-      f32x16_t s = times_rows<T, kD>(kt, 32 * e, q, lane);
-      const f32x16_t dp = times_rows<T, kD>(vt, 32 * e, dout, lane);
+    for (int i = 0; i < kNext; ++i) fetch(i, i);
+  }
+
+  RowFrags<T, kD> q, dout;
+  load_row<T, kD>(q, static_cast<const T*>(a.q) + b * a.pq.b + me.t * a.pq.t + head * a.pq.head,
+                  me.sees, a.h, lane);
+  load_row<T, kD>(dout, static_cast<const T*>(a.dout) + b * a.pdo.b + me.t * a.pdo.t +
+                            head * a.pdo.head, me.sees, a.h, lane);
+  float D = 0.f;
 #pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[x], a.c, -lse));
-        s[x] = p * (dp[x] - D);
+  for (int i = 0; i < X::kPairs; ++i) {
+    const int at = (2 * i + (lane >> 5)) * X::kEach;
+    const bool on = me.sees && at < a.h;
+    const u32x4_t x = on ? *reinterpret_cast<const u32x4_t*>(static_cast<const T*>(a.out) + flat +
+                                                            at) : u32x4_t{};
+    if constexpr (sizeof(T) == 2) {
+      const uint2 y = on ? *reinterpret_cast<const uint2*>(a.rest + flat + at) : uint2{};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t word = e < 4 ? y.x : y.y;
+        const int rest = (int)(word << (24 - 8 * (e & 3))) >> 24;
+        const uint32_t hi = (x[e >> 1] >> (16 * (e & 1))) & 0xffffu,
+                       g = (dout.v[i][e >> 1] >> (16 * (e & 1))) & 0xffffu;
+        D = fmaf(with_rest(hi, rest), bf16_bits_to_f32((uint16_t)g), D);
       }
-      if (!whole) {
+    } else {
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const int j = j0 + 32 * e + 8 * (x >> 2) + 4 * (lane >> 5) + (x & 3);
-          if (j < lo || j > hi) s[x] = 0.f;
-        }
-      }
-      add_columns<T, kD>(dq, kt, 32 * e, s, lane);
+      for (int e = 0; e < 4; ++e)
+        D = fmaf(__uint_as_float(x[e]), __uint_as_float(dout.v[i][e]), D);
     }
   }
-  store_row<T, kD>(static_cast<T*>(a.dq) + flat, dq, a.scale, sees, there, a.h, lane);
+  D = sum_halves(D);
+  if (me.there && lane < 32) a.delta[row] = -D;
+  const float lse = me.sees ? a.lse[row] : INFINITY;
+  const float inv = sizeof(T) == 4 && me.sees ? a.inv[row] : 0.f;
+  Walk<(sizeof(T) == 2 ? kD : 64)> walk;
+  if constexpr (sizeof(T) == 2) walk.init(lane);
+  f32x16_t dq[X::kBlocks] = {};
+
+  auto step = [&](int i, int stage) __attribute__((always_inline)) {
+    transfers_left<(kNext - 1) * kCount>();
+    __syncthreads();
+    fetch(i + kNext, (stage + kNext) % kStages);
+    const int j0 = (first + i) * kKeys;
+    if (j0 > mine.hi || j0 + kKeys <= mine.lo) return;
+    const bool whole = j0 >= mine.lo_all && j0 + kKeys - 1 <= mine.hi_all;
+    const int kt = stage * 2 * kBytes, vt = kt + kBytes;
+    auto masked = [&](f32x16_t& x, int e) __attribute__((always_inline)) {
+      const int from = j0 + 32 * e + 4 * (lane >> 5) - me.lo;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if ((uint32_t)(from + 8 * (i >> 2) + (i & 3)) > (uint32_t)me.span) x[i] = 0.f;
+    };
+    if constexpr (sizeof(T) == 2) {
+      // Fragment u of a block of 32 keys: the keys' rows, the values', the keys' columns.
+      constexpr int kFront = 2 * X::kPairs, kCols = 2 * X::kBlocks, kAll = kFront + kCols;
+      u32x4_t ring[kAhead];
+      auto read = [&](int u) __attribute__((always_inline)) {
+        const int e = u / kAll, v = u % kAll, c = v - kFront;
+        if (e >= kParts) return;
+        ring[u % kAhead] = v < kFront
+            ? walk.row(v < X::kPairs ? kt : vt, e, v % X::kPairs)
+            : walk.col(kt, e, c / X::kBlocks % 2, c % X::kBlocks);
+      };
+      DPC_WALL();
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) read(u);
+      DPC_WALL();
+#pragma unroll
+      for (int e = 0; e < kParts; ++e) {
+        f32x16_t s = {}, dp = {};
+#pragma unroll
+        for (int v = 0; v < kFront; ++v) {
+          const int u = e * kAll + v, i = v % X::kPairs;
+          if (v < X::kPairs)
+            s = mma_bf16(ring[u % kAhead], q.v[i], s);
+          else
+            dp = mma_bf16(ring[u % kAhead], dout.v[i], dp);
+          read(u + kAhead);
+          // The probabilities, once the scores are out, between the other product.
+          if (v >= X::kPairs) {
+#pragma unroll
+            for (int x = i * 16 / X::kPairs; x < (i + 1) * 16 / X::kPairs; ++x)
+              s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], a.c, -lse));
+          }
+          DPC_WALL();
+        }
+#pragma unroll
+        for (int x = 0; x < 16; ++x) s[x] *= dp[x] - D;
+        if (!whole) masked(s, e);
+        const u32x4_t p[2] = {packed_half(s, 0), packed_half(s, 1)};
+        DPC_WALL();
+#pragma unroll
+        for (int v = 0; v < kCols; ++v) {
+          const int u = e * kAll + kFront + v, d = v % X::kBlocks;
+          dq[d] = mma_bf16(ring[u % kAhead], p[v / X::kBlocks], dq[d]);
+          read(u + kAhead);
+          DPC_WALL();
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kParts; ++e) {
+        f32x16_t s = times_rows<kD>(kt, 32 * e, q, lane);
+        const f32x16_t dp = times_rows<kD>(vt, 32 * e, dout, lane);
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], a.c, -lse)) * inv * (dp[x] - D);
+        if (!whole) masked(s, e);
+        add_columns<kD>(dq, kt, 32 * e, s, lane);
+      }
+    }
+  };
+  for (int i = 0; i < n; i += kStages) {
+#pragma unroll
+    for (int x = 0; x < kStages; ++x)
+      if (x == 0 || i + x < n) step(i + x, x);
+  }
+  transfers_left<0>();
+  store_row<T, kD>(static_cast<T*>(a.dq) + flat, nullptr, dq, a.scale, me.sees, me.there, a.h,
+                   lane);
 }
 
 // ---------------------------------------------------------------------------
 // dk and dv: keys fixed, rows walked.
 // ---------------------------------------------------------------------------
 
-template <typename T, int kD>
+// Key tiles of kWaves x 32 keys, a wave a SIMD; stages as RowsShape's.
+template <typename T, int kD, int kWaves>
 struct KeysShape {
   static constexpr int kRow = Tile<T, kD>::kRow;
-  static constexpr int kRows = kRow <= 512 ? 64 : 32;  // of queries, a tile
+  static constexpr int kRows = kRow < 512 ? 64 : 32;  // of queries, a tile
   static constexpr int kBytes = kRows * kRow;
-  static constexpr int kLds = 4 * kBytes + 2 * 2 * 256;  // two stages; each 64 of lse and D
-  // Keys and values of a lane in registers, beside their gradients' 2 kD / 2 accumulators.
+  static constexpr int kStats = 4 * 256;  // 64 of lse, -D, inv; and a place for nothing
+  static constexpr int kStage = 2 * kBytes + kStats;
+  static constexpr int kFit = 135168 / kStage;
+  static constexpr int kStages = kWaves == 1 ? 2 : (kFit < 4 ? kFit : 4);
+  static constexpr int kLds = kStages * kStage;
+  // Keys and values of a lane in registers, beside their gradients' accumulators.
   static constexpr bool kHold = kRow <= 512;
 };
 
-template <typename T, int kD>
-__global__ void __launch_bounds__(256, 1) attn_dkv_kernel(AttnArgs a) {
+template <typename T, int kD, int kWaves>
+__global__ void __launch_bounds__(64 * kWaves, 1) attn_dkv_kernel(AttnArgs a) {
   typedef Tile<T, kD> X;
-  typedef KeysShape<T, kD> Sh;
-  constexpr int kRows = Sh::kRows, kWaves = 4, kBytes = Sh::kBytes;
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  typedef KeysShape<T, kD, kWaves> Sh;
+  constexpr int kRows = Sh::kRows, kBytes = Sh::kBytes, kParts = kRows / 32;
+  constexpr int kStages = Sh::kStages, kNext = kStages - 1;
+  const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
   int bk, tile;  // the first keys are seen by most rows
-  place_of(blockIdx.x, a.B * a.KV * a.tiles, a.tiles, &bk, &tile);
-  const int b = bk / a.KV, kv = bk - b * a.KV;
+  place_of(a, a.tiles, &bk, &tile);
+  const int b = uniform(a.by_kv.of(bk)), kv = bk - b * a.KV;
   const Sight sight(a, b);
   const int j0 = tile * kRowsWave * kWaves, jw = j0 + w * kRowsWave;
   const int key = jw + (lane & 31);
   const bool there = key < a.S, seen = key < sight.len;
   const T* krow = static_cast<const T*>(a.k) + b * a.pk.b + kv * a.pk.head + key * a.pk.t;
   const T* vrow = static_cast<const T*>(a.v) + b * a.pv.b + kv * a.pv.head + key * a.pv.t;
-  RowFrags<T, kD> k, v;
-  if constexpr (Sh::kHold) {
-    load_row<T, kD>(k, krow, seen, a.h, lane);
-    load_row<T, kD>(v, vrow, seen, a.h, lane);
-  }
-  f32x16_t dk[X::kBlocks] = {}, dv[X::kBlocks] = {};
 
   // The tokens that may see one of these keys.
   int ta = sight.first(0), tb = sight.last(a.T - 1);
@@ -651,84 +901,214 @@ __global__ void __launch_bounds__(256, 1) attn_dkv_kernel(AttnArgs a) {
     if (sight.window) tb = min(tb, j1 + sight.window - 1 - sight.start);
   }
   if (j0 > j1) tb = ta - 1;
-  const int64_t r0 = (int64_t)ta * a.rep, r1 = (int64_t)(tb + 1) * a.rep;
-  const int n = tb < ta ? 0 : (int)((r1 - r0 + kRows - 1) / kRows);
+  ta = uniform(ta);
+  tb = uniform(tb);
+  const RowTiles tiles(a, kRows);
+  const bool grouped = a.rep <= kRows;
+  const int n = tb < ta ? 0
+      : uniform((int)((unsigned)(tb - ta + tiles.tokens) / (unsigned)tiles.tokens)) * tiles.chunks;
 
-  const float inv = 1.f / (float)a.rep;
   const T* qbase = static_cast<const T*>(a.q) + b * a.pq.b + (int64_t)kv * a.rep * a.pq.head;
   const T* dbase = static_cast<const T*>(a.dout) + b * a.pdo.b + (int64_t)kv * a.rep * a.pdo.head;
-  const int qt = (int)(a.pq.t * sizeof(T)), qh = (int)(a.pq.head * sizeof(T)),
-            dt = (int)(a.pdo.t * sizeof(T)), dh = (int)(a.pdo.head * sizeof(T));
-  Loader<T, kD, kRows, kWaves> loader;
-  loader.init(a.h, w, lane);
-  const uint32_t lds0 = lds_addr(lds_dyn);
-  const float* lse = a.lse + (int64_t)bk * a.rows;
-  const float* delta = a.delta + (int64_t)bk * a.rows;
-  auto fetch = [&](int i) __attribute__((always_inline)) {
-    const int64_t r = r0 + (int64_t)i * kRows;
-    const int t = (int)(r / a.rep), g0 = (int)(r - (int64_t)t * a.rep);
-    const int limit = (int)min((int64_t)kRows, r1 - r);
-    const uint32_t at = lds0 + (i & 1) * 2 * kBytes;
-    loader.shared(qbase + (int64_t)t * a.pq.t, g0, a.rep, inv, qt, qh, limit, at, w);
-    loader.shared(dbase + (int64_t)t * a.pdo.t, g0, a.rep, inv, dt, dh, limit, at + kBytes, w);
-    // (Rows past the last are zeros in all four: p = 1, and nothing comes of it.)
-    if (w < 2)
-      dma4(wave_buffer((w ? delta : lse) + r, limit * 4), __builtin_amdgcn_readfirstlane(lds0 + 4 * kBytes + (i & 1) * 512 + w * 256),
-           lane * 4, 0);
+  Loader<T, kD, kRows, kWaves> qload, dload;
+  int unit[Loader<T, kD, kRows, kWaves>::kCount];  // a row's token (or head) in the tile
+#pragma unroll
+  for (int j = 0; j < qload.kCount; ++j) {
+    const int r = qload.row(j, w, lane), c = qload.chunk(j, a.h, w, lane);
+    const int t = grouped ? a.by_rep.of(r) : 0, g = r - t * a.rep;
+    unit[j] = grouped ? t : g;
+    const bool on = c != kOutOfRange && t < tiles.tokens;
+    qload.voff[j] = on ? (int)((t * a.pq.t + g * a.pq.head) * sizeof(T)) + c : kOutOfRange;
+    dload.voff[j] = on ? (int)((t * a.pdo.t + g * a.pdo.head) * sizeof(T)) + c : kOutOfRange;
+  }
+  const uint32_t lds_base = lds_addr(lds_dyn);
+  const int64_t stat0 = (int64_t)bk * a.rows;
+  // Tile (t, c): tokens from t on (heads from c kRows on).  Rows past the last are zeros in
+  // all of their operands, and so is what comes of them.
+  auto fetch = [&](int t, int c, int stage) __attribute__((always_inline)) {
+    const uint32_t at = lds_base + stage * Sh::kStage;
+    const int left = grouped ? tb - t + 1 : a.rep - c * kRows;  // tokens, or heads
+    const int full = grouped ? tiles.tokens : kRows;
+    const u32x4_t qb = wave_buffer(qbase + t * a.pq.t + c * kRows * a.pq.head, kBufferBytes),
+                  db = wave_buffer(dbase + t * a.pdo.t + c * kRows * a.pdo.head, kBufferBytes);
+#pragma unroll
+    for (int j = 0; j < qload.kCount; ++j) {
+      const uint32_t to = uniform(at + (w + kWaves * j) * 1024);
+      const bool on = unit[j] < left;
+      dma16(qb, to, on ? qload.voff[j] : kOutOfRange, 0);
+      dma16(db, to + kBytes, on ? dload.voff[j] : kOutOfRange, 0);
+    }
+    // (One transfer a wave, so that all of them count the same.)
+#pragma unroll
+    for (int x = 0; x < (kWaves == 1 ? 3 : 1); ++x) {
+      const int which = kWaves == 1 ? x : w;
+      const bool some = which < (sizeof(T) == 4 ? 3 : 2);
+      const float* from = (which == 0 ? a.lse : which == 1 ? a.delta : a.inv);
+      const int count = some ? min(left, full) * (grouped ? a.rep : 1) : 0;
+      dma4(wave_buffer(some ? from + stat0 + t * a.rep + c * kRows : a.lse, count * 4),
+           uniform(at + 2 * kBytes + min(which, 3) * 256), lane * 4, 0);
+    }
   };
-  if (n > 0) fetch(0);
-  for (int i = 0; i < n; ++i) {
-    transfers_done();
+  constexpr int kCount = 2 * decltype(qload)::kCount + (kWaves == 1 ? 3 : 1);
+  int ft = ta, fc = 0, t = ta, c = 0;  // the tile that is fetched next, and the current one
+  auto next = [&](int* t, int* c) __attribute__((always_inline)) {
+    if (++*c >= tiles.chunks) {
+      *c = 0;
+      *t += tiles.tokens;
+    }
+  };
+  // (Past the last tile: that again.)
+  auto fetch_next = [&](int stage) __attribute__((always_inline)) {
+    fetch(ft, fc, stage);
+    if (ft + tiles.tokens <= tb || fc + 1 < tiles.chunks) next(&ft, &fc);
+  };
+  if (n > 0) {
+#pragma unroll
+    for (int i = 0; i < kNext; ++i) fetch_next(i);
+  }
+  RowFrags<T, kD> k, v;
+  if constexpr (Sh::kHold) {
+    load_row<T, kD>(k, krow, seen, a.h, lane);
+    load_row<T, kD>(v, vrow, seen, a.h, lane);
+  }
+  f32x16_t dk[X::kBlocks] = {}, dv[X::kBlocks] = {};
+  Walk<(sizeof(T) == 2 ? kD : 64)> walk;
+  if constexpr (sizeof(T) == 2) walk.init(lane);
+  const int stat_at = (int)lds_base + 16 * (lane >> 5);
+
+  auto step = [&](int i, int stage) __attribute__((always_inline)) {
+    transfers_left<(kNext - 1) * kCount>();
     __syncthreads();
-    if (i + 1 < n) fetch(i + 1);
-    const int64_t r = r0 + (int64_t)i * kRows;
-    const int ti = (int)(r / a.rep), tj = min(tb, (int)((r + kRows - 1) / a.rep));
-    if (jw > sight.hi(tj) || jw + kRowsWave <= sight.lo(ti) || jw >= sight.len) continue;
-    const bool whole = jw >= sight.lo(tj) && jw + kRowsWave - 1 <= sight.hi(ti) &&
-                       jw + kRowsWave <= sight.len;
-    const uint8_t* qt_ = lds_dyn + (i & 1) * 2 * kBytes;
-    const uint8_t* dt_ = qt_ + kBytes;
-    const float* st = reinterpret_cast<const float*>(lds_dyn + 4 * kBytes + (i & 1) * 512);
-#pragma unroll
-    for (int e = 0; e < kRows / 32; ++e) {
-      if constexpr (!Sh::kHold) load_row<T, kD>(k, krow, seen, a.h, lane);
-      f32x16_t s = times_rows<T, kD>(qt_, 32 * e, k, lane);
-      f32x4_t ls[4], dl[4];
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        const int at = 32 * e + 8 * x + 4 * (lane >> 5);
-        ls[x] = *reinterpret_cast<const f32x4_t*>(st + at);
-        dl[x] = *reinterpret_cast<const f32x4_t*>(st + 64 + at);
-      }
-#pragma unroll
-      for (int x = 0; x < 16; ++x)
-        s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], a.c, -ls[x >> 2][x & 3]));
-      if (!whole) {
-        const int g0 = (int)(r - (int64_t)ti * a.rep);
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const int at = g0 + 32 * e + 8 * (x >> 2) + 4 * (lane >> 5) + (x & 3);
-          int t = (int)((float)at * inv);
-          t -= t * a.rep > at;
-          t += (t + 1) * a.rep <= at;
-          t += ti;
-          if (key < sight.lo(t) || key > sight.hi(t)) s[x] = 0.f;
-        }
-      }
-      add_columns<T, kD>(dv, dt_, 32 * e, s, lane);
-      if constexpr (!Sh::kHold) load_row<T, kD>(v, vrow, seen, a.h, lane);
-      const f32x16_t dp = times_rows<T, kD>(dt_, 32 * e, v, lane);
+    fetch_next((stage + kNext) % kStages);
+    const int ti = t, tj = min(tb, t + tiles.tokens - 1);
+    next(&t, &c);
+    const int lo_i = sight.lo(ti), lo_j = sight.lo(tj), hi_i = sight.hi(ti), hi_j = sight.hi(tj);
+    if (jw > hi_j || jw + kRowsWave <= lo_i || jw >= sight.len) return;
+    const bool whole = jw >= lo_j && jw + kRowsWave - 1 <= hi_i;
+    const int qt = stage * Sh::kStage, dt = qt + kBytes, st = dt + kBytes;
+    f32x16_t s[kParts] = {}, dp[kParts];
+    auto quad = [&](int which, int e, int x) __attribute__((always_inline)) {
+      return lds_read<f32x4_t>(stat_at + (st + which * 256 + (32 * e + 8 * x) * 4));
+    };
+    // Probabilities of rows that do not see the key: zero (and then so is ds).
+    auto masked = [&](f32x16_t& p, f32x16_t& ds, int e) __attribute__((always_inline)) {
 #pragma unroll
       for (int x = 0; x < 16; ++x) {
-        const float ds = s[x] * (dp[x] - dl[x >> 2][x & 3]);
-        s[x] = s[x] == 0.f ? 0.f : ds;
+        const int at = ti + (grouped ? a.by_rep.of(32 * e + column_row(x, lane)) : 0);
+        if (key < sight.lo(at) || key > sight.hi(at)) p[x] = ds[x] = 0.f;
       }
-      add_columns<T, kD>(dk, qt_, 32 * e, s, lane);
+    };
+    if constexpr (sizeof(T) == 2) {
+      constexpr int kRowsRead = 2 * X::kPairs, kFront = kParts * kRowsRead,
+                    kCols = 4 * X::kBlocks, kHalf = 2 * X::kBlocks;
+      u32x4_t ring[kAhead];
+      // Fragment u of the tile: of each block of 32 rows the queries' rows and the output
+      // gradients', then of each block the gradients' columns and the queries'.
+      auto read = [&](int u) __attribute__((always_inline)) {
+        if (u < kFront) {
+          const int x = u % kRowsRead;
+          ring[u % kAhead] = walk.row(x < X::kPairs ? qt : dt, u / kRowsRead, x % X::kPairs);
+        } else if (u < kFront + kParts * kCols) {
+          const int x = (u - kFront) % kCols;
+          ring[u % kAhead] = walk.col(x < kHalf ? dt : qt, (u - kFront) / kCols,
+                                      x / X::kBlocks % 2, x % X::kBlocks);
+        }
+      };
+      // The output gradients' product starts at -D.
+      f32x4_t ls[4];
+      auto take_lse = [&](int e) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) ls[x] = quad(0, e, x);
+      };
+      auto take_d = [&](int e) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          const f32x4_t d = quad(1, e, x >> 2);
+          dp[e][x] = d[x & 3];
+        }
+      };
+      // s becomes p, dp becomes ds.
+      auto element = [&](int e, int x) __attribute__((always_inline)) {
+        s[e][x] = __builtin_amdgcn_exp2f(fmaf(s[e][x], a.c, -ls[x >> 2][x & 3]));
+        dp[e][x] *= s[e][x];
+      };
+      DPC_WALL();
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) read(u);
+      take_lse(0);
+      DPC_WALL();
+#pragma unroll
+      for (int e = 0; e < kParts; ++e) {
+        take_d(e);
+#pragma unroll
+        for (int x = 0; x < kRowsRead; ++x) {
+          const int u = e * kRowsRead + x, i = x % X::kPairs;
+          if (x < X::kPairs)
+            s[e] = mma_bf16(ring[u % kAhead], k.v[i], s[e]);
+          else
+            dp[e] = mma_bf16(ring[u % kAhead], v.v[i], dp[e]);
+          read(u + kAhead);
+          if (e > 0) {
+#pragma unroll
+            for (int y = x * 16 / kRowsRead; y < (x + 1) * 16 / kRowsRead; ++y) element(e - 1, y);
+          }
+          DPC_WALL();
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kParts; ++e) {
+        if (kParts == 1) {
+#pragma unroll
+          for (int y = 0; y < 16; ++y) element(e, y);
+        }
+        if (!whole) masked(s[e], dp[e], e);
+        const u32x4_t p[4] = {packed_half(s[e], 0), packed_half(s[e], 1), packed_half(dp[e], 0),
+                              packed_half(dp[e], 1)};
+        if (e + 1 < kParts) take_lse(e + 1);
+        DPC_WALL();
+#pragma unroll
+        for (int x = 0; x < kCols; ++x) {
+          const int u = kFront + e * kCols + x, d = x % X::kBlocks;
+          if (x < kHalf)
+            dv[d] = mma_bf16(ring[u % kAhead], p[x / X::kBlocks], dv[d]);
+          else
+            dk[d] = mma_bf16(ring[u % kAhead], p[x / X::kBlocks], dk[d]);
+          read(u + kAhead);
+          if (e + 1 < kParts) {
+#pragma unroll
+            for (int y = x * 16 / kCols; y < (x + 1) * 16 / kCols; ++y) element(e + 1, y);
+          }
+          DPC_WALL();
+        }
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kParts; ++e) {
+        if constexpr (!Sh::kHold) load_row<T, kD>(k, krow, seen, a.h, lane);
+        s[e] = times_rows<kD>(qt, 32 * e, k, lane);
+        if constexpr (!Sh::kHold) load_row<T, kD>(v, vrow, seen, a.h, lane);
+        dp[e] = times_rows<kD>(dt, 32 * e, v, lane);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+          s[e][x] = __builtin_amdgcn_exp2f(fmaf(s[e][x], a.c, -quad(0, e, x >> 2)[x & 3])) *
+                    quad(2, e, x >> 2)[x & 3];
+          dp[e][x] = s[e][x] * (dp[e][x] + quad(1, e, x >> 2)[x & 3]);
+        }
+        if (!whole) masked(s[e], dp[e], e);
+        add_columns<kD>(dv, dt, 32 * e, s[e], lane);
+        add_columns<kD>(dk, qt, 32 * e, dp[e], lane);
+      }
     }
+  };
+  for (int i = 0; i < n; i += kStages) {
+#pragma unroll
+    for (int x = 0; x < kStages; ++x)
+      if (x == 0 || i + x < n) step(i + x, x);
   }
-  const int64_t flat = ((int64_t)(b * (int64_t)a.S + key) * a.KV + kv) * a.h;
-  store_row<T, kD>(static_cast<T*>(a.dk) + flat, dk, a.scale, seen, there, a.h, lane);
-  store_row<T, kD>(static_cast<T*>(a.dv) + flat, dv, 1.f, seen, there, a.h, lane);
+  transfers_left<0>();
+  const int64_t flat = (((int64_t)b * a.S + key) * a.KV + kv) * a.h;
+  store_row<T, kD>(static_cast<T*>(a.dk) + flat, nullptr, dk, a.scale, seen, there, a.h, lane);
+  store_row<T, kD>(static_cast<T*>(a.dv) + flat, nullptr, dv, 1.f, seen, there, a.h, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -737,57 +1117,84 @@ __global__ void __launch_bounds__(256, 1) attn_dkv_kernel(AttnArgs a) {
 
 constexpr int kUnits = 256;
 
+Divisor divisor(int d) {
+  int s = 0;
+  while ((1ll << s) < d) ++s;
+  return Divisor{(uint32_t)(((1ull << (31 + s)) + d - 1) / d), 31 + s, d};
+}
+
+// Key heads of an XCD, and as many of them at a time as make four rounds of its 32 units.
+void spread(AttnArgs& a, int tiles) {
+  const int heads = a.B * a.KV;
+  a.per_xcd = heads % 8 ? 0 : heads / 8;
+  const int most = a.per_xcd ? a.per_xcd : heads, want = (a.per_xcd ? 128 : 1024) / tiles + 1;
+  a.chunk = want < most ? want : most;
+}
+
 template <typename T, int kD>
 struct Launch {
-  static constexpr int kSplitWaves = ForwardShape<T, kD>::kSplitWaves;
-  static int allow(const void* f, int bytes) {
-    if (bytes > 65536)
-      DPC_HIP_CHECK(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    return DPC_OK;
-  }
-  static int forward(AttnArgs& a, hipStream_t s) {
-    typedef ForwardShape<T, kD> Sh;
-    if (a.splits > 0) {
-      a.tiles = (int)((a.rows + kRowsWave - 1) / kRowsWave);
-      const int rc = allow((const void*)attn_forward_kernel<T, kD, true>, Sh::kSplitLds);
-      if (rc) return rc;
-      hipLaunchKernelGGL((attn_forward_kernel<T, kD, true>),
-                         dim3((unsigned)((int64_t)a.B * a.KV * a.tiles * a.splits)),
-                         dim3(64 * Sh::kSplitWaves), Sh::kSplitLds, s, a);
-      DPC_HIP_CHECK(hipGetLastError());
-      const int64_t rows = (int64_t)a.B * a.KV * a.rows;
-      hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s,
-                         a, a.splits * Sh::kSplitWaves);
-      DPC_HIP_CHECK(hipGetLastError());
-      return DPC_OK;
-    }
-    a.tiles = (int)((a.rows + 127) / 128);
-    const int rc = allow((const void*)attn_forward_kernel<T, kD, false>, Sh::kLds);
-    if (rc) return rc;
-    hipLaunchKernelGGL((attn_forward_kernel<T, kD, false>),
-                       dim3((unsigned)((int64_t)a.B * a.KV * a.tiles)), dim3(256), Sh::kLds, s, a);
+  static constexpr int kSplitWaves = SplitShape<T, kD>::kWaves;
+
+  template <typename K>
+  static int go(K kernel, AttnArgs& a, int64_t grid, int threads, int lds, hipStream_t s) {
+    if (lds > 65536)
+      DPC_HIP_CHECK(hipFuncSetAttribute((const void*)kernel,
+                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, s, a);
     DPC_HIP_CHECK(hipGetLastError());
     return DPC_OK;
   }
+  static int64_t heads(const AttnArgs& a) { return (int64_t)a.B * a.KV; }
+
+  template <int kWaves>
+  static int forward_rows(AttnArgs& a, hipStream_t s) {
+    a.tiles = (a.rows + 32 * kWaves - 1) / (32 * kWaves);
+    spread(a, a.tiles);
+    return go(attn_forward_kernel<T, kD, kWaves, false>, a, heads(a) * a.tiles, 64 * kWaves,
+              RowsShape<T, kD, kWaves>::kLds, s);
+  }
+  static int forward(AttnArgs& a, hipStream_t s) {
+    if (a.splits == 0) return forward_rows<kMostWaves<T, kD>>(a, s);
+    a.tiles = (a.rows + kRowsWave - 1) / kRowsWave;
+    a.by_splits = divisor(a.splits);
+    spread(a, a.tiles * a.splits);
+    const int rc = go(attn_forward_kernel<T, kD, kSplitWaves, true>, a,
+                      heads(a) * a.tiles * a.splits, 64 * kSplitWaves, SplitShape<T, kD>::kLds, s);
+    if (rc) return rc;
+    const int64_t rows = heads(a) * a.rows;
+    hipLaunchKernelGGL((attn_join_kernel<T>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a,
+                       a.splits * kSplitWaves);
+    DPC_HIP_CHECK(hipGetLastError());
+    return DPC_OK;
+  }
+
+  template <int kWaves>
+  static int dq(AttnArgs& a, hipStream_t s) {
+    a.tiles = (a.rows + 32 * kWaves - 1) / (32 * kWaves);
+    spread(a, a.tiles);
+    return go(attn_dq_kernel<T, kD, kWaves>, a, heads(a) * a.tiles, 64 * kWaves,
+              RowsShape<T, kD, kWaves>::kLds, s);
+  }
+  template <int kWaves>
+  static int dkv(AttnArgs& a, hipStream_t s) {
+    a.tiles = (a.S + 32 * kWaves - 1) / (32 * kWaves);
+    spread(a, a.tiles);
+    return go(attn_dkv_kernel<T, kD, kWaves>, a, heads(a) * a.tiles, 64 * kWaves,
+              KeysShape<T, kD, kWaves>::kLds, s);
+  }
+  // The widest tiles that give every compute unit one; else the narrowest.
+  static bool fills(const AttnArgs& a, int64_t n, int waves) {
+    return heads(a) * ((n + 32 * waves - 1) / (32 * waves)) >= kUnits;
+  }
   static int backward(AttnArgs& a, hipStream_t s) {
     if (a.rows > 0) {
-      a.tiles = (int)((a.rows + 127) / 128);
-      constexpr int kLds = ForwardShape<T, kD>::kLds;
-      const int rc = allow((const void*)attn_dq_kernel<T, kD>, kLds);
+      constexpr int kMost = kMostWaves<T, kD>;
+      const int rc = fills(a, a.rows, kMost) ? dq<kMost>(a, s)
+                     : fills(a, a.rows, 4)   ? dq<4>(a, s)
+                                             : dq<1>(a, s);
       if (rc) return rc;
-      hipLaunchKernelGGL((attn_dq_kernel<T, kD>),
-                         dim3((unsigned)((int64_t)a.B * a.KV * a.tiles)), dim3(256), kLds, s, a);
-      DPC_HIP_CHECK(hipGetLastError());
     }
-    if (a.S > 0 && a.dk) {
-      a.tiles = (a.S + 127) / 128;
-      constexpr int kLds = KeysShape<T, kD>::kLds;
-      const int rc = allow((const void*)attn_dkv_kernel<T, kD>, kLds);
-      if (rc) return rc;
-      hipLaunchKernelGGL((attn_dkv_kernel<T, kD>),
-                         dim3((unsigned)((int64_t)a.B * a.KV * a.tiles)), dim3(256), kLds, s, a);
-      DPC_HIP_CHECK(hipGetLastError());
-    }
+    if (a.S > 0 && a.dk) return fills(a, a.S, 4) ? dkv<4>(a, s) : dkv<1>(a, s);
     return DPC_OK;
   }
 };
@@ -818,14 +1225,15 @@ bool valid_sizes(int64_t B, int64_t T, int64_t S, int H, int KV, int h, int dtyp
   if (B > (1ll << 30)) return false;
   // Workgroups of a launch, by rows, by keys, and by rows in splits.
   const int64_t most = INT32_MAX, rows = T * (H / KV);
-  return B * KV <= most / ((rows + 31) / 32 + 1) && B * KV <= most / ((S + 127) / 128 + 1);
+  if (rows > 1 << 30) return false;
+  return B * KV <= most / ((rows + 31) / 32 + 1) && B * KV <= most / ((S + 31) / 32 + 1);
 }
 
 // Splits of the keys (0: none): where whole row tiles would leave compute units idle,
 // enough workgroups of 32 rows for two rounds, none with fewer than four tiles of 32 keys a wave.
 int splits_of(int64_t B, int64_t T, int64_t S, int H, int KV, int h, int dtype) {
   const int64_t rows = T * (H / KV), heads = B * KV;
-  if (heads * ((rows + 127) / 128) >= kUnits) return 0;
+  if (heads * ((rows + 255) / 256) >= kUnits) return 0;
   const int64_t groups = heads * ((rows + 31) / 32);
   int64_t n = (2 * kUnits + groups - 1) / groups;
   const int64_t most = S / (32 * 4 * (h * (dtype == DPC_F32 ? 4 : 2) <= 256 ? 4 : 1));
@@ -837,8 +1245,10 @@ int splits_of(int64_t B, int64_t T, int64_t S, int H, int KV, int h, int dtype) 
 
 namespace {
 
-int tensor_places(const int64_t* s, int bytes, int rep, Places* p) {
+// `rows`: of keys and values, of which more than one may not overlap.
+int tensor_places(const int64_t* s, int bytes, int rep, int64_t rows, int h, Places* p) {
   *p = Places{s[0], s[1], s[2]};
+  if (rows > 1 && s[1] < h) return DPC_ENOTSUP;
   const int64_t most = (int64_t)kOutOfRange - (1 << 20);
   if (s[1] < 0 || s[2] < 0 || s[1] > most || s[2] > most) return DPC_ENOTSUP;
   // A tile's 64 rows (of shared key heads: 65 tokens at most) in one buffer.
@@ -848,7 +1258,25 @@ int tensor_places(const int64_t* s, int bytes, int rep, Places* p) {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
+void keep_in(AttnArgs& a, void* state, int64_t n, int dtype) {
+  if (!state) return;
+  a.lse = static_cast<float*>(state);
+  uint8_t* second = static_cast<uint8_t*>(state) + up256(n * 4);
+  if (dtype == DPC_F32)
+    a.inv = reinterpret_cast<float*>(second);
+  else
+    a.rest = reinterpret_cast<int8_t*>(second);
+}
+
 }  // namespace
+
+extern "C" size_t dpc_attention_state_bytes(int64_t B, int64_t T, int H, int h, int dtype) {
+  if (B <= 0 || T <= 0 || H <= 0 || h <= 0) return 0;
+  const size_t n = (size_t)(B * T * H);
+  return up256(n * 4) + n * (dtype == DPC_F32 ? 4 : h);
+}
 
 extern "C" size_t dpc_attention_workspace_bytes(int64_t B, int64_t T, int64_t S, int H, int KV,
                                                 int h, int dtype) {
@@ -860,8 +1288,8 @@ extern "C" size_t dpc_attention_workspace_bytes(int64_t B, int64_t T, int64_t S,
 extern "C" int dpc_attention(const void* q, const void* k, const void* v, const int64_t* strides,
                              int64_t B, int64_t T, int64_t S, int H, int KV, int h, int dtype,
                              const int64_t* lengths, const int64_t* starts, int causal, int window,
-                             double scale, void* out, float* lse, void* ws, size_t ws_bytes,
-                             void* stream) {
+                             double scale, void* out, void* state, size_t state_bytes, void* ws,
+                             size_t ws_bytes, void* stream) {
   if (!valid_sizes(B, T, S, H, KV, h, dtype) || !strides || window < 0 || (window && !causal) ||
       !((float)scale > 0.f) || !isfinite((float)scale))
     return DPC_EINVAL;
@@ -872,23 +1300,27 @@ extern "C" int dpc_attention(const void* q, const void* k, const void* v, const 
   AttnArgs a = {};
   const int bytes = dtype == DPC_F32 ? 4 : 2;
   a.rep = H / KV;
-  if (const int rc = tensor_places(strides, bytes, a.rep, &a.pq)) return rc;
-  if (const int rc = tensor_places(strides + 3, bytes, 1, &a.pk)) return rc;
-  if (const int rc = tensor_places(strides + 6, bytes, 1, &a.pv)) return rc;
+  if (const int rc = tensor_places(strides, bytes, a.rep, 0, h, &a.pq)) return rc;
+  if (const int rc = tensor_places(strides + 3, bytes, 1, S, h, &a.pk)) return rc;
+  if (const int rc = tensor_places(strides + 6, bytes, 1, S, h, &a.pv)) return rc;
   const size_t need = dpc_attention_workspace_bytes(B, T, S, H, KV, h, dtype);
-  if (ws_bytes < need) return DPC_ENOSPC;
-  if (need && (!ws || ((uintptr_t)ws & 255))) return DPC_EINVAL;
+  if (ws_bytes < need ||
+      (state && state_bytes < dpc_attention_state_bytes(B, T, H, h, dtype)))
+    return DPC_ENOSPC;
+  if ((need && (!ws || ((uintptr_t)ws & 255))) || ((uintptr_t)state & 255)) return DPC_EINVAL;
   a.q = q;
   a.k = k;
   a.v = v;
   a.o = out;
-  a.lse = lse;
+  keep_in(a, state, B * T * H, dtype);
   a.B = (int)B;
   a.T = (int)T;
   a.S = (int)S;
   a.KV = KV;
   a.h = h;
-  a.rows = T * a.rep;
+  a.rows = (int)(T * a.rep);
+  a.by_rep = divisor(a.rep);
+  a.by_kv = divisor(KV);
   a.lengths = lengths;
   a.starts = starts;
   a.causal = causal != 0;
@@ -911,26 +1343,28 @@ extern "C" int dpc_attention_grad(const void* q, const void* k, const void* v, c
                                   const void* dout, const int64_t* strides, int64_t B, int64_t T,
                                   int64_t S, int H, int KV, int h, int dtype,
                                   const int64_t* lengths, const int64_t* starts, int causal,
-                                  int window, double scale, const float* lse, void* dq, void* dk,
-                                  void* dv, void* ws, size_t ws_bytes, void* stream) {
+                                  int window, double scale, const void* state, size_t state_bytes,
+                                  void* dq, void* dk, void* dv, void* ws, size_t ws_bytes,
+                                  void* stream) {
   if (!valid_sizes(B, T, S, H, KV, h, dtype) || !strides || window < 0 || (window && !causal) ||
       !((float)scale > 0.f) || !isfinite((float)scale))
     return DPC_EINVAL;
   if (B == 0 || (T == 0 && S == 0)) return DPC_OK;
-  if ((T && (!q || !out || !dout || !lse || !dq)) || (S && (!k || !v)) || (!dk != !dv) ||
+  if ((T && (!q || !out || !dout || !state || !dq)) || (S && (!k || !v)) || (!dk != !dv) ||
       !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(dout) ||
       !aligned16(dq) || !aligned16(dk) || !aligned16(dv))
     return DPC_EINVAL;
   AttnArgs a = {};
   const int bytes = dtype == DPC_F32 ? 4 : 2;
   a.rep = H / KV;
-  if (const int rc = tensor_places(strides, bytes, a.rep, &a.pq)) return rc;
-  if (const int rc = tensor_places(strides + 3, bytes, 1, &a.pk)) return rc;
-  if (const int rc = tensor_places(strides + 6, bytes, 1, &a.pv)) return rc;
-  if (const int rc = tensor_places(strides + 9, bytes, a.rep, &a.pdo)) return rc;
+  if (const int rc = tensor_places(strides, bytes, a.rep, 0, h, &a.pq)) return rc;
+  if (const int rc = tensor_places(strides + 3, bytes, 1, S, h, &a.pk)) return rc;
+  if (const int rc = tensor_places(strides + 6, bytes, 1, S, h, &a.pv)) return rc;
+  if (const int rc = tensor_places(strides + 9, bytes, a.rep, 0, h, &a.pdo)) return rc;
   const size_t need = dpc_attention_grad_workspace_bytes(B, T, H);
-  if (ws_bytes < need) return DPC_ENOSPC;
-  if (need && (!ws || ((uintptr_t)ws & 255))) return DPC_EINVAL;
+  if (ws_bytes < need || state_bytes < dpc_attention_state_bytes(B, T, H, h, dtype))
+    return DPC_ENOSPC;
+  if ((need && (!ws || ((uintptr_t)ws & 255))) || ((uintptr_t)state & 255)) return DPC_EINVAL;
   a.q = q;
   a.k = k;
   a.v = v;
@@ -939,14 +1373,16 @@ extern "C" int dpc_attention_grad(const void* q, const void* k, const void* v, c
   a.dq = dq;
   a.dk = dk;
   a.dv = dv;
-  a.lse = const_cast<float*>(lse);
+  keep_in(a, const_cast<void*>(state), B * T * H, dtype);
   a.delta = static_cast<float*>(ws);
   a.B = (int)B;
   a.T = (int)T;
   a.S = (int)S;
   a.KV = KV;
   a.h = h;
-  a.rows = T * a.rep;
+  a.rows = (int)(T * a.rep);
+  a.by_rep = divisor(a.rep);
+  a.by_kv = divisor(KV);
   a.lengths = lengths;
   a.starts = starts;
   a.causal = causal != 0;

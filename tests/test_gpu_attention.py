@@ -4,8 +4,8 @@ Tolerances are elementwise and follow the roundings, with u = 2^-23 for a float3
 operation in any order of its sum, K terms each (K + 8) u of the sum of their magnitudes.
 A score is within es = (h + 8) u scale (|q| |k|) of its own, relative errors of
 probabilities are then ep = 2 max es + 32 u (exponential, maximum, sum).  bf16: probabilities
-and ds go to the products in bf16 (2^-8 of themselves more), D is taken of the rounded
-output (2^-8 |do| |o|), and the results are rounded (2^-8).
+and ds go to the products in bf16 (2^-8 of themselves more), and the results are rounded
+(2^-8); D is taken of the output with what that took from it, within 2^-17.
 """
 
 from __future__ import annotations
@@ -61,11 +61,12 @@ def _reference(q, k, v, up, causal=True, window=None, lengths=None, starts=None,
     o = p @ vd
     pv = p @ vd.abs()
     eo = (ep + half + (S + 8) * U) * pv
+    eD = eo + (2.0 ** -17 * o.abs() if half else 0.0)
     eo = eo + half * (o.abs() + eo)
     dp = gd @ vd.mT
     D = (gd * o).sum(-1, keepdim=True)
     edp = (h + 8) * U * (gd.abs() @ vd.abs().mT)
-    eD = (gd.abs() * eo).sum(-1, keepdim=True) + (h + 8) * U * (gd.abs() * o.abs()).sum(
+    eD = (gd.abs() * eD).sum(-1, keepdim=True) + (h + 8) * U * (gd.abs() * o.abs()).sum(
         -1, keepdim=True)
     ds = p * (dp - D)
     eds = p * (edp + eD) + (ep + half + 4 * U) * p * (dp.abs() + D.abs())
