@@ -200,31 +200,63 @@ DPC_DEVICE f32x16_t mma_bf16(u32x4_t a, u32x4_t b, f32x16_t c) {
 template <int kD>
 struct Walk {
   typedef Tile<uint16_t, kD> X;
-  int row_at[X::kPairs], col_at[2 * X::kBlocks];
-  DPC_DEVICE void init(int lane) {
-    const int row = lane & 31, sw = swizzle<X::kChunks>(row) ^ (lane >> 5);
-    const int base = (int)lds_addr(lds_dyn);
-#pragma unroll
-    for (int i = 0; i < X::kPairs; ++i) row_at[i] = base + row * X::kRow + (((2 * i) ^ sw) << 4);
+  int row0, col0[2];  // of pair 0; of block 0, either half
+  // `first`: a row that the blocks are counted from.
+  DPC_DEVICE void init(int lane, int first) {
+    const int row = lane & 31, base = (int)lds_addr(lds_dyn) + first * X::kRow;
+    row0 = base + row * X::kRow + ((swizzle<X::kChunks>(row) ^ (lane >> 5)) << 4);
     const int L = lane & 15, r = 4 * (lane >> 5) + (L >> 2);
     const int chunk = ((lane >> 4) & 1) * 2 + ((L & 3) >> 1);
 #pragma unroll
-    for (int d = 0; d < X::kBlocks; ++d)
+    for (int half = 0; half < 2; ++half)
+      col0[half] = base + (r + 8 * half) * X::kRow +
+                   ((chunk ^ swizzle<X::kChunks>(r + 8 * half)) << 4) + (L & 1) * 8;
+  }
+  // The places of a phase's reads, made for it: kept, they would take the registers that
+  // keep operands from spilling.  (The swizzle turns bits of the chunk's place alone.)
+  struct Rows {
+    int at[X::kPairs];
+  };
+  struct Cols {
+    int at[2 * X::kBlocks];
+  };
+  DPC_DEVICE Rows rows() const {
+    Rows r;
+    int from = row0;
+    asm volatile("" : "+v"(from));
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
-        col_at[2 * d + half] =
-            base + (r + 8 * half) * X::kRow +
-            (((4 * d + chunk) ^ swizzle<X::kChunks>(r + 8 * half)) << 4) + (L & 1) * 8;
+    for (int i = 0; i < X::kPairs; ++i) r.at[i] = from ^ (i << 5);
+    return r;
+  }
+  DPC_DEVICE Cols cols() const {
+    Cols r;
+    int a = col0[0], b = col0[1];
+    asm volatile("" : "+v"(a), "+v"(b));
+#pragma unroll
+    for (int d = 0; d < X::kBlocks; ++d) {
+      r.at[2 * d] = a ^ (d << 6);
+      r.at[2 * d + 1] = b ^ (d << 6);
+    }
+    return r;
+  }
+  // Pair i's place from pair 0's, which is opaque so that each use has its own.
+  DPC_DEVICE int first_row() const {
+    int from = row0;
+    asm volatile("" : "+v"(from));
+    return from;
+  }
+  static DPC_DEVICE u32x4_t row_from(int from, int at, int e, int i) {
+    return lds_read<u32x4_t>((from ^ (i << 5)) + (at + e * 32 * X::kRow));
   }
   // Block e of 32 rows of the tile at `at`.
-  DPC_DEVICE u32x4_t row(int at, int e, int i) const {
-    return lds_read<u32x4_t>(row_at[i] + (at + e * 32 * X::kRow));
+  static DPC_DEVICE u32x4_t row(const Rows& r, int at, int e, int i) {
+    return lds_read<u32x4_t>(r.at[i] + (at + e * 32 * X::kRow));
   }
   // Rows 16 j .. of block e, columns of block d.
-  DPC_DEVICE u32x4_t col(int at, int e, int j, int d) const {
+  static DPC_DEVICE u32x4_t col(const Cols& r, int at, int e, int j, int d) {
     const int o = at + (32 * e + 16 * j) * X::kRow;
-    return __builtin_bit_cast(u32x4_t, join_frag(lds_read_tr(col_at[2 * d] + o),
-                                                 lds_read_tr(col_at[2 * d + 1] + o)));
+    return __builtin_bit_cast(u32x4_t, join_frag(lds_read_tr(r.at[2 * d] + o),
+                                                 lds_read_tr(r.at[2 * d + 1] + o)));
   }
 };
 
@@ -433,6 +465,10 @@ struct RowsShape {
   static constexpr int kFit = 131072 / (2 * kBytes);
   static constexpr int kStages = kWaves == 1 ? 2 : (kFit < 4 ? kFit : 4);
   static constexpr int kLds = kStages * 2 * kBytes;
+  // Two waves a SIMD: the second half of them a product behind (see `late`), which needs a
+  // tile for one step longer.
+  static constexpr bool kLate = kWaves == 8;
+  static constexpr int kNext = kStages - (kLate ? 2 : 1);
 };
 // Keys in splits: a wave takes 32 keys at a time into LDS of its own.
 template <typename T, int kD>
@@ -447,7 +483,7 @@ constexpr int kMostWaves = sizeof(T) == 2 && kD <= 128 ? 8 : 4;
 
 // Fragments in flight between LDS and the matrix cores: a read is issued that many
 // instructions (of 32 cycles) before its product.
-constexpr int kAhead = 8;
+constexpr int kAheadRows = 8, kAheadDq = 5, kAheadKeys = 4;
 
 template <typename T, int kD, int kWaves, bool kSplit>
 __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
@@ -455,7 +491,8 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
   typedef Tile<T, kD> X;
   typedef RowsShape<T, kD, kWaves> Sh;
   constexpr int kKeys = kSplit ? 32 : Sh::kKeys, kStages = kSplit ? 2 : Sh::kStages;
-  constexpr int kBytes = kKeys * X::kRow, kParts = kKeys / 32, kNext = kStages - 1;
+  constexpr int kBytes = kKeys * X::kRow, kParts = kKeys / 32, kNext = kSplit ? 1 : Sh::kNext;
+  constexpr bool kLate = !kSplit && Sh::kLate;
   const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
   int bk, tile, split = 0;
   place_of(a, kSplit ? a.tiles * a.splits : a.tiles, &bk, &tile);
@@ -487,7 +524,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
   const int lds0 = kSplit ? w * 4 * kBytes : 0;  // in lds_dyn
   const uint32_t lds_base = lds_addr(lds_dyn);
   Walk<(sizeof(T) == 2 ? kD : 64)> walk;
-  if constexpr (sizeof(T) == 2) walk.init(lane);
+  if constexpr (sizeof(T) == 2) walk.init(lane, 0);
 
   f32x16_t o[X::kBlocks] = {};
   float m = -INFINITY, l = 0.f, l2 = 0.f;
@@ -541,76 +578,96 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
     }
     return m == -INFINITY ? 0.f : m;
   };
-  auto step = [&](int i, int stage) __attribute__((always_inline)) {
-    transfers_left<(kNext - 1) * kCount>();
-    if (!kSplit) __syncthreads();
-    fetch(i + kNext, (stage + kNext) % kStages);
-    const int j0 = (first + i) * kKeys;
-    if (j0 > mine.hi || j0 + kKeys <= mine.lo) return;
-    const int kt = lds0 + stage * 2 * kBytes, vt = kt + kBytes;
-    f32x16_t s[kParts] = {};
+  // A tile in three: its scores, their probabilities, and the product with the values.
+  f32x16_t s[kParts];
+  u32x4_t p[2 * kParts];
+  auto front = [&](int stage) __attribute__((always_inline)) {
+    const int kt = lds0 + stage * 2 * kBytes;
+#pragma unroll
+    for (int e = 0; e < kParts; ++e) s[e] = f32x16_t{};
     if constexpr (sizeof(T) == 2) {
-      constexpr int kScores = kParts * X::kPairs, kValues = kParts * 2 * X::kBlocks;
-      u32x4_t ring[kAhead];
-      // Fragment u of the tile: the keys' rows, then the values' columns.
+      constexpr int kAll = kParts * X::kPairs;
+      const auto at = walk.rows();
+      u32x4_t ring[kAheadRows];
       auto read = [&](int u) __attribute__((always_inline)) {
-        if (u < kScores)
-          ring[u % kAhead] = walk.row(kt, u / X::kPairs, u % X::kPairs);
-        else if (u < kScores + kValues)
-          ring[u % kAhead] = walk.col(vt, (u - kScores) / (2 * X::kBlocks),
-                                      (u - kScores) / X::kBlocks % 2, (u - kScores) % X::kBlocks);
+        if (u < kAll) ring[u % kAheadRows] = walk.row(at, kt, u / X::kPairs, u % X::kPairs);
       };
       DPC_WALL();
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) read(u);
+      for (int u = 0; u < kAheadRows; ++u) read(u);
       DPC_WALL();
 #pragma unroll
-      for (int u = 0; u < kScores; ++u) {
-        s[u / X::kPairs] = mma_bf16(ring[u % kAhead], q.v[u % X::kPairs], s[u / X::kPairs]);
-        read(u + kAhead);
+      for (int u = 0; u < kAll; ++u) {
+        s[u / X::kPairs] = mma_bf16(ring[u % kAheadRows], q.v[u % X::kPairs], s[u / X::kPairs]);
+        read(u + kAheadRows);
         DPC_WALL();
-      }
-      const float from = statistics(s, j0);
-#pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        s[0][x] = __builtin_amdgcn_exp2f(fmaf(s[0][x], a.c, -from));
-        (x & 1 ? l2 : l) += s[0][x];
-      }
-      // The next block's exponentials go between this one's products.
-#pragma unroll
-      for (int e = 0; e < kParts; ++e) {
-        const u32x4_t p[2] = {packed_half(s[e], 0), packed_half(s[e], 1)};
-        DPC_WALL();
-#pragma unroll
-        for (int u = 0; u < 2 * X::kBlocks; ++u) {
-          const int at = kScores + e * 2 * X::kBlocks + u, d = u % X::kBlocks;
-          o[d] = mma_bf16(ring[at % kAhead], p[u / X::kBlocks], o[d]);
-          read(at + kAhead);
-          if (e + 1 < kParts) {
-            constexpr int kEach = 16 / (2 * X::kBlocks);
-#pragma unroll
-            for (int x = u * kEach; x < (u + 1) * kEach; ++x) {
-              s[e + 1][x] = __builtin_amdgcn_exp2f(fmaf(s[e + 1][x], a.c, -from));
-              (x & 1 ? l2 : l) += s[e + 1][x];
-            }
-          }
-          DPC_WALL();
-        }
       }
     } else {
 #pragma unroll
       for (int e = 0; e < kParts; ++e) s[e] = times_rows<kD>(kt, 32 * e, q, lane);
-      const float from = statistics(s, j0);
+    }
+  };
+  auto middle = [&](int i) __attribute__((always_inline)) {
+    const float from = statistics(s, (first + i) * kKeys);
 #pragma unroll
-      for (int e = 0; e < kParts; ++e) {
+    for (int e = 0; e < kParts; ++e) {
 #pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          s[e][x] = __builtin_amdgcn_exp2f(fmaf(s[e][x], a.c, -from));
-          l += s[e][x];
-        }
-        add_columns<kD>(o, vt, 32 * e, s[e], lane);
+      for (int x = 0; x < 16; ++x) {
+        s[e][x] = __builtin_amdgcn_exp2f(fmaf(s[e][x], a.c, -from));
+        (x & 1 ? l2 : l) += s[e][x];
+      }
+      if constexpr (sizeof(T) == 2) {
+        p[2 * e] = packed_half(s[e], 0);
+        p[2 * e + 1] = packed_half(s[e], 1);
       }
     }
+  };
+  auto back = [&](int stage) __attribute__((always_inline)) {
+    const int vt = lds0 + stage * 2 * kBytes + kBytes;
+    if constexpr (sizeof(T) == 2) {
+      constexpr int kAll = 2 * kParts * X::kBlocks;
+      const auto at = walk.cols();
+      u32x4_t ring[kAheadRows];
+      auto read = [&](int u) __attribute__((always_inline)) {
+        if (u < kAll)
+          ring[u % kAheadRows] = walk.col(at, vt, u / (2 * X::kBlocks), u / X::kBlocks % 2, u % X::kBlocks);
+      };
+      DPC_WALL();
+#pragma unroll
+      for (int u = 0; u < kAheadRows; ++u) read(u);
+      DPC_WALL();
+#pragma unroll
+      for (int u = 0; u < kAll; ++u) {
+        o[u % X::kBlocks] = mma_bf16(ring[u % kAheadRows], p[u / X::kBlocks], o[u % X::kBlocks]);
+        read(u + kAheadRows);
+        DPC_WALL();
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kParts; ++e) add_columns<kD>(o, vt, 32 * e, s[e], lane);
+    }
+  };
+  // Two waves a SIMD take turns: the first half of them have products (of the last tile's
+  // probabilities, then scores) while the second have probabilities to form of the scores
+  // that they left the step before, and then the other way round.  In step with each
+  // other both would wait for the same unit.  One wave a SIMD goes tile by tile.
+  const bool late = kLate && w >= kWaves / 2;
+  bool pending = false;  // a tile is not through
+  auto step = [&](int i, int stage) __attribute__((always_inline)) {
+    transfers_left<(kNext - 1) * kCount>();
+    if (!kSplit) __syncthreads();
+    const int before = (stage + kStages - 1) % kStages, j0 = (first + i) * kKeys;
+    const bool now = !(j0 > mine.hi || j0 + kKeys <= mine.lo);
+    if (late || !kLate) fetch(i + kNext, (stage + kNext) % kStages);
+    if (kLate && pending) {
+      if (late) middle(i - 1);
+      back(before);
+    }
+    if (now) front(stage);
+    if (kLate && !late) fetch(i + kNext, (stage + kNext) % kStages);
+    if (now && !late) middle(i);
+    if (now && !kLate) back(stage);
+    pending = now;
   };
   if (n > 0) {
 #pragma unroll
@@ -620,6 +677,13 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
 #pragma unroll
     for (int x = 0; x < kStages; ++x)
       if (x == 0 || i + x < n) step(i + x, x);
+  }
+  if (kLate && pending) {
+    if (late) middle(n - 1);
+    const int stage = uniform((n - 1) % kStages);
+#pragma unroll
+    for (int x = 0; x < kStages; ++x)
+      if (x == stage) back(x);
   }
   transfers_left<0>();  // none may land in LDS that is another's
   l = sum_halves(l + l2);
@@ -701,7 +765,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
   typedef Tile<T, kD> X;
   typedef RowsShape<T, kD, kWaves> Sh;
   constexpr int kKeys = Sh::kKeys, kBytes = Sh::kBytes, kStages = Sh::kStages;
-  constexpr int kParts = kKeys / 32, kNext = kStages - 1;
+  constexpr int kParts = kKeys / 32, kNext = Sh::kNext;
   const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
   int bk, tile;
   place_of(a, a.tiles, &bk, &tile);
@@ -770,87 +834,127 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
   const float lse = me.sees ? a.lse[row] : INFINITY;
   const float inv = sizeof(T) == 4 && me.sees ? a.inv[row] : 0.f;
   Walk<(sizeof(T) == 2 ? kD : 64)> walk;
-  if constexpr (sizeof(T) == 2) walk.init(lane);
+  if constexpr (sizeof(T) == 2) walk.init(lane, 0);
   f32x16_t dq[X::kBlocks] = {};
 
-  auto step = [&](int i, int stage) __attribute__((always_inline)) {
-    transfers_left<(kNext - 1) * kCount>();
-    __syncthreads();
-    fetch(i + kNext, (stage + kNext) % kStages);
-    const int j0 = (first + i) * kKeys;
-    if (j0 > mine.hi || j0 + kKeys <= mine.lo) return;
-    const bool whole = j0 >= mine.lo_all && j0 + kKeys - 1 <= mine.hi_all;
+  // A tile in three: the two products, ds of them, and its product.
+  f32x16_t s[kParts], dp[kParts];
+  u32x4_t p[2 * kParts];
+  auto front = [&](int stage) __attribute__((always_inline)) {
     const int kt = stage * 2 * kBytes, vt = kt + kBytes;
-    auto masked = [&](f32x16_t& x, int e) __attribute__((always_inline)) {
-      const int from = j0 + 32 * e + 4 * (lane >> 5) - me.lo;
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if ((uint32_t)(from + 8 * (i >> 2) + (i & 3)) > (uint32_t)me.span) x[i] = 0.f;
-    };
     if constexpr (sizeof(T) == 2) {
-      // Fragment u of a block of 32 keys: the keys' rows, the values', the keys' columns.
-      constexpr int kFront = 2 * X::kPairs, kCols = 2 * X::kBlocks, kAll = kFront + kCols;
-      u32x4_t ring[kAhead];
+      // Fragment u: of each block of 32 keys the keys' rows, then the values'.
+      constexpr int kFront = 2 * X::kPairs;
+      const auto at = walk.rows();
+      u32x4_t ring[kAheadDq];
       auto read = [&](int u) __attribute__((always_inline)) {
-        const int e = u / kAll, v = u % kAll, c = v - kFront;
-        if (e >= kParts) return;
-        ring[u % kAhead] = v < kFront
-            ? walk.row(v < X::kPairs ? kt : vt, e, v % X::kPairs)
-            : walk.col(kt, e, c / X::kBlocks % 2, c % X::kBlocks);
+        const int e = u / kFront, v = u % kFront;
+        if (e < kParts)
+          ring[u % kAheadDq] = walk.row(at, v < X::kPairs ? kt : vt, e, v % X::kPairs);
       };
       DPC_WALL();
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) read(u);
+      for (int u = 0; u < kAheadDq; ++u) read(u);
       DPC_WALL();
 #pragma unroll
       for (int e = 0; e < kParts; ++e) {
-        f32x16_t s = {}, dp = {};
+        s[e] = dp[e] = f32x16_t{};
 #pragma unroll
         for (int v = 0; v < kFront; ++v) {
-          const int u = e * kAll + v, i = v % X::kPairs;
+          const int u = e * kFront + v, i = v % X::kPairs;
           if (v < X::kPairs)
-            s = mma_bf16(ring[u % kAhead], q.v[i], s);
+            s[e] = mma_bf16(ring[u % kAheadDq], q.v[i], s[e]);
           else
-            dp = mma_bf16(ring[u % kAhead], dout.v[i], dp);
-          read(u + kAhead);
-          // The probabilities, once the scores are out, between the other product.
-          if (v >= X::kPairs) {
-#pragma unroll
-            for (int x = i * 16 / X::kPairs; x < (i + 1) * 16 / X::kPairs; ++x)
-              s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], a.c, -lse));
-          }
-          DPC_WALL();
-        }
-#pragma unroll
-        for (int x = 0; x < 16; ++x) s[x] *= dp[x] - D;
-        if (!whole) masked(s, e);
-        const u32x4_t p[2] = {packed_half(s, 0), packed_half(s, 1)};
-        DPC_WALL();
-#pragma unroll
-        for (int v = 0; v < kCols; ++v) {
-          const int u = e * kAll + kFront + v, d = v % X::kBlocks;
-          dq[d] = mma_bf16(ring[u % kAhead], p[v / X::kBlocks], dq[d]);
-          read(u + kAhead);
+            dp[e] = mma_bf16(ring[u % kAheadDq], dout.v[i], dp[e]);
+          read(u + kAheadDq);
           DPC_WALL();
         }
       }
     } else {
 #pragma unroll
       for (int e = 0; e < kParts; ++e) {
-        f32x16_t s = times_rows<kD>(kt, 32 * e, q, lane);
-        const f32x16_t dp = times_rows<kD>(vt, 32 * e, dout, lane);
-#pragma unroll
-        for (int x = 0; x < 16; ++x)
-          s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], a.c, -lse)) * inv * (dp[x] - D);
-        if (!whole) masked(s, e);
-        add_columns<kD>(dq, kt, 32 * e, s, lane);
+        s[e] = times_rows<kD>(kt, 32 * e, q, lane);
+        dp[e] = times_rows<kD>(vt, 32 * e, dout, lane);
       }
     }
+  };
+  auto middle = [&](int i) __attribute__((always_inline)) {
+    const int j0 = (first + i) * kKeys;
+    const bool whole = j0 >= mine.lo_all && j0 + kKeys - 1 <= mine.hi_all;
+#pragma unroll
+    for (int e = 0; e < kParts; ++e) {
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        float p = __builtin_amdgcn_exp2f(fmaf(s[e][x], a.c, -lse));
+        if (sizeof(T) == 4) p *= inv;
+        s[e][x] = p * (dp[e][x] - D);
+      }
+      if (!whole) {
+        const int from = j0 + 32 * e + 4 * (lane >> 5) - me.lo;
+#pragma unroll
+        for (int x = 0; x < 16; ++x)
+          if ((uint32_t)(from + 8 * (x >> 2) + (x & 3)) > (uint32_t)me.span) s[e][x] = 0.f;
+      }
+      if constexpr (sizeof(T) == 2) {
+        p[2 * e] = packed_half(s[e], 0);
+        p[2 * e + 1] = packed_half(s[e], 1);
+      }
+    }
+  };
+  auto back = [&](int stage) __attribute__((always_inline)) {
+    const int kt = stage * 2 * kBytes;
+    if constexpr (sizeof(T) == 2) {
+      constexpr int kAll = 2 * kParts * X::kBlocks;
+      const auto at = walk.cols();
+      u32x4_t ring[kAheadDq];
+      auto read = [&](int u) __attribute__((always_inline)) {
+        if (u < kAll)
+          ring[u % kAheadDq] = walk.col(at, kt, u / (2 * X::kBlocks), u / X::kBlocks % 2, u % X::kBlocks);
+      };
+      DPC_WALL();
+#pragma unroll
+      for (int u = 0; u < kAheadDq; ++u) read(u);
+      DPC_WALL();
+#pragma unroll
+      for (int u = 0; u < kAll; ++u) {
+        dq[u % X::kBlocks] = mma_bf16(ring[u % kAheadDq], p[u / X::kBlocks], dq[u % X::kBlocks]);
+        read(u + kAheadDq);
+        DPC_WALL();
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kParts; ++e) add_columns<kD>(dq, kt, 32 * e, s[e], lane);
+    }
+  };
+  const bool late = Sh::kLate && w >= kWaves / 2;  // as in the forward
+  bool pending = false;
+  auto step = [&](int i, int stage) __attribute__((always_inline)) {
+    transfers_left<(kNext - 1) * kCount>();
+    __syncthreads();
+    const int before = (stage + kStages - 1) % kStages, j0 = (first + i) * kKeys;
+    const bool now = !(j0 > mine.hi || j0 + kKeys <= mine.lo);
+    if (late || !Sh::kLate) fetch(i + kNext, (stage + kNext) % kStages);
+    if (Sh::kLate && pending) {
+      if (late) middle(i - 1);
+      back(before);
+    }
+    if (now) front(stage);
+    if (Sh::kLate && !late) fetch(i + kNext, (stage + kNext) % kStages);
+    if (now && !late) middle(i);
+    if (now && !Sh::kLate) back(stage);
+    pending = now;
   };
   for (int i = 0; i < n; i += kStages) {
 #pragma unroll
     for (int x = 0; x < kStages; ++x)
       if (x == 0 || i + x < n) step(i + x, x);
+  }
+  if (Sh::kLate && pending) {
+    if (late) middle(n - 1);
+    const int stage = uniform((n - 1) % kStages);
+#pragma unroll
+    for (int x = 0; x < kStages; ++x)
+      if (x == stage) back(x);
   }
   transfers_left<0>();
   store_row<T, kD>(static_cast<T*>(a.dq) + flat, nullptr, dq, a.scale, me.sees, me.there, a.h,
@@ -861,7 +965,9 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
 // dk and dv: keys fixed, rows walked.
 // ---------------------------------------------------------------------------
 
-// Key tiles of kWaves x 32 keys, a wave a SIMD; stages as RowsShape's.
+// Key tiles of 32 keys a wave, or of 4 x 32 keys for 8 waves: then the wave and the one four on
+// have the same keys, and every tile's first and second 32 rows (their sums are added
+// up at the end).  Stages of row tiles as RowsShape's.
 template <typename T, int kD, int kWaves>
 struct KeysShape {
   static constexpr int kRow = Tile<T, kD>::kRow;
@@ -869,33 +975,42 @@ struct KeysShape {
   static constexpr int kBytes = kRows * kRow;
   static constexpr int kStats = 4 * 256;  // 64 of lse, -D, inv; and a place for nothing
   static constexpr int kStage = 2 * kBytes + kStats;
-  static constexpr int kFit = 135168 / kStage;
+  static constexpr bool kTwo = kWaves == 8;
+  static constexpr int kKeys = kTwo ? 128 : 32 * kWaves;
+  // Operands of a lane's key in registers, beside 2 kD / 2 of its gradients; two waves a SIMD
+  // have room for one of them, and the values stay in LDS.
+  static constexpr bool kHoldK = kRow <= 512, kHoldV = kHoldK && !kTwo;
+  static constexpr int kValues = kTwo ? kKeys * kRow : 0;
+  static constexpr int kFit = (135168 - kValues) / kStage;
   static constexpr int kStages = kWaves == 1 ? 2 : (kFit < 4 ? kFit : 4);
-  static constexpr int kLds = kStages * kStage;
-  // Keys and values of a lane in registers, beside their gradients' accumulators.
-  static constexpr bool kHold = kRow <= 512;
+  static constexpr bool kLate = kTwo;
+  static constexpr int kNext = kStages - (kLate ? 2 : 1);
+  static constexpr int kLds = kStages * kStage + kValues;
 };
 
 template <typename T, int kD, int kWaves>
-__global__ void __launch_bounds__(64 * kWaves, 1) attn_dkv_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1)) attn_dkv_kernel(AttnArgs a) {
   typedef Tile<T, kD> X;
   typedef KeysShape<T, kD, kWaves> Sh;
-  constexpr int kRows = Sh::kRows, kBytes = Sh::kBytes, kParts = kRows / 32;
-  constexpr int kStages = Sh::kStages, kNext = kStages - 1;
+  constexpr int kRows = Sh::kRows, kBytes = Sh::kBytes;
+  constexpr int kParts = kRows / 32 / (Sh::kTwo ? 2 : 1);  // of a tile, this wave's blocks
+  constexpr int kStages = Sh::kStages, kNext = Sh::kNext;
   const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
+  const int group = Sh::kTwo ? w >> 2 : 0, own = Sh::kTwo ? w & 3 : w;
   int bk, tile;  // the first keys are seen by most rows
   place_of(a, a.tiles, &bk, &tile);
   const int b = uniform(a.by_kv.of(bk)), kv = bk - b * a.KV;
   const Sight sight(a, b);
-  const int j0 = tile * kRowsWave * kWaves, jw = j0 + w * kRowsWave;
+  const int j0 = tile * Sh::kKeys, jw = j0 + own * 32;
   const int key = jw + (lane & 31);
   const bool there = key < a.S, seen = key < sight.len;
   const T* krow = static_cast<const T*>(a.k) + b * a.pk.b + kv * a.pk.head + key * a.pk.t;
-  const T* vrow = static_cast<const T*>(a.v) + b * a.pv.b + kv * a.pv.head + key * a.pv.t;
+  const T* vbase = static_cast<const T*>(a.v) + b * a.pv.b + kv * a.pv.head;
+  const T* vrow = vbase + key * a.pv.t;
 
   // The tokens that may see one of these keys.
   int ta = sight.first(0), tb = sight.last(a.T - 1);
-  const int j1 = min(j0 + kRowsWave * kWaves, sight.len) - 1;
+  const int j1 = min(j0 + Sh::kKeys, sight.len) - 1;
   if (sight.causal) {
     ta = max(ta, j0 - sight.start);
     if (sight.window) tb = min(tb, j1 + sight.window - 1 - sight.start);
@@ -910,6 +1025,14 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attn_dkv_kernel(AttnArgs a) {
 
   const T* qbase = static_cast<const T*>(a.q) + b * a.pq.b + (int64_t)kv * a.rep * a.pq.head;
   const T* dbase = static_cast<const T*>(a.dout) + b * a.pdo.b + (int64_t)kv * a.rep * a.pdo.head;
+  const uint32_t lds_base = lds_addr(lds_dyn);
+  constexpr int kValuesAt = kStages * Sh::kStage;
+  if (Sh::kTwo && n > 0) {
+    Loader<T, kD, Sh::kKeys, kWaves> vload;
+    const int stride = (int)(a.pv.t * sizeof(T));
+    vload.init(stride, a.h, w, lane);
+    vload.rows(vbase + j0 * a.pv.t, stride, sight.len - j0, a.h, lds_base + kValuesAt, w);
+  }
   Loader<T, kD, kRows, kWaves> qload, dload;
   int unit[Loader<T, kD, kRows, kWaves>::kCount];  // a row's token (or head) in the tile
 #pragma unroll
@@ -921,7 +1044,6 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attn_dkv_kernel(AttnArgs a) {
     qload.voff[j] = on ? (int)((t * a.pq.t + g * a.pq.head) * sizeof(T)) + c : kOutOfRange;
     dload.voff[j] = on ? (int)((t * a.pdo.t + g * a.pdo.head) * sizeof(T)) + c : kOutOfRange;
   }
-  const uint32_t lds_base = lds_addr(lds_dyn);
   const int64_t stat0 = (int64_t)bk * a.rows;
   // Tile (t, c): tokens from t on (heads from c kRows on).  Rows past the last are zeros in
   // all of their operands, and so is what comes of them.
@@ -967,116 +1089,71 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attn_dkv_kernel(AttnArgs a) {
     for (int i = 0; i < kNext; ++i) fetch_next(i);
   }
   RowFrags<T, kD> k, v;
-  if constexpr (Sh::kHold) {
-    load_row<T, kD>(k, krow, seen, a.h, lane);
-    load_row<T, kD>(v, vrow, seen, a.h, lane);
-  }
+  if constexpr (Sh::kHoldK) load_row<T, kD>(k, krow, seen, a.h, lane);
+  if constexpr (Sh::kHoldV) load_row<T, kD>(v, vrow, seen, a.h, lane);
   f32x16_t dk[X::kBlocks] = {}, dv[X::kBlocks] = {};
   Walk<(sizeof(T) == 2 ? kD : 64)> walk;
-  if constexpr (sizeof(T) == 2) walk.init(lane);
-  const int stat_at = (int)lds_base + 16 * (lane >> 5);
+  if constexpr (sizeof(T) == 2) walk.init(lane, group * 32);
+  const int stat_at = (int)lds_base + 16 * (lane >> 5) + 128 * group;
+  const int values_at = uniform(kValuesAt + (own - group) * 32 * X::kRow);  // (walk: group's)
 
-  auto step = [&](int i, int stage) __attribute__((always_inline)) {
-    transfers_left<(kNext - 1) * kCount>();
-    __syncthreads();
-    fetch_next((stage + kNext) % kStages);
-    const int ti = t, tj = min(tb, t + tiles.tokens - 1);
-    next(&t, &c);
-    const int lo_i = sight.lo(ti), lo_j = sight.lo(tj), hi_i = sight.hi(ti), hi_j = sight.hi(tj);
-    if (jw > hi_j || jw + kRowsWave <= lo_i || jw >= sight.len) return;
-    const bool whole = jw >= lo_j && jw + kRowsWave - 1 <= hi_i;
-    const int qt = stage * Sh::kStage, dt = qt + kBytes, st = dt + kBytes;
-    f32x16_t s[kParts] = {}, dp[kParts];
-    auto quad = [&](int which, int e, int x) __attribute__((always_inline)) {
-      return lds_read<f32x4_t>(stat_at + (st + which * 256 + (32 * e + 8 * x) * 4));
-    };
-    // Probabilities of rows that do not see the key: zero (and then so is ds).
-    auto masked = [&](f32x16_t& p, f32x16_t& ds, int e) __attribute__((always_inline)) {
-#pragma unroll
-      for (int x = 0; x < 16; ++x) {
-        const int at = ti + (grouped ? a.by_rep.of(32 * e + column_row(x, lane)) : 0);
-        if (key < sight.lo(at) || key > sight.hi(at)) p[x] = ds[x] = 0.f;
-      }
-    };
+  // A tile in three: the two products, probabilities and ds, and their products.
+  f32x16_t s[kParts], dp[kParts];
+  u32x4_t p[4 * kParts];
+  auto quad = [&](int which, int stage, int e, int x) __attribute__((always_inline)) {
+    return lds_read<f32x4_t>(stat_at + (stage * Sh::kStage + 2 * kBytes + which * 256 +
+                                        (32 * e + 8 * x) * 4));
+  };
+  auto front = [&](int stage) __attribute__((always_inline)) {
+    const int qt = stage * Sh::kStage, dt = qt + kBytes;
     if constexpr (sizeof(T) == 2) {
-      constexpr int kRowsRead = 2 * X::kPairs, kFront = kParts * kRowsRead,
-                    kCols = 4 * X::kBlocks, kHalf = 2 * X::kBlocks;
-      u32x4_t ring[kAhead];
-      // Fragment u of the tile: of each block of 32 rows the queries' rows and the output
-      // gradients', then of each block the gradients' columns and the queries'.
+      // Fragment u: of each block of 32 rows the queries' rows, then the output gradients'
+      // (and the values' before each, if they are not held).
+      constexpr int kEach = (Sh::kHoldV ? 2 : 3) * X::kPairs, kAll = kParts * kEach;
+      const int q0 = walk.first_row(), d0 = walk.first_row(), v0 = walk.first_row() + values_at;
+      u32x4_t ring[kAheadKeys];
       auto read = [&](int u) __attribute__((always_inline)) {
-        if (u < kFront) {
-          const int x = u % kRowsRead;
-          ring[u % kAhead] = walk.row(x < X::kPairs ? qt : dt, u / kRowsRead, x % X::kPairs);
-        } else if (u < kFront + kParts * kCols) {
-          const int x = (u - kFront) % kCols;
-          ring[u % kAhead] = walk.col(x < kHalf ? dt : qt, (u - kFront) / kCols,
-                                      x / X::kBlocks % 2, x % X::kBlocks);
-        }
+        if (u >= kAll) return;
+        const int e = u / kEach, x = u % kEach, y = x - X::kPairs;
+        if (x < X::kPairs)
+          ring[u % kAheadKeys] = walk.row_from(q0, qt, e, x);
+        else if (Sh::kHoldV)
+          ring[u % kAheadKeys] = walk.row_from(d0, dt, e, y);
+        else
+          ring[u % kAheadKeys] = y & 1 ? walk.row_from(d0, dt, e, y >> 1)
+                                       : walk.row_from(v0, 0, 0, y >> 1);
       };
-      // The output gradients' product starts at -D.
-      f32x4_t ls[4];
-      auto take_lse = [&](int e) __attribute__((always_inline)) {
+      DPC_WALL();
 #pragma unroll
-        for (int x = 0; x < 4; ++x) ls[x] = quad(0, e, x);
-      };
-      auto take_d = [&](int e) __attribute__((always_inline)) {
+      for (int u = 0; u < kAheadKeys; ++u) read(u);
+#pragma unroll
+      for (int e = 0; e < kParts; ++e) {
+        // The output gradients' product starts at -D.
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
-          const f32x4_t d = quad(1, e, x >> 2);
+          const f32x4_t d = quad(1, stage, e, x >> 2);
           dp[e][x] = d[x & 3];
         }
-      };
-      // s becomes p, dp becomes ds.
-      auto element = [&](int e, int x) __attribute__((always_inline)) {
-        s[e][x] = __builtin_amdgcn_exp2f(fmaf(s[e][x], a.c, -ls[x >> 2][x & 3]));
-        dp[e][x] *= s[e][x];
-      };
-      DPC_WALL();
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) read(u);
-      take_lse(0);
-      DPC_WALL();
-#pragma unroll
-      for (int e = 0; e < kParts; ++e) {
-        take_d(e);
-#pragma unroll
-        for (int x = 0; x < kRowsRead; ++x) {
-          const int u = e * kRowsRead + x, i = x % X::kPairs;
-          if (x < X::kPairs)
-            s[e] = mma_bf16(ring[u % kAhead], k.v[i], s[e]);
-          else
-            dp[e] = mma_bf16(ring[u % kAhead], v.v[i], dp[e]);
-          read(u + kAhead);
-          if (e > 0) {
-#pragma unroll
-            for (int y = x * 16 / kRowsRead; y < (x + 1) * 16 / kRowsRead; ++y) element(e - 1, y);
-          }
-          DPC_WALL();
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < kParts; ++e) {
-        if (kParts == 1) {
-#pragma unroll
-          for (int y = 0; y < 16; ++y) element(e, y);
-        }
-        if (!whole) masked(s[e], dp[e], e);
-        const u32x4_t p[4] = {packed_half(s[e], 0), packed_half(s[e], 1), packed_half(dp[e], 0),
-                              packed_half(dp[e], 1)};
-        if (e + 1 < kParts) take_lse(e + 1);
+        s[e] = f32x16_t{};
         DPC_WALL();
 #pragma unroll
-        for (int x = 0; x < kCols; ++x) {
-          const int u = kFront + e * kCols + x, d = x % X::kBlocks;
-          if (x < kHalf)
-            dv[d] = mma_bf16(ring[u % kAhead], p[x / X::kBlocks], dv[d]);
-          else
-            dk[d] = mma_bf16(ring[u % kAhead], p[x / X::kBlocks], dk[d]);
-          read(u + kAhead);
-          if (e + 1 < kParts) {
+        for (int x = 0; x < X::kPairs; ++x) {
+          const int u = e * kEach + x;
+          s[e] = mma_bf16(ring[u % kAheadKeys], k.v[x], s[e]);
+          read(u + kAheadKeys);
+          DPC_WALL();
+        }
 #pragma unroll
-            for (int y = x * 16 / kCols; y < (x + 1) * 16 / kCols; ++y) element(e + 1, y);
+        for (int x = 0; x < X::kPairs; ++x) {
+          if constexpr (Sh::kHoldV) {
+            const int u = e * kEach + X::kPairs + x;
+            dp[e] = mma_bf16(ring[u % kAheadKeys], v.v[x], dp[e]);
+            read(u + kAheadKeys);
+          } else {
+            const int u = e * kEach + X::kPairs + 2 * x;
+            dp[e] = mma_bf16(ring[(u + 1) % kAheadKeys], ring[u % kAheadKeys], dp[e]);
+            read(u + kAheadKeys);
+            read(u + 1 + kAheadKeys);
           }
           DPC_WALL();
         }
@@ -1084,31 +1161,143 @@ __global__ void __launch_bounds__(64 * kWaves, 1) attn_dkv_kernel(AttnArgs a) {
     } else {
 #pragma unroll
       for (int e = 0; e < kParts; ++e) {
-        if constexpr (!Sh::kHold) load_row<T, kD>(k, krow, seen, a.h, lane);
+        if constexpr (!Sh::kHoldK) load_row<T, kD>(k, krow, seen, a.h, lane);
         s[e] = times_rows<kD>(qt, 32 * e, k, lane);
-        if constexpr (!Sh::kHold) load_row<T, kD>(v, vrow, seen, a.h, lane);
+        if constexpr (!Sh::kHoldK) load_row<T, kD>(v, vrow, seen, a.h, lane);
         dp[e] = times_rows<kD>(dt, 32 * e, v, lane);
+      }
+    }
+  };
+  // Of the tile of tokens ti .. tj.
+  auto middle = [&](int ti, int tj, int stage) __attribute__((always_inline)) {
+    const bool whole = jw >= sight.lo(tj) && jw + kRowsWave - 1 <= sight.hi(ti);
+#pragma unroll
+    for (int e = 0; e < kParts; ++e) {
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        s[e][x] = __builtin_amdgcn_exp2f(fmaf(s[e][x], a.c, -quad(0, stage, e, x >> 2)[x & 3]));
+        if (sizeof(T) == 4) {
+          s[e][x] *= quad(2, stage, e, x >> 2)[x & 3];
+          dp[e][x] += quad(1, stage, e, x >> 2)[x & 3];
+        }
+        dp[e][x] *= s[e][x];
+      }
+      if (!whole) {  // rows that do not see the key: zero, and then so is ds
+        int r0 = 32 * (e + group) + column_row(0, lane);
+        asm volatile("" : "+v"(r0));  // (its rows' tokens are not kept between tiles)
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
-          s[e][x] = __builtin_amdgcn_exp2f(fmaf(s[e][x], a.c, -quad(0, e, x >> 2)[x & 3])) *
-                    quad(2, e, x >> 2)[x & 3];
-          dp[e][x] = s[e][x] * (dp[e][x] + quad(1, e, x >> 2)[x & 3]);
+          const int at = ti + (grouped ? a.by_rep.of(r0 + column_row(x, 0)) : 0);
+          if (key < sight.lo(at) || key > sight.hi(at)) s[e][x] = dp[e][x] = 0.f;
         }
-        if (!whole) masked(s[e], dp[e], e);
+      }
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          p[4 * e + x] = packed_half(s[e], x);
+          p[4 * e + 2 + x] = packed_half(dp[e], x);
+        }
+      }
+    }
+  };
+  auto back = [&](int stage) __attribute__((always_inline)) {
+    const int qt = stage * Sh::kStage, dt = qt + kBytes;
+    if constexpr (sizeof(T) == 2) {
+      // Fragment u: of each block the output gradients' columns, then the queries'.
+      constexpr int kHalf = 2 * X::kBlocks, kAll = 2 * kParts * kHalf;
+      const auto at = walk.cols();
+      u32x4_t ring[kAheadKeys];
+      auto read = [&](int u) __attribute__((always_inline)) {
+        const int e = u / (2 * kHalf), x = u % (2 * kHalf);
+        if (u < kAll)
+          ring[u % kAheadKeys] = walk.col(at, x < kHalf ? dt : qt, e, x / X::kBlocks % 2, x % X::kBlocks);
+      };
+      DPC_WALL();
+#pragma unroll
+      for (int u = 0; u < kAheadKeys; ++u) read(u);
+      DPC_WALL();
+#pragma unroll
+      for (int u = 0; u < kAll; ++u) {
+        const int d = u % X::kBlocks;
+        if (u % (2 * kHalf) < kHalf)
+          dv[d] = mma_bf16(ring[u % kAheadKeys], p[u / X::kBlocks], dv[d]);
+        else
+          dk[d] = mma_bf16(ring[u % kAheadKeys], p[u / X::kBlocks], dk[d]);
+        read(u + kAheadKeys);
+        DPC_WALL();
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kParts; ++e) {
         add_columns<kD>(dv, dt, 32 * e, s[e], lane);
         add_columns<kD>(dk, qt, 32 * e, dp[e], lane);
       }
     }
+  };
+  const bool late = Sh::kLate && group > 0;  // as in the forward
+  bool pending = false;
+  int pi = 0, pj = 0;  // the tokens of the tile that is not through
+  auto step = [&](int i, int stage) __attribute__((always_inline)) {
+    transfers_left<(kNext - 1) * kCount>();
+    __syncthreads();
+    const int before = (stage + kStages - 1) % kStages;
+    const int ti = t, tj = min(tb, t + tiles.tokens - 1);
+    next(&t, &c);
+    const bool now = !(jw > sight.hi(tj) || jw + kRowsWave <= sight.lo(ti) || jw >= sight.len);
+    if (late || !Sh::kLate) fetch_next((stage + kNext) % kStages);
+    if (Sh::kLate && pending) {
+      if (late) middle(pi, pj, before);
+      back(before);
+    }
+    if (now) front(stage);
+    if (Sh::kLate && !late) fetch_next((stage + kNext) % kStages);
+    if (now && !late) middle(ti, tj, stage);
+    if (now && !Sh::kLate) back(stage);
+    pending = now;
+    pi = ti;
+    pj = tj;
   };
   for (int i = 0; i < n; i += kStages) {
 #pragma unroll
     for (int x = 0; x < kStages; ++x)
       if (x == 0 || i + x < n) step(i + x, x);
   }
+  if (Sh::kLate && pending) {
+    const int stage = uniform((n - 1) % kStages);
+#pragma unroll
+    for (int x = 0; x < kStages; ++x)
+      if (x == stage) {
+        if (late) middle(pi, pj, x);
+        back(x);
+      }
+  }
   transfers_left<0>();
   const int64_t flat = (((int64_t)b * a.S + key) * a.KV + kv) * a.h;
-  store_row<T, kD>(static_cast<T*>(a.dk) + flat, nullptr, dk, a.scale, seen, there, a.h, lane);
-  store_row<T, kD>(static_cast<T*>(a.dv) + flat, nullptr, dv, 1.f, seen, there, a.h, lane);
+  if constexpr (Sh::kTwo) {
+    // The first wave of two gives its dv away and adds the other's dk to its own.
+    __syncthreads();
+    constexpr int kWords = X::kBlocks * 16;
+    static_assert(kWaves * kWords * 256 <= Sh::kLds, "LDS holds what is exchanged");
+    float* to = reinterpret_cast<float*>(lds_dyn) + w * kWords * 64 + lane;
+    const float* from = reinterpret_cast<const float*>(lds_dyn) + (w ^ 4) * kWords * 64 + lane;
+#pragma unroll
+    for (int d = 0; d < X::kBlocks; ++d)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) to[(d * 16 + x) * 64] = group ? dk[d][x] : dv[d][x];
+    __syncthreads();
+#pragma unroll
+    for (int d = 0; d < X::kBlocks; ++d)
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {
+        const float other = from[(d * 16 + x) * 64];
+        dk[d][x] = group ? other + dv[d][x] : dk[d][x] + other;
+      }
+    store_row<T, kD>(static_cast<T*>(group ? a.dv : a.dk) + flat, nullptr, dk,
+                     group ? 1.f : a.scale, seen, there, a.h, lane);
+  } else {
+    store_row<T, kD>(static_cast<T*>(a.dk) + flat, nullptr, dk, a.scale, seen, there, a.h, lane);
+    store_row<T, kD>(static_cast<T*>(a.dv) + flat, nullptr, dv, 1.f, seen, there, a.h, lane);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1177,7 +1366,8 @@ struct Launch {
   }
   template <int kWaves>
   static int dkv(AttnArgs& a, hipStream_t s) {
-    a.tiles = (a.S + 32 * kWaves - 1) / (32 * kWaves);
+    constexpr int kKeys = KeysShape<T, kD, kWaves>::kKeys;
+    a.tiles = (a.S + kKeys - 1) / kKeys;
     spread(a, a.tiles);
     return go(attn_dkv_kernel<T, kD, kWaves>, a, heads(a) * a.tiles, 64 * kWaves,
               KeysShape<T, kD, kWaves>::kLds, s);
@@ -1194,7 +1384,7 @@ struct Launch {
                                              : dq<1>(a, s);
       if (rc) return rc;
     }
-    if (a.S > 0 && a.dk) return fills(a, a.S, 4) ? dkv<4>(a, s) : dkv<1>(a, s);
+    if (a.S > 0 && a.dk) return fills(a, a.S, 4) ? dkv<kMostWaves<T, kD>>(a, s) : dkv<1>(a, s);
     return DPC_OK;
   }
 };
