@@ -624,7 +624,9 @@ int dpc_rotary(const void* q, const void* k, int64_t B, int64_t T, int H, int KV
  *   z = x w^T = [g, u] [N, 2 F],  h [N, F] = act(g) u
  * with act DPC_ACT_SILU (g / (1 + exp(-g))) or DPC_ACT_GELU (g times the normal
  * distribution function).  h is rounded once from float32; z, if not NULL, is written in
- * `dtype` for dpc_gated_linear_act_grad, which makes dz [N, 2 F] of it and dh [N, F].
+ * `dtype`, and for bf16 rest [N, 2 F] (8 bits each: what rounding took from z, so that both
+ * give z within 2^-17; fp32: NULL), for dpc_gated_linear_act_grad, which makes dz [N, 2 F] of
+ * them and dh [N, F].
  * dpc_gated_linear_grad takes dz to dx [N, D] = dz w and dw [2 F, D] =
  * dz^T x (either may be NULL; x is not read without dw, w not without dx).
  *
@@ -636,9 +638,10 @@ int dpc_rotary(const void* q, const void* k, int64_t B, int64_t T, int H, int KV
 enum { DPC_ACT_SILU = 0, DPC_ACT_GELU = 1 };
 size_t dpc_gated_linear_workspace_bytes(int64_t N, int D, int F, int dtype);
 int dpc_gated_linear(const void* x, const void* w, int64_t N, int D, int F, int dtype,
-                     int activation, void* h, void* z, void* ws, size_t ws_bytes, void* stream);
-int dpc_gated_linear_act_grad(const void* z, const void* dh, int64_t N, int F, int dtype,
-                              int activation, void* dz, void* stream);
+                     int activation, void* h, void* z, void* rest, void* ws, size_t ws_bytes,
+                     void* stream);
+int dpc_gated_linear_act_grad(const void* z, const void* rest, const void* dh, int64_t N, int F,
+                              int dtype, int activation, void* dz, void* stream);
 size_t dpc_gated_linear_grad_workspace_bytes(int64_t N, int D, int F, int dtype, int want_x,
                                              int want_w);
 int dpc_gated_linear_grad(const void* x, const void* w, const void* dz, int64_t N, int D, int F,

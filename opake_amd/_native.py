@@ -209,12 +209,11 @@ SIGNATURES = {
     "dpc_gated_linear_workspace_bytes": (_c_size_t, [_c_i64] + [_c_int] * 3),
     "dpc_gated_linear": (
         _c_int,
-        [_c_void_p, _c_void_p, _c_i64] + [_c_int] * 4 + [_c_void_p, _c_void_p, _c_void_p,
-         _c_size_t, _c_void_p],
+        [_c_void_p, _c_void_p, _c_i64] + [_c_int] * 4 + [_c_void_p] * 4 + [_c_size_t, _c_void_p],
     ),
     "dpc_gated_linear_act_grad": (
         _c_int,
-        [_c_void_p, _c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
+        [_c_void_p, _c_void_p, _c_void_p, _c_i64, _c_int, _c_int, _c_int, _c_void_p, _c_void_p],
     ),
     "dpc_gated_linear_grad_workspace_bytes": (_c_size_t, [_c_i64] + [_c_int] * 5),
     "dpc_gated_linear_grad": (

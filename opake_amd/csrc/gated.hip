@@ -15,9 +15,10 @@
 // have a shift each in the products that do not sum over them, w one for the tensor; in dw
 // the shift of a row of dz is undone in its row of x before that is shifted as a whole.
 //
-// Held in fewer than 32 bits, bf16 inputs: z as it is kept for the backward, and dz,
-// which the products take as their operand: 2^-8 of themselves at most, the size of the
-// gradients' own rounding.  h is formed from the float32 accumulators.
+// Held in fewer than 32 bits, bf16 inputs: dz, which the products take as their operand
+// (2^-8 of itself at most, the size of the gradients' own rounding).  z is kept with 8 bits
+// more than bf16 has (`rest`, 2^-17): of a z in bf16 the gradients would be 3.0e-3 from
+// 64 bits in the mean square, so 2.4e-3.  h is formed from the float32 accumulators.
 #include <math.h>
 
 #include "common.h"
@@ -30,19 +31,32 @@ constexpr float kLog2e = 1.44269504088896340736f;
 __shared__ __attribute__((aligned(16))) uint8_t lds_all[131072];
 
 // s(g), and act'(g) where asked for: act' = s + g s'.  kExact: float32's results.
+// GELU: with a = |g| / sqrt 2 the normal distribution's tail is erfc(a) / 2, and erfc(a) =
+// exp(-a^2) t P(t), t = 1 / (1 + 0.4 a), P a polynomial fitted to exp(a^2) erfc(a) / t
+// at Chebyshev's points of t for a from 0 to 35 (1.0e-7 of it at most).
 template <bool kExact>
 DPC_DEVICE float gate_of(float g, int act, float* slope) {
+  auto exp_of = [](float x) { return kExact ? expf(x) : __builtin_amdgcn_exp2f(x * kLog2e); };
+  auto over = [](float x) { return kExact ? 1.0f / x : __builtin_amdgcn_rcpf(x); };
   if (act == DPC_ACT_SILU) {
-    const float e = kExact ? expf(-g) : __builtin_amdgcn_exp2f(-g * kLog2e);
-    const float s = kExact ? 1.0f / (1.0f + e) : __builtin_amdgcn_rcpf(1.0f + e);
+    const float s = over(1.0f + exp_of(-g));
     if (slope) *slope = s * (1.0f + g * (1.0f - s));
     return s;
   }
-  const float s = 0.5f * erfcf(g * -0.70710678118654752f);
-  if (slope) {
-    const float e = kExact ? expf(-0.5f * g * g) : __builtin_amdgcn_exp2f(-0.5f * kLog2e * g * g);
-    *slope = s + g * e * 0.39894228040143267794f;
-  }
+  const float t = over(fmaf(fabsf(g), 0.4f * 0.70710678118654752f, 1.0f));
+  const float e = exp_of(-0.5f * g * g);
+  float p = 0.0469222845f;
+  p = fmaf(p, t, -0.167397184f);
+  p = fmaf(p, t, 0.138786424f);
+  p = fmaf(p, t, 0.0267844172f);
+  p = fmaf(p, t, 0.120832299f);
+  p = fmaf(p, t, 0.17646823f);
+  p = fmaf(p, t, 0.206053677f);
+  p = fmaf(p, t, 0.225884548f);
+  p = fmaf(p, t, 0.225665403f);
+  const float tail = 0.5f * p * t * e;
+  const float s = g > 0.0f ? 1.0f - tail : tail;
+  if (slope) *slope = fmaf(g * 0.39894228040143267794f, e, s);
   return s;
 }
 
@@ -200,13 +214,54 @@ struct ProductArgs {
   const uint32_t* all;  // and the tensor's, or dw's
   int act;
   void* out;         // h, dx or dw
-  void* z;           // forward: [N, 2 F], or null
+  void* z;           // forward: [N, 2 F], or null,
+  int8_t* rest;      // and bf16: what rounding took from it
   int bf16;
 };
 
 template <int kKind>
 DPC_DEVICE int tensor_shift(const uint32_t* all) {
   return -(kKind == kWeight ? mixed_shift(*all) : half_shift(*all));
+}
+
+// What rounding x to the bf16 `hi` took from it, to 8 more bits: (hi << 16) + (rest << 8)
+// as a float's bits is x within 2^-17.
+DPC_DEVICE int rest_of(float x, uint32_t hi) {
+  const int d = (int)(__float_as_uint(x) - (hi << 16));
+  return max(-128, min(127, (d + 128) >> 8));
+}
+DPC_DEVICE float with_rest(uint32_t hi, int rest) {
+  return __uint_as_float((hi << 16) + ((uint32_t)rest << 8));
+}
+
+// Quads of two neighbouring 16-column blocks, as the matrix cores leave them (lane l: columns
+// 4 (l / 16) .. of either), to 8 columns a lane, and those as bf16: first block 8 (l / 32) ..
+// for even l / 16, second for odd.  64 bytes of a row a store instead of 32.
+struct Eight {
+  u32x4_t hi;
+  uint2 rest;
+};
+DPC_DEVICE Eight eight_columns(f32x4_t a, f32x4_t b, bool want_rest) {
+  uint32_t p[4] = {f32x2_to_bf16x2_bits(a[0], a[1]), f32x2_to_bf16x2_bits(a[2], a[3]),
+                   f32x2_to_bf16x2_bits(b[0], b[1]), f32x2_to_bf16x2_bits(b[2], b[3])};
+  const auto lo = __builtin_amdgcn_permlane16_swap(p[0], p[2], false, false);
+  const auto hi = __builtin_amdgcn_permlane16_swap(p[1], p[3], false, false);
+  Eight r;
+  r.hi = u32x4_t{lo[0], hi[0], lo[1], hi[1]};
+  r.rest = make_uint2(0, 0);
+  if (want_rest) {
+    uint32_t q[2] = {};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t wa = p[e >> 1] >> (16 * (e & 1)) & 0xffffu,
+                     wb = p[2 + (e >> 1)] >> (16 * (e & 1)) & 0xffffu;
+      q[0] |= (uint32_t)(rest_of(a[e], wa) & 255) << (8 * e);
+      q[1] |= (uint32_t)(rest_of(b[e], wb) & 255) << (8 * e);
+    }
+    const auto t = __builtin_amdgcn_permlane16_swap(q[0], q[1], false, false);
+    r.rest = make_uint2(t[0], t[1]);
+  }
+  return r;
 }
 
 // Four columns f .. f + 3 of row n's g and u: z and h.
@@ -217,11 +272,42 @@ DPC_DEVICE void gated_out(const ProductArgs& s, int64_t n, int f, bool whole, f3
   if (s.z) {
     store_row4(s.z, n * 2 * F + f, left, whole, s.bf16, g);
     store_row4(s.z, n * 2 * F + F + f, left, whole, s.bf16, u);
+    if (!kHalf) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (r < left) {
+          s.rest[n * 2 * F + f + r] = (int8_t)rest_of(g[r], f32_to_bf16_bits(g[r]));
+          s.rest[n * 2 * F + F + f + r] = (int8_t)rest_of(u[r], f32_to_bf16_bits(u[r]));
+        }
+    }
   }
   f32x4_t h;
 #pragma unroll
   for (int r = 0; r < 4; ++r) h[r] = g[r] * gate_of<kHalf>(g[r], s.act, nullptr) * u[r];
   store_row4(s.out, n * F + f, left, whole, s.bf16, h);
+}
+
+// The same, bf16, of two neighbouring blocks of 16 columns: eight from f on of row n.
+DPC_DEVICE void gated_out8(const ProductArgs& s, int64_t n, int f, f32x4_t g0, f32x4_t g1,
+                           f32x4_t u0, f32x4_t u1) {
+  const int F = s.rows_a;
+  f32x4_t h0, h1;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    h0[r] = g0[r] * gate_of<false>(g0[r], s.act, nullptr) * u0[r];
+    h1[r] = g1[r] * gate_of<false>(g1[r], s.act, nullptr) * u1[r];
+  }
+  const Eight h = eight_columns(h0, h1, false);
+  const bool in = f < F;
+  if (in) *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(s.out) + n * F + f) = h.hi;
+  if (!s.z) return;
+  const Eight g = eight_columns(g0, g1, true), u = eight_columns(u0, u1, true);
+  if (!in) return;
+  const int64_t at = n * 2 * F + f;
+  *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(s.z) + at) = g.hi;
+  *reinterpret_cast<u32x4_t*>(static_cast<uint16_t*>(s.z) + at + F) = u.hi;
+  *reinterpret_cast<uint2*>(s.rest + at) = g.rest;
+  *reinterpret_cast<uint2*>(s.rest + at + F) = u.rest;
 }
 
 template <int kKind, bool kHalf>
@@ -239,6 +325,14 @@ DPC_DEVICE void product_epilogue(const ProductArgs& s, MmAcc<kKind == kHidden>& 
     const int b = b0 + 16 * j;
     if (b >= s.rows_b) continue;
     const int shift = kHalf ? all - (s.row ? half_shift(s.row[b]) : 0) : 0;
+    if constexpr (kPairs && !kHalf) {
+      if (!s.partial && s.rows_a % 8 == 0) {
+        const int f = a0 - 4 * (lane >> 4) + 16 * ((lane >> 4) & 1) + 8 * (lane >> 5);
+        gated_out8(s, b, f, acc.v[0][j], acc.v[1][j], acc.v[4][j], acc.v[5][j]);
+        gated_out8(s, b, f + 32, acc.v[2][j], acc.v[3][j], acc.v[6][j], acc.v[7][j]);
+        continue;
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kBlocks; ++i) {
       const int a = a0 + 16 * i;
@@ -316,8 +410,13 @@ __global__ void __launch_bounds__(256) gated_reduce_kernel(ProductArgs s) {
 // element's), the last vector of a row may be short.
 template <typename T, int kVec>
 __global__ void __launch_bounds__(256) gated_act_grad_kernel(const T* __restrict__ z,
+                                                             const int8_t* __restrict__ rest,
                                                              const T* __restrict__ dh, int64_t N,
                                                              int F, int act, T* __restrict__ dz) {
+  typedef int8_t bytes_t __attribute__((ext_vector_type(kVec)));
+  struct __attribute__((packed, aligned(1))) loose_bytes_t {
+    bytes_t v;
+  };
   typedef T vec_t __attribute__((ext_vector_type(kVec)));
   struct __attribute__((packed, aligned(sizeof(T)))) loose_t {
     vec_t v;
@@ -331,11 +430,17 @@ __global__ void __launch_bounds__(256) gated_act_grad_kernel(const T* __restrict
     const T *pg = z + n * 2 * F + f, *pu = pg + F, *pd = dh + n * F + f;
     T *qg = dz + n * 2 * F + f, *qu = qg + F;
     vec_t g, u, d, og, ou;
+    bytes_t rg = {}, ru = {};
+    const int8_t *prg = rest + n * 2 * F + f, *pru = prg + F;
     const bool all = f + kVec <= F;
     if (all) {
       g = reinterpret_cast<const loose_t*>(pg)->v;
       u = reinterpret_cast<const loose_t*>(pu)->v;
       d = reinterpret_cast<const loose_t*>(pd)->v;
+      if constexpr (sizeof(T) == 2) {
+        rg = reinterpret_cast<const loose_bytes_t*>(prg)->v;
+        ru = reinterpret_cast<const loose_bytes_t*>(pru)->v;
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < kVec; ++e) {
@@ -343,16 +448,25 @@ __global__ void __launch_bounds__(256) gated_act_grad_kernel(const T* __restrict
         g[e] = in ? pg[e] : T(0);
         u[e] = in ? pu[e] : T(0);
         d[e] = in ? pd[e] : T(0);
+        if constexpr (sizeof(T) == 2) {
+          rg[e] = in ? prg[e] : 0;
+          ru[e] = in ? pru[e] : 0;
+        }
       }
     }
 #pragma unroll
     for (int e = 0; e < kVec; ++e) {
       constexpr bool kExact = sizeof(T) == 4;
-      auto wide = [](T x) __attribute__((always_inline)) {
-        if constexpr (kExact) return (float)x;
-        else return bf16_bits_to_f32(x);
-      };
-      const float gf = wide(g[e]), uf = wide(u[e]), df = wide(d[e]);
+      float gf, uf, df;
+      if constexpr (kExact) {
+        gf = g[e];
+        uf = u[e];
+        df = d[e];
+      } else {
+        gf = with_rest(g[e], rg[e]);
+        uf = with_rest(u[e], ru[e]);
+        df = bf16_bits_to_f32(d[e]);
+      }
       float slope;
       const float s = gate_of<kExact>(gf, act, &slope);
       const float dg = df * uf * slope, du = df * (gf * s);
@@ -515,14 +629,14 @@ extern "C" size_t dpc_gated_linear_workspace_bytes(int64_t N, int D, int F, int 
 }
 
 extern "C" int dpc_gated_linear(const void* x, const void* w, int64_t N, int D, int F, int dtype,
-                                int activation, void* h, void* z, void* ws, size_t ws_bytes,
-                                void* stream) {
+                                int activation, void* h, void* z, void* rest, void* ws,
+                                size_t ws_bytes, void* stream) {
   if (!valid_sizes(N, D, F, dtype) ||
       (activation != DPC_ACT_SILU && activation != DPC_ACT_GELU))
     return DPC_EINVAL;
   if (N == 0) return DPC_OK;
   if (!x || !w || !h || !ws || !aligned16(x) || !aligned16(w) || !aligned16(h) || !aligned16(z) ||
-      ((uintptr_t)ws & 255))
+      !aligned16(rest) || (z && dtype == DPC_BF16 && !rest) || ((uintptr_t)ws & 255))
     return DPC_EINVAL;
   const Plan p(N, D, F, dtype, true, false, false);
   if (ws_bytes < p.total) return DPC_ENOSPC;
@@ -555,28 +669,33 @@ extern "C" int dpc_gated_linear(const void* x, const void* w, int64_t N, int D, 
   a.act = activation;
   a.out = h;
   a.z = z;
+  a.rest = static_cast<int8_t*>(rest);
   a.bf16 = !p.half;
   return product<kForward>(a, p.half, s);
 }
 
-extern "C" int dpc_gated_linear_act_grad(const void* z, const void* dh, int64_t N, int F,
-                                         int dtype, int activation, void* dz, void* stream) {
+extern "C" int dpc_gated_linear_act_grad(const void* z, const void* rest, const void* dh,
+                                         int64_t N, int F, int dtype, int activation, void* dz,
+                                         void* stream) {
   if (!valid_sizes(N, 1, F, dtype) ||
       (activation != DPC_ACT_SILU && activation != DPC_ACT_GELU))
     return DPC_EINVAL;
   if (N == 0) return DPC_OK;
-  if (!z || !dh || !dz || !aligned16(z) || !aligned16(dh) || !aligned16(dz)) return DPC_EINVAL;
+  if (!z || !dh || !dz || !aligned16(z) || !aligned16(dh) || !aligned16(dz) ||
+      (dtype == DPC_BF16 && !rest))
+    return DPC_EINVAL;
   const int vec = dtype == DPC_BF16 ? 8 : 4;
   int64_t grid = (N * ceil_div(F, vec) + 255) / 256;
   if (grid > 65536) grid = 65536;
   if (dtype == DPC_BF16)
     hipLaunchKernelGGL((gated_act_grad_kernel<uint16_t, 8>), dim3((unsigned)grid), dim3(256), 0,
                        (hipStream_t)stream, static_cast<const uint16_t*>(z),
+                       static_cast<const int8_t*>(rest),
                        static_cast<const uint16_t*>(dh), N, F, activation,
                        static_cast<uint16_t*>(dz));
   else
     hipLaunchKernelGGL((gated_act_grad_kernel<float, 4>), dim3((unsigned)grid), dim3(256), 0,
-                       (hipStream_t)stream, static_cast<const float*>(z),
+                       (hipStream_t)stream, static_cast<const float*>(z), nullptr,
                        static_cast<const float*>(dh), N, F, activation, static_cast<float*>(dz));
   DPC_HIP_CHECK(hipGetLastError());
   return DPC_OK;

@@ -25,7 +25,7 @@ _ACTIVATIONS = {"silu": nat.ACT_SILU, "gelu": nat.ACT_GELU}
 
 
 def _forward(x, weight, options, keep: bool):
-    """``h``, and the projections ``z`` where kept."""
+    """``h``, and where kept the projections ``z`` and (bfloat16) what rounding took from them."""
     code, act = options
     dev = x.device
     xa, w = _aligned(x), _aligned(weight)
@@ -33,11 +33,15 @@ def _forward(x, weight, options, keep: bool):
     N = xa.numel() // D
     h = torch.empty((*x.shape[:-1], F), dtype=x.dtype, device=dev)
     z = torch.empty((*x.shape[:-1], 2 * F), dtype=x.dtype, device=dev) if keep else None
+    rest = None
+    if keep and x.dtype == torch.bfloat16:
+        rest = torch.empty(z.shape, dtype=torch.int8, device=dev)
     ws_bytes = nat.load().dpc_gated_linear_workspace_bytes(N, D, F, code)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
     nat.call_on(dev, "dpc_gated_linear", xa.data_ptr(), w.data_ptr(), N, D, F, code, act,
-                h.data_ptr(), z.data_ptr() if keep else 0, ws.data_ptr(), ws_bytes)
-    return h, z
+                h.data_ptr(), *(0 if t is None else t.data_ptr() for t in (z, rest)), ws.data_ptr(),
+                ws_bytes)
+    return h, z, rest
 
 
 class _Project(torch.autograd.Function):
@@ -46,8 +50,8 @@ class _Project(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, options, box):
         note_leaves(ctx)
-        h, z = _forward(x, weight, options, True)
-        box.append(h)
+        h, z, rest = _forward(x, weight, options, True)
+        box += (h, rest)
         ctx.save_for_backward(x, weight)
         ctx.code = options[0]
         return z
@@ -81,20 +85,23 @@ class _Product(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, z, options, box):
-        ctx.save_for_backward(z)
+        h, rest = box
+        box.clear()
+        ctx.save_for_backward(z, rest)
         ctx.options = options
-        return box.pop()
+        return h
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh):
-        (z,) = ctx.saved_tensors
+        z, rest = ctx.saved_tensors
         code, act = ctx.options
         F = z.shape[-1] // 2
         z, dh = _aligned(z), _aligned(dh)
         dz = torch.empty_like(z)
-        nat.call_on(z.device, "dpc_gated_linear_act_grad", z.data_ptr(), dh.data_ptr(),
-                    dh.numel() // F, F, code, act, dz.data_ptr())
+        nat.call_on(z.device, "dpc_gated_linear_act_grad", z.data_ptr(),
+                    0 if rest is None else rest.data_ptr(), dh.data_ptr(), dh.numel() // F, F, code,
+                    act, dz.data_ptr())
         return dz, None, None
 
 
@@ -118,7 +125,7 @@ def _gated(x: torch.Tensor, weight: torch.Tensor, activation: str):
             f"tokens, got x {tuple(x.shape)} and weight {tuple(weight.shape)}")
     options = (nat.dtype_code(x.dtype), _ACTIVATIONS[activation])
     if not torch.is_grad_enabled() or not (x.requires_grad or weight.requires_grad):
-        return _forward(x, weight, options, False)
+        return _forward(x, weight, options, False)[:2]
     box: list = []
     z = _Project.apply(x, weight, options, box)
     return _Product.apply(z, options, box), z
@@ -130,7 +137,8 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, *,
 
     ``x`` [..., D] and ``weight`` [2 F, D] share a dtype (bfloat16 or float32).
     ``activation``: ``"silu"`` or ``"gelu"`` (with the normal distribution function).  Gradients
-    reach both; for them the projections [..., 2 F] are kept, in the inputs' dtype."""
+    reach both; for them the projections [..., 2 F] are kept, in the inputs' dtype (bfloat16: and 8
+    bits more of each)."""
     return _gated(x, weight, activation)[0]
 
 

@@ -4,8 +4,8 @@ Tolerances are elementwise and follow the roundings.  A product of K terms is wi
 (K 2^-23 + 2^-21) sum |a b| of its own: float32 sums in any order, and for float32 operands
 the two planes' 2^-21 a term.  act is 1.13-Lipschitz and act' 0.8-Lipschitz (SiLU: 1.1 and
 0.5; GELU: 1.13 and 0.8); act, act' and the products round a few times more (16 x 2^-23
-covers them, and the fast exponential and reciprocal of bf16 inputs).  bf16: the result,
-the kept projections, dz and the gradients are rounded to it, 2^-8 of each.
+covers them, and the fast exponential and reciprocal of bf16 inputs).  bf16: the result, dz
+and the gradients are rounded to it, 2^-8 of each; the projections are kept within 2^-17.
 """
 
 from __future__ import annotations
@@ -53,7 +53,8 @@ def _reference(x, w, up, act, dtype):
     h = a * u
     eh = 1.13 * eg * (u.abs() + eu) + a.abs() * eu + FEW * h.abs()
     # The backward reads z as it was kept.
-    eg, eu = _rounded(g, eg, half), _rounded(u, eu, half)
+    kept = 2.0 ** -17 if half else 0.0
+    eg, eu = _rounded(g, eg, kept), _rounded(u, eu, kept)
     dz = torch.cat([up * u * slope, up * a], 1)
     es, ea = 0.8 * eg + FEW * (slope.abs() + g.abs()), 1.13 * eg + FEW * a.abs()
     edz = torch.cat([up.abs() * ((u.abs() + eu) * es + slope.abs() * eu), up.abs() * ea], 1)
@@ -247,7 +248,7 @@ def test_entry_points_refuse(dev):
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
 
     def call(N=4, D=16, F=8, code=nat.DPC_F32, act=0, xp=x.data_ptr(), size=n):
-        return lib.dpc_gated_linear(xp, w.data_ptr(), N, D, F, code, act, h.data_ptr(), 0,
+        return lib.dpc_gated_linear(xp, w.data_ptr(), N, D, F, code, act, h.data_ptr(), 0, 0,
                                     ws.data_ptr(), size, 0)
 
     assert call(size=n - 1) == nat.DPC_ENOSPC
