@@ -474,7 +474,7 @@ struct RowsShape {
 template <typename T, int kD>
 struct SplitShape {
   static constexpr int kRow = Tile<T, kD>::kRow;
-  static constexpr int kWaves = kRow <= 256 ? 4 : (kRow == 512 ? 2 : 1);
+  static constexpr int kWaves = kRow <= 128 ? 4 : (kRow == 256 ? 2 : 1);
   static constexpr int kLds = kWaves * 4 * 32 * kRow;
 };
 // Rows of whose tiles two waves share a SIMD (256 registers each).
@@ -709,24 +709,54 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
                    me.there, a.h, lane);
 }
 
-// The splits of a row joined: one wave a row.
+// The splits of a row joined: one wave a row.  Lane p has parts p, p + 64, ... weighed
+// (kMostParts), then the wave adds up the parts' outputs, eight loads in flight.
+constexpr int kMostParts = 256;
+
+DPC_DEVICE float wave_max(float x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x = fmaxf(x, __shfl_xor(x, d));
+  return x;
+}
+DPC_DEVICE float wave_sum(float x) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+  return x;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int parts) {
-  const int lane = threadIdx.x & 63;
+  __shared__ float weights[4][kMostParts];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t n = (int64_t)a.B * a.KV * a.rows;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t row = (int64_t)blockIdx.x * 4 + w;
   if (row >= n) return;
+  float2 x[kMostParts / 64];
   float m = -INFINITY;
-  for (int p = 0; p < parts; ++p) m = fmaxf(m, a.part_ml[p * n + row].x);
+#pragma unroll
+  for (int e = 0; e < kMostParts / 64; ++e) {
+    const int p = lane + 64 * e;
+    x[e] = p < parts ? a.part_ml[p * n + row] : make_float2(-INFINITY, 0.f);
+    m = fmaxf(m, x[e].x);
+  }
+  m = wave_max(m);
   const float from = m == -INFINITY ? 0.f : m;
   float l = 0.f, o[4] = {};
-  for (int p = 0; p < parts; ++p) {
-    const float2 x = a.part_ml[p * n + row];
-    const float f = __builtin_amdgcn_exp2f(x.x - from);
-    l += x.y * f;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (lane + 64 * e < a.h) o[e] += a.part_o[(p * n + row) * a.h + lane + 64 * e] * f;
+  for (int e = 0; e < kMostParts / 64; ++e) {
+    const float f = __builtin_amdgcn_exp2f(x[e].x - from);
+    l += x[e].y * f;
+    weights[w][lane + 64 * e] = f;  // (the wave's own)
+  }
+  l = wave_sum(l);
+  const int blocks = (a.h + 63) >> 6;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (e >= blocks) break;
+    const int c = min(lane + 64 * e, a.h - 1);
+    const float* from_o = a.part_o + row * a.h + c;
+#pragma unroll 8
+    for (int p = 0; p < parts; ++p) o[e] = fmaf(from_o[p * n * a.h], weights[w][p], o[e]);
   }
   const bool some = l != 0.f;
   const int64_t bk = row / a.rows, r = row - bk * a.rows, b = bk / a.KV, kv = bk - b * a.KV,
@@ -1343,7 +1373,9 @@ struct Launch {
               RowsShape<T, kD, kWaves>::kLds, s);
   }
   static int forward(AttnArgs& a, hipStream_t s) {
-    if (a.splits == 0) return forward_rows<kMostWaves<T, kD>>(a, s);
+    if (a.splits == 0)
+      return fills(a, a.rows, kMostWaves<T, kD>) ? forward_rows<kMostWaves<T, kD>>(a, s)
+                                                 : forward_rows<4>(a, s);
     a.tiles = (a.rows + kRowsWave - 1) / kRowsWave;
     a.by_splits = divisor(a.splits);
     spread(a, a.tiles * a.splits);
@@ -1419,14 +1451,22 @@ bool valid_sizes(int64_t B, int64_t T, int64_t S, int H, int KV, int h, int dtyp
   return B * KV <= most / ((rows + 31) / 32 + 1) && B * KV <= most / ((S + 31) / 32 + 1);
 }
 
-// Splits of the keys (0: none): where whole row tiles would leave compute units idle,
-// enough workgroups of 32 rows for two rounds, none with fewer than four tiles of 32 keys a wave.
+// Splits of the keys (0: none).  Where tiles of 256 rows leave compute units idle, either of
+// two is taken that costs less: tiles of 128 rows (6 us and 1.1 a round's 64 keys), or rows by
+// 32 with their keys in splits, which are joined (12 us and 1.2 for 32 keys of 32 rows, four
+// waves a unit): then enough splits for four workgroups a unit, none with fewer than four tiles of
+// 32 keys a wave.  (9 x 443 tokens, 6 heads over 2: 18 us in 198 tiles, 29 in splits.  16
+// tokens of 32 heads over 8, 8192 keys at most: 228 us in tiles, 75 in 8 splits.)
 int splits_of(int64_t B, int64_t T, int64_t S, int H, int KV, int h, int dtype) {
   const int64_t rows = T * (H / KV), heads = B * KV;
   if (heads * ((rows + 255) / 256) >= kUnits) return 0;
   const int64_t groups = heads * ((rows + 31) / 32);
-  int64_t n = (2 * kUnits + groups - 1) / groups;
-  const int64_t most = S / (32 * 4 * (h * (dtype == DPC_F32 ? 4 : 2) <= 256 ? 4 : 1));
+  const int64_t rounds = (heads * ((rows + 127) / 128) + kUnits - 1) / kUnits;
+  const double tiled = 6.0 + 1.1 * (double)(rounds * S) / 64,
+               split = 12.0 + 1.2 * (double)(groups * S) / (32.0 * 4 * kUnits);
+  if (tiled <= split) return 0;
+  int64_t n = (4 * kUnits + groups - 1) / groups;
+  const int64_t most = S / (32 * 4 * split_waves(dtype, h));
   if (n > most) n = most;
   return n < 1 ? 1 : (n > 64 ? 64 : (int)n);
 }

@@ -34,7 +34,7 @@ def test_forward(lib):
                 dict(B=1 << 29, T=1 << 20),
                 dict(strides=_strides(1 << 12, 64, 17, *([1 << 12, 64, 16] * 2)))):
         assert call(**bad) == nat.DPC_EINVAL, bad
-    assert call() == nat.DPC_ENOSPC
+    assert call(T=1, S=1 << 14) == nat.DPC_ENOSPC  # keys in splits
     for far in (_strides(1 << 12, 1 << 30, 16, *([1 << 12, 64, 16] * 2)),
                 _strides(*([1 << 12, 64, 16] * 2), 1 << 12, 8, 16)):  # values overlap
         assert call(strides=far) == nat.DPC_ENOTSUP
@@ -58,7 +58,8 @@ def test_workspaces(lib):
 
     assert size(16, 1024, 1024, 16, 16, 128) == 0  # whole row tiles
     assert size(0, 1, 1, 1, 1, 8) == size(1, 0, 1, 1, 1, 8) == 0
-    assert size(1, 1, 64, 1, 1, 64) == 4 * (64 * 4 + 8)  # one split of four waves
+    assert size(1, 1, 64, 1, 1, 64) == 0
+    assert size(1, 1, 512, 1, 1, 64) == 4 * (64 * 4 + 8)  # one split of four waves
     assert lib.dpc_attention_grad_workspace_bytes(2, 3, 4) == 96
     assert lib.dpc_attention_state_bytes(2, 3, 4, 16, nat.DPC_BF16) == 256 + 24 * 16
     assert lib.dpc_attention_state_bytes(2, 3, 4, 16, nat.DPC_F32) == 256 + 96

@@ -117,7 +117,9 @@ def _run(q, k, v, up, **kw):
     (1, 64, 64, 2, 2, 128), (1, 65, 65, 6, 2, 80), (1, 129, 129, 8, 2, 128),
     (2, 200, 200, 7, 1, 96), (1, 130, 130, 2, 1, 256), (1, 70, 70, 1, 1, 192),
     (1, 5, 77, 4, 2, 64), (3, 1, 300, 8, 2, 128), (1, 40, 500, 16, 1, 32), (1, 2, 130, 2, 2, 256),
-    (2, 20, 20, 2, 1, 7), (1, 50, 20, 2, 2, 24), (1, 300, 300, 2, 2, 64), (1, 1, 2100, 4, 4, 64)])
+    (2, 20, 20, 2, 1, 7), (1, 50, 20, 2, 2, 24), (1, 300, 300, 2, 2, 64), (1, 1, 2100, 4, 4, 64),
+    (2, 3, 1500, 6, 2, 256), (1, 33, 700, 16, 1, 96), (1, 2, 900, 70, 1, 64), (1, 130, 130, 130, 1, 16),
+    (16, 260, 260, 16, 16, 64), (3, 500, 500, 48, 24, 128)])
 def test_causal(dev, dtype, B, T, S, H, KV, h):
     x = _inputs(B, T, S, H, KV, h, DTYPES[dtype], dev)
     _check(_run(*x), _reference(*x))
