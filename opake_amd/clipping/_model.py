@@ -105,24 +105,34 @@ class GhostGradAux:
 
 class _Capture:
     """Forward hook that keeps a linear layer's input, its (graph-attached)
-    output and the row segments the caller declared for this call."""
+    output and the row segments the caller declared for this call.  A layer
+    that returns something made of its projections (``gated.GatedLinear``)
+    leaves those for the time of the capture: they are what ``A`` multiplies."""
 
     def __init__(self, module: torch.nn.Linear):
         self.A = None
         self.out = None
         self.segments = None
         self.calls = 0
+        self._gated = module if hasattr(module, "dpc_keep_projections") else None
+        if self._gated is not None:
+            module.dpc_keep_projections = True
         self._handle = module.register_forward_hook(self._fwd)
 
     def _fwd(self, module, inputs, output):
         self.calls += 1
         self.A = inputs[0].detach()
         self.out = output
+        if self._gated is not None:
+            self.out, module.dpc_projections = module.dpc_projections, None
         seg = getattr(module, "dpc_row_segments", None)
         self.segments = None if seg is None else [int(v) for v in seg]
 
     def remove(self):
         self._handle.remove()
+        if self._gated is not None:
+            self._gated.dpc_keep_projections = False
+            self._gated.dpc_projections = None
 
 
 def _trainable_modules(model: torch.nn.Module):

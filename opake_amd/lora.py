@@ -15,7 +15,9 @@ clipping forms their per-example gradients directly (``dpc_per_example_grads``:
 ``LoRABlock`` is the 8B-shaped block of the LoRA configuration: pre-norm
 attention with grouped-query heads (separate q / k / v / o projections) and a
 SwiGLU FFN (gate / up / down), every projection a ``LoRALinear``; the norms
-and base weights are frozen.  Its attention core runs in float32.
+and base weights are frozen.  Its attention core runs in float32; with
+``fused`` (on the GPU, bfloat16 or float32) ``rotary`` and ``attention`` take
+the projections as they are, key heads shared and not repeated.
 """
 
 from __future__ import annotations
@@ -26,6 +28,8 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from opake_amd.attention import attention
+from opake_amd.rotary import rotary, rotary_frequencies
 from opake_amd.transformer import apply_rotary, rotary_tables
 
 
@@ -50,11 +54,12 @@ class LoRALinear(nn.Module):
 class LoRABlock(nn.Module):
     def __init__(self, d: int = 4096, n_heads: int = 32, n_kv_heads: int = 8,
                  ffn: int = 14336, r: int = 16, alpha: float = 32.0, eps: float = 1e-5, *,
-                 dtype=None, device=None):
+                 fused: bool = False, dtype=None, device=None):
         super().__init__()
         if d % n_heads or n_heads % n_kv_heads:
             raise ValueError("d must divide into n_heads, n_heads into n_kv_heads")
         self.d, self.n_heads, self.n_kv, self.ffn = d, n_heads, n_kv_heads, ffn
+        self.fused = fused
         hd = d // n_heads
         kw = dict(dtype=dtype, device=device)
         lk = dict(r=r, alpha=alpha, **kw)
@@ -71,23 +76,35 @@ class LoRABlock(nn.Module):
         self.mlp_norm.requires_grad_(False)
         self._rope = {}
 
+    def _fused_attention(self, q, k, v):
+        if q.device not in self._rope:
+            self._rope[q.device] = rotary_frequencies(q.shape[-1], device=q.device)[0]
+        q, k = rotary(q, k, self._rope[q.device])
+        return attention(q, k, v)
+
+    def _attention(self, q, k, v):
+        B, T, H, hd = q.shape
+        q, k, v = (t.transpose(1, 2) for t in (q, k, v))
+        key = (T, q.device)
+        if key not in self._rope:
+            self._rope[key] = rotary_tables(T, hd, device=q.device)
+        cos, sin = self._rope[key]
+        q, k = apply_rotary(q, cos, sin), apply_rotary(k, cos, sin)
+        rep = H // self.n_kv
+        k = k.repeat_interleave(rep, dim=1)
+        v = v.repeat_interleave(rep, dim=1)
+        att = F.scaled_dot_product_attention(q.float(), k.float(), v.float(), is_causal=True)
+        return att.to(v.dtype).transpose(1, 2)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         B, T, d = x.shape
         H, KV, hd = self.n_heads, self.n_kv, d // self.n_heads
         h = self.attn_norm(x)
-        q = self.q(h).view(B, T, H, hd).transpose(1, 2)
-        k = self.k(h).view(B, T, KV, hd).transpose(1, 2)
-        v = self.v(h).view(B, T, KV, hd).transpose(1, 2)
-        key = (T, x.device)
-        if key not in self._rope:
-            self._rope[key] = rotary_tables(T, hd, device=x.device)
-        cos, sin = self._rope[key]
-        q, k = apply_rotary(q, cos, sin), apply_rotary(k, cos, sin)
-        rep = H // KV
-        k = k.repeat_interleave(rep, dim=1)
-        v = v.repeat_interleave(rep, dim=1)
-        att = F.scaled_dot_product_attention(q.float(), k.float(), v.float(), is_causal=True)
-        x = x + self.o(att.to(x.dtype).transpose(1, 2).reshape(B, T, d))
+        q = self.q(h).view(B, T, H, hd)
+        k = self.k(h).view(B, T, KV, hd)
+        v = self.v(h).view(B, T, KV, hd)
+        att = (self._fused_attention if self.fused else self._attention)(q, k, v)
+        x = x + self.o(att.reshape(B, T, d))
         h = self.mlp_norm(x)
         a = F.silu(self.gate(h).float()).to(x.dtype) * self.up(h)
         return x + self.down(a)

@@ -14,6 +14,12 @@ output head (the clipped parameters are the block's) and returns logits.
 The attention core runs in float32 (``scaled_dot_product_attention`` on
 float32 q, k, v, cast back): bf16 batched products whose right operand is a
 transposed view -- which attention's backward issues -- are avoided.
+
+With ``fused`` the block (on the GPU, bfloat16 or float32) runs ``rotary``,
+``attention`` and ``gated_linear`` instead, which keep q, k, v and the
+projections in the model's type and nothing of size [T, T]; parameters and
+their names are the same.  Ghost clipping takes the fused block like the other
+one; ``vmap`` and the other function transforms do not take these operators.
 """
 
 from __future__ import annotations
@@ -21,6 +27,10 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 from torch import nn
+
+from opake_amd.attention import attention
+from opake_amd.gated import GatedLinear
+from opake_amd.rotary import rotary, rotary_frequencies
 
 
 def rotary_tables(T: int, head_dim: int, base: float = 10000.0, device=None):
@@ -42,17 +52,18 @@ def apply_rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch
 
 class LlamaBlock(nn.Module):
     def __init__(self, d: int = 2048, n_heads: int = 16, ffn: int = 8192, eps: float = 1e-5, *,
-                 dtype=None, device=None):
+                 fused: bool = False, dtype=None, device=None):
         super().__init__()
         if d % n_heads:
             raise ValueError("d must be a multiple of n_heads")
-        self.d, self.n_heads, self.ffn = d, n_heads, ffn
+        self.d, self.n_heads, self.ffn, self.fused = d, n_heads, ffn, fused
         kw = dict(dtype=dtype, device=device)
         self.attn_norm = nn.RMSNorm(d, eps=eps, **kw)
         self.qkv = nn.Linear(d, 3 * d, bias=False, **kw)
         self.o = nn.Linear(d, d, bias=False, **kw)
         self.mlp_norm = nn.RMSNorm(d, eps=eps, **kw)
-        self.gate_up = nn.Linear(d, 2 * ffn, bias=False, **kw)
+        self.gate_up = (GatedLinear(d, ffn, **kw) if fused
+                        else nn.Linear(d, 2 * ffn, bias=False, **kw))
         self.down = nn.Linear(ffn, d, bias=False, **kw)
         self._rope = {}
 
@@ -62,10 +73,19 @@ class LlamaBlock(nn.Module):
             self._rope[key] = rotary_tables(T, self.d // self.n_heads, device=device)
         return self._rope[key]
 
+    def _freqs(self, device):
+        if device not in self._rope:
+            self._rope[device] = rotary_frequencies(self.d // self.n_heads, device=device)[0]
+        return self._rope[device]
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         B, T, d = x.shape
         H, hd = self.n_heads, d // self.n_heads
         qkv = self.qkv(self.attn_norm(x)).view(B, T, 3, H, hd)
+        if self.fused:
+            q, k = rotary(qkv[:, :, 0], qkv[:, :, 1], self._freqs(x.device))
+            x = x + self.o(attention(q, k, qkv[:, :, 2]).reshape(B, T, d))
+            return x + self.down(self.gate_up(self.mlp_norm(x)))
         q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
         cos, sin = self._tables(T, x.device)
         q, k = apply_rotary(q, cos, sin), apply_rotary(k, cos, sin)
@@ -81,11 +101,11 @@ class BlockLM(nn.Module):
     """Frozen embedding -> one ``LlamaBlock`` -> frozen head: logits [B, T, V]."""
 
     def __init__(self, vocab: int = 32000, d: int = 2048, n_heads: int = 16, ffn: int = 8192, *,
-                 dtype=None, device=None):
+                 fused: bool = False, dtype=None, device=None):
         super().__init__()
         kw = dict(dtype=dtype, device=device)
         self.embed = nn.Embedding(vocab, d, **kw)
-        self.block = LlamaBlock(d, n_heads, ffn, **kw)
+        self.block = LlamaBlock(d, n_heads, ffn, fused=fused, **kw)
         self.head = nn.Linear(d, vocab, bias=False, **kw)
         self.embed.weight.requires_grad_(False)
         self.head.weight.requires_grad_(False)
