@@ -8,7 +8,8 @@
 // Forward: one product whose 256 x 256 tiles hold the gate and the up projection of 128
 // columns, so that h is formed in the accumulators (mm_tile.h, kPaired); z is written
 // too where a gradient will be asked for.  Few tiles: the K steps go out in slices, whose
-// float32 sums are added up, in order, by a second launch that forms h.
+// float32 sums are added up, in order, by a second launch that forms h.  Few tokens:
+// a kernel of their own, which reads the weights as they are.
 // Backward: dz in one pass over z and dh, and two products.
 //
 // float32 operands are multiplied as two fp16 planes (mm_tile.h).  Rows of x and of dz
@@ -74,21 +75,34 @@ struct Tops {
   uint32_t* all;  // one word, or null (zero before the launch)
 };
 
-// One wave a row; blockIdx.y: the tensor.
+// One wave a row; blockIdx.y: the tensor.  Few and large workgroups, since each ends in an
+// atomic on one word (1366 of them: 23 us of 22 MB; 256 with wide loads: 12).
+constexpr int kTopsWaves = 16;
+
 struct TopsArgs {
   Tops t[2];
 };
 
-__global__ void __launch_bounds__(256) gated_tops_kernel(TopsArgs args) {
-  __shared__ uint32_t waves[4];
+__global__ void __launch_bounds__(64 * kTopsWaves) gated_tops_kernel(TopsArgs args) {
+  __shared__ uint32_t waves[kTopsWaves];
   const Tops a = args.t[blockIdx.y];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   uint32_t top = 0;
-  for (int64_t r = blockIdx.x * 4ll + w; r < a.rows; r += gridDim.x * 4ll) {
+  for (int64_t r = blockIdx.x * (int64_t)kTopsWaves + w; r < a.rows;
+       r += gridDim.x * (int64_t)kTopsWaves) {
     const float* x = a.src + r * a.cols;
     uint32_t mine = 0;
+    // Up to the first 16-byte boundary, from there in whole quads, and what is left.
+    const int head = min((int)(-((uintptr_t)x >> 2) & 3), a.cols), quads = (a.cols - head) / 4;
+    const f32x4_t* q = reinterpret_cast<const f32x4_t*>(x + head);
 #pragma unroll 4
-    for (int c = lane; c < a.cols; c += 64) mine = max(mine, finite_bits(x[c]));
+    for (int c = lane; c < quads; c += 64) {
+      const f32x4_t v = q[c];
+      mine = max(max(mine, max(finite_bits(v[0]), finite_bits(v[1]))),
+                 max(finite_bits(v[2]), finite_bits(v[3])));
+    }
+    if (lane < head) mine = max(mine, finite_bits(x[lane]));
+    if (head + 4 * quads + lane < a.cols) mine = max(mine, finite_bits(x[head + 4 * quads + lane]));
     mine = wave_max_bits(mine);
     if (a.row && lane == 0) a.row[r] = mine;
     top = max(top, mine);
@@ -97,7 +111,7 @@ __global__ void __launch_bounds__(256) gated_tops_kernel(TopsArgs args) {
   if (lane == 0) waves[w] = top;
   __syncthreads();
   if (threadIdx.x == 0) {
-    top = max(max(waves[0], waves[1]), max(waves[2], waves[3]));
+    for (int i = 1; i < kTopsWaves; ++i) top = max(top, waves[i]);
     if (top) atomicMax(a.all, top);
   }
 }
@@ -403,6 +417,113 @@ __global__ void __launch_bounds__(256) gated_reduce_kernel(ProductArgs s) {
 }
 
 // ---------------------------------------------------------------------------
+// Few tokens: the weights' way from memory is all there is.
+// ---------------------------------------------------------------------------
+
+// h (and z) of up to 16 kBlocks tokens: a workgroup takes 16 gate rows of w and their up
+// rows, each wave the products of every eighth run of four fragments along D (256 bytes of a row, so
+// that whole lines are asked for), and the waves' sums are added up in order.  The next
+// run's loads are on their way while one is multiplied.  Rows and tokens past the last are
+// read as the last one's, and left out when h is written; behind D there are zeros.
+// Bound by memory: 16 tokens of D = 4096, F = 14336 in bf16 take 50 us, 4.7 TB/s of weights,
+// one 44 (5.3 TB/s); beyond 16 by the tokens' reads from L2, as long as the weights'.
+// float32: each lane's 16 bytes are four k of its row, one for each of four products (the
+// k of a product may be any, if both operands have the same), so nothing is split or shifted.
+template <bool kHalf, int kBlocks>
+__global__ void __launch_bounds__(512) gated_few_kernel(const void* __restrict__ x,
+                                                        const void* __restrict__ wt, int D,
+                                                        ProductArgs s) {
+  constexpr int kSize = kHalf ? 4 : 2, kLane = 16 / kSize, kStep = 4 * kLane, kRun = 4 * kStep;
+  constexpr int kWaves = 8;
+  __shared__ f32x4_t sums[kWaves * 2 * kBlocks * 64];  // [wave][gate, up][token block][lane]
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int F = s.rows_a, N = s.rows_b, f0 = blockIdx.x * 16;
+  const int at = kLane * (lane >> 4);
+  const int64_t row = min(f0 + (lane & 15), F - 1);
+  const uint8_t* pw[2] = {static_cast<const uint8_t*>(wt) + (row * D + at) * kSize,
+                          static_cast<const uint8_t*>(wt) + ((row + F) * D + at) * kSize};
+  const uint8_t* px[kBlocks];
+#pragma unroll
+  for (int j = 0; j < kBlocks; ++j)
+    px[j] = static_cast<const uint8_t*>(x) +
+            ((int64_t)min(16 * j + (lane & 15), N - 1) * D + at) * kSize;
+  struct Run {
+    u32x4_t w[4][2], x[4][kBlocks];
+  };
+  f32x4_t acc[2][kBlocks] = {};
+  auto load = [&](Run& r, int k0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = (k0 + i * kStep) * kSize;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) r.w[i][p] = *reinterpret_cast<const u32x4_t*>(pw[p] + k);
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j) r.x[i][j] = *reinterpret_cast<const u32x4_t*>(px[j] + k);
+    }
+  };
+  auto multiply = [&](const Run& r) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          if constexpr (kHalf) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              acc[p][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(
+                  __uint_as_float(r.w[i][p][e]), __uint_as_float(r.x[i][j][e]), acc[p][j], 0, 0, 0);
+          } else {
+            acc[p][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(bf16x8_t, r.w[i][p]), __builtin_bit_cast(bf16x8_t, r.x[i][j]),
+                acc[p][j], 0, 0, 0);
+          }
+        }
+  };
+  const int runs = D / kRun;
+  Run a, b;
+  int r = w;
+  if (r < runs) load(a, r * kRun);
+  while (r < runs) {
+    if (r + kWaves < runs) load(b, (r + kWaves) * kRun);
+    multiply(a);
+    r += kWaves;
+    if (r >= runs) break;
+    if (r + kWaves < runs) load(a, (r + kWaves) * kRun);
+    multiply(b);
+    r += kWaves;
+  }
+  if (r == runs && runs * kRun < D) {  // what is left: the next wave in turn
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = (runs * kRun + i * kStep) * kSize;
+      const bool in = runs * kRun + i * kStep + at < D;
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        a.w[i][p] = in ? *reinterpret_cast<const u32x4_t*>(pw[p] + k) : u32x4_t{};
+#pragma unroll
+      for (int j = 0; j < kBlocks; ++j)
+        a.x[i][j] = in ? *reinterpret_cast<const u32x4_t*>(px[j] + k) : u32x4_t{};
+    }
+    multiply(a);
+  }
+#pragma unroll
+  for (int p = 0; p < 2; ++p)
+#pragma unroll
+    for (int j = 0; j < kBlocks; ++j) sums[((w * 2 + p) * kBlocks + j) * 64 + lane] = acc[p][j];
+  __syncthreads();
+  if (w >= kBlocks) return;
+  f32x4_t g = {}, u = {};
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    g += sums[(2 * i * kBlocks + w) * 64 + lane];
+    u += sums[((2 * i + 1) * kBlocks + w) * 64 + lane];
+  }
+  const int n = 16 * w + (lane & 15), f = f0 + 4 * (lane >> 4);
+  if (n < N && f < F) gated_out<kHalf>(s, n, f, F % 4 == 0, g, u);
+}
+
+// ---------------------------------------------------------------------------
 // dz from z and dh: one pass, bound by memory.
 // ---------------------------------------------------------------------------
 
@@ -511,6 +632,14 @@ struct Operand {
   size_t at, bytes;  // in the workspace
 };
 
+// So many tokens at most go to gated_few_kernel, rows of whole 16-byte chunks given.  D = 4096,
+// F = 14336, from memory, against the tiles: bf16 (tiles 67 us) one token 44 us, 16 50, 32 68,
+// 48 87; float32 (tiles 433, with the planes' making) one 91, 16 102, 32 151, 64 248.
+// (D = 2048, F = 8192, bf16: 14.6, 15, 21, 27; tiles 28.)
+bool few(int64_t N, int D, int dtype) {
+  return dtype == DPC_BF16 ? N <= 32 && D % 8 == 0 : N <= 64 && D % 4 == 0;
+}
+
 struct Plan {
   int64_t N;
   int D, F;
@@ -547,10 +676,11 @@ struct Plan {
     take(&row_x, half ? (size_t)N * 4 : 0);
     take(&row_dz, half && !forward ? (size_t)N * 4 : 0);
     x = w = dz = Operand{};
+    for (int& v : splits) v = 1;
+    if (forward && few(N, D, dtype)) return;
     if (forward || want_w) operand(&x, N, D, N);
     if (forward || want_x) operand(&w, 2ll * F, D, 2ll * F);
     if (!forward) operand(&dz, N, 2 * F, N);
-    for (int& s : splits) s = 1;
     if (forward)
       product(kForward, (F + 127) / 128, blocks_of(N), D, N, 2 * up(F, 4));
     if (want_x && !forward) product(kHidden, blocks_of(D), blocks_of(N), 2ll * F, N, up(D, 4));
@@ -562,9 +692,9 @@ struct Plan {
 int tops(const TopsArgs& a, int n, hipStream_t s) {
   int64_t rows = a.t[0].rows;
   if (n > 1 && a.t[1].rows > rows) rows = a.t[1].rows;
-  int64_t grid = (rows + 3) / 4;
-  if (grid > 2048) grid = 2048;
-  hipLaunchKernelGGL(gated_tops_kernel, dim3((unsigned)grid, n), dim3(256), 0, s, a);
+  int64_t grid = (rows + kTopsWaves - 1) / kTopsWaves;
+  if (grid > kUnits) grid = kUnits;
+  hipLaunchKernelGGL(gated_tops_kernel, dim3((unsigned)grid, n), dim3(64 * kTopsWaves), 0, s, a);
   DPC_HIP_CHECK(hipGetLastError());
   return DPC_OK;
 }
@@ -620,6 +750,19 @@ Pack pack_of(const Operand& o, const void* src, uint8_t* ws, const uint32_t* row
               all, mixed};
 }
 
+template <bool kHalf>
+int few_product(const ProductArgs& a, const void* x, const void* w, int D, hipStream_t s) {
+  const dim3 grid((unsigned)((a.rows_a + 15) / 16)), block(512);
+  if (a.rows_b <= 16)
+    hipLaunchKernelGGL((gated_few_kernel<kHalf, 1>), grid, block, 0, s, x, w, D, a);
+  else if (a.rows_b <= 32)
+    hipLaunchKernelGGL((gated_few_kernel<kHalf, 2>), grid, block, 0, s, x, w, D, a);
+  else if constexpr (kHalf)
+    hipLaunchKernelGGL((gated_few_kernel<kHalf, 4>), grid, block, 0, s, x, w, D, a);
+  DPC_HIP_CHECK(hipGetLastError());
+  return DPC_OK;
+}
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
@@ -642,6 +785,16 @@ extern "C" int dpc_gated_linear(const void* x, const void* w, int64_t N, int D, 
   if (ws_bytes < p.total) return DPC_ENOSPC;
   hipStream_t s = (hipStream_t)stream;
   uint8_t* base = static_cast<uint8_t*>(ws);
+  ProductArgs a = {};
+  a.rows_b = (int)N;
+  a.rows_a = F;
+  a.act = activation;
+  a.out = h;
+  a.z = z;
+  a.rest = static_cast<int8_t*>(rest);
+  a.bf16 = !p.half;
+  if (few(N, D, dtype))
+    return p.half ? few_product<true>(a, x, w, D, s) : few_product<false>(a, x, w, D, s);
   uint32_t* words = reinterpret_cast<uint32_t*>(base + p.tops);
   uint32_t* row_x = reinterpret_cast<uint32_t*>(base + p.row_x);
   if (p.half) {
@@ -652,25 +805,17 @@ extern "C" int dpc_gated_linear(const void* x, const void* w, int64_t N, int D, 
     if (const int rc = tops(t, 2, s)) return rc;
   }
   if (p.x.copied) {
-    const PackArgs a = {{pack_of(p.x, x, base, row_x, nullptr, 0),
+    const PackArgs k = {{pack_of(p.x, x, base, row_x, nullptr, 0),
                          pack_of(p.w, w, base, nullptr, words, 0)}};
-    if (const int rc = pack(a, 2, p.half, s)) return rc;
+    if (const int rc = pack(k, 2, p.half, s)) return rc;
   }
-  ProductArgs a = {};
   a.mm = MmArgs{mm_operand(p.w, w, base, F), mm_operand(p.x, x, base, N), (int)up(D, 8),
                 (F + 127) / 128, (int)blocks_of(N), p.splits[kForward]};
-  a.rows_b = (int)N;
-  a.rows_a = F;
   a.partial = reinterpret_cast<float*>(base + p.partial);
   a.lda = 2 * up(F, 4);
   a.plane = N * a.lda;
   a.row = row_x;
   a.all = words;
-  a.act = activation;
-  a.out = h;
-  a.z = z;
-  a.rest = static_cast<int8_t*>(rest);
-  a.bf16 = !p.half;
   return product<kForward>(a, p.half, s);
 }
 
