@@ -29,8 +29,8 @@ import torch.nn.functional as F
 from torch import nn
 
 from opake_amd.attention import attention
-from opake_amd.rotary import rotary, rotary_frequencies
-from opake_amd.transformer import apply_rotary, rotary_tables
+from opake_amd.rotary import rotary
+from opake_amd.transformer import RotaryFrequencies, apply_rotary, rotary_tables
 
 
 class LoRALinear(nn.Module):
@@ -75,11 +75,11 @@ class LoRABlock(nn.Module):
         self.attn_norm.requires_grad_(False)
         self.mlp_norm.requires_grad_(False)
         self._rope = {}
+        if fused:
+            self.rope = RotaryFrequencies(hd, device=device)
 
     def _fused_attention(self, q, k, v):
-        if q.device not in self._rope:
-            self._rope[q.device] = rotary_frequencies(q.shape[-1], device=q.device)[0]
-        q, k = rotary(q, k, self._rope[q.device])
+        q, k = rotary(q, k, self.rope.freqs)
         return attention(q, k, v)
 
     def _attention(self, q, k, v):

@@ -50,6 +50,21 @@ def apply_rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch
     return out.to(x.dtype)
 
 
+class RotaryFrequencies(nn.Module):
+    """``rotary``'s frequencies of a block: float64, on its device, whatever it is cast to."""
+
+    def __init__(self, dims: int, device=None):
+        super().__init__()
+        self.dims = dims
+        self.register_buffer("freqs", rotary_frequencies(dims, device=device)[0],
+                             persistent=False)
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self.freqs = rotary_frequencies(self.dims, device=self.freqs.device)[0]
+        return self
+
+
 class LlamaBlock(nn.Module):
     def __init__(self, d: int = 2048, n_heads: int = 16, ffn: int = 8192, eps: float = 1e-5, *,
                  fused: bool = False, dtype=None, device=None):
@@ -66,6 +81,8 @@ class LlamaBlock(nn.Module):
                         else nn.Linear(d, 2 * ffn, bias=False, **kw))
         self.down = nn.Linear(ffn, d, bias=False, **kw)
         self._rope = {}
+        if fused:
+            self.rope = RotaryFrequencies(d // n_heads, device=device)
 
     def _tables(self, T, device):
         key = (T, device)
@@ -73,17 +90,12 @@ class LlamaBlock(nn.Module):
             self._rope[key] = rotary_tables(T, self.d // self.n_heads, device=device)
         return self._rope[key]
 
-    def _freqs(self, device):
-        if device not in self._rope:
-            self._rope[device] = rotary_frequencies(self.d // self.n_heads, device=device)[0]
-        return self._rope[device]
-
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         B, T, d = x.shape
         H, hd = self.n_heads, d // self.n_heads
         qkv = self.qkv(self.attn_norm(x)).view(B, T, 3, H, hd)
         if self.fused:
-            q, k = rotary(qkv[:, :, 0], qkv[:, :, 1], self._freqs(x.device))
+            q, k = rotary(qkv[:, :, 0], qkv[:, :, 1], self.rope.freqs)
             x = x + self.o(attention(q, k, qkv[:, :, 2]).reshape(B, T, d))
             return x + self.down(self.gate_up(self.mlp_norm(x)))
         q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
@@ -122,4 +134,5 @@ def per_example_lm_loss(logits: torch.Tensor, targets: torch.Tensor) -> torch.Te
     return ce.view(B, T).mean(dim=1)
 
 
-__all__ = ["BlockLM", "LlamaBlock", "apply_rotary", "per_example_lm_loss", "rotary_tables"]
+__all__ = ["BlockLM", "LlamaBlock", "RotaryFrequencies", "apply_rotary", "per_example_lm_loss",
+           "rotary_tables"]

@@ -1,0 +1,194 @@
+"""The block's operators (GPU): differences, few tokens, two streams, captured blocks.
+
+References and their tolerances are those of the operators' own test files.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from opake_amd.attention import attention
+from opake_amd.clipping import ghost_clipped_grad
+from opake_amd.gated import gated_linear
+from opake_amd.lora import LoRABlock
+from opake_amd.rotary import rotary, rotary_frequencies
+from opake_amd.transformer import BlockLM, LlamaBlock, per_example_lm_loss
+from test_gpu_gated import DTYPES, _act, _check, _inputs, _reference
+
+pytestmark = pytest.mark.gpu
+
+
+# Up to 32 tokens in bfloat16 and 64 in float32 have a kernel of their own: one to four blocks of 16
+# tokens, whole runs along D and rests of them (a run is 128 or 64 wide, eight at a time), rows
+# of F that end in a block, and widths that are not whole chunks, which it does not take.
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("N", [1, 15, 16, 17, 32, 33, 64, 65])
+@pytest.mark.parametrize("D,F", [(8, 5), (1024, 16), (1160, 17), (4, 36), (100, 50), (2176, 33)])
+def test_few_tokens(dev, dtype, N, D, F):
+    x, w, up = _inputs((N, D), F, DTYPES[dtype], dev, seed=N + D)
+    with torch.no_grad():
+        alone = gated_linear(x, w)
+    h = gated_linear(x, w)
+    assert torch.equal(alone, h)
+    dx, dw = torch.autograd.grad(h, [x, w], up)
+    for got, ref in zip((h, dx, dw), _reference(x, w, up, "silu", x.dtype)):
+        _check(got, ref)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_few_tokens_stay_their_own(dev, dtype):
+    """Neither another token nor another weight row's infinities and NaN."""
+    x, w, _ = _inputs((20, 200), 24, DTYPES[dtype], dev, seed=2)
+    want = gated_linear(x, w).detach()
+    with torch.no_grad():
+        x[3, 7] = float("nan")
+        x[19, 199] = float("inf")
+        w[5, 0] = float("inf")
+        got = gated_linear(x, w)
+    keep = torch.ones(20, dtype=torch.bool, device=dev)
+    keep[[3, 19]] = False
+    cols = torch.ones(24, dtype=torch.bool, device=dev)
+    cols[5] = False
+    assert torch.equal(got[keep][:, cols], want[keep][:, cols])
+    assert bool(got[3].isnan().all()) and not bool(got[19].isfinite().any())
+
+
+def test_gated_gradients_against_differences(dev):
+    """In float32, against central differences of the formula in float64."""
+    for act in ("silu", "gelu"):
+        x, w, up = _inputs((5, 12), 7, torch.float32, dev, seed=9)
+        grads = torch.autograd.grad(gated_linear(x, w, activation=act), [x, w], up)
+        for i, g in enumerate(grads):
+            way = torch.randn(g.shape, generator=torch.Generator().manual_seed(i)).double()
+
+            def loss(step):
+                t = [x.detach().cpu().double(), w.detach().cpu().double()]
+                t[i] = t[i] + step * way
+                z = t[0] @ t[1].T
+                return (_act(z[:, :7], act)[0] * z[:, 7:] * up.cpu().double()).sum().item()
+
+            d = 1e-4  # third derivatives of order one: 1e-8
+            slope = (loss(d) - loss(-d)) / (2 * d)
+            assert abs(slope - (g.cpu().double() * way).sum().item()) < 1e-5 * max(1.0, abs(slope))
+
+
+def test_rotary_gradients_against_differences(dev):
+    """The rotation is linear: its differences are its derivative, 2^-22 of either value off."""
+    g = torch.Generator().manual_seed(4)
+    for interleaved in (False, True):
+        q, way, up = (torch.randn(2, 9, 3, 24, generator=g).to(dev) for _ in range(3))
+        q.requires_grad_()
+        freqs, amplitude = rotary_frequencies(16, scaling={"kind": "linear", "factor": 3.0},
+                                              device=dev)
+        turn = lambda t: rotary(t, None, freqs, interleaved=interleaved,  # noqa: E731
+                                amplitude=1.25 * amplitude)
+        (dq,) = torch.autograd.grad(turn(q), [q], up)
+        slope = ((turn(q + way) - turn(q)).double() * up.double()).sum().item()
+        size = (up.double() ** 2).sum().sqrt().item() * (q.double() ** 2).sum().sqrt().item()
+        assert abs(slope - (dq.double() * way.double()).sum().item()) < 2.0 ** -18 * size
+
+
+def test_one_tensor_as_queries_keys_and_values(dev):
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(2, 77, 4, 32, generator=g).to(dev).requires_grad_()
+    up = torch.randn(2, 77, 4, 32, generator=g).to(dev)
+    (got,) = torch.autograd.grad(attention(x, x, x), [x], up)
+    parts = [x.detach().clone().requires_grad_() for _ in range(3)]
+    want = torch.autograd.grad(attention(*parts), parts, up)
+    torch.testing.assert_close(got, want[0] + want[1] + want[2], rtol=2.0 ** -20, atol=1e-6)
+    freqs, _ = rotary_frequencies(32, device=dev)
+    a, b = rotary(x, x, freqs)
+    assert torch.equal(a, b)
+    (got,) = torch.autograd.grad((a, b), [x], (up, up))
+    (once,) = torch.autograd.grad(rotary(x, None, freqs), [x], up)
+    assert torch.equal(got, 2 * once)
+
+
+def test_two_streams_at_once(dev):
+    """Calls beside each other have their own workspaces, and answer as one by one."""
+    torch.manual_seed(1)
+    blocks = [LlamaBlock(128, 2, 192, fused=True, dtype=torch.bfloat16).to(dev) for _ in range(2)]
+    xs = [torch.randn(2, 300, 128, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+    caches = [torch.randn(4, 3000, 2, 64, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+    ones = [torch.randn(4, 1, 8, 64, dtype=torch.bfloat16, device=dev) for _ in range(2)]
+
+    def work(i):
+        x = xs[i].detach().requires_grad_()
+        y = blocks[i](x)
+        (dx,) = torch.autograd.grad(y, [x], torch.ones_like(y))
+        return y.detach(), dx, attention(ones[i], caches[i], caches[i])
+
+    want = [work(0), work(1)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(work(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for outs in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_captured_block(dev, dtype):
+    """A fused block's forward and its input's gradient in one graph, replayed."""
+    torch.manual_seed(2)
+    block = LlamaBlock(128, 2, 192, fused=True, dtype=DTYPES[dtype]).to(dev)
+    block.requires_grad_(False)
+    x = torch.randn(2, 150, 128, dtype=DTYPES[dtype], device=dev)
+    up = torch.randn_like(x)
+
+    def step():
+        leaf = x.detach().requires_grad_()
+        y = block(leaf)
+        return y.detach(), torch.autograd.grad(y, [leaf], up)[0]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(4):
+        x.copy_(torch.randn_like(x))
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(out, step()):
+            assert torch.equal(got, want)
+
+
+def test_frequencies_follow_the_block(dev):
+    """Casts leave them in float64, and moves take them along."""
+    for make in (lambda: LlamaBlock(64, 2, 24, fused=True),
+                 lambda: LoRABlock(64, 2, 1, 24, 4, fused=True)):
+        block = make().to(torch.bfloat16).to(dev)
+        want, _ = rotary_frequencies(32, device=dev)
+        assert torch.equal(block.rope.freqs, want) and not any("rope" in n for n in block.state_dict())
+        x = torch.randn(1, 5, 64, dtype=torch.bfloat16, device=dev)
+        assert torch.isfinite(block(x)).all()
+
+
+def test_a_failed_capture_leaves_the_layer_as_it_was(dev):
+    model = BlockLM(11, 32, 2, 24, fused=True, dtype=torch.float32).to(dev)
+    ids = torch.zeros(2, 4, dtype=torch.int64, device=dev)
+    layer = model.block.gate_up
+
+    def broken(logits, targets):
+        raise RuntimeError("no loss")
+
+    fn, st = ghost_clipped_grad(model, broken, clipping_norm=1.0)
+    with pytest.raises(RuntimeError, match="no loss"):
+        fn(ids, ids, state=st)
+    assert not layer.dpc_keep_projections and layer.dpc_projections is None
+    model(ids)
+    assert layer.dpc_projections is None
+    fn, st = ghost_clipped_grad(model, per_example_lm_loss, clipping_norm=1.0)
+    out, _ = fn(ids, ids, state=st)
+    assert all(torch.isfinite(t).all() for t in out.pytree.values())
