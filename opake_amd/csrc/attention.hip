@@ -96,7 +96,7 @@ struct AttnArgs {
   float scale, c;          // c = scale log2(e)
   int tiles;               // row tiles (dk, dv: key tiles) of a key head
   int per_xcd, chunk;      // key heads of an XCD (0: not divided among them), of a chunk
-  Divisor by_rep, by_kv, by_splits;
+  Divisor by_rep, by_kv;
   // Keys in splits (few rows): partial results.
   int splits;
   float* part_o;           // [splits][B * KV * rows][h]
@@ -163,6 +163,18 @@ DPC_DEVICE void place_of(const AttnArgs& a, int tiles, int* bk, int* tile) {
   const int now = min(a.chunk, heads - c * a.chunk);
   *tile = uniform((uint32_t)r / (uint32_t)now);
   *bk = first + c * a.chunk + r - *tile * now;
+}
+
+// Keys in splits: linear id -> (key head, row tile, split).  Sequences differ in length, so each
+// XCD, and with every split each unit, gets another example's heads; the row tiles of a
+// split's keys follow each other on one XCD, if the heads are a multiple of eight.  (16
+// sequences of 1 to 8192 keys, 8 key heads: 59 us, 4.6 TB/s; each XCD with its own heads 69.)
+DPC_DEVICE void place_of_split(const AttnArgs& a, int* bk, int* tile, int* split) {
+  const uint32_t heads = a.B * a.KV, all = heads * a.tiles, x = blockIdx.x, s = x / all,
+                 r = x - s * all, t = r / heads;
+  *split = uniform(s);
+  *tile = uniform(t);
+  *bk = uniform((r - t * heads + s * 3 * a.KV) % heads);
 }
 
 // ---------------------------------------------------------------------------
@@ -452,7 +464,11 @@ DPC_DEVICE int column_row(int x, int lane) { return 8 * (x >> 2) + 4 * (lane >> 
 #define DPC_WALL() __builtin_amdgcn_sched_barrier(0)
 
 // ---------------------------------------------------------------------------
-// Forward.
+// Forward.  Bound by the matrix cores and by what vector instructions the exponentials
+// and the statistics cannot hide behind them; a workgroup takes 6 us before its first
+// product.  bf16, causal, h = 128: 1 x 16384 tokens of 16 heads 1091 us (1.0 PFLOP/s of visible pairs,
+// the matrix cores half busy, vector instructions 40%), 8 x 2048 of 32 over 8 358 (0.77),
+// 16 x 1024 of 16 132 (0.52: half of each key head's tiles cross the diagonal).
 // ---------------------------------------------------------------------------
 
 // Row tiles of kWaves x 32 rows.  Stages of key and value tiles in LDS: as many as 128 KiB
@@ -477,12 +493,15 @@ struct SplitShape {
   static constexpr int kWaves = kRow <= 128 ? 4 : (kRow == 256 ? 2 : 1);
   static constexpr int kLds = kWaves * 4 * 32 * kRow;
 };
-// Rows of whose tiles two waves share a SIMD (256 registers each).
+// Rows of whose tiles two waves share a SIMD (256 registers each) and take turns: one has
+// products while the other has exponentials (forward of 16 x 1024 tokens of 16 heads, h =
+// 128: 144 us with one wave, 132 with two; 8 x 2048 of 32 over 8: 372 and 358).
 template <typename T, int kD>
 constexpr int kMostWaves = sizeof(T) == 2 && kD <= 128 ? 8 : 4;
 
 // Fragments in flight between LDS and the matrix cores: a read is issued that many
-// instructions (of 32 cycles) before its product.
+// instructions (of 32 cycles) before its product.  (Reads waited for one by one: 170 us
+// for the 16 x 1024 tokens above, 156 with these; longer rings spill.)
 constexpr int kAheadRows = 8, kAheadDq = 5, kAheadKeys = 4;
 
 template <typename T, int kD, int kWaves, bool kSplit>
@@ -495,11 +514,11 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
   constexpr bool kLate = !kSplit && Sh::kLate;
   const int lane = threadIdx.x & 63, w = uniform(threadIdx.x >> 6);
   int bk, tile, split = 0;
-  place_of(a, kSplit ? a.tiles * a.splits : a.tiles, &bk, &tile);
   if (kSplit) {
-    const int t = uniform(a.by_splits.of(tile));
-    split = (tile - t * a.splits) * kWaves + w;
-    tile = t;
+    place_of_split(a, &bk, &tile, &split);
+    split = split * kWaves + w;
+  } else {
+    place_of(a, a.tiles, &bk, &tile);
   }
   tile = a.tiles - 1 - tile;  // the longest first
   const int b = uniform(a.by_kv.of(bk)), kv = bk - b * a.KV;
@@ -786,7 +805,9 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int parts) {
 }
 
 // ---------------------------------------------------------------------------
-// dq and D: rows fixed, keys walked.
+// dq and D: rows fixed, keys walked.  The forward's walk with a product more; what bounds
+// it is the same: 8 x 2048 tokens of 32 heads over 8 513 us (0.80 PFLOP/s of its three
+// products), 16 x 1024 of 16 194 (0.53).
 // ---------------------------------------------------------------------------
 
 template <typename T, int kD, int kWaves>
@@ -992,7 +1013,8 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
 }
 
 // ---------------------------------------------------------------------------
-// dk and dv: keys fixed, rows walked.
+// dk and dv: keys fixed, rows walked.  Four products: 8 x 2048 tokens of 32 heads over 8
+// 630 us (0.87 PFLOP/s), 16 x 1024 of 16 266 (0.52).
 // ---------------------------------------------------------------------------
 
 // Key tiles of 32 keys a wave, or of 4 x 32 keys for 8 waves: then the wave and the one four on
@@ -1377,8 +1399,6 @@ struct Launch {
       return fills(a, a.rows, kMostWaves<T, kD>) ? forward_rows<kMostWaves<T, kD>>(a, s)
                                                  : forward_rows<4>(a, s);
     a.tiles = (a.rows + kRowsWave - 1) / kRowsWave;
-    a.by_splits = divisor(a.splits);
-    spread(a, a.tiles * a.splits);
     const int rc = go(attn_forward_kernel<T, kD, kSplitWaves, true>, a,
                       heads(a) * a.tiles * a.splits, 64 * kSplitWaves, SplitShape<T, kD>::kLds, s);
     if (rc) return rc;
@@ -1456,7 +1476,7 @@ bool valid_sizes(int64_t B, int64_t T, int64_t S, int H, int KV, int h, int dtyp
 // 32 with their keys in splits, which are joined (12 us and 1.2 for 32 keys of 32 rows, four
 // waves a unit): then enough splits for four workgroups a unit, none with fewer than four tiles of
 // 32 keys a wave.  (9 x 443 tokens, 6 heads over 2: 18 us in 198 tiles, 29 in splits.  16
-// tokens of 32 heads over 8, 8192 keys at most: 228 us in tiles, 75 in 8 splits.)
+// tokens of 32 heads over 8, 8192 keys at most: 228 us in tiles, 64 in 8 splits.)
 int splits_of(int64_t B, int64_t T, int64_t S, int H, int KV, int h, int dtype) {
   const int64_t rows = T * (H / KV), heads = B * KV;
   if (heads * ((rows + 255) / 256) >= kUnits) return 0;

@@ -12,7 +12,9 @@
 // are float32 Taylor sums.  All heads of a token share them: a workgroup makes the
 // tables of its few tokens in LDS (one thread a pair) and then walks their heads.
 //
-// Memory bounds it: each element is read and written once.
+// Memory bounds it: each element is read and written once.  (16 x 1024 tokens, 16 and 16
+// heads of 128, bf16: 54 us, 5.0 TB/s; 5 x 1999 of 32 and 8, half of each head, neighbours:
+// 46 us, 4.4 TB/s.)
 #include <math.h>
 
 #include "common.h"
