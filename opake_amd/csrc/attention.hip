@@ -1008,7 +1008,8 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
       if (x == stage) back(x);
   }
   transfers_left<0>();
-  store_row<T, kD>(static_cast<T*>(a.dq) + flat, nullptr, dq, a.scale, me.sees, me.there, a.h,
+  // One key alone: its probability is one, and ds zero, whatever rounding left of it.
+  store_row<T, kD>(static_cast<T*>(a.dq) + flat, nullptr, dq, a.scale, me.span > 0, me.there, a.h,
                    lane);
 }
 
@@ -1234,13 +1235,17 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1)) attn_dkv_k
         }
         dp[e][x] *= s[e][x];
       }
-      if (!whole) {  // rows that do not see the key: zero, and then so is ds
+      // Rows that do not see the key: zero, and then so is ds; it is zero too where a row sees one
+      // key alone (never in a whole tile), whatever the rounding of dp - D left.
+      if (!whole) {
         int r0 = 32 * (e + group) + column_row(0, lane);
         asm volatile("" : "+v"(r0));  // (its rows' tokens are not kept between tiles)
 #pragma unroll
         for (int x = 0; x < 16; ++x) {
           const int at = ti + (grouped ? a.by_rep.of(r0 + column_row(x, 0)) : 0);
-          if (key < sight.lo(at) || key > sight.hi(at)) s[e][x] = dp[e][x] = 0.f;
+          const int lo = sight.lo(at), hi = sight.hi(at);
+          if (key < lo || key > hi) s[e][x] = 0.f;
+          if (key < lo || key > hi || lo == hi) dp[e][x] = 0.f;
         }
       }
       if constexpr (sizeof(T) == 2) {

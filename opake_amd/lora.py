@@ -94,7 +94,7 @@ class LoRABlock(nn.Module):
         k = k.repeat_interleave(rep, dim=1)
         v = v.repeat_interleave(rep, dim=1)
         att = F.scaled_dot_product_attention(q.float(), k.float(), v.float(), is_causal=True)
-        return att.to(v.dtype).transpose(1, 2)
+        return att.transpose(1, 2)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         B, T, d = x.shape
@@ -104,7 +104,7 @@ class LoRABlock(nn.Module):
         k = self.k(h).view(B, T, KV, hd)
         v = self.v(h).view(B, T, KV, hd)
         att = (self._fused_attention if self.fused else self._attention)(q, k, v)
-        x = x + self.o(att.reshape(B, T, d))
+        x = x + self.o(att.to(x.dtype).reshape(B, T, d))
         h = self.mlp_norm(x)
         a = F.silu(self.gate(h).float()).to(x.dtype) * self.up(h)
         return x + self.down(a)

@@ -105,6 +105,32 @@ def test_one_tensor_as_queries_keys_and_values(dev):
     assert torch.equal(got, 2 * once)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("h", [16, 128, 256])
+def test_a_query_that_sees_one_key(dev, dtype, h):
+    """Its probability is one whatever the score: no gradient of query or key, exactly."""
+    g = torch.Generator().manual_seed(h)
+    for B, T, S, options in ((2, 300, 300, dict(window=1)), (1, 1, 1, {}), (2, 70, 1, dict(causal=False)),
+                             (20, 900, 900, dict(window=1)), (2, 40, 90, dict(window=1))):
+        q, k, v, up = (torch.randn(B, n, heads, h, generator=g).to(DTYPES[dtype]).to(dev)
+                       for n, heads in ((T, 4), (S, 2), (S, 2), (T, 4)))
+        q, k, v = (t.requires_grad_() for t in (q, k, v))
+        out = attention(q, k, v, **options)
+        dq, dk, dv = torch.autograd.grad(out, [q, k, v], up)
+        assert not dq.any() and not dk.any() and dv.any()
+        own = v[:, -T:].repeat_interleave(2, 2) if S > 1 else v.repeat_interleave(2, 2).expand_as(q)
+        # (p v) (1 / p): three float32 roundings, 3 x 2^-24 of v; in bfloat16 rounded away.
+        off = 3 * 2.0 ** -24 if dtype == "fp32" else 0.0
+        assert bool(((out.double() - own.double()).abs() <= off * own.double().abs()).all())
+    # The first token of a sequence, and a sequence of one.
+    q, k, v, up = (torch.randn(2, 150, 2, h, generator=g).to(DTYPES[dtype]).to(dev).requires_grad_()
+                   for _ in range(4))
+    lengths = torch.tensor([150, 1], device=dev)
+    dq, dk, _ = torch.autograd.grad(
+        attention(q, k, v, lengths=lengths, starts=torch.zeros_like(lengths)), [q, k, v], up)
+    assert not dq[:, 0].any() and not dk[1].any() and dq[0, 1:].any() and dk[0].any()
+
+
 def test_two_streams_at_once(dev):
     """Calls beside each other have their own workspaces, and answer as one by one."""
     torch.manual_seed(1)
