@@ -218,3 +218,46 @@ def test_a_failed_capture_leaves_the_layer_as_it_was(dev):
     fn, st = ghost_clipped_grad(model, per_example_lm_loss, clipping_norm=1.0)
     out, _ = fn(ids, ids, state=st)
     assert all(torch.isfinite(t).all() for t in out.pytree.values())
+
+
+def test_caches_past_32_bits(dev):
+    """Keys whose elements lie past 2^31: a window at the end of the last of three sequences."""
+    B, S, KV, h, window = 3, 1 << 20, 8, 128, 90
+    g = torch.Generator().manual_seed(8)
+    q = torch.randn(B, 2, 16, h, generator=g).to(torch.bfloat16).to(dev)
+    k, v = (torch.zeros(B, S, KV, h, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    assert k.numel() > 2 ** 31
+    for t in (k, v):
+        t[:, -400:] = torch.randn(B, 400, KV, h, generator=g).to(torch.bfloat16).to(dev)
+    lengths = torch.tensor([S, S - 300, S - 7], device=dev)
+    got = attention(q, k, v, window=window, lengths=lengths, starts=lengths - 2)
+    near = attention(q, k[:, -400:].contiguous(), v[:, -400:].contiguous(), window=window,
+                     lengths=lengths - (S - 400), starts=lengths - 2 - (S - 400))
+    # Either rounds p to 2^-8 of itself and the result once more, in an order of its own.
+    assert ((got.double() - near.double()).abs() <= 2.0 ** -6 * v[:, -400:].abs().max()).all()
+    assert torch.isfinite(got).all() and got.abs().max() > 0.1
+
+
+def test_tokens_past_32_bits(dev):
+    """Results whose elements lie past 2^31, against a few of the last tokens by themselves."""
+    N, D, F, few = 70001, 64, 16384, 65
+    x, w, _ = _inputs((N, D), F, torch.bfloat16, dev, seed=5)
+    h = gated_linear(x, w)
+    up = torch.randn_like(h)
+    (dx,) = torch.autograd.grad(h, [x], up)
+    assert N * 2 * F > 2 ** 31
+    last = x.detach()[-few:].clone().requires_grad_()
+    want = gated_linear(last, w.detach())
+    (dlast,) = torch.autograd.grad(want, [last], up[-few:])
+    for got, ref in zip((h[-few:], dx[-few:]), (want, dlast)):
+        # The same operands in other tiles: float32 sums in another order, one rounding each.
+        off = 2.0 ** -7 * ref.double().abs() + 2.0 ** -12 * ref.double().abs().max()
+        assert bool(((got.double() - ref.double()).abs() <= off).all())
+    del h, up, dx
+    T = 270001
+    q = torch.randn(1, T, 64, 128, dtype=torch.bfloat16, device=dev)
+    assert q.numel() > 2 ** 31
+    freqs, _ = rotary_frequencies(128, device=dev)
+    far = rotary(q, None, freqs)
+    positions = torch.arange(T - 9, T, device=dev)
+    assert torch.equal(far[:, -9:], rotary(q[:, -9:], None, freqs, positions=positions))
