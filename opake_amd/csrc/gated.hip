@@ -772,7 +772,8 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 }  // namespace
 
 extern "C" size_t dpc_gated_linear_workspace_bytes(int64_t N, int D, int F, int dtype) {
-  return valid_sizes(N, D, F, dtype) ? Plan(N, D, F, dtype, true, false, false).total : 0;
+  if (!valid_sizes(N, D, F, dtype) || N == 0) return 0;
+  return Plan(N, D, F, dtype, true, false, false).total;
 }
 
 extern "C" int dpc_gated_linear(const void* x, const void* w, int64_t N, int D, int F, int dtype,
@@ -852,7 +853,8 @@ extern "C" int dpc_gated_linear_act_grad(const void* z, const void* rest, const 
 
 extern "C" size_t dpc_gated_linear_grad_workspace_bytes(int64_t N, int D, int F, int dtype,
                                                         int want_x, int want_w) {
-  return valid_sizes(N, D, F, dtype) ? Plan(N, D, F, dtype, false, want_x, want_w).total : 0;
+  if (!valid_sizes(N, D, F, dtype) || N == 0) return 0;
+  return Plan(N, D, F, dtype, false, want_x, want_w).total;
 }
 
 extern "C" int dpc_gated_linear_grad(const void* x, const void* w, const void* dz, int64_t N,

@@ -43,7 +43,7 @@ constexpr int kUnits = 256;  // compute units of an MI355X
 constexpr int kMostSliced = 512;  // tiles times slices, if more than one
 
 DPC_HOST_DEVICE int slices(int64_t tiles, int64_t steps) {
-  if (2 * tiles > kMostSliced || steps < 16) return 1;
+  if (tiles < 1 || 2 * tiles > kMostSliced || steps < 16) return 1;
   const int n = (int)tiles, k = steps < 1 << 20 ? (int)steps : 1 << 20;
   int best = 1, least = 140 * k + 1000;  // (one round: more than 256 tiles do not get here)
   for (int r = 1; r <= kMostSliced / kUnits; ++r) {

@@ -196,6 +196,27 @@ def test_clipped_experts_match_per_example_oracle(dev, dtype, d, inter, T, starv
         assert _rel(aux.group_norms[name], res.group_norms[name]) < TOL[dtype], name
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradient_of_the_input_beside_an_expert_without_tokens(dev, dtype):
+    """Widths at which the products' sums are cut in slices."""
+    d, inter, E = 64, 1024, 4
+    ref, model = _pair(lambda **kw: TopKMoE(d, inter, E, 2, **kw), dtype, dev, std=0.05, seed=16)
+    g = torch.Generator().manual_seed(17)
+    x = torch.randn(2, 9, d, generator=g).to(dtype)
+    logits = torch.randn(2, 9, E, generator=g)
+    logits[..., 3] = -50.0
+    xr, xd = x.double().requires_grad_(), x.to(dev).requires_grad_()
+    _sq(ref(xr, logits.double()), torch.zeros(2, 9, d)).sum().backward()
+    _sq(model(xd, logits.to(dev)), torch.zeros(2, 9, d, device=dev)).sum().backward()
+    assert model.last_counts[3].sum() == 0
+    assert _rel(xd.grad, xr.grad) < TOL[dtype]
+    for (n, p), (_, q) in zip(model.named_parameters(), ref.named_parameters()):
+        if "experts.3" in n:
+            assert not p.grad.any(), n
+        elif p.requires_grad:
+            assert _rel(p.grad, q.grad) < TOL[dtype], n
+
+
 def test_clipped_routed_model_equals_the_default_one(dev):
     """The whole model, all three operators with the head's loss and the router's choice."""
     V, d = 61, 32

@@ -119,6 +119,18 @@ def test_no_token(dev):
         assert h.shape == (0, 8) and dx.shape == x.shape and not dw.any()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("D,F", [(2048, 8192), (1024, 1408), (1001, 512), (64, 512)])
+def test_no_token_at_the_widths_of_a_block(dev, dtype, D, F):
+    """Sums long enough to be cut in slices, of no tiles."""
+    x, w, up = _inputs((0, D), F, DTYPES[dtype], dev, seed=1)
+    h = gated_linear(x, w)
+    assert h.shape == (0, F) and gated_linear(x.detach(), w.detach()).shape == (0, F)
+    for want in ([x, w], [x], [w]):
+        got = torch.autograd.grad(h, want, up, retain_graph=True)
+        assert all(t.shape == o.shape and not t.any() for t, o in zip(got, want))
+
+
 def test_strided_and_unaligned_operands(dev):
     g = torch.Generator().manual_seed(5)
     base = torch.randn(40, 3, 65, generator=g).to(torch.bfloat16).to(dev)
