@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import torch
 from torch import nn
+from torch.autograd.forward_ad import unpack_dual
 
 from opake_amd import _native as nat
 from opake_amd._autograd import check_leaves, note_leaves
@@ -125,6 +126,9 @@ def _gated(x: torch.Tensor, weight: torch.Tensor, activation: str):
             f"tokens, got x {tuple(x.shape)} and weight {tuple(weight.shape)}")
     options = (nat.dtype_code(x.dtype), _ACTIVATIONS[activation])
     if not torch.is_grad_enabled() or not (x.requires_grad or weight.requires_grad):
+        # Past the autograd functions, which refuse tangents themselves.
+        if unpack_dual(x).tangent is not None or unpack_dual(weight).tangent is not None:
+            raise NotImplementedError("gated_linear has no forward-mode derivative")
         return _forward(x, weight, options, False)[:2]
     box: list = []
     z = _Project.apply(x, weight, options, box)

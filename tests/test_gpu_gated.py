@@ -267,3 +267,16 @@ def test_entry_points_refuse(dev):
     for bad in (dict(N=-1), dict(D=0), dict(F=0), dict(code=nat.DPC_F16), dict(act=2), dict(xp=0),
                 dict(xp=x.data_ptr() + 4)):
         assert call(**bad) == nat.DPC_EINVAL, bad
+
+
+def test_tangents_are_refused(dev):
+    """Forward-mode differentiation, with gradients and without."""
+    x, w, _ = _inputs((4, 16), 8, torch.float32, dev, seed=1)
+    layer = GatedLinear(16, 8, dtype=torch.float32, device=dev)
+    for grad in (True, False):
+        with torch.set_grad_enabled(grad), torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(x.detach(), torch.ones_like(x))
+            for call in (lambda: gated_linear(dual, w), lambda: gated_linear(dual, w.detach()),
+                         lambda: layer(dual)):
+                with pytest.raises(NotImplementedError):
+                    call()
