@@ -714,18 +714,18 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
     store_row<float, kD>(a.part_o + at * a.h, nullptr, o, 1.f, me.sees, me.there, a.h, lane);
     return;
   }
-  const bool some = me.sees && l != 0.f;  // (NaN too)
+  // (A row that sees keys has l > 0, but where all of its scores are -inf: NaN there.)
   if (me.there && lane < 32 && a.lse) {
     if constexpr (sizeof(T) == 2) {
-      a.lse[row] = some ? m + __builtin_amdgcn_logf(l) : INFINITY;
+      a.lse[row] = me.sees ? m + __builtin_amdgcn_logf(l) : INFINITY;
     } else {
-      a.lse[row] = some ? m : INFINITY;
-      a.inv[row] = some ? 1.f / l : 0.f;
+      a.lse[row] = me.sees ? m : INFINITY;
+      a.inv[row] = me.sees ? 1.f / l : 0.f;
     }
   }
   const int64_t flat = (((int64_t)b * a.T + me.t) * a.KV * a.rep + head) * a.h;
-  store_row<T, kD>(static_cast<T*>(a.o) + flat, a.rest ? a.rest + flat : nullptr, o, 1.f / l, some,
-                   me.there, a.h, lane);
+  store_row<T, kD>(static_cast<T*>(a.o) + flat, a.rest ? a.rest + flat : nullptr, o, 1.f / l,
+                   me.sees, me.there, a.h, lane);
 }
 
 // The splits of a row joined: one wave a row.  Lane p has parts p, p + 64, ... weighed
@@ -777,9 +777,10 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int parts) {
 #pragma unroll 8
     for (int p = 0; p < parts; ++p) o[e] = fmaf(from_o[p * n * a.h], weights[w][p], o[e]);
   }
-  const bool some = l != 0.f;
   const int64_t bk = row / a.rows, r = row - bk * a.rows, b = bk / a.KV, kv = bk - b * a.KV,
                 t = r / a.rep, g = r - t * a.rep;
+  const Sight sight(a, uniform((int)b));
+  const bool some = sight.first((int)t) == (int)t && sight.last((int)t) == (int)t;
   if (a.lse && lane == 0) {
     if constexpr (sizeof(T) == 2) {
       a.lse[row] = some ? m + __builtin_amdgcn_logf(l) : INFINITY;

@@ -314,3 +314,30 @@ def test_refusals(dev):
     for kw in (dict(window=1.5), dict(window=True), dict(lengths=n.float()), dict(scale="1")):
         with pytest.raises(InputTypeError):
             attention(q, k, v, **kw)
+
+
+# One row tile and several, two waves a compute unit's SIMD, keys in splits.
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("B,T,S,H,KV,h", [
+    (2, 2, 2, 2, 2, 16), (2, 70, 70, 4, 2, 64), (2, 130, 130, 2, 1, 256), (16, 260, 260, 16, 16, 64),
+    (2, 1, 900, 8, 2, 128), (2, 3, 1500, 2, 2, 64)])
+def test_scores_that_are_all_minus_infinity(dev, dtype, B, T, S, H, KV, h):
+    """No probabilities come of them: NaN, as their softmax is, and not the zeros of a row that
+    sees no key."""
+    q, k, v, up = (t.detach().clone() for t in _inputs(B, T, S, H, KV, h, DTYPES[dtype], dev))
+    k[..., 0] = k[..., 0].abs() + 1
+    q[..., 0] = q[..., 0].abs()
+    want = _run(*(t.requires_grad_() for t in (q, k, v)), up)
+    t, head = T // 2, H - 1
+    with torch.no_grad():
+        q[0, t, head, 0] = -math.inf
+    out, dq, dk, dv = got = _run(q, k, v, up)
+    for x, w in zip(got[:2], want):
+        assert bool(x[0, t, head].isnan().all())
+        others = torch.ones(x.shape[:3], dtype=torch.bool, device=dev)
+        others[0, t, head] = False
+        assert torch.equal(x[others], w[others])
+    seen = S - T + t + 1  # keys of the head's group
+    assert bool(dk[0, :seen, -1].isnan().all()) and bool(dv[0, :seen, -1].isnan().all())
+    for x, w in zip(got[2:], want[2:]):
+        assert torch.equal(x[1:], w[1:]) and torch.equal(x[0, :, :-1], w[0, :, :-1])
