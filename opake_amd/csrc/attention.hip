@@ -1009,9 +1009,10 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
       if (x == stage) back(x);
   }
   transfers_left<0>();
-  // One key alone: its probability is one, and ds zero, whatever rounding left of it.
-  store_row<T, kD>(static_cast<T*>(a.dq) + flat, nullptr, dq, a.scale, me.span > 0, me.there, a.h,
-                   lane);
+  // One key alone: its probability is one, and ds zero, whatever rounding left of it; but not
+  // where D is no number (do, its value or its score is not finite), and so ds neither.
+  const bool keep = me.span > 0 || (me.sees && !(fabsf(D) < INFINITY));
+  store_row<T, kD>(static_cast<T*>(a.dq) + flat, nullptr, dq, a.scale, keep, me.there, a.h, lane);
 }
 
 // ---------------------------------------------------------------------------
@@ -1237,7 +1238,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1)) attn_dkv_k
         dp[e][x] *= s[e][x];
       }
       // Rows that do not see the key: zero, and then so is ds; it is zero too where a row sees one
-      // key alone (never in a whole tile), whatever the rounding of dp - D left.
+      // key alone (never in a whole tile), whatever the rounding of dp - D left, if it is finite.
       if (!whole) {
         int r0 = 32 * (e + group) + column_row(0, lane);
         asm volatile("" : "+v"(r0));  // (its rows' tokens are not kept between tiles)
@@ -1246,7 +1247,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1)) attn_dkv_k
           const int at = ti + (grouped ? a.by_rep.of(r0 + column_row(x, 0)) : 0);
           const int lo = sight.lo(at), hi = sight.hi(at);
           if (key < lo || key > hi) s[e][x] = 0.f;
-          if (key < lo || key > hi || lo == hi) dp[e][x] = 0.f;
+          if (key < lo || key > hi || (lo == hi && fabsf(dp[e][x]) < INFINITY)) dp[e][x] = 0.f;
         }
       }
       if constexpr (sizeof(T) == 2) {

@@ -341,3 +341,28 @@ def test_scores_that_are_all_minus_infinity(dev, dtype, B, T, S, H, KV, h):
     assert bool(dk[0, :seen, -1].isnan().all()) and bool(dv[0, :seen, -1].isnan().all())
     for x, w in zip(got[2:], want[2:]):
         assert torch.equal(x[1:], w[1:]) and torch.equal(x[0, :, :-1], w[0, :, :-1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("which", ["q", "k", "v", "up"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("B,T,S,h", [(2, 1, 1, 16), (2, 70, 70, 64), (2, 33, 33, 256),
+                                     (64, 260, 260, 128), (2, 5, 700, 64)])
+def test_one_key_of_values_that_are_not_finite(dev, dtype, which, bad, B, T, S, h):
+    """A query that sees one key has no gradient of query and key, unless what it is formed of
+    is not finite: then it is what the formula gives, and not zero."""
+    x = [t.detach().clone() for t in _inputs(B, T, S, 4, 4, h, DTYPES[dtype], dev)]
+    for t in x[:2]:
+        t[..., 0] = t[..., 0].abs() + 1  # (a score is the infinity's, not NaN of its zero)
+    want = _run(*(t.requires_grad_() for t in x[:3]), x[3], window=1)
+    assert not want[1].any() and not want[2].any()
+    t, i = T - 1, ["q", "k", "v", "up"].index(which)
+    with torch.no_grad():  # the last token and its key
+        x[i][1, -1, 2, 0] = bad
+    out, dq, dk, dv = got = _run(*x, window=1)
+    assert bool(dq[1, t, 2].isnan().all()) and bool(dk[1, -1, 2].isnan().all())
+    assert bool(dv[1, -1, 2].isnan().all()) == (i < 2) and bool(out[1, t, 2].isnan().all()) == (i < 2)
+    for a, b in zip(got, want):  # the other heads and examples
+        others = torch.ones(a.shape[:3], dtype=torch.bool, device=dev)
+        others[1, :, 2] = False
+        assert torch.equal(a[others], b[others])
