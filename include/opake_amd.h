@@ -670,7 +670,8 @@ int dpc_gated_linear_grad(const void* x, const void* w, const void* dz, int64_t 
  * dv [B, S, KV, h] (both or neither).  state is not changed.
  * Probabilities are formed again; nothing of size [T, S] is kept.  Sums and statistics are
  * float32; bf16 products take probabilities and their gradients in bf16.  All results are
- * deterministic.  h <= 256, a multiple of 16 bytes; T, S <= 2^24, T H / KV <= 2^30.  A
+ * deterministic.  h <= 256, a multiple of 16 bytes; T, S <= 2^24, T H / KV <= 2^30, and
+ * B KV (ceil(n / 32) + 1) below 2^31 for n = T H / KV and n = S.  A
  * tensor whose 65 tokens and H / KV heads span 2 GiB or more is refused (DPC_ENOTSUP), and
  * so are keys or values whose tokens overlap (a stride below h).  Workspaces are 256-byte
  * aligned.

@@ -96,6 +96,7 @@ struct AttnArgs {
   float scale, c;          // c = scale log2(e)
   int tiles;               // row tiles (dk, dv: key tiles) of a key head
   int per_xcd, chunk;      // key heads of an XCD (0: not divided among them), of a chunk
+  int block0;              // workgroups in the launches before (see Launch::go)
   Divisor by_rep, by_kv;
   // Keys in splits (few rows): partial results.
   int splits;
@@ -152,7 +153,7 @@ struct RowRange {
 // others (8 x 2048 tokens, 32 heads over 8: a quarter of the time with each key head's
 // tiles by themselves).
 DPC_DEVICE void place_of(const AttnArgs& a, int tiles, int* bk, int* tile) {
-  int x = blockIdx.x, first = 0, heads = a.B * a.KV;
+  int x = a.block0 + blockIdx.x, first = 0, heads = a.B * a.KV;
   if (a.per_xcd) {
     heads = a.per_xcd;
     first = (x & 7) * heads;
@@ -1388,8 +1389,14 @@ struct Launch {
     if (lds > 65536)
       DPC_HIP_CHECK(hipFuncSetAttribute((const void*)kernel,
                                         hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, s, a);
-    DPC_HIP_CHECK(hipGetLastError());
+    // A launch has fewer than 2^32 threads; whole rounds of the XCDs keep place_of's heads there.
+    const int64_t most = UINT32_MAX / threads / 8 * 8;
+    for (int64_t at = 0; at < grid; at += most) {
+      a.block0 = (int)at;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)(grid - at < most ? grid - at : most)),
+                         dim3(threads), lds, s, a);
+      DPC_HIP_CHECK(hipGetLastError());
+    }
     return DPC_OK;
   }
   static int64_t heads(const AttnArgs& a) { return (int64_t)a.B * a.KV; }

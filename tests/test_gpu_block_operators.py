@@ -261,3 +261,15 @@ def test_tokens_past_32_bits(dev):
     far = rotary(q, None, freqs)
     positions = torch.arange(T - 9, T, device=dev)
     assert torch.equal(far[:, -9:], rotary(q[:, -9:], None, freqs, positions=positions))
+
+
+def test_more_sequences_than_a_launch_takes(dev):
+    """2^23 key heads of one token, 512 threads each: they go out in two launches."""
+    B, KV, h = 1 << 21, 4, 8
+    g = torch.Generator(device=dev).manual_seed(3)
+    q, k, v, up = (torch.randn(B, 1, KV, h, generator=g, device=dev, dtype=torch.bfloat16)
+                   for _ in range(4))
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+    out = attention(q, k, v)
+    dq, dk, dv = torch.autograd.grad(out, [q, k, v], up)
+    assert torch.equal(out, v) and torch.equal(dv, up) and not dq.any() and not dk.any()
