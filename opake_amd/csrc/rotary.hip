@@ -44,6 +44,7 @@ struct Heads {
 struct RotaryArgs {
   Heads part[2];
   int64_t T, tokens;
+  int64_t block0;            // workgroups in the launches before
   const int64_t* positions;  // or null: the token's index
   int64_t pos_b, pos_t;
   const double* freqs;
@@ -96,7 +97,7 @@ template <typename T, int kVec, bool kInterleaved>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a) {
   typedef T pack_t __attribute__((ext_vector_type(kVec)));
   __shared__ float2 table[kTable];
-  const int64_t first = (int64_t)blockIdx.x * a.tokens_each;
+  const int64_t first = (a.block0 + blockIdx.x) * a.tokens_each;
   const int tokens = (int)min((int64_t)a.tokens_each, a.tokens - first);
   for (int i = threadIdx.x; i < tokens * a.pairs; i += kThreads) {
     const int n = i / a.pairs, p = i - n * a.pairs;
@@ -183,14 +184,15 @@ int launch(RotaryArgs& a, hipStream_t s) {
   if (a.pairs && each > kTable / a.pairs) each = kTable / a.pairs;
   a.tokens_each = each < 1 ? 1 : each;
   const int64_t grid = (a.tokens + a.tokens_each - 1) / a.tokens_each;
-  if (grid > 0x7fffffff) return DPC_EINVAL;
-  if (a.interleaved)
-    hipLaunchKernelGGL((rotary_kernel<T, kVec, true>), dim3((unsigned)grid), dim3(kThreads), 0, s,
-                       a);
-  else
-    hipLaunchKernelGGL((rotary_kernel<T, kVec, false>), dim3((unsigned)grid), dim3(kThreads), 0, s,
-                       a);
-  DPC_HIP_CHECK(hipGetLastError());
+  const int64_t most = UINT32_MAX / kThreads;  // a launch has fewer than 2^32 threads
+  for (a.block0 = 0; a.block0 < grid; a.block0 += most) {
+    const dim3 blocks((unsigned)(grid - a.block0 < most ? grid - a.block0 : most));
+    if (a.interleaved)
+      hipLaunchKernelGGL((rotary_kernel<T, kVec, true>), blocks, dim3(kThreads), 0, s, a);
+    else
+      hipLaunchKernelGGL((rotary_kernel<T, kVec, false>), blocks, dim3(kThreads), 0, s, a);
+    DPC_HIP_CHECK(hipGetLastError());
+  }
   return DPC_OK;
 }
 

@@ -273,3 +273,17 @@ def test_more_sequences_than_a_launch_takes(dev):
     out = attention(q, k, v)
     dq, dk, dv = torch.autograd.grad(out, [q, k, v], up)
     assert torch.equal(out, v) and torch.equal(dv, up) and not dq.any() and not dk.any()
+
+
+def test_more_tokens_than_a_launch_takes(dev):
+    """2^24 tokens of a workgroup each: they go out in two launches."""
+    N, h = (1 << 24) + 3, 1026
+    g = torch.Generator(device=dev).manual_seed(3)
+    q = torch.randn(1, 1, 1, h, generator=g, device=dev, dtype=torch.bfloat16)
+    freqs, _ = rotary_frequencies(h, device=dev)
+    positions = (torch.arange(N, device=dev) % 7).view(N, 1)
+    out = rotary(q.expand(N, 1, 1, h), None, freqs, positions=positions)
+    want = rotary(q.expand(7, 1, 1, h), None, freqs, positions=positions[:7])
+    for at in range(0, N, 7 << 18):
+        part = out[at:at + (7 << 18)]
+        assert torch.equal(part, want[positions[at:at + (7 << 18), 0]])
