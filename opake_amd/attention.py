@@ -161,4 +161,4 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     return out[..., :h] if odd else out
 
 
-__all__ = ["attention"]
+__all__ = ["MAX_HEAD", "attention"]

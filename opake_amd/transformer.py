@@ -28,7 +28,8 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
-from opake_amd.attention import attention
+from opake_amd.attention import MAX_HEAD, attention
+from opake_amd.exceptions import ConfigurationError
 from opake_amd.gated import GatedLinear
 from opake_amd.rotary import rotary, rotary_frequencies
 
@@ -51,10 +52,13 @@ def apply_rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch
 
 
 class RotaryFrequencies(nn.Module):
-    """``rotary``'s frequencies of a block: float64, on its device, whatever it is cast to."""
+    """``rotary``'s frequencies of a fused block: float64, on its device, whatever it is cast to.
+    Heads that ``attention`` does not take are refused here, where the block is made."""
 
     def __init__(self, dims: int, device=None):
         super().__init__()
+        if dims > MAX_HEAD:
+            raise ConfigurationError(f"fused heads are at most {MAX_HEAD} wide, got {dims}")
         self.dims = dims
         self.register_buffer("freqs", rotary_frequencies(dims, device=device)[0],
                              persistent=False)

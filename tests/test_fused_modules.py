@@ -1,0 +1,23 @@
+"""What the fused blocks are as torch modules (CPU)."""
+
+from __future__ import annotations
+
+import pytest
+
+from opake_amd.exceptions import ConfigurationError
+from opake_amd.lora import LoRABlock
+from opake_amd.moe import RoutedLM
+from opake_amd.transformer import BlockLM, LlamaBlock
+
+
+@pytest.mark.parametrize("make", [
+    lambda d, **kw: LlamaBlock(d, 2, 8, device="meta", **kw),
+    lambda d, **kw: BlockLM(7, d, 2, 8, device="meta", **kw),
+    lambda d, **kw: LoRABlock(d, 2, 1, 8, 2, device="meta", **kw),
+    lambda d, **kw: RoutedLM(7, d, 2, 8, 4, 3, device="meta", **kw)])
+def test_heads_that_attention_does_not_take_are_refused_when_the_block_is_made(make):
+    make(512, fused=True)
+    make(528), make(6)
+    for d in (528, 6):  # 264 wide, and three
+        with pytest.raises(ConfigurationError):
+            make(d, fused=True)
