@@ -52,6 +52,8 @@ class LoRALinear(nn.Module):
 
 
 class LoRABlock(nn.Module):
+    fused = False  # (of blocks that were pickled before they could be)
+
     def __init__(self, d: int = 4096, n_heads: int = 32, n_kv_heads: int = 8,
                  ffn: int = 14336, r: int = 16, alpha: float = 32.0, eps: float = 1e-5, *,
                  fused: bool = False, dtype=None, device=None):

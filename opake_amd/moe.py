@@ -48,6 +48,8 @@ from opake_amd.transformer import LlamaBlock
 
 
 class SwiGLUExpert(nn.Module):
+    fused = False  # (of blocks that were pickled before they could be)
+
     def __init__(self, d: int, inter: int, *, fused: bool = False, dtype=None, device=None):
         super().__init__()
         self.inter, self.fused = inter, fused

@@ -70,6 +70,8 @@ class RotaryFrequencies(nn.Module):
 
 
 class LlamaBlock(nn.Module):
+    fused = False  # (of blocks that were pickled before they could be)
+
     def __init__(self, d: int = 2048, n_heads: int = 16, ffn: int = 8192, eps: float = 1e-5, *,
                  fused: bool = False, dtype=None, device=None):
         super().__init__()

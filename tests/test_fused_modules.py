@@ -2,11 +2,14 @@
 
 from __future__ import annotations
 
+import io
+
 import pytest
+import torch
 
 from opake_amd.exceptions import ConfigurationError
 from opake_amd.lora import LoRABlock
-from opake_amd.moe import RoutedLM
+from opake_amd.moe import RoutedLM, TopKMoE
 from opake_amd.transformer import BlockLM, LlamaBlock
 
 
@@ -21,3 +24,19 @@ def test_heads_that_attention_does_not_take_are_refused_when_the_block_is_made(m
     for d in (528, 6):  # 264 wide, and three
         with pytest.raises(ConfigurationError):
             make(d, fused=True)
+
+
+@pytest.mark.parametrize("make,x", [
+    (lambda: LlamaBlock(8, 2, 6), (2, 3, 8)), (lambda: LoRABlock(8, 2, 1, 6, 2), (2, 3, 8)),
+    (lambda: TopKMoE(8, 6, 3), (2, 3, 8))])
+def test_blocks_pickled_before_there_were_fused_ones(make, x):
+    """Their dictionaries lack ``fused``: they run as they did."""
+    block, x = make(), torch.randn(*x)
+    with torch.no_grad():
+        want = block(x)
+        for m in block.modules():
+            m.__dict__.pop("fused", None)
+        buffer = io.BytesIO()
+        torch.save(block, buffer)
+        buffer.seek(0)
+        assert torch.equal(torch.load(buffer, weights_only=False)(x), want)
