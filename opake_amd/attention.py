@@ -26,9 +26,12 @@ MAX_TOKENS = 1 << 24
 _MOST_BYTES = 0x7ff00000 - (1 << 20)
 
 
-def _rows(t: torch.Tensor, rep: int = 1, apart: int = 0) -> torch.Tensor:
-    """Rows of whole 16-byte chunks, at least ``apart`` elements from each other, and tiles
-    of 65 tokens within a buffer's range."""
+def _rows(t: torch.Tensor, odd: int, rep: int = 1, apart: int = 0) -> torch.Tensor:
+    """Rows of whole 16-byte chunks (``odd`` zeros more, which add nothing to a score and come
+    out as zeros), at least ``apart`` elements from each other, and tiles of 65 tokens
+    within a buffer's range."""
+    if odd:
+        t = F.pad(t, (0, odd))
     size = t.element_size()
     b, n, head, last = t.stride()
     if (last == 1 and (n >= apart or t.shape[1] < 2) and t.data_ptr() % 16 == 0 and b * size % 16 == 0 and n * size % 16 == 0
@@ -46,12 +49,17 @@ def _call(name, dev, tensors, strides, sizes, lengths, starts, options, *rest):
 
 
 class _Attention(torch.autograd.Function):
+    """Of q, k and v as they are, so that the leaves among them are its own; its output has the
+    copied rows' width."""
+
     @staticmethod
     def forward(ctx, q, k, v, lengths, starts, code, options, grad_enabled):
         dev = q.device
         B, T, H, h = q.shape
         S, KV = k.shape[1:3]
-        qr, kr, vr = _rows(q, H // KV), _rows(k, 1, h), _rows(v, 1, h)
+        odd = -h % (4 if q.dtype == torch.float32 else 8)
+        h += odd
+        qr, kr, vr = _rows(q, odd, H // KV), _rows(k, odd, 1, h), _rows(v, odd, 1, h)
         sizes = (B, T, S, H, KV, h, code)
         out = torch.empty((B, T, H, h), dtype=q.dtype, device=dev)
         lib, state, state_bytes = nat.load(), None, 0
@@ -61,7 +69,7 @@ class _Attention(torch.autograd.Function):
             state_bytes = lib.dpc_attention_state_bytes(B, T, H, h, code)
             state = torch.empty(state_bytes, dtype=torch.uint8, device=dev)
             ctx.save_for_backward(q, k, v, out, state, lengths, starts)
-            ctx.sizes, ctx.options = sizes, options
+            ctx.sizes, ctx.options, ctx.odd = sizes, options, odd
         ws_bytes = lib.dpc_attention_workspace_bytes(*sizes)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         _call("dpc_attention", dev, (qr, kr, vr),
@@ -77,8 +85,9 @@ class _Attention(torch.autograd.Function):
         q, k, v, out, state, lengths, starts = ctx.saved_tensors
         dev, sizes = q.device, ctx.sizes
         B, T, S, H, KV, h, _ = sizes
-        rep = H // KV
-        qr, kr, vr, gr = _rows(q, rep), _rows(k, 1, h), _rows(v, 1, h), _rows(grad, rep)
+        rep, odd = H // KV, ctx.odd
+        qr, kr, vr = _rows(q, odd, rep), _rows(k, odd, 1, h), _rows(v, odd, 1, h)
+        gr = _rows(grad, 0, rep)
         dq = torch.empty((B, T, H, h), dtype=q.dtype, device=dev)
         dk = dv = None
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
@@ -89,6 +98,8 @@ class _Attention(torch.autograd.Function):
               (*qr.stride()[:3], *kr.stride()[:3], *vr.stride()[:3], *gr.stride()[:3]), sizes,
               lengths, starts, ctx.options, state.data_ptr(), state.numel(), dq.data_ptr(),
               *(0 if t is None else t.data_ptr() for t in (dk, dv)), ws.data_ptr(), ws_bytes)
+        if odd:
+            dq, dk, dv = (t if t is None else t[..., :h - odd] for t in (dq, dk, dv))
         return dq, dk, dv, None, None, None, None, None
 
 
@@ -153,12 +164,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     if not 1e-30 < scale < 1e30:
         raise ConfigurationError(f"scale must be between 1e-30 and 1e30, got {scale}")
     options = (int(bool(causal)), min(window or 0, MAX_TOKENS), float(scale))
-    odd = -h % (4 if q.dtype == torch.float32 else 8)
-    if odd:  # zeros add nothing to a score, and come out as zeros
-        q, k, v = (F.pad(t, (0, odd)) for t in (q, k, v))
     out = _Attention.apply(q, k, v, _whole(lengths, "lengths", B), _whole(starts, "starts", B),
                            code, options, torch.is_grad_enabled())
-    return out[..., :h] if odd else out
+    return out if out.shape[3] == h else out[..., :h]
 
 
 __all__ = ["MAX_HEAD", "attention"]

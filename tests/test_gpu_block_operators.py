@@ -10,6 +10,7 @@ import torch
 
 from opake_amd.attention import attention
 from opake_amd.clipping import ghost_clipped_grad
+from opake_amd.exceptions import OperationError
 from opake_amd.gated import gated_linear
 from opake_amd.lora import LoRABlock
 from opake_amd.rotary import rotary, rotary_frequencies
@@ -287,3 +288,36 @@ def test_more_tokens_than_a_launch_takes(dev):
     for at in range(0, N, 7 << 18):
         part = out[at:at + (7 << 18)]
         assert torch.equal(part, want[positions[at:at + (7 << 18), 0]])
+
+
+def test_odd_widths_are_refused_beside_a_living_eager_graph_too(dev):
+    """Heads that are no whole chunks, whose rows are copied: the leaves are seen all the same."""
+    g = torch.Generator().manual_seed(7)
+    q, k, v, up = (torch.randn(2, 30, 2, 7, generator=g).to(dev) for _ in range(4))
+    q, k, v = (t.requires_grad_() for t in (q, k, v))
+
+    def step():
+        out = attention(q, k, v)
+        return (out, *torch.autograd.grad(out, [q, k, v], up))
+
+    alive = attention(q, k, v)
+    assert len(alive.grad_fn.next_functions[0][0].accumulators) == 3
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    with pytest.raises(OperationError):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(3):
+        with torch.no_grad():
+            q.copy_(torch.randn_like(q))
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, want in zip(out, step()):
+            assert torch.equal(got, want)
