@@ -98,6 +98,27 @@ def test_block_output_and_ordinary_gradients(dev, dtype, B, T, d, heads, ffn):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_token_has_no_gradient_of_queries_and_keys(dev, dtype):
+    """Exactly zero: one key's probability is one, and rotary and the layer keep zeros."""
+    d = 64
+    block = LlamaBlock(d, 1, 8, fused=True, dtype=dtype, device=dev)
+    lora = LoRABlock(d, 2, 1, 8, 2, fused=True, dtype=dtype, device=dev)
+    with torch.no_grad():
+        for n, p in lora.named_parameters():
+            if p.requires_grad:
+                p.normal_(0.0, 0.1)
+    g = torch.Generator().manual_seed(18)
+    x, up = (torch.randn(2, 1, d, generator=g).to(dtype).to(dev) for _ in range(2))
+    for model in (block, lora):
+        (model(x) * up).sum().backward()
+    grad = block.qkv.weight.grad
+    assert not grad[:2 * d].any() and grad[2 * d:].any()
+    for n, p in lora.named_parameters():
+        if p.requires_grad:
+            assert bool(p.grad.any()) == (n.split(".")[0] not in ("q", "k")), n
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("per_group", [False, True])
 def test_clipped_block_matches_per_example_oracle(dev, dtype, per_group):
     V, d, B, T = 61, 64, 3, 40
