@@ -625,8 +625,8 @@ int dpc_rotary(const void* q, const void* k, int64_t B, int64_t T, int H, int KV
  * with act DPC_ACT_SILU (g / (1 + exp(-g))) or DPC_ACT_GELU (g times the normal
  * distribution function).  h is rounded once from float32; z, if not NULL, is written in
  * `dtype`, and for bf16 rest [N, 2 F] (8 bits each: what rounding took from z, so that both
- * give z within 2^-17; fp32: NULL), for dpc_gated_linear_act_grad, which makes dz [N, 2 F] of
- * them and dh [N, F].
+ * give z within 2^-16, and within 2^-15 where it is nearly the middle of two bf16 values; fp32:
+ * NULL), for dpc_gated_linear_act_grad, which makes dz [N, 2 F] of them and dh [N, F].
  * dpc_gated_linear_grad takes dz to dx [N, D] = dz w and dw [2 F, D] =
  * dz^T x (either may be NULL; x is not read without dw, w not without dx).
  *

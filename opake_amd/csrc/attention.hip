@@ -390,16 +390,6 @@ DPC_DEVICE float sum_halves(float x) {
   return a + b;
 }
 
-// What rounding x to the bf16 `hi` took from it, to 8 more bits: (hi << 16) + (rest << 8)
-// as a float's bits is x within 2^-17.
-DPC_DEVICE int rest_of(float x, uint32_t hi) {
-  const int d = (int)(__float_as_uint(x) - (hi << 16));
-  return max(-128, min(127, (d + 128) >> 8));
-}
-DPC_DEVICE float with_rest(uint32_t hi, int rest) {
-  return __uint_as_float((hi << 16) + ((uint32_t)rest << 8));
-}
-
 // Stores a lane's column (kD elements in the row products' order, kD / 32 blocks) times f
 // as row `out`, or zeros where !keep; bf16: and `rest`, if not null.
 template <typename T, int kD>

@@ -85,6 +85,18 @@ DPC_HOST_DEVICE uint32_t f32x2_to_bf16x2_bits(float a, float b) {
 #endif
 }
 
+// What rounding x to the bf16 `hi` took from it, to 8 more bits: (hi << 16) + (rest << 8) as
+// a float's bits is x within 2^-16 (128 of the 2^23 of a binade), but within 2^-15 where x
+// lies so near the middle of two bf16 values that the byte would be 128 (one x in 500).
+DPC_DEVICE int rest_of(float x, uint32_t hi) {
+  const int d = (int)(__builtin_bit_cast(uint32_t, x) - (hi << 16));
+  const int r = (d + 128) >> 8;
+  return r < -128 ? -128 : (r < 127 ? r : 127);
+}
+DPC_DEVICE float with_rest(uint32_t hi, int rest) {
+  return __builtin_bit_cast(float, (hi << 16) + ((uint32_t)rest << 8));
+}
+
 // ---------------------------------------------------------------------------
 // Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy
 // as 1, 2, 3", SC'11).  Counter (c0..c3), key (k0, k1); ten rounds of the

@@ -18,7 +18,7 @@
 //
 // Held in fewer than 32 bits, bf16 inputs: dz, which the products take as their operand
 // (2^-8 of itself at most, the size of the gradients' own rounding).  z is kept with 8 bits
-// more than bf16 has (`rest`, 2^-17): of a z in bf16 the gradients would be 3.0e-3 from
+// more than bf16 has (`rest`, 2^-16): of a z in bf16 the gradients would be 3.0e-3 from
 // 64 bits in the mean square, so 2.4e-3.  h is formed from the float32 accumulators.
 #include <math.h>
 
@@ -240,16 +240,6 @@ struct ProductArgs {
 template <int kKind>
 DPC_DEVICE int tensor_shift(const uint32_t* all) {
   return -(kKind == kWeight ? mixed_shift(*all) : half_shift(*all));
-}
-
-// What rounding x to the bf16 `hi` took from it, to 8 more bits: (hi << 16) + (rest << 8)
-// as a float's bits is x within 2^-17.
-DPC_DEVICE int rest_of(float x, uint32_t hi) {
-  const int d = (int)(__float_as_uint(x) - (hi << 16));
-  return max(-128, min(127, (d + 128) >> 8));
-}
-DPC_DEVICE float with_rest(uint32_t hi, int rest) {
-  return __uint_as_float((hi << 16) + ((uint32_t)rest << 8));
 }
 
 // Quads of two neighbouring 16-column blocks, as the matrix cores leave them (lane l: columns

@@ -280,3 +280,35 @@ def test_tangents_are_refused(dev):
                          lambda: layer(dual)):
                 with pytest.raises(NotImplementedError):
                     call()
+
+
+def test_what_is_kept_of_projections(dev):
+    """bfloat16: z and its rest give the float32 sum within 2^-16, half a step of 8 bits more;
+    within 2^-15 (a step) where the rest would pass its byte, |z - bf16(z)| >= 127.5 / 128 of half
+    a bf16 step.  Sums of a pair are exact here, so what is off is the rest alone."""
+    F, D, N = 64, 8, 300  # (tiles; the few tokens' kernel takes the first 5)
+    g = torch.Generator().manual_seed(8)
+    x = torch.zeros(N, D)
+    x[:, 0] = 1.0
+    x[:, 1] = torch.randint(-256, 257, (N,), generator=g) * 2.0 ** -16  # up to half a bf16 step
+    w = torch.zeros(2 * F, D)
+    w[:, 0] = 1 + torch.randint(0, 128, (2 * F,), generator=g) / 128
+    w[:, 1] = 1.0
+    x, w = x.bfloat16(), w.bfloat16()
+    z = x.double() @ w.double().T
+    assert torch.equal(z.float().double(), z)  # exact in float32
+    near = (z - z.float().bfloat16().double()).abs() >= 127.5 / 128 * 2.0 ** -8
+    assert near.any() and not near.all()
+    lib, xd, wd = nat.load(), x.to(dev), w.to(dev)
+    for n in (5, N):
+        h, kept = (torch.empty(n, c, dtype=torch.bfloat16, device=dev) for c in (F, 2 * F))
+        rest = torch.empty(n, 2 * F, dtype=torch.int8, device=dev)
+        size = lib.dpc_gated_linear_workspace_bytes(n, D, F, nat.DPC_BF16)
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        nat.call_on(xd.device, "dpc_gated_linear", xd.data_ptr(), wd.data_ptr(), n, D, F,
+                    nat.DPC_BF16, nat.ACT_SILU, h.data_ptr(), kept.data_ptr(), rest.data_ptr(),
+                    ws.data_ptr(), size)
+        bits = (kept.view(torch.int16).int() << 16) + (rest.int() << 8)
+        off = (bits.view(torch.float32).cpu().double() - z[:n]).abs() / z[:n]
+        assert torch.equal(kept.cpu(), z[:n].float().bfloat16())
+        assert bool((off <= torch.where(near[:n], 2.0 ** -15, 2.0 ** -16)).all())
