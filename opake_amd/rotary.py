@@ -94,17 +94,24 @@ def rotary_frequencies(dims: int, base: float = 10000.0, *, scaling: dict | None
     return freq * keep + freq / factor * (1.0 - keep), amplitude
 
 
+def _heads(t: torch.Tensor) -> torch.Tensor:
+    """Any strides of examples and tokens, but heads within 32 bits of each other and each one's
+    elements side by side."""
+    if t.stride(-1) == 1 and t.stride(2) < 1 << 31:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _rotate(tensors, positions, freqs, options, inverse: int):
     code, interleaved, amplitude = options
     q, k = tensors
     dev = q.device
-    # Any strides between heads and tokens, but each head's elements side by side.
-    q = q if q.stride(-1) == 1 else q.contiguous()
+    q = _heads(q)
     out = [torch.empty(q.shape, dtype=q.dtype, device=dev)]
     KV, kp, kop = 0, 0, 0
     strides = [*q.stride()[:3], 0, 0, 0]
     if k is not None:
-        k = k if k.stride(-1) == 1 else k.contiguous()
+        k = _heads(k)
         out.append(torch.empty(k.shape, dtype=k.dtype, device=dev))
         KV, kp, kop = k.shape[2], k.data_ptr(), out[1].data_ptr()
         strides[3:] = k.stride()[:3]

@@ -172,3 +172,14 @@ def test_refusals(dev):
     strides = (nat._c_i64 * 6)(*([0, 0, 1 << 40] * 2))
     assert lib.dpc_rotary(q.data_ptr(), 0, 2, 3, 4, 0, 16, nat.DPC_F32, strides, 0, 0, 0,
                           freqs.data_ptr(), 8, 0, 1.0, 0, q.data_ptr(), 0, 0) == nat.DPC_EINVAL
+
+
+def test_heads_far_from_each_other(dev):
+    """Strides past 32 bits, of which one head alone takes no memory."""
+    freqs, _ = rotary_frequencies(16, device=dev)
+    base = torch.randn(2, 5, 16, device=dev)
+    q = base.as_strided((2, 5, 1, 16), (80, 16, 1 << 40, 1))
+    want = rotary(base.view(2, 5, 1, 16), None, freqs)
+    assert torch.equal(rotary(q, None, freqs), want)
+    for got in rotary(base.view(2, 5, 1, 16), q, freqs):
+        assert torch.equal(got, want)
