@@ -660,7 +660,8 @@ int dpc_gated_linear_grad(const void* x, const void* w, const void* dz, int64_t 
  * Example b has lengths[b] keys (NULL: S; clamped to 0 .. S).  Without `causal` every
  * query sees them all.  With it, token t is at position starts[b] + t (NULL: S - T + t)
  * and sees the keys up to it, or with window > 0 the last `window` of those; positions
- * below 0 or from lengths[b] on are padding.  Queries that see nothing have output 0 and no
+ * below 0 or from lengths[b] on are padding.  Queries that see nothing have output 0 (those
+ * whose scores are all -inf have NaN) and no
  * part in any gradient; what lies in keys, values and queries that are padding reaches
  * nothing, whatever it is.  scale > 0.
  *

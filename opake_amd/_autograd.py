@@ -5,7 +5,10 @@ accumulators.  An accumulator lives as long as any graph of its leaf and keeps t
 that it was made on, so where an eager graph of the same leaf is alive while a backward is
 captured into a HIP graph, that wait leaves the capture, and the runtime ends the process
 at its end.  The operators' functions note here, on each leaf's accumulator, whether it was made
-outside a capture, and their backward raises before the engine gets that far.
+outside a capture, and their backward raises before the engine gets that far.  Torch does not
+tell the age of an accumulator, so they see leaves that are their own inputs, in eager graphs
+that went through them; graphs of other operators alone, and leaves further up, torch's engine
+meets as it meets any model's.
 """
 
 from __future__ import annotations

@@ -127,11 +127,17 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
     them; a token at a position below 0 or not below the length is padding.  ``scale``:
     positive, 1 / sqrt(h) by default.
 
-    A query that sees no key has output 0 and no part in any gradient.  What padding holds
-    reaches nothing; what a token holds reaches its own example's head group alone, but there a
+    Scores, statistics and sums are float32.  bfloat16: probabilities and the gradients of
+    scores are rounded to it (2^-8 of each at most) before their products, so that output and
+    gradients are 2.0e-3 and 2.4e-3 from 64 bits in the mean square, where the rounding of
+    either alone leaves 1.7e-3; float32: 2e-7.
+
+    A query that sees no key has output 0 and no part in any gradient; one whose scores are all
+    -inf has NaN, as their softmax is.  What padding holds reaches nothing; what a token holds reaches its own example's head group alone, but there a
     value that is not finite may reach queries that do not see it.  Gradients reach ``q``,
     ``k`` and ``v``.  For one token of each of several sequences: T = 1, keys and values
-    the caches [B, S, KV, h], ``lengths`` the sequences' and ``starts`` one less."""
+    the caches [B, S, KV, h], ``lengths`` the sequences' and ``starts`` one less.  65 tokens of
+    all heads of a tensor must take less than 2 GiB."""
     nat.require_device(q, k, v, lengths, starts)
     if (q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[0] != k.shape[0]
             or q.shape[3] != k.shape[3]):

@@ -802,7 +802,8 @@ def _capture(model, layers, others, loss_fn, inputs, targets):
                         f"module {name!r} was called {cap.calls} times; ghost clipping needs "
                         "one call per module and step")
             # Gradients with respect to the module outputs only: autograd
-            # prunes the weight-gradient GEMMs, which the clipped sum replaces.
+            # prunes the weight-gradient GEMMs, which the clipped sum replaces
+            # (but not that of a GatedLinear, whose function forms both gradients).
             grads = torch.autograd.grad(losses.sum(), [c.out for _, c in named],
                                         allow_unused=True)
     finally:

@@ -169,7 +169,7 @@ DPC_DEVICE void place_of(const AttnArgs& a, int tiles, int* bk, int* tile) {
 // Keys in splits: linear id -> (key head, row tile, split).  Sequences differ in length, so each
 // XCD, and with every split each unit, gets another example's heads; the row tiles of a
 // split's keys follow each other on one XCD, if the heads are a multiple of eight.  (16
-// sequences of 1 to 8192 keys, 8 key heads: 59 us, 4.6 TB/s; each XCD with its own heads 69.)
+// sequences of 1 to 8192 keys, 8 key heads: 58 us, 4.6 TB/s; each XCD with its own heads 69.)
 DPC_DEVICE void place_of_split(const AttnArgs& a, int* bk, int* tile, int* split) {
   const uint32_t heads = a.B * a.KV, all = heads * a.tiles, x = blockIdx.x, s = x / all,
                  r = x - s * all, t = r / heads;
@@ -457,9 +457,10 @@ DPC_DEVICE int column_row(int x, int lane) { return 8 * (x >> 2) + 4 * (lane >> 
 // ---------------------------------------------------------------------------
 // Forward.  Bound by the matrix cores and by what vector instructions the exponentials
 // and the statistics cannot hide behind them; a workgroup takes 6 us before its first
-// product.  bf16, causal, h = 128: 1 x 16384 tokens of 16 heads 1091 us (1.0 PFLOP/s of visible pairs,
-// the matrix cores half busy, vector instructions 40%), 8 x 2048 of 32 over 8 358 (0.77),
-// 16 x 1024 of 16 132 (0.52: half of each key head's tiles cross the diagonal).
+// product.  bf16, causal, h = 128: 1 x 16384 tokens of 16 heads 1117 us (1.0 PFLOP/s of visible
+// pairs, the matrix cores half busy, vector instructions 40%), 8 x 2048 of 32 over 8 359 (0.77),
+// 16 x 1024 of 16 135 (0.51: half of each key head's tiles cross the diagonal).  float32, 8 x 1024
+// of 16: h = 64 214 us, 128 422 (81 TFLOP/s).
 // ---------------------------------------------------------------------------
 
 // Row tiles of kWaves x 32 rows.  Stages of key and value tiles in LDS: as many as 128 KiB
@@ -798,8 +799,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, int parts) {
 
 // ---------------------------------------------------------------------------
 // dq and D: rows fixed, keys walked.  The forward's walk with a product more; what bounds
-// it is the same: 8 x 2048 tokens of 32 heads over 8 513 us (0.80 PFLOP/s of its three
-// products), 16 x 1024 of 16 194 (0.53).
+// it is the same: 8 x 2048 tokens of 32 heads over 8 515 us (0.80 PFLOP/s of its three
+// products), 16 x 1024 of 16 199 (0.52).  float32, 8 x 1024 of 16: h = 64 286 us, 128 559.
 // ---------------------------------------------------------------------------
 
 template <typename T, int kD, int kWaves>
@@ -1008,7 +1009,8 @@ __global__ void __launch_bounds__(64 * kWaves, (kWaves == 8 ? 2 : 1))
 
 // ---------------------------------------------------------------------------
 // dk and dv: keys fixed, rows walked.  Four products: 8 x 2048 tokens of 32 heads over 8
-// 630 us (0.87 PFLOP/s), 16 x 1024 of 16 266 (0.52).
+// 638 us (0.86 PFLOP/s), 16 x 1024 of 16 273 (0.50).  float32, 8 x 1024 of 16: h = 64 418 us, 128
+// 844.
 // ---------------------------------------------------------------------------
 
 // Key tiles of 32 keys a wave, or of 4 x 32 keys for 8 waves: then the wave and the one four on
@@ -1428,7 +1430,12 @@ struct Launch {
     return go(attn_dkv_kernel<T, kD, kWaves>, a, heads(a) * a.tiles, 64 * kWaves,
               KeysShape<T, kD, kWaves>::kLds, s);
   }
-  // The widest tiles that give every compute unit one; else the narrowest.
+  // The widest tiles that give every compute unit one; else the narrowest (dq: 128 rows between
+  // the two).  bf16, h = 128, us of 256 / 128 / 32 rows: dq of 1 x 1024 tokens of 8 heads 40 / 33 /
+  // 32, of 4 x 1024 46 / 36 / 41; the forward of 4 x 1024 33 / 31.  dk and dv, 128 / 32 keys:
+  // 4 x 1024 39 / 58.  Below a tile a unit 32 keys win where few rows see a key (9 x 443, 6 heads of
+  // 80 over 2, a window of 200: 49 / 42), and lose without a window (1 x 1024 of 8 heads: 37 / 45,
+  // of 32 over 8: 116 / 153).
   static bool fills(const AttnArgs& a, int64_t n, int waves) {
     return heads(a) * ((n + 32 * waves - 1) / (32 * waves)) >= kUnits;
   }
@@ -1480,7 +1487,8 @@ bool valid_sizes(int64_t B, int64_t T, int64_t S, int H, int KV, int h, int dtyp
 // 32 with their keys in splits, which are joined (12 us and 1.2 for 32 keys of 32 rows, four
 // waves a unit): then enough splits for four workgroups a unit, none with fewer than four tiles of
 // 32 keys a wave.  (9 x 443 tokens, 6 heads over 2: 18 us in 198 tiles, 29 in splits.  16
-// tokens of 32 heads over 8, 8192 keys at most: 228 us in tiles, 64 in 8 splits.)
+// tokens of 32 heads over 8, 8192 keys at most: 228 us in tiles, 64 in 8 splits.)  The prices are
+// bf16's at h = 128, and S is counted whatever a window or the lengths leave of it.
 int splits_of(int64_t B, int64_t T, int64_t S, int H, int KV, int h, int dtype) {
   const int64_t rows = T * (H / KV), heads = B * KV;
   if (heads * ((rows + 255) / 256) >= kUnits) return 0;

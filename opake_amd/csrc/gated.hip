@@ -215,9 +215,10 @@ __global__ void __launch_bounds__(256) gated_pack_kernel(PackArgs args) {
 
 // ---------------------------------------------------------------------------
 // The products.  Bound by the K loop (mm_tile.h), the forward also by what it writes.  16384
-// tokens, D = 2048, F = 8192, bf16: forward 1056 us (1.04 PFLOP/s; 1.07 GB of h, z and rest),
-// dx 829 (1.33), dw 798 (1.38).  1773 tokens, D = 1000, F = 2731, float32: forward 108, dx 65,
-// 154 and 28 tiles of 256, so that units are left idle or the sum is cut in slices.
+// tokens, D = 2048, F = 8192, bf16: forward 1062 us (1.04 PFLOP/s; 1.07 GB of h, z and rest),
+// dx 848 (1.30), dw 815 (1.35).  1773 tokens, D = 1000, F = 2731, float32: forward 105, dx 64,
+// 154 and 28 tiles of 256, so that units are left idle or the sum is cut in slices; 8192 tokens
+// of it 372, 235 and dw 271.
 // ---------------------------------------------------------------------------
 
 enum Kind { kForward, kHidden, kWeight };
@@ -420,7 +421,8 @@ __global__ void __launch_bounds__(256) gated_reduce_kernel(ProductArgs s) {
 // run's loads are on their way while one is multiplied.  Rows and tokens past the last are
 // read as the last one's, and left out when h is written; behind D there are zeros.
 // Bound by memory: 16 tokens of D = 4096, F = 14336 in bf16 take 50 us, 4.7 TB/s of weights,
-// one 44 (5.3 TB/s); beyond 16 by the tokens' reads from L2, as long as the weights'.
+// one 44 (5.3 TB/s); called again at once, with part of the weights still in the cache, the 16
+// take 46.  Beyond 16 by the tokens' reads from L2, as long as the weights'.
 // float32: each lane's 16 bytes are four k of its row, one for each of four products (the
 // k of a product may be any, if both operands have the same), so nothing is split or shifted.
 template <bool kHalf, int kBlocks>
@@ -518,7 +520,7 @@ __global__ void __launch_bounds__(512) gated_few_kernel(const void* __restrict__
 }
 
 // ---------------------------------------------------------------------------
-// dz from z and dh: one pass, bound by memory (16384 tokens, F = 8192, bf16: 334 us, 4.8 TB/s).
+// dz from z and dh: one pass, bound by memory (16384 tokens, F = 8192, bf16: 331 us, 4.9 TB/s).
 // ---------------------------------------------------------------------------
 
 // kVec columns a thread; rows need not start at a vector (the loads' own alignment is the

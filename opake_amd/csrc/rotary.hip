@@ -14,7 +14,7 @@
 //
 // Memory bounds it: each element is read and written once.  (16 x 1024 tokens, 16 and 16
 // heads of 128, bf16: 54 us, 5.0 TB/s; 5 x 1999 of 32 and 8, half of each head, neighbours:
-// 46 us, 4.4 TB/s.)
+// 46 us, 4.4 TB/s; 16 x 1024 of 16 and 16 in float32: 101 us, 5.3 TB/s.)
 #include <math.h>
 
 #include "common.h"

@@ -17,7 +17,8 @@ attention with grouped-query heads (separate q / k / v / o projections) and a
 SwiGLU FFN (gate / up / down), every projection a ``LoRALinear``; the norms
 and base weights are frozen.  Its attention core runs in float32; with
 ``fused`` (on the GPU, bfloat16 or float32) ``rotary`` and ``attention`` take
-the projections as they are, key heads shared and not repeated.
+the projections as they are, key heads shared and not repeated; in bfloat16
+probabilities and the gradients of scores are then rounded to it.
 """
 
 from __future__ import annotations

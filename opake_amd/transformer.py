@@ -17,8 +17,10 @@ transposed view -- which attention's backward issues -- are avoided.
 
 With ``fused`` the block (on the GPU, bfloat16 or float32) runs ``rotary``,
 ``attention`` and ``gated_linear`` instead, which keep q, k, v and the
-projections in the model's type and nothing of size [T, T]; parameters and
-their names are the same.  Ghost clipping takes the fused block like the other
+projections in the model's type and nothing of size [T, T]; in bfloat16 they
+also round probabilities and the gradients of scores and projections to it
+before the next product, which the float32 core does not (``attention``,
+``gated_linear``).  Parameters and their names are the same.  Ghost clipping takes the fused block like the other
 one; ``vmap`` and the other function transforms do not take these operators.
 """
 
