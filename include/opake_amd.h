@@ -660,10 +660,9 @@ int dpc_gated_linear_grad(const void* x, const void* w, const void* dz, int64_t 
  * Example b has lengths[b] keys (NULL: S; clamped to 0 .. S).  Without `causal` every
  * query sees them all.  With it, token t is at position starts[b] + t (NULL: S - T + t)
  * and sees the keys up to it, or with window > 0 the last `window` of those; positions
- * below 0 or from lengths[b] on are padding.  Queries that see nothing have output 0 (those
- * whose scores are all -inf have NaN) and no
- * part in any gradient; what lies in keys, values and queries that are padding reaches
- * nothing, whatever it is.  scale > 0.
+ * below 0 or from lengths[b] on are padding.  Queries that see nothing have output 0 and no
+ * part in any gradient, those whose scores are all -inf NaN; what lies in keys, values and
+ * queries that are padding reaches nothing, whatever it is.  scale > 0.
  *
  * state (dpc_attention_state_bytes, 256-byte aligned; NULL without a gradient) keeps each
  * row's statistics and, for bf16, what rounding took from out, for dpc_attention_grad,
