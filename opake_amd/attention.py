@@ -129,8 +129,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool
 
     Scores, statistics and sums are float32.  bfloat16: probabilities and the gradients of
     scores are rounded to it (2^-8 of each at most) before their products, so that output and
-    gradients are 2.0e-3 and 2.4e-3 from 64 bits in the mean square, where the rounding of
-    either alone leaves 1.7e-3; float32: 2e-7.
+    gradients are 2.0e-3 and 2.4e-3 from 64 bits in the mean square (2.8e-3 at most), where the
+    rounding of either alone leaves 1.7e-3; float32: 2e-7 (2e-6 at most).
 
     A query that sees no key has output 0 and no part in any gradient; one whose scores are all
     -inf has NaN, as their softmax is.  What padding holds reaches nothing; what a token holds reaches its own example's head group alone, but there a

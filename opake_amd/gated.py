@@ -143,8 +143,8 @@ def gated_linear(x: torch.Tensor, weight: torch.Tensor, *,
     ``activation``: ``"silu"`` or ``"gelu"`` (with the normal distribution function).  Gradients
     reach both; for them the projections [..., 2 F] are kept, in the inputs' dtype (bfloat16: and 8
     bits more of each).  bfloat16: the projections' gradient is rounded to it before its products,
-    so that gradients are 2.3e-3 from 64 bits in the mean square (1.7e-3: the rounding of the
-    results alone).  There is no forward-mode derivative."""
+    so that gradients are 2.3e-3 from 64 bits in the mean square, 2.7e-3 at most (1.7e-3: the
+    rounding of the results alone).  There is no forward-mode derivative."""
     return _gated(x, weight, activation)[0]
 
 

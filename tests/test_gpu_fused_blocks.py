@@ -326,3 +326,17 @@ def test_widths_the_default_block_takes(dev):
         ref, model = _pair(lambda **kw: LlamaBlock(d, heads, 24, **kw), torch.float32, dev)
         x = torch.randn(2, 9, d, generator=torch.Generator().manual_seed(d))
         assert _rel(model(x.to(dev)), ref(x.double())) < TOL[torch.float32]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(2, 0, 64), (0, 5, 64)])
+def test_blocks_of_no_tokens(dev, dtype, shape):
+    """An empty batch or sequence, forward and backward, at widths whose sums are cut in slices."""
+    kw = dict(fused=True, dtype=dtype, device=dev)
+    for model in (LlamaBlock(64, 1, 1024, **kw), LoRABlock(64, 2, 1, 96, 4, **kw),
+                  TopKMoE(64, 1024, 4, 2, **kw)):
+        x = torch.zeros(shape, dtype=dtype, device=dev, requires_grad=True)
+        y = model(x)
+        y.sum().backward()
+        assert y.shape == shape and x.grad.shape == shape
+        assert not any(p.grad is not None and p.grad.any() for p in model.parameters())
