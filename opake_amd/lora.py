@@ -31,7 +31,7 @@ from torch import nn
 
 from opake_amd.attention import attention
 from opake_amd.rotary import rotary
-from opake_amd.transformer import RotaryFrequencies, apply_rotary, rotary_tables
+from opake_amd.transformer import apply_rotary, fused_frequencies, rotary_tables
 
 
 class LoRALinear(nn.Module):
@@ -79,7 +79,7 @@ class LoRABlock(nn.Module):
         self.mlp_norm.requires_grad_(False)
         self._rope = {}
         if fused:
-            self.rope = RotaryFrequencies(hd, device=device)
+            self.rope = fused_frequencies(hd, device=device)
 
     def _fused_attention(self, q, k, v):
         q, k = rotary(q, k, self.rope.freqs)

@@ -54,13 +54,10 @@ def apply_rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch
 
 
 class RotaryFrequencies(nn.Module):
-    """``rotary``'s frequencies of a fused block: float64, on its device, whatever it is cast to.
-    Heads that ``attention`` does not take are refused here, where the block is made."""
+    """``rotary``'s frequencies of a block: float64, on its device, whatever it is cast to."""
 
     def __init__(self, dims: int, device=None):
         super().__init__()
-        if dims > MAX_HEAD:
-            raise ConfigurationError(f"fused heads are at most {MAX_HEAD} wide, got {dims}")
         self.dims = dims
         self.register_buffer("freqs", rotary_frequencies(dims, device=device)[0],
                              persistent=False)
@@ -69,6 +66,13 @@ class RotaryFrequencies(nn.Module):
         super()._apply(fn, recurse)
         self.freqs = rotary_frequencies(self.dims, device=self.freqs.device)[0]
         return self
+
+
+def fused_frequencies(head_dim: int, device=None) -> RotaryFrequencies:
+    """Those of a fused block, which is refused here if ``attention`` does not take its heads."""
+    if head_dim > MAX_HEAD:
+        raise ConfigurationError(f"fused heads are at most {MAX_HEAD} wide, got {head_dim}")
+    return RotaryFrequencies(head_dim, device=device)
 
 
 class LlamaBlock(nn.Module):
@@ -90,7 +94,7 @@ class LlamaBlock(nn.Module):
         self.down = nn.Linear(ffn, d, bias=False, **kw)
         self._rope = {}
         if fused:
-            self.rope = RotaryFrequencies(d // n_heads, device=device)
+            self.rope = fused_frequencies(d // n_heads, device=device)
 
     def _tables(self, T, device):
         key = (T, device)

@@ -10,7 +10,7 @@ import torch
 from opake_amd.exceptions import ConfigurationError
 from opake_amd.lora import LoRABlock
 from opake_amd.moe import RoutedLM, TopKMoE
-from opake_amd.transformer import BlockLM, LlamaBlock
+from opake_amd.transformer import BlockLM, LlamaBlock, RotaryFrequencies
 
 
 @pytest.mark.parametrize("make", [
@@ -24,6 +24,7 @@ def test_heads_that_attention_does_not_take_are_refused_when_the_block_is_made(m
     for d in (528, 6):  # 264 wide, and three
         with pytest.raises(ConfigurationError):
             make(d, fused=True)
+    assert RotaryFrequencies(512).freqs.shape == (256,)  # (rotary takes them)
 
 
 @pytest.mark.parametrize("make,x", [
